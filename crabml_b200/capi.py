@@ -10,6 +10,7 @@ LIB_PATH = os.path.join(HERE, "lib", "libcrabml_cuda.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "crabml_cuda.h")
 RUNNER_HEADER = os.path.join(os.path.dirname(HERE), "include", "crabml_runner.h")
 SEQOPS_HEADER = os.path.join(os.path.dirname(HERE), "include", "crabml_seqops.h")
+PAGED_HEADER = os.path.join(os.path.dirname(HERE), "include", "crabml_paged.h")
 ZATORAX_HEADER = os.path.join(os.path.dirname(HERE), "include", "crabml_zatorax.h")
 
 CC_OK, CC_ERR_TENSOR, CC_ERR_CUDA, CC_ERR_ARG, CC_ERR_UNSUPPORTED = 0, 1, 2, 3, 4
@@ -18,7 +19,8 @@ CC_MAX_DIMS = 4
 # GGMLType ids (crabml-core/src/gguf.rs:86-108)
 F32, F16, Q4_0, Q4_1, Q5_0, Q5_1, Q8_0, Q8_1 = 0, 1, 2, 3, 6, 7, 8, 9
 Q2_K, Q3_K, Q4_K, Q5_K, Q6_K, Q8_K = 10, 11, 12, 13, 14, 15
-I32, BF16 = 26, 30
+I8, I32, BF16 = 24, 26, 30
+ARRAY_TYPES = {F32: ("<f4", 4), F16: ("<f2", 2), I8: ("|i1", 1), I32: ("<i4", 4)}      # plain types that numpy has a name for, and their bytes
 ACT_NONE, ACT_SILU, ACT_GELU_TANH, ACT_SWISH, ACT_SIGMOID, ACT_RELU_SQUARED = 0, 1, 2, 3, 4, 5
 ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1
 ROPE_LLAMA, ROPE_NEOX = 0, 1
@@ -46,7 +48,7 @@ class cc_device_options(C.Structure):
 def declared_symbols():
     """Every CC_API prototype name in the headers (used by the CPU-side export test)."""
     out = []
-    for h in (HEADER, RUNNER_HEADER, SEQOPS_HEADER, ZATORAX_HEADER):
+    for h in (HEADER, RUNNER_HEADER, SEQOPS_HEADER, PAGED_HEADER, ZATORAX_HEADER):
         with open(h) as f:
             out += re.findall(r"^CC_API [\w\s\*]+?\b(c[cz]r?_\w*)\(", f.read(), flags=re.M)
     return out
@@ -179,6 +181,15 @@ class cvd_layer_weights(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in CVD_WEIGHT_FIELDS]
 
 
+class cc_page_plan_desc(C.Structure):            # include/crabml_paged.h
+    _fields_ = [("n_seqs", C.c_int32), ("page_size", C.c_int32), ("table_cols", C.c_int32), ("n_pages", C.c_int64), ("n_slots", C.c_int64), ("pos0", C.c_void_p),
+                ("counts", C.c_void_p), ("table", C.c_void_p), ("slots", C.c_void_p)]
+
+
+class cc_paged_cache(C.Structure):
+    _fields_ = [(n, cc_view) for n in ("k", "v", "k_scale", "v_scale", "k_open", "v_open")]
+
+
 class cc_route_params(C.Structure):              # include/crabml_seqops.h
     _fields_ = [(n, C.c_int32) for n in ("score", "top", "n_groups", "keep_groups", "group_top", "renormalise")] + [("renorm_eps", C.c_float), ("scale", C.c_float)]
 
@@ -256,6 +267,15 @@ def load_library(build_if_missing: bool = True):
         "cc_bench_timer_begin": (i32, [vp]),
         "cc_bench_timer_end": (i32, [vp, C.POINTER(f32)]),
     }
+    sig.update({          # several sequences in pages (include/crabml_paged.h), 8-bit products
+        "cc_tensor_data": (vp, [vp]),
+        "cc_page_plan_create": (i32, [vp, C.POINTER(cc_page_plan_desc), pp]),
+        "cc_page_plan_release": (None, [vp]),
+        "cc_page_plan_tokens": (i64, [vp]),
+        "cc_paged_append": (i32, [vp, vp, C.POINTER(cc_paged_cache), pv, i32, pv, i32, pv, i32, i32, pv, i32, i32, f32, pp]),
+        "cc_paged_attention": (i32, [vp, vp, C.POINTER(cc_paged_cache), pv, i32, f32, i32, f32, pv, pp]),
+        "cc_product_i8": (i32, [vp, pv, pv, pv, pp]),
+    })
     sig.update({
         "ccr_runner_create": (i32, [vp, C.POINTER(ccr_llama_config), C.POINTER(ccr_llama_weights), i32, pp]),
         "ccr_runner_destroy": (None, [vp]),

@@ -110,6 +110,7 @@ extern "C" CC_API int cc_copy_rows_from(cc_device* dev, const cc_view* dst, cons
     int dt = dst->buf->dtype;
     CC_REQUIRE(dev, dt == CC_F32 || dt == CC_F16, "only f32/f16 can be copied to");
     int64_t cols = dst->shape[dst->ndim - 1];
+    CC_REQUIRE(dev, src->buf->dtype != CC_I8, "copy_rows_from: 8-bit codes have no values of their own");
     int be = cc_block_elems(src->buf->dtype);
     CC_REQUIRE(dev, cols % be == 0, "copy_rows_from: row length %lld is not block aligned", (long long)cols);
     CC_REQUIRE(dev, !cc_is_quant(src->buf->dtype) || cols == src->buf->cols, "copy_rows_from: row length %lld does not match the quantized matrix (%lld columns)",
@@ -256,6 +257,7 @@ extern "C" CC_API int cc_copy_rows_from_slot(cc_device* dev, const cc_view* dst,
     CC_REQUIRE(dev, dst->buf->pooled, "not owned");
     CC_REQUIRE(dev, view_contiguous(dst) && view_contiguous(src), "copy_rows_from_slot: tensors must be contiguous");
     CC_REQUIRE(dev, src->ndim == 2, "copy_rows_from_slot: src tensor is not 2d");
+    CC_REQUIRE(dev, src->buf->dtype != CC_I8, "copy_rows_from_slot: 8-bit codes have no values of their own");
     CC_REQUIRE(dev, slot >= 0 && slot < CC_N_SLOTS, "copy_rows_from_slot: slot %d out of range", slot);
     int dt = dst->buf->dtype;
     CC_REQUIRE(dev, dt == CC_F32 || dt == CC_F16, "only f32/f16 can be copied to");

@@ -47,6 +47,7 @@
 #define CC_MAX_PLANES 4
 #define CC_N_SLOTS 16
 #define CC_HISTORY_CAP 65536
+#define CC_PLAN_BUFFERS 4
 
 struct cc_device;
 
@@ -151,6 +152,13 @@ struct cc_device {
     // overlaps the DMA of the previous chunk and the repack kernels of the previous tensor
     void* up_pinned[2] = {nullptr, nullptr};
     cudaEvent_t up_ev[2] = {nullptr, nullptr};
+
+    // plans of steps over several sequences on their way to the device (paged.cu)
+    std::mutex plan_mu;
+    void* plan_pinned[CC_PLAN_BUFFERS] = {};
+    size_t plan_bytes[CC_PLAN_BUFFERS] = {};
+    cudaEvent_t plan_ev[CC_PLAN_BUFFERS] = {};
+    unsigned plan_turn = 0;
 
     // debug tap
     std::map<std::string, std::vector<float>> debug_tensors;

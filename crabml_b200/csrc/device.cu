@@ -4,6 +4,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include "../../include/crabml_seqops.h"
 #include "common.cuh"
 
 static std::string g_create_error;
@@ -21,7 +22,7 @@ int cc_fail(cc_device* dev, int code, const char* fmt, ...) {
 // ---- type facts (crabml-core/src/gguf.rs:86-108) ------------------
 int cc_block_elems(int t) {
     switch (t) {
-    case CC_F32: case CC_F16: case CC_BF16: case CC_I32: return 1;
+    case CC_F32: case CC_F16: case CC_BF16: case CC_I32: case CC_I8: return 1;
     case CC_Q4_0: case CC_Q4_1: case CC_Q5_0: case CC_Q5_1: case CC_Q8_0: case CC_Q8_1: return 32;
     case CC_Q2_K: case CC_Q3_K: case CC_Q4_K: case CC_Q5_K: case CC_Q6_K: case CC_Q8_K: return 256;
     }
@@ -29,7 +30,7 @@ int cc_block_elems(int t) {
 }
 size_t cc_block_bytes(int t) {
     switch (t) {
-    case CC_F32: case CC_I32: return 4; case CC_F16: case CC_BF16: return 2;
+    case CC_F32: case CC_I32: return 4; case CC_F16: case CC_BF16: return 2; case CC_I8: return 1;
     case CC_Q4_0: return 18; case CC_Q4_1: return 20; case CC_Q5_0: return 22; case CC_Q5_1: return 24;
     case CC_Q8_0: return 34; case CC_Q8_1: return 36;
     case CC_Q2_K: return 84; case CC_Q3_K: return 110; case CC_Q4_K: return 144; case CC_Q5_K: return 176;
@@ -122,6 +123,7 @@ extern "C" CC_API void cc_device_destroy(cc_device* dev) {
     if (dev->export_host) cudaFreeHost(dev->export_host);
     for (int i = 0; i < 2; i++) { if (dev->up_pinned[i]) cudaFreeHost(dev->up_pinned[i]); if (dev->up_ev[i]) cudaEventDestroy(dev->up_ev[i]); }
     for (int i = 0; i < 2; i++) { if (dev->rope_pinned[i]) cudaFreeHost(dev->rope_pinned[i]); if (dev->rope_ev[i]) cudaEventDestroy(dev->rope_ev[i]); }
+    for (int i = 0; i < CC_PLAN_BUFFERS; i++) { if (dev->plan_pinned[i]) cudaFreeHost(dev->plan_pinned[i]); if (dev->plan_ev[i]) cudaEventDestroy(dev->plan_ev[i]); }
     if (dev->err_host) cudaFreeHost(dev->err_host);
     if (dev->err_dev) cudaFree(dev->err_dev);
     if (dev->slots) cudaFree(dev->slots);
@@ -210,7 +212,7 @@ void cc_pool_free(cc_device* dev, void* p, size_t cls) {
 }
 
 int cc_new_activation(cc_device* dev, int64_t nelems, int dtype, bool zero, cc_buf** out) {
-    size_t esz = (dtype == CC_F32 || dtype == CC_I32) ? 4 : 2;
+    const size_t esz = cc_block_bytes(dtype);
     void* p = nullptr;
     size_t cls = 0;
     int rc = cc_pool_alloc(dev, (size_t)nelems * esz, &p, &cls);
@@ -272,6 +274,7 @@ extern "C" CC_API void cc_tensor_release(cc_buf* b) {
     delete b;
 }
 extern "C" CC_API int32_t cc_tensor_dtype(const cc_buf* b) { return b ? b->dtype : -1; }
+extern "C" CC_API void* cc_tensor_data(cc_buf* b) { return b && !cc_is_quant(b->dtype) ? b->plane[0] : nullptr; }
 extern "C" CC_API int64_t cc_tensor_capacity(const cc_buf* b) { return b ? b->nelems : 0; }
 
 static int64_t prod(const int64_t* shape, int ndim) {
@@ -283,7 +286,7 @@ static int64_t prod(const int64_t* shape, int ndim) {
 extern "C" CC_API int cc_tensor_alloc(cc_device* dev, const int64_t* shape, int32_t ndim, int32_t t, cc_buf** out) {
     if (!dev || !shape || !out || ndim < 1 || ndim > CC_MAX_DIMS) return cc_fail(dev, CC_ERR_ARG, "cc_tensor_alloc: bad argument");
     CC_ENTER(dev);
-    CC_REQUIRE(dev, t == CC_F32 || t == CC_F16 || t == CC_I32, "only f32/f16 is supported");   // cpu_tensor.rs:139-141; I32: index state of the sequence ops
+    CC_REQUIRE(dev, t == CC_F32 || t == CC_F16 || t == CC_I32 || t == CC_I8, "only f32/f16 is supported");   // cpu_tensor.rs:139-141; I32: index state of the sequence ops; I8: pages of codes
     // F32 is zero-filled (vec![0.0; n]); F16 is uninitialised in the reference (buf_f16.rs:23-28), zeroed here
     return cc_new_activation(dev, prod(shape, ndim), t, true, out);
 }

@@ -1,0 +1,296 @@
+// paged.cu -- pages of a cache that several sequences share (include/crabml_paged.h): the plan of a step, and what lies between the projections and the pages.
+//
+// The plan is checked on the host as a whole, so that no kernel meets a page or slot number that it would have to doubt, and copied to the device once a step.
+// The append's unit is a segment, the new tokens of one sequence in one block, times a job: one key head, one value head or some query heads.  A segment that
+// completes a block of an 8-bit cache has the whole block of a head in shared memory (old rows from the open block, new ones turned and rounded), so the largest
+// magnitude is known before a code is written and every number is rounded once.
+//
+// The turn is computed in 64 bits: a far position times a frequency loses its fraction in 32 (position 100000: 0.008 of a radian), and a key next to a rounding
+// border would get another code from another order of the same 32-bit operations.
+#include <math.h>
+#include <string.h>
+
+#include <algorithm>
+#include <new>
+
+#include "paged.cuh"
+
+// ---- the plan ---------------------------------------------------------------------------------------------------------------------------
+// pinned staging of plans on their way to the device, by turns; the oldest copy has to be through before its buffer is used again
+static int pg_upload(cc_device* dev, void* dst, const std::vector<uint8_t>& bytes) {
+    std::lock_guard<std::mutex> g(dev->plan_mu);
+    const int i = dev->plan_turn++ % CC_PLAN_BUFFERS;
+    if (!dev->plan_ev[i]) CC_CUDA(dev, cudaEventCreateWithFlags(&dev->plan_ev[i], cudaEventDisableTiming));
+    CC_CUDA(dev, cudaEventSynchronize(dev->plan_ev[i]));
+    if (dev->plan_bytes[i] < bytes.size()) {
+        if (dev->plan_pinned[i]) { CC_CUDA(dev, cudaFreeHost(dev->plan_pinned[i])); dev->plan_pinned[i] = nullptr; dev->plan_bytes[i] = 0; }
+        size_t n = 64 << 10;
+        while (n < bytes.size()) n *= 2;
+        CC_CUDA(dev, cudaMallocHost(&dev->plan_pinned[i], n));
+        dev->plan_bytes[i] = n;
+    }
+    memcpy(dev->plan_pinned[i], bytes.data(), bytes.size());
+    CC_CUDA(dev, cudaMemcpyAsync(dst, dev->plan_pinned[i], bytes.size(), cudaMemcpyHostToDevice, dev->stream));
+    CC_CUDA(dev, cudaEventRecord(dev->plan_ev[i], dev->stream));
+    return CC_OK;
+}
+
+static int pg_plan(cc_device* dev, const cc_page_plan_desc* d, cc_page_plan* p) {
+    if (d->n_seqs > 0 && (!d->pos0 || !d->counts || (d->table_cols > 0 && !d->table))) return cc_fail(dev, CC_ERR_ARG, "page_plan: a NULL array");
+    PgParts parts;
+    const std::string wrong = pg_build(*d, parts);
+    CC_REQUIRE(dev, wrong.empty(), "page_plan: %s", wrong.c_str());
+    p->dev = dev; p->n_seqs = d->n_seqs; p->page = d->page_size; p->table_cols = d->table_cols; p->n_pages = d->n_pages; p->n_slots = d->n_slots;
+    p->n_items = parts.n_items; p->tokens = parts.tokens;
+    while ((1 << p->shift) < p->page) p->shift++;
+    const size_t seg = parts.segments.size() * sizeof(PgSegment), sq = parts.seqs.size() * sizeof(PgSeq), tab = parts.table.size() * sizeof(int);
+    std::vector<uint8_t> bytes(seg + sq + tab + 16);
+    if (seg) memcpy(bytes.data(), parts.segments.data(), seg);
+    if (sq) memcpy(bytes.data() + seg, parts.seqs.data(), sq);
+    if (tab) memcpy(bytes.data() + seg + sq, parts.table.data(), tab);
+    p->seqs = std::move(parts.seqs);
+    int rc = cc_pool_alloc(dev, bytes.size(), &p->base, &p->cls);
+    if (!rc) rc = pg_upload(dev, p->base, bytes);
+    if (rc) return rc;
+    p->d_segments = (const PgSegment*)p->base;
+    p->d_seqs = (const PgSeq*)((uint8_t*)p->base + seg);
+    p->d_table = (const int*)((uint8_t*)p->base + seg + sq);
+    return CC_OK;
+}
+extern "C" CC_API int cc_page_plan_create(cc_device* dev, const cc_page_plan_desc* desc, cc_page_plan** out) {
+    if (!dev) return CC_ERR_ARG;
+    CC_ENTER(dev);
+    if (!desc || !out) return cc_fail(dev, CC_ERR_ARG, "page_plan: a NULL argument");
+    *out = nullptr;
+    if (LAZY(dev)) return cc_fail(dev, CC_ERR_UNSUPPORTED, "page_plan: not available on a lazy (graph / megakernel) device");
+    cc_page_plan* p = new (std::nothrow) cc_page_plan();
+    if (!p) return cc_fail(dev, CC_ERR_ARG, "page_plan: out of memory");
+    int rc;
+    try {
+        rc = pg_plan(dev, desc, p);
+    } catch (const std::bad_alloc&) {
+        rc = cc_fail(dev, CC_ERR_ARG, "page_plan: out of memory");
+    }
+    if (rc) { cc_page_plan_release(p); return rc; }
+    *out = p;
+    return CC_OK;
+}
+extern "C" CC_API void cc_page_plan_release(cc_page_plan* plan) {
+    if (!plan) return;
+    if (plan->base) cc_pool_free(plan->dev, plan->base, plan->cls);
+    delete plan;
+}
+extern "C" CC_API int64_t cc_page_plan_tokens(const cc_page_plan* plan) { return plan ? plan->tokens : 0; }
+
+// ---- a cache's views ----------------------------------------------------------------------------------------------------------------------
+static int pg_check_pages(cc_device* dev, const cc_view* v, int dtype, int ndim, const char* what, const char* name) {
+    if (!view_ok(v)) return cc_fail(dev, CC_ERR_ARG, "%s: bad view of %s", what, name);
+    CC_REQUIRE(dev, view_in_bounds(v) && view_contiguous(v) && v->ndim == ndim, "%s: %s is not a contiguous tensor of %d dimensions inside its buffer", what, name, ndim);
+    CC_REQUIRE(dev, v->buf->dev == dev, "%s: %s is another device's", what, name);
+    CC_REQUIRE(dev, v->buf->dtype == dtype, "%s: %s has type %d, not %d", what, name, v->buf->dtype, dtype);
+    CC_REQUIRE(dev, ((uintptr_t)v->buf->plane[0] & 15) == 0, "%s: %s does not start at a multiple of 16 bytes", what, name);
+    return CC_OK;
+}
+int pg_check_cache(cc_device* dev, const cc_page_plan* plan, const cc_paged_cache* c, const char* what, PgCache* o) {
+    if (!c || !view_ok(&c->k) || !view_ok(&c->v)) return cc_fail(dev, CC_ERR_ARG, "%s: bad cache", what);
+    const int type = c->k.buf->dtype;
+    CC_REQUIRE(dev, type == CC_F16 || type == CC_I8, "%s: pages of type %d (F16 or I8)", what, type);
+    int rc = pg_check_pages(dev, &c->k, type, 4, what, "k");
+    if (!rc) rc = pg_check_pages(dev, &c->v, type, 4, what, "v");
+    if (rc) return rc;
+    const int64_t G = c->k.shape[1], dk = c->k.shape[3], dv = c->v.shape[3];
+    CC_REQUIRE(dev, c->k.shape[0] == c->v.shape[0] && c->v.shape[1] == G && c->k.shape[2] == plan->page && c->v.shape[2] == plan->page,
+               "%s: k and v are not [pages, heads, %d, size] alike", what, plan->page);
+    CC_REQUIRE(dev, c->k.shape[0] >= plan->n_pages, "%s: %lld pages, the plan has %lld", what, (long long)c->k.shape[0], (long long)plan->n_pages);
+    CC_REQUIRE(dev, G >= 1 && G <= 1024 && dk >= 16 && dk <= 256 && dk % 16 == 0 && dv >= 16 && dv <= 256 && dv % 16 == 0,
+               "%s: %lld heads of %lld and %lld (multiples of 16 up to 256)", what, (long long)G, (long long)dk, (long long)dv);
+    *o = PgCache{};
+    o->k = c->k.buf->plane[0]; o->v = c->v.buf->plane[0]; o->G = (int)G; o->dk = (int)dk; o->dv = (int)dv; o->i8 = type == CC_I8;
+    if (!o->i8) return CC_OK;
+    const cc_view* more[4] = {&c->k_scale, &c->v_scale, &c->k_open, &c->v_open};
+    const char* names[4] = {"k_scale", "v_scale", "k_open", "v_open"};
+    for (int i = 0; i < 4 && !rc; i++) rc = pg_check_pages(dev, more[i], i < 2 ? CC_F32 : CC_F16, i < 2 ? 2 : 4, what, names[i]);
+    if (rc) return rc;
+    for (int i = 0; i < 2; i++) {
+        const cc_view *s = more[i], *w = more[2 + i];
+        CC_REQUIRE(dev, s->shape[0] >= plan->n_pages && s->shape[1] == G, "%s: %s is not [pages, heads]", what, names[i]);
+        CC_REQUIRE(dev, plan->n_slots > 0 || plan->n_seqs == 0, "%s: 8-bit pages need a plan with slots", what);
+        CC_REQUIRE(dev, w->shape[0] >= 2 * plan->n_slots && w->shape[1] == G && w->shape[2] == plan->page && w->shape[3] == (i ? dv : dk),
+                   "%s: %s is not [2 * %lld, %lld, %d, size]", what, names[2 + i], (long long)plan->n_slots, (long long)G, plan->page);
+    }
+    o->ks = (float*)c->k_scale.buf->plane[0]; o->vs = (float*)c->v_scale.buf->plane[0];
+    o->ko = (__half*)c->k_open.buf->plane[0]; o->vo = (__half*)c->v_open.buf->plane[0];
+    return CC_OK;
+}
+
+// ---- append --------------------------------------------------------------------------------------------------------------------------------
+#define PA_THREADS 256
+struct PaArgs {
+    const PgSegment* segments;
+    const float *q, *k, *v, *freq;
+    float* qo;
+    uint8_t *kp, *vp;
+    float *ks, *vs;
+    __half *ko, *vo;
+    int64_t qrs, krs, vrs;                   // row strides
+    int H, G, dk, dv, page, pairs, offset, step, gap, hq, q_jobs;        // pair i: columns offset + step * i and + gap behind it; hq: query heads of a job
+    double mag;
+};
+// F16 of a 32-bit number; what is finite stays finite
+__device__ __forceinline__ __half pa_half(float x) {
+    __half h = __float2half_rn(x);
+    if (__hisinf(h) && !isinf(x)) h = __ushort_as_half((unsigned short)(x > 0.0f ? 0x7bff : 0xfbff));
+    return h;
+}
+// cos and sin of the pairs of rows pos0 .. in 64 bits
+__device__ __forceinline__ void pa_angles(double2* cs, const PaArgs& a, int pos0, int rows) {
+    for (int e = threadIdx.x; e < rows * a.pairs; e += PA_THREADS) {
+        const int r = e / a.pairs, i = e - r * a.pairs;
+        double s, c;
+        sincos((double)(pos0 + r) * (double)a.freq[i], &s, &c);
+        cs[e] = make_double2(c * a.mag, s * a.mag);
+    }
+}
+#define PA_ROWS 16                           // rows of angles that are made at a time
+// every column of a head's row through `put` (column, number), turned where it belongs to a pair.  unit e: pair e, or one of the columns that stay
+template <class Put>
+__device__ __forceinline__ void pa_unit(const PaArgs& a, const float* row, int e, const double2* cs, Put put) {
+    if (e < a.pairs) {
+        const int c = a.offset + a.step * e;
+        const double x = (double)row[c], y = (double)row[c + a.gap];
+        put(c, (float)fma(x, cs[e].x, -(y * cs[e].y)));
+        put(c + a.gap, (float)fma(x, cs[e].y, y * cs[e].x));
+    } else {
+        int c = e - a.pairs;
+        if (c >= a.offset) c += 2 * a.pairs;
+        put(c, row[c]);
+    }
+}
+// grid (items, jobs): jobs 0 .. G - 1 key heads, then G value heads, then query heads by hq
+template <bool I8>
+__global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const PaArgs a) {
+    extern __shared__ __align__(16) uint8_t pa_sm[];
+    double2* cs = (double2*)pa_sm;                              // [PA_ROWS][pairs]
+    __half* block = (__half*)(pa_sm + (size_t)PA_ROWS * a.pairs * sizeof(double2));      // [page][d]
+    __shared__ unsigned top;
+    const int job = blockIdx.y, tid = threadIdx.x;
+    const bool is_k = job < a.G, is_v = !is_k && job < 2 * a.G;
+    pdl_enter();
+    for (int at = blockIdx.x; at >= 0;) {
+        const PgSegment g = a.segments[at];
+        at = g.next;
+        if (!is_k && !is_v) {                                   // query heads
+            const int h0 = (job - 2 * a.G) * a.hq, nh = min(a.hq, a.H - h0), units = a.dk - a.pairs;
+            for (int r0 = 0; r0 < g.rows; r0 += PA_ROWS) {
+                const int n = min(PA_ROWS, g.rows - r0);
+                pa_angles(cs, a, g.pos0 + r0, n);
+                __syncthreads();
+                for (int e = tid; e < n * nh * units; e += PA_THREADS) {
+                    const int rh = e / units, u = e - rh * units, r = rh / nh, h = h0 + rh - r * nh;
+                    const int64_t t = g.token0 + r0 + r;
+                    float* dst = a.qo + (t * a.H + h) * a.dk;
+                    pa_unit(a, a.q + t * a.qrs + (int64_t)h * a.dk, u, cs + r * a.pairs, [&](int c, float x) { dst[c] = x; });
+                }
+                __syncthreads();
+            }
+            continue;
+        }
+        const int head = is_k ? job : job - a.G, d = is_k ? a.dk : a.dv, units = is_k ? a.dk - a.pairs : a.dv;
+        const float* src = is_k ? a.k : a.v;
+        const int64_t rs = is_k ? a.krs : a.vrs;
+        const size_t page_at = ((size_t)g.page * a.G + head) * a.page * d;
+        const size_t open_at = ((size_t)g.half * a.G + head) * a.page * d;
+        __half* open = I8 ? (is_k ? a.ko : a.vo) + open_at : nullptr;
+        __half* rows = I8 ? block : (__half*)(is_k ? a.kp : a.vp) + page_at;      // 16-bit pages: straight to their place
+        if (I8 && (g.flags & PG_FULL))                          // the block's older rows
+            for (int e = tid; e < g.row0 * d; e += PA_THREADS) block[e] = open[e];
+        if (tid == 0) top = 0;
+        for (int r0 = 0; r0 < g.rows; r0 += PA_ROWS) {
+            const int n = min(PA_ROWS, g.rows - r0);
+            if (is_k) pa_angles(cs, a, g.pos0 + r0, n);
+            __syncthreads();
+            for (int e = tid; e < n * units; e += PA_THREADS) {
+                const int r = e / units, u = e - r * units;
+                const float* row = src + (int64_t)(g.token0 + r0 + r) * rs + (int64_t)head * d;
+                __half* dst = rows + (size_t)(g.row0 + r0 + r) * d;
+                if (is_k) pa_unit(a, row, u, cs + r * a.pairs, [&](int c, float x) { dst[c] = pa_half(x); });
+                else dst[u] = pa_half(row[u]);
+            }
+            __syncthreads();
+        }
+        if (!I8) continue;
+        if (g.flags & PG_KEPT)
+            for (int e = tid; e < g.rows * d; e += PA_THREADS) open[g.row0 * d + e] = block[g.row0 * d + e];
+        if (g.flags & PG_FULL) {
+            unsigned m = 0;
+            for (int e = tid; e < a.page * d; e += PA_THREADS) m = max(m, (unsigned)__half_as_ushort(block[e]) & 0x7fffu);
+            m = __reduce_max_sync(0xffffffffu, m);
+            if ((tid & 31) == 0) atomicMax(&top, m);
+            __syncthreads();
+            const bool finite = top < 0x7c00u;
+            const float most = __half2float(__ushort_as_half((unsigned short)top));
+            // numbers and their largest have 11 bits: 127 x is exact, and a quotient that is not a tie is further from one than a 32-bit division errs
+            int8_t* codes = (int8_t*)(is_k ? a.kp : a.vp) + page_at;
+            for (int e = tid; e < a.page * d; e += PA_THREADS) codes[e] = finite && top ? (int8_t)rintf(__half2float(block[e]) * 127.0f / most) : (int8_t)0;
+            if (tid == 0) (is_k ? a.ks : a.vs)[(size_t)g.page * a.G + head] = finite ? most / 127.0f : NAN;
+        }
+        __syncthreads();                                        // the block and `top`, before the next segment
+    }
+}
+extern "C" CC_API int cc_paged_append(cc_device* dev, const cc_page_plan* plan, const cc_paged_cache* cache, const cc_view* q_src, int32_t q_col0, const cc_view* k_src,
+                                      int32_t k_col0, const cc_view* v_src, int32_t v_col0, int32_t H, const cc_view* freq, int32_t pairing, int32_t offset, float mag,
+                                      cc_buf** out) {
+    PG_ENTER(dev, plan, "paged_append");
+    if (!out) return cc_fail(dev, CC_ERR_ARG, "paged_append: out is NULL");
+    *out = nullptr;
+    PgCache c;
+    int rc = pg_check_cache(dev, plan, cache, "paged_append", &c);
+    if (rc) return rc;
+    PG_ROWS(dev, k_src, "paged_append keys"); PG_ROWS(dev, v_src, "paged_append values");
+    if (q_src) PG_ROWS(dev, q_src, "paged_append queries");
+    const int64_t T = plan->tokens;
+    CC_REQUIRE(dev, k_src->shape[0] == T && v_src->shape[0] == T && (!q_src || q_src->shape[0] == T), "paged_append: the plan has %lld tokens, not the sources' rows", (long long)T);
+    CC_REQUIRE(dev, !q_src || (H > 0 && H <= 65536 && H % c.G == 0), "paged_append: %d query heads over %d", H, c.G);
+    CC_REQUIRE(dev, k_col0 >= 0 && v_col0 >= 0 && k_col0 + (int64_t)c.G * c.dk <= k_src->shape[1] && v_col0 + (int64_t)c.G * c.dv <= v_src->shape[1] &&
+               (!q_src || (q_col0 >= 0 && q_col0 + (int64_t)H * c.dk <= q_src->shape[1])), "paged_append: columns %d / %d / %d do not fit %d and %d heads of %d and %d", q_col0,
+               k_col0, v_col0, H, c.G, c.dk, c.dv);
+    CC_REQUIRE(dev, pairing == CC_ROPE_NEIGHBOURS || pairing == CC_ROPE_HALVES, "paged_append: pairing %d", pairing);
+    int64_t pairs = 0;
+    if (freq) {
+        if (!view_ok(freq)) return cc_fail(dev, CC_ERR_ARG, "paged_append: bad view of freq");
+        CC_REQUIRE(dev, view_in_bounds(freq) && view_contiguous(freq) && freq->buf->dev == dev && freq->buf->dtype == CC_F32, "paged_append: freq is not contiguous F32 of this device");
+        pairs = view_len(freq);
+        CC_REQUIRE(dev, offset >= 0 && offset + 2 * pairs <= c.dk, "paged_append: %lld pairs from column %d do not fit heads of %d", (long long)pairs, offset, c.dk);
+    }
+    cc_buf* o = nullptr;
+    if (q_src) {
+        rc = cc_new_activation(dev, T * H * c.dk, CC_F32, false, &o);
+        if (rc) return rc;
+    }
+    if (T > 0) {
+        PaArgs a{};
+        a.segments = plan->d_segments;
+        if (q_src) { a.q = (const float*)q_src->buf->plane[0] + q_col0; a.qrs = q_src->strides[0]; a.qo = (float*)o->base; }
+        a.k = (const float*)k_src->buf->plane[0] + k_col0; a.krs = k_src->strides[0];
+        a.v = (const float*)v_src->buf->plane[0] + v_col0; a.vrs = v_src->strides[0];
+        a.freq = freq ? (const float*)freq->buf->plane[0] : nullptr;
+        a.kp = c.k; a.vp = c.v; a.ks = c.ks; a.vs = c.vs; a.ko = c.ko; a.vo = c.vo;
+        a.H = q_src ? H : 0; a.G = c.G; a.dk = c.dk; a.dv = c.dv; a.page = plan->page; a.pairs = (int)pairs; a.offset = offset; a.mag = (double)mag;
+        a.step = pairing == CC_ROPE_NEIGHBOURS ? 2 : 1; a.gap = pairing == CC_ROPE_NEIGHBOURS ? 1 : (int)pairs;
+        a.hq = 4; a.q_jobs = (a.H + a.hq - 1) / a.hq;
+        const size_t smem = (size_t)PA_ROWS * a.pairs * sizeof(double2) + (c.i8 ? (size_t)a.page * std::max(c.dk, c.dv) * 2 : 0);
+        const dim3 grid((unsigned)plan->n_items, (unsigned)(2 * c.G + a.q_jobs));
+        cudaError_t e;
+        if (c.i8) {
+            e = cudaFuncSetAttribute(paged_append_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            if (e == cudaSuccess) e = cc_launch_pdl(dev, paged_append_kernel<true>, grid, PA_THREADS, smem, a);
+        } else e = cc_launch_pdl(dev, paged_append_kernel<false>, grid, PA_THREADS, smem, a);
+        dev->launches++;
+        if (e != cudaSuccess) {
+            if (o) cc_tensor_release(o);
+            return cc_fail(dev, CC_ERR_CUDA, "paged_append: %s", cudaGetErrorString(e));
+        }
+    }
+    *out = o;
+    return CC_OK;
+}

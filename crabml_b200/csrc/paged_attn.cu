@@ -1,0 +1,585 @@
+// paged_attn.cu -- attention over the pages of a cache (include/crabml_paged.h).
+//
+// 32-bit results from 16-bit tensor-core products.  Codes and 16-bit numbers are exact as f16 operands; a query or weight x is two of them, h = f16(x) and
+// l = f16(x - h), 22 bits together.  A query row is first brought near 2^14 by a power of two, weights are at most 2^12, so that l keeps its bits.
+//
+// Few rows (paged_few_kernel; a row is a query of one head).  mma.sync.m16n8k16 has room for 16 rows: eight rows' h above, the same rows' l below, and both
+// products are one instruction whose accumulators a thread adds up itself.  A warp takes 16 keys at a time.  Its lanes keep, read and convert the pieces of the
+// cache that the instruction's layout gives them and no others: which four columns of a row a lane puts into a step is free as long as queries and keys agree, and so
+// is the order of the value columns, so a lane takes 16 neighbouring bytes of a row, and the way through shared memory (cp.async, a ring per warp) needs no barrier.
+#include <math.h>
+
+#include <algorithm>
+
+#include "paged.cuh"
+
+#define PT_WARPS 4
+#define PT_THREADS (PT_WARPS * 32)
+#define PT_SHIFT 12.0f                        // weights are exp2(score - largest + PT_SHIFT)
+#define PT_MOST_SPLIT 2048                    // keys of a slice
+#define PT_LOG2E 1.4426950408889634f
+
+struct PtArgs {
+    const PgSeq* seqs;
+    const int* table;
+    const uint8_t *k, *v;
+    const float *ks, *vs, *q, *sink;
+    const __half *ko, *vo;
+    float *out, *part;                        // part: [item][head][8][dvp] sums of a slice, behind them ml
+    float2* ml;                               // [item][head][8]: largest score (base 2) and sum of weights
+    float scale, softcap;
+    int n_seqs, table_cols, page, shift, H, G, R, dk, dv, window, split, rows_lo, rows_hi;
+};
+struct PtItem { int seq, split, tile, n_split; };
+
+// keys [from, to) that the sequence's new tokens see together, from at a multiple of 16
+__host__ __device__ __forceinline__ void pt_range(const PgSeq& s, int window, int* from, int* to) {
+    *to = s.pos0 + s.count;
+    *from = window > 0 && s.pos0 - window + 1 > 0 ? (s.pos0 - window + 1) & ~15 : 0;
+}
+__host__ __device__ __forceinline__ int pt_splits(const PgSeq& s, const PtArgs& a) {
+    const int64_t rows = (int64_t)s.count * a.R;
+    if (rows < a.rows_lo || rows > a.rows_hi) return 0;
+    int from, to;
+    pt_range(s, a.window, &from, &to);
+    return (to - from + a.split - 1) / a.split;
+}
+// the place of number n in the sequences' counts: every lane gets the sequence and what is left of n
+template <class Count>
+__device__ __forceinline__ int pt_find(const PtArgs& a, int n, Count count, int* rest) {
+    const int lane = threadIdx.x & 31;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
+        const int s = s0 + lane, mine = s < a.n_seqs ? count(a.seqs[s]) : 0;
+        int sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const int x = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += x;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, n < sum);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            *rest = n - __shfl_sync(0xffffffffu, sum - mine, l);
+            return s0 + l;
+        }
+        n -= __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return -1;
+}
+
+__device__ __forceinline__ void pt_copy16(unsigned dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void pt_copy8(unsigned dst, const void* src, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(there ? 8 : 0) : "memory");
+}
+__device__ __forceinline__ void pt_mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// two 8-bit numbers, 128 added to each, in the bytes that `pick` takes, as f16: 1024 + 128 + x is 0x6400 | byte, and 1152 leaves exactly
+__device__ __forceinline__ unsigned pt_half2(unsigned biased, unsigned pick) {
+    const unsigned u = __byte_perm(biased, 0x64646464u, pick);
+    const __half2 h = __hsub2(*(const __half2*)&u, __floats2half2_rn(1152.0f, 1152.0f));
+    return *(const unsigned*)&h;
+}
+__device__ __forceinline__ unsigned pt_pack(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *(const unsigned*)&h;
+}
+// x, y as f16 (h) and what is left of them as f16 (l)
+__device__ __forceinline__ void pt_cut(float x, float y, unsigned& h, unsigned& l) {
+    const __half2 a = __floats2half2_rn(x, y);
+    const float2 b = __half22float2(a);
+    h = *(const unsigned*)&a;
+    l = pt_pack(x - b.x, y - b.y);
+}
+// halves that are an infinity or a NaN: as a mask of 16 ones each
+__device__ __forceinline__ unsigned pt_wild(unsigned u) {
+    return ((u & 0x7c00u) == 0x7c00u ? 0xffffu : 0u) | ((u & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u);
+}
+
+// what a warp keeps of its eight rows
+template <int D>
+struct PtRows {
+    unsigned q[D / 16][4];                    // h and l of the lane's columns, as the instruction takes them
+    float o[D / 8][4];                        // sums of weighted values: tile i, columns 2 t and 2 t + 1 of its eight, rows h and l
+    float inv, m, l, vref, ivref;             // power of two that q was divided by; largest score so far; the lane's sum of weights; power of two at the largest value factor so far
+    int pos, lo;                              // the row's position and the first key it sees (pos -1: no row)
+};
+// 16 scores of the row -> weights; x: raw sums of keys 2 t, 2 t + 1, 8 + 2 t, 9 + 2 t.  kf, vf: the keys' and values' factors.  edge: some row does not see some key
+template <int D>
+__device__ __forceinline__ void pt_weights(PtRows<D>& r, float (&x)[4], int key0, float kf, float vf, bool edge, const PtArgs& a, unsigned (&p)[4], unsigned& seen) {
+    const int t = threadIdx.x & 3;
+    const float f = a.softcap > 0.0f ? r.inv * kf * a.scale : r.inv * kf * (a.scale * PT_LOG2E);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        x[i] *= f;
+        if (a.softcap > 0.0f) x[i] = a.softcap * tanhf(x[i] / a.softcap) * PT_LOG2E;
+    }
+    seen = 15u;
+    if (edge) {
+        seen = 0u;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int key = key0 + (i >> 1) * 8 + 2 * t + (i & 1);
+            if (key <= r.pos && key >= r.lo) seen |= 1u << i;
+            else x[i] = -INFINITY;
+        }
+    }
+    float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    const float m = fmaxf(r.m, mx);
+    // the largest value factor so far, as the power of two below it: a block that the row does not see leaves its bits as they are
+    const float vp = fminf(fmaxf(__uint_as_float(__float_as_uint(vf) & 0x7f800000u), 0x1p-100f), 0x1p100f);
+    const bool up = m > r.m, wider = vp > r.vref && vf > 0.0f;
+    if (__any_sync(0xffffffffu, up || wider)) {
+        float alpha = r.m == -INFINITY ? 0.0f : exp2f(r.m - m);
+        if (m == r.m) alpha = 1.0f;
+        r.l *= alpha;
+        if (wider) {
+            alpha *= r.vref / vp;
+            r.vref = vp; r.ivref = 1.0f / vp;
+        }
+        r.m = m;
+#pragma unroll
+        for (int i = 0; i < D / 8; i++) { r.o[i][0] *= alpha; r.o[i][1] *= alpha; r.o[i][2] *= alpha; r.o[i][3] *= alpha; }
+    }
+    const float base = m == -INFINITY ? 0.0f : m - PT_SHIFT, vr = vf * r.ivref;
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = exp2f(x[i] - base);
+    r.l += (x[0] + x[1]) + (x[2] + x[3]);
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = seen & (1u << i) ? x[i] * vr : 0.0f;
+    pt_cut(x[0], x[1], p[0], p[1]);
+    pt_cut(x[2], x[3], p[2], p[3]);
+}
+
+// ---- 16 keys of 8-bit codes ----------------------------------------------------------------------------------------------------------------
+template <int D>
+struct PtI8 {
+    static constexpr int KC = D / 64, VB = D == 64 ? 8 : 16, VC = D == 64 ? 1 : D / 128, BYTES = 32 * D;
+    static __device__ __forceinline__ void load(unsigned st, const uint8_t* k, const uint8_t* v, const PtArgs& a) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int c = 0; c < KC; c++) {
+                const bool in = c * 64 + t * 16 < a.dk;
+                pt_copy16(st + (j * KC + c) * 512 + lane * 16, in ? k + (8 * j + g) * a.dk + c * 64 + t * 16 : k, in);
+            }
+        st += 2 * KC * 512;
+#pragma unroll
+        for (int x = 0; x < 4; x++)
+#pragma unroll
+            for (int c = 0; c < VC; c++) {
+                const int col = c * 128 + g * VB, key = 2 * t + (x & 1) + (x >> 1) * 8;
+                const bool in = col < a.dv;
+                if (VB == 8) pt_copy8(st + x * 256 + lane * 8, in ? v + key * a.dv + col : v, in);
+                else pt_copy16(st + (x * VC + c) * 512 + lane * 16, in ? v + key * a.dv + col : v, in);
+            }
+    }
+    static __device__ __forceinline__ void use(PtRows<D>& r, const uint8_t* st, int key0, float kf, float vf, bool edge, const PtArgs& a) {
+        const int lane = threadIdx.x & 31;
+        float s[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < KC; c++) {
+                const uint4 w4 = *(const uint4*)(st + (j * KC + c) * 512 + lane * 16);
+                const unsigned w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const unsigned u = w[e] ^ 0x80808080u;
+                    pt_mma(s[j], r.q[c * 4 + e], pt_half2(u, 0x4140), pt_half2(u, 0x4342));
+                }
+            }
+        }
+        float x[4] = {s[0][0] + s[0][2], s[0][1] + s[0][3], s[1][0] + s[1][2], s[1][1] + s[1][3]};
+        unsigned p[4], seen;
+        pt_weights<D>(r, x, key0, kf, vf, edge, a, p, seen);
+        st += 2 * KC * 512;
+#pragma unroll
+        for (int c = 0; c < VC; c++) {
+            unsigned w[4][4];
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+                if (VB == 8) {
+                    const uint2 v = *(const uint2*)(st + y * 256 + lane * 8);
+                    w[y][0] = v.x ^ 0x80808080u; w[y][1] = v.y ^ 0x80808080u;
+                } else {
+                    const uint4 v = *(const uint4*)(st + (y * VC + c) * 512 + lane * 16);
+                    w[y][0] = v.x ^ 0x80808080u; w[y][1] = v.y ^ 0x80808080u; w[y][2] = v.z ^ 0x80808080u; w[y][3] = v.w ^ 0x80808080u;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < VB / 4; e++) {
+                const unsigned a01 = __byte_perm(w[0][e], w[1][e], 0x5140), a23 = __byte_perm(w[0][e], w[1][e], 0x7362);
+                const unsigned b01 = __byte_perm(w[2][e], w[3][e], 0x5140), b23 = __byte_perm(w[2][e], w[3][e], 0x7362);
+                float(*o)[4] = r.o + c * 16 + e * 4;
+                pt_mma(o[0], p, pt_half2(a01, 0x4140), pt_half2(b01, 0x4140));
+                pt_mma(o[1], p, pt_half2(a01, 0x4342), pt_half2(b01, 0x4342));
+                pt_mma(o[2], p, pt_half2(a23, 0x4140), pt_half2(b23, 0x4140));
+                pt_mma(o[3], p, pt_half2(a23, 0x4342), pt_half2(b23, 0x4342));
+            }
+        }
+    }
+};
+// ---- 16 keys of 16-bit numbers.  WIDE: with the columns dealt out as for codes (a block that is open beside pages of codes) ------------------------------
+template <int D, bool WIDE>
+struct PtF16 {
+    static constexpr int EK = WIDE ? 16 : 8, KC = D / (4 * EK), KP = EK / 8;          // elements of a lane and chunk of a key row; 16-byte pieces of them
+    static constexpr int CW = WIDE && D >= 128 ? 128 : 64, VC = D / CW, VP = CW / 64, BYTES = 64 * D;
+    // rows from `there` on are zeros
+    static __device__ __forceinline__ void load(unsigned st, const __half* k, const __half* v, int there, const PtArgs& a) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int c = 0; c < KC; c++)
+#pragma unroll
+                for (int h = 0; h < KP; h++) {
+                    const int col = c * 4 * EK + t * EK + h * 8, key = 8 * j + g;
+                    const bool in = col < a.dk && key < there;
+                    pt_copy16(st + ((j * KC + c) * KP + h) * 512 + lane * 16, in ? k + key * a.dk + col : k, in);
+                }
+        st += 2 * KC * KP * 512;
+#pragma unroll
+        for (int x = 0; x < 4; x++)
+#pragma unroll
+            for (int c = 0; c < VC; c++)
+#pragma unroll
+                for (int h = 0; h < VP; h++) {
+                    const int col = c * CW + g * (CW / 8) + h * 8, key = 2 * t + (x & 1) + (x >> 1) * 8;
+                    const bool in = col < a.dv && key < there;
+                    pt_copy16(st + ((x * VC + c) * VP + h) * 512 + lane * 16, in ? v + key * a.dv + col : v, in);
+                }
+    }
+    static __device__ __forceinline__ void use(PtRows<D>& r, const uint8_t* st, int key0, bool edge, const PtArgs& a) {
+        const int lane = threadIdx.x & 31;
+        float s[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < KC * KP; c++) {
+                const uint4 w = *(const uint4*)(st + (j * KC * KP + c) * 512 + lane * 16);
+                pt_mma(s[j], r.q[c * 2], w.x, w.y);
+                pt_mma(s[j], r.q[c * 2 + 1], w.z, w.w);
+            }
+        }
+        float x[4] = {s[0][0] + s[0][2], s[0][1] + s[0][3], s[1][0] + s[1][2], s[1][1] + s[1][3]};
+        unsigned p[4], seen;
+        pt_weights<D>(r, x, key0, 1.0f, 1.0f, edge, a, p, seen);
+        st += 2 * KC * KP * 512;
+        // a value that is not finite must not meet a weight of zero in the sums of a row that does not see it
+        bool wild = false;
+        if (edge) {
+#pragma unroll 1
+            for (int y = 0; y < 4 * VC * VP; y++) {
+                const uint4 v = *(const uint4*)(st + y * 512 + lane * 16);
+                wild |= (pt_wild(v.x) | pt_wild(v.y) | pt_wild(v.z) | pt_wild(v.w)) != 0u;
+            }
+            wild = __any_sync(0xffffffffu, wild);
+        }
+#pragma unroll
+        for (int c = 0; c < VC * VP; c++) {
+            unsigned w[4][4];
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+                const uint4 v = *(const uint4*)(st + (y * VC * VP + c) * 512 + lane * 16);
+                w[y][0] = v.x; w[y][1] = v.y; w[y][2] = v.z; w[y][3] = v.w;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                unsigned b0 = __byte_perm(w[0][e / 2], w[1][e / 2], e & 1 ? 0x7632 : 0x5410), b1 = __byte_perm(w[2][e / 2], w[3][e / 2], e & 1 ? 0x7632 : 0x5410);
+                if (wild) {                                        // how many of them each row sees, by a product of ones; the sums of those that do are NaN
+                    const unsigned w0 = pt_wild(b0), w1 = pt_wild(b1);
+                    const unsigned ones[4] = {(seen & 1u ? 0x3c00u : 0u) | (seen & 2u ? 0x3c000000u : 0u), 0u, (seen & 4u ? 0x3c00u : 0u) | (seen & 8u ? 0x3c000000u : 0u), 0u};
+                    float n[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    pt_mma(n, ones, w0 & 0x3c003c00u, w1 & 0x3c003c00u);
+                    if (n[0] > 0.0f) r.o[c * 8 + e][0] = NAN;
+                    if (n[1] > 0.0f) r.o[c * 8 + e][1] = NAN;
+                    b0 &= ~w0; b1 &= ~w1;
+                }
+                pt_mma(r.o[c * 8 + e], p, b0, b1);
+            }
+        }
+    }
+};
+
+template <int D, bool I8>
+__global__ void __launch_bounds__(PT_THREADS) paged_few_kernel(const PtArgs a) {
+    using Mine = PtF16<D, I8>;                                     // 16-bit rows: pages, or the open block beside codes
+    constexpr int RING = 128 * D, STAGES = RING / Mine::BYTES, STAGES8 = RING / PtI8<D>::BYTES, CW = I8 && D >= 128 ? 128 : 64;
+    extern __shared__ __align__(16) uint8_t pt_sm[];
+    __shared__ int pid[PT_MOST_SPLIT / 16 + 1];
+    __shared__ float kfs[PT_MOST_SPLIT / 16 + 1], vfs[PT_MOST_SPLIT / 16 + 1];
+    __shared__ float2 ml[PT_WARPS][8];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, kvh = blockIdx.y;
+    uint8_t* ring = pt_sm + w * RING;
+    const unsigned ring_at = (unsigned)__cvta_generic_to_shared(ring);
+    pdl_enter();
+    int rest;
+    const int seq = pt_find(a, blockIdx.x, [&](const PgSeq& s) { return pt_splits(s, a) * (int)(((int64_t)s.count * a.R + 7) >> 3); }, &rest);
+    if (seq < 0) return;
+    const PgSeq s = a.seqs[seq];
+    const int rows = s.count * a.R, tiles = (rows + 7) >> 3, split = rest / tiles, tile = rest - split * tiles, n_split = pt_splits(s, a);
+    int from, to;
+    pt_range(s, a.window, &from, &to);
+    const int row = tile * 8 + g, tok = row / a.R, pos_first = s.pos0 + tile * 8 / a.R, pos_last = s.pos0 + (min(rows, tile * 8 + 8) - 1) / a.R;
+    const int k0 = from + split * a.split, k1 = min(min(to, k0 + a.split), pos_last + 1);       // keys of the slice that some row of the tile may see
+    const int lo = a.window > 0 ? max(k0, (pos_first - a.window + 1) & ~15) : k0, units = k1 > lo ? (k1 - lo + 15) >> 4 : 0;
+    const int p0 = lo >> a.shift, opens = I8 ? to >> a.shift << a.shift : 0;                  // the first key that is not in a page of codes
+    for (int i = threadIdx.x; units > 0 && i <= ((k1 - 1) >> a.shift) - p0; i += PT_THREADS) {
+        const int page = a.table[(int64_t)seq * a.table_cols + p0 + i];
+        pid[i] = page;
+        if (I8) { kfs[i] = a.ks[(int64_t)page * a.G + kvh]; vfs[i] = a.vs[(int64_t)page * a.G + kvh]; }
+    }
+    PtRows<D> r;
+    {                                                              // the lane's columns of its row
+        const bool in = row < rows;
+        const float* q = a.q + ((int64_t)(s.first + (in ? tok : 0)) * a.H + kvh * a.R + (in ? row - tok * a.R : 0)) * a.dk;
+        constexpr int E = I8 ? 16 : 8;
+        float v[D / 4], top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 4; i++) {
+            const int col = i / E * 4 * E + t * E + i % E;
+            v[i] = in && col < a.dk ? q[col] : 0.0f;
+            top = fmaxf(top, fabsf(v[i]));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        int ex = 14;
+        if (top > 0.0f && top < INFINITY) frexpf(top, &ex);
+        ex = max(ex, -100);
+        const float f = ldexpf(1.0f, 14 - ex);
+        r.inv = ldexpf(1.0f, ex - 14);
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) {
+            pt_cut(v[4 * i] * f, v[4 * i + 1] * f, r.q[i][0], r.q[i][1]);
+            pt_cut(v[4 * i + 2] * f, v[4 * i + 3] * f, r.q[i][2], r.q[i][3]);
+        }
+        r.pos = in ? s.pos0 + tok : -1;
+        r.lo = a.window > 0 ? r.pos - a.window + 1 : 0;
+        r.m = -INFINITY; r.l = 0.0f; r.vref = I8 ? 0.0f : 1.0f; r.ivref = I8 ? 0.0f : 1.0f;
+#pragma unroll
+        for (int i = 0; i < D / 8; i++) r.o[i][0] = r.o[i][1] = r.o[i][2] = r.o[i][3] = 0.0f;
+    }
+    __syncthreads();
+    const int units8 = I8 ? max(0, min(units, (opens - lo) >> 4)) : 0;
+    auto edge = [&](int key0) { return key0 + 15 > pos_first || (a.window > 0 && key0 < pos_last - a.window + 1); };
+    if constexpr (I8) {
+        auto load = [&](int u) {
+            if (u < units8) {
+                const int key0 = lo + u * 16, i = (key0 >> a.shift) - p0;
+                const size_t at = ((size_t)pid[i] * a.G + kvh) * a.page + (key0 & (a.page - 1));
+                PtI8<D>::load(ring_at + (u / PT_WARPS % STAGES8) * PtI8<D>::BYTES, a.k + at * a.dk, a.v + at * a.dv, a);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int i = 0; i < STAGES8 - 1; i++) load(w + i * PT_WARPS);
+        for (int u = w; u < units8; u += PT_WARPS) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES8 - 2) : "memory");
+            load(u + (STAGES8 - 1) * PT_WARPS);
+            const int key0 = lo + u * 16, i = (key0 >> a.shift) - p0;
+            PtI8<D>::use(r, ring + (u / PT_WARPS % STAGES8) * PtI8<D>::BYTES, key0, kfs[i], vfs[i], edge(key0), a);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    }
+    {
+        const __half *kb = I8 ? a.ko : (const __half*)a.k, *vb = I8 ? a.vo : (const __half*)a.v;
+        auto load = [&](int u) {
+            if (u < units) {
+                const int key0 = lo + u * 16, i = (key0 >> a.shift) - p0;
+                const size_t block = I8 ? (size_t)(2 * s.slot + ((to >> a.shift) & 1)) : (size_t)pid[i], at = (block * a.G + kvh) * a.page + (key0 & (a.page - 1));
+                Mine::load(ring_at + (u / PT_WARPS % STAGES) * Mine::BYTES, kb + at * a.dk, vb + at * a.dv, to - key0, a);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        const int first = units8 + (w - units8 % PT_WARPS + PT_WARPS) % PT_WARPS;             // this warp's first unit behind the codes
+        load(first);
+        for (int u = first; u < units; u += PT_WARPS) {
+            load(u + PT_WARPS);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            const int key0 = lo + u * 16;
+            Mine::use(r, ring + (u / PT_WARPS % STAGES) * Mine::BYTES, key0, edge(key0), a);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    }
+    // the warps' sums, in the order of the warps
+    r.l += __shfl_xor_sync(0xffffffffu, r.l, 1);
+    r.l += __shfl_xor_sync(0xffffffffu, r.l, 2);
+    __syncthreads();                                               // the rings are free
+    float* sums = (float*)pt_sm;                                   // [warp][8][D]
+#pragma unroll
+    for (int i = 0; i < D / 8; i++)
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            const int col = i / (CW / 8) * CW + (2 * t + x) * (CW / 8) + i % (CW / 8);
+            sums[(w * 8 + g) * D + col] = (r.o[i][x] + r.o[i][2 + x]) * r.vref;
+        }
+    if (t == 0) ml[w][g] = make_float2(r.m, r.l);
+    __syncthreads();
+    const int n = min(8, rows - tile * 8);
+    const size_t at = (size_t)blockIdx.x * a.G + kvh;
+    for (int e = threadIdx.x; e < n * a.dv; e += PT_THREADS) {
+        const int y = e / a.dv, col = e - y * a.dv;
+        float m = -INFINITY, l = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int x = 0; x < PT_WARPS; x++) m = fmaxf(m, ml[x][y].x);
+#pragma unroll
+        for (int x = 0; x < PT_WARPS; x++) {
+            const float f = ml[x][y].x == -INFINITY ? (ml[x][y].y == 0.0f ? 0.0f : 1.0f) : exp2f(ml[x][y].x - m);
+            l = fmaf(f, ml[x][y].y, l);
+            o = fmaf(f, sums[(x * 8 + y) * D + col], o);
+        }
+        if (n_split > 1) {
+            a.part[(at * 8 + y) * a.dv + col] = o;
+            if (col == 0) a.ml[at * 8 + y] = make_float2(m, l);
+            continue;
+        }
+        const int rr = tile * 8 + y, tk = rr / a.R, head = kvh * a.R + rr - tk * a.R;
+        if (a.sink) {
+            const float sk = a.sink[head] * PT_LOG2E, m2 = fmaxf(m, sk), f = m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : exp2f(m - m2);
+            l = f * l + (sk == -INFINITY ? 0.0f : exp2f(sk - m2 + PT_SHIFT));
+            o *= f;
+        }
+        a.out[((int64_t)(s.first + tk) * a.H + head) * a.dv + col] = o / l;
+    }
+}
+// the slices of a row added up: a CTA a row, its threads take 32 columns of 4 numbers ... by four groups of slices
+__global__ void __launch_bounds__(128) paged_sum_kernel(const PtArgs a) {
+    __shared__ float so[4][256];
+    __shared__ float2 sm[4];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, kvh = blockIdx.y;
+    pdl_enter();
+    int row, items = 0;
+    const int seq = pt_find(a, blockIdx.x, [&](const PgSeq& s) { return pt_splits(s, a) > 1 ? s.count * a.R : 0; }, &row);
+    if (seq < 0) return;
+    for (int x = lane; x < seq; x += 32) items += pt_splits(a.seqs[x], a) * ((a.seqs[x].count * a.R + 7) >> 3);
+    items = warp_sum_i(items);
+    const PgSeq s = a.seqs[seq];
+    const int tiles = (s.count * a.R + 7) >> 3, n = pt_splits(s, a), tile = row >> 3, y = row & 7;
+    auto at = [&](int x) { return ((size_t)(items + x * tiles + tile) * a.G + kvh) * 8 + y; };
+    float m = -INFINITY;
+    for (int x = lane; x < n; x += 32) m = fmaxf(m, a.ml[at(x)].x);
+    m = warp_max(m);
+    float l = 0.0f;
+    for (int c0 = 0; c0 < a.dv; c0 += 128) {
+        const int col = c0 + lane * 4;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float sum = 0.0f;
+#pragma unroll 4
+        for (int x = w; x < n; x += 4) {
+            const float2 z = a.ml[at(x)];
+            const float f = z.x == -INFINITY ? (z.y == 0.0f ? 0.0f : 1.0f) : exp2f(z.x - m);
+            sum = fmaf(f, z.y, sum);
+            if (col < a.dv) {
+                const float4 v = *(const float4*)(a.part + at(x) * a.dv + col);
+                o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
+            }
+        }
+        l = sum;
+        if (col < a.dv) *(float4*)&so[w][col] = o;
+    }
+    if (lane == 0) sm[w] = make_float2(m, l);
+    __syncthreads();
+    const int tok = row / a.R, head = kvh * a.R + row - tok * a.R;
+    l = ((sm[0].y + sm[1].y) + sm[2].y) + sm[3].y;
+    float f = 1.0f;
+    if (a.sink) {
+        const float sk = a.sink[head] * PT_LOG2E, m2 = fmaxf(m, sk);
+        f = m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : exp2f(m - m2);
+        l = f * l + (sk == -INFINITY ? 0.0f : exp2f(sk - m2 + PT_SHIFT));
+    }
+    for (int c = threadIdx.x; c < a.dv; c += 128)
+        a.out[((int64_t)(s.first + tok) * a.H + head) * a.dv + c] = (((so[0][c] + so[1][c]) + so[2][c]) + so[3][c]) * f / l;
+}
+
+template <int D, bool I8>
+static cudaError_t pt_launch_few(cc_device* dev, const PtArgs& a, unsigned items) {
+    constexpr int smem = PT_WARPS * 128 * D;
+    cudaError_t e = cudaFuncSetAttribute(paged_few_kernel<D, I8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) e = cc_launch_pdl(dev, paged_few_kernel<D, I8>, dim3(items, (unsigned)a.G), PT_THREADS, smem, a);
+    dev->launches++;
+    return e;
+}
+static int pt_few(cc_device* dev, const cc_page_plan* plan, PtArgs a, bool i8) {
+    int64_t keys = 0, items = 0, split_rows = 0;
+    for (const PgSeq& s : plan->seqs) {
+        const int64_t rows = (int64_t)s.count * a.R;
+        if (rows < a.rows_lo || rows > a.rows_hi) continue;
+        int from, to;
+        pt_range(s, a.window, &from, &to);
+        keys += (int64_t)(to - from) * ((rows + 7) / 8) * a.G;
+    }
+    if (!keys) return CC_OK;
+    const int64_t slots = (int64_t)dev->sm_count * 3;
+    int64_t each = (keys + slots - 1) / slots;
+    each = std::min<int64_t>(PT_MOST_SPLIT - 16, std::max<int64_t>(128, (each + 63) / 64 * 64));
+    if (each > 512) each = 512;
+    a.split = (int)each;
+    for (const PgSeq& s : plan->seqs) {
+        const int n = pt_splits(s, a);
+        items += (int64_t)n * (((int64_t)s.count * a.R + 7) / 8);
+        if (n > 1) split_rows += (int64_t)s.count * a.R;
+    }
+    CC_REQUIRE(dev, items < ((int64_t)1 << 31) && a.G <= 65535, "paged_attention: too many rows");
+    void* ws = nullptr; size_t cls = 0;
+    if (split_rows) {
+        const size_t part = (size_t)items * a.G * 8 * a.dv * sizeof(float), ml = (size_t)items * a.G * 8 * sizeof(float2);
+        const int rc = cc_pool_alloc(dev, part + ml, &ws, &cls);
+        if (rc) return rc;
+        a.part = (float*)ws; a.ml = (float2*)((uint8_t*)ws + part);
+    }
+    const int d = std::max(a.dk, a.dv);
+    cudaError_t e = i8 ? (d <= 64 ? pt_launch_few<64, true>(dev, a, (unsigned)items) : d <= 128 ? pt_launch_few<128, true>(dev, a, (unsigned)items) : pt_launch_few<256, true>(dev, a, (unsigned)items))
+                       : (d <= 64 ? pt_launch_few<64, false>(dev, a, (unsigned)items) : d <= 128 ? pt_launch_few<128, false>(dev, a, (unsigned)items) : pt_launch_few<256, false>(dev, a, (unsigned)items));
+    if (e == cudaSuccess && split_rows) {
+        e = cc_launch_pdl(dev, paged_sum_kernel, dim3((unsigned)split_rows, (unsigned)a.G), 128, 0, a);
+        dev->launches++;
+    }
+    if (ws) cc_pool_free(dev, ws, cls);
+    if (e != cudaSuccess) return cc_fail(dev, CC_ERR_CUDA, "paged_attention: %s", cudaGetErrorString(e));
+    return CC_OK;
+}
+
+extern "C" CC_API int cc_paged_attention(cc_device* dev, const cc_page_plan* plan, const cc_paged_cache* cache, const cc_view* q, int32_t H, float scale, int32_t window,
+                                         float softcap, const cc_view* sink, cc_buf** out) {
+    PG_ENTER(dev, plan, "paged_attention");
+    if (!out) return cc_fail(dev, CC_ERR_ARG, "paged_attention: out is NULL");
+    *out = nullptr;
+    PgCache c;
+    int rc = pg_check_cache(dev, plan, cache, "paged_attention", &c);
+    if (rc) return rc;
+    PG_ROWS(dev, q, "paged_attention q");
+    CC_REQUIRE(dev, view_contiguous(q), "paged_attention q: not contiguous");
+    const int64_t T = plan->tokens;
+    CC_REQUIRE(dev, H > 0 && H <= 65536 && H % c.G == 0, "paged_attention: %d query heads over %d", H, c.G);
+    CC_REQUIRE(dev, q->shape[0] == T && q->shape[1] == (int64_t)H * c.dk, "paged_attention: q is not [%lld, %d * %d]", (long long)T, H, c.dk);
+    if (sink) {
+        if (!view_ok(sink)) return cc_fail(dev, CC_ERR_ARG, "paged_attention: bad view of sink");
+        CC_REQUIRE(dev, view_in_bounds(sink) && view_contiguous(sink) && view_len(sink) == H && sink->buf->dtype == CC_F32 && sink->buf->dev == dev,
+                   "paged_attention: sink is not contiguous F32 [%d] of this device", H);
+    }
+    cc_buf* o = nullptr;
+    rc = cc_new_activation(dev, T * H * c.dv, CC_F32, false, &o);
+    if (rc) return rc;
+    if (T > 0) {
+        PtArgs a{};
+        a.seqs = plan->d_seqs; a.table = plan->d_table; a.k = c.k; a.v = c.v; a.ks = c.ks; a.vs = c.vs; a.ko = c.ko; a.vo = c.vo;
+        a.q = (const float*)q->buf->plane[0]; a.sink = sink ? (const float*)sink->buf->plane[0] : nullptr; a.out = (float*)o->base;
+        a.scale = scale; a.softcap = softcap; a.window = window > 0 ? window : 0;
+        a.n_seqs = plan->n_seqs; a.table_cols = plan->table_cols; a.page = plan->page; a.shift = plan->shift;
+        a.H = H; a.G = c.G; a.R = H / c.G; a.dk = c.dk; a.dv = c.dv;
+        a.rows_lo = 1; a.rows_hi = 0x7fffffff;
+        rc = pt_few(dev, plan, a, c.i8);
+    }
+    if (rc) { cc_tensor_release(o); return rc; }
+    *out = o;
+    return CC_OK;
+}

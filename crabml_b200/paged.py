@@ -1,0 +1,93 @@
+"""Python handles on include/crabml_paged.h: the plan of a step over several sequences, a layer's cache in pages of 16 or 8 bits, the append and the attention.
+
+    plan = PagePlan(dev, page_size=64, n_pages=n, table=pages_of_each_sequence, pos0=lengths, counts=new_tokens, n_slots=max_sequences)
+    for layer in layers:                                          # rows of qkv: the new tokens, sequence after sequence
+        q = append(plan, layer.cache, qkv, 0, qkv, H * d, qkv, (H + G) * d, H, freq=freq)
+        y = attention(plan, layer.cache, q, H, d ** -0.5)
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+
+from . import capi
+from .capi import TensorError
+from .tensor import CudaTensor, TensorStrider, _Buf
+
+
+class PagePlan:
+    """What the sequences of a step have in the cache (pos0), bring along (counts) and own (table: rows of page numbers, an array or lists of any lengths; slots:
+    their open blocks, sequence i slot i where it is None).  Checked once; every layer's append and attention take it."""
+
+    def __init__(self, device, page_size, n_pages, table, pos0, counts, n_slots=0, slots=None):
+        self.device, self.handle = device, None
+        counts = np.ascontiguousarray(counts, np.int32).reshape(-1)
+        pos0 = np.ascontiguousarray(pos0, np.int64).reshape(-1)
+        n = len(counts)
+        if not isinstance(table, np.ndarray):
+            rows, width = [list(r) for r in table], max([len(r) for r in table], default=0)
+            table = np.full((len(rows), width), -1, np.int32)       # a page that is needed and was not given is refused
+            for i, r in enumerate(rows):
+                table[i, :len(r)] = r
+        if len(pos0) != n or table.ndim != 2 or len(table) != n or (slots is not None and len(slots) != n):
+            raise TensorError(f"page_plan: {n} counts, {len(pos0)} positions, table {table.shape}" + ("" if slots is None else f", {len(slots)} slots"))
+        if table.size and (table.min() < -(1 << 31) or table.max() >= 1 << 31):
+            raise TensorError("page_plan: page numbers of more than 32 bits")
+        table = np.ascontiguousarray(table, np.int32)
+        slots = None if slots is None else np.ascontiguousarray(slots, np.int32)
+        d = capi.cc_page_plan_desc(n, int(page_size), table.shape[1], int(n_pages), int(n_slots), *(None if a is None else a.ctypes.data for a in (pos0, counts, table, slots)))
+        h = C.c_void_p()
+        device.check(device.lib.cc_page_plan_create(device.handle, C.byref(d), C.byref(h)))
+        self.handle = h
+        self.tokens = int(device.lib.cc_page_plan_tokens(h))
+
+    def __del__(self):
+        try:
+            if self.handle and self.device.handle:
+                self.device.lib.cc_page_plan_release(self.handle)
+        except Exception:
+            pass
+
+
+class PagedCache:
+    """One layer's pages: k, v [pages, heads, page size, size] in F16, or in I8 with factors [pages, heads] and open blocks [2 * slots, heads, page size, size]"""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None, k_open=None, v_open=None):
+        self.k, self.v, self.k_scale, self.v_scale, self.k_open, self.v_open = k, v, k_scale, v_scale, k_open, v_open
+
+    @classmethod
+    def alloc(cls, device, n_pages, n_kv, page_size, dk, dv=None, dtype=capi.I8, n_slots=0):
+        dv = dk if dv is None else dv
+        t = [CudaTensor.alloc([n_pages, n_kv, page_size, d], dtype, device) for d in (dk, dv)]
+        if dtype == capi.I8:
+            t += [CudaTensor.alloc([n_pages, n_kv], capi.F32, device) for _ in range(2)]
+            t += [CudaTensor.alloc([2 * n_slots, n_kv, page_size, d], capi.F16, device) for d in (dk, dv)]
+        return cls(*t)
+
+    def _struct(self):
+        s = capi.cc_paged_cache()
+        for name in ("k", "v", "k_scale", "v_scale", "k_open", "v_open"):
+            t = getattr(self, name)
+            if t is not None:
+                setattr(s, name, t._view())
+        return s
+
+
+def _v(t):
+    return C.byref(t._view()) if t is not None else None
+
+
+def append(plan, cache, q_src, q_col0, k_src, k_col0, v_src, v_col0, n_heads=0, freq=None, pairing=capi.ROPE_NEIGHBOURS, offset=0, mag=1.0):
+    """keys and values of the plan's tokens, turned by their positions, into the pages -> the turned queries [T, n_heads * dk] (q_src None: None)"""
+    dev, h, s = plan.device, C.c_void_p(), cache._struct()
+    dev.check(dev.lib.cc_paged_append(dev.handle, plan.handle, C.byref(s), _v(q_src), int(q_col0), _v(k_src), int(k_col0), _v(v_src), int(v_col0), int(n_heads), _v(freq),
+                                      int(pairing), int(offset), float(mag), C.byref(h)))
+    return None if q_src is None else CudaTensor(_Buf(dev, h), TensorStrider([plan.tokens, n_heads * cache.k.shape()[3]]), dev)
+
+
+def attention(plan, cache, q, n_heads, scale, window=0, softcap=0.0, sink=None):
+    """-> [T, n_heads * dv]"""
+    dev, h, s = plan.device, C.c_void_p(), cache._struct()
+    dev.check(dev.lib.cc_paged_attention(dev.handle, plan.handle, C.byref(s), _v(q), int(n_heads), float(scale), int(window), float(softcap), _v(sink), C.byref(h)))
+    return CudaTensor(_Buf(dev, h), TensorStrider([plan.tokens, n_heads * cache.v.shape()[3]]), dev)

@@ -399,3 +399,10 @@ def joined_product_accumulate(dst, w, a, src=None, gate_col0=0, up_col0=0, ff=0,
     P = capi.cc_glu_params(int(act), float(alpha), float(limit), float(up_shift))
     dst.device.check(dst.device.lib.cc_joined_product_accumulate(dst.device.handle, _v(dst), _v(w), _v(a), _v(src), int(gate_col0), int(up_col0), int(ff), C.byref(P)))
     return dst
+
+
+def product_i8(w, w_scale, x):
+    """x [T, k] coded in 8 bits row by row, times the codes w [m, k] with a factor per channel -> [T, m]"""
+    h = C.c_void_p()
+    x.device.check(x.device.lib.cc_product_i8(x.device.handle, _v(w), _v(w_scale), _v(x), C.byref(h)))
+    return _new(x.device, h, [x.shape()[0], w.shape()[0]])

@@ -89,6 +89,10 @@ class CudaTensorDevice:
 
     def synchronize(self): self.check(self.lib.cc_device_synchronize(self.handle))
 
+    def stream(self) -> int:
+        """the cudaStream_t on which all work of this device runs"""
+        return int(self.lib.cc_device_stream(self.handle))
+
     # ---- sharded path: exchange window of this rank (comm.cu).  `exchange(bytes) -> [bytes of every rank]` is any
     # all-gather of small host blobs (torch.distributed.all_gather_object in bench.py / the tests) ----------------------------
     def init_comm(self, rank, world, exchange=None, transport="p2p"):
@@ -189,6 +193,17 @@ class CudaTensor:
         for i, (s, t) in enumerate(zip(self._strider.shape, self._strider.strides)):
             v.shape[i], v.strides[i] = s, t
         return v
+
+    @property
+    def __cuda_array_interface__(self):
+        """the tensor's own memory for other libraries (torch.as_tensor and the like), ordered by the device's stream"""
+        if self.dtype() not in capi.ARRAY_TYPES:
+            raise AttributeError(f"a tensor of type {self.dtype()} is not a plain array")
+        self.device.flush()
+        kind, size = capi.ARRAY_TYPES[self.dtype()]
+        empty = self._strider.len() == 0
+        return {"shape": tuple(self.shape()), "typestr": kind, "data": (0 if empty else int(self.device.lib.cc_tensor_data(self.buf.handle)), False),
+                "strides": tuple(s * size for s in self._strider.strides), "stream": self.device.stream(), "version": 3}
 
     def _new(self, handle, shape):
         return CudaTensor(_Buf(self.device, handle), TensorStrider(shape), self.device)

@@ -25,6 +25,10 @@ extern "C" {
  * CC_ACT_RELU_SQUARED: max(z, 0)^2. */
 enum cc_activation { CC_ACT_NONE = 0, CC_ACT_SILU = 1, CC_ACT_GELU_TANH = 2, CC_ACT_SWISH = 3, CC_ACT_SIGMOID = 4, CC_ACT_RELU_SQUARED = 5 };
 
+/* The device address of a plain tensor's first element (NULL: a quantised one), for kernels and libraries of the caller's own: it stays valid while the caller
+ * holds the tensor, and what is read or written there has to be ordered with the device's stream (cc_device_stream, cc_device_synchronize). */
+CC_API void* cc_tensor_data(cc_buf* buf);
+
 /* x (any shape) = 0 */
 CC_API int cc_tensor_zero(cc_device* dev, const cc_view* x);
 
@@ -325,6 +329,13 @@ CC_API int cc_layer_norm_product(cc_device* dev, const cc_view* x, const cc_view
  * unit of cc_glu_params.  ff = 0: dst += W a (src and glu may be NULL).  dst: [T, m]. */
 CC_API int cc_joined_product_accumulate(cc_device* dev, const cc_view* dst, const cc_view* w, const cc_view* a, const cc_view* src, int32_t gate_col0, int32_t up_col0,
                                         int32_t ff, const cc_glu_params* glu);
+
+/* ---- products in 8-bit integers -------------------------------------------------------------------------------------------------- */
+/* out = W x with 8-bit operands: w: I8 [m, k] codes (-127 .. 127, as rounding to a factor gives them; -128 counts as it stands), w_scale: F32 [m] one factor per
+ * output channel, x: F32 [T, k], coded on the way with one factor per token: with a the largest magnitude of the row, x_scale = a / 127 and the codes
+ * round(127 x / a), ties to even.  out[t, c] = (sum of the codes' products, exact) * x_scale[t] * w_scale[c], F32 [T, m].  k <= 131072.  A row that holds an
+ * infinity or a NaN has the result NaN. */
+CC_API int cc_product_i8(cc_device* dev, const cc_view* w, const cc_view* w_scale, const cc_view* x, cc_buf** out);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,116 @@
+"""The plan of a step over several sequences (crabml_b200/csrc/paged_plan.hpp) on the CPU: what is refused, and that the segments cover every new token once, keep what
+has to be kept and stand in an order in which no open row is overwritten before it is read.  CPU only."""
+import os
+import random
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+FULL, KEPT = 1, 2
+
+
+@pytest.fixture(scope="module")
+def build(tmp_path_factory):
+    exe = str(tmp_path_factory.mktemp("plan") / "plan")
+    subprocess.run(["g++", "-std=c++17", "-O1", os.path.join(ROOT, "tests", "host", "paged_plan_check.cpp"), "-o", exe], check=True, capture_output=True, timeout=300)
+
+    def run(page, n_pages, table, pos0, counts, n_slots=0, slots=None):
+        cols = max([len(r) for r in table], default=0)
+        text = [len(counts), page, cols, n_pages, n_slots, int(slots is not None), *pos0, *counts]
+        for r in table:
+            text += list(r) + [-1] * (cols - len(r))
+        text += slots or []
+        out = subprocess.run([exe], input=" ".join(map(str, text)), check=True, capture_output=True, text=True, timeout=60).stdout.strip().split("\n")
+        if out[0].startswith("wrong"):
+            return out[0], []
+        keys = ("seq", "block", "page", "token0", "row0", "rows", "half", "flags", "next", "pos0")
+        return [int(x) for x in out[0].split()[1:]], [dict(zip(keys, map(int, r.split()))) for r in out[1:]]
+    return run
+
+
+REFUSED = [
+    ("page size", dict(page=48, n_pages=4, table=[[0]], pos0=[0], counts=[1]), "pages of 48"),
+    ("negative count", dict(page=16, n_pages=4, table=[[0]], pos0=[0], counts=[-1]), "new ones"),
+    ("negative position", dict(page=16, n_pages=4, table=[[0]], pos0=[-1], counts=[1]), "new ones"),
+    ("position beyond 31 bits", dict(page=16, n_pages=4, table=[[0]], pos0=[1 << 31], counts=[1]), "new ones"),
+    ("a page too few", dict(page=16, n_pages=4, table=[[0]], pos0=[16], counts=[1]), "needs more than 1 pages"),
+    ("no such page", dict(page=16, n_pages=4, table=[[4]], pos0=[0], counts=[1]), "page 4 of sequence 0"),
+    ("no page given", dict(page=16, n_pages=4, table=[[0], [1, 2]], pos0=[16, 0], counts=[1, 1]), "page -1 of sequence 0"),
+    ("a read page out of range", dict(page=16, n_pages=4, table=[[9, 1]], pos0=[16], counts=[1]), "page 9 of sequence 0"),
+    ("one page for two sequences", dict(page=16, n_pages=4, table=[[0], [0]], pos0=[0, 3], counts=[1, 1]), "page 0 takes tokens"),
+    ("one page twice in a row", dict(page=16, n_pages=4, table=[[0, 0]], pos0=[0], counts=[20]), "page 0 takes tokens"),
+    ("an older page again", dict(page=16, n_pages=4, table=[[0, 0]], pos0=[16], counts=[2]), "page 0 takes new tokens"),
+    ("a page another one reads", dict(page=16, n_pages=4, table=[[0, 1], [1, 2]], pos0=[16, 16], counts=[1, 1]), "page 1 takes new tokens"),
+    ("a page that a resting one reads", dict(page=16, n_pages=4, table=[[0, 1], [1, 2]], pos0=[16, 17], counts=[1, 0]), "page 1 takes new tokens"),
+    ("no such slot", dict(page=16, n_pages=4, table=[[0]], pos0=[0], counts=[1], n_slots=1, slots=[1]), "slot 1 of sequence 0"),
+    ("one slot for two", dict(page=16, n_pages=4, table=[[0], [1]], pos0=[0, 0], counts=[1, 1], n_slots=3, slots=[2, 2]), "two sequences with slot 2"),
+    ("more sequences than slots", dict(page=16, n_pages=4, table=[[0], [1]], pos0=[0, 0], counts=[1, 1], n_slots=1), "slot 1 of sequence 1"),
+    ("too many tokens", dict(page=128, n_pages=1 << 18, table=[list(range(1 << 17))], pos0=[0], counts=[1 << 24]), "16 million"),
+]
+
+
+@pytest.mark.parametrize("what,plan,text", REFUSED, ids=[r[0] for r in REFUSED])
+def test_refused(build, what, plan, text):
+    head, _ = build(**plan)
+    assert isinstance(head, str) and text in head
+
+
+def test_allowed(build):
+    # a shared prefix that nothing is appended to, a sequence at rest, pages that are not needed, no sequence at all
+    assert build(16, 9, [[3, 4], [3, 5]], [16, 20], [1, 2])[0] == [2, 3, 2]
+    assert build(16, 9, [[3], [4]], [5, 6], [0, 1])[0] == [1, 1, 1]
+    assert build(16, 9, [[3, -1, 99]], [0], [16])[0] == [1, 16, 1]
+    assert build(16, 0, [], [], [])[0] == [0, 0, 0]
+    assert build(16, 0, [[]], [0], [0], n_slots=1)[0] == [0, 0, 0]
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_segments(build, seed):
+    r = random.Random(seed)
+    P, n = r.choice([16, 32, 64, 128]), r.randint(1, 9)
+    pos0 = [r.choice([0, r.randint(0, 5 * P), P * r.randint(0, 4), P * r.randint(1, 4) - 1]) for _ in range(n)]
+    counts = [r.choice([0, 1, 1, r.randint(1, 6 * P), P, 2 * P]) for _ in range(n)]
+    need = [(p + c + P - 1) // P for p, c in zip(pos0, counts)]
+    pages = r.sample(range(sum(need) + 5), sum(need))
+    table, at = [], 0
+    for k in need:
+        table.append(pages[at:at + k])
+        at += k
+    slots = r.sample(range(n + 3), n)
+    (items, tokens, n_segments), segs = build(P, sum(need) + 5, table, pos0, counts, n + 3, slots)
+    assert tokens == sum(counts) and n_segments == len(segs)
+    first, seen = [sum(counts[:i]) for i in range(n)], [0] * tokens
+    for g in segs:
+        i = g["seq"]
+        assert g["page"] == table[i][g["block"]] and g["half"] == 2 * slots[i] + g["block"] % 2
+        assert 0 <= g["row0"] and g["rows"] > 0 and g["row0"] + g["rows"] <= P
+        assert g["pos0"] == g["block"] * P + g["row0"] == pos0[i] + g["token0"] - first[i]
+        end = pos0[i] + counts[i]
+        assert bool(g["flags"] & FULL) == ((g["block"] + 1) * P <= end)
+        assert bool(g["flags"] & KEPT) == (g["block"] >= end // P - 1)
+        for t in range(g["token0"], g["token0"] + g["rows"]):
+            seen[t] += 1
+    assert seen == [1] * tokens
+    # chains: every segment is reached once, and one that writes open rows that another one of its sequence reads stands behind it in the same chain
+    reached = []
+    for head in range(items):
+        chain, at = [], head
+        while at >= 0:
+            chain.append(segs[at])
+            at = segs[at]["next"]
+        reached += [id(g) for g in chain]
+        for later, g in enumerate(chain):
+            assert g["seq"] == chain[0]["seq"] and (later == 0 or g["block"] > chain[later - 1]["block"])
+    assert sorted(reached) == sorted(id(g) for g in segs)
+    where = {}
+    for head in range(items):
+        at, place = head, 0
+        while at >= 0:
+            where[at] = (head, place)
+            at, place = segs[at]["next"], place + 1
+    for a, g in enumerate(segs):
+        for b, h in enumerate(segs):
+            reads = h["row0"] > 0 and h["flags"] & FULL
+            if a != b and g["flags"] & KEPT and reads and g["half"] == h["half"]:
+                assert where[a][0] == where[b][0] and where[a][1] > where[b][1]
