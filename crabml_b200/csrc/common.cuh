@@ -249,6 +249,7 @@ int cc_prefill_rows_plain(cc_device* dev, const float* x, int64_t rows, int64_t 
 int cc_launch_prefill_operand(cc_device* dev, const cc_buf* w, float* out, int64_t m, int64_t k, int64_t b, const float* res);
 // tensor map (CUtensorMap) of a bfloat16 matrix [rows][k], box 64 columns x box_rows rows, 128-byte swizzle
 int cc_make_tmap_bf16(cc_device* dev, void* tm, const void* base, int64_t rows, int64_t k, int box_rows);
+int cc_make_tmap_i8(cc_device* dev, void* tm, const void* base, int64_t rows, int64_t k, int box_rows);      // .. of 8-bit numbers, 128 columns; k a multiple of 16
 
 // ---- dense.cu: plain F32 / BF16 weight matrices with a batch of activation rows -------------------
 bool cc_dense_supported(int wtype, int64_t b);

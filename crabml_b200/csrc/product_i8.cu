@@ -1,9 +1,12 @@
 // product_i8.cu -- products in 8-bit integers (cc_product_i8 of include/crabml_seqops.h): activations coded row by row, exact integer sums, one factor per token
 // and one per output channel.
+#include <cooperative_groups.h>
+#include <cuda.h>
 #include <math.h>
 
 #include "../../include/crabml_seqops.h"
 #include "capi_checks.cuh"
+#include "split_gemm.cuh"
 
 // ---- activations -> codes ------------------------------------------------------------------------------------------------------------------
 // round(127 x / a), ties to even, as the exact quotient rounds.  127 / a and the product err by less than 1e-4 of a step; where that leaves it open (one number
@@ -70,6 +73,261 @@ __global__ void __launch_bounds__(I8_THREADS) i8_few_kernel(const int8_t* __rest
         for (int i = 0; i < n; i++) out[(int64_t)(t0 + i) * m + row] = (float)acc[i] * ws[row] * xs[t0 + i];
 }
 
+
+// ---- many rows: tcgen05.mma on 8-bit tiles -----------------------------------------------------------------------------------------------------
+// A tile is 128 output channels (the instruction's rows, TMEM's lanes) x BN tokens; a step of 128 codes of both comes by TMA into a ring, one thread issues
+// four instructions of 32 codes for it (kind::i8, 32-bit integer accumulators in TMEM), four warps finish.  Lanes are neighbouring channels: an output row is stored
+// 128 bytes at a time.  A CTA walks over tiles with two accumulators, so that a tile's end overlaps the next one's steps.  Few tiles: a cluster shares the
+// depth of one, each CTA sends the others the integer sums of the lanes that they finish, and any order gives the same sum.
+// Every wait is bounded (sg_wait): on expiry the CTA raises `fail`, all roles leave their loops, TMEM is freed and the host reports it.
+#define GI_THREADS 256
+#define GI_K 128
+struct GiShared {
+    unsigned long long full[8], empty[8], acc_full[2], acc_empty[2], drained;
+    unsigned tmem_base;
+    int fail;
+};
+__host__ __device__ constexpr int gi_stages(int bn) { return 192 * 1024 / ((128 + bn) * GI_K) < 8 ? 192 * 1024 / ((128 + bn) * GI_K) : 8; }
+__host__ __device__ constexpr size_t gi_smem(int bn) { return (size_t)gi_stages(bn) * (128 + bn) * GI_K + 1024; }
+__device__ __forceinline__ void gi_umma(unsigned tmem_d, uint64_t a, uint64_t b, unsigned idesc, unsigned accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// 32-bit integer accumulator, signed 8-bit A and B, both K-major
+__host__ __device__ constexpr unsigned gi_desc(int n) { return (2u << 4) | (1u << 7) | (1u << 10) | ((unsigned)(n >> 3) << 17) | (8u << 24); }
+
+template <int N>
+__device__ __forceinline__ void gi_load(unsigned addr, unsigned (&v)[N]) {
+    static_assert(N == 16 || N == 32, "");
+    sg_tmem16(addr, *(unsigned(*)[16])v);
+    if (N == 32) sg_tmem16(addr + 16, *(unsigned(*)[16])(v + N - 16));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; i++) asm volatile("" : "+r"(v[i]));       // nothing is done with them before
+}
+
+template <int BN>
+__global__ void __launch_bounds__(GI_THREADS, 1) i8_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const float* __restrict__ ws,
+                                                                const float* __restrict__ xs, float* __restrict__ out, int T, int m, int steps_all, int n_tiles, int parts, unsigned* err_dev,
+                                                                unsigned* err_host) {
+    namespace cg = cooperative_groups;
+    constexpr int ST = gi_stages(BN), RUN = BN < 32 ? BN : 32;
+    constexpr unsigned A_BYTES = 128 * GI_K, B_BYTES = BN * GI_K, COLS = 2 * BN < 32 ? 32 : 2 * BN;
+    extern __shared__ __align__(1024) uint8_t gi_raw[];
+    __shared__ GiShared sh;
+    uint8_t* ring = (uint8_t*)(((uintptr_t)gi_raw + 1023) & ~(uintptr_t)1023);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int part = parts > 1 ? (int)cg::this_cluster().block_rank() : 0;
+    const int s0 = (int)((int64_t)steps_all * part / parts), steps = (int)((int64_t)steps_all * (part + 1) / parts) - s0;
+    const int tiles_n = (T + BN - 1) / BN, first = blockIdx.x / parts, stride = gridDim.x / parts;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < ST; i++) { pg_mbar_init(pg_smem(&sh.full[i]), 1); pg_mbar_init(pg_smem(&sh.empty[i]), 1); }
+        for (int i = 0; i < 2; i++) { pg_mbar_init(pg_smem(&sh.acc_full[i]), 1); pg_mbar_init(pg_smem(&sh.acc_empty[i]), 4); }
+        pg_mbar_init(pg_smem(&sh.drained), 1);
+        sh.fail = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pg_smem(&sh.tmem_base)), "n"(COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pg_fence_before();
+    __syncthreads();
+    pg_fence_after();
+    const unsigned tmem = sh.tmem_base;
+    pdl_enter();
+    if (warp == 0) {
+        if (lane == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
+            unsigned g = 0;
+            bool ok = true;
+            for (int tile = first; tile < n_tiles && ok; tile += stride) {
+                const int mt = tile / tiles_n, nt = tile - mt * tiles_n;
+                for (int s = 0; s < steps; s++, g++) {
+                    const unsigned slot = g % ST, full = pg_smem(&sh.full[slot]), at = pg_smem(ring + (size_t)slot * (A_BYTES + B_BYTES));
+                    if (!(ok = sg_wait(pg_smem(&sh.empty[slot]), ((g / ST) & 1u) ^ 1u, &sh.fail))) break;
+                    pg_mbar_expect_tx(full, A_BYTES + B_BYTES);
+                    pg_tma_load_2d(at, &map_w, full, (s0 + s) * GI_K, mt * 128);
+                    pg_tma_load_2d(at + A_BYTES, &map_x, full, (s0 + s) * GI_K, nt * BN);
+                }
+            }
+            int never = 0;                                            // no copy is under way when the CTA ends
+            for (unsigned i = g > ST ? g - ST : 0; i < g; i++) sg_wait(pg_smem(&sh.full[i % ST]), (i / ST) & 1u, &never);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            unsigned g = 0, nth = 0;
+            bool ok = true;
+            for (int tile = first; tile < n_tiles && ok; tile += stride, nth++) {
+                const unsigned acc = tmem + (nth & 1u) * BN;
+                if (!(ok = sg_wait(pg_smem(&sh.acc_empty[nth & 1u]), ((nth >> 1) & 1u) ^ 1u, &sh.fail))) break;
+                pg_fence_after();
+                for (int s = 0; s < steps; s++, g++) {
+                    const unsigned slot = g % ST, at = pg_smem(ring + (size_t)slot * (A_BYTES + B_BYTES));
+                    if (!(ok = sg_wait(pg_smem(&sh.full[slot]), (g / ST) & 1u, &sh.fail))) break;
+                    pg_fence_after();
+                    const uint64_t a = pg_smem_desc(at), b = pg_smem_desc(at + A_BYTES);
+#pragma unroll
+                    for (int kk = 0; kk < GI_K / 32; kk++) gi_umma(acc, a + 2 * kk, b + 2 * kk, gi_desc(BN), s > 0 || kk > 0);
+                    pg_umma_commit(pg_smem(&sh.empty[slot]));
+                }
+                if (ok) pg_umma_commit(pg_smem(&sh.acc_full[nth & 1u]));
+            }
+            int never = 0;                                            // nothing of this CTA is in flight when its TMEM is given back
+            pg_umma_commit(pg_smem(&sh.drained));
+            sg_wait(pg_smem(&sh.drained), 0, &never);
+        }
+        __syncwarp();
+    } else if (warp >= 4 && parts == 1) {
+        const int q = warp & 3;
+        unsigned nth = 0;
+        for (int tile = first; tile < n_tiles; tile += stride, nth++) {
+            const int mt = tile / tiles_n, n0 = (tile - mt * tiles_n) * BN, row = mt * 128 + q * 32 + lane;
+            if (!sg_wait_warp(pg_smem(&sh.acc_full[nth & 1u]), (nth >> 1) & 1u, &sh.fail)) break;
+            pg_fence_after();
+            const unsigned from = tmem + (nth & 1u) * BN + ((unsigned)(q * 32) << 16);
+            const float factor = row < m ? ws[row] : 0.0f;
+#pragma unroll 1
+            for (int c0 = 0; c0 < BN && n0 + c0 < T; c0 += RUN) {
+                unsigned v[RUN];
+                gi_load<RUN>(from + c0, v);
+                const float mine = lane < RUN && n0 + c0 + lane < T ? xs[n0 + c0 + lane] : 0.0f;
+                if (c0 + RUN >= BN || n0 + c0 + RUN >= T) {           // the last of the accumulator: it may be filled again
+                    pg_fence_before();
+                    sg_arrive(pg_smem(&sh.acc_empty[nth & 1u]));
+                }
+                float* o = out + (int64_t)(n0 + c0) * m + row;
+#pragma unroll
+                for (int j = 0; j < RUN; j++) {
+                    const float f = __shfl_sync(0xffffffffu, mine, j);
+                    if (row < m && n0 + c0 + j < T) *o = (float)(int)v[j] * factor * f;
+                    o += m;
+                }
+            }
+        }
+    }
+    if (parts > 1) {                                                  // one tile: CTA p finishes the lanes of its 4 / parts warps
+        cg::cluster_group cluster = cg::this_cluster();
+        const int q = warp & 3, owners = 4 / parts, owner = q / owners, mt = first / tiles_n, n0 = (first - mt * tiles_n) * BN, row = mt * 128 + q * 32 + lane;
+        if (warp >= 4) sg_wait_warp(pg_smem(&sh.acc_full[0]), 0, &sh.fail);
+        pg_fence_after();
+        __syncthreads();
+        const int bad = *(volatile int*)&sh.fail;
+        cluster.sync();                                               // every CTA's products are done: the rings are free
+        const unsigned from = tmem + ((unsigned)(q * 32) << 16);
+        // [sender][warp of the owner][column][lane]
+        auto box = [&](int from_part, int at_part) { return ((size_t)(from_part < at_part ? from_part : from_part - 1) * owners + q % owners) * BN * 32; };
+        if (warp >= 4 && owner != part) {
+            int* to = cluster.map_shared_rank((int*)ring, owner) + box(part, owner);
+#pragma unroll 1
+            for (int c0 = 0; c0 < BN && n0 + c0 < T; c0 += RUN) {
+                unsigned v[RUN];
+                gi_load<RUN>(from + c0, v);
+#pragma unroll
+                for (int j = 0; j < RUN; j++) to[(c0 + j) * 32 + lane] = (int)v[j];
+            }
+        }
+        cluster.sync();
+        if (warp >= 4 && owner == part && !bad) {
+            const float factor = row < m ? ws[row] : 0.0f;
+#pragma unroll 1
+            for (int c0 = 0; c0 < BN && n0 + c0 < T; c0 += RUN) {
+                unsigned v[RUN];
+                gi_load<RUN>(from + c0, v);
+                const float mine = lane < RUN && n0 + c0 + lane < T ? xs[n0 + c0 + lane] : 0.0f;
+                for (int p = 0; p < parts; p++) {
+                    if (p == part) continue;
+                    const int* o = (const int*)ring + box(p, part) + c0 * 32 + lane;
+#pragma unroll
+                    for (int j = 0; j < RUN; j++) v[j] += (unsigned)o[j * 32];
+                }
+                float* o = out + (int64_t)(n0 + c0) * m + row;
+#pragma unroll
+                for (int j = 0; j < RUN; j++) {
+                    const float f = __shfl_sync(0xffffffffu, mine, j);
+                    if (row < m && n0 + c0 + j < T) *o = (float)(int)v[j] * factor * f;
+                    o += m;
+                }
+            }
+        }
+    }
+    pg_fence_before();
+    __syncthreads();
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(COLS) : "memory");
+    if (threadIdx.x == 0 && sh.fail) {
+        if (err_dev) atomicExch(err_dev, 5u);
+        if (err_host) { *(volatile unsigned*)err_host = 5u; __threadfence_system(); }
+    }
+}
+template <int BN>
+static int gi_launch(cc_device* dev, const int8_t* w, const float* ws, const int8_t* x, const float* xs, float* out, int T, int m, int kp) {
+    CUtensorMap mw, mx;
+    int rc = cc_make_tmap_i8(dev, &mw, w, m, kp, 128);
+    if (!rc) rc = cc_make_tmap_i8(dev, &mx, x, T, kp, BN);
+    if (rc) return rc;
+    const int64_t tiles = (int64_t)((m + 127) / 128) * ((T + BN - 1) / BN);
+    const int steps = (kp + GI_K - 1) / GI_K;
+    int parts = 1;
+    while (parts < 4 && tiles * parts * 2 <= dev->sm_count && steps / (parts * 2) >= 2) parts *= 2;
+    CC_REQUIRE(dev, tiles < ((int64_t)1 << 30), "product_i8: %lld tiles", (long long)tiles);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(parts > 1 ? tiles * parts : tiles < dev->sm_count ? tiles : dev->sm_count));
+    cfg.blockDim = dim3(GI_THREADS); cfg.dynamicSmemBytes = gi_smem(BN); cfg.stream = dev->stream;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = dev->pdl ? 1 : 0;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)parts; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = 2;
+    CC_CUDA(dev, cudaFuncSetAttribute(i8_tile_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)gi_smem(BN)));
+    CC_CUDA(dev, cudaLaunchKernelEx(&cfg, i8_tile_kernel<BN>, mw, mx, ws, xs, out, T, m, steps, (int)tiles, parts, dev->err_dev, dev->err_host));
+    CC_LAUNCH_CHECK(dev);
+    return CC_OK;
+}
+// rows of k codes -> rows of kp, zeros behind: what TMA can read where k is no multiple of 16
+__global__ void i8_pad_kernel(const int8_t* __restrict__ w, int8_t* __restrict__ to, int64_t n4, int k, int kp4) {
+    pdl_enter();
+    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= n4) return;
+    const int64_t row = i / kp4;
+    const int c = (int)(i - row * kp4) * 4;
+    unsigned u = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (c + j < k) u |= (unsigned)(uint8_t)w[row * k + c + j] << (8 * j);
+    ((unsigned*)to)[i] = u;
+}
+
+static int i8_product(cc_device* dev, const int8_t* w, const float* ws, const float* x, int64_t rs, float* out, int T, int m, int k) {
+    const int kp = (k + 15) / 16 * 16;
+    const bool tiles = T > 8, pad = tiles && k != kp;
+    const size_t codes = ((size_t)T * kp + 255) / 256 * 256, factors = ((size_t)T * 4 + 255) / 256 * 256;
+    void* ws_mem = nullptr; size_t cls = 0;
+    int rc = cc_pool_alloc(dev, codes + factors + (pad ? (size_t)m * kp : 0), &ws_mem, &cls);
+    if (rc) return rc;
+    int8_t* xq = (int8_t*)ws_mem;
+    float* xs = (float*)((uint8_t*)ws_mem + codes);
+    cudaError_t e = cc_launch_pdl(dev, i8_rows_kernel, (unsigned)T, I8_THREADS, 0, x, rs, k, kp, xq, xs);
+    dev->launches++;
+    if (pad && e == cudaSuccess) {
+        int8_t* wp = (int8_t*)ws_mem + codes + factors;
+        const int64_t n4 = (int64_t)m * (kp / 4);
+        e = cc_launch_pdl(dev, i8_pad_kernel, (unsigned)((n4 + 255) / 256), 256, 0, w, wp, n4, k, kp / 4);
+        dev->launches++;
+        w = wp;
+    }
+    if (e == cudaSuccess && !tiles) {
+        e = cc_launch_pdl(dev, i8_few_kernel, dim3((unsigned)((m + I8_THREADS / 32 - 1) / (I8_THREADS / 32)), (unsigned)((T + I8_ROWS - 1) / I8_ROWS)), I8_THREADS, 0, w, ws, xq, xs, out, T, m, k, kp);
+        dev->launches++;
+    }
+    if (e != cudaSuccess) rc = cc_fail(dev, CC_ERR_CUDA, "product_i8: %s", cudaGetErrorString(e));
+    else if (tiles) rc = T <= 16 ? gi_launch<16>(dev, w, ws, xq, xs, out, T, m, kp) : T <= 32 ? gi_launch<32>(dev, w, ws, xq, xs, out, T, m, kp)
+                       : T <= 64 ? gi_launch<64>(dev, w, ws, xq, xs, out, T, m, kp) : T <= 128 ? gi_launch<128>(dev, w, ws, xq, xs, out, T, m, kp) : gi_launch<256>(dev, w, ws, xq, xs, out, T, m, kp);
+    cc_pool_free(dev, ws_mem, cls);
+    return rc;
+}
+
 extern "C" CC_API int cc_product_i8(cc_device* dev, const cc_view* w, const cc_view* w_scale, const cc_view* x, cc_buf** out) {
     if (!dev) return CC_ERR_ARG;
     CC_ENTER(dev);
@@ -88,24 +346,9 @@ extern "C" CC_API int cc_product_i8(cc_device* dev, const cc_view* w, const cc_v
     cc_buf* o = nullptr;
     int rc = cc_new_activation(dev, T * m, CC_F32, false, &o);
     if (rc) return rc;
-    if (T > 0 && m > 0) {
-        const int kp = (int)((k + 15) / 16 * 16);
-        void* ws = nullptr; size_t cls = 0;
-        const size_t codes = ((size_t)T * kp + 255) / 256 * 256;
-        rc = cc_pool_alloc(dev, codes + (size_t)T * 4, &ws, &cls);
-        if (rc) { cc_tensor_release(o); return rc; }
-        int8_t* xq = (int8_t*)ws;
-        float* xs = (float*)((uint8_t*)ws + codes);
-        cudaError_t e = cc_launch_pdl(dev, i8_rows_kernel, (unsigned)T, I8_THREADS, 0, (const float*)x->buf->plane[0], x->strides[0], (int)k, kp, xq, xs);
-        dev->launches++;
-        if (e == cudaSuccess) {
-            e = cc_launch_pdl(dev, i8_few_kernel, dim3((unsigned)((m + I8_THREADS / 32 - 1) / (I8_THREADS / 32)), (unsigned)((T + I8_ROWS - 1) / I8_ROWS)), I8_THREADS, 0,
-                              (const int8_t*)w->buf->plane[0], (const float*)w_scale->buf->plane[0], xq, xs, (float*)o->base, (int)T, (int)m, (int)k, kp);
-            dev->launches++;
-        }
-        cc_pool_free(dev, ws, cls);
-        if (e != cudaSuccess) { cc_tensor_release(o); return cc_fail(dev, CC_ERR_CUDA, "product_i8: %s", cudaGetErrorString(e)); }
-    }
+    if (T > 0 && m > 0) rc = i8_product(dev, (const int8_t*)w->buf->plane[0], (const float*)w_scale->buf->plane[0], (const float*)x->buf->plane[0], x->strides[0], (float*)o->base, (int)T,
+                                        (int)m, (int)k);
+    if (rc) { cc_tensor_release(o); return rc; }
     *out = o;
     return CC_OK;
 }
