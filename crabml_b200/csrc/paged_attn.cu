@@ -17,6 +17,7 @@
 #define PT_THREADS (PT_WARPS * 32)
 #define PT_SHIFT 12.0f                        // weights are exp2(score - largest + PT_SHIFT)
 #define PT_MOST_SPLIT 2048                    // keys of a slice
+#define PT_FEW 32
 #define PT_LOG2E 1.4426950408889634f
 
 struct PtArgs {
@@ -25,10 +26,11 @@ struct PtArgs {
     const uint8_t *k, *v;
     const float *ks, *vs, *q, *sink;
     const __half *ko, *vo;
-    float *out, *part;                        // part: [item][head][8][dvp] sums of a slice, behind them ml
-    float2* ml;                               // [item][head][8]: largest score (base 2) and sum of weights
+    float *out, *part;                        // part: [item][head][tile_rows][dv] sums of a slice, behind them ml
+    float2* ml;                               // [item][head][tile_rows]: largest score (base 2) and sum of weights
     float scale, softcap;
     int n_seqs, table_cols, page, shift, H, G, R, dk, dv, window, split, rows_lo, rows_hi;
+    int tile_rows;                            // of an item: 8 (paged_few_kernel) or 128 (paged_tile_kernel)
 };
 struct PtItem { int seq, split, tile, n_split; };
 
@@ -460,11 +462,13 @@ __global__ void __launch_bounds__(128) paged_sum_kernel(const PtArgs a) {
     int row, items = 0;
     const int seq = pt_find(a, blockIdx.x, [&](const PgSeq& s) { return pt_splits(s, a) > 1 ? s.count * a.R : 0; }, &row);
     if (seq < 0) return;
-    for (int x = lane; x < seq; x += 32) items += pt_splits(a.seqs[x], a) * ((a.seqs[x].count * a.R + 7) >> 3);
+    for (int x = lane; x < seq; x += 32) items += pt_splits(a.seqs[x], a) * ((a.seqs[x].count * a.R + a.tile_rows - 1) / a.tile_rows);
     items = warp_sum_i(items);
     const PgSeq s = a.seqs[seq];
-    const int tiles = (s.count * a.R + 7) >> 3, n = pt_splits(s, a), tile = row >> 3, y = row & 7;
-    auto at = [&](int x) { return ((size_t)(items + x * tiles + tile) * a.G + kvh) * 8 + y; };
+    const int tiles = (s.count * a.R + a.tile_rows - 1) / a.tile_rows, n = pt_splits(s, a), tile = row / a.tile_rows, y = row - tile * a.tile_rows;
+    // items of a sequence: slice by slice where a tile is 8 rows, tile by tile from the last one on where it is 128
+    const int first = a.tile_rows == 8 ? tile : (tiles - 1 - tile) * n, by = a.tile_rows == 8 ? tiles : 1;
+    auto at = [&](int x) { return ((size_t)(items + first + x * by) * a.G + kvh) * a.tile_rows + y; };
     float m = -INFINITY;
     for (int x = lane; x < n; x += 32) m = fmaxf(m, a.ml[at(x)].x);
     m = warp_max(m);
@@ -508,37 +512,46 @@ static cudaError_t pt_launch_few(cc_device* dev, const PtArgs& a, unsigned items
     dev->launches++;
     return e;
 }
-static int pt_few(cc_device* dev, const cc_page_plan* plan, PtArgs a, bool i8) {
+#include "paged_tile.cuh"
+
+// the sequences of rows_lo .. rows_hi rows, in tiles of tile_rows: slices of `most` keys at most, as many as leave no SM without one
+static int pt_run(cc_device* dev, const cc_page_plan* plan, PtArgs a, bool i8) {
+    const bool few = a.tile_rows == 8;
     int64_t keys = 0, items = 0, split_rows = 0;
     for (const PgSeq& s : plan->seqs) {
         const int64_t rows = (int64_t)s.count * a.R;
         if (rows < a.rows_lo || rows > a.rows_hi) continue;
         int from, to;
         pt_range(s, a.window, &from, &to);
-        keys += (int64_t)(to - from) * ((rows + 7) / 8) * a.G;
+        keys += (int64_t)(to - from) * ((rows + a.tile_rows - 1) / a.tile_rows) * a.G;
     }
     if (!keys) return CC_OK;
-    const int64_t slots = (int64_t)dev->sm_count * 3;
-    int64_t each = (keys + slots - 1) / slots;
-    each = std::min<int64_t>(PT_MOST_SPLIT - 16, std::max<int64_t>(128, (each + 63) / 64 * 64));
-    if (each > 512) each = 512;
-    a.split = (int)each;
+    const int64_t slots = (int64_t)dev->sm_count * (few ? 3 : 1), each = (keys + slots - 1) / slots;
+    a.split = (int)(few ? std::min<int64_t>(512, std::max<int64_t>(128, (each + 63) / 64 * 64)) : std::min<int64_t>(TI_MOST, std::max<int64_t>(512, (each + 127) / 128 * 128)));
     for (const PgSeq& s : plan->seqs) {
         const int n = pt_splits(s, a);
-        items += (int64_t)n * (((int64_t)s.count * a.R + 7) / 8);
+        items += (int64_t)n * (((int64_t)s.count * a.R + a.tile_rows - 1) / a.tile_rows);
         if (n > 1) split_rows += (int64_t)s.count * a.R;
     }
-    CC_REQUIRE(dev, items < ((int64_t)1 << 31) && a.G <= 65535, "paged_attention: too many rows");
+    CC_REQUIRE(dev, items < ((int64_t)1 << 31) && split_rows < ((int64_t)1 << 31), "paged_attention: too many rows");
     void* ws = nullptr; size_t cls = 0;
     if (split_rows) {
-        const size_t part = (size_t)items * a.G * 8 * a.dv * sizeof(float), ml = (size_t)items * a.G * 8 * sizeof(float2);
+        const size_t part = (size_t)items * a.G * a.tile_rows * a.dv * sizeof(float), ml = (size_t)items * a.G * a.tile_rows * sizeof(float2);
         const int rc = cc_pool_alloc(dev, part + ml, &ws, &cls);
         if (rc) return rc;
         a.part = (float*)ws; a.ml = (float2*)((uint8_t*)ws + part);
     }
     const int d = std::max(a.dk, a.dv);
-    cudaError_t e = i8 ? (d <= 64 ? pt_launch_few<64, true>(dev, a, (unsigned)items) : d <= 128 ? pt_launch_few<128, true>(dev, a, (unsigned)items) : pt_launch_few<256, true>(dev, a, (unsigned)items))
-                       : (d <= 64 ? pt_launch_few<64, false>(dev, a, (unsigned)items) : d <= 128 ? pt_launch_few<128, false>(dev, a, (unsigned)items) : pt_launch_few<256, false>(dev, a, (unsigned)items));
+    cudaError_t e;
+    if (few) {
+        e = i8 ? (d <= 64 ? pt_launch_few<64, true>(dev, a, (unsigned)items) : d <= 128 ? pt_launch_few<128, true>(dev, a, (unsigned)items) : pt_launch_few<256, true>(dev, a, (unsigned)items))
+               : (d <= 64 ? pt_launch_few<64, false>(dev, a, (unsigned)items) : d <= 128 ? pt_launch_few<128, false>(dev, a, (unsigned)items) : pt_launch_few<256, false>(dev, a, (unsigned)items));
+    } else {
+        auto kernel = i8 ? paged_tile_kernel<true> : paged_tile_kernel<false>;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TI_SMEM);
+        if (e == cudaSuccess) e = cc_launch_pdl(dev, kernel, dim3((unsigned)items, (unsigned)a.G), TI_THREADS, TI_SMEM, a, dev->err_dev, dev->err_host);
+        dev->launches++;
+    }
     if (e == cudaSuccess && split_rows) {
         e = cc_launch_pdl(dev, paged_sum_kernel, dim3((unsigned)split_rows, (unsigned)a.G), 128, 0, a);
         dev->launches++;
@@ -566,6 +579,7 @@ extern "C" CC_API int cc_paged_attention(cc_device* dev, const cc_page_plan* pla
         CC_REQUIRE(dev, view_in_bounds(sink) && view_contiguous(sink) && view_len(sink) == H && sink->buf->dtype == CC_F32 && sink->buf->dev == dev,
                    "paged_attention: sink is not contiguous F32 [%d] of this device", H);
     }
+    CC_REQUIRE(dev, T * H < ((int64_t)1 << 31), "paged_attention: %lld tokens of %d heads", (long long)T, H);
     cc_buf* o = nullptr;
     rc = cc_new_activation(dev, T * H * c.dv, CC_F32, false, &o);
     if (rc) return rc;
@@ -576,8 +590,13 @@ extern "C" CC_API int cc_paged_attention(cc_device* dev, const cc_page_plan* pla
         a.scale = scale; a.softcap = softcap; a.window = window > 0 ? window : 0;
         a.n_seqs = plan->n_seqs; a.table_cols = plan->table_cols; a.page = plan->page; a.shift = plan->shift;
         a.H = H; a.G = c.G; a.R = H / c.G; a.dk = c.dk; a.dv = c.dv;
-        a.rows_lo = 1; a.rows_hi = 0x7fffffff;
-        rc = pt_few(dev, plan, a, c.i8);
+        // rows of a sequence and key head: up to PT_FEW in tiles of 8, more in tiles of 128 where a head's numbers have room there
+        a.rows_lo = 1; a.rows_hi = c.dk <= TI_D && c.dv <= TI_D ? PT_FEW : 0x7fffffff; a.tile_rows = 8;
+        rc = pt_run(dev, plan, a, c.i8);
+        if (!rc && a.rows_hi == PT_FEW) {
+            a.rows_lo = PT_FEW + 1; a.rows_hi = 0x7fffffff; a.tile_rows = TI_ROWS;
+            rc = pt_run(dev, plan, a, c.i8);
+        }
     }
     if (rc) { cc_tensor_release(o); return rc; }
     *out = o;

@@ -4,75 +4,172 @@
 #include <cuda.h>
 #include <math.h>
 
+#include <algorithm>
+
 #include "../../include/crabml_seqops.h"
 #include "capi_checks.cuh"
 #include "split_gemm.cuh"
 
 // ---- activations -> codes ------------------------------------------------------------------------------------------------------------------
-// round(127 x / a), ties to even, as the exact quotient rounds.  127 / a and the product err by less than 1e-4 of a step; where that leaves it open (one number
-// in 500 is so near to a border) and for rows whose 127 / a is no ordinary number the quotient is taken in 64 bits: two 24-bit numbers' quotient that is not a tie is
-// 2^-25 of itself away from one at least.
+// round(127 x / a), ties to even, as the exact quotient rounds.  127 / a and the product err by less than 2e-5 of a step; where that leaves it open, and for rows whose
+// 127 / a is no ordinary number, the quotient is taken in 64 bits: two 24-bit numbers' quotient that is not a tie is 2^-25 of itself away from one at least.
 __device__ __forceinline__ int i8_code(float x, float a, float r) {
     const float y = x * r, n = rintf(y);
-    if (fabsf(y - n) < 0.499f && a > 1e-30f) return (int)n;
+    if (fabsf(y - n) < 0.49998f && a > 1e-30f) return (int)n;
     return (int)rint((double)x * 127.0 / (double)a);
 }
+__device__ __forceinline__ unsigned i8_code4(const float4& v, float a, float r) {
+    return ((unsigned)i8_code(v.x, a, r) & 255u) | ((unsigned)i8_code(v.y, a, r) & 255u) << 8 | ((unsigned)i8_code(v.z, a, r) & 255u) << 16 | (unsigned)i8_code(v.w, a, r) << 24;
+}
+__device__ __forceinline__ unsigned i8_top4(const float4& v) {
+    const unsigned x = __float_as_uint(v.x) & 0x7fffffffu, y = __float_as_uint(v.y) & 0x7fffffffu, z = __float_as_uint(v.z) & 0x7fffffffu, w = __float_as_uint(v.w) & 0x7fffffffu;
+    return max(max(x, y), max(z, w));
+}
+// four numbers of a row of k from c on, zeros behind it
+__device__ __forceinline__ float4 i8_load4(const float* row, int c, int k, bool vec) {
+    if (vec && c + 4 <= k) return *(const float4*)(row + c);
+    return make_float4(c < k ? row[c] : 0.0f, c + 1 < k ? row[c + 1] : 0.0f, c + 2 < k ? row[c + 2] : 0.0f, c + 3 < k ? row[c + 3] : 0.0f);
+}
 #define I8_THREADS 256
+#define I8_KEEP 4                            // float4 of a row that a thread keeps: rows of up to 16 THREADS are read once.  16 of them, 256 threads for all rows, left two CTAs
+                                             // an SM: 2048 rows of 4096 took 24 us instead of I8_ROWS_US
 // codes [T][kp], zeros behind a row's k; factors [T].  A CTA a row
-__global__ void __launch_bounds__(I8_THREADS) i8_rows_kernel(const float* __restrict__ x, int64_t rs, int k, int kp, int8_t* __restrict__ codes, float* __restrict__ factors) {
-    __shared__ unsigned tops[I8_THREADS / 32];
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) i8_rows_kernel(const float* __restrict__ x, int64_t rs, int k, int kp, int vec, int8_t* __restrict__ codes, float* __restrict__ factors) {
+    __shared__ unsigned tops[THREADS / 32];
     pdl_enter();
     const int64_t t = blockIdx.x;
     const float* row = x + t * rs;
     unsigned top = 0;
-    for (int c = threadIdx.x; c < k; c += I8_THREADS) top = max(top, __float_as_uint(row[c]) & 0x7fffffffu);
+    float4 keep[I8_KEEP];
+#pragma unroll
+    for (int i = 0; i < I8_KEEP; i++) {
+        const int c = (i * THREADS + threadIdx.x) * 4;
+        if (i * THREADS * 4 >= k) break;
+        keep[i] = i8_load4(row, c, k, vec);
+    }
+#pragma unroll
+    for (int i = 0; i < I8_KEEP; i++) {
+        if (i * THREADS * 4 >= k) break;
+        top = max(top, i8_top4(keep[i]));
+    }
+    for (int c = (I8_KEEP * THREADS + threadIdx.x) * 4; c < k; c += THREADS * 4) top = max(top, i8_top4(i8_load4(row, c, k, vec)));
     top = __reduce_max_sync(0xffffffffu, top);
     if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < I8_THREADS / 32; w++) top = max(top, tops[w]);
-    const bool finite = top < 0x7f800000u;
+    for (int w = 0; w < THREADS / 32; w++) top = max(top, tops[w]);
+    const bool finite = top < 0x7f800000u, some = finite && top;
     const float a = __uint_as_float(top), r = 127.0f / a;
-    for (int c = threadIdx.x; c < kp; c += I8_THREADS) codes[t * kp + c] = c < k && finite && top ? (int8_t)i8_code(row[c], a, r) : (int8_t)0;
+    unsigned* to = (unsigned*)(codes + t * kp);
+#pragma unroll
+    for (int i = 0; i < I8_KEEP; i++) {
+        const int c = (i * THREADS + threadIdx.x) * 4;
+        if (c < kp) to[c >> 2] = some && c < k ? i8_code4(keep[i], a, r) : 0u;
+    }
+    for (int c = (I8_KEEP * THREADS + threadIdx.x) * 4; c < kp; c += THREADS * 4) to[c >> 2] = some ? i8_code4(i8_load4(row, c, k, vec), a, r) : 0u;
     if (threadIdx.x == 0) factors[t] = finite ? a / 127.0f : NAN;
 }
 
-// ---- few rows: a warp an output channel ------------------------------------------------------------------------------------------------------
-#define I8_ROWS 8
-__global__ void __launch_bounds__(I8_THREADS) i8_few_kernel(const int8_t* __restrict__ w, const float* __restrict__ ws, const int8_t* __restrict__ x, const float* __restrict__ xs,
-                                                            float* __restrict__ out, int T, int m, int k, int kp) {
-    pdl_enter();
-    const int lane = threadIdx.x & 31, t0 = blockIdx.y * I8_ROWS, n = min(I8_ROWS, T - t0);
-    const int64_t row = (int64_t)blockIdx.x * (I8_THREADS / 32) + (threadIdx.x >> 5);
-    if (row >= m) return;
-    const int8_t* wr = w + row * k;
-    const bool vec = k % 16 == 0;
-    int acc[I8_ROWS];
+// ---- up to I8_FEW tokens: one kernel ------------------------------------------------------------------------------------------------------------
+// Every CTA codes the tokens by itself, into shared memory, while its first weights are on their way; a warp takes an output channel, 4096 codes of it at a time,
+// the next ones under way behind the sums of these.
+#define I8_FEW 8
+#define I8_RUN 8                             // pieces of 16 codes of a lane: 4096 codes of a warp
+// 16 codes of a row that may start anywhere: the five words around them; near the end of the matrix byte by byte
+__device__ __forceinline__ int4 i8_load16(const int8_t* p, const int8_t* end) {
+    if (p + 20 <= end) {
+        const unsigned* u = (const unsigned*)((uintptr_t)p & ~(uintptr_t)3);
+        const unsigned s = ((unsigned)(uintptr_t)p & 3u) * 8u, u0 = u[0], u1 = u[1], u2 = u[2], u3 = u[3], u4 = s ? u[4] : 0u;
+        return make_int4((int)__funnelshift_r(u0, u1, s), (int)__funnelshift_r(u1, u2, s), (int)__funnelshift_r(u2, u3, s), (int)__funnelshift_r(u3, u4, s));
+    }
+    int z[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < I8_ROWS; i++) acc[i] = 0;
-    for (int c = lane * 16; c < k; c += 512) {
-        int4 u;
-        if (vec) u = ld_stream_16(wr + c);
-        else {
-            int z[4] = {0, 0, 0, 0};
+    for (int j = 0; j < 16; j++)
+        if (p + j < end) z[j / 4] |= (int)(uint8_t)p[j] << (j % 4 * 8);
+    return make_int4(z[0], z[1], z[2], z[3]);
+}
+template <int TB>
+__global__ void __launch_bounds__(I8_THREADS) i8_few_kernel(const int8_t* __restrict__ w, const float* __restrict__ ws, const float* __restrict__ x, int64_t rs, float* __restrict__ out, int T,
+                                                            int m, int k, int kp, int vec) {
+    extern __shared__ __align__(16) int8_t i8_codes[];              // [TB][kp]
+    __shared__ unsigned tops[I8_THREADS / 32][TB];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = gridDim.x * (I8_THREADS / 32), segs = (k + 4095) >> 12;
+    const bool wide = (k & 15) == 0;
+    const int8_t* end = w + (int64_t)m * k;
+    int row = blockIdx.x * (I8_THREADS / 32) + warp, seg = 0;
+    int4 next[I8_RUN];
+    auto fetch = [&](int r, int s) {
 #pragma unroll
-            for (int j = 0; j < 16; j++)
-                if (c + j < k) z[j / 4] |= (int)(uint8_t)wr[c + j] << (j % 4 * 8);
-            u = make_int4(z[0], z[1], z[2], z[3]);
+        for (int i = 0; i < I8_RUN; i++) {
+            const int c = s * 4096 + i * 512 + lane * 16;
+            if (r < m && c < k) next[i] = wide ? ld_stream_16(w + (int64_t)r * k + c) : i8_load16(w + (int64_t)r * k + c, end);
         }
+    };
+    pdl_enter();
+    fetch(row, 0);
+    float xs[TB];
 #pragma unroll
-        for (int i = 0; i < I8_ROWS; i++) {
-            if (i >= n) break;
-            const int4 v = *(const int4*)(x + (int64_t)(t0 + i) * kp + c);
-            acc[i] = __dp4a(u.x, v.x, __dp4a(u.y, v.y, __dp4a(u.z, v.z, __dp4a(u.w, v.w, acc[i]))));
+    for (int t = 0; t < TB; t++) {
+        unsigned top = 0;
+        if (t < T)
+            for (int c = threadIdx.x * 4; c < k; c += I8_THREADS * 4) top = max(top, i8_top4(i8_load4(x + t * rs, c, k, vec)));
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (lane == 0) tops[warp][t] = top;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < TB; t++) {
+        unsigned top = 0;
+#pragma unroll
+        for (int i = 0; i < I8_THREADS / 32; i++) top = max(top, tops[i][t]);
+        const bool finite = top < 0x7f800000u, some = finite && top && t < T;
+        const float a = __uint_as_float(top), r = 127.0f / a;
+        for (int c = threadIdx.x * 4; c < kp; c += I8_THREADS * 4) *(unsigned*)(i8_codes + t * kp + c) = some ? i8_code4(i8_load4(x + t * rs, c, k, vec), a, r) : 0u;
+        xs[t] = finite ? a / 127.0f : NAN;
+    }
+    __syncthreads();
+    int acc[TB];
+#pragma unroll
+    for (int t = 0; t < TB; t++) acc[t] = 0;
+    while (row < m) {
+        int4 u[I8_RUN];
+#pragma unroll
+        for (int i = 0; i < I8_RUN; i++) u[i] = next[i];
+        const int s = seg, r = row;
+        if (++seg == segs) { seg = 0; row += warps; }
+        fetch(row, seg);
+#pragma unroll
+        for (int i = 0; i < I8_RUN; i++) {
+            const int c = s * 4096 + i * 512 + lane * 16;
+            if (c >= k) break;
+#pragma unroll
+            for (int t = 0; t < TB; t++) {
+                const int4 v = *(const int4*)(i8_codes + t * kp + c);
+                acc[t] = __dp4a(u[i].x, v.x, __dp4a(u[i].y, v.y, __dp4a(u[i].z, v.z, __dp4a(u[i].w, v.w, acc[t]))));
+            }
+        }
+        if (seg) continue;
+        const float factor = ws[r];
+#pragma unroll
+        for (int t = 0; t < TB; t++) {
+            const int sum = __reduce_add_sync(0xffffffffu, acc[t]);
+            if (lane == 0 && t < T) out[(int64_t)t * m + r] = (float)sum * factor * xs[t];
+            acc[t] = 0;
         }
     }
-#pragma unroll
-    for (int i = 0; i < I8_ROWS; i++) acc[i] = warp_sum_i(acc[i]);
-    if (lane == 0)
-        for (int i = 0; i < n; i++) out[(int64_t)(t0 + i) * m + row] = (float)acc[i] * ws[row] * xs[t0 + i];
 }
-
+template <int TB>
+static cudaError_t i8_launch_few(cc_device* dev, const int8_t* w, const float* ws, const float* x, int64_t rs, float* out, int T, int m, int k, int kp, int vec) {
+    const size_t smem = (size_t)TB * kp;
+    const int per = (int)std::min<size_t>(4, 200 * 1024 / (smem + 1024)), rows = I8_THREADS / 32;
+    const int64_t grid = std::min<int64_t>((m + rows - 1) / rows, (int64_t)per * dev->sm_count);
+    cudaError_t e = cudaSuccess;
+    if (smem > 48 * 1024) e = cudaFuncSetAttribute(i8_few_kernel<TB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) e = cc_launch_pdl(dev, i8_few_kernel<TB>, (unsigned)grid, I8_THREADS, smem, w, ws, x, rs, out, T, m, k, kp, vec);
+    dev->launches++;
+    return e;
+}
 
 // ---- many rows: tcgen05.mma on 8-bit tiles -----------------------------------------------------------------------------------------------------
 // A tile is 128 output channels (the instruction's rows, TMEM's lanes) x BN tokens; a step of 128 codes of both comes by TMA into a ring, one thread issues
@@ -300,31 +397,34 @@ __global__ void i8_pad_kernel(const int8_t* __restrict__ w, int8_t* __restrict__
 }
 
 static int i8_product(cc_device* dev, const int8_t* w, const float* ws, const float* x, int64_t rs, float* out, int T, int m, int k) {
-    const int kp = (k + 15) / 16 * 16;
-    const bool tiles = T > 8, pad = tiles && k != kp;
+    const int kp = (k + 15) / 16 * 16, vec = rs % 4 == 0 && ((uintptr_t)x & 15) == 0;
+    cudaError_t e;
+    if (T <= I8_FEW && (size_t)(T <= 1 ? 1 : T <= 2 ? 2 : T <= 4 ? 4 : 8) * kp <= 160 * 1024) {
+        e = T <= 1 ? i8_launch_few<1>(dev, w, ws, x, rs, out, T, m, k, kp, vec) : T <= 2 ? i8_launch_few<2>(dev, w, ws, x, rs, out, T, m, k, kp, vec)
+            : T <= 4 ? i8_launch_few<4>(dev, w, ws, x, rs, out, T, m, k, kp, vec) : i8_launch_few<8>(dev, w, ws, x, rs, out, T, m, k, kp, vec);
+        return e == cudaSuccess ? CC_OK : cc_fail(dev, CC_ERR_CUDA, "product_i8: %s", cudaGetErrorString(e));
+    }
+    const bool pad = k != kp;
     const size_t codes = ((size_t)T * kp + 255) / 256 * 256, factors = ((size_t)T * 4 + 255) / 256 * 256;
-    void* ws_mem = nullptr; size_t cls = 0;
-    int rc = cc_pool_alloc(dev, codes + factors + (pad ? (size_t)m * kp : 0), &ws_mem, &cls);
+    void* mem = nullptr; size_t cls = 0;
+    int rc = cc_pool_alloc(dev, codes + factors + (pad ? (size_t)m * kp : 0), &mem, &cls);
     if (rc) return rc;
-    int8_t* xq = (int8_t*)ws_mem;
-    float* xs = (float*)((uint8_t*)ws_mem + codes);
-    cudaError_t e = cc_launch_pdl(dev, i8_rows_kernel, (unsigned)T, I8_THREADS, 0, x, rs, k, kp, xq, xs);
+    int8_t* xq = (int8_t*)mem;
+    float* xs = (float*)((uint8_t*)mem + codes);
+    e = k <= 4096 ? cc_launch_pdl(dev, i8_rows_kernel<256>, (unsigned)T, 256, 0, x, rs, k, kp, vec, xq, xs)
+        : k <= 8192 ? cc_launch_pdl(dev, i8_rows_kernel<512>, (unsigned)T, 512, 0, x, rs, k, kp, vec, xq, xs) : cc_launch_pdl(dev, i8_rows_kernel<1024>, (unsigned)T, 1024, 0, x, rs, k, kp, vec, xq, xs);
     dev->launches++;
     if (pad && e == cudaSuccess) {
-        int8_t* wp = (int8_t*)ws_mem + codes + factors;
+        int8_t* wp = (int8_t*)mem + codes + factors;
         const int64_t n4 = (int64_t)m * (kp / 4);
         e = cc_launch_pdl(dev, i8_pad_kernel, (unsigned)((n4 + 255) / 256), 256, 0, w, wp, n4, k, kp / 4);
         dev->launches++;
         w = wp;
     }
-    if (e == cudaSuccess && !tiles) {
-        e = cc_launch_pdl(dev, i8_few_kernel, dim3((unsigned)((m + I8_THREADS / 32 - 1) / (I8_THREADS / 32)), (unsigned)((T + I8_ROWS - 1) / I8_ROWS)), I8_THREADS, 0, w, ws, xq, xs, out, T, m, k, kp);
-        dev->launches++;
-    }
     if (e != cudaSuccess) rc = cc_fail(dev, CC_ERR_CUDA, "product_i8: %s", cudaGetErrorString(e));
-    else if (tiles) rc = T <= 16 ? gi_launch<16>(dev, w, ws, xq, xs, out, T, m, kp) : T <= 32 ? gi_launch<32>(dev, w, ws, xq, xs, out, T, m, kp)
-                       : T <= 64 ? gi_launch<64>(dev, w, ws, xq, xs, out, T, m, kp) : T <= 128 ? gi_launch<128>(dev, w, ws, xq, xs, out, T, m, kp) : gi_launch<256>(dev, w, ws, xq, xs, out, T, m, kp);
-    cc_pool_free(dev, ws_mem, cls);
+    else rc = T <= 16 ? gi_launch<16>(dev, w, ws, xq, xs, out, T, m, kp) : T <= 32 ? gi_launch<32>(dev, w, ws, xq, xs, out, T, m, kp)
+              : T <= 64 ? gi_launch<64>(dev, w, ws, xq, xs, out, T, m, kp) : T <= 128 ? gi_launch<128>(dev, w, ws, xq, xs, out, T, m, kp) : gi_launch<256>(dev, w, ws, xq, xs, out, T, m, kp);
+    cc_pool_free(dev, mem, cls);
     return rc;
 }
 

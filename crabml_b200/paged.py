@@ -54,7 +54,15 @@ class PagedCache:
     """One layer's pages: k, v [pages, heads, page size, size] in F16, or in I8 with factors [pages, heads] and open blocks [2 * slots, heads, page size, size]"""
 
     def __init__(self, k, v, k_scale=None, v_scale=None, k_open=None, v_open=None):
-        self.k, self.v, self.k_scale, self.v_scale, self.k_open, self.v_open = k, v, k_scale, v_scale, k_open, v_open
+        self._tensors = {"k": k, "v": v, "k_scale": k_scale, "v_scale": v_scale, "k_open": k_open, "v_open": v_open}
+        self._c = capi.cc_paged_cache(**{n: t._view() for n, t in self._tensors.items() if t is not None})
+
+    k = property(lambda self: self._tensors["k"])
+    v = property(lambda self: self._tensors["v"])
+    k_scale = property(lambda self: self._tensors["k_scale"])
+    v_scale = property(lambda self: self._tensors["v_scale"])
+    k_open = property(lambda self: self._tensors["k_open"])
+    v_open = property(lambda self: self._tensors["v_open"])
 
     @classmethod
     def alloc(cls, device, n_pages, n_kv, page_size, dk, dv=None, dtype=capi.I8, n_slots=0):
@@ -65,14 +73,6 @@ class PagedCache:
             t += [CudaTensor.alloc([2 * n_slots, n_kv, page_size, d], capi.F16, device) for d in (dk, dv)]
         return cls(*t)
 
-    def _struct(self):
-        s = capi.cc_paged_cache()
-        for name in ("k", "v", "k_scale", "v_scale", "k_open", "v_open"):
-            t = getattr(self, name)
-            if t is not None:
-                setattr(s, name, t._view())
-        return s
-
 
 def _v(t):
     return C.byref(t._view()) if t is not None else None
@@ -80,14 +80,14 @@ def _v(t):
 
 def append(plan, cache, q_src, q_col0, k_src, k_col0, v_src, v_col0, n_heads=0, freq=None, pairing=capi.ROPE_NEIGHBOURS, offset=0, mag=1.0):
     """keys and values of the plan's tokens, turned by their positions, into the pages -> the turned queries [T, n_heads * dk] (q_src None: None)"""
-    dev, h, s = plan.device, C.c_void_p(), cache._struct()
-    dev.check(dev.lib.cc_paged_append(dev.handle, plan.handle, C.byref(s), _v(q_src), int(q_col0), _v(k_src), int(k_col0), _v(v_src), int(v_col0), int(n_heads), _v(freq),
+    dev, h = plan.device, C.c_void_p()
+    dev.check(dev.lib.cc_paged_append(dev.handle, plan.handle, C.byref(cache._c), _v(q_src), int(q_col0), _v(k_src), int(k_col0), _v(v_src), int(v_col0), int(n_heads), _v(freq),
                                       int(pairing), int(offset), float(mag), C.byref(h)))
     return None if q_src is None else CudaTensor(_Buf(dev, h), TensorStrider([plan.tokens, n_heads * cache.k.shape()[3]]), dev)
 
 
 def attention(plan, cache, q, n_heads, scale, window=0, softcap=0.0, sink=None):
     """-> [T, n_heads * dv]"""
-    dev, h, s = plan.device, C.c_void_p(), cache._struct()
-    dev.check(dev.lib.cc_paged_attention(dev.handle, plan.handle, C.byref(s), _v(q), int(n_heads), float(scale), int(window), float(softcap), _v(sink), C.byref(h)))
+    dev, h = plan.device, C.c_void_p()
+    dev.check(dev.lib.cc_paged_attention(dev.handle, plan.handle, C.byref(cache._c), _v(q), int(n_heads), float(scale), int(window), float(softcap), _v(sink), C.byref(h)))
     return CudaTensor(_Buf(dev, h), TensorStrider([plan.tokens, n_heads * cache.v.shape()[3]]), dev)

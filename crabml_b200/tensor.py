@@ -182,9 +182,12 @@ def _shape_arr(shape):
 class CudaTensor:
     def __init__(self, buf: _Buf, strider: TensorStrider, device: CudaTensorDevice, name=None):
         self.buf, self._strider, self.device, self.name = buf, strider, device, name
+        self._cview = self._cview_of = None
 
     # -- plumbing ------------------------------------------------------------------------------
     def _view(self):
+        if self._cview_of is self._strider:                        # made once for a tensor's strider: a call has half a dozen of them
+            return self._cview
         v = cc_view()
         v.buf = self.buf.handle
         v.ndim = len(self._strider.shape)
@@ -192,18 +195,19 @@ class CudaTensor:
             raise TensorError("too many dims")
         for i, (s, t) in enumerate(zip(self._strider.shape, self._strider.strides)):
             v.shape[i], v.strides[i] = s, t
+        self._cview, self._cview_of = v, self._strider
         return v
 
     @property
     def __cuda_array_interface__(self):
         """the tensor's own memory for other libraries (torch.as_tensor and the like), ordered by the device's stream"""
-        if self.dtype() not in capi.ARRAY_TYPES:
+        kind, size = capi.ARRAY_TYPES.get(self.dtype(), (None, 0))
+        if kind is None:
             raise AttributeError(f"a tensor of type {self.dtype()} is not a plain array")
         self.device.flush()
-        kind, size = capi.ARRAY_TYPES[self.dtype()]
-        empty = self._strider.len() == 0
-        return {"shape": tuple(self.shape()), "typestr": kind, "data": (0 if empty else int(self.device.lib.cc_tensor_data(self.buf.handle)), False),
-                "strides": tuple(s * size for s in self._strider.strides), "stream": self.device.stream(), "version": 3}
+        shape = tuple(self._strider.shape)
+        return {"shape": shape, "typestr": kind, "data": (0 if 0 in shape else self.device.lib.cc_tensor_data(self.buf.handle), False),
+                "strides": None if self._strider.is_contiguous() else tuple(s * size for s in self._strider.strides), "stream": self.device.stream(), "version": 3}
 
     def _new(self, handle, shape):
         return CudaTensor(_Buf(self.device, handle), TensorStrider(shape), self.device)

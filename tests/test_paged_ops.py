@@ -257,6 +257,26 @@ def test_attention_shapes(dev, shape, i8):
     check_attention(dev, 32, G, Rh, dk, dv, i8, [0, 100, 31, 32, 700], [1, 1, 1, 2, 1], seed=dk)
 
 
+TILES = [(1, 1, 16, 16), (2, 4, 64, 64), (1, 8, 128, 128), (2, 3, 80, 96), (1, 5, 96, 48), (1, 2, 32, 128), (1, 7, 112, 16), (1, 2, 256, 128), (1, 1, 64, 256)]
+
+
+@pytest.mark.parametrize("i8", [False, True], ids=["f16", "i8"])
+@pytest.mark.parametrize("shape", TILES, ids=["x".join(map(str, s)) for s in TILES])
+def test_attention_of_many_rows(dev, shape, i8):
+    """prompts of ragged lengths, from the start and late, beside a decoded token and a sequence at rest"""
+    G, Rh, dk, dv = shape
+    check_attention(dev, 32, G, Rh, dk, dv, i8, [0, 100, 31, 5, 300], [70, 33, 0, 1, 129], seed=dk + dv)
+
+
+@pytest.mark.parametrize("i8", [False, True], ids=["f16", "i8"])
+@pytest.mark.parametrize("P,pos0,counts,kw", [(16, [5000], [20], {}), (64, [2999, 10], [17, 300], {}), (128, [4500], [40], dict(window=3000, sink=True)), (32, [0], [600], dict(softcap=20.0)),
+                                              (64, [1000], [50], dict(window=1)), (16, [3000], [33], dict(window=130, sink=True, softcap=5.0))],
+                         ids=["slices", "mixed", "window", "prompt", "itself", "all"])
+def test_attention_of_many_rows_far(dev, P, pos0, counts, kw, i8):
+    """few rows over long caches are dealt out in slices; windows that leave most of a cache out"""
+    check_attention(dev, P, 1, 8, 64, 64, i8, pos0, counts, seed=P, **kw)
+
+
 @pytest.mark.parametrize("i8", [False, True], ids=["f16", "i8"])
 @pytest.mark.parametrize("P", [16, 32, 64, 128])
 @pytest.mark.parametrize("pos0,counts", [([0], [1]), ([14, 15, 16], [1, 1, 1]), ([2000], [1]), ([0, 0, 5], [17, 0, 40]), ([127, 128, 129, 640], [3, 1, 2, 64]), ([0], [200])],
@@ -288,7 +308,7 @@ def test_attention_sizes_of_numbers(dev, q_scale, i8):
 
 
 @pytest.mark.parametrize("i8", [False, True], ids=["f16", "i8"])
-@pytest.mark.parametrize("counts", [[1, 6], [1, 70]], ids=["few", "many"])
+@pytest.mark.parametrize("counts", [[1, 6], [1, 70], [1, 300]], ids=["few", "many", "more"])
 def test_what_a_query_does_not_see(dev, i8, counts):
     """NaN and infinities in keys and values reach the queries that see them and no others; rows behind a sequence's end are not looked at"""
     G, Rh, d, P, pos0 = 1, 4, 64, 32, [40, 100]
