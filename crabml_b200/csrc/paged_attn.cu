@@ -547,7 +547,8 @@ static int pt_run(cc_device* dev, const cc_page_plan* plan, PtArgs a, bool i8) {
         e = i8 ? (d <= 64 ? pt_launch_few<64, true>(dev, a, (unsigned)items) : d <= 128 ? pt_launch_few<128, true>(dev, a, (unsigned)items) : pt_launch_few<256, true>(dev, a, (unsigned)items))
                : (d <= 64 ? pt_launch_few<64, false>(dev, a, (unsigned)items) : d <= 128 ? pt_launch_few<128, false>(dev, a, (unsigned)items) : pt_launch_few<256, false>(dev, a, (unsigned)items));
     } else {
-        auto kernel = i8 ? paged_tile_kernel<true> : paged_tile_kernel<false>;
+        const bool cap = a.softcap > 0.0f;
+        auto kernel = i8 ? (cap ? paged_tile_kernel<true, true> : paged_tile_kernel<true, false>) : (cap ? paged_tile_kernel<false, true> : paged_tile_kernel<false, false>);
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TI_SMEM);
         if (e == cudaSuccess) e = cc_launch_pdl(dev, kernel, dim3((unsigned)items, (unsigned)a.G), TI_THREADS, TI_SMEM, a, dev->err_dev, dev->err_host);
         dev->launches++;

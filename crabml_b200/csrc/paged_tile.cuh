@@ -17,8 +17,7 @@
 #define TI_KEYS 128
 #define TI_THREADS 384                        // three warps a scheduler: 168 registers a thread (a thirteenth warp would leave 128)
 #define TI_SOFT 256
-#define TI_LOAD 96
-#define TI_EACH 11                            // pieces of 16 bytes of a unit of 16 KB, a thread of TI_LOAD
+#define TI_LOADERS 3
 #define TI_MOST 4096                          // keys of a slice
 #define TI_D 128                              // largest dk and dv
 
@@ -28,6 +27,8 @@ struct TiShared {
     int fail, wild[4];                        // wild[step % 4] == step + 1: values that are not finite were left out of the step's sums
     int page[TI_MOST / 16 + 8];              // of every 16 keys: -1 - block for the open one
     float kf[TI_MOST / 16 + 8], vf[TI_MOST / 16 + 8];
+    int lost;                                // some factor is not finite: it counts as 0, and NaN goes to the rows that see its keys (nan)
+    uint8_t nan[TI_MOST / 16 + 8];
     float top[2][2][TI_ROWS], sum[2][TI_ROWS];
 };
 #define TI_OPERAND (TI_KEYS * TI_D * 2)       // bytes of a tile of f16: two blocks of 64 columns, rows of 128 bytes under the 128-byte swizzle
@@ -52,7 +53,7 @@ __device__ __forceinline__ float ti_exp2(float x) {
 }
 __device__ __forceinline__ void ti_soft_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-template <bool I8>
+template <bool I8, bool CAP>
 __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const PtArgs a, unsigned* err_dev, unsigned* err_host) {
     extern __shared__ __align__(1024) uint8_t ti_raw[];
     __shared__ TiShared sh;
@@ -62,15 +63,16 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const PtArgs 
     if (tid == 0) {
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            pg_mbar_init(pg_smem(&sh.k_full[i]), TI_LOAD / 32); pg_mbar_init(pg_smem(&sh.v_full[i]), TI_LOAD / 32); pg_mbar_init(pg_smem(&sh.k_empty[i]), 1); pg_mbar_init(pg_smem(&sh.v_empty[i]), 1);
+            pg_mbar_init(pg_smem(&sh.k_full[i]), TI_KEYS / 16); pg_mbar_init(pg_smem(&sh.v_full[i]), TI_KEYS / 16); pg_mbar_init(pg_smem(&sh.k_empty[i]), 1); pg_mbar_init(pg_smem(&sh.v_empty[i]), 1);
             pg_mbar_init(pg_smem(&sh.s_full[i]), 1); pg_mbar_init(pg_smem(&sh.p_full[i]), 8); pg_mbar_init(pg_smem(&sh.o_full[i]), 1); pg_mbar_init(pg_smem(&sh.o_empty[i]), 8);
             sh.wild[i] = sh.wild[i + 2] = 0;
         }
         pg_mbar_init(pg_smem(&sh.drained), 1);
-        sh.fail = 0;
+        sh.fail = sh.lost = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_enter();
+    __syncthreads();
     int rest;
     const int seq = pt_find(a, blockIdx.x, [&](const PgSeq& s) { return pt_splits(s, a) * (int)(((int64_t)s.count * a.R + TI_ROWS - 1) / TI_ROWS); }, &rest);
     if (seq < 0) return;                                              // (the grid has as many CTAs as there are items)
@@ -91,7 +93,9 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const PtArgs 
             if (I8 && key >= opens) page = -1 - (2 * s.slot + ((to >> a.shift) & 1));
             else if (I8) { kf = a.ks[(int64_t)page * a.G + kvh]; vf = a.vs[(int64_t)page * a.G + kvh]; }
         }
-        sh.page[i] = page; sh.kf[i] = kf; sh.vf[i] = vf;
+        const bool bad = !(vf >= 0.0f && vf < INFINITY && kf >= 0.0f && kf < INFINITY);
+        sh.page[i] = page; sh.kf[i] = bad ? 0.0f : kf; sh.vf[i] = bad ? 0.0f : vf; sh.nan[i] = bad;
+        if (bad) sh.lost = 1;
     }
     if (warp == 11) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pg_smem(&sh.tmem_base)), "n"(512) : "memory");
@@ -115,7 +119,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const PtArgs 
         int ex = 14;
         if (top > 0.0f && top < INFINITY) frexpf(top, &ex);
         ex = max(ex, -100);
-        const float f = ldexpf(1.0f, 14 - ex);
+        const float f = copysignf(ldexpf(1.0f, 14 - ex), a.scale);      // (so that a larger sum is a larger score)
         inv = ldexpf(1.0f, ex - 14);
         for (int j = half; j < a.dk / 8; j += 2) {
             float v[8];
@@ -174,98 +178,99 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const PtArgs 
         }
         __syncwarp();
     } else if (warp >= 8) {
-        // ===== keys and values: pieces of 16 bytes, TI_EACH of a thread at a time (a unit); the next unit's are under way while these are converted =====
-        const int t = tid - TI_SOFT, E = I8 ? 16 : 8;
-        constexpr int PER = I8 ? 1 : 2;                               // units of an operand
-        const int units = steps * 2 * PER;
-        int4 raw[2][TI_EACH];
-        // pieces i * TI_LOAD + t of a unit, rows of `per` pieces: the first one's row and piece, and what TI_LOAD pieces further on are, for keys and for values
-        const int per_k = a.dk / E, per_v = a.dv / E, row_k = t / per_k, row_v = t / per_v;
-        auto pieces = [&](int unit, auto each) {
-            const int op = unit / PER, n = TI_KEYS / PER, first = (unit - op * PER) * n;
-            const bool val = op & 1;
-            const int per = val ? per_v : per_k, row_by = TI_LOAD / per, piece_by = TI_LOAD - row_by * per;
-            int key = val ? row_v : row_k, piece = t - key * per;
+        // ===== keys and values: a warp takes 16 rows of an operand at a time (a group: they lie in one page), the next two groups' are under way =====
+        constexpr int N = I8 ? 4 : 8, E = I8 ? 16 : 8, AHEAD = 2;      // pieces of 16 bytes of a lane and group, numbers of a piece
+        const int groups = steps * (TI_KEYS / 8);                      // of keys and values by turns of a step
+        const int per_k = a.dk / E, per_v = a.dv / E;
+        int4 raw[AHEAD + 1][N];
+        auto where = [&](int u, int& step, bool& val, int& g) { step = u / (TI_KEYS / 8); val = u & (TI_KEYS / 16); g = u & (TI_KEYS / 16 - 1); };
+        auto fetch = [&](int u, int4 (&r)[N]) {
+            int step, g;
+            bool val;
+            where(u, step, val, g);
+            if (u >= groups) return;
+            const int key = lo + step * TI_KEYS + g * 16, page = sh.page[step * (TI_KEYS / 16) + g], d = val ? a.dv : a.dk, n = 16 * (val ? per_v : per_k), there = min(16, to - key) * (val ? per_v : per_k);
+            if (I8 && page < 0) return;                                // the open block's rows come when they are stored
+            const size_t at = (((size_t)page * a.G + kvh) * a.page + (key & (a.page - 1))) * d;
+            const int4* p = (const int4*)((val ? a.v : a.k) + (I8 ? at : at * 2)) + lane;
 #pragma unroll
-            for (int i = 0; i < TI_EACH; i++) {
-                if (key < n) each(i, op >> 1, val, first + key, piece);
-                key += row_by; piece += piece_by;
-                if (piece >= per) { piece -= per; key++; }
-            }
+            for (int i = 0; i < N; i++) r[i] = i * 32 + lane < n && i * 32 + lane < there ? __ldg(p + i * 32) : make_int4(0, 0, 0, 0);       // zeros behind the end
         };
-        auto fetch = [&](int unit, int4 (&r)[TI_EACH]) {
-            if (unit >= units) return;
-            pieces(unit, [&](int i, int step, bool val, int key, int piece) {
-                const int abs_key = lo + step * TI_KEYS + key, page = sh.page[step * (TI_KEYS / 16) + (key >> 4)], d = val ? a.dv : a.dk;
-                r[i] = make_int4(0, 0, 0, 0);
-                if (abs_key >= to || (I8 && page < 0)) return;        // zeros behind the end; the open block's rows come when they are stored
-                const size_t at = (((size_t)page * a.G + kvh) * a.page + (abs_key & (a.page - 1))) * d;
-                r[i] = __ldg((const int4*)((val ? a.v : a.k) + (I8 ? at : at * 2)) + piece);
-            });
-        };
-        auto store = [&](int unit, const int4 (&r)[TI_EACH]) {
-            bool wild = false;
-            int at_step = 0;
-            pieces(unit, [&](int i, int step, bool val, int key, int piece) {
-                uint8_t* to_smem = (val ? vs : ks) + (size_t)(step & 1) * TI_OPERAND;
-                at_step = step;
-                if (I8) {
-                    const int page = sh.page[step * (TI_KEYS / 16) + (key >> 4)], abs_key = lo + step * TI_KEYS + key, d = val ? a.dv : a.dk;
-                    uint4 x, y;
-                    if (page < 0) {
-                        const __half* p = (val ? a.vo : a.ko) + (((size_t)(-1 - page) * a.G + kvh) * a.page + (abs_key & (a.page - 1))) * d + piece * 16;
-                        x = y = make_uint4(0, 0, 0, 0);
-                        if (abs_key < to) { x = *(const uint4*)p; y = *(const uint4*)(p + 8); }
-                        if (val) {
-                            wild |= (pt_wild(x.x) | pt_wild(x.y) | pt_wild(x.z) | pt_wild(x.w) | pt_wild(y.x) | pt_wild(y.y) | pt_wild(y.z) | pt_wild(y.w)) != 0u;
-                            x.x &= ~pt_wild(x.x); x.y &= ~pt_wild(x.y); x.z &= ~pt_wild(x.z); x.w &= ~pt_wild(x.w);
-                            y.x &= ~pt_wild(y.x); y.y &= ~pt_wild(y.y); y.z &= ~pt_wild(y.z); y.w &= ~pt_wild(y.w);
-                        }
-                    } else {
-                        const unsigned u0 = (unsigned)r[i].x ^ 0x80808080u, u1 = (unsigned)r[i].y ^ 0x80808080u, u2 = (unsigned)r[i].z ^ 0x80808080u, u3 = (unsigned)r[i].w ^ 0x80808080u;
-                        x = make_uint4(pt_half2(u0, 0x4140), pt_half2(u0, 0x4342), pt_half2(u1, 0x4140), pt_half2(u1, 0x4342));
-                        y = make_uint4(pt_half2(u2, 0x4140), pt_half2(u2, 0x4342), pt_half2(u3, 0x4140), pt_half2(u3, 0x4342));
-                        if (abs_key >= to) x = y = make_uint4(0, 0, 0, 0);
-                    }
-                    const bool odd = piece & 4;                       // the lanes of a row fill all banks at once
-                    *(uint4*)(to_smem + ti_at(key, 2 * piece + odd)) = odd ? y : x;
-                    *(uint4*)(to_smem + ti_at(key, 2 * piece + !odd)) = odd ? x : y;
-                } else {
-                    uint4 x = make_uint4((unsigned)r[i].x, (unsigned)r[i].y, (unsigned)r[i].z, (unsigned)r[i].w);
-                    if (val) {
-                        const unsigned w0 = pt_wild(x.x), w1 = pt_wild(x.y), w2 = pt_wild(x.z), w3 = pt_wild(x.w);
-                        wild |= (w0 | w1 | w2 | w3) != 0u;
-                        x.x &= ~w0; x.y &= ~w1; x.z &= ~w2; x.w &= ~w3;
-                    }
-                    *(uint4*)(to_smem + ti_at(key, piece)) = x;
+        auto store = [&](int u, const int4 (&r)[N]) {
+            int step, g;
+            bool val, wild = false;
+            where(u, step, val, g);
+            uint8_t* base = (val ? vs : ks) + (size_t)(step & 1) * TI_OPERAND + g * 2048;
+            const int per = val ? per_v : per_k, page = sh.page[step * (TI_KEYS / 16) + g], key = lo + step * TI_KEYS + g * 16, d = val ? a.dv : a.dk;
+            int row = lane / per, piece = lane - row * per;
+            const int row_by = 32 / per, piece_by = 32 - row_by * per;
+            auto clean = [&](uint4& x) {
+                const unsigned w0 = pt_wild(x.x), w1 = pt_wild(x.y), w2 = pt_wild(x.z), w3 = pt_wild(x.w);
+                wild |= (w0 | w1 | w2 | w3) != 0u;
+                x.x &= ~w0; x.y &= ~w1; x.z &= ~w2; x.w &= ~w3;
+            };
+            if (I8 && page < 0) {                                      // 16-bit rows of the open block
+                const __half* p = (val ? a.vo : a.ko) + (((size_t)(-1 - page) * a.G + kvh) * a.page + (key & (a.page - 1))) * d;
+#pragma unroll 1
+                for (int e = lane; e < 16 * (d / 8); e += 32) {
+                    const int rr = e / (d / 8), chunk = e - rr * (d / 8);
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (key + rr < to) x = ((const uint4*)p)[e];
+                    if (val) clean(x);
+                    *(uint4*)(base + ti_at(rr, chunk)) = x;
                 }
-            });
-            if (wild) atomicExch(&sh.wild[at_step & 3], at_step + 1);
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    if (row < 16) {
+                        if (I8) {
+                            const unsigned u0 = (unsigned)r[i].x ^ 0x80808080u, u1 = (unsigned)r[i].y ^ 0x80808080u, u2 = (unsigned)r[i].z ^ 0x80808080u, u3 = (unsigned)r[i].w ^ 0x80808080u;
+                            const uint4 x = make_uint4(pt_half2(u0, 0x4140), pt_half2(u0, 0x4342), pt_half2(u1, 0x4140), pt_half2(u1, 0x4342));
+                            const uint4 y = make_uint4(pt_half2(u2, 0x4140), pt_half2(u2, 0x4342), pt_half2(u3, 0x4140), pt_half2(u3, 0x4342));
+                            const bool odd = piece & 4;                // the lanes of a row fill all banks at once
+                            uint8_t* q = base + ti_at(row, 2 * piece);
+                            const int other = 16 - 32 * (row & 1);     // chunk 2 piece + 1 lies beside it under the swizzle
+                            *(uint4*)(odd ? q + other : q) = odd ? y : x;
+                            *(uint4*)(odd ? q : q + other) = odd ? x : y;
+                        } else {
+                            uint4 x = make_uint4((unsigned)r[i].x, (unsigned)r[i].y, (unsigned)r[i].z, (unsigned)r[i].w);
+                            if (val) clean(x);
+                            *(uint4*)(base + ti_at(row, piece)) = x;
+                        }
+                    }
+                    row += row_by; piece += piece_by;
+                    if (piece >= per) { piece -= per; row++; }
+                }
+            }
+            if (wild) atomicExch(&sh.wild[step & 3], step + 1);
         };
         bool ok = true;
-        fetch(0, raw[0]);
-        for (int u0 = 0; u0 < units && ok; u0 += 2) {
+        const int first = warp - TI_SOFT / 32;
 #pragma unroll
-            for (int x = 0; x < 2; x++) {
-                const int unit = u0 + x, op = unit / PER, step = op >> 1;
-                const unsigned slot = step & 1, ph = (step >> 1) & 1u;
-                if (unit >= units || !ok) break;
-                fetch(unit + 1, raw[x ^ 1]);
-                if (unit % PER == 0 && !(ok = sg_wait_warp(pg_smem(op & 1 ? &sh.v_empty[slot] : &sh.k_empty[slot]), ph ^ 1u, &sh.fail))) break;
-                store(unit, raw[x]);
-                if (unit % PER == PER - 1) {
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    sg_arrive(pg_smem(op & 1 ? &sh.v_full[slot] : &sh.k_full[slot]));
-                }
-            }
+        for (int i = 0; i < AHEAD; i++) fetch(first + i * TI_LOADERS, raw[i]);
+#pragma unroll 1
+        for (int u = first; u < groups; u += TI_LOADERS) {
+            int step, g;
+            bool val;
+            where(u, step, val, g);
+            fetch(u + AHEAD * TI_LOADERS, raw[AHEAD]);
+            if (!(ok = sg_wait_warp(pg_smem(val ? &sh.v_empty[step & 1] : &sh.k_empty[step & 1]), ((step >> 1) & 1u) ^ 1u, &sh.fail))) break;
+            store(u, raw[0]);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            sg_arrive(pg_smem(val ? &sh.v_full[step & 1] : &sh.k_full[step & 1]));
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++)
+#pragma unroll
+                for (int j = 0; j < N; j++) raw[i][j] = raw[i + 1][j];
         }
     } else {
         // ===== weights and sums =====
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
         const int c_first = half ? ((a.dv / 2 + 15) & ~15) : 0, cols = half ? a.dv - c_first : (a.dv / 2 + 15) & ~15;      // this thread's columns of O
         const int pos = in ? s.pos0 + tok : -1, key_lo = a.window > 0 ? pos - a.window + 1 : 0, key_hi = min(pos, k1 - 1);      // the last step may reach into the next slice
-        const float f0 = a.softcap > 0.0f ? inv * a.scale : inv * (a.scale * PT_LOG2E);
+        const float f0 = inv * fabsf(a.scale) * (CAP ? 1.0f : PT_LOG2E);
         float acc[TI_D / 2], m = -INFINITY, l = 0.0f, alpha_prev = 0.0f, vref_prev = 0.0f;
+        unsigned lost0 = 0u, lost1 = 0u;                              // columns of this thread that have met a value that is not finite
 #pragma unroll
         for (int i = 0; i < TI_D / 2; i++) acc[i] = 0.0f;
         bool ok = true;
@@ -282,30 +287,33 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const PtArgs 
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     asm volatile("" : "+r"(v[i]));
-                    acc[c + i] = fmaf(__uint_as_float(v[i]), vref_prev, acc[c + i] * alpha_prev);
+                    acc[c + i] = I8 ? fmaf(__uint_as_float(v[i]), vref_prev, acc[c + i] * alpha_prev) : fmaf(acc[c + i], alpha_prev, __uint_as_float(v[i]));
                 }
             }
             pg_fence_before();
-            if (*(volatile int*)&sh.wild[k & 3] == k + 1) {            // NaN for the rows that see them
+            sg_arrive(pg_smem(&sh.o_empty[slot]));
+            if (*(volatile int*)&sh.wild[k & 3] == k + 1 || sh.lost) {
+#pragma unroll 1
                 for (int j = 0; j < TI_KEYS; j++) {
-                    const int key = lo + k * TI_KEYS + j;
+                    const int key = lo + k * TI_KEYS + j, g = k * (TI_KEYS / 16) + (j >> 4), page = sh.page[g];
                     if (key > key_hi || key < key_lo) continue;
-                    const int page = sh.page[k * (TI_KEYS / 16) + (j >> 4)];
+                    if (sh.nan[g]) lost0 = lost1 = ~0u;
                     if (I8 && page >= 0) continue;
                     const __half* p = (I8 ? a.vo : (const __half*)a.v) + (((size_t)(I8 ? -1 - page : page) * a.G + kvh) * a.page + (key & (a.page - 1))) * a.dv + c_first;
-#pragma unroll
-                    for (int c = 0; c < TI_D / 2; c++)
-                        if (c < cols && ((unsigned)__half_as_ushort(p[c]) & 0x7c00u) == 0x7c00u) acc[c] = NAN;
+#pragma unroll 1
+                    for (int c = 0; c < cols; c++) {
+                        const unsigned bit = ((unsigned)__half_as_ushort(p[c]) & 0x7c00u) == 0x7c00u ? 1u << (c & 31) : 0u;
+                        if (c < 32) lost0 |= bit; else lost1 |= bit;
+                    }
                 }
             }
-            sg_arrive(pg_smem(&sh.o_empty[slot]));
         };
+#pragma unroll 1
         for (int k = 0; k < steps; k++) {
             const unsigned slot = k & 1;
             const int key0 = lo + k * TI_KEYS + half * 64;
             ok = ok && sg_wait_warp(pg_smem(&sh.s_full[slot]), (k >> 1) & 1u, &sh.fail);
             unsigned x[64];
-            float vmax = 0.0f;
             if (ok) {
                 pg_fence_after();
 #pragma unroll
@@ -314,32 +322,46 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const PtArgs 
 #pragma unroll
                 for (int c = 0; c < 64; c++) asm volatile("" : "+r"(x[c]));
             }
-            const float* kf = sh.kf + k * (TI_KEYS / 16) + half * 4;
-            const float* vfs = sh.vf + k * (TI_KEYS / 16);
-            float mx = -INFINITY;
+            float f[4];                                               // factor of 16 keys' sums; 0 (a block of zeros) must not meet the -inf of a hidden key
 #pragma unroll
-            for (int c = 0; c < 64; c++) {
-                float y = __uint_as_float(x[c]) * (f0 * kf[c / 16]);
-                if (a.softcap > 0.0f) y = a.softcap * tanhf(y / a.softcap) * PT_LOG2E;
-                x[c] = __float_as_uint(y);
+            for (int g = 0; g < 4; g++) {
+                f[g] = f0 * sh.kf[k * (TI_KEYS / 16) + half * 4 + g];
+                f[g] = f[g] == 0.0f ? 1e-37f : f[g];
+            }
+            if (CAP) {
+#pragma unroll
+                for (int c = 0; c < 64; c++) x[c] = __float_as_uint(a.softcap * tanhf(__uint_as_float(x[c]) * f[c / 16] / a.softcap) * PT_LOG2E);
+#pragma unroll
+                for (int g = 0; g < 4; g++) f[g] = 1.0f;
             }
             if (lo + k * TI_KEYS + TI_KEYS - 1 > min(pos_first, k1 - 1) || (a.window > 0 && lo + k * TI_KEYS < pos_last - a.window + 1)) {
+                const int c_lo = key_lo - key0, c_hi = key_hi - key0;
 #pragma unroll
                 for (int c = 0; c < 64; c++)
-                    if (key0 + c > key_hi || key0 + c < key_lo) x[c] = 0xff800000u;
+                    if (c > c_hi || c < c_lo) x[c] = 0xff800000u;
             }
+            float mx = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < 64; c++) mx = fmaxf(mx, __uint_as_float(x[c]));
+            for (int g = 0; g < 4; g++) {
+                float y = __uint_as_float(x[g * 16]);
+#pragma unroll
+                for (int c = 1; c < 16; c++) y = fmaxf(y, __uint_as_float(x[g * 16 + c]));
+                mx = fmaxf(mx, y * f[g]);
+            }
             sh.top[slot][half][row] = mx;
             ti_soft_sync();                                           // .. and both halves have read S
             mx = fmaxf(mx, sh.top[slot][half ^ 1][row]);
+            // the step's value factors relative to a power of two
+            float vref = 1.0f, ivref = 1.0f;
+            const float* vfs = sh.vf + k * (TI_KEYS / 16);
             if (I8) {
+                float vmax = 0.0f;
 #pragma unroll
                 for (int g = 0; g < TI_KEYS / 16; g++) vmax = fmaxf(vmax, vfs[g]);
-            } else vmax = 1.0f;
-            // the step's value factors relative to a power of two
-            const float vref = fminf(fmaxf(__uint_as_float(__float_as_uint(vmax) & 0x7f800000u), 0x1p-100f), 0x1p100f), ivref = 1.0f / vref;
-            const float m_new = fmaxf(m, mx), base = m_new == -INFINITY ? 0.0f : m_new - PT_SHIFT;
+                vref = fminf(fmaxf(__uint_as_float(__float_as_uint(vmax) & 0x7f800000u), 0x1p-100f), 0x1p100f);
+                ivref = __uint_as_float(0x7f000000u - __float_as_uint(vref));                    // 1 / vref
+            }
+            const float m_new = fmaxf(m, mx), base = m_new == -INFINITY ? 0.0f : PT_SHIFT - m_new;
             const float alpha = m == m_new ? 1.0f : ti_exp2(m - m_new);
             m = m_new;
             float sum = 0.0f;
@@ -350,12 +372,9 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const PtArgs 
                     const float vr = I8 ? vfs[half * 4 + g] * ivref : 1.0f;
 #pragma unroll
                     for (int c = 0; c < 16; c += 2) {
-                        float p0 = ti_exp2(__uint_as_float(x[g * 16 + c]) - base), p1 = ti_exp2(__uint_as_float(x[g * 16 + c + 1]) - base);
+                        float p0 = ti_exp2(fmaf(__uint_as_float(x[g * 16 + c]), f[g], base)), p1 = ti_exp2(fmaf(__uint_as_float(x[g * 16 + c + 1]), f[g], base));
                         sum += p0 + p1;
-                        if (I8) {                                     // a weight of zero stays one beside a factor that is NaN
-                            p0 = p0 == 0.0f ? 0.0f : p0 * vr;
-                            p1 = p1 == 0.0f ? 0.0f : p1 * vr;
-                        }
+                        if (I8) { p0 *= vr; p1 *= vr; }
                         pt_cut(p0, p1, h[c / 2], w[c / 2]);
                     }
                     ti_store8(tmem + slot * 128 + lanes + half * 32 + g * 8, h);
@@ -370,6 +389,11 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const PtArgs 
             alpha_prev = alpha; vref_prev = vref;
         }
         if (steps > 0) add(steps - 1);
+        if (lost0 | lost1) {
+#pragma unroll
+            for (int c = 0; c < TI_D / 2; c++)
+                if ((c < 32 ? lost0 : lost1) >> (c & 31) & 1u) acc[c] = NAN;
+        }
         sh.sum[half][row] = l;
         ti_soft_sync();
         l = sh.sum[0][row] + sh.sum[1][row];
