@@ -6,18 +6,22 @@
 //   O = P_h V + P_l V         in an accumulator of its own, added to 32-bit registers afterwards: the tensor core cuts its sums off at 24 bits, a chain over
 //                             thousands of keys would drift (1e-5 of a result after 2000 keys of one sign)
 // S and O have two buffers each (512 TMEM columns), K and V two stages of f16 (128 KB beside the 64 KB of Q): while warps 0-7 make the weights of one step, the
-// tensor core computes the scores of the next and the sums of the one before, and warps 8-10 read, convert and store the keys and values behind.
+// tensor core computes the scores of the next and the sums of the one before, and warps 8-14 read, convert and store the keys and values behind.
 // A row's 128 scores lie with two threads, lane and half; they exchange their largest score once a step.
-// Warps 0-7 weights and sums, 8-10 keys and values, 11 issues the products.  Every wait is bounded (sg_wait); where one ran out all roles run to their ends without
+// Warps 0-7 weights and sums, 8-14 keys and values, 15 issues the products.  Every wait is bounded (sg_wait); where one ran out all roles run to their ends without
 // waiting (the barrier of warps 0-7 included) and the host reports it.
 #pragma once
 #include "split_gemm.cuh"
 
 #define TI_ROWS 128
 #define TI_KEYS 128
-#define TI_THREADS 384                        // three warps a scheduler: 168 registers a thread (a thirteenth warp would leave 128)
+#define TI_THREADS 512                        // 8 warps of weights and sums, 7 of keys and values, one that issues
 #define TI_SOFT 256
-#define TI_LOADERS 3
+#define TI_LOADERS 7
+// 512 threads of 128 registers at launch are 256 of 168 and 256 of 88 afterwards (65536 either way)
+#define TI_REGS_SOFT 168
+#define TI_REGS_REST 88
+static_assert(TI_SOFT * TI_REGS_SOFT + (TI_THREADS - TI_SOFT) * TI_REGS_REST <= TI_THREADS * 128, "more registers than the block was launched with");
 #define TI_MOST 4096                          // keys of a slice
 #define TI_D 128                              // largest dk and dv
 
@@ -50,6 +54,38 @@ __device__ __forceinline__ float ti_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// pairs of 32-bit numbers in one instruction
+typedef unsigned long long ti_f2;
+__device__ __forceinline__ ti_f2 ti_two(float x, float y) {
+    ti_f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 ti_one(ti_f2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ ti_f2 ti_fma2(ti_f2 a, ti_f2 b, ti_f2 c) {
+    ti_f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ ti_f2 ti_mul2(ti_f2 a, ti_f2 b) {
+    ti_f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ ti_f2 ti_add2(ti_f2 a, ti_f2 b) {
+    ti_f2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float ti_max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 __device__ __forceinline__ void ti_soft_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
@@ -97,7 +133,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const PtArgs 
         sh.page[i] = page; sh.kf[i] = bad ? 0.0f : kf; sh.vf[i] = bad ? 0.0f : vf; sh.nan[i] = bad;
         if (bad) sh.lost = 1;
     }
-    if (warp == 11) {
+    if (warp == 15) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pg_smem(&sh.tmem_base)), "n"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -140,7 +176,9 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const PtArgs 
     pg_fence_after();
     const unsigned tmem = sh.tmem_base;
 
-    if (warp == 11) {
+    if (warp >= TI_SOFT / 32) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TI_REGS_REST));
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TI_REGS_SOFT));
+    if (warp == 15) {
         // ===== products: one thread =====
         if (lane == 0) {
             const unsigned idesc_s = pg_instr_desc(128, TI_KEYS), idesc_o = pg_instr_desc(128, a.dv) | 1u << 16;
@@ -178,11 +216,21 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const PtArgs 
         }
         __syncwarp();
     } else if (warp >= 8) {
-        // ===== keys and values: a warp takes 16 rows of an operand at a time (a group: they lie in one page), the next two groups' are under way =====
-        constexpr int N = I8 ? 4 : 8, E = I8 ? 16 : 8, AHEAD = 2;      // pieces of 16 bytes of a lane and group, numbers of a piece
+        // ===== keys and values: a warp takes 16 rows of an operand at a time (a group: they lie in one page), its next groups' are under way =====
+        constexpr int N = I8 ? 4 : 8, E = I8 ? 16 : 8, AHEAD = I8 ? 2 : 1;      // pieces of 16 bytes of a lane and group, numbers of a piece
         const int groups = steps * (TI_KEYS / 8);                      // of keys and values by turns of a step
         const int per_k = a.dk / E, per_v = a.dv / E;
         int4 raw[AHEAD + 1][N];
+        // where the lane's pieces lie in a group's 16 rows; 8-bit: the chunk that is stored first, bit 0 set where that is the piece's second one
+        unsigned off_k[N], off_v[N];
+#pragma unroll
+        for (int i = 0; i < N; i++)
+#pragma unroll
+            for (int v = 0; v < 2; v++) {
+                const int per = v ? per_v : per_k, e = i * 32 + lane, row = e / per, piece = e - row * per, second = piece >> 2 & 1;
+                const unsigned off = row >= 16 ? ~0u : I8 ? ti_at(row, 2 * piece + second) | second : ti_at(row, piece);
+                (v ? off_v : off_k)[i] = off;
+            }
         auto where = [&](int u, int& step, bool& val, int& g) { step = u / (TI_KEYS / 8); val = u & (TI_KEYS / 16); g = u & (TI_KEYS / 16 - 1); };
         auto fetch = [&](int u, int4 (&r)[N]) {
             int step, g;
@@ -201,9 +249,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const PtArgs 
             bool val, wild = false;
             where(u, step, val, g);
             uint8_t* base = (val ? vs : ks) + (size_t)(step & 1) * TI_OPERAND + g * 2048;
-            const int per = val ? per_v : per_k, page = sh.page[step * (TI_KEYS / 16) + g], key = lo + step * TI_KEYS + g * 16, d = val ? a.dv : a.dk;
-            int row = lane / per, piece = lane - row * per;
-            const int row_by = 32 / per, piece_by = 32 - row_by * per;
+            const int page = sh.page[step * (TI_KEYS / 16) + g], key = lo + step * TI_KEYS + g * 16, d = val ? a.dv : a.dk;
             auto clean = [&](uint4& x) {
                 const unsigned w0 = pt_wild(x.x), w1 = pt_wild(x.y), w2 = pt_wild(x.z), w3 = pt_wild(x.w);
                 wild |= (w0 | w1 | w2 | w3) != 0u;
@@ -222,24 +268,21 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const PtArgs 
             } else {
 #pragma unroll
                 for (int i = 0; i < N; i++) {
-                    if (row < 16) {
-                        if (I8) {
-                            const unsigned u0 = (unsigned)r[i].x ^ 0x80808080u, u1 = (unsigned)r[i].y ^ 0x80808080u, u2 = (unsigned)r[i].z ^ 0x80808080u, u3 = (unsigned)r[i].w ^ 0x80808080u;
-                            const uint4 x = make_uint4(pt_half2(u0, 0x4140), pt_half2(u0, 0x4342), pt_half2(u1, 0x4140), pt_half2(u1, 0x4342));
-                            const uint4 y = make_uint4(pt_half2(u2, 0x4140), pt_half2(u2, 0x4342), pt_half2(u3, 0x4140), pt_half2(u3, 0x4342));
-                            const bool odd = piece & 4;                // the lanes of a row fill all banks at once
-                            uint8_t* q = base + ti_at(row, 2 * piece);
-                            const int other = 16 - 32 * (row & 1);     // chunk 2 piece + 1 lies beside it under the swizzle
-                            *(uint4*)(odd ? q + other : q) = odd ? y : x;
-                            *(uint4*)(odd ? q : q + other) = odd ? x : y;
-                        } else {
-                            uint4 x = make_uint4((unsigned)r[i].x, (unsigned)r[i].y, (unsigned)r[i].z, (unsigned)r[i].w);
-                            if (val) clean(x);
-                            *(uint4*)(base + ti_at(row, piece)) = x;
-                        }
+                    const unsigned off = val ? off_v[i] : off_k[i];
+                    if (off == ~0u) continue;
+                    if (I8) {
+                        // the lanes of a row fill all banks at once: those of its second half store their second 8 numbers first (chunk 2 p + 1 is chunk 2 p with 16 flipped)
+                        const bool odd = off & 1u;
+                        const unsigned a0 = (unsigned)(odd ? r[i].z : r[i].x) ^ 0x80808080u, a1 = (unsigned)(odd ? r[i].w : r[i].y) ^ 0x80808080u;
+                        const unsigned b0 = (unsigned)(odd ? r[i].x : r[i].z) ^ 0x80808080u, b1 = (unsigned)(odd ? r[i].y : r[i].w) ^ 0x80808080u;
+                        const unsigned at = off & ~1u;
+                        *(uint4*)(base + at) = make_uint4(pt_half2(a0, 0x4140), pt_half2(a0, 0x4342), pt_half2(a1, 0x4140), pt_half2(a1, 0x4342));
+                        *(uint4*)(base + (at ^ 16u)) = make_uint4(pt_half2(b0, 0x4140), pt_half2(b0, 0x4342), pt_half2(b1, 0x4140), pt_half2(b1, 0x4342));
+                    } else {
+                        uint4 x = make_uint4((unsigned)r[i].x, (unsigned)r[i].y, (unsigned)r[i].z, (unsigned)r[i].w);
+                        if (val) clean(x);
+                        *(uint4*)(base + off) = x;
                     }
-                    row += row_by; piece += piece_by;
-                    if (piece >= per) { piece -= per; row++; }
                 }
             }
             if (wild) atomicExch(&sh.wild[step & 3], step + 1);
@@ -269,15 +312,17 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const PtArgs 
         const int c_first = half ? ((a.dv / 2 + 15) & ~15) : 0, cols = half ? a.dv - c_first : (a.dv / 2 + 15) & ~15;      // this thread's columns of O
         const int pos = in ? s.pos0 + tok : -1, key_lo = a.window > 0 ? pos - a.window + 1 : 0, key_hi = min(pos, k1 - 1);      // the last step may reach into the next slice
         const float f0 = inv * fabsf(a.scale) * (CAP ? 1.0f : PT_LOG2E);
-        float acc[TI_D / 2], m = -INFINITY, l = 0.0f, alpha_prev = 0.0f, vref_prev = 0.0f;
+        ti_f2 acc[TI_D / 4];
+        float m = -INFINITY, l = 0.0f, alpha_prev = 0.0f, vref_prev = 0.0f;
         unsigned lost0 = 0u, lost1 = 0u;                              // columns of this thread that have met a value that is not finite
 #pragma unroll
-        for (int i = 0; i < TI_D / 2; i++) acc[i] = 0.0f;
+        for (int i = 0; i < TI_D / 4; i++) acc[i] = 0ull;
         bool ok = true;
         auto add = [&](int k) {                                       // the sums of step k
             const unsigned slot = k & 1;
             if (!(ok = ok && sg_wait_warp(pg_smem(&sh.o_full[slot]), (k >> 1) & 1u, &sh.fail))) return;
             pg_fence_after();
+            const ti_f2 alpha2 = ti_two(alpha_prev, alpha_prev), vref2 = ti_two(vref_prev, vref_prev);
 #pragma unroll
             for (int c = 0; c < TI_D / 2; c += 16) {
                 if (c >= cols) break;
@@ -285,9 +330,11 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const PtArgs 
                 sg_tmem16(tmem + 256 + slot * 128 + lanes + c_first + c, v);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    asm volatile("" : "+r"(v[i]));
-                    acc[c + i] = I8 ? fmaf(__uint_as_float(v[i]), vref_prev, acc[c + i] * alpha_prev) : fmaf(acc[c + i], alpha_prev, __uint_as_float(v[i]));
+                for (int i = 0; i < 16; i += 2) {
+                    asm volatile("" : "+r"(v[i]), "+r"(v[i + 1]));
+                    const ti_f2 o = ti_two(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                    ti_f2& to = acc[(c + i) / 2];
+                    to = I8 ? ti_fma2(o, vref2, ti_mul2(to, alpha2)) : ti_fma2(to, alpha2, o);
                 }
             }
             pg_fence_before();
@@ -343,9 +390,9 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const PtArgs 
             float mx = -INFINITY;
 #pragma unroll
             for (int g = 0; g < 4; g++) {
-                float y = __uint_as_float(x[g * 16]);
+                float y = fmaxf(__uint_as_float(x[g * 16]), __uint_as_float(x[g * 16 + 1]));
 #pragma unroll
-                for (int c = 1; c < 16; c++) y = fmaxf(y, __uint_as_float(x[g * 16 + c]));
+                for (int c = 2; c < 16; c += 2) y = ti_max3(y, __uint_as_float(x[g * 16 + c]), __uint_as_float(x[g * 16 + c + 1]));
                 mx = fmaxf(mx, y * f[g]);
             }
             sh.top[slot][half][row] = mx;
@@ -364,18 +411,25 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const PtArgs 
             const float m_new = fmaxf(m, mx), base = m_new == -INFINITY ? 0.0f : PT_SHIFT - m_new;
             const float alpha = m == m_new ? 1.0f : ti_exp2(m - m_new);
             m = m_new;
-            float sum = 0.0f;
+            ti_f2 sum = 0ull;
             if (ok) {
+                const ti_f2 base2 = ti_two(base, base);
 #pragma unroll
                 for (int g = 0; g < 4; g++) {                         // 16 keys at a time: 8 words of h, 8 of l
                     unsigned h[8], w[8];
                     const float vr = I8 ? vfs[half * 4 + g] * ivref : 1.0f;
+                    const ti_f2 f2 = ti_two(f[g], f[g]), vr2 = ti_two(vr, vr), minus = ti_two(-1.0f, -1.0f);
 #pragma unroll
                     for (int c = 0; c < 16; c += 2) {
-                        float p0 = ti_exp2(fmaf(__uint_as_float(x[g * 16 + c]), f[g], base)), p1 = ti_exp2(fmaf(__uint_as_float(x[g * 16 + c + 1]), f[g], base));
-                        sum += p0 + p1;
-                        if (I8) { p0 *= vr; p1 *= vr; }
-                        pt_cut(p0, p1, h[c / 2], w[c / 2]);
+                        const float2 y = ti_one(ti_fma2(ti_two(__uint_as_float(x[g * 16 + c]), __uint_as_float(x[g * 16 + c + 1])), f2, base2));
+                        ti_f2 p = ti_two(ti_exp2(y.x), ti_exp2(y.y));
+                        sum = ti_add2(sum, p);
+                        if (I8) p = ti_mul2(p, vr2);
+                        const float2 q = ti_one(p);
+                        const __half2 a2 = __floats2half2_rn(q.x, q.y);
+                        const float2 b2 = __half22float2(a2), rest2 = ti_one(ti_fma2(ti_two(b2.x, b2.y), minus, p));
+                        h[c / 2] = *(const unsigned*)&a2;
+                        w[c / 2] = pt_pack(rest2.x, rest2.y);
                     }
                     ti_store8(tmem + slot * 128 + lanes + half * 32 + g * 8, h);
                     ti_store8(tmem + slot * 128 + lanes + 64 + half * 32 + g * 8, w);
@@ -384,15 +438,18 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const PtArgs 
                 pg_fence_before();
                 sg_arrive(pg_smem(&sh.p_full[slot]));
             }
-            l = fmaf(l, alpha, sum);
+            const float2 sums = ti_one(sum);
+            l = fmaf(l, alpha, sums.x + sums.y);
             if (k > 0) add(k - 1);
             alpha_prev = alpha; vref_prev = vref;
         }
         if (steps > 0) add(steps - 1);
-        if (lost0 | lost1) {
+        float o4[TI_D / 2];
 #pragma unroll
-            for (int c = 0; c < TI_D / 2; c++)
-                if ((c < 32 ? lost0 : lost1) >> (c & 31) & 1u) acc[c] = NAN;
+        for (int c = 0; c < TI_D / 2; c += 2) {
+            const float2 u = ti_one(acc[c / 2]);
+            o4[c] = (c < 32 ? lost0 : lost1) >> (c & 31) & 1u ? NAN : u.x;
+            o4[c + 1] = (c < 32 ? lost0 : lost1) >> ((c + 1) & 31) & 1u ? NAN : u.y;
         }
         sh.sum[half][row] = l;
         ti_soft_sync();
@@ -403,7 +460,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const PtArgs 
                 float* o = a.part + at * a.dv + c_first;
 #pragma unroll
                 for (int c = 0; c < TI_D / 2; c += 4)
-                    if (c < cols) *(float4*)(o + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+                    if (c < cols) *(float4*)(o + c) = make_float4(o4[c], o4[c + 1], o4[c + 2], o4[c + 3]);
                 if (half == 0) a.ml[at] = make_float2(m, l);
             } else {
                 float f = 1.0f;
@@ -416,13 +473,13 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const PtArgs 
                 f = f / l;
 #pragma unroll
                 for (int c = 0; c < TI_D / 2; c += 4)
-                    if (c < cols) *(float4*)(o + c) = make_float4(acc[c] * f, acc[c + 1] * f, acc[c + 2] * f, acc[c + 3] * f);
+                    if (c < cols) *(float4*)(o + c) = make_float4(o4[c] * f, o4[c + 1] * f, o4[c + 2] * f, o4[c + 3] * f);
             }
         }
     }
     pg_fence_before();
     __syncthreads();
-    if (warp == 11) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
+    if (warp == 15) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
     if (tid == 0 && sh.fail) {
         if (err_dev) atomicExch(err_dev, 5u);
         if (err_host) { *(volatile unsigned*)err_host = 5u; __threadfence_system(); }
