@@ -41,7 +41,7 @@ static int pg_plan(cc_device* dev, const cc_page_plan_desc* d, cc_page_plan* p) 
     const std::string wrong = pg_build(*d, parts);
     CC_REQUIRE(dev, wrong.empty(), "page_plan: %s", wrong.c_str());
     p->dev = dev; p->n_seqs = d->n_seqs; p->page = d->page_size; p->table_cols = d->table_cols; p->n_pages = d->n_pages; p->n_slots = d->n_slots;
-    p->n_items = parts.n_items; p->tokens = parts.tokens;
+    p->n_items = parts.n_items; p->n_segments = (int)parts.segments.size(); p->tokens = parts.tokens;
     while ((1 << p->shift) < p->page) p->shift++;
     const size_t seg = parts.segments.size() * sizeof(PgSegment), sq = parts.seqs.size() * sizeof(PgSeq), tab = parts.table.size() * sizeof(int);
     std::vector<uint8_t> bytes(seg + sq + tab + 16);
@@ -125,15 +125,18 @@ int pg_check_cache(cc_device* dev, const cc_page_plan* plan, const cc_paged_cach
 
 // ---- append --------------------------------------------------------------------------------------------------------------------------------
 #define PA_THREADS 256
+#define PA_WARPS (PA_THREADS / 32)
+#define PA_ROWS 4                            // rows of angles that a CTA makes for itself at a time
 struct PaArgs {
     const PgSegment* segments;
     const float *q, *k, *v, *freq;
+    double2* angles;                         // [T][pairs] cos and sin times mag, or NULL: every CTA makes its own
     float* qo;
     uint8_t *kp, *vp;
     float *ks, *vs;
     __half *ko, *vo;
     int64_t qrs, krs, vrs;                   // row strides
-    int H, G, dk, dv, page, pairs, offset, step, gap, hq, q_jobs;        // pair i: columns offset + step * i and + gap behind it; hq: query heads of a job
+    int H, G, dk, dv, page, pairs, offset, step, gap, hq, q_parts, vec;      // pair i: columns offset + step * i and + gap behind it; hq: query heads of a job, which takes PA_Q_ROWS rows where q_parts > 1; vec: neighbours that can be read as one
     double mag;
 };
 // F16 of a 32-bit number; what is finite stays finite
@@ -142,99 +145,169 @@ __device__ __forceinline__ __half pa_half(float x) {
     if (__hisinf(h) && !isinf(x)) h = __ushort_as_half((unsigned short)(x > 0.0f ? 0x7bff : 0xfbff));
     return h;
 }
-// cos and sin of the pairs of rows pos0 .. in 64 bits
-__device__ __forceinline__ void pa_angles(double2* cs, const PaArgs& a, int pos0, int rows) {
-    for (int e = threadIdx.x; e < rows * a.pairs; e += PA_THREADS) {
-        const int r = e / a.pairs, i = e - r * a.pairs;
-        double s, c;
-        sincos((double)(pos0 + r) * (double)a.freq[i], &s, &c);
-        cs[e] = make_double2(c * a.mag, s * a.mag);
+__device__ __forceinline__ double2 pa_angle(const PaArgs& a, int pos, int i) {
+    double s, c;
+    sincos((double)pos * (double)a.freq[i], &s, &c);
+    return make_double2(c * a.mag, s * a.mag);
+}
+// the angles of all tokens, once for all heads: a thread a pair of a token, CTAs of a segment
+__global__ void __launch_bounds__(PA_THREADS) paged_angles_kernel(const PaArgs a, int n_segments) {
+    pdl_enter();
+    for (int at = blockIdx.x; at < n_segments; at += gridDim.x) {
+        const PgSegment g = a.segments[at];
+        for (int e = blockIdx.y * PA_THREADS + threadIdx.x; e < g.rows * a.pairs; e += gridDim.y * PA_THREADS) {
+            const int r = e / a.pairs, i = e - r * a.pairs;
+            a.angles[(int64_t)(g.token0 + r) * a.pairs + i] = pa_angle(a, g.pos0 + r, i);
+        }
     }
 }
-#define PA_ROWS 16                           // rows of angles that are made at a time
-// every column of a head's row through `put` (column, number), turned where it belongs to a pair.  unit e: pair e, or one of the columns that stay
+// Units of a head's row: pairs, which are turned, and behind them the columns that stay.  Where unit u lies, and its numbers through `put` (column, number)
+__device__ __forceinline__ int pa_column(const PaArgs& a, int u) {
+    if (u < a.pairs) return a.offset + a.step * u;
+    const int c = u - a.pairs;
+    return c >= a.offset ? c + 2 * a.pairs : c;
+}
+__device__ __forceinline__ float2 pa_read(const PaArgs& a, const float* row, int u, int c) {
+    if (u >= a.pairs) return make_float2(__ldg(row + c), 0.0f);
+    if (a.vec) return __ldg((const float2*)(row + c));
+    return make_float2(__ldg(row + c), __ldg(row + c + a.gap));
+}
 template <class Put>
-__device__ __forceinline__ void pa_unit(const PaArgs& a, const float* row, int e, const double2* cs, Put put) {
-    if (e < a.pairs) {
-        const int c = a.offset + a.step * e;
-        const double x = (double)row[c], y = (double)row[c + a.gap];
-        put(c, (float)fma(x, cs[e].x, -(y * cs[e].y)));
-        put(c + a.gap, (float)fma(x, cs[e].y, y * cs[e].x));
-    } else {
-        int c = e - a.pairs;
-        if (c >= a.offset) c += 2 * a.pairs;
-        put(c, row[c]);
-    }
+__device__ __forceinline__ void pa_write(const PaArgs& a, float2 v, int u, int c, const double2& t, Put put) {
+    if (u >= a.pairs) { put(c, v.x); return; }
+    const double x = (double)v.x, y = (double)v.y;
+    put(c, (float)fma(x, t.x, -(y * t.y)));
+    put(c + a.gap, (float)fma(x, t.y, y * t.x));
 }
-// grid (items, jobs): jobs 0 .. G - 1 key heads, then G value heads, then query heads by hq
-template <bool I8>
-__global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const PaArgs a) {
+#define PA_Q_ROWS 16
+#define PA_AHEAD 4                           // rows of a head, or heads of a row, that a warp reads before it turns the first
+// grid (segments, jobs): jobs 0 .. G - 1 key heads, then G value heads (of the first n_items segments, and those behind them in their chains), then query heads by hq (and their rows by PA_Q_ROWS).
+// A warp takes 32 units of a head, in rows so many further on as warps share them
+template <bool I8, bool TABLE>
+__global__ void __launch_bounds__(PA_THREADS, 4) paged_append_kernel(const PaArgs a, int n_items) {
     extern __shared__ __align__(16) uint8_t pa_sm[];
-    double2* cs = (double2*)pa_sm;                              // [PA_ROWS][pairs]
-    __half* block = (__half*)(pa_sm + (size_t)PA_ROWS * a.pairs * sizeof(double2));      // [page][d]
-    __shared__ unsigned top;
-    const int job = blockIdx.y, tid = threadIdx.x;
-    const bool is_k = job < a.G, is_v = !is_k && job < 2 * a.G;
+    double2* made = (double2*)pa_sm;                            // [PA_ROWS][pairs], where the angles are not there already
+    __half* block = (__half*)(pa_sm + (TABLE ? 0 : (size_t)PA_ROWS * a.pairs * sizeof(double2)));      // [page][d]
+    __shared__ unsigned tops[PA_WARPS];
+    const int job = blockIdx.y, tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+    const bool is_k = job < a.G, is_v = !is_k && job < 2 * a.G, is_q = !is_k && !is_v;
+    if (!is_q && blockIdx.x >= n_items) return;
     pdl_enter();
     for (int at = blockIdx.x; at >= 0;) {
         const PgSegment g = a.segments[at];
-        at = g.next;
-        if (!is_k && !is_v) {                                   // query heads
-            const int h0 = (job - 2 * a.G) * a.hq, nh = min(a.hq, a.H - h0), units = a.dk - a.pairs;
-            for (int r0 = 0; r0 < g.rows; r0 += PA_ROWS) {
-                const int n = min(PA_ROWS, g.rows - r0);
-                pa_angles(cs, a, g.pos0 + r0, n);
+        at = is_q ? -1 : g.next;
+        const int part = is_q ? (job - 2 * a.G) % a.q_parts : 0, row_from = part * PA_Q_ROWS, row_to = is_q && a.q_parts > 1 ? min(g.rows, row_from + PA_Q_ROWS) : g.rows;
+        // f(row r0, so many rows, their angles): all rows of the job, or portions whose angles the CTA makes first
+        auto portions = [&](bool turned, auto f) {
+            if (TABLE || !turned || a.pairs == 0) { f(row_from, row_to - row_from, a.angles + (int64_t)(g.token0 + row_from) * a.pairs); return; }
+            for (int r0 = 0; r0 < g.rows && !TABLE; r0 += PA_ROWS) {
+                const int rows = min(PA_ROWS, g.rows - r0);
                 __syncthreads();
-                for (int e = tid; e < n * nh * units; e += PA_THREADS) {
-                    const int rh = e / units, u = e - rh * units, r = rh / nh, h = h0 + rh - r * nh;
-                    const int64_t t = g.token0 + r0 + r;
-                    float* dst = a.qo + (t * a.H + h) * a.dk;
-                    pa_unit(a, a.q + t * a.qrs + (int64_t)h * a.dk, u, cs + r * a.pairs, [&](int c, float x) { dst[c] = x; });
-                }
+                for (int e = tid; e < rows * a.pairs; e += PA_THREADS) { const int r = e / a.pairs; made[e] = pa_angle(a, g.pos0 + r0 + r, e - r * a.pairs); }
                 __syncthreads();
+                f(r0, rows, made);
             }
+        };
+        // the CTA's warps over `kinds` kinds of work and rows: f(kind, first row, rows from one to the next)
+        auto share = [&](int kinds, auto f) {
+            const int at_once = min(kinds, PA_WARPS), by = PA_WARPS / at_once, first = w / at_once;
+            if (first < by)
+                for (int k = w - first * at_once; k < kinds; k += at_once) f(k, first, by);
+        };
+        if (is_q) {
+            const int h0 = (job - 2 * a.G) / a.q_parts * a.hq, nh = min(a.hq, a.H - h0), units = a.dk - a.pairs, runs = (units + 31) >> 5, batches = (nh + PA_AHEAD - 1) / PA_AHEAD;
+            portions(true, [&](int r0, int rows, const double2* cs) {
+                share(runs * batches, [&](int kind, int first, int by) {
+                    const int b = kind / runs, u = (kind - b * runs) * 32 + lane, n = min(PA_AHEAD, nh - b * PA_AHEAD), c = pa_column(a, u);
+                    if (u >= units) return;
+                    for (int r = first; r < rows; r += by) {
+                        const int64_t t = g.token0 + r0 + r;
+                        const float* src = a.q + t * a.qrs + (int64_t)(h0 + b * PA_AHEAD) * a.dk;
+                        float* dst = a.qo + (t * a.H + h0 + b * PA_AHEAD) * a.dk;
+                        float2 v[PA_AHEAD];
+                        double2 z = make_double2(0.0, 0.0);
+#pragma unroll
+                        for (int i = 0; i < PA_AHEAD; i++)
+                            if (i < n) v[i] = pa_read(a, src + i * a.dk, u, c);
+                        if (u < a.pairs) z = cs[r * a.pairs + u];
+#pragma unroll
+                        for (int i = 0; i < PA_AHEAD; i++)
+                            if (i < n) pa_write(a, v[i], u, c, z, [&](int col, float x) { dst[i * a.dk + col] = x; });
+                    }
+                });
+            });
             continue;
         }
-        const int head = is_k ? job : job - a.G, d = is_k ? a.dk : a.dv, units = is_k ? a.dk - a.pairs : a.dv;
-        const float* src = is_k ? a.k : a.v;
-        const int64_t rs = is_k ? a.krs : a.vrs;
+        const int head = is_k ? job : job - a.G, d = is_k ? a.dk : a.dv;
         const size_t page_at = ((size_t)g.page * a.G + head) * a.page * d;
-        const size_t open_at = ((size_t)g.half * a.G + head) * a.page * d;
-        __half* open = I8 ? (is_k ? a.ko : a.vo) + open_at : nullptr;
-        __half* rows = I8 ? block : (__half*)(is_k ? a.kp : a.vp) + page_at;      // 16-bit pages: straight to their place
+        __half* open = I8 ? (is_k ? a.ko : a.vo) + ((size_t)g.half * a.G + head) * a.page * d : nullptr;
+        __half* to = (I8 ? block : (__half*)(is_k ? a.kp : a.vp) + page_at) + g.row0 * d;      // 16-bit pages: straight to their place
         if (I8 && (g.flags & PG_FULL))                          // the block's older rows
-            for (int e = tid; e < g.row0 * d; e += PA_THREADS) block[e] = open[e];
-        if (tid == 0) top = 0;
-        for (int r0 = 0; r0 < g.rows; r0 += PA_ROWS) {
-            const int n = min(PA_ROWS, g.rows - r0);
-            if (is_k) pa_angles(cs, a, g.pos0 + r0, n);
-            __syncthreads();
-            for (int e = tid; e < n * units; e += PA_THREADS) {
-                const int r = e / units, u = e - r * units;
-                const float* row = src + (int64_t)(g.token0 + r0 + r) * rs + (int64_t)head * d;
-                __half* dst = rows + (size_t)(g.row0 + r0 + r) * d;
-                if (is_k) pa_unit(a, row, u, cs + r * a.pairs, [&](int c, float x) { dst[c] = pa_half(x); });
-                else dst[u] = pa_half(row[u]);
-            }
-            __syncthreads();
-        }
+            for (int e = tid; e < g.row0 * d / 8; e += PA_THREADS) ((uint4*)block)[e] = ((const uint4*)open)[e];
+        const float* src = (is_k ? a.k : a.v) + (int64_t)head * d;
+        const int64_t rs = is_k ? a.krs : a.vrs;
+        const int units = is_k ? d - a.pairs : d;
+        portions(is_k, [&](int r0, int rows, const double2* cs) {
+            share((units + 31) >> 5, [&](int kind, int first, int by) {
+                constexpr int AHEAD = TABLE ? PA_AHEAD : 1;
+                const int u = kind * 32 + lane, c = is_k ? pa_column(a, u) : u;
+                if (u >= units) return;
+                for (int r = first; r < rows; r += by * AHEAD) {
+                    float2 v[AHEAD];
+                    double2 z[AHEAD];
+#pragma unroll
+                    for (int i = 0; i < AHEAD; i++) {
+                        const int x = r + i * by;
+                        if (x >= rows) continue;
+                        const float* row = src + (g.token0 + r0 + x) * rs;
+                        if (is_k) {
+                            v[i] = pa_read(a, row, u, c);
+                            if (u < a.pairs) z[i] = cs[x * a.pairs + u];
+                        } else v[i].x = __ldg(row + c);
+                    }
+#pragma unroll
+                    for (int i = 0; i < AHEAD; i++) {
+                        const int x = r + i * by;
+                        if (x >= rows) continue;
+                        __half* dst = to + (r0 + x) * d;
+                        if (is_k) pa_write(a, v[i], u, c, z[i], [&](int col, float y) { dst[col] = pa_half(y); });
+                        else dst[c] = pa_half(v[i].x);
+                    }
+                }
+            });
+        });
         if (!I8) continue;
+        __syncthreads();
         if (g.flags & PG_KEPT)
-            for (int e = tid; e < g.rows * d; e += PA_THREADS) open[g.row0 * d + e] = block[g.row0 * d + e];
+            for (int e = tid; e < g.rows * d / 8; e += PA_THREADS) ((uint4*)(open + g.row0 * d))[e] = ((const uint4*)(block + g.row0 * d))[e];
         if (g.flags & PG_FULL) {
             unsigned m = 0;
-            for (int e = tid; e < a.page * d; e += PA_THREADS) m = max(m, (unsigned)__half_as_ushort(block[e]) & 0x7fffu);
-            m = __reduce_max_sync(0xffffffffu, m);
-            if ((tid & 31) == 0) atomicMax(&top, m);
+            for (int e = tid; e < a.page * d / 2; e += PA_THREADS) m = __vmaxu2(m, ((const unsigned*)block)[e] & 0x7fff7fffu);
+            m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
+            if (lane == 0) tops[w] = m;
             __syncthreads();
+            unsigned top = 0;
+#pragma unroll
+            for (int i = 0; i < PA_WARPS; i++) top = max(top, tops[i]);
             const bool finite = top < 0x7c00u;
             const float most = __half2float(__ushort_as_half((unsigned short)top));
             // numbers and their largest have 11 bits: 127 x is exact, and a quotient that is not a tie is further from one than a 32-bit division errs
-            int8_t* codes = (int8_t*)(is_k ? a.kp : a.vp) + page_at;
-            for (int e = tid; e < a.page * d; e += PA_THREADS) codes[e] = finite && top ? (int8_t)rintf(__half2float(block[e]) * 127.0f / most) : (int8_t)0;
+            uint2* codes = (uint2*)((is_k ? a.kp : a.vp) + page_at);
+            for (int e = tid; e < a.page * d / 8; e += PA_THREADS) {
+                const uint4 x = ((const uint4*)block)[e];
+                const unsigned in[4] = {x.x, x.y, x.z, x.w};
+                unsigned c[8];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float2 y = __half22float2(*(const __half2*)&in[i]);
+                    c[2 * i] = finite && top ? (unsigned)(int)rintf(y.x * 127.0f / most) & 255u : 0u;
+                    c[2 * i + 1] = finite && top ? (unsigned)(int)rintf(y.y * 127.0f / most) & 255u : 0u;
+                }
+                codes[e] = make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
+            }
             if (tid == 0) (is_k ? a.ks : a.vs)[(size_t)g.page * a.G + head] = finite ? most / 127.0f : NAN;
         }
-        __syncthreads();                                        // the block and `top`, before the next segment
+        __syncthreads();                                        // the block and `tops`, before the next segment
     }
 }
 extern "C" CC_API int cc_paged_append(cc_device* dev, const cc_page_plan* plan, const cc_paged_cache* cache, const cc_view* q_src, int32_t q_col0, const cc_view* k_src,
@@ -277,15 +350,31 @@ extern "C" CC_API int cc_paged_append(cc_device* dev, const cc_page_plan* plan, 
         a.kp = c.k; a.vp = c.v; a.ks = c.ks; a.vs = c.vs; a.ko = c.ko; a.vo = c.vo;
         a.H = q_src ? H : 0; a.G = c.G; a.dk = c.dk; a.dv = c.dv; a.page = plan->page; a.pairs = (int)pairs; a.offset = offset; a.mag = (double)mag;
         a.step = pairing == CC_ROPE_NEIGHBOURS ? 2 : 1; a.gap = pairing == CC_ROPE_NEIGHBOURS ? 1 : (int)pairs;
-        a.hq = 4; a.q_jobs = (a.H + a.hq - 1) / a.hq;
-        const size_t smem = (size_t)PA_ROWS * a.pairs * sizeof(double2) + (c.i8 ? (size_t)a.page * std::max(c.dk, c.dv) * 2 : 0);
-        const dim3 grid((unsigned)plan->n_items, (unsigned)(2 * c.G + a.q_jobs));
-        cudaError_t e;
-        if (c.i8) {
-            e = cudaFuncSetAttribute(paged_append_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-            if (e == cudaSuccess) e = cc_launch_pdl(dev, paged_append_kernel<true>, grid, PA_THREADS, smem, a);
-        } else e = cc_launch_pdl(dev, paged_append_kernel<false>, grid, PA_THREADS, smem, a);
+        a.vec = pairing == CC_ROPE_NEIGHBOURS && ((offset | c.dk | k_col0 | (int)(a.krs & 1)) & 1) == 0 && (!q_src || ((q_col0 | (int)(a.qrs & 1)) & 1) == 0) &&
+                (((uintptr_t)k_src->buf->plane[0] | (q_src ? (uintptr_t)q_src->buf->plane[0] : 0)) & 7) == 0;
+        // a portion of many rows a block: the angles once for all heads, in a kernel of their own (64 rows of 64 pairs made by each of 16 CTAs:
+        // three prompts of 1657 tokens, 32 heads on 8, 125 us, with the table 4 + 33); single tokens: by every CTA
+        const bool table = pairs > 0 && T > 4 * (int64_t)plan->n_segments;
+        a.hq = table ? 4 : 8; a.q_parts = table ? plan->page / PA_Q_ROWS : 1;
+        void* ws = nullptr; size_t cls = 0;
+        if (table) {
+            rc = cc_pool_alloc(dev, (size_t)T * pairs * sizeof(double2), &ws, &cls);
+            if (rc) { if (o) cc_tensor_release(o); return rc; }
+            a.angles = (double2*)ws;
+        }
+        const size_t smem = (table ? 0 : (size_t)PA_ROWS * a.pairs * sizeof(double2)) + (c.i8 ? (size_t)a.page * std::max(c.dk, c.dv) * 2 : 0);
+        const dim3 grid((unsigned)plan->n_segments, (unsigned)(2 * c.G + (a.H + a.hq - 1) / a.hq * a.q_parts));
+        cudaError_t e = cudaSuccess;
+        if (table) {
+            const int64_t per = ((int64_t)plan->page * pairs + PA_THREADS - 1) / PA_THREADS;
+            e = cc_launch_pdl(dev, paged_angles_kernel, dim3((unsigned)std::min(plan->n_segments, 65535), (unsigned)std::min<int64_t>(per, 16)), PA_THREADS, 0, a, plan->n_segments);
+            dev->launches++;
+        }
+        auto kernel = c.i8 ? (table ? paged_append_kernel<true, true> : paged_append_kernel<true, false>) : (table ? paged_append_kernel<false, true> : paged_append_kernel<false, false>);
+        if (e == cudaSuccess && smem > 40 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e == cudaSuccess) e = cc_launch_pdl(dev, kernel, grid, PA_THREADS, smem, a, plan->n_items);
         dev->launches++;
+        if (ws) cc_pool_free(dev, ws, cls);
         if (e != cudaSuccess) {
             if (o) cc_tensor_release(o);
             return cc_fail(dev, CC_ERR_CUDA, "paged_append: %s", cudaGetErrorString(e));

@@ -6,7 +6,7 @@
 
 struct cc_page_plan {
     cc_device* dev = nullptr;
-    int n_seqs = 0, page = 0, shift = 0, table_cols = 0, n_items = 0;
+    int n_seqs = 0, page = 0, shift = 0, table_cols = 0, n_items = 0, n_segments = 0;
     int64_t n_pages = 0, n_slots = 0, tokens = 0;
     std::vector<PgSeq> seqs;
     void* base = nullptr; size_t cls = 0;                // the device's copy

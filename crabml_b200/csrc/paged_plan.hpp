@@ -67,8 +67,7 @@ inline std::string pg_build(const cc_page_plan_desc& d, PgParts& out) {
         PgSeq s;
         s.first = (int)out.tokens; s.count = (int)n; s.pos0 = (int)pos0; s.slot = d.n_slots > 0 ? (int)slot : 0;
         out.seqs.push_back(s);
-        std::vector<PgSegment>* last = nullptr;          // where the chain of the sequence's first segment ends
-        size_t last_at = 0;
+        size_t first = 0;                                // the sequence's first segment
         for (int64_t b = pos0 / P; n > 0 && b <= (end - 1) / P; b++) {
             const int64_t lo = std::max(pos0, b * P), hi = std::min(end, (b + 1) * P);
             PgSegment g{};
@@ -79,15 +78,14 @@ inline std::string pg_build(const cc_page_plan_desc& d, PgParts& out) {
             g.next = -1;
             PG_NEED(owner[(size_t)g.page] == 0, "page %d takes tokens of two blocks", g.page);
             owner[(size_t)g.page] = 1 + i;
-            // a block that is kept may overwrite the open rows that the sequence's first block began with: the same CTA takes it behind that one
-            if (last && (g.flags & PG_KEPT)) {
-                (*last)[last_at].next = (int)rest.size();
+            if (b == pos0 / P) first = heads.size();
+            const PgSegment* f = b == pos0 / P ? nullptr : &heads[first];
+            // a block that is kept overwrites the open rows that the sequence's first block began with, where both lie in one half: the same CTA takes it behind that one (there is
+            // one such block at most: of the two that are kept every second lies there)
+            if (f && (g.flags & PG_KEPT) && (f->flags & PG_FULL) && f->row0 > 0 && f->half == g.half) {
+                heads[first].next = (int)rest.size();
                 rest.push_back(g);
-                last = &rest; last_at = rest.size() - 1;
-            } else {
-                heads.push_back(g);
-                if (!last) { last = &heads; last_at = heads.size() - 1; }
-            }
+            } else heads.push_back(g);
         }
         out.tokens += n;
     }
