@@ -20,6 +20,7 @@
 #define PT_FEW 32
 #define PT_LOG2E 1.4426950408889634f
 
+struct TiInfo;
 struct PtArgs {
     const PgSeq* seqs;
     const int* table;
@@ -30,20 +31,23 @@ struct PtArgs {
     float2* ml;                               // [item][head][tile_rows]: largest score (base 2) and sum of weights
     float scale, softcap;
     int n_seqs, table_cols, page, shift, H, G, R, dk, dv, window, split, rows_lo, rows_hi;
-    int tile_rows;                            // of an item: 8 (paged_few_kernel) or 128 (paged_tile_kernel)
+    int tile_rows, align;                     // of an item: 8 (paged_few_kernel) or 128 (paged_tile_kernel); what keys count from is a multiple of align
+    int head0, heads;                         // key heads of this launch
+    uint8_t *k_image, *v_image;               // paged_tile.cuh
+    struct TiInfo* info;
 };
 struct PtItem { int seq, split, tile, n_split; };
 
-// keys [from, to) that the sequence's new tokens see together, from at a multiple of 16
-__host__ __device__ __forceinline__ void pt_range(const PgSeq& s, int window, int* from, int* to) {
+// keys [from, to) that the sequence's new tokens see together
+__host__ __device__ __forceinline__ void pt_range(const PgSeq& s, const PtArgs& a, int* from, int* to) {
     *to = s.pos0 + s.count;
-    *from = window > 0 && s.pos0 - window + 1 > 0 ? (s.pos0 - window + 1) & ~15 : 0;
+    *from = a.window > 0 && s.pos0 - a.window + 1 > 0 ? (s.pos0 - a.window + 1) & ~(a.align - 1) : 0;
 }
 __host__ __device__ __forceinline__ int pt_splits(const PgSeq& s, const PtArgs& a) {
     const int64_t rows = (int64_t)s.count * a.R;
     if (rows < a.rows_lo || rows > a.rows_hi) return 0;
     int from, to;
-    pt_range(s, a.window, &from, &to);
+    pt_range(s, a, &from, &to);
     return (to - from + a.split - 1) / a.split;
 }
 // the place of number n in the sequences' counts: every lane gets the sequence and what is left of n
@@ -320,7 +324,7 @@ __global__ void __launch_bounds__(PT_THREADS) paged_few_kernel(const PtArgs a) {
     __shared__ int pid[PT_MOST_SPLIT / 16 + 1];
     __shared__ float kfs[PT_MOST_SPLIT / 16 + 1], vfs[PT_MOST_SPLIT / 16 + 1];
     __shared__ float2 ml[PT_WARPS][8];
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, kvh = blockIdx.y;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, kvh = a.head0 + blockIdx.y;
     uint8_t* ring = pt_sm + w * RING;
     const unsigned ring_at = (unsigned)__cvta_generic_to_shared(ring);
     pdl_enter();
@@ -330,7 +334,7 @@ __global__ void __launch_bounds__(PT_THREADS) paged_few_kernel(const PtArgs a) {
     const PgSeq s = a.seqs[seq];
     const int rows = s.count * a.R, tiles = (rows + 7) >> 3, split = rest / tiles, tile = rest - split * tiles, n_split = pt_splits(s, a);
     int from, to;
-    pt_range(s, a.window, &from, &to);
+    pt_range(s, a, &from, &to);
     const int row = tile * 8 + g, tok = row / a.R, pos_first = s.pos0 + tile * 8 / a.R, pos_last = s.pos0 + (min(rows, tile * 8 + 8) - 1) / a.R;
     const int k0 = from + split * a.split, k1 = min(min(to, k0 + a.split), pos_last + 1);       // keys of the slice that some row of the tile may see
     const int lo = a.window > 0 ? max(k0, (pos_first - a.window + 1) & ~15) : k0, units = k1 > lo ? (k1 - lo + 15) >> 4 : 0;
@@ -427,7 +431,7 @@ __global__ void __launch_bounds__(PT_THREADS) paged_few_kernel(const PtArgs a) {
     if (t == 0) ml[w][g] = make_float2(r.m, r.l);
     __syncthreads();
     const int n = min(8, rows - tile * 8);
-    const size_t at = (size_t)blockIdx.x * a.G + kvh;
+    const size_t at = (size_t)blockIdx.x * a.heads + blockIdx.y;
     for (int e = threadIdx.x; e < n * a.dv; e += PT_THREADS) {
         const int y = e / a.dv, col = e - y * a.dv;
         float m = -INFINITY, l = 0.0f, o = 0.0f;
@@ -457,7 +461,7 @@ __global__ void __launch_bounds__(PT_THREADS) paged_few_kernel(const PtArgs a) {
 __global__ void __launch_bounds__(128) paged_sum_kernel(const PtArgs a) {
     __shared__ float so[4][256];
     __shared__ float2 sm[4];
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, kvh = blockIdx.y;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, kvh = a.head0 + blockIdx.y;
     pdl_enter();
     int row, items = 0;
     const int seq = pt_find(a, blockIdx.x, [&](const PgSeq& s) { return pt_splits(s, a) > 1 ? s.count * a.R : 0; }, &row);
@@ -468,7 +472,7 @@ __global__ void __launch_bounds__(128) paged_sum_kernel(const PtArgs a) {
     const int tiles = (s.count * a.R + a.tile_rows - 1) / a.tile_rows, n = pt_splits(s, a), tile = row / a.tile_rows, y = row - tile * a.tile_rows;
     // items of a sequence: slice by slice where a tile is 8 rows, tile by tile from the last one on where it is 128
     const int first = a.tile_rows == 8 ? tile : (tiles - 1 - tile) * n, by = a.tile_rows == 8 ? tiles : 1;
-    auto at = [&](int x) { return ((size_t)(items + first + x * by) * a.G + kvh) * a.tile_rows + y; };
+    auto at = [&](int x) { return ((size_t)(items + first + x * by) * a.heads + blockIdx.y) * a.tile_rows + y; };
     float m = -INFINITY;
     for (int x = lane; x < n; x += 32) m = fmaxf(m, a.ml[at(x)].x);
     m = warp_max(m);
@@ -508,22 +512,25 @@ template <int D, bool I8>
 static cudaError_t pt_launch_few(cc_device* dev, const PtArgs& a, unsigned items) {
     constexpr int smem = PT_WARPS * 128 * D;
     cudaError_t e = cudaFuncSetAttribute(paged_few_kernel<D, I8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess) e = cc_launch_pdl(dev, paged_few_kernel<D, I8>, dim3(items, (unsigned)a.G), PT_THREADS, smem, a);
+    if (e == cudaSuccess) e = cc_launch_pdl(dev, paged_few_kernel<D, I8>, dim3(items, (unsigned)a.heads), PT_THREADS, smem, a);
     dev->launches++;
     return e;
 }
 #include "paged_tile.cuh"
 
+#define TI_WORKSPACE ((int64_t)256 << 20)     // bytes of images that a call has at a time, as long as one head's are no more
+
 // the sequences of rows_lo .. rows_hi rows, in tiles of tile_rows: slices of `most` keys at most, as many as leave no SM without one
 static int pt_run(cc_device* dev, const cc_page_plan* plan, PtArgs a, bool i8) {
     const bool few = a.tile_rows == 8;
-    int64_t keys = 0, items = 0, split_rows = 0;
+    int64_t keys = 0, items = 0, split_rows = 0, key_tiles = 0;
     for (const PgSeq& s : plan->seqs) {
         const int64_t rows = (int64_t)s.count * a.R;
         if (rows < a.rows_lo || rows > a.rows_hi) continue;
         int from, to;
-        pt_range(s, a.window, &from, &to);
+        pt_range(s, a, &from, &to);
         keys += (int64_t)(to - from) * ((rows + a.tile_rows - 1) / a.tile_rows) * a.G;
+        key_tiles += ti_key_tiles(s, a);
     }
     if (!keys) return CC_OK;
     const int64_t slots = (int64_t)dev->sm_count * (few ? 3 : 1), each = (keys + slots - 1) / slots;
@@ -533,29 +540,37 @@ static int pt_run(cc_device* dev, const cc_page_plan* plan, PtArgs a, bool i8) {
         items += (int64_t)n * (((int64_t)s.count * a.R + a.tile_rows - 1) / a.tile_rows);
         if (n > 1) split_rows += (int64_t)s.count * a.R;
     }
-    CC_REQUIRE(dev, items < ((int64_t)1 << 31) && split_rows < ((int64_t)1 << 31), "paged_attention: too many rows");
+    CC_REQUIRE(dev, items < ((int64_t)1 << 31) && split_rows < ((int64_t)1 << 31) && key_tiles < ((int64_t)1 << 31), "paged_attention: too many rows");
+    const size_t kb = (size_t)((a.dk + 63) / 64) * TI_BLOCK, vb = (size_t)((a.dv + 63) / 64) * TI_BLOCK, per_head = few ? 0 : (size_t)key_tiles * (kb + vb + sizeof(TiInfo));
+    a.heads = few || (int64_t)per_head * a.G <= TI_WORKSPACE ? a.G : (int)std::max<int64_t>(1, TI_WORKSPACE / (int64_t)per_head);
+    const size_t part = split_rows ? (size_t)items * a.heads * a.tile_rows * a.dv * sizeof(float) : 0, ml = split_rows ? (size_t)items * a.heads * a.tile_rows * sizeof(float2) : 0;
     void* ws = nullptr; size_t cls = 0;
-    if (split_rows) {
-        const size_t part = (size_t)items * a.G * a.tile_rows * a.dv * sizeof(float), ml = (size_t)items * a.G * a.tile_rows * sizeof(float2);
-        const int rc = cc_pool_alloc(dev, part + ml, &ws, &cls);
+    if (part + per_head) {
+        const int rc = cc_pool_alloc(dev, part + ml + per_head * a.heads + 256, &ws, &cls);
         if (rc) return rc;
-        a.part = (float*)ws; a.ml = (float2*)((uint8_t*)ws + part);
+        a.k_image = (uint8_t*)ws; a.v_image = a.k_image + (few ? 0 : key_tiles * a.heads * kb);
+        a.part = (float*)(a.v_image + (few ? 0 : key_tiles * a.heads * vb));
+        a.ml = (float2*)((uint8_t*)a.part + part); a.info = (TiInfo*)((uint8_t*)a.ml + ml);
     }
-    const int d = std::max(a.dk, a.dv);
-    cudaError_t e;
-    if (few) {
-        e = i8 ? (d <= 64 ? pt_launch_few<64, true>(dev, a, (unsigned)items) : d <= 128 ? pt_launch_few<128, true>(dev, a, (unsigned)items) : pt_launch_few<256, true>(dev, a, (unsigned)items))
-               : (d <= 64 ? pt_launch_few<64, false>(dev, a, (unsigned)items) : d <= 128 ? pt_launch_few<128, false>(dev, a, (unsigned)items) : pt_launch_few<256, false>(dev, a, (unsigned)items));
-    } else {
-        const bool cap = a.softcap > 0.0f;
-        auto kernel = i8 ? (cap ? paged_tile_kernel<true, true> : paged_tile_kernel<true, false>) : (cap ? paged_tile_kernel<false, true> : paged_tile_kernel<false, false>);
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TI_SMEM);
-        if (e == cudaSuccess) e = cc_launch_pdl(dev, kernel, dim3((unsigned)items, (unsigned)a.G), TI_THREADS, TI_SMEM, a, dev->err_dev, dev->err_host);
-        dev->launches++;
-    }
-    if (e == cudaSuccess && split_rows) {
-        e = cc_launch_pdl(dev, paged_sum_kernel, dim3((unsigned)split_rows, (unsigned)a.G), 128, 0, a);
-        dev->launches++;
+    const int d = std::max(a.dk, a.dv), all = a.heads;
+    cudaError_t e = cudaSuccess;
+    for (a.head0 = 0; a.head0 < a.G && e == cudaSuccess; a.head0 += all) {
+        a.heads = std::min(all, a.G - a.head0);
+        if (few) {
+            e = i8 ? (d <= 64 ? pt_launch_few<64, true>(dev, a, (unsigned)items) : d <= 128 ? pt_launch_few<128, true>(dev, a, (unsigned)items) : pt_launch_few<256, true>(dev, a, (unsigned)items))
+                   : (d <= 64 ? pt_launch_few<64, false>(dev, a, (unsigned)items) : d <= 128 ? pt_launch_few<128, false>(dev, a, (unsigned)items) : pt_launch_few<256, false>(dev, a, (unsigned)items));
+        } else {
+            const bool cap = a.softcap > 0.0f;
+            auto kernel = i8 ? (cap ? paged_tile_kernel<true, true> : paged_tile_kernel<true, false>) : (cap ? paged_tile_kernel<false, true> : paged_tile_kernel<false, false>);
+            e = cc_launch_pdl(dev, i8 ? paged_unpack_kernel<true> : paged_unpack_kernel<false>, dim3((unsigned)key_tiles, (unsigned)a.heads), TU_THREADS, 0, a);
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TI_SMEM);
+            if (e == cudaSuccess) e = cc_launch_pdl(dev, kernel, dim3((unsigned)items, (unsigned)a.heads), TI_THREADS, TI_SMEM, a, dev->err_dev, dev->err_host);
+            dev->launches += 2;
+        }
+        if (e == cudaSuccess && split_rows) {
+            e = cc_launch_pdl(dev, paged_sum_kernel, dim3((unsigned)split_rows, (unsigned)a.heads), 128, 0, a);
+            dev->launches++;
+        }
     }
     if (ws) cc_pool_free(dev, ws, cls);
     if (e != cudaSuccess) return cc_fail(dev, CC_ERR_CUDA, "paged_attention: %s", cudaGetErrorString(e));
@@ -592,10 +607,10 @@ extern "C" CC_API int cc_paged_attention(cc_device* dev, const cc_page_plan* pla
         a.n_seqs = plan->n_seqs; a.table_cols = plan->table_cols; a.page = plan->page; a.shift = plan->shift;
         a.H = H; a.G = c.G; a.R = H / c.G; a.dk = c.dk; a.dv = c.dv;
         // rows of a sequence and key head: up to PT_FEW in tiles of 8, more in tiles of 128 where a head's numbers have room there
-        a.rows_lo = 1; a.rows_hi = c.dk <= TI_D && c.dv <= TI_D ? PT_FEW : 0x7fffffff; a.tile_rows = 8;
+        a.rows_lo = 1; a.rows_hi = c.dk <= TI_D && c.dv <= TI_D ? PT_FEW : 0x7fffffff; a.tile_rows = 8; a.align = 16;
         rc = pt_run(dev, plan, a, c.i8);
         if (!rc && a.rows_hi == PT_FEW) {
-            a.rows_lo = PT_FEW + 1; a.rows_hi = 0x7fffffff; a.tile_rows = TI_ROWS;
+            a.rows_lo = PT_FEW + 1; a.rows_hi = 0x7fffffff; a.tile_rows = TI_ROWS; a.align = TI_KEYS;
             rc = pt_run(dev, plan, a, c.i8);
         }
     }

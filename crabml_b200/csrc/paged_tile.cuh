@@ -1,44 +1,57 @@
 // paged_tile.cuh -- attention of many rows over pages (prompts, drafts of many heads), on tcgen05.mma.  Included by paged_attn.cu behind its few-row kernel.
 //
+// paged_unpack_kernel lays out the visible keys and values once for all rows: per 128 keys and head an image of each operand as f16 (codes and 16-bit numbers are exact),
+// in the order of the 128-byte swizzle, that a bulk copy brings into shared memory as it is, beside the factors of its pages.  (Converted by warps of the kernel below
+// for each of its tiles instead, portions of three prompts took 285 us: 2700 of 8000 instructions of a step, and an instruction cache that did not hold all roles.)
+//
 // A tile is 128 rows (a row: a query of one head; the heads of a key head side by side) x the keys they see, 128 at a time:
-//   S = Q_h K^T + Q_l K^T     (K as f16 in shared memory: codes and 16-bit numbers are exact)     2 x 128 x 128 x dk products
+//   S = Q_h K^T + Q_l K^T                                                                         2 x 128 x 128 x dk products
 //   P = exp2(S f - largest) as f16 h and l, written over S in TMEM, the first operand of
 //   O = P_h V + P_l V         in an accumulator of its own, added to 32-bit registers afterwards: the tensor core cuts its sums off at 24 bits, a chain over
 //                             thousands of keys would drift (1e-5 of a result after 2000 keys of one sign)
-// S and O have two buffers each (512 TMEM columns), K and V two stages of f16 (128 KB beside the 64 KB of Q): while warps 0-7 make the weights of one step, the
-// tensor core computes the scores of the next and the sums of the one before, and warps 8-13 read, convert and store the keys and values behind.
-// A row's 128 scores lie with two threads, lane and half; they exchange their largest score once a step.
-// Warps 0-7 weights and sums, 8-13 keys and values, 15 issues the products.  Every wait is bounded (sg_wait); where one ran out all roles run to their ends without
-// waiting (the barrier of warps 0-7 included) and the host reports it.
+// S and O have two buffers each (512 TMEM columns), K and V two stages (128 KB beside the 64 KB of Q): while 8 warps make the weights of one step, the tensor core
+// computes the scores of the next and the sums of the one before.
+// A row's 128 scores lie with two threads, a half each, which exchange their largest score once a step.  Warps 0-7 weights and sums, 8 the copies, 9 the products.
+// Every wait is bounded (sg_wait); where one ran out all roles run to their ends without waiting (the barrier of warps 0-7 included) and the host reports it.
 #pragma once
 #include "split_gemm.cuh"
 
 #define TI_ROWS 128
 #define TI_KEYS 128
-#define TI_THREADS 512                        // 8 warps of weights and sums, 6 of keys and values, one that issues the products, one idle
-#define TI_SOFT 256
-#define TI_LOADERS 6
-// 512 threads of 128 registers at launch are 256 of 200 and 256 of 56 afterwards (65536 either way)
-#define TI_REGS_SOFT 200
-#define TI_REGS_REST 56
-static_assert(TI_SOFT * TI_REGS_SOFT + (TI_THREADS - TI_SOFT) * TI_REGS_REST <= TI_THREADS * 128, "more registers than the block was launched with");
+#define TI_SPLIT 2                            // threads of a row: half of a step's keys and of the value columns each
+#define TI_SOFT (TI_ROWS * TI_SPLIT)
+#define TI_SOFT_WARPS (TI_SOFT / 32)
+#define TI_THREADS (TI_SOFT + 128)
+// 384 threads of 168 registers at launch are 256 of 216 and 128 of 72 afterwards.  No register of a step may spill: shared memory leaves next to no L1, and with 80 numbers
+// a thread spilled (four threads a row, 96 registers) a step took twice as long
+#define TI_REGS 168
+#define TI_REGS_SOFT 216
+#define TI_REGS_REST 72
+static_assert(TI_SOFT * TI_REGS_SOFT + (TI_THREADS - TI_SOFT) * TI_REGS_REST <= TI_THREADS * TI_REGS, "more registers than the block was launched with");
+#define TI_XC (TI_KEYS / TI_SPLIT)
+#define TI_OC (TI_D / TI_SPLIT)
 #define TI_MOST 4096                          // keys of a slice
 #define TI_D 128                              // largest dk and dv
+#define TI_STEPS (TI_MOST / TI_KEYS)
 
+// what stands beside the images of 128 keys of a head
+struct TiInfo {
+    float kf[TI_KEYS / 16], vf[TI_KEYS / 16]; // factors of 16 keys each; vf relative to vref, a power of two near the largest
+    float vref;
+    int wild;                                 // values that are not finite are zeros in the image
+    unsigned nan;                             // groups of 16 keys with a factor that is not finite (it counts as 0)
+    int pad;
+};
 struct TiShared {
     unsigned long long k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], o_empty[2], drained;
     unsigned tmem_base;
-    int fail, wild[4];                        // wild[step % 4] == step + 1: values that are not finite were left out of the step's sums
-    int page[TI_MOST / 16 + 8];              // of every 16 keys: -1 - block for the open one
-    float kf[TI_MOST / 16 + 8], vf[TI_MOST / 16 + 8];      // vf: relative to vref, a power of two near a step's largest
-    float vref[TI_MOST / TI_KEYS + 1];
-    int lost;                                // some factor is not finite: it counts as 0, and NaN goes to the rows that see its keys (nan)
-    uint8_t nan[TI_MOST / 16 + 8];
-    float top[2][2][TI_ROWS], sum[2][TI_ROWS];
+    int fail;
+    TiInfo info[TI_STEPS];
+    float top[2][TI_SPLIT][TI_ROWS], sum[TI_SPLIT][TI_ROWS];
 };
 #define TI_OPERAND (TI_KEYS * TI_D * 2)       // bytes of a tile of f16: two blocks of 64 columns, rows of 128 bytes under the 128-byte swizzle
-#define TI_GROUP 2048                         // bytes of a group as it lies in its page, two slots a warp
-#define TI_SMEM (6 * TI_OPERAND + 2 * TI_LOADERS * TI_GROUP + 1024)
+#define TI_SMEM (6 * TI_OPERAND + 1024)
+#define TI_BLOCK (TI_OPERAND / 2)             // 64 columns of an operand; an image is as many as d has
 
 __device__ __forceinline__ unsigned ti_at(int row, int chunk) { return (unsigned)((chunk >> 3) * (TI_OPERAND / 2) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)); }
 // B whose rows are the sum's index and whose columns (64 of them in 128 bytes) are the result's: blocks of 64 columns are TI_OPERAND / 2 apart, groups of 8 rows 1024 bytes
@@ -101,55 +114,101 @@ __device__ __forceinline__ float ti_max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-__device__ __forceinline__ void ti_soft_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void ti_soft_sync() { asm volatile("bar.sync 1, %0;" ::"n"(TI_SOFT) : "memory"); }
 
-// What hot loops do not hold: the kernel's roles share an instruction cache, and with everything in line they waited for it most of the time (285 -> TI_COLD_US us).
-// 16 rows of an open block into an operand, values that are not finite as zeros: whether there were any
-__device__ __noinline__ bool ti_open_rows(uint8_t* base, const __half* p, int d, int there, bool val) {
-    bool wild = false;
-    for (int e = threadIdx.x & 31; e < 16 * (d / 8); e += 32) {
-        const int r = e / (d / 8);
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (r < there) x = ((const uint4*)p)[e];
-        if (val) {
-            const unsigned w0 = pt_wild(x.x), w1 = pt_wild(x.y), w2 = pt_wild(x.z), w3 = pt_wild(x.w);
-            wild |= (w0 | w1 | w2 | w3) != 0u;
-            x.x &= ~w0; x.y &= ~w1; x.z &= ~w2; x.w &= ~w3;
-        }
-        *(uint4*)(base + ti_at(r, e - r * (d / 8))) = x;
-    }
-    return wild;
+// images of the sequences with a tile of 128 rows: their tiles of keys count from the first that a new token sees, sequence after sequence
+__host__ __device__ __forceinline__ int ti_key_tiles(const PgSeq& s, const PtArgs& a) {
+    const int64_t rows = (int64_t)s.count * a.R;
+    if (rows < a.rows_lo || rows > a.rows_hi) return 0;
+    int from, to;
+    pt_range(s, a, &from, &to);
+    return (to - from + TI_KEYS - 1) / TI_KEYS;
 }
-// the columns, of `cols` from c_first on, that are not finite in a value that the row sees among the keys key0 .. key0 + TI_KEYS (all of them for a factor that is not)
+#define TU_THREADS 256
+// grid (tiles of keys, heads of this call)
 template <bool I8>
-__device__ __noinline__ unsigned long long ti_lost(const PtArgs& a, const int* page, const uint8_t* nan, int kvh, int key0, int key_lo, int key_hi, int c_first, int cols) {
-    unsigned long long lost = 0;
-    for (int key = max(key0, key_lo); key <= min(key0 + TI_KEYS - 1, key_hi); key++) {
-        const int g = (key - key0) >> 4;
-        if (nan[g]) lost = ~0ull;
-        if (I8 && page[g] >= 0) continue;
-        const __half* p = (I8 ? a.vo : (const __half*)a.v) + (((size_t)(I8 ? -1 - page[g] : page[g]) * a.G + kvh) * a.page + (key & (a.page - 1))) * a.dv + c_first;
-        for (int c = 0; c < cols; c++)
-            if (((unsigned)__half_as_ushort(p[c]) & 0x7c00u) == 0x7c00u) lost |= 1ull << c;
+__global__ void __launch_bounds__(TU_THREADS) paged_unpack_kernel(const PtArgs a) {
+    __shared__ int pages[TI_KEYS / 16];
+    __shared__ TiInfo info;
+    const int tid = threadIdx.x, kvh = a.head0 + blockIdx.y;
+    pdl_enter();
+    int kt;
+    const int seq = pt_find(a, blockIdx.x, [&](const PgSeq& s) { return ti_key_tiles(s, a); }, &kt);
+    if (seq < 0) return;
+    const PgSeq s = a.seqs[seq];
+    int from, to;
+    pt_range(s, a, &from, &to);
+    const int key0 = from + kt * TI_KEYS, opens = I8 ? to >> a.shift << a.shift : 0, open = 2 * s.slot + ((to >> a.shift) & 1);
+    if (tid < 32) {
+        float kf = 1.0f, vf = 1.0f;
+        const int key = key0 + (tid & 7) * 16;
+        int page = -1;                                        // nothing there, or the open block
+        if (key < to && (!I8 || key < opens)) {
+            page = a.table[(int64_t)seq * a.table_cols + (key >> a.shift)];
+            if (I8) { kf = a.ks[(int64_t)page * a.G + kvh]; vf = a.vs[(int64_t)page * a.G + kvh]; }
+        }
+        const bool bad = !(vf >= 0.0f && vf < INFINITY && kf >= 0.0f && kf < INFINITY);
+        if (bad) kf = vf = 0.0f;
+        const float vmax = warp_max(vf), vref = fminf(fmaxf(__uint_as_float(__float_as_uint(vmax) & 0x7f800000u), 0x1p-100f), 0x1p100f);
+        const unsigned nan = __ballot_sync(0xffffffffu, bad) & 0xffu;
+        if (tid < TI_KEYS / 16) { pages[tid] = page; info.kf[tid] = kf; info.vf[tid] = vf / vref; }
+        if (tid == 0) { info.vref = vref; info.nan = nan; info.pad = 0; }
     }
-    return lost;
+    __syncthreads();
+    const size_t at = (size_t)blockIdx.x * a.heads + blockIdx.y;
+    bool wild = false;
+#pragma unroll
+    for (int v = 0; v < 2; v++) {
+        const int d = v ? a.dv : a.dk;
+        uint8_t* image = (v ? a.v_image : a.k_image) + at * ((d + 63) / 64) * TI_BLOCK;
+        // a lane takes 16 numbers of a row: two chunks of its image
+#pragma unroll 4
+        for (int e = tid; e < TI_KEYS * (d / 16); e += TU_THREADS) {
+            const int r = e / (d / 16), piece = e - r * (d / 16), key = key0 + r, page = pages[r >> 4], row = key & (a.page - 1);
+            uint4 x = make_uint4(0, 0, 0, 0), y = x;
+            if (I8 && page >= 0) {
+                const uint4 c = __ldg((const uint4*)((v ? a.v : a.k) + (((size_t)page * a.G + kvh) * a.page + row) * d) + piece);
+                const unsigned u0 = c.x ^ 0x80808080u, u1 = c.y ^ 0x80808080u, u2 = c.z ^ 0x80808080u, u3 = c.w ^ 0x80808080u;
+                x = make_uint4(pt_half2(u0, 0x4140), pt_half2(u0, 0x4342), pt_half2(u1, 0x4140), pt_half2(u1, 0x4342));
+                y = make_uint4(pt_half2(u2, 0x4140), pt_half2(u2, 0x4342), pt_half2(u3, 0x4140), pt_half2(u3, 0x4342));
+            } else if (key < to) {
+                const __half* p = I8 ? (v ? a.vo : a.ko) + (((size_t)open * a.G + kvh) * a.page + row) * d : (const __half*)(v ? a.v : a.k) + (((size_t)page * a.G + kvh) * a.page + row) * d;
+                x = __ldg((const uint4*)p + 2 * piece); y = __ldg((const uint4*)p + 2 * piece + 1);
+                if (v) {
+                    unsigned* u[8] = {&x.x, &x.y, &x.z, &x.w, &y.x, &y.y, &y.z, &y.w};
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const unsigned w = pt_wild(*u[i]);
+                        wild |= w != 0u;
+                        *u[i] &= ~w;
+                    }
+                }
+            }
+            *(uint4*)(image + ti_at(r, 2 * piece)) = x;
+            *(uint4*)(image + ti_at(r, 2 * piece + 1)) = y;
+        }
+    }
+    wild = __syncthreads_or(wild);
+    if (tid == 0) info.wild = wild;
+    __syncthreads();
+    if (tid < (int)(sizeof(TiInfo) / 4)) ((int*)(a.info + at))[tid] = ((const int*)&info)[tid];
 }
+
 template <bool I8, bool CAP>
 __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_constant__ PtArgs a, unsigned* err_dev, unsigned* err_host) {
     extern __shared__ __align__(1024) uint8_t ti_raw[];
     __shared__ TiShared sh;
     uint8_t* qs = (uint8_t*)(((uintptr_t)ti_raw + 1023) & ~(uintptr_t)1023);      // Q_h, Q_l
     uint8_t *ks = qs + 2 * TI_OPERAND, *vs = ks + 2 * TI_OPERAND;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.y;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = a.head0 + blockIdx.y;
     if (tid == 0) {
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            pg_mbar_init(pg_smem(&sh.k_full[i]), I8 ? TI_KEYS / 16 : TI_KEYS / 8); pg_mbar_init(pg_smem(&sh.v_full[i]), I8 ? TI_KEYS / 16 : TI_KEYS / 8); pg_mbar_init(pg_smem(&sh.k_empty[i]), 1); pg_mbar_init(pg_smem(&sh.v_empty[i]), 1);
-            pg_mbar_init(pg_smem(&sh.s_full[i]), 1); pg_mbar_init(pg_smem(&sh.p_full[i]), 8); pg_mbar_init(pg_smem(&sh.o_full[i]), 1); pg_mbar_init(pg_smem(&sh.o_empty[i]), 8);
-            sh.wild[i] = sh.wild[i + 2] = 0;
+            pg_mbar_init(pg_smem(&sh.k_full[i]), 1); pg_mbar_init(pg_smem(&sh.v_full[i]), 1); pg_mbar_init(pg_smem(&sh.k_empty[i]), 1); pg_mbar_init(pg_smem(&sh.v_empty[i]), 1);
+            pg_mbar_init(pg_smem(&sh.s_full[i]), 1); pg_mbar_init(pg_smem(&sh.p_full[i]), TI_SOFT_WARPS); pg_mbar_init(pg_smem(&sh.o_full[i]), 1); pg_mbar_init(pg_smem(&sh.o_empty[i]), TI_SOFT_WARPS);
         }
         pg_mbar_init(pg_smem(&sh.drained), 1);
-        sh.fail = sh.lost = 0;
+        sh.fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_enter();
@@ -160,59 +219,45 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
     const PgSeq s = a.seqs[seq];
     const int rows = s.count * a.R, tiles = (rows + TI_ROWS - 1) / TI_ROWS, n_split = pt_splits(s, a), tile = tiles - 1 - rest / n_split, split = rest % n_split;      // late rows, which see most, first
     int from, to;
-    pt_range(s, a.window, &from, &to);
+    pt_range(s, a, &from, &to);
     const int row0 = tile * TI_ROWS, n_rows = min(TI_ROWS, rows - row0), pos_first = s.pos0 + row0 / a.R, pos_last = s.pos0 + (row0 + n_rows - 1) / a.R;
     const int k0 = from + split * a.split, k1 = min(min(to, k0 + a.split), pos_last + 1);
-    const int lo = a.window > 0 ? max(k0, (pos_first - a.window + 1) & ~15) : k0, steps = k1 > lo ? (k1 - lo + TI_KEYS - 1) / TI_KEYS : 0;
+    const int lo = a.window > 0 ? max(k0, (pos_first - a.window + 1) & ~(TI_KEYS - 1)) : k0, steps = k1 > lo ? (k1 - lo + TI_KEYS - 1) / TI_KEYS : 0;
     const int opens = I8 ? to >> a.shift << a.shift : 0;
-    for (int i = tid; i < steps * (TI_KEYS / 16); i += TI_THREADS) {
-        const int key = lo + i * 16;
-        float kf = 1.0f, vf = 1.0f;
-        int page = 0;
-        if (key < to) {
-            page = a.table[(int64_t)seq * a.table_cols + (key >> a.shift)];
-            if (I8 && key >= opens) page = -1 - (2 * s.slot + ((to >> a.shift) & 1));
-            else if (I8) { kf = a.ks[(int64_t)page * a.G + kvh]; vf = a.vs[(int64_t)page * a.G + kvh]; }
-        }
-        const bool bad = !(vf >= 0.0f && vf < INFINITY && kf >= 0.0f && kf < INFINITY);
-        sh.page[i] = page; sh.kf[i] = bad ? 0.0f : kf; sh.vf[i] = bad ? 0.0f : vf; sh.nan[i] = bad;
-        if (bad) sh.lost = 1;
+    // the images of the first step, and what stands beside those of all steps
+    int before = 0;
+    for (int x = lane; x < seq; x += 32) before += ti_key_tiles(a.seqs[x], a);
+    const size_t image = (size_t)(warp_sum_i(before) + (lo - from) / TI_KEYS) * a.heads + blockIdx.y;
+    for (int i = tid; i < steps * (int)(sizeof(TiInfo) / 4); i += TI_THREADS) {
+        const int k = i / (int)(sizeof(TiInfo) / 4);
+        ((int*)sh.info)[i] = ((const int*)(a.info + image + (size_t)k * a.heads))[i - k * (int)(sizeof(TiInfo) / 4)];
     }
-    __syncthreads();
-    for (int k = tid; k < steps; k += TI_THREADS) {
-        float most = 0.0f;
-#pragma unroll
-        for (int g = 0; g < TI_KEYS / 16; g++) most = fmaxf(most, sh.vf[k * (TI_KEYS / 16) + g]);
-        const float vref = fminf(fmaxf(__uint_as_float(__float_as_uint(most) & 0x7f800000u), 0x1p-100f), 0x1p100f);
-        sh.vref[k] = vref;
-#pragma unroll
-        for (int g = 0; g < TI_KEYS / 16; g++) sh.vf[k * (TI_KEYS / 16) + g] /= vref;
-    }
-    if (warp == 15) {
+    if (warp == (TI_SOFT_WARPS + 1)) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pg_smem(&sh.tmem_base)), "n"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     // the queries as h and l, near 2^14
-    const int row = (warp & 3) * 32 + lane, half = (warp >> 2) & 1;   // warps 0-7: TMEM lane and half of the columns
+    const int row = (warp & 3) * 32 + lane, part = warp >> 2;         // of weights and sums: TMEM lane, part of the columns
     const int tok = (row0 + row) / a.R, head = kvh * a.R + (row0 + row) - tok * a.R;
-    const bool in = warp < 8 && row < n_rows;
+    const bool in = warp < TI_SOFT_WARPS && row < n_rows;
     float inv = 1.0f;
-    if (warp < 8) {
+    if (warp < TI_SOFT_WARPS) {
         const float* q = a.q + ((int64_t)(s.first + tok) * a.H + head) * a.dk;
         float top = 0.0f;
-        for (int c = half * 4; c < a.dk; c += 8) {
+        for (int c = part * 4; c < a.dk; c += 4 * TI_SPLIT) {
             const float4 v = in ? *(const float4*)(q + c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
         }
-        sh.top[0][half][row] = top;
+        sh.top[0][part][row] = top;
         ti_soft_sync();
-        top = fmaxf(top, sh.top[0][half ^ 1][row]);
+#pragma unroll
+        for (int i = 0; i < TI_SPLIT; i++) top = fmaxf(top, sh.top[0][i][row]);
         int ex = 14;
         if (top > 0.0f && top < INFINITY) frexpf(top, &ex);
         ex = max(ex, -100);
         const float f = copysignf(ldexpf(1.0f, 14 - ex), a.scale);      // (so that a larger sum is a larger score)
         inv = ldexpf(1.0f, ex - 14);
-        for (int j = half; j < a.dk / 8; j += 2) {
+        for (int j = part; j < a.dk / 8; j += TI_SPLIT) {
             float v[8];
 #pragma unroll
             for (int i = 0; i < 8; i += 4) {
@@ -231,9 +276,9 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
     pg_fence_after();
     const unsigned tmem = sh.tmem_base;
 
-    if (warp >= TI_SOFT / 32) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TI_REGS_REST));
-    else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TI_REGS_SOFT));
-    if (warp == 15) {
+    if (warp >= TI_SOFT_WARPS) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TI_REGS_REST));
+        if (warp == TI_SOFT_WARPS + 1) {
         // ===== products: one thread =====
         if (lane == 0) {
             const unsigned idesc_s = pg_instr_desc(128, TI_KEYS), idesc_o = pg_instr_desc(128, a.dv) | 1u << 16;
@@ -270,94 +315,41 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
             ti_wait(pg_smem(&sh.drained), 0, &never);
         }
         __syncwarp();
-    } else if (warp >= 8) {
-        // ===== keys and values: a warp takes 2 KB of an operand at a time (a group: 16 rows of codes or 8 of 16-bit numbers, in one page), its next one is under way to
-        // shared memory meanwhile; every lane reads there what it copied itself =====
-        constexpr int N = TI_GROUP / 512, E = I8 ? 16 : 8, GR = I8 ? 16 : 8, PER = TI_KEYS / GR;      // pieces of 16 bytes of a lane, numbers of a piece, rows of a group, groups of an operand
-        const int groups = warp < TI_SOFT / 32 + TI_LOADERS ? steps * 2 * PER : 0, per_k = a.dk / E, per_v = a.dv / E;
-        uint8_t* mine = vs + 2 * TI_OPERAND + (size_t)(warp - TI_SOFT / 32) * 2 * TI_GROUP + lane * 16;
-        const unsigned mine_at = pg_smem(mine);
-        // where the lane's pieces lie in an operand's rows; 8-bit: the chunk that is stored first, bit 0 set where that is the piece's second one
-        unsigned off_k[N], off_v[N];
-#pragma unroll
-        for (int i = 0; i < N; i++)
-#pragma unroll
-            for (int v = 0; v < 2; v++) {
-                const int per = v ? per_v : per_k, e = i * 32 + lane, row = e / per, piece = e - row * per, second = piece >> 2 & 1;
-                (v ? off_v : off_k)[i] = row >= GR ? ~0u : I8 ? ti_at(row, 2 * piece + second) | second : ti_at(row, piece);
+        } else if (warp == TI_SOFT_WARPS) {
+        // ===== copies of the images: one thread =====
+        if (lane == 0) {
+            const unsigned kb = (unsigned)((a.dk + 63) / 64) * TI_BLOCK, vb = (unsigned)((a.dv + 63) / 64) * TI_BLOCK;
+            auto copy = [&](uint8_t* to_smem, const uint8_t* src, unsigned bytes, unsigned bar) {
+                pg_mbar_expect_tx(bar, bytes);
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(pg_smem(to_smem)), "l"(src), "r"(bytes), "r"(bar) : "memory");
+            };
+            int k = 0, v = 0;                                         // copies begun
+            for (; k < steps; k++) {
+                const unsigned slot = k & 1, ph = ((k >> 1) & 1u) ^ 1u;
+                const size_t at = image + (size_t)k * a.heads;
+                if (!ti_wait(pg_smem(&sh.k_empty[slot]), ph, &sh.fail)) break;
+                copy(ks + (size_t)slot * TI_OPERAND, a.k_image + at * kb, kb, pg_smem(&sh.k_full[slot]));
+                if (!ti_wait(pg_smem(&sh.v_empty[slot]), ph, &sh.fail)) { k++; break; }
+                copy(vs + (size_t)slot * TI_OPERAND, a.v_image + at * vb, vb, pg_smem(&sh.v_full[slot]));
+                v++;
             }
-        auto fetch = [&](int u, unsigned to_smem) {
-            if (u < groups) {
-                const int step = u / (2 * PER), g = u & (PER - 1), key = lo + step * TI_KEYS + g * GR, page = sh.page[(step * TI_KEYS + g * GR) >> 4];
-                const bool val = u & PER;
-                const int d = val ? a.dv : a.dk, there = min(GR, to - key) * (d / E);
-                if (!I8 || page >= 0) {                                // (the open block's rows come when they are stored)
-                    const size_t at = (((size_t)page * a.G + kvh) * a.page + (key & (a.page - 1))) * d;
-                    const uint8_t* p = (val ? a.v : a.k) + (I8 ? at : at * 2);
-#pragma unroll
-                    for (int i = 0; i < N; i++) pt_copy16(to_smem + i * 512, i * 32 + lane < there ? p + (i * 32 + lane) * 16 : p, i * 32 + lane < there);      // zeros behind the end
-                }
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
-        bool ok = true;
-        const int first = warp - TI_SOFT / 32;
-        unsigned turn = 0;
-        fetch(first, mine_at);
-#pragma unroll 1
-        for (int u = first; u < groups; u += TI_LOADERS, turn ^= TI_GROUP) {
-            const int step = u / (2 * PER), g = u & (PER - 1);
-            const bool val = u & PER;
-            fetch(u + TI_LOADERS, mine_at + (turn ^ TI_GROUP));
-            if (!(ok = ti_wait_warp(pg_smem(val ? &sh.v_empty[step & 1] : &sh.k_empty[step & 1]), ((step >> 1) & 1u) ^ 1u, &sh.fail))) break;
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-            uint8_t* base = (val ? vs : ks) + (size_t)(step & 1) * TI_OPERAND + g * GR * 128;
-            const int page = sh.page[(step * TI_KEYS + g * GR) >> 4];
-            bool wild = false;
-            if (I8 && page < 0) {
-                const int key = lo + step * TI_KEYS + g * GR, d = val ? a.dv : a.dk;
-                wild = ti_open_rows(base, (val ? a.vo : a.ko) + (((size_t)(-1 - page) * a.G + kvh) * a.page + (key & (a.page - 1))) * d, d, to - key, val);
-            } else {
-#pragma unroll
-                for (int i = 0; i < N; i++) {
-                    const unsigned off = val ? off_v[i] : off_k[i];
-                    if (off == ~0u) continue;
-                    const uint4 r = *(const uint4*)(mine + turn + i * 512);
-                    if (I8) {
-                        // the lanes of a row fill all banks at once: those of its second half store their second 8 numbers first (chunk 2 p + 1 is chunk 2 p with 16 flipped)
-                        const bool odd = off & 1u;
-                        const unsigned a0 = (odd ? r.z : r.x) ^ 0x80808080u, a1 = (odd ? r.w : r.y) ^ 0x80808080u;
-                        const unsigned b0 = (odd ? r.x : r.z) ^ 0x80808080u, b1 = (odd ? r.y : r.w) ^ 0x80808080u;
-                        const unsigned at = off & ~1u;
-                        *(uint4*)(base + at) = make_uint4(pt_half2(a0, 0x4140), pt_half2(a0, 0x4342), pt_half2(a1, 0x4140), pt_half2(a1, 0x4342));
-                        *(uint4*)(base + (at ^ 16u)) = make_uint4(pt_half2(b0, 0x4140), pt_half2(b0, 0x4342), pt_half2(b1, 0x4140), pt_half2(b1, 0x4342));
-                    } else {
-                        uint4 x = r;
-                        if (val) {
-                            const unsigned w0 = pt_wild(x.x), w1 = pt_wild(x.y), w2 = pt_wild(x.z), w3 = pt_wild(x.w);
-                            wild |= (w0 | w1 | w2 | w3) != 0u;
-                            x.x &= ~w0; x.y &= ~w1; x.z &= ~w2; x.w &= ~w3;
-                        }
-                        *(uint4*)(base + off) = x;
-                    }
-                }
-            }
-            if (wild) atomicExch(&sh.wild[step & 3], step + 1);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            sg_arrive(pg_smem(val ? &sh.v_full[step & 1] : &sh.k_full[step & 1]));
+            int never = 0;                                            // no copy is under way when the CTA ends
+            for (int i = max(0, k - 2); i < k; i++) ti_wait(pg_smem(&sh.k_full[i & 1]), (i >> 1) & 1u, &never);
+            for (int i = max(0, v - 2); i < v; i++) ti_wait(pg_smem(&sh.v_full[i & 1]), (i >> 1) & 1u, &never);
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
+        }
     } else {
         // ===== weights and sums =====
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TI_REGS_SOFT));
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
-        const int c_first = half ? ((a.dv / 2 + 15) & ~15) : 0, cols = half ? a.dv - c_first : (a.dv / 2 + 15) & ~15;      // this thread's columns of O
+        const int width = (a.dv + 16 * TI_SPLIT - 1) / (16 * TI_SPLIT) * 16, c_first = part * width, cols = max(0, min(width, a.dv - c_first));      // this thread's columns of O
         const int pos = in ? s.pos0 + tok : -1, key_lo = a.window > 0 ? pos - a.window + 1 : 0, key_hi = min(pos, k1 - 1);      // the last step may reach into the next slice
         const float f0 = inv * fabsf(a.scale) * (CAP ? 1.0f : PT_LOG2E);
-        ti_f2 acc[TI_D / 4];
+        ti_f2 acc[TI_OC / 2];
         float m = -INFINITY, l = 0.0f, alpha_prev = 0.0f, vref_prev = 0.0f;
-        unsigned long long lost = 0;                                  // columns of this thread that have met a value that is not finite
 #pragma unroll
-        for (int i = 0; i < TI_D / 4; i++) acc[i] = 0ull;
+        for (int i = 0; i < TI_OC / 2; i++) acc[i] = 0ull;
         bool ok = true;
         auto add = [&](int k) {                                       // the sums of step k
             const unsigned slot = k & 1;
@@ -365,7 +357,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
             pg_fence_after();
             const ti_f2 alpha2 = ti_two(alpha_prev, alpha_prev), vref2 = ti_two(vref_prev, vref_prev);
 #pragma unroll
-            for (int c = 0; c < TI_D / 2; c += 32) {
+            for (int c = 0; c < TI_OC; c += 32) {
                 if (c >= cols) break;
                 unsigned v[32];
                 sg_tmem16(tmem + 256 + slot * 128 + lanes + c_first + c, *(unsigned(*)[16])v);
@@ -382,53 +374,52 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
             }
             pg_fence_before();
             sg_arrive(pg_smem(&sh.o_empty[slot]));
-            if (*(volatile int*)&sh.wild[k & 3] == k + 1 || sh.lost)
-                lost |= ti_lost<I8>(a, sh.page + k * (TI_KEYS / 16), sh.nan + k * (TI_KEYS / 16), kvh, lo + k * TI_KEYS, key_lo, key_hi, c_first, cols);
         };
 #pragma unroll 1
         for (int k = 0; k < steps; k++) {
             const unsigned slot = k & 1;
-            const int key0 = lo + k * TI_KEYS + half * 64;
-            float f[4];                                               // factor of 16 keys' sums; 0 (a block of zeros) must not meet the -inf of a hidden key
+            const int key0 = lo + k * TI_KEYS + part * TI_XC;
+            float f[TI_XC / 16];                                               // factor of 16 keys' sums; 0 (a block of zeros) must not meet the -inf of a hidden key
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
-                f[g] = f0 * sh.kf[k * (TI_KEYS / 16) + half * 4 + g];
+            for (int g = 0; g < TI_XC / 16; g++) {
+                f[g] = f0 * sh.info[k].kf[part * (TI_XC / 16) + g];
                 f[g] = f[g] == 0.0f ? 1e-37f : f[g];
             }
             ok = ok && ti_wait_warp(pg_smem(&sh.s_full[slot]), (k >> 1) & 1u, &sh.fail);
-            unsigned x[64];
+            unsigned x[TI_XC];
             if (ok) {
                 pg_fence_after();
 #pragma unroll
-                for (int c = 0; c < 64; c += 16) sg_tmem16(tmem + slot * 128 + lanes + half * 64 + c, *(unsigned(*)[16])(x + c));
+                for (int c = 0; c < TI_XC; c += 16) sg_tmem16(tmem + slot * 128 + lanes + part * TI_XC + c, *(unsigned(*)[16])(x + c));
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                for (int c = 0; c < 64; c++) asm volatile("" : "+r"(x[c]));
+                for (int c = 0; c < TI_XC; c++) asm volatile("" : "+r"(x[c]));
             }
             if (CAP) {
 #pragma unroll
-                for (int c = 0; c < 64; c++) x[c] = __float_as_uint(a.softcap * tanhf(__uint_as_float(x[c]) * f[c / 16] / a.softcap) * PT_LOG2E);
+                for (int c = 0; c < TI_XC; c++) x[c] = __float_as_uint(a.softcap * tanhf(__uint_as_float(x[c]) * f[c / 16] / a.softcap) * PT_LOG2E);
 #pragma unroll
-                for (int g = 0; g < 4; g++) f[g] = 1.0f;
+                for (int g = 0; g < TI_XC / 16; g++) f[g] = 1.0f;
             }
             if (lo + k * TI_KEYS + TI_KEYS - 1 > min(pos_first, k1 - 1) || (a.window > 0 && lo + k * TI_KEYS < pos_last - a.window + 1)) {
                 const int c_lo = key_lo - key0, c_hi = key_hi - key0;
 #pragma unroll
-                for (int c = 0; c < 64; c++)
+                for (int c = 0; c < TI_XC; c++)
                     if (c > c_hi || c < c_lo) x[c] = 0xff800000u;
             }
             float mx = -INFINITY;
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
+            for (int g = 0; g < TI_XC / 16; g++) {
                 float y = fmaxf(__uint_as_float(x[g * 16]), __uint_as_float(x[g * 16 + 1]));
 #pragma unroll
                 for (int c = 2; c < 16; c += 2) y = ti_max3(y, __uint_as_float(x[g * 16 + c]), __uint_as_float(x[g * 16 + c + 1]));
                 mx = fmaxf(mx, y * f[g]);
             }
-            sh.top[slot][half][row] = mx;
-            ti_soft_sync();                                           // .. and both halves have read S
-            mx = fmaxf(mx, sh.top[slot][half ^ 1][row]);
-            const float* vfs = sh.vf + k * (TI_KEYS / 16);
+            sh.top[slot][part][row] = mx;
+            ti_soft_sync();                                           // .. and all parts have read S
+#pragma unroll
+            for (int i = 0; i < TI_SPLIT; i++) mx = fmaxf(mx, sh.top[slot][i][row]);
+            const float* vfs = sh.info[k].vf;
             const float m_new = fmaxf(m, mx), base = m_new == -INFINITY ? 0.0f : PT_SHIFT - m_new;
             const float alpha = m == m_new ? 1.0f : ti_exp2(m - m_new);
             m = m_new;
@@ -436,9 +427,9 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
             if (ok) {
                 const ti_f2 base2 = ti_two(base, base);
 #pragma unroll
-                for (int g = 0; g < 4; g++) {                         // 16 keys at a time: 8 words of h, 8 of l
+                for (int g = 0; g < TI_XC / 16; g++) {                         // 16 keys at a time: 8 words of h, 8 of l
                     unsigned h[8], w[8];
-                    const float vr = I8 ? vfs[half * 4 + g] : 1.0f;
+                    const float vr = I8 ? vfs[part * (TI_XC / 16) + g] : 1.0f;
                     const ti_f2 f2 = ti_two(f[g], f[g]), vr2 = ti_two(vr, vr), minus = ti_two(-1.0f, -1.0f);
 #pragma unroll
                     for (int c = 0; c < 16; c += 2) {
@@ -452,8 +443,8 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
                         h[c / 2] = *(const unsigned*)&a2;
                         w[c / 2] = pt_pack(rest2.x, rest2.y);
                     }
-                    ti_store8(tmem + slot * 128 + lanes + half * 32 + g * 8, h);
-                    ti_store8(tmem + slot * 128 + lanes + 64 + half * 32 + g * 8, w);
+                    ti_store8(tmem + slot * 128 + lanes + part * (TI_XC / 2) + g * 8, h);
+                    ti_store8(tmem + slot * 128 + lanes + 64 + part * (TI_XC / 2) + g * 8, w);
                 }
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 pg_fence_before();
@@ -462,27 +453,47 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
             const float2 sums = ti_one(sum);
             l = fmaf(l, alpha, sums.x + sums.y);
             if (k > 0) add(k - 1);
-            alpha_prev = alpha; vref_prev = I8 ? sh.vref[k] : 1.0f;
+            alpha_prev = alpha; vref_prev = I8 ? sh.info[k].vref : 1.0f;
         }
         if (steps > 0) add(steps - 1);
-        float o4[TI_D / 2];
+        // values and factors that are not finite were left out: NaN for the rows that see them
+        unsigned long long lost = 0;
+#pragma unroll 1
+        for (int k = 0; k < steps; k++) {
+            const unsigned nan = sh.info[k].nan;
+            if (!(nan | (unsigned)sh.info[k].wild)) continue;
+            const int key0 = lo + k * TI_KEYS;
+#pragma unroll 1
+            for (int key = max(key0, key_lo); key <= min(key0 + TI_KEYS - 1, key_hi); key++) {
+                if (nan >> ((key - key0) >> 4) & 1u) lost = ~0ull;
+                if (I8 && key < opens) continue;
+                const __half* p = (I8 ? a.vo + ((size_t)(2 * s.slot + ((to >> a.shift) & 1)) * a.G + kvh) * a.page * a.dv
+                                      : (const __half*)a.v + ((size_t)a.table[(int64_t)seq * a.table_cols + (key >> a.shift)] * a.G + kvh) * a.page * a.dv) + (size_t)(key & (a.page - 1)) * a.dv + c_first;
+#pragma unroll 1
+                for (int c = 0; c < cols; c++)
+                    if (((unsigned)__half_as_ushort(p[c]) & 0x7c00u) == 0x7c00u) lost |= 1ull << c;
+            }
+        }
+        float o4[TI_OC];
 #pragma unroll
-        for (int c = 0; c < TI_D / 2; c += 2) {
+        for (int c = 0; c < TI_OC; c += 2) {
             const float2 u = ti_one(acc[c / 2]);
             o4[c] = lost >> c & 1u ? NAN : u.x;
             o4[c + 1] = lost >> (c + 1) & 1u ? NAN : u.y;
         }
-        sh.sum[half][row] = l;
+        sh.sum[part][row] = l;
         ti_soft_sync();
-        l = sh.sum[0][row] + sh.sum[1][row];
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < TI_SPLIT; i++) l += sh.sum[i][row];
         if (in && ok) {
             if (n_split > 1) {
-                const size_t at = ((size_t)blockIdx.x * a.G + kvh) * TI_ROWS + row;
+                const size_t at = ((size_t)blockIdx.x * a.heads + blockIdx.y) * TI_ROWS + row;
                 float* o = a.part + at * a.dv + c_first;
 #pragma unroll
-                for (int c = 0; c < TI_D / 2; c += 4)
+                for (int c = 0; c < TI_OC; c += 4)
                     if (c < cols) *(float4*)(o + c) = make_float4(o4[c], o4[c + 1], o4[c + 2], o4[c + 3]);
-                if (half == 0) a.ml[at] = make_float2(m, l);
+                if (part == 0) a.ml[at] = make_float2(m, l);
             } else {
                 float f = 1.0f;
                 if (a.sink) {
@@ -493,14 +504,14 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
                 float* o = a.out + ((int64_t)(s.first + tok) * a.H + head) * a.dv + c_first;
                 f = f / l;
 #pragma unroll
-                for (int c = 0; c < TI_D / 2; c += 4)
+                for (int c = 0; c < TI_OC; c += 4)
                     if (c < cols) *(float4*)(o + c) = make_float4(o4[c] * f, o4[c + 1] * f, o4[c + 2] * f, o4[c + 3] * f);
             }
         }
     }
     pg_fence_before();
     __syncthreads();
-    if (warp == 15) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
+    if (warp == (TI_SOFT_WARPS + 1)) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
     if (tid == 0 && sh.fail) {
         if (err_dev) atomicExch(err_dev, 5u);
         if (err_host) { *(volatile unsigned*)err_host = 5u; __threadfence_system(); }
