@@ -9,8 +9,8 @@
 //   P = exp2(S f - largest) as f16 h and l, written over S in TMEM, the first operand of
 //   O = P_h V + P_l V         in an accumulator of its own, added to 32-bit registers afterwards: the tensor core cuts its sums off at 24 bits, a chain over
 //                             thousands of keys would drift (1e-5 of a result after 2000 keys of one sign)
-// S and O have two buffers each (512 TMEM columns), K and V two stages (128 KB beside the 64 KB of Q): while 8 warps make the weights of one step, the tensor core
-// computes the scores of the next and the sums of the one before.
+// TMEM holds S twice, O, Q_h and Q_l (512 columns), shared memory two stages of K and V (128 KB): while 8 warps make the weights of one step, the tensor core computes the
+// scores of the next and the sums of the one before.  With Q in shared memory a step's products read 192 KB there and took 3100 cycles instead of 2050.
 // A row's 128 scores lie with two threads, a half each, which exchange their largest score once a step.  Warps 0-7 weights and sums, 8 the copies, 9 the products.
 // Every wait is bounded (sg_wait); where one ran out all roles run to their ends without waiting (the barrier of warps 0-7 included) and the host reports it.
 #pragma once
@@ -43,14 +43,16 @@ struct TiInfo {
     int pad;
 };
 struct TiShared {
-    unsigned long long k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], o_empty[2], drained;
+    unsigned long long k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full, drained;
     unsigned tmem_base;
     int fail;
     TiInfo info[TI_STEPS];
-    float top[2][TI_SPLIT][TI_ROWS], sum[TI_SPLIT][TI_ROWS];
+    float top[2][TI_SPLIT][TI_ROWS], sum[TI_SPLIT][TI_ROWS], inv[TI_ROWS];
 };
 #define TI_OPERAND (TI_KEYS * TI_D * 2)       // bytes of a tile of f16: two blocks of 64 columns, rows of 128 bytes under the 128-byte swizzle
 #define TI_SMEM (6 * TI_OPERAND + 1024)
+#define TI_O 256                              // TMEM columns: S and P at 0 and 128
+#define TI_Q 384
 #define TI_BLOCK (TI_OPERAND / 2)             // 64 columns of an operand; an image is as many as d has
 
 __device__ __forceinline__ unsigned ti_at(int row, int chunk) { return (unsigned)((chunk >> 3) * (TI_OPERAND / 2) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)); }
@@ -198,25 +200,31 @@ template <bool I8, bool CAP>
 __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_constant__ PtArgs a, unsigned* err_dev, unsigned* err_host) {
     extern __shared__ __align__(1024) uint8_t ti_raw[];
     __shared__ TiShared sh;
-    uint8_t* qs = (uint8_t*)(((uintptr_t)ti_raw + 1023) & ~(uintptr_t)1023);      // Q_h, Q_l
+    uint8_t* qs = (uint8_t*)(((uintptr_t)ti_raw + 1023) & ~(uintptr_t)1023);      // 64 KB on the way: queries into TMEM, results out
     uint8_t *ks = qs + 2 * TI_OPERAND, *vs = ks + 2 * TI_OPERAND;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = a.head0 + blockIdx.y;
     if (tid == 0) {
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             pg_mbar_init(pg_smem(&sh.k_full[i]), 1); pg_mbar_init(pg_smem(&sh.v_full[i]), 1); pg_mbar_init(pg_smem(&sh.k_empty[i]), 1); pg_mbar_init(pg_smem(&sh.v_empty[i]), 1);
-            pg_mbar_init(pg_smem(&sh.s_full[i]), 1); pg_mbar_init(pg_smem(&sh.p_full[i]), TI_SOFT_WARPS); pg_mbar_init(pg_smem(&sh.o_full[i]), 1); pg_mbar_init(pg_smem(&sh.o_empty[i]), TI_SOFT_WARPS);
-        }
+            pg_mbar_init(pg_smem(&sh.s_full[i]), 1); pg_mbar_init(pg_smem(&sh.p_full[i]), TI_SOFT_WARPS);         }
+        pg_mbar_init(pg_smem(&sh.o_full), 1);
         pg_mbar_init(pg_smem(&sh.drained), 1);
         sh.fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (warp == (TI_SOFT_WARPS + 1)) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pg_smem(&sh.tmem_base)), "n"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
     pdl_enter();
+    pg_fence_before();
     __syncthreads();
+    pg_fence_after();
+    const unsigned tmem = sh.tmem_base;
     int rest;
     const int seq = pt_find(a, blockIdx.x, [&](const PgSeq& s) { return pt_splits(s, a) * (int)(((int64_t)s.count * a.R + TI_ROWS - 1) / TI_ROWS); }, &rest);
-    if (seq < 0) return;                                              // (the grid has as many CTAs as there are items)
-    const PgSeq s = a.seqs[seq];
+    const PgSeq s = a.seqs[max(seq, 0)];                              // (the grid has as many CTAs as there are items)
     const int rows = s.count * a.R, tiles = (rows + TI_ROWS - 1) / TI_ROWS, n_split = pt_splits(s, a), tile = tiles - 1 - rest / n_split, split = rest % n_split;      // late rows, which see most, first
     int from, to;
     pt_range(s, a, &from, &to);
@@ -232,49 +240,60 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
         const int k = i / (int)(sizeof(TiInfo) / 4);
         ((int*)sh.info)[i] = ((const int*)(a.info + image + (size_t)k * a.heads))[i - k * (int)(sizeof(TiInfo) / 4)];
     }
-    if (warp == (TI_SOFT_WARPS + 1)) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pg_smem(&sh.tmem_base)), "n"(512) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
     // the queries as h and l, near 2^14
     const int row = (warp & 3) * 32 + lane, part = warp >> 2;         // of weights and sums: TMEM lane, part of the columns
     const int tok = (row0 + row) / a.R, head = kvh * a.R + (row0 + row) - tok * a.R;
     const bool in = warp < TI_SOFT_WARPS && row < n_rows;
-    float inv = 1.0f;
+    const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
+    const unsigned k_bytes = (unsigned)((a.dk + 63) / 64) * TI_BLOCK, v_bytes = (unsigned)((a.dv + 63) / 64) * TI_BLOCK;
+    auto copy = [&](uint8_t* to_smem, const uint8_t* src, unsigned bytes, unsigned bar) {
+        pg_mbar_expect_tx(bar, bytes);
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(pg_smem(to_smem)), "l"(src), "r"(bytes), "r"(bar) : "memory");
+    };
+    auto copy_k = [&](int k) { copy(ks + (size_t)(k & 1) * TI_OPERAND, a.k_image + (image + (size_t)k * a.heads) * k_bytes, k_bytes, pg_smem(&sh.k_full[k & 1])); };
+    auto copy_v = [&](int k) { copy(vs + (size_t)(k & 1) * TI_OPERAND, a.v_image + (image + (size_t)k * a.heads) * v_bytes, v_bytes, pg_smem(&sh.v_full[k & 1])); };
+    if (warp == TI_SOFT_WARPS && lane == 0)                           // the first images come while the queries are cut
+        for (int k = 0; k < min(steps, 2); k++) { copy_k(k); copy_v(k); }
     if (warp < TI_SOFT_WARPS) {
-        const float* q = a.q + ((int64_t)(s.first + tok) * a.H + head) * a.dk;
-        float top = 0.0f;
-        for (int c = part * 4; c < a.dk; c += 4 * TI_SPLIT) {
-            const float4 v = in ? *(const float4*)(q + c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-        }
-        sh.top[0][part][row] = top;
-        ti_soft_sync();
+        // a warp reads 16 rows, eight at a time; staged by rows of 512 bytes (h, then l; chunk j of 16 bytes at j ^ row % 8), then every thread stores its row's half to TMEM
+#pragma unroll 1
+        for (int r0 = warp * 16; r0 < warp * 16 + 16; r0 += 8) {
+            float4 v[8];
 #pragma unroll
-        for (int i = 0; i < TI_SPLIT; i++) top = fmaxf(top, sh.top[0][i][row]);
-        int ex = 14;
-        if (top > 0.0f && top < INFINITY) frexpf(top, &ex);
-        ex = max(ex, -100);
-        const float f = copysignf(ldexpf(1.0f, 14 - ex), a.scale);      // (so that a larger sum is a larger score)
-        inv = ldexpf(1.0f, ex - 14);
-        for (int j = part; j < a.dk / 8; j += TI_SPLIT) {
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 8; i += 4) {
-                const float4 u = in ? *(const float4*)(q + j * 8 + i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                v[i] = u.x * f; v[i + 1] = u.y * f; v[i + 2] = u.z * f; v[i + 3] = u.w * f;
+            for (int i = 0; i < 8; i++) {
+                const int r = r0 + i, tk = (row0 + r) / a.R, hd = kvh * a.R + (row0 + r) - tk * a.R;
+                v[i] = r < n_rows && lane * 4 < a.dk ? __ldg((const float4*)(a.q + ((int64_t)(s.first + tk) * a.H + hd) * a.dk) + lane) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             }
-            uint4 h, l;
-            pt_cut(v[0], v[1], h.x, l.x); pt_cut(v[2], v[3], h.y, l.y); pt_cut(v[4], v[5], h.z, l.z); pt_cut(v[6], v[7], h.w, l.w);
-            *(uint4*)(qs + ti_at(row, j)) = h;
-            *(uint4*)(qs + TI_OPERAND + ti_at(row, j)) = l;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int r = r0 + i;
+                const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)))));
+                // 2^(14 - e) for a largest number in [2^(e - 1), 2^e); zeros, subnormal and wild ones as they are
+                int ex = (int)(top >> 23) - 126;
+                if (top < 0x00800000u || top >= 0x7f800000u) ex = 14;
+                ex = max(ex, -100);
+                const float f = copysignf(__uint_as_float((unsigned)(14 - ex + 127) << 23), a.scale);      // (so that a larger sum is a larger score)
+                uint2 h, l;
+                pt_cut(v[i].x * f, v[i].y * f, h.x, l.x); pt_cut(v[i].z * f, v[i].w * f, h.y, l.y);
+                uint8_t* at = qs + r * 512 + (((lane >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8;
+                *(uint2*)at = h; *(uint2*)(at + 256) = l;
+                if (lane == 0) sh.inv[r] = __uint_as_float((unsigned)(ex - 14 + 127) << 23);
+            }
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        ti_soft_sync();
+#pragma unroll 1
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                const uint4 u = *(const uint4*)(qs + row * 512 + x * 256 + (((part * 8 + j) ^ (row & 7)) << 4)), w = *(const uint4*)(qs + row * 512 + x * 256 + (((part * 8 + j + 1) ^ (row & 7)) << 4));
+                const unsigned words[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+                ti_store8(tmem + lanes + TI_Q + x * 64 + part * 32 + j * 4, words);
+            }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
     }
     pg_fence_before();
     __syncthreads();
     pg_fence_after();
-    const unsigned tmem = sh.tmem_base;
 
     if (warp >= TI_SOFT_WARPS) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TI_REGS_REST));
@@ -282,17 +301,14 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
         // ===== products: one thread =====
         if (lane == 0) {
             const unsigned idesc_s = pg_instr_desc(128, TI_KEYS), idesc_o = pg_instr_desc(128, a.dv) | 1u << 16;
-            const unsigned qa = pg_smem(qs);
             bool ok = true;
             auto scores = [&](int k) {
                 const unsigned slot = k & 1, at = pg_smem(ks + (size_t)slot * TI_OPERAND);
                 if (!(ok = ti_wait(pg_smem(&sh.k_full[slot]), (k >> 1) & 1u, &sh.fail))) return;
                 pg_fence_after();
                 for (int x = 0; x < 2; x++)
-                    for (int kk = 0; kk < a.dk / 16; kk++) {
-                        const unsigned off = (unsigned)((kk >> 2) * (TI_OPERAND / 2) + (kk & 3) * 32);
-                        pg_umma_f16(tmem + slot * 128, pg_smem_desc(qa + x * TI_OPERAND + off), pg_smem_desc(at + off), idesc_s, x > 0 || kk > 0);
-                    }
+                    for (int kk = 0; kk < a.dk / 16; kk++)
+                        ti_umma_ts(tmem + slot * 128, tmem + TI_Q + x * 64 + kk * 8, pg_smem_desc(at + (unsigned)((kk >> 2) * TI_BLOCK + (kk & 3) * 32)), idesc_s, x > 0 || kk > 0);
                 pg_umma_commit(pg_smem(&sh.s_full[slot]));
                 pg_umma_commit(pg_smem(&sh.k_empty[slot]));
             };
@@ -300,14 +316,13 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
             for (int k = 0; k < steps && ok; k++) {
                 const unsigned slot = k & 1, ph = (k >> 1) & 1u;
                 if (k + 1 < steps) scores(k + 1);
-                if (!ok || !(ok = ti_wait(pg_smem(&sh.p_full[slot]), ph, &sh.fail) && ti_wait(pg_smem(&sh.v_full[slot]), ph, &sh.fail) &&
-                                  ti_wait(pg_smem(&sh.o_empty[slot]), ph ^ 1u, &sh.fail))) break;
+                if (!ok || !(ok = ti_wait(pg_smem(&sh.p_full[slot]), ph, &sh.fail) && ti_wait(pg_smem(&sh.v_full[slot]), ph, &sh.fail))) break;
                 pg_fence_after();
                 const unsigned at = pg_smem(vs + (size_t)slot * TI_OPERAND);
                 for (int x = 0; x < 2; x++)
                     for (int kk = 0; kk < TI_KEYS / 16; kk++)
-                        ti_umma_ts(tmem + 256 + slot * 128, tmem + slot * 128 + x * 64 + kk * 8, ti_desc_mn(at + kk * 2048), idesc_o, x > 0 || kk > 0);
-                pg_umma_commit(pg_smem(&sh.o_full[slot]));
+                        ti_umma_ts(tmem + TI_O, tmem + slot * 128 + x * 64 + kk * 8, ti_desc_mn(at + kk * 2048), idesc_o, x > 0 || kk > 0);
+                pg_umma_commit(pg_smem(&sh.o_full));
                 pg_umma_commit(pg_smem(&sh.v_empty[slot]));
             }
             int never = 0;                                            // nothing of this CTA is in flight when its TMEM is given back
@@ -318,19 +333,13 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
         } else if (warp == TI_SOFT_WARPS) {
         // ===== copies of the images: one thread =====
         if (lane == 0) {
-            const unsigned kb = (unsigned)((a.dk + 63) / 64) * TI_BLOCK, vb = (unsigned)((a.dv + 63) / 64) * TI_BLOCK;
-            auto copy = [&](uint8_t* to_smem, const uint8_t* src, unsigned bytes, unsigned bar) {
-                pg_mbar_expect_tx(bar, bytes);
-                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(pg_smem(to_smem)), "l"(src), "r"(bytes), "r"(bar) : "memory");
-            };
-            int k = 0, v = 0;                                         // copies begun
+            int k = min(steps, 2), v = k;                             // copies begun
             for (; k < steps; k++) {
                 const unsigned slot = k & 1, ph = ((k >> 1) & 1u) ^ 1u;
-                const size_t at = image + (size_t)k * a.heads;
                 if (!ti_wait(pg_smem(&sh.k_empty[slot]), ph, &sh.fail)) break;
-                copy(ks + (size_t)slot * TI_OPERAND, a.k_image + at * kb, kb, pg_smem(&sh.k_full[slot]));
+                copy_k(k);
                 if (!ti_wait(pg_smem(&sh.v_empty[slot]), ph, &sh.fail)) { k++; break; }
-                copy(vs + (size_t)slot * TI_OPERAND, a.v_image + at * vb, vb, pg_smem(&sh.v_full[slot]));
+                copy_v(k);
                 v++;
             }
             int never = 0;                                            // no copy is under way when the CTA ends
@@ -342,26 +351,24 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
     } else {
         // ===== weights and sums =====
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TI_REGS_SOFT));
-        const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
         const int width = (a.dv + 16 * TI_SPLIT - 1) / (16 * TI_SPLIT) * 16, c_first = part * width, cols = max(0, min(width, a.dv - c_first));      // this thread's columns of O
         const int pos = in ? s.pos0 + tok : -1, key_lo = a.window > 0 ? pos - a.window + 1 : 0, key_hi = min(pos, k1 - 1);      // the last step may reach into the next slice
-        const float f0 = inv * fabsf(a.scale) * (CAP ? 1.0f : PT_LOG2E);
+        const float f0 = sh.inv[row] * fabsf(a.scale) * (CAP ? 1.0f : PT_LOG2E);
         ti_f2 acc[TI_OC / 2];
         float m = -INFINITY, l = 0.0f, alpha_prev = 0.0f, vref_prev = 0.0f;
 #pragma unroll
         for (int i = 0; i < TI_OC / 2; i++) acc[i] = 0ull;
         bool ok = true;
         auto add = [&](int k) {                                       // the sums of step k
-            const unsigned slot = k & 1;
-            if (!(ok = ok && ti_wait_warp(pg_smem(&sh.o_full[slot]), (k >> 1) & 1u, &sh.fail))) return;
+            if (!(ok = ok && ti_wait_warp(pg_smem(&sh.o_full), k & 1, &sh.fail))) return;
             pg_fence_after();
             const ti_f2 alpha2 = ti_two(alpha_prev, alpha_prev), vref2 = ti_two(vref_prev, vref_prev);
 #pragma unroll
             for (int c = 0; c < TI_OC; c += 32) {
                 if (c >= cols) break;
                 unsigned v[32];
-                sg_tmem16(tmem + 256 + slot * 128 + lanes + c_first + c, *(unsigned(*)[16])v);
-                if (c + 16 < cols) sg_tmem16(tmem + 256 + slot * 128 + lanes + c_first + c + 16, *(unsigned(*)[16])(v + 16));
+                sg_tmem16(tmem + TI_O + lanes + c_first + c, *(unsigned(*)[16])v);
+                if (c + 16 < cols) sg_tmem16(tmem + TI_O + lanes + c_first + c + 16, *(unsigned(*)[16])(v + 16));
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
                 for (int i = 0; i < 32; i += 2) {
@@ -373,7 +380,6 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
                 }
             }
             pg_fence_before();
-            sg_arrive(pg_smem(&sh.o_empty[slot]));
         };
 #pragma unroll 1
         for (int k = 0; k < steps; k++) {
@@ -424,35 +430,40 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
             const float alpha = m == m_new ? 1.0f : ti_exp2(m - m_new);
             m = m_new;
             ti_f2 sum = 0ull;
-            if (ok) {
-                const ti_f2 base2 = ti_two(base, base);
+            const ti_f2 base2 = ti_two(base, base), minus = ti_two(-1.0f, -1.0f);
+            auto weights = [&](int g) {                               // of 16 keys: 8 words of h, 8 of l
+                unsigned h[8], w[8];
+                const float vr = I8 ? vfs[part * (TI_XC / 16) + g] : 1.0f;
+                const ti_f2 f2 = ti_two(f[g], f[g]), vr2 = ti_two(vr, vr);
 #pragma unroll
-                for (int g = 0; g < TI_XC / 16; g++) {                         // 16 keys at a time: 8 words of h, 8 of l
-                    unsigned h[8], w[8];
-                    const float vr = I8 ? vfs[part * (TI_XC / 16) + g] : 1.0f;
-                    const ti_f2 f2 = ti_two(f[g], f[g]), vr2 = ti_two(vr, vr), minus = ti_two(-1.0f, -1.0f);
-#pragma unroll
-                    for (int c = 0; c < 16; c += 2) {
-                        const float2 y = ti_one(ti_fma2(ti_two(__uint_as_float(x[g * 16 + c]), __uint_as_float(x[g * 16 + c + 1])), f2, base2));
-                        ti_f2 p = ti_two(ti_exp2(y.x), ti_exp2(y.y));
-                        sum = ti_add2(sum, p);
-                        if (I8) p = ti_mul2(p, vr2);
-                        const float2 q = ti_one(p);
-                        const __half2 a2 = __floats2half2_rn(q.x, q.y);
-                        const float2 b2 = __half22float2(a2), rest2 = ti_one(ti_fma2(ti_two(b2.x, b2.y), minus, p));
-                        h[c / 2] = *(const unsigned*)&a2;
-                        w[c / 2] = pt_pack(rest2.x, rest2.y);
-                    }
-                    ti_store8(tmem + slot * 128 + lanes + part * (TI_XC / 2) + g * 8, h);
-                    ti_store8(tmem + slot * 128 + lanes + 64 + part * (TI_XC / 2) + g * 8, w);
+                for (int c = 0; c < 16; c += 2) {
+                    const float2 y = ti_one(ti_fma2(ti_two(__uint_as_float(x[g * 16 + c]), __uint_as_float(x[g * 16 + c + 1])), f2, base2));
+                    ti_f2 p = ti_two(ti_exp2(y.x), ti_exp2(y.y));
+                    sum = ti_add2(sum, p);
+                    if (I8) p = ti_mul2(p, vr2);
+                    const float2 q = ti_one(p);
+                    const __half2 a2 = __floats2half2_rn(q.x, q.y);
+                    const float2 b2 = __half22float2(a2), rest2 = ti_one(ti_fma2(ti_two(b2.x, b2.y), minus, p));
+                    h[c / 2] = *(const unsigned*)&a2;
+                    w[c / 2] = pt_pack(rest2.x, rest2.y);
                 }
+                ti_store8(tmem + slot * 128 + lanes + part * (TI_XC / 2) + g * 8, h);
+                ti_store8(tmem + slot * 128 + lanes + 64 + part * (TI_XC / 2) + g * 8, w);
+            };
+            if (ok) {
+#pragma unroll
+                for (int g = 0; g < TI_XC / 32; g++) weights(g);
+            }
+            if (k > 0) add(k - 1);                                    // by now its products are done, and those of this step wait for the room
+            if (ok) {
+#pragma unroll
+                for (int g = TI_XC / 32; g < TI_XC / 16; g++) weights(g);
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 pg_fence_before();
                 sg_arrive(pg_smem(&sh.p_full[slot]));
             }
             const float2 sums = ti_one(sum);
             l = fmaf(l, alpha, sums.x + sums.y);
-            if (k > 0) add(k - 1);
             alpha_prev = alpha; vref_prev = I8 ? sh.info[k].vref : 1.0f;
         }
         if (steps > 0) add(steps - 1);
@@ -486,27 +497,27 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
         l = 0.0f;
 #pragma unroll
         for (int i = 0; i < TI_SPLIT; i++) l += sh.sum[i][row];
-        if (in && ok) {
-            if (n_split > 1) {
-                const size_t at = ((size_t)blockIdx.x * a.heads + blockIdx.y) * TI_ROWS + row;
-                float* o = a.part + at * a.dv + c_first;
-#pragma unroll
-                for (int c = 0; c < TI_OC; c += 4)
-                    if (c < cols) *(float4*)(o + c) = make_float4(o4[c], o4[c + 1], o4[c + 2], o4[c + 3]);
-                if (part == 0) a.ml[at] = make_float2(m, l);
-            } else {
-                float f = 1.0f;
-                if (a.sink) {
-                    const float sk = a.sink[head] * PT_LOG2E, m2 = fmaxf(m, sk);
-                    f = m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : exp2f(m - m2);
-                    l = f * l + (sk == -INFINITY ? 0.0f : exp2f(sk - m2 + PT_SHIFT));
-                }
-                float* o = a.out + ((int64_t)(s.first + tok) * a.H + head) * a.dv + c_first;
-                f = f / l;
-#pragma unroll
-                for (int c = 0; c < TI_OC; c += 4)
-                    if (c < cols) *(float4*)(o + c) = make_float4(o4[c] * f, o4[c + 1] * f, o4[c + 2] * f, o4[c + 3] * f);
+        float f = 1.0f;
+        const size_t at = ((size_t)blockIdx.x * a.heads + blockIdx.y) * TI_ROWS;
+        if (n_split > 1) {
+            if (in && part == 0) a.ml[at + row] = make_float2(m, l);
+        } else {
+            if (a.sink && in) {
+                const float sk = a.sink[head] * PT_LOG2E, m2 = fmaxf(m, sk);
+                f = m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : exp2f(m - m2);
+                l = f * l + (sk == -INFINITY ? 0.0f : exp2f(sk - m2 + PT_SHIFT));
             }
+            f = f / l;
+        }
+        // by way of shared memory, 16 bytes j of a row at j ^ row % 8, so that whole rows are stored at a time
+#pragma unroll
+        for (int c = 0; c < TI_OC; c += 4)
+            if (c < cols) *(float4*)(qs + row * 512 + ((((c_first + c) >> 2) ^ (row & 7)) << 4)) = make_float4(o4[c] * f, o4[c + 1] * f, o4[c + 2] * f, o4[c + 3] * f);
+        ti_soft_sync();
+        for (int r = warp; r < n_rows && ok; r += TI_SOFT_WARPS) {
+            const int tk = (row0 + r) / a.R, hd = kvh * a.R + (row0 + r) - tk * a.R;
+            float* o = n_split > 1 ? a.part + (at + r) * a.dv : a.out + ((int64_t)(s.first + tk) * a.H + hd) * a.dv;
+            if (lane * 4 < a.dv) ((float4*)o)[lane] = *(const float4*)(qs + r * 512 + ((lane ^ (r & 7)) << 4));
         }
     }
     pg_fence_before();
