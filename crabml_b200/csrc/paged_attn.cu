@@ -540,7 +540,7 @@ static int pt_run(cc_device* dev, const cc_page_plan* plan, PtArgs a, bool i8) {
         items += (int64_t)n * (((int64_t)s.count * a.R + a.tile_rows - 1) / a.tile_rows);
         if (n > 1) split_rows += (int64_t)s.count * a.R;
     }
-    CC_REQUIRE(dev, items < ((int64_t)1 << 31) && split_rows < ((int64_t)1 << 31) && key_tiles < ((int64_t)1 << 31), "paged_attention: too many rows");
+    CC_REQUIRE(dev, items * a.G < ((int64_t)1 << 31) && split_rows < ((int64_t)1 << 31) && key_tiles < ((int64_t)1 << 31), "paged_attention: too many rows");
     const size_t kb = (size_t)((a.dk + 63) / 64) * TI_BLOCK, vb = (size_t)((a.dv + 63) / 64) * TI_BLOCK, per_head = few ? 0 : (size_t)key_tiles * (kb + vb + sizeof(TiInfo));
     a.heads = few || (int64_t)per_head * a.G <= TI_WORKSPACE ? a.G : (int)std::max<int64_t>(1, TI_WORKSPACE / (int64_t)per_head);
     const size_t part = split_rows ? (size_t)items * a.heads * a.tile_rows * a.dv * sizeof(float) : 0, ml = split_rows ? (size_t)items * a.heads * a.tile_rows * sizeof(float2) : 0;
@@ -564,7 +564,7 @@ static int pt_run(cc_device* dev, const cc_page_plan* plan, PtArgs a, bool i8) {
             auto kernel = i8 ? (cap ? paged_tile_kernel<true, true> : paged_tile_kernel<true, false>) : (cap ? paged_tile_kernel<false, true> : paged_tile_kernel<false, false>);
             e = cc_launch_pdl(dev, i8 ? paged_unpack_kernel<true> : paged_unpack_kernel<false>, dim3((unsigned)key_tiles, (unsigned)a.heads), TU_THREADS, 0, a);
             if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TI_SMEM);
-            if (e == cudaSuccess) e = cc_launch_pdl(dev, kernel, dim3((unsigned)items, (unsigned)a.heads), TI_THREADS, TI_SMEM, a, dev->err_dev, dev->err_host);
+            if (e == cudaSuccess) e = cc_launch_pdl(dev, kernel, (unsigned)(items * a.heads), TI_THREADS, TI_SMEM, a, dev->err_dev, dev->err_host);
             dev->launches += 2;
         }
         if (e == cudaSuccess && split_rows) {

@@ -39,8 +39,7 @@ struct TiInfo {
     float kf[TI_KEYS / 16], vf[TI_KEYS / 16]; // factors of 16 keys each; vf relative to vref, a power of two near the largest
     float vref;
     int wild;                                 // values that are not finite are zeros in the image
-    unsigned nan;                             // groups of 16 keys with a factor that is not finite (it counts as 0)
-    int pad;
+    unsigned bad[TI_KEYS / 32];               // keys whose factors or numbers are not finite (they count as 0): NaN for the rows that see one
 };
 struct TiShared {
     unsigned long long k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full, drained;
@@ -51,6 +50,7 @@ struct TiShared {
 };
 #define TI_OPERAND (TI_KEYS * TI_D * 2)       // bytes of a tile of f16: two blocks of 64 columns, rows of 128 bytes under the 128-byte swizzle
 #define TI_SMEM (6 * TI_OPERAND + 1024)
+#define TI_SFU 10                             // of 16 weights those that the special function unit makes
 #define TI_O 256                              // TMEM columns: S and P at 0 and 128
 #define TI_Q 384
 #define TI_BLOCK (TI_OPERAND / 2)             // 64 columns of an operand; an image is as many as d has
@@ -86,6 +86,8 @@ __device__ __forceinline__ float ti_exp2(float x) {
 }
 // pairs of 32-bit numbers in one instruction
 typedef unsigned long long ti_f2;
+__device__ __forceinline__ ti_f2 ti_fma2(ti_f2 a, ti_f2 b, ti_f2 c);
+__device__ __forceinline__ ti_f2 ti_add2(ti_f2 a, ti_f2 b);
 __device__ __forceinline__ ti_f2 ti_two(float x, float y) {
     ti_f2 r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
@@ -110,6 +112,21 @@ __device__ __forceinline__ ti_f2 ti_add2(ti_f2 a, ti_f2 b) {
     ti_f2 r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
+}
+// 2^x of a pair by multiply-adds: the special function unit makes 4 results a cycle and scheduler, which alone would take half of a step.  x = n + r with |r| <= 1/2 by way
+// of a number whose last place is 1; 2^r by its series up to r^6 (the rest is below 2^-22 r^7 / 5040 (ln 2)^7 < 2^-24); n goes into the exponent.  x >= -126 here
+__device__ __forceinline__ ti_f2 ti_exp2_two(float2 x) {
+    const ti_f2 big = ti_two(12582912.0f, 12582912.0f), minus = ti_two(-1.0f, -1.0f);
+    const ti_f2 v = ti_two(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f)), t = ti_add2(v, big), n = ti_add2(t, ti_two(-12582912.0f, -12582912.0f)), r = ti_fma2(n, minus, v);
+    ti_f2 p = ti_two(1.5403530e-4f, 1.5403530e-4f);                  // (ln 2)^i / i!, i = 6 .. 0
+    p = ti_fma2(p, r, ti_two(1.3333558e-3f, 1.3333558e-3f));
+    p = ti_fma2(p, r, ti_two(9.6181291e-3f, 9.6181291e-3f));
+    p = ti_fma2(p, r, ti_two(5.5504109e-2f, 5.5504109e-2f));
+    p = ti_fma2(p, r, ti_two(2.4022651e-1f, 2.4022651e-1f));
+    p = ti_fma2(p, r, ti_two(6.9314718e-1f, 6.9314718e-1f));
+    p = ti_fma2(p, r, ti_two(1.0f, 1.0f));
+    const float2 q = ti_one(p), m = ti_one(t);
+    return ti_two(__uint_as_float(__float_as_uint(q.x) + (__float_as_uint(m.x) << 23)), __uint_as_float(__float_as_uint(q.y) + (__float_as_uint(m.y) << 23)));
 }
 __device__ __forceinline__ float ti_max3(float a, float b, float c) {
     float r;
@@ -152,9 +169,10 @@ __global__ void __launch_bounds__(TU_THREADS) paged_unpack_kernel(const PtArgs a
         const bool bad = !(vf >= 0.0f && vf < INFINITY && kf >= 0.0f && kf < INFINITY);
         if (bad) kf = vf = 0.0f;
         const float vmax = warp_max(vf), vref = fminf(fmaxf(__uint_as_float(__float_as_uint(vmax) & 0x7f800000u), 0x1p-100f), 0x1p100f);
-        const unsigned nan = __ballot_sync(0xffffffffu, bad) & 0xffu;
+        const unsigned nan = __ballot_sync(0xffffffffu, bad) >> 2 * (tid & 3);      // the lanes' groups repeat after 8
         if (tid < TI_KEYS / 16) { pages[tid] = page; info.kf[tid] = kf; info.vf[tid] = vf / vref; }
-        if (tid == 0) { info.vref = vref; info.nan = nan; info.pad = 0; }
+        if (tid < TI_KEYS / 32) info.bad[tid] = (nan & 1u ? 0xffffu : 0u) | (nan & 2u ? 0xffff0000u : 0u);
+        if (tid == 0) info.vref = vref;
     }
     __syncthreads();
     const size_t at = (size_t)blockIdx.x * a.heads + blockIdx.y;
@@ -176,15 +194,15 @@ __global__ void __launch_bounds__(TU_THREADS) paged_unpack_kernel(const PtArgs a
             } else if (key < to) {
                 const __half* p = I8 ? (v ? a.vo : a.ko) + (((size_t)open * a.G + kvh) * a.page + row) * d : (const __half*)(v ? a.v : a.k) + (((size_t)page * a.G + kvh) * a.page + row) * d;
                 x = __ldg((const uint4*)p + 2 * piece); y = __ldg((const uint4*)p + 2 * piece + 1);
-                if (v) {
-                    unsigned* u[8] = {&x.x, &x.y, &x.z, &x.w, &y.x, &y.y, &y.z, &y.w};
+                unsigned* u[8] = {&x.x, &x.y, &x.z, &x.w, &y.x, &y.y, &y.z, &y.w}, any = 0;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const unsigned w = pt_wild(*u[i]);
-                        wild |= w != 0u;
-                        *u[i] &= ~w;
-                    }
+                for (int i = 0; i < 8; i++) {
+                    const unsigned w = pt_wild(*u[i]);
+                    any |= w;
+                    *u[i] &= ~w;
                 }
+                if (any && v) wild = true;
+                if (any && !v) atomicOr(&info.bad[r >> 5], 1u << (r & 31));
             }
             *(uint4*)(image + ti_at(r, 2 * piece)) = x;
             *(uint4*)(image + ti_at(r, 2 * piece + 1)) = y;
@@ -202,7 +220,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
     __shared__ TiShared sh;
     uint8_t* qs = (uint8_t*)(((uintptr_t)ti_raw + 1023) & ~(uintptr_t)1023);      // 64 KB on the way: queries into TMEM, results out
     uint8_t *ks = qs + 2 * TI_OPERAND, *vs = ks + 2 * TI_OPERAND;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = a.head0 + blockIdx.y;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, item = (int)(blockIdx.x / (unsigned)a.heads), head_at = (int)(blockIdx.x - (unsigned)item * a.heads), kvh = a.head0 + head_at;      // heads fastest: the items that see most come first
     if (tid == 0) {
 #pragma unroll
         for (int i = 0; i < 2; i++) {
@@ -223,7 +241,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
     pg_fence_after();
     const unsigned tmem = sh.tmem_base;
     int rest;
-    const int seq = pt_find(a, blockIdx.x, [&](const PgSeq& s) { return pt_splits(s, a) * (int)(((int64_t)s.count * a.R + TI_ROWS - 1) / TI_ROWS); }, &rest);
+    const int seq = pt_find(a, item, [&](const PgSeq& s) { return pt_splits(s, a) * (int)(((int64_t)s.count * a.R + TI_ROWS - 1) / TI_ROWS); }, &rest);
     const PgSeq s = a.seqs[max(seq, 0)];                              // (the grid has as many CTAs as there are items)
     const int rows = s.count * a.R, tiles = (rows + TI_ROWS - 1) / TI_ROWS, n_split = pt_splits(s, a), tile = tiles - 1 - rest / n_split, split = rest % n_split;      // late rows, which see most, first
     int from, to;
@@ -235,7 +253,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
     // the images of the first step, and what stands beside those of all steps
     int before = 0;
     for (int x = lane; x < seq; x += 32) before += ti_key_tiles(a.seqs[x], a);
-    const size_t image = (size_t)(warp_sum_i(before) + (lo - from) / TI_KEYS) * a.heads + blockIdx.y;
+    const size_t image = (size_t)(warp_sum_i(before) + (lo - from) / TI_KEYS) * a.heads + head_at;
     for (int i = tid; i < steps * (int)(sizeof(TiInfo) / 4); i += TI_THREADS) {
         const int k = i / (int)(sizeof(TiInfo) / 4);
         ((int*)sh.info)[i] = ((const int*)(a.info + image + (size_t)k * a.heads))[i - k * (int)(sizeof(TiInfo) / 4)];
@@ -438,7 +456,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
 #pragma unroll
                 for (int c = 0; c < 16; c += 2) {
                     const float2 y = ti_one(ti_fma2(ti_two(__uint_as_float(x[g * 16 + c]), __uint_as_float(x[g * 16 + c + 1])), f2, base2));
-                    ti_f2 p = ti_two(ti_exp2(y.x), ti_exp2(y.y));
+                    ti_f2 p = c % 16 >= TI_SFU ? ti_exp2_two(y) : ti_two(ti_exp2(y.x), ti_exp2(y.y));
                     sum = ti_add2(sum, p);
                     if (I8) p = ti_mul2(p, vr2);
                     const float2 q = ti_one(p);
@@ -471,12 +489,12 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
         unsigned long long lost = 0;
 #pragma unroll 1
         for (int k = 0; k < steps; k++) {
-            const unsigned nan = sh.info[k].nan;
-            if (!(nan | (unsigned)sh.info[k].wild)) continue;
+            const unsigned* bad = sh.info[k].bad;
+            if (!(bad[0] | bad[1] | bad[2] | bad[3] | (unsigned)sh.info[k].wild)) continue;
             const int key0 = lo + k * TI_KEYS;
 #pragma unroll 1
             for (int key = max(key0, key_lo); key <= min(key0 + TI_KEYS - 1, key_hi); key++) {
-                if (nan >> ((key - key0) >> 4) & 1u) lost = ~0ull;
+                if (bad[(key - key0) >> 5] >> ((key - key0) & 31) & 1u) lost = ~0ull;
                 if (I8 && key < opens) continue;
                 const __half* p = (I8 ? a.vo + ((size_t)(2 * s.slot + ((to >> a.shift) & 1)) * a.G + kvh) * a.page * a.dv
                                       : (const __half*)a.v + ((size_t)a.table[(int64_t)seq * a.table_cols + (key >> a.shift)] * a.G + kvh) * a.page * a.dv) + (size_t)(key & (a.page - 1)) * a.dv + c_first;
@@ -498,7 +516,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
 #pragma unroll
         for (int i = 0; i < TI_SPLIT; i++) l += sh.sum[i][row];
         float f = 1.0f;
-        const size_t at = ((size_t)blockIdx.x * a.heads + blockIdx.y) * TI_ROWS;
+        const size_t at = ((size_t)item * a.heads + head_at) * TI_ROWS;
         if (n_split > 1) {
             if (in && part == 0) a.ml[at + row] = make_float2(m, l);
         } else {
