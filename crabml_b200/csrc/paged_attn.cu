@@ -1,7 +1,7 @@
 // paged_attn.cu -- attention over the pages of a cache (include/crabml_paged.h).
 //
 // 32-bit results from 16-bit tensor-core products.  Codes and 16-bit numbers are exact as f16 operands; a query or weight x is two of them, h = f16(x) and
-// l = f16(x - h), 22 bits together.  A query row is first brought near 2^14 by a power of two, weights are at most 2^12, so that l keeps its bits.
+// l = f16(x - h), 22 bits together.  A query row is first brought near 2^14 by a power of two, weights go up to 2^15, so that l keeps its bits.
 //
 // Few rows (paged_few_kernel; a row is a query of one head).  mma.sync.m16n8k16 has room for 16 rows: eight rows' h above, the same rows' l below, and both
 // products are one instruction whose accumulators a thread adds up itself.  A warp takes 16 keys at a time.  Its lanes keep, read and convert the pieces of the
@@ -15,9 +15,11 @@
 
 #define PT_WARPS 4
 #define PT_THREADS (PT_WARPS * 32)
-#define PT_SHIFT 12.0f                        // weights are exp2(score - largest + PT_SHIFT)
+#define PT_SHIFT 9.0f                         // weights are exp2(score - base + PT_SHIFT), base the largest score so far, or up to PT_LAG less: weights stay below 2^15, and the sums
+#define PT_LAG 6.0f                           // of a row are not scaled again for every score that is a little larger
 #define PT_MOST_SPLIT 2048                    // keys of a slice
 #define PT_FEW 32
+#define PT_TILE 72
 #define PT_LOG2E 1.4426950408889634f
 
 struct TiInfo;
@@ -49,6 +51,11 @@ __host__ __device__ __forceinline__ int pt_splits(const PgSeq& s, const PtArgs& 
     int from, to;
     pt_range(s, a, &from, &to);
     return (to - from + a.split - 1) / a.split;
+}
+// keys of a slice: the sequence's in equal parts, whole steps of 64 (few rows) or of TI_KEYS
+__host__ __device__ __forceinline__ int pt_each(int keys, int n_split, const PtArgs& a) {
+    const int step = a.tile_rows == 8 ? 64 : 128;
+    return ((keys + n_split - 1) / n_split + step - 1) / step * step;
 }
 // the place of number n in the sequences' counts: every lane gets the sequence and what is left of n
 template <class Count>
@@ -93,6 +100,12 @@ __device__ __forceinline__ unsigned pt_pack(float x, float y) {
     const __half2 h = __floats2half2_rn(x, y);
     return *(const unsigned*)&h;
 }
+// 2^x; what is below 2^-126 is 0
+__device__ __forceinline__ float pt_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // x, y as f16 (h) and what is left of them as f16 (l)
 __device__ __forceinline__ void pt_cut(float x, float y, unsigned& h, unsigned& l) {
     const __half2 a = __floats2half2_rn(x, y);
@@ -110,7 +123,7 @@ template <int D>
 struct PtRows {
     unsigned q[D / 16][4];                    // h and l of the lane's columns, as the instruction takes them
     float o[D / 8][4];                        // sums of weighted values: tile i, columns 2 t and 2 t + 1 of its eight, rows h and l
-    float inv, m, l, vref, ivref;             // power of two that q was divided by; largest score so far; the lane's sum of weights; power of two at the largest value factor so far
+    float inv, m, l, vref, ivref;             // power of two that q was divided by; base of the weights; the lane's sum of weights; power of two at the largest value factor so far
     int pos, lo;                              // the row's position and the first key it sees (pos -1: no row)
 };
 // 16 scores of the row -> weights; x: raw sums of keys 2 t, 2 t + 1, 8 + 2 t, 9 + 2 t.  kf, vf: the keys' and values' factors.  edge: some row does not see some key
@@ -136,25 +149,26 @@ __device__ __forceinline__ void pt_weights(PtRows<D>& r, float (&x)[4], int key0
     float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    const float m = fmaxf(r.m, mx);
     // the largest value factor so far, as the power of two below it: a block that the row does not see leaves its bits as they are
     const float vp = fminf(fmaxf(__uint_as_float(__float_as_uint(vf) & 0x7f800000u), 0x1p-100f), 0x1p100f);
-    const bool up = m > r.m, wider = vp > r.vref && vf > 0.0f;
+    const bool up = mx > r.m + PT_LAG, wider = vp > r.vref && vf > 0.0f;      // (r.m -inf: every score is more)
     if (__any_sync(0xffffffffu, up || wider)) {
-        float alpha = r.m == -INFINITY ? 0.0f : exp2f(r.m - m);
-        if (m == r.m) alpha = 1.0f;
+        float alpha = 1.0f;
+        if (up) {
+            alpha = r.m == -INFINITY ? 0.0f : pt_exp2(r.m - mx);
+            r.m = mx;
+        }
         r.l *= alpha;
         if (wider) {
             alpha *= r.vref / vp;
             r.vref = vp; r.ivref = 1.0f / vp;
         }
-        r.m = m;
 #pragma unroll
         for (int i = 0; i < D / 8; i++) { r.o[i][0] *= alpha; r.o[i][1] *= alpha; r.o[i][2] *= alpha; r.o[i][3] *= alpha; }
     }
-    const float base = m == -INFINITY ? 0.0f : m - PT_SHIFT, vr = vf * r.ivref;
+    const float base = r.m == -INFINITY ? 0.0f : PT_SHIFT - r.m, vr = vf * r.ivref;
 #pragma unroll
-    for (int i = 0; i < 4; i++) x[i] = exp2f(x[i] - base);
+    for (int i = 0; i < 4; i++) x[i] = pt_exp2(x[i] + base);
     r.l += (x[0] + x[1]) + (x[2] + x[3]);
 #pragma unroll
     for (int i = 0; i < 4; i++) x[i] = seen & (1u << i) ? x[i] * vr : 0.0f;
@@ -317,7 +331,7 @@ struct PtF16 {
 };
 
 template <int D, bool I8>
-__global__ void __launch_bounds__(PT_THREADS) paged_few_kernel(const PtArgs a) {
+__global__ void __launch_bounds__(PT_THREADS, D <= 64 ? 4 : D <= 128 ? 3 : 1) paged_few_kernel(const PtArgs a) {
     using Mine = PtF16<D, I8>;                                     // 16-bit rows: pages, or the open block beside codes
     constexpr int RING = 128 * D, STAGES = RING / Mine::BYTES, STAGES8 = RING / PtI8<D>::BYTES, CW = I8 && D >= 128 ? 128 : 64;
     extern __shared__ __align__(16) uint8_t pt_sm[];
@@ -336,14 +350,38 @@ __global__ void __launch_bounds__(PT_THREADS) paged_few_kernel(const PtArgs a) {
     int from, to;
     pt_range(s, a, &from, &to);
     const int row = tile * 8 + g, tok = row / a.R, pos_first = s.pos0 + tile * 8 / a.R, pos_last = s.pos0 + (min(rows, tile * 8 + 8) - 1) / a.R;
-    const int k0 = from + split * a.split, k1 = min(min(to, k0 + a.split), pos_last + 1);       // keys of the slice that some row of the tile may see
+    const int each = pt_each(to - from, n_split, a), k0 = from + split * each, k1 = min(min(to, k0 + each), pos_last + 1);       // keys of the slice that some row of the tile may see
     const int lo = a.window > 0 ? max(k0, (pos_first - a.window + 1) & ~15) : k0, units = k1 > lo ? (k1 - lo + 15) >> 4 : 0;
     const int p0 = lo >> a.shift, opens = I8 ? to >> a.shift << a.shift : 0;                  // the first key that is not in a page of codes
-    for (int i = threadIdx.x; units > 0 && i <= ((k1 - 1) >> a.shift) - p0; i += PT_THREADS) {
-        const int page = a.table[(int64_t)seq * a.table_cols + p0 + i];
-        pid[i] = page;
-        if (I8) { kfs[i] = a.ks[(int64_t)page * a.G + kvh]; vfs[i] = a.vs[(int64_t)page * a.G + kvh]; }
-    }
+    const int n_pages = units > 0 ? ((k1 - 1) >> a.shift) - p0 + 1 : 0, units8 = I8 ? max(0, min(units, (opens - lo) >> 4)) : 0;
+    for (int i = threadIdx.x; i < n_pages; i += PT_THREADS) pid[i] = a.table[(int64_t)seq * a.table_cols + p0 + i];
+    __syncthreads();
+    // 16 keys' rows on their way into a place of the ring: codes, and 16-bit rows (`first` on: this warp's units behind the codes)
+    auto load8 = [&](int u) {
+        if (I8 && u < units8) {
+            const int key0 = lo + u * 16;
+            const size_t at = ((size_t)pid[(key0 >> a.shift) - p0] * a.G + kvh) * a.page + (key0 & (a.page - 1));
+            PtI8<D>::load(ring_at + (u / PT_WARPS % STAGES8) * PtI8<D>::BYTES, a.k + at * a.dk, a.v + at * a.dv, a);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    const __half *kb = I8 ? a.ko : (const __half*)a.k, *vb = I8 ? a.vo : (const __half*)a.v;
+    auto load16 = [&](int u) {
+        if (u < units) {
+            const int key0 = lo + u * 16;
+            const size_t block = I8 ? (size_t)(2 * s.slot + ((to >> a.shift) & 1)) : (size_t)pid[(key0 >> a.shift) - p0], at = (block * a.G + kvh) * a.page + (key0 & (a.page - 1));
+            Mine::load(ring_at + (u / PT_WARPS % STAGES) * Mine::BYTES, kb + at * a.dk, vb + at * a.dv, to - key0, a);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    const int first = units8 + (w - units8 % PT_WARPS + PT_WARPS) % PT_WARPS;
+    // the first of them come while the factors are read and the queries cut
+    if (I8) {
+#pragma unroll
+        for (int i = 0; i < STAGES8 - 1; i++) load8(w + i * PT_WARPS);
+    } else load16(first);
+    if (I8)
+        for (int i = threadIdx.x; i < n_pages; i += PT_THREADS) { kfs[i] = a.ks[(int64_t)pid[i] * a.G + kvh]; vfs[i] = a.vs[(int64_t)pid[i] * a.G + kvh]; }
     PtRows<D> r;
     {                                                              // the lane's columns of its row
         const bool in = row < rows;
@@ -375,65 +413,40 @@ __global__ void __launch_bounds__(PT_THREADS) paged_few_kernel(const PtArgs a) {
         for (int i = 0; i < D / 8; i++) r.o[i][0] = r.o[i][1] = r.o[i][2] = r.o[i][3] = 0.0f;
     }
     __syncthreads();
-    const int units8 = I8 ? max(0, min(units, (opens - lo) >> 4)) : 0;
     auto edge = [&](int key0) { return key0 + 15 > pos_first || (a.window > 0 && key0 < pos_last - a.window + 1); };
     if constexpr (I8) {
-        auto load = [&](int u) {
-            if (u < units8) {
-                const int key0 = lo + u * 16, i = (key0 >> a.shift) - p0;
-                const size_t at = ((size_t)pid[i] * a.G + kvh) * a.page + (key0 & (a.page - 1));
-                PtI8<D>::load(ring_at + (u / PT_WARPS % STAGES8) * PtI8<D>::BYTES, a.k + at * a.dk, a.v + at * a.dv, a);
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
-#pragma unroll
-        for (int i = 0; i < STAGES8 - 1; i++) load(w + i * PT_WARPS);
         for (int u = w; u < units8; u += PT_WARPS) {
             asm volatile("cp.async.wait_group %0;" ::"n"(STAGES8 - 2) : "memory");
-            load(u + (STAGES8 - 1) * PT_WARPS);
+            load8(u + (STAGES8 - 1) * PT_WARPS);
             const int key0 = lo + u * 16, i = (key0 >> a.shift) - p0;
             PtI8<D>::use(r, ring + (u / PT_WARPS % STAGES8) * PtI8<D>::BYTES, key0, kfs[i], vfs[i], edge(key0), a);
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
+        load16(first);
     }
-    {
-        const __half *kb = I8 ? a.ko : (const __half*)a.k, *vb = I8 ? a.vo : (const __half*)a.v;
-        auto load = [&](int u) {
-            if (u < units) {
-                const int key0 = lo + u * 16, i = (key0 >> a.shift) - p0;
-                const size_t block = I8 ? (size_t)(2 * s.slot + ((to >> a.shift) & 1)) : (size_t)pid[i], at = (block * a.G + kvh) * a.page + (key0 & (a.page - 1));
-                Mine::load(ring_at + (u / PT_WARPS % STAGES) * Mine::BYTES, kb + at * a.dk, vb + at * a.dv, to - key0, a);
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
-        const int first = units8 + (w - units8 % PT_WARPS + PT_WARPS) % PT_WARPS;             // this warp's first unit behind the codes
-        load(first);
-        for (int u = first; u < units; u += PT_WARPS) {
-            load(u + PT_WARPS);
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-            const int key0 = lo + u * 16;
-            Mine::use(r, ring + (u / PT_WARPS % STAGES) * Mine::BYTES, key0, edge(key0), a);
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
+    for (int u = first; u < units; u += PT_WARPS) {
+        load16(u + PT_WARPS);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        const int key0 = lo + u * 16;
+        Mine::use(r, ring + (u / PT_WARPS % STAGES) * Mine::BYTES, key0, edge(key0), a);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     // the warps' sums, in the order of the warps
     r.l += __shfl_xor_sync(0xffffffffu, r.l, 1);
     r.l += __shfl_xor_sync(0xffffffffu, r.l, 2);
     __syncthreads();                                               // the rings are free
-    float* sums = (float*)pt_sm;                                   // [warp][8][D]
+    // [warp][tile of 8 columns][row][column], tiles PT_TILE floats apart: no two lanes in one bank, neither here nor below
+    float* sums = (float*)pt_sm;
 #pragma unroll
     for (int i = 0; i < D / 8; i++)
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-            const int col = i / (CW / 8) * CW + (2 * t + x) * (CW / 8) + i % (CW / 8);
-            sums[(w * 8 + g) * D + col] = (r.o[i][x] + r.o[i][2 + x]) * r.vref;
-        }
+        *(float2*)(sums + (w * (D / 8) + i) * PT_TILE + g * 8 + 2 * t) = make_float2((r.o[i][0] + r.o[i][2]) * r.vref, (r.o[i][1] + r.o[i][3]) * r.vref);
     if (t == 0) ml[w][g] = make_float2(r.m, r.l);
     __syncthreads();
     const int n = min(8, rows - tile * 8);
     const size_t at = (size_t)blockIdx.x * a.heads + blockIdx.y;
-    for (int e = threadIdx.x; e < n * a.dv; e += PT_THREADS) {
-        const int y = e / a.dv, col = e - y * a.dv;
+    for (int e = threadIdx.x; e < n * D; e += PT_THREADS) {
+        const int y = e / D, i = e % D >> 3, x8 = e & 7, col = i / (CW / 8) * CW + x8 * (CW / 8) + i % (CW / 8);      // column x8 of tile i
+        if (col >= a.dv) continue;
         float m = -INFINITY, l = 0.0f, o = 0.0f;
 #pragma unroll
         for (int x = 0; x < PT_WARPS; x++) m = fmaxf(m, ml[x][y].x);
@@ -441,7 +454,7 @@ __global__ void __launch_bounds__(PT_THREADS) paged_few_kernel(const PtArgs a) {
         for (int x = 0; x < PT_WARPS; x++) {
             const float f = ml[x][y].x == -INFINITY ? (ml[x][y].y == 0.0f ? 0.0f : 1.0f) : exp2f(ml[x][y].x - m);
             l = fmaf(f, ml[x][y].y, l);
-            o = fmaf(f, sums[(x * 8 + y) * D + col], o);
+            o = fmaf(f, sums[(x * (D / 8) + i) * PT_TILE + y * 8 + x8], o);
         }
         if (n_split > 1) {
             a.part[(at * 8 + y) * a.dv + col] = o;
@@ -534,7 +547,7 @@ static int pt_run(cc_device* dev, const cc_page_plan* plan, PtArgs a, bool i8) {
     }
     if (!keys) return CC_OK;
     const int64_t slots = (int64_t)dev->sm_count * (few ? 3 : 1), each = (keys + slots - 1) / slots;
-    a.split = (int)(few ? std::min<int64_t>(512, std::max<int64_t>(128, (each + 63) / 64 * 64)) : std::min<int64_t>(TI_MOST, std::max<int64_t>(512, (each + 127) / 128 * 128)));
+    a.split = (int)(few ? std::min<int64_t>(1024, std::max<int64_t>(128, (each + 63) / 64 * 64)) : std::min<int64_t>(TI_MOST, std::max<int64_t>(512, (each + 127) / 128 * 128)));
     for (const PgSeq& s : plan->seqs) {
         const int n = pt_splits(s, a);
         items += (int64_t)n * (((int64_t)s.count * a.R + a.tile_rows - 1) / a.tile_rows);

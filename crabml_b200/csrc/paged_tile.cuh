@@ -79,11 +79,6 @@ __device__ __forceinline__ bool ti_wait(unsigned bar, unsigned parity, int* fail
     return false;
 }
 __device__ __forceinline__ bool ti_wait_warp(unsigned bar, unsigned parity, int* fail) { return __all_sync(0xffffffffu, ti_wait(bar, parity, fail)); }
-__device__ __forceinline__ float ti_exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 // pairs of 32-bit numbers in one instruction
 typedef unsigned long long ti_f2;
 __device__ __forceinline__ ti_f2 ti_fma2(ti_f2 a, ti_f2 b, ti_f2 c);
@@ -115,7 +110,7 @@ __device__ __forceinline__ ti_f2 ti_add2(ti_f2 a, ti_f2 b) {
 }
 // 2^x of a pair by multiply-adds: the special function unit makes 4 results a cycle and scheduler, which alone would take half of a step.  x = n + r with |r| <= 1/2 by way
 // of a number whose last place is 1; 2^r by its series up to r^6 (the rest is below 2^-22 r^7 / 5040 (ln 2)^7 < 2^-24); n goes into the exponent.  x >= -126 here
-__device__ __forceinline__ ti_f2 ti_exp2_two(float2 x) {
+__device__ __forceinline__ ti_f2 ti_exp2_pair(float2 x) {
     const ti_f2 big = ti_two(12582912.0f, 12582912.0f), minus = ti_two(-1.0f, -1.0f);
     const ti_f2 v = ti_two(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f)), t = ti_add2(v, big), n = ti_add2(t, ti_two(-12582912.0f, -12582912.0f)), r = ti_fma2(n, minus, v);
     ti_f2 p = ti_two(1.5403530e-4f, 1.5403530e-4f);                  // (ln 2)^i / i!, i = 6 .. 0
@@ -247,7 +242,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
     int from, to;
     pt_range(s, a, &from, &to);
     const int row0 = tile * TI_ROWS, n_rows = min(TI_ROWS, rows - row0), pos_first = s.pos0 + row0 / a.R, pos_last = s.pos0 + (row0 + n_rows - 1) / a.R;
-    const int k0 = from + split * a.split, k1 = min(min(to, k0 + a.split), pos_last + 1);
+    const int each = pt_each(to - from, n_split, a), k0 = from + split * each, k1 = min(min(to, k0 + each), pos_last + 1);
     const int lo = a.window > 0 ? max(k0, (pos_first - a.window + 1) & ~(TI_KEYS - 1)) : k0, steps = k1 > lo ? (k1 - lo + TI_KEYS - 1) / TI_KEYS : 0;
     const int opens = I8 ? to >> a.shift << a.shift : 0;
     // the images of the first step, and what stands beside those of all steps
@@ -445,7 +440,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
             for (int i = 0; i < TI_SPLIT; i++) mx = fmaxf(mx, sh.top[slot][i][row]);
             const float* vfs = sh.info[k].vf;
             const float m_new = fmaxf(m, mx), base = m_new == -INFINITY ? 0.0f : PT_SHIFT - m_new;
-            const float alpha = m == m_new ? 1.0f : ti_exp2(m - m_new);
+            const float alpha = m == m_new ? 1.0f : pt_exp2(m - m_new);
             m = m_new;
             ti_f2 sum = 0ull;
             const ti_f2 base2 = ti_two(base, base), minus = ti_two(-1.0f, -1.0f);
@@ -456,7 +451,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
 #pragma unroll
                 for (int c = 0; c < 16; c += 2) {
                     const float2 y = ti_one(ti_fma2(ti_two(__uint_as_float(x[g * 16 + c]), __uint_as_float(x[g * 16 + c + 1])), f2, base2));
-                    ti_f2 p = c % 16 >= TI_SFU ? ti_exp2_two(y) : ti_two(ti_exp2(y.x), ti_exp2(y.y));
+                    ti_f2 p = c % 16 >= TI_SFU ? ti_exp2_pair(y) : ti_two(pt_exp2(y.x), pt_exp2(y.y));
                     sum = ti_add2(sum, p);
                     if (I8) p = ti_mul2(p, vr2);
                     const float2 q = ti_one(p);
