@@ -17,7 +17,9 @@
 #define PT_THREADS (PT_WARPS * 32)
 #define PT_SHIFT 9.0f                         // weights are exp2(score - base + PT_SHIFT), base the largest score so far, or up to PT_LAG less: weights stay below 2^15, and the sums
 #define PT_LAG 6.0f                           // of a row are not scaled again for every score that is a little larger
-#define PT_MOST_SPLIT 2048                    // keys of a slice
+#define PT_STEP 64                            // keys that few rows are dealt out by
+#define PT_BEGIN 5                            // what a segment's begin and end cost, in steps (finding it, the queries, the sums: 13 thousand cycles)
+#define PT_CHUNK 4096                         // keys whose page numbers and factors a CTA holds at a time
 #define PT_FEW 32
 #define PT_TILE 72
 #define PT_LOG2E 1.4426950408889634f
@@ -29,7 +31,7 @@ struct PtArgs {
     const uint8_t *k, *v;
     const float *ks, *vs, *q, *sink;
     const __half *ko, *vo;
-    float *out, *part;                        // part: [item][head][tile_rows][dv] sums of a slice, behind them ml
+    float *out, *part;                        // part: [item][head][tile_rows][dv] sums of a slice (few rows: [2 x CTA][8][dv], of its first and its last segment)
     float2* ml;                               // [item][head][tile_rows]: largest score (base 2) and sum of weights
     float scale, softcap;
     int n_seqs, table_cols, page, shift, H, G, R, dk, dv, window, split, rows_lo, rows_hi;
@@ -38,6 +40,11 @@ struct PtArgs {
     uint8_t *k_image, *v_image;               // paged_tile.cuh
     struct TiInfo* info;
 };
+// few rows: segments are (sequence, 8 rows, key head), of steps of PT_STEP keys behind PT_BEGIN more for the segment itself.  `ctas` CTAs take equal runs of them: where the run of CTA c
+// begins, dealt out on the host (a search by each CTA took 3 to 5 us at the start); ctas 0: a CTA a segment
+#define PT_CTAS 592
+struct PtDeal { int ctas, run_lo, run_more; struct { int seq, seg, off; } at[PT_CTAS]; };      // the first run_more runs are of run_lo + 1 steps
+struct PtCuts { struct { int seq, seg, slot, cta, n; } at[PT_CTAS]; };      // segments that are in several runs: the place of the first one's sums, the next CTA, how many
 struct PtItem { int seq, split, tile, n_split; };
 
 // keys [from, to) that the sequence's new tokens see together
@@ -52,10 +59,17 @@ __host__ __device__ __forceinline__ int pt_splits(const PgSeq& s, const PtArgs& 
     pt_range(s, a, &from, &to);
     return (to - from + a.split - 1) / a.split;
 }
-// keys of a slice: the sequence's in equal parts, whole steps of 64 (few rows) or of TI_KEYS
-__host__ __device__ __forceinline__ int pt_each(int keys, int n_split, const PtArgs& a) {
-    const int step = a.tile_rows == 8 ? 64 : 128;
-    return ((keys + n_split - 1) / n_split + step - 1) / step * step;
+// keys of a slice: the sequence's in equal parts
+__host__ __device__ __forceinline__ int pt_each(int keys, int n_split) { return ((keys + n_split - 1) / n_split + 127) / 128 * 128; }
+// few rows: a segment is (sequence, 8 rows, key head); a sequence's segments, and the steps of each
+__host__ __device__ __forceinline__ int pt_segments(const PgSeq& s, const PtArgs& a) {
+    const int64_t rows = (int64_t)s.count * a.R;
+    return rows < a.rows_lo || rows > a.rows_hi ? 0 : (int)((rows + 7) / 8) * a.G;
+}
+__host__ __device__ __forceinline__ int pt_steps(const PgSeq& s, const PtArgs& a) {
+    int from, to;
+    pt_range(s, a, &from, &to);
+    return PT_BEGIN + (to - from + PT_STEP - 1) / PT_STEP;
 }
 // the place of number n in the sequences' counts: every lane gets the sequence and what is left of n
 template <class Count>
@@ -80,6 +94,7 @@ __device__ __forceinline__ int pt_find(const PtArgs& a, int n, Count count, int*
     return -1;
 }
 
+__device__ __forceinline__ void pt_copy4(unsigned dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void pt_copy16(unsigned dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
@@ -331,29 +346,61 @@ struct PtF16 {
 };
 
 template <int D, bool I8>
-__global__ void __launch_bounds__(PT_THREADS, D <= 64 ? 4 : D <= 128 ? 3 : 1) paged_few_kernel(const PtArgs a) {
+__global__ void __launch_bounds__(PT_THREADS, D <= 64 ? 4 : D <= 128 ? 3 : 1) paged_few_kernel(const PtArgs a, const __grid_constant__ PtDeal deal) {
     using Mine = PtF16<D, I8>;                                     // 16-bit rows: pages, or the open block beside codes
     constexpr int RING = 128 * D, STAGES = RING / Mine::BYTES, STAGES8 = RING / PtI8<D>::BYTES, CW = I8 && D >= 128 ? 128 : 64;
     extern __shared__ __align__(16) uint8_t pt_sm[];
-    __shared__ int pid[PT_MOST_SPLIT / 16 + 1];
-    __shared__ float kfs[PT_MOST_SPLIT / 16 + 1], vfs[PT_MOST_SPLIT / 16 + 1];
+    __shared__ int pid[PT_CHUNK / 16 + 1];
+    __shared__ float kfs[PT_CHUNK / 16 + 1], vfs[PT_CHUNK / 16 + 1];
     __shared__ float2 ml[PT_WARPS][8];
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, kvh = a.head0 + blockIdx.y;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     uint8_t* ring = pt_sm + w * RING;
     const unsigned ring_at = (unsigned)__cvta_generic_to_shared(ring);
     pdl_enter();
-    int rest;
-    const int seq = pt_find(a, blockIdx.x, [&](const PgSeq& s) { return pt_splits(s, a) * (int)(((int64_t)s.count * a.R + 7) >> 3); }, &rest);
-    if (seq < 0) return;
-    const PgSeq s = a.seqs[seq];
-    const int rows = s.count * a.R, tiles = (rows + 7) >> 3, split = rest / tiles, tile = rest - split * tiles, n_split = pt_splits(s, a);
+    // this CTA's run of steps; pieces of it, a segment each
+    const int c = blockIdx.x, run = deal.ctas ? deal.run_lo + (c < deal.run_more ? 1 : 0) : 1;
+    int seq, seg, off = 0, more = 0;                               // more: segments of the sequence behind this one
+    if (deal.ctas) {
+        seq = deal.at[c].seq; seg = deal.at[c].seg; off = deal.at[c].off;
+        more = pt_segments(a.seqs[seq], a) - 1 - seg;
+    } else if ((seq = pt_find(a, c, [&](const PgSeq& s) { return pt_segments(s, a); }, &seg)) < 0) return;
+    for (int at = 0; at < run;) {
     int from, to;
+    if (at > 0) {
+        off = 0;
+        if (more-- > 0) seg++;
+        else {
+            do if (++seq >= a.n_seqs) return;
+            while ((more = pt_segments(a.seqs[seq], a) - 1) < 0);
+            seg = 0;
+        }
+    }
+    const PgSeq s = a.seqs[seq];
     pt_range(s, a, &from, &to);
+    const int all = pt_steps(s, a), upto = deal.ctas ? min(all, off + run - at) : all;
+    const int rows = s.count * a.R, tile = seg / a.G, kvh = seg - tile * a.G, slot = 2 * c + (at == 0 ? 0 : 1);
+    const bool whole = off <= PT_BEGIN && upto == all;
+    at += upto - off;
+    if (upto <= PT_BEGIN) break;                                   // the next CTA has all its keys
     const int row = tile * 8 + g, tok = row / a.R, pos_first = s.pos0 + tile * 8 / a.R, pos_last = s.pos0 + (min(rows, tile * 8 + 8) - 1) / a.R;
-    const int each = pt_each(to - from, n_split, a), k0 = from + split * each, k1 = min(min(to, k0 + each), pos_last + 1);       // keys of the slice that some row of the tile may see
-    const int lo = a.window > 0 ? max(k0, (pos_first - a.window + 1) & ~15) : k0, units = k1 > lo ? (k1 - lo + 15) >> 4 : 0;
-    const int p0 = lo >> a.shift, opens = I8 ? to >> a.shift << a.shift : 0;                  // the first key that is not in a page of codes
-    const int n_pages = units > 0 ? ((k1 - 1) >> a.shift) - p0 + 1 : 0, units8 = I8 ? max(0, min(units, (opens - lo) >> 4)) : 0;
+    const int k0 = from + max(off - PT_BEGIN, 0) * PT_STEP, k1 = min(min(to, from + (upto - PT_BEGIN) * PT_STEP), pos_last + 1);       // keys of the piece that some row of the tile may see
+    const int lo0 = a.window > 0 ? max(k0, (pos_first - a.window + 1) & ~15) : k0, opens = I8 ? to >> a.shift << a.shift : 0;      // opens: the first key that is not in a page of codes
+    // the lane's columns of its row
+    const bool in = row < rows;
+    constexpr int E = I8 ? 16 : 8;
+    PtRows<D> r;
+    float v[D / 4];
+    {
+        const float* q = a.q + ((int64_t)(s.first + (in ? tok : 0)) * a.H + kvh * a.R + (in ? row - tok * a.R : 0)) * a.dk;
+#pragma unroll
+        for (int i = 0; i < D / 4; i++) {
+            const int col = i / E * 4 * E + t * E + i % E;
+            v[i] = in && col < a.dk ? q[col] : 0.0f;
+        }
+    }
+    for (int lo = lo0;; lo += PT_CHUNK) {                          // (once, but for the longest pieces)
+    const int hi = min(k1, lo + PT_CHUNK), units = hi > lo ? (hi - lo + 15) >> 4 : 0, p0 = lo >> a.shift;
+    const int n_pages = units > 0 ? ((hi - 1) >> a.shift) - p0 + 1 : 0, units8 = I8 ? max(0, min(units, (opens - lo) >> 4)) : 0;
     for (int i = threadIdx.x; i < n_pages; i += PT_THREADS) pid[i] = a.table[(int64_t)seq * a.table_cols + p0 + i];
     __syncthreads();
     // 16 keys' rows on their way into a place of the ring: codes, and 16-bit rows (`first` on: this warp's units behind the codes)
@@ -375,25 +422,21 @@ __global__ void __launch_bounds__(PT_THREADS, D <= 64 ? 4 : D <= 128 ? 3 : 1) pa
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     const int first = units8 + (w - units8 % PT_WARPS + PT_WARPS) % PT_WARPS;
-    // the first of them come while the factors are read and the queries cut
+    if (I8)
+        for (int i = threadIdx.x; i < n_pages; i += PT_THREADS) {     // (copies too, that the first rows bring with them)
+            const size_t at = (size_t)pid[i] * a.G + kvh;
+            pt_copy4((unsigned)__cvta_generic_to_shared(kfs + i), a.ks + at);
+            pt_copy4((unsigned)__cvta_generic_to_shared(vfs + i), a.vs + at);
+        }
+    // the first rows come while the queries are cut
     if (I8) {
 #pragma unroll
         for (int i = 0; i < STAGES8 - 1; i++) load8(w + i * PT_WARPS);
     } else load16(first);
-    if (I8)
-        for (int i = threadIdx.x; i < n_pages; i += PT_THREADS) { kfs[i] = a.ks[(int64_t)pid[i] * a.G + kvh]; vfs[i] = a.vs[(int64_t)pid[i] * a.G + kvh]; }
-    PtRows<D> r;
-    {                                                              // the lane's columns of its row
-        const bool in = row < rows;
-        const float* q = a.q + ((int64_t)(s.first + (in ? tok : 0)) * a.H + kvh * a.R + (in ? row - tok * a.R : 0)) * a.dk;
-        constexpr int E = I8 ? 16 : 8;
-        float v[D / 4], top = 0.0f;
+    if (lo == lo0) {
+        float top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < D / 4; i++) {
-            const int col = i / E * 4 * E + t * E + i % E;
-            v[i] = in && col < a.dk ? q[col] : 0.0f;
-            top = fmaxf(top, fabsf(v[i]));
-        }
+        for (int i = 0; i < D / 4; i++) top = fmaxf(top, fabsf(v[i]));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         int ex = 14;
@@ -412,6 +455,7 @@ __global__ void __launch_bounds__(PT_THREADS, D <= 64 ? 4 : D <= 128 ? 3 : 1) pa
 #pragma unroll
         for (int i = 0; i < D / 8; i++) r.o[i][0] = r.o[i][1] = r.o[i][2] = r.o[i][3] = 0.0f;
     }
+    if (I8) asm volatile("cp.async.wait_group %0;" ::"n"(STAGES8 - 2) : "memory");
     __syncthreads();
     auto edge = [&](int key0) { return key0 + 15 > pos_first || (a.window > 0 && key0 < pos_last - a.window + 1); };
     if constexpr (I8) {
@@ -431,10 +475,12 @@ __global__ void __launch_bounds__(PT_THREADS, D <= 64 ? 4 : D <= 128 ? 3 : 1) pa
         Mine::use(r, ring + (u / PT_WARPS % STAGES) * Mine::BYTES, key0, edge(key0), a);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();                                               // the rings, page numbers and factors are free
+    if (hi >= k1) break;
+    }
     // the warps' sums, in the order of the warps
     r.l += __shfl_xor_sync(0xffffffffu, r.l, 1);
     r.l += __shfl_xor_sync(0xffffffffu, r.l, 2);
-    __syncthreads();                                               // the rings are free
     // [warp][tile of 8 columns][row][column], tiles PT_TILE floats apart: no two lanes in one bank, neither here nor below
     float* sums = (float*)pt_sm;
 #pragma unroll
@@ -443,7 +489,6 @@ __global__ void __launch_bounds__(PT_THREADS, D <= 64 ? 4 : D <= 128 ? 3 : 1) pa
     if (t == 0) ml[w][g] = make_float2(r.m, r.l);
     __syncthreads();
     const int n = min(8, rows - tile * 8);
-    const size_t at = (size_t)blockIdx.x * a.heads + blockIdx.y;
     for (int e = threadIdx.x; e < n * D; e += PT_THREADS) {
         const int y = e / D, i = e % D >> 3, x8 = e & 7, col = i / (CW / 8) * CW + x8 * (CW / 8) + i % (CW / 8);      // column x8 of tile i
         if (col >= a.dv) continue;
@@ -456,9 +501,9 @@ __global__ void __launch_bounds__(PT_THREADS, D <= 64 ? 4 : D <= 128 ? 3 : 1) pa
             l = fmaf(f, ml[x][y].y, l);
             o = fmaf(f, sums[(x * (D / 8) + i) * PT_TILE + y * 8 + x8], o);
         }
-        if (n_split > 1) {
-            a.part[(at * 8 + y) * a.dv + col] = o;
-            if (col == 0) a.ml[at * 8 + y] = make_float2(m, l);
+        if (!whole) {
+            a.part[((size_t)slot * 8 + y) * a.dv + col] = o;
+            if (col == 0) a.ml[slot * 8 + y] = make_float2(m, l);
             continue;
         }
         const int rr = tile * 8 + y, tk = rr / a.R, head = kvh * a.R + rr - tk * a.R;
@@ -469,25 +514,18 @@ __global__ void __launch_bounds__(PT_THREADS, D <= 64 ? 4 : D <= 128 ? 3 : 1) pa
         }
         a.out[((int64_t)(s.first + tk) * a.H + head) * a.dv + col] = o / l;
     }
+    __syncthreads();                                               // the sums, before the next piece's rows
+    }
 }
-// the slices of a row added up: a CTA a row, its threads take 32 columns of 4 numbers ... by four groups of slices
-__global__ void __launch_bounds__(128) paged_sum_kernel(const PtArgs a) {
-    __shared__ float so[4][256];
-    __shared__ float2 sm[4];
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, kvh = a.head0 + blockIdx.y;
-    pdl_enter();
-    int row, items = 0;
-    const int seq = pt_find(a, blockIdx.x, [&](const PgSeq& s) { return pt_splits(s, a) > 1 ? s.count * a.R : 0; }, &row);
-    if (seq < 0) return;
-    for (int x = lane; x < seq; x += 32) items += pt_splits(a.seqs[x], a) * ((a.seqs[x].count * a.R + a.tile_rows - 1) / a.tile_rows);
-    items = warp_sum_i(items);
-    const PgSeq s = a.seqs[seq];
-    const int tiles = (s.count * a.R + a.tile_rows - 1) / a.tile_rows, n = pt_splits(s, a), tile = row / a.tile_rows, y = row - tile * a.tile_rows;
-    // items of a sequence: slice by slice where a tile is 8 rows, tile by tile from the last one on where it is 128
-    const int first = a.tile_rows == 8 ? tile : (tiles - 1 - tile) * n, by = a.tile_rows == 8 ? tiles : 1;
-    auto at = [&](int x) { return ((size_t)(items + first + x * by) * a.heads + blockIdx.y) * a.tile_rows + y; };
+#define PT_JOIN 4                             // warps
+// n slices of a row added up by a CTA: a warp takes every PT_JOINth of them, a lane 4 neighbouring columns; part and ml of slice x at place(x)
+template <class Place>
+__device__ __forceinline__ void pt_join(const PtArgs& a, int n, Place place, float* out, int head) {
+    __shared__ float so[PT_JOIN][256];
+    __shared__ float2 sm[PT_JOIN];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     float m = -INFINITY;
-    for (int x = lane; x < n; x += 32) m = fmaxf(m, a.ml[at(x)].x);
+    for (int x = lane; x < n; x += 32) m = fmaxf(m, a.ml[place(x)].x);
     m = warp_max(m);
     float l = 0.0f;
     for (int c0 = 0; c0 < a.dv; c0 += 128) {
@@ -495,12 +533,12 @@ __global__ void __launch_bounds__(128) paged_sum_kernel(const PtArgs a) {
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         float sum = 0.0f;
 #pragma unroll 4
-        for (int x = w; x < n; x += 4) {
-            const float2 z = a.ml[at(x)];
+        for (int x = w; x < n; x += PT_JOIN) {
+            const float2 z = a.ml[place(x)];
             const float f = z.x == -INFINITY ? (z.y == 0.0f ? 0.0f : 1.0f) : exp2f(z.x - m);
             sum = fmaf(f, z.y, sum);
             if (col < a.dv) {
-                const float4 v = *(const float4*)(a.part + at(x) * a.dv + col);
+                const float4 v = *(const float4*)(a.part + place(x) * a.dv + col);
                 o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
             }
         }
@@ -509,33 +547,121 @@ __global__ void __launch_bounds__(128) paged_sum_kernel(const PtArgs a) {
     }
     if (lane == 0) sm[w] = make_float2(m, l);
     __syncthreads();
-    const int tok = row / a.R, head = kvh * a.R + row - tok * a.R;
-    l = ((sm[0].y + sm[1].y) + sm[2].y) + sm[3].y;
+    l = 0.0f;
+#pragma unroll
+    for (int x = 0; x < PT_JOIN; x++) l += sm[x].y;
     float f = 1.0f;
     if (a.sink) {
         const float sk = a.sink[head] * PT_LOG2E, m2 = fmaxf(m, sk);
         f = m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : exp2f(m - m2);
         l = f * l + (sk == -INFINITY ? 0.0f : exp2f(sk - m2 + PT_SHIFT));
     }
-    for (int c = threadIdx.x; c < a.dv; c += 128)
-        a.out[((int64_t)(s.first + tok) * a.H + head) * a.dv + c] = (((so[0][c] + so[1][c]) + so[2][c]) + so[3][c]) * f / l;
+    for (int c = threadIdx.x; c < a.dv; c += 32 * PT_JOIN) {
+        float o = 0.0f;
+#pragma unroll
+        for (int x = 0; x < PT_JOIN; x++) o += so[x][c];
+        out[c] = o * f / l;
+    }
+}
+// few rows: grid (segments in several runs, 8 rows)
+__global__ void __launch_bounds__(32 * PT_JOIN) paged_join_kernel(const PtArgs a, const __grid_constant__ PtCuts cuts) {
+    pdl_enter();
+    const auto cut = cuts.at[blockIdx.x];
+    const PgSeq s = a.seqs[cut.seq];
+    const int y = blockIdx.y, tile = cut.seg / a.G, kvh = cut.seg - tile * a.G, row = tile * 8 + y;
+    if (row >= s.count * a.R) return;
+    const int tok = row / a.R, head = kvh * a.R + row - tok * a.R;
+    pt_join(a, cut.n, [&](int x) { return (size_t)(x == 0 ? cut.slot : 2 * (cut.cta + x - 1)) * 8 + y; }, a.out + ((int64_t)(s.first + tok) * a.H + head) * a.dv, head);
+}
+// tiles of 128 rows: the slices of a row, grid (rows, key heads)
+__global__ void __launch_bounds__(32 * PT_JOIN) paged_sum_kernel(const PtArgs a) {
+    const int lane = threadIdx.x & 31, kvh = a.head0 + blockIdx.y;
+    pdl_enter();
+    int row, items = 0;
+    const int seq = pt_find(a, blockIdx.x, [&](const PgSeq& s) { return pt_splits(s, a) > 1 ? s.count * a.R : 0; }, &row);
+    if (seq < 0) return;
+    for (int x = lane; x < seq; x += 32) items += pt_splits(a.seqs[x], a) * ((a.seqs[x].count * a.R + a.tile_rows - 1) / a.tile_rows);
+    items = warp_sum_i(items);
+    const PgSeq s = a.seqs[seq];
+    const int tiles = (s.count * a.R + a.tile_rows - 1) / a.tile_rows, n = pt_splits(s, a), tile = row / a.tile_rows, y = row - tile * a.tile_rows;
+    const int tok = row / a.R, head = kvh * a.R + row - tok * a.R, first = items + (tiles - 1 - tile) * n;      // items of a sequence: tile by tile from the last one on
+    pt_join(a, n, [&](int x) { return ((size_t)(first + x) * a.heads + blockIdx.y) * a.tile_rows + y; }, a.out + ((int64_t)(s.first + tok) * a.H + head) * a.dv, head);
 }
 
 template <int D, bool I8>
-static cudaError_t pt_launch_few(cc_device* dev, const PtArgs& a, unsigned items) {
+static cudaError_t pt_launch_few(cc_device* dev, const PtArgs& a, const PtDeal& deal, unsigned ctas) {
     constexpr int smem = PT_WARPS * 128 * D;
     cudaError_t e = cudaFuncSetAttribute(paged_few_kernel<D, I8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess) e = cc_launch_pdl(dev, paged_few_kernel<D, I8>, dim3(items, (unsigned)a.heads), PT_THREADS, smem, a);
+    if (e == cudaSuccess) e = cc_launch_pdl(dev, paged_few_kernel<D, I8>, ctas, PT_THREADS, smem, a, deal);
     dev->launches++;
     return e;
+}
+// the runs of deal.ctas CTAs over all steps, and the segments that are in several of them (returned: how many; `rows` of the longest)
+static int pt_deal(const cc_page_plan* plan, const PtArgs& a, int64_t steps, PtDeal& deal, PtCuts& cuts) {
+    deal.run_lo = (int)(steps / deal.ctas); deal.run_more = (int)(steps % deal.ctas);
+    int64_t before = 0, next = 0;                                  // steps in front of the sequence, and of run c
+    int c = 0, n_cuts = 0;
+    for (int seq = 0; seq < (int)plan->seqs.size() && c < deal.ctas; seq++) {
+        const int n = pt_segments(plan->seqs[seq], a), all = n ? pt_steps(plan->seqs[seq], a) : 0;
+        for (; c < deal.ctas && next < before + (int64_t)n * all; next += deal.run_lo + (c < deal.run_more ? 1 : 0), c++) {
+            const int seg = (int)((next - before) / all), off = (int)((next - before) - (int64_t)seg * all);
+            deal.at[c] = {seq, seg, off};
+            if (off <= PT_BEGIN) continue;                         // the segment's keys are all this run's, or there are none of them in front
+            auto& cut = cuts.at[n_cuts ? n_cuts - 1 : 0];
+            if (n_cuts && cut.seq == seq && cut.seg == seg) { cut.n++; continue; }
+            const auto& last = deal.at[c - 1];                     // the run in front begins with the segment, or within its first PT_BEGIN steps, or ends with it
+            cuts.at[n_cuts++] = {seq, seg, 2 * (c - 1) + (last.seq == seq && last.seg == seg ? 0 : 1), c, 2};
+        }
+        before += (int64_t)n * all;
+    }
+    return n_cuts;
+}
+// Sequences of few rows.  Segments of up to PT_WHOLE steps, or very many of them: a CTA each, nothing to add up.  Longer ones: all steps in equal runs, as many CTAs as the device holds
+// at a time, so that none waits for a last wave and few begin anew.  (Slices of up to 1024 keys, a CTA each: 64 sequences of up to 4000 tokens, 32 heads on 8, 8-bit pages: 90 us, in runs 82; 16-bit pages 77 and 75)
+#define PT_WHOLE 8
+static int pt_run_few(cc_device* dev, const cc_page_plan* plan, PtArgs a, bool i8) {
+    int64_t segments = 0, steps = 0;
+    int most = 0;
+    for (const PgSeq& s : plan->seqs) {
+        const int n = pt_segments(s, a);
+        if (!n) continue;
+        const int all = pt_steps(s, a);
+        segments += n;
+        steps += (int64_t)n * all;
+        most = std::max(most, all - PT_BEGIN);
+    }
+    if (!segments) return CC_OK;
+    CC_REQUIRE(dev, segments < ((int64_t)1 << 31), "paged_attention: too many rows");
+    const int d = std::max(a.dk, a.dv), per_sm = d <= 64 ? 4 : d <= 128 ? 3 : 1;
+    const int64_t slots = std::min<int64_t>(PT_CTAS, (int64_t)per_sm * dev->sm_count);
+    PtDeal deal;
+    PtCuts cuts;
+    deal.ctas = most <= PT_WHOLE || segments >= 8 * slots ? 0 : (int)std::min<int64_t>(slots, (steps + PT_BEGIN + 1) / (PT_BEGIN + 2));
+    const int n_cuts = deal.ctas ? pt_deal(plan, a, steps, deal, cuts) : 0;
+    void* ws = nullptr; size_t cls = 0;
+    if (n_cuts) {
+        const size_t part = (size_t)2 * deal.ctas * 8 * a.dv * sizeof(float);
+        const int rc = cc_pool_alloc(dev, part + (size_t)2 * deal.ctas * 8 * sizeof(float2), &ws, &cls);
+        if (rc) return rc;
+        a.part = (float*)ws; a.ml = (float2*)((uint8_t*)ws + part);
+    }
+    const unsigned ctas = deal.ctas ? (unsigned)deal.ctas : (unsigned)segments;
+    cudaError_t e = i8 ? (d <= 64 ? pt_launch_few<64, true>(dev, a, deal, ctas) : d <= 128 ? pt_launch_few<128, true>(dev, a, deal, ctas) : pt_launch_few<256, true>(dev, a, deal, ctas))
+                       : (d <= 64 ? pt_launch_few<64, false>(dev, a, deal, ctas) : d <= 128 ? pt_launch_few<128, false>(dev, a, deal, ctas) : pt_launch_few<256, false>(dev, a, deal, ctas));
+    if (e == cudaSuccess && n_cuts) {
+        e = cc_launch_pdl(dev, paged_join_kernel, dim3((unsigned)n_cuts, 8), 32 * PT_JOIN, 0, a, cuts);
+        dev->launches++;
+    }
+    if (ws) cc_pool_free(dev, ws, cls);
+    if (e != cudaSuccess) return cc_fail(dev, CC_ERR_CUDA, "paged_attention: %s", cudaGetErrorString(e));
+    return CC_OK;
 }
 #include "paged_tile.cuh"
 
 #define TI_WORKSPACE ((int64_t)256 << 20)     // bytes of images that a call has at a time, as long as one head's are no more
 
-// the sequences of rows_lo .. rows_hi rows, in tiles of tile_rows: slices of `most` keys at most, as many as leave no SM without one
-static int pt_run(cc_device* dev, const cc_page_plan* plan, PtArgs a, bool i8) {
-    const bool few = a.tile_rows == 8;
+// sequences of many rows: slices of TI_MOST keys at most, as many as leave no SM without one
+static int pt_run_tiles(cc_device* dev, const cc_page_plan* plan, PtArgs a, bool i8) {
     int64_t keys = 0, items = 0, split_rows = 0, key_tiles = 0;
     for (const PgSeq& s : plan->seqs) {
         const int64_t rows = (int64_t)s.count * a.R;
@@ -546,42 +672,35 @@ static int pt_run(cc_device* dev, const cc_page_plan* plan, PtArgs a, bool i8) {
         key_tiles += ti_key_tiles(s, a);
     }
     if (!keys) return CC_OK;
-    const int64_t slots = (int64_t)dev->sm_count * (few ? 3 : 1), each = (keys + slots - 1) / slots;
-    a.split = (int)(few ? std::min<int64_t>(1024, std::max<int64_t>(128, (each + 63) / 64 * 64)) : std::min<int64_t>(TI_MOST, std::max<int64_t>(512, (each + 127) / 128 * 128)));
+    const int64_t each = (keys + dev->sm_count - 1) / dev->sm_count;
+    a.split = (int)std::min<int64_t>(TI_MOST, std::max<int64_t>(512, (each + 127) / 128 * 128));
     for (const PgSeq& s : plan->seqs) {
         const int n = pt_splits(s, a);
         items += (int64_t)n * (((int64_t)s.count * a.R + a.tile_rows - 1) / a.tile_rows);
         if (n > 1) split_rows += (int64_t)s.count * a.R;
     }
     CC_REQUIRE(dev, items * a.G < ((int64_t)1 << 31) && split_rows < ((int64_t)1 << 31) && key_tiles < ((int64_t)1 << 31), "paged_attention: too many rows");
-    const size_t kb = (size_t)((a.dk + 63) / 64) * TI_BLOCK, vb = (size_t)((a.dv + 63) / 64) * TI_BLOCK, per_head = few ? 0 : (size_t)key_tiles * (kb + vb + sizeof(TiInfo));
-    a.heads = few || (int64_t)per_head * a.G <= TI_WORKSPACE ? a.G : (int)std::max<int64_t>(1, TI_WORKSPACE / (int64_t)per_head);
+    const size_t kb = (size_t)((a.dk + 63) / 64) * TI_BLOCK, vb = (size_t)((a.dv + 63) / 64) * TI_BLOCK, per_head = (size_t)key_tiles * (kb + vb + sizeof(TiInfo));
+    a.heads = (int64_t)per_head * a.G <= TI_WORKSPACE ? a.G : (int)std::max<int64_t>(1, TI_WORKSPACE / (int64_t)per_head);
     const size_t part = split_rows ? (size_t)items * a.heads * a.tile_rows * a.dv * sizeof(float) : 0, ml = split_rows ? (size_t)items * a.heads * a.tile_rows * sizeof(float2) : 0;
     void* ws = nullptr; size_t cls = 0;
-    if (part + per_head) {
-        const int rc = cc_pool_alloc(dev, part + ml + per_head * a.heads + 256, &ws, &cls);
-        if (rc) return rc;
-        a.k_image = (uint8_t*)ws; a.v_image = a.k_image + (few ? 0 : key_tiles * a.heads * kb);
-        a.part = (float*)(a.v_image + (few ? 0 : key_tiles * a.heads * vb));
-        a.ml = (float2*)((uint8_t*)a.part + part); a.info = (TiInfo*)((uint8_t*)a.ml + ml);
-    }
-    const int d = std::max(a.dk, a.dv), all = a.heads;
+    const int rc = cc_pool_alloc(dev, part + ml + per_head * a.heads + 256, &ws, &cls);
+    if (rc) return rc;
+    a.k_image = (uint8_t*)ws; a.v_image = a.k_image + key_tiles * a.heads * kb;
+    a.part = (float*)(a.v_image + key_tiles * a.heads * vb);
+    a.ml = (float2*)((uint8_t*)a.part + part); a.info = (TiInfo*)((uint8_t*)a.ml + ml);
+    const int all = a.heads;
+    const bool cap = a.softcap > 0.0f;
+    auto kernel = i8 ? (cap ? paged_tile_kernel<true, true> : paged_tile_kernel<true, false>) : (cap ? paged_tile_kernel<false, true> : paged_tile_kernel<false, false>);
     cudaError_t e = cudaSuccess;
     for (a.head0 = 0; a.head0 < a.G && e == cudaSuccess; a.head0 += all) {
         a.heads = std::min(all, a.G - a.head0);
-        if (few) {
-            e = i8 ? (d <= 64 ? pt_launch_few<64, true>(dev, a, (unsigned)items) : d <= 128 ? pt_launch_few<128, true>(dev, a, (unsigned)items) : pt_launch_few<256, true>(dev, a, (unsigned)items))
-                   : (d <= 64 ? pt_launch_few<64, false>(dev, a, (unsigned)items) : d <= 128 ? pt_launch_few<128, false>(dev, a, (unsigned)items) : pt_launch_few<256, false>(dev, a, (unsigned)items));
-        } else {
-            const bool cap = a.softcap > 0.0f;
-            auto kernel = i8 ? (cap ? paged_tile_kernel<true, true> : paged_tile_kernel<true, false>) : (cap ? paged_tile_kernel<false, true> : paged_tile_kernel<false, false>);
-            e = cc_launch_pdl(dev, i8 ? paged_unpack_kernel<true> : paged_unpack_kernel<false>, dim3((unsigned)key_tiles, (unsigned)a.heads), TU_THREADS, 0, a);
-            if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TI_SMEM);
-            if (e == cudaSuccess) e = cc_launch_pdl(dev, kernel, (unsigned)(items * a.heads), TI_THREADS, TI_SMEM, a, dev->err_dev, dev->err_host);
-            dev->launches += 2;
-        }
+        e = cc_launch_pdl(dev, i8 ? paged_unpack_kernel<true> : paged_unpack_kernel<false>, dim3((unsigned)key_tiles, (unsigned)a.heads), TU_THREADS, 0, a);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TI_SMEM);
+        if (e == cudaSuccess) e = cc_launch_pdl(dev, kernel, (unsigned)(items * a.heads), TI_THREADS, TI_SMEM, a, dev->err_dev, dev->err_host);
+        dev->launches += 2;
         if (e == cudaSuccess && split_rows) {
-            e = cc_launch_pdl(dev, paged_sum_kernel, dim3((unsigned)split_rows, (unsigned)a.heads), 128, 0, a);
+            e = cc_launch_pdl(dev, paged_sum_kernel, dim3((unsigned)split_rows, (unsigned)a.heads), 32 * PT_JOIN, 0, a);
             dev->launches++;
         }
     }
@@ -621,10 +740,10 @@ extern "C" CC_API int cc_paged_attention(cc_device* dev, const cc_page_plan* pla
         a.H = H; a.G = c.G; a.R = H / c.G; a.dk = c.dk; a.dv = c.dv;
         // rows of a sequence and key head: up to PT_FEW in tiles of 8, more in tiles of 128 where a head's numbers have room there
         a.rows_lo = 1; a.rows_hi = c.dk <= TI_D && c.dv <= TI_D ? PT_FEW : 0x7fffffff; a.tile_rows = 8; a.align = 16;
-        rc = pt_run(dev, plan, a, c.i8);
+        rc = pt_run_few(dev, plan, a, c.i8);
         if (!rc && a.rows_hi == PT_FEW) {
             a.rows_lo = PT_FEW + 1; a.rows_hi = 0x7fffffff; a.tile_rows = TI_ROWS; a.align = TI_KEYS;
-            rc = pt_run(dev, plan, a, c.i8);
+            rc = pt_run_tiles(dev, plan, a, c.i8);
         }
     }
     if (rc) { cc_tensor_release(o); return rc; }

@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
     int from, to;
     pt_range(s, a, &from, &to);
     const int row0 = tile * TI_ROWS, n_rows = min(TI_ROWS, rows - row0), pos_first = s.pos0 + row0 / a.R, pos_last = s.pos0 + (row0 + n_rows - 1) / a.R;
-    const int each = pt_each(to - from, n_split, a), k0 = from + split * each, k1 = min(min(to, k0 + each), pos_last + 1);
+    const int each = pt_each(to - from, n_split), k0 = from + split * each, k1 = min(min(to, k0 + each), pos_last + 1);
     const int lo = a.window > 0 ? max(k0, (pos_first - a.window + 1) & ~(TI_KEYS - 1)) : k0, steps = k1 > lo ? (k1 - lo + TI_KEYS - 1) / TI_KEYS : 0;
     const int opens = I8 ? to >> a.shift << a.shift : 0;
     // the images of the first step, and what stands beside those of all steps
