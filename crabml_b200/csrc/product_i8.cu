@@ -13,13 +13,20 @@
 // ---- activations -> codes ------------------------------------------------------------------------------------------------------------------
 // round(127 x / a), ties to even, as the exact quotient rounds.  127 / a and the product err by less than 2e-5 of a step; where that leaves it open, and for rows whose
 // 127 / a is no ordinary number, the quotient is taken in 64 bits: two 24-bit numbers' quotient that is not a tie is 2^-25 of itself away from one at least.
-__device__ __forceinline__ int i8_code(float x, float a, float r) {
-    const float y = x * r, n = rintf(y);
-    if (fabsf(y - n) < 0.49998f && a > 1e-30f) return (int)n;
-    return (int)rint((double)x * 127.0 / (double)a);
-}
+// Four of them, one question for all (2048 rows of 4096: 12 us with a question each and conversions, 11 so): y + 1.5 * 2^23 has the nearest whole number in its lowest bits
+__device__ __forceinline__ int i8_code(float x, float a) { return (int)rint((double)x * 127.0 / (double)a); }
 __device__ __forceinline__ unsigned i8_code4(const float4& v, float a, float r) {
-    return ((unsigned)i8_code(v.x, a, r) & 255u) | ((unsigned)i8_code(v.y, a, r) & 255u) << 8 | ((unsigned)i8_code(v.z, a, r) & 255u) << 16 | (unsigned)i8_code(v.w, a, r) << 24;
+    constexpr float M = 12582912.0f;
+    const float y[4] = {v.x * r, v.y * r, v.z * r, v.w * r};
+    float n[4], far = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        n[i] = y[i] + M;
+        far = fmaxf(far, fabsf(y[i] - (n[i] - M)));
+    }
+    if (far < 0.49998f && a > 1e-30f)
+        return __byte_perm(__byte_perm(__float_as_uint(n[0]), __float_as_uint(n[1]), 0x0040), __byte_perm(__float_as_uint(n[2]), __float_as_uint(n[3]), 0x0040), 0x5410);
+    return ((unsigned)i8_code(v.x, a) & 255u) | ((unsigned)i8_code(v.y, a) & 255u) << 8 | ((unsigned)i8_code(v.z, a) & 255u) << 16 | (unsigned)i8_code(v.w, a) << 24;
 }
 __device__ __forceinline__ unsigned i8_top4(const float4& v) {
     const unsigned x = __float_as_uint(v.x) & 0x7fffffffu, y = __float_as_uint(v.y) & 0x7fffffffu, z = __float_as_uint(v.z) & 0x7fffffffu, w = __float_as_uint(v.w) & 0x7fffffffu;
@@ -32,7 +39,7 @@ __device__ __forceinline__ float4 i8_load4(const float* row, int c, int k, bool 
 }
 #define I8_THREADS 256
 #define I8_KEEP 4                            // float4 of a row that a thread keeps: rows of up to 16 THREADS are read once.  16 of them, 256 threads for all rows, left two CTAs
-                                             // an SM: 2048 rows of 4096 took 24 us instead of I8_ROWS_US
+                                             // an SM: 2048 rows of 4096 took 24 us instead of 11
 // codes [T][kp], zeros behind a row's k; factors [T].  A CTA a row
 template <int THREADS>
 __global__ void __launch_bounds__(THREADS) i8_rows_kernel(const float* __restrict__ x, int64_t rs, int k, int kp, int vec, int8_t* __restrict__ codes, float* __restrict__ factors) {
@@ -71,10 +78,11 @@ __global__ void __launch_bounds__(THREADS) i8_rows_kernel(const float* __restric
     if (threadIdx.x == 0) factors[t] = finite ? a / 127.0f : NAN;
 }
 
-// ---- up to I8_FEW tokens: one kernel ------------------------------------------------------------------------------------------------------------
-// Every CTA codes the tokens by itself, into shared memory, while its first weights are on their way; a warp takes an output channel, 4096 codes of it at a time,
-// the next ones under way behind the sums of these.
-#define I8_FEW 8
+// ---- one token: one kernel ------------------------------------------------------------------------------------------------------------------
+// Every CTA codes the token by itself, into shared memory, while its first weights are on their way; a warp takes an output channel, 4096 codes of it at a time,
+// the next ones under way behind the sums of these.  (From two tokens on the two kernels below are as fast or faster: this one with 2, 4 and 8 tokens against
+// 11008 x 4096 took 18, 28 and 56 us, they take 17.  So they are where every CTA would code much: one token against 11008 x 4096 14 and 17 us, 4096 x 14336 23 and 18.)
+#define I8_TOKEN_K 8192
 #define I8_RUN 8                             // pieces of 16 codes of a lane: 4096 codes of a warp
 // 16 codes of a row that may start anywhere: the five words around them; near the end of the matrix byte by byte
 __device__ __forceinline__ int4 i8_load16(const int8_t* p, const int8_t* end) {
@@ -89,11 +97,10 @@ __device__ __forceinline__ int4 i8_load16(const int8_t* p, const int8_t* end) {
         if (p + j < end) z[j / 4] |= (int)(uint8_t)p[j] << (j % 4 * 8);
     return make_int4(z[0], z[1], z[2], z[3]);
 }
-template <int TB>
-__global__ void __launch_bounds__(I8_THREADS) i8_few_kernel(const int8_t* __restrict__ w, const float* __restrict__ ws, const float* __restrict__ x, int64_t rs, float* __restrict__ out, int T,
-                                                            int m, int k, int kp, int vec) {
-    extern __shared__ __align__(16) int8_t i8_codes[];              // [TB][kp]
-    __shared__ unsigned tops[I8_THREADS / 32][TB];
+__global__ void __launch_bounds__(I8_THREADS) i8_token_kernel(const int8_t* __restrict__ w, const float* __restrict__ ws, const float* __restrict__ x, float* __restrict__ out, int m, int k, int kp,
+                                                              int vec) {
+    extern __shared__ __align__(16) int8_t i8_codes[];              // [kp]
+    __shared__ unsigned tops[I8_THREADS / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = gridDim.x * (I8_THREADS / 32), segs = (k + 4095) >> 12;
     const bool wide = (k & 15) == 0;
     const int8_t* end = w + (int64_t)m * k;
@@ -108,30 +115,18 @@ __global__ void __launch_bounds__(I8_THREADS) i8_few_kernel(const int8_t* __rest
     };
     pdl_enter();
     fetch(row, 0);
-    float xs[TB];
-#pragma unroll
-    for (int t = 0; t < TB; t++) {
-        unsigned top = 0;
-        if (t < T)
-            for (int c = threadIdx.x * 4; c < k; c += I8_THREADS * 4) top = max(top, i8_top4(i8_load4(x + t * rs, c, k, vec)));
-        top = __reduce_max_sync(0xffffffffu, top);
-        if (lane == 0) tops[warp][t] = top;
-    }
+    unsigned top = 0;
+    for (int c = threadIdx.x * 4; c < k; c += I8_THREADS * 4) top = max(top, i8_top4(i8_load4(x, c, k, vec)));
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) tops[warp] = top;
     __syncthreads();
 #pragma unroll
-    for (int t = 0; t < TB; t++) {
-        unsigned top = 0;
-#pragma unroll
-        for (int i = 0; i < I8_THREADS / 32; i++) top = max(top, tops[i][t]);
-        const bool finite = top < 0x7f800000u, some = finite && top && t < T;
-        const float a = __uint_as_float(top), r = 127.0f / a;
-        for (int c = threadIdx.x * 4; c < kp; c += I8_THREADS * 4) *(unsigned*)(i8_codes + t * kp + c) = some ? i8_code4(i8_load4(x + t * rs, c, k, vec), a, r) : 0u;
-        xs[t] = finite ? a / 127.0f : NAN;
-    }
+    for (int i = 0; i < I8_THREADS / 32; i++) top = max(top, tops[i]);
+    const bool finite = top < 0x7f800000u, some = finite && top;
+    const float a = __uint_as_float(top), xs = finite ? a / 127.0f : NAN;
+    for (int c = threadIdx.x * 4; c < kp; c += I8_THREADS * 4) *(unsigned*)(i8_codes + c) = some ? i8_code4(i8_load4(x, c, k, vec), a, 127.0f / a) : 0u;
     __syncthreads();
-    int acc[TB];
-#pragma unroll
-    for (int t = 0; t < TB; t++) acc[t] = 0;
+    int acc = 0;
     while (row < m) {
         int4 u[I8_RUN];
 #pragma unroll
@@ -143,32 +138,19 @@ __global__ void __launch_bounds__(I8_THREADS) i8_few_kernel(const int8_t* __rest
         for (int i = 0; i < I8_RUN; i++) {
             const int c = s * 4096 + i * 512 + lane * 16;
             if (c >= k) break;
-#pragma unroll
-            for (int t = 0; t < TB; t++) {
-                const int4 v = *(const int4*)(i8_codes + t * kp + c);
-                acc[t] = __dp4a(u[i].x, v.x, __dp4a(u[i].y, v.y, __dp4a(u[i].z, v.z, __dp4a(u[i].w, v.w, acc[t]))));
-            }
+            const int4 v = *(const int4*)(i8_codes + c);
+            acc = __dp4a(u[i].x, v.x, __dp4a(u[i].y, v.y, __dp4a(u[i].z, v.z, __dp4a(u[i].w, v.w, acc))));
         }
         if (seg) continue;
-        const float factor = ws[r];
-#pragma unroll
-        for (int t = 0; t < TB; t++) {
-            const int sum = __reduce_add_sync(0xffffffffu, acc[t]);
-            if (lane == 0 && t < T) out[(int64_t)t * m + r] = (float)sum * factor * xs[t];
-            acc[t] = 0;
-        }
+        const int sum = __reduce_add_sync(0xffffffffu, acc);
+        if (lane == 0) out[r] = (float)sum * ws[r] * xs;
+        acc = 0;
     }
 }
-template <int TB>
-static cudaError_t i8_launch_few(cc_device* dev, const int8_t* w, const float* ws, const float* x, int64_t rs, float* out, int T, int m, int k, int kp, int vec) {
-    const size_t smem = (size_t)TB * kp;
-    const int per = (int)std::min<size_t>(4, 200 * 1024 / (smem + 1024)), rows = I8_THREADS / 32;
-    const int64_t grid = std::min<int64_t>((m + rows - 1) / rows, (int64_t)per * dev->sm_count);
-    cudaError_t e = cudaSuccess;
-    if (smem > 48 * 1024) e = cudaFuncSetAttribute(i8_few_kernel<TB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) e = cc_launch_pdl(dev, i8_few_kernel<TB>, (unsigned)grid, I8_THREADS, smem, w, ws, x, rs, out, T, m, k, kp, vec);
+static cudaError_t i8_launch_token(cc_device* dev, const int8_t* w, const float* ws, const float* x, float* out, int m, int k, int kp, int vec) {
+    const int rows = I8_THREADS / 32;
     dev->launches++;
-    return e;
+    return cc_launch_pdl(dev, i8_token_kernel, (unsigned)std::min<int64_t>((m + rows - 1) / rows, (int64_t)4 * dev->sm_count), I8_THREADS, (size_t)kp, w, ws, x, out, m, k, kp, vec);
 }
 
 // ---- many rows: tcgen05.mma on 8-bit tiles -----------------------------------------------------------------------------------------------------
@@ -382,6 +364,179 @@ static int gi_launch(cc_device* dev, const int8_t* w, const float* ws, const int
     CC_LAUNCH_CHECK(dev);
     return CC_OK;
 }
+
+// ---- the same with two SMs on a tile ----------------------------------------------------------------------------------------------------------
+// A step of 128 x 256 x 128 takes the tensor core 512 cycles and brings 48 KB, which are written to shared memory and read from it once: 750 cycles of its 128 bytes.  A pair of SMs (a
+// cluster of two, cta_group::2) has 256 channels x BN tokens: each holds 128 channels and half of the tokens, 32 KB a step, and the pair's instruction reads both halves.  The
+// even CTA issues the products; the copies of both are counted on its barriers, and what it commits arrives in both.
+struct GpShared {
+    unsigned long long full[8], empty[8], acc_full[2], acc_empty[2], drained;
+    unsigned tmem_base;
+    int fail;
+};
+__host__ __device__ constexpr int gp_bytes(int bn) { return (128 + bn / 2) * GI_K; }
+__host__ __device__ constexpr int gp_stages(int bn) { return 192 * 1024 / gp_bytes(bn) < 8 ? 192 * 1024 / gp_bytes(bn) : 8; }
+__host__ __device__ constexpr size_t gp_smem(int bn) { return (size_t)gp_stages(bn) * gp_bytes(bn) + 1024; }
+__device__ __forceinline__ void gp_umma(unsigned tmem_d, uint64_t a, uint64_t b, unsigned idesc, unsigned accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// what this thread has issued so far arrives on the barrier, when it is complete, in both CTAs
+__device__ __forceinline__ void gp_commit(unsigned bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ unsigned gp_even(unsigned addr) {         // the even CTA's own of it
+    unsigned a;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(addr));
+    return a;
+}
+__device__ __forceinline__ void gp_tma_load(unsigned dst, const void* tmap, unsigned bar, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(tmap), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+template <int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GI_THREADS, 1) i8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_cut,
+                                                                                         const float* __restrict__ ws, const float* __restrict__ xs, float* __restrict__ out, int T, int m, int steps, int n_whole, int cut,
+                                                                                         int n_tiles, unsigned* err_dev, unsigned* err_host) {
+    namespace cg = cooperative_groups;
+    constexpr int ST = gp_stages(BN);
+    constexpr unsigned A_BYTES = 128 * GI_K, BYTES = gp_bytes(BN), COLS = 2 * BN;
+    extern __shared__ __align__(1024) uint8_t gi_raw[];
+    __shared__ GpShared sh;
+    uint8_t* ring = (uint8_t*)(((uintptr_t)gi_raw + 1023) & ~(uintptr_t)1023);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cg::this_cluster().block_rank();
+    const int tiles_n = (T + BN - 1) / BN, first = blockIdx.x / 2, stride = gridDim.x / 2;
+    // the first n_whole tiles are 256 x BN, the ones behind them BN / cut wide
+    auto place = [&](int tile, int& mt, int& n0) {
+        const int of = tile < n_whole ? tile : n_whole + (tile - n_whole) / cut;
+        mt = of / tiles_n;
+        n0 = (of - mt * tiles_n) * BN + (tile < n_whole ? 0 : (tile - n_whole) % cut * (BN / cut));
+        return tile < n_whole ? BN : BN / cut;
+    };
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < ST; i++) { pg_mbar_init(pg_smem(&sh.full[i]), 1); pg_mbar_init(pg_smem(&sh.empty[i]), 1); }
+        for (int i = 0; i < 2; i++) { pg_mbar_init(pg_smem(&sh.acc_full[i]), 1); pg_mbar_init(pg_smem(&sh.acc_empty[i]), 8); }
+        pg_mbar_init(pg_smem(&sh.drained), 1);
+        sh.fail = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pg_smem(&sh.tmem_base)), "n"(COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    pg_fence_before();
+    __syncthreads();
+    cg::this_cluster().sync();
+    pg_fence_after();
+    const unsigned tmem = sh.tmem_base;
+    pdl_enter();
+    if (warp == 0) {
+        if (lane == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
+            unsigned g = 0;
+            bool ok = true;
+            for (int tile = first; tile < n_tiles && ok; tile += stride) {
+                int mt, n0;
+                const int wide = place(tile, mt, n0);
+                for (int s = 0; s < steps; s++, g++) {
+                    const unsigned slot = g % ST, own = pg_smem(&sh.full[slot]), full = gp_even(own), at = pg_smem(ring + (size_t)slot * BYTES);
+                    if (!(ok = sg_wait(pg_smem(&sh.empty[slot]), ((g / ST) & 1u) ^ 1u, &sh.fail))) break;
+                    if (rank == 0) pg_mbar_expect_tx(own, 2 * A_BYTES + wide * GI_K);
+                    gp_tma_load(at, &map_w, full, s * GI_K, mt * 256 + rank * 128);
+                    gp_tma_load(at + A_BYTES, wide == BN ? &map_x : &map_cut, full, s * GI_K, n0 + rank * (wide / 2));
+                }
+            }
+            int never = 0;                                            // no copy is under way when the CTAs end (the even one sees those of both), and no arrival
+            for (unsigned i = g > ST ? g - ST : 0; i < g; i++) {
+                if (rank == 0) sg_wait(pg_smem(&sh.full[i % ST]), (i / ST) & 1u, &never);
+                sg_wait(pg_smem(&sh.empty[i % ST]), (i / ST) & 1u, &never);
+            }
+            if (!ok || never)                                         // something did not come in time: a while for whatever is still to
+                for (int i = 0; i < 1000; i++) __nanosleep(1000);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        int never = 0;                                                // nothing is in flight when the TMEM is given back
+        if (lane == 0 && rank == 1) sg_wait(pg_smem(&sh.drained), 0, &never);
+        if (lane == 0 && rank == 0) {
+            unsigned g = 0, nth = 0;
+            bool ok = true;
+            for (int tile = first; tile < n_tiles && ok; tile += stride, nth++) {
+                int mt, n0;
+                const unsigned acc = tmem + (nth & 1u) * BN, desc = gi_desc(place(tile, mt, n0)) + (8u << 24);
+                if (!(ok = sg_wait(pg_smem(&sh.acc_empty[nth & 1u]), ((nth >> 1) & 1u) ^ 1u, &sh.fail))) break;
+                pg_fence_after();
+                for (int s = 0; s < steps; s++, g++) {
+                    const unsigned slot = g % ST, at = pg_smem(ring + (size_t)slot * BYTES);
+                    if (!(ok = sg_wait(pg_smem(&sh.full[slot]), (g / ST) & 1u, &sh.fail))) break;
+                    pg_fence_after();
+                    const uint64_t a = pg_smem_desc(at), b = pg_smem_desc(at + A_BYTES);
+#pragma unroll
+                    for (int kk = 0; kk < GI_K / 32; kk++) gp_umma(acc, a + 2 * kk, b + 2 * kk, desc, s > 0 || kk > 0);
+                    gp_commit(pg_smem(&sh.empty[slot]));
+                }
+                if (ok) gp_commit(pg_smem(&sh.acc_full[nth & 1u]));
+            }
+            gp_commit(pg_smem(&sh.drained));
+            sg_wait(pg_smem(&sh.drained), 0, &never);
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        const int q = warp & 3;
+        unsigned nth = 0;
+        for (int tile = first; tile < n_tiles; tile += stride, nth++) {
+            int mt, n0;
+            const int wide = place(tile, mt, n0), row = mt * 256 + rank * 128 + q * 32 + lane;
+            if (!sg_wait_warp(pg_smem(&sh.acc_full[nth & 1u]), (nth >> 1) & 1u, &sh.fail)) break;
+            pg_fence_after();
+            const unsigned from = tmem + (nth & 1u) * BN + ((unsigned)(q * 32) << 16);
+            const float factor = row < m ? ws[row] : 0.0f;
+#pragma unroll 1
+            for (int c0 = 0; c0 < wide && n0 + c0 < T; c0 += 32) {
+                unsigned v[32];
+                gi_load<32>(from + c0, v);
+                const float mine = n0 + c0 + lane < T ? xs[n0 + c0 + lane] : 0.0f;
+                float* o = out + (int64_t)(n0 + c0) * m + row;
+#pragma unroll
+                for (int j = 0; j < 32; j++) {
+                    const float f = __shfl_sync(0xffffffffu, mine, j);
+                    if (row < m && n0 + c0 + j < T) *o = (float)(int)v[j] * factor * f;
+                    o += m;
+                }
+            }
+            pg_fence_before();                                        // the accumulator may be filled again
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(gp_even(pg_smem(&sh.acc_empty[nth & 1u]))) : "memory");
+        }
+    }
+    pg_fence_before();
+    __syncthreads();
+    cg::this_cluster().sync();
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(COLS) : "memory");
+    if (threadIdx.x == 0 && sh.fail) {
+        if (err_dev) atomicExch(err_dev, 5u);
+        if (err_host) { *(volatile unsigned*)err_host = 5u; __threadfence_system(); }
+    }
+}
+// tiles of 256 x 256, whole waves of them; those of the last one that is not full are cut across the tokens, as far as there are pairs: 2048 tokens, 14336 x 4096 are 6 waves of 74 and 4 tiles more
+static int gp_launch(cc_device* dev, const int8_t* w, const float* ws, const int8_t* x, const float* xs, float* out, int T, int m, int kp) {
+    constexpr int BN = 256;
+    const int64_t tiles = (int64_t)((m + 255) / 256) * ((T + BN - 1) / BN);
+    CC_REQUIRE(dev, tiles < ((int64_t)1 << 30), "product_i8: %lld tiles", (long long)tiles);
+    const int pairs = dev->sm_count / 2, rest = (int)(tiles % pairs), whole = (int)tiles - rest;
+    int cut = 1;
+    while (cut < 8 && rest * cut * 2 <= pairs) cut *= 2;
+    CUtensorMap mw, mx, mc;
+    int rc = cc_make_tmap_i8(dev, &mw, w, m, kp, 128);
+    if (!rc) rc = cc_make_tmap_i8(dev, &mx, x, T, kp, BN / 2);
+    if (!rc) rc = cc_make_tmap_i8(dev, &mc, x, T, kp, BN / 2 / cut);
+    if (rc) return rc;
+    CC_CUDA(dev, cudaFuncSetAttribute(i8_pair_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)gp_smem(BN)));
+    CC_CUDA(dev, cc_launch_pdl(dev, i8_pair_kernel<BN>, (unsigned)(2 * std::min(whole + rest * cut, pairs)), GI_THREADS, gp_smem(BN), mw, mx, mc, ws, xs, out, T, m, (kp + GI_K - 1) / GI_K, whole, cut,
+                               whole + rest * cut, dev->err_dev, dev->err_host));
+    dev->launches++;
+    return CC_OK;
+}
+
 // rows of k codes -> rows of kp, zeros behind: what TMA can read where k is no multiple of 16
 __global__ void i8_pad_kernel(const int8_t* __restrict__ w, int8_t* __restrict__ to, int64_t n4, int k, int kp4) {
     pdl_enter();
@@ -399,9 +554,8 @@ __global__ void i8_pad_kernel(const int8_t* __restrict__ w, int8_t* __restrict__
 static int i8_product(cc_device* dev, const int8_t* w, const float* ws, const float* x, int64_t rs, float* out, int T, int m, int k) {
     const int kp = (k + 15) / 16 * 16, vec = rs % 4 == 0 && ((uintptr_t)x & 15) == 0;
     cudaError_t e;
-    if (T <= I8_FEW && (size_t)(T <= 1 ? 1 : T <= 2 ? 2 : T <= 4 ? 4 : 8) * kp <= 160 * 1024) {
-        e = T <= 1 ? i8_launch_few<1>(dev, w, ws, x, rs, out, T, m, k, kp, vec) : T <= 2 ? i8_launch_few<2>(dev, w, ws, x, rs, out, T, m, k, kp, vec)
-            : T <= 4 ? i8_launch_few<4>(dev, w, ws, x, rs, out, T, m, k, kp, vec) : i8_launch_few<8>(dev, w, ws, x, rs, out, T, m, k, kp, vec);
+    if (T == 1 && k <= I8_TOKEN_K) {
+        e = i8_launch_token(dev, w, ws, x, out, m, k, kp, vec);
         return e == cudaSuccess ? CC_OK : cc_fail(dev, CC_ERR_CUDA, "product_i8: %s", cudaGetErrorString(e));
     }
     const bool pad = k != kp;
@@ -422,6 +576,9 @@ static int i8_product(cc_device* dev, const int8_t* w, const float* ws, const fl
         w = wp;
     }
     if (e != cudaSuccess) rc = cc_fail(dev, CC_ERR_CUDA, "product_i8: %s", cudaGetErrorString(e));
+    // Whole waves of tiles of 256 x 256 for pairs of SMs: those (2048 tokens, 14336 x 4096: 102 us instead of 115 with one SM a tile; 512 tokens, 11008 x 4096: 40 and 43).  Else tiles of 128
+    // channels, whose depth a cluster shares where they are few (512 tokens, 4096 x 14336: 47 us, by pairs 59), as wide as the tokens: 16 columns cost a step what its weights cost
+    else if (T > 128 && (int64_t)((m + 255) / 256) * ((T + 255) / 256) >= dev->sm_count / 2) rc = gp_launch(dev, w, ws, xq, xs, out, T, m, kp);
     else rc = T <= 16 ? gi_launch<16>(dev, w, ws, xq, xs, out, T, m, kp) : T <= 32 ? gi_launch<32>(dev, w, ws, xq, xs, out, T, m, kp)
               : T <= 64 ? gi_launch<64>(dev, w, ws, xq, xs, out, T, m, kp) : T <= 128 ? gi_launch<128>(dev, w, ws, xq, xs, out, T, m, kp) : gi_launch<256>(dev, w, ws, xq, xs, out, T, m, kp);
     cc_pool_free(dev, mem, cls);

@@ -42,6 +42,14 @@ def test_product(dev, rows, m, k):
     check(dev, w, ws, r.normal(size=(rows, k)).astype(np.float32) * np.float32(10.0 ** r.uniform(-3, 3)))
 
 
+@pytest.mark.parametrize("rows,m,k", [(129, 19000, 64), (300, 9500, 130), (600, 9217, 272), (1100, 6145, 16), (1500, 13000, 48)])
+def test_product_of_many_tiles(dev, rows, m, k):
+    """more tiles than pairs of SMs, with a last wave of few, of many, and of tiles that end behind the tokens and the channels"""
+    r = np.random.default_rng(m)
+    w, ws = weights(r, m, k)
+    check(dev, w, ws, r.normal(size=(rows, k)).astype(np.float32))
+
+
 @pytest.mark.parametrize("rows", [1, 20, 200])
 def test_extremes(dev, rows):
     """the largest sums there are, -128 among the weights, rows of zeros, of tiny and of huge numbers"""
