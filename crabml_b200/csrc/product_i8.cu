@@ -166,7 +166,9 @@ struct GiShared {
     unsigned tmem_base;
     int fail;
 };
-__host__ __device__ constexpr int gi_stages(int bn) { return 192 * 1024 / ((128 + bn) * GI_K) < 8 ? 192 * 1024 / ((128 + bn) * GI_K) : 8; }
+__host__ __device__ constexpr int gi_ctas(int bn) { return bn <= 32 ? 2 : 1; }      // of an SM: narrow tiles are read from memory, and twice as many may share a depth
+__host__ __device__ constexpr int gi_ring(int bn) { return (gi_ctas(bn) == 2 ? 112 : 192) * 1024 / ((128 + bn) * GI_K); }
+__host__ __device__ constexpr int gi_stages(int bn) { return gi_ring(bn) < 8 ? gi_ring(bn) : 8; }
 __host__ __device__ constexpr size_t gi_smem(int bn) { return (size_t)gi_stages(bn) * (128 + bn) * GI_K + 1024; }
 __device__ __forceinline__ void gi_umma(unsigned tmem_d, uint64_t a, uint64_t b, unsigned idesc, unsigned accumulate) {
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
@@ -185,7 +187,7 @@ __device__ __forceinline__ void gi_load(unsigned addr, unsigned (&v)[N]) {
 }
 
 template <int BN>
-__global__ void __launch_bounds__(GI_THREADS, 1) i8_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const float* __restrict__ ws,
+__global__ void __launch_bounds__(GI_THREADS, gi_ctas(BN)) i8_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const float* __restrict__ ws,
                                                                 const float* __restrict__ xs, float* __restrict__ out, int T, int m, int steps_all, int n_tiles, int parts, unsigned* err_dev,
                                                                 unsigned* err_host) {
     namespace cg = cooperative_groups;
@@ -346,12 +348,12 @@ static int gi_launch(cc_device* dev, const int8_t* w, const float* ws, const int
     if (!rc) rc = cc_make_tmap_i8(dev, &mx, x, T, kp, BN);
     if (rc) return rc;
     const int64_t tiles = (int64_t)((m + 127) / 128) * ((T + BN - 1) / BN);
-    const int steps = (kp + GI_K - 1) / GI_K;
+    const int steps = (kp + GI_K - 1) / GI_K, slots = gi_ctas(BN) * dev->sm_count;
     int parts = 1;
-    while (parts < 4 && tiles * parts * 2 <= dev->sm_count && steps / (parts * 2) >= 2) parts *= 2;
+    while (parts < 4 && tiles * parts * 2 <= slots && steps / (parts * 2) >= 2) parts *= 2;
     CC_REQUIRE(dev, tiles < ((int64_t)1 << 30), "product_i8: %lld tiles", (long long)tiles);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(parts > 1 ? tiles * parts : tiles < dev->sm_count ? tiles : dev->sm_count));
+    cfg.gridDim = dim3((unsigned)(parts > 1 ? tiles * parts : tiles < slots ? tiles : slots));
     cfg.blockDim = dim3(GI_THREADS); cfg.dynamicSmemBytes = gi_smem(BN); cfg.stream = dev->stream;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
