@@ -390,6 +390,67 @@ def test_many_sequences(dev):
     check_attention(dev, 16, 1, 2, 32, 32, True, pos0, counts, seed=6)
 
 
+@pytest.mark.parametrize("i8", [False, True], ids=["f16", "i8"])
+@pytest.mark.parametrize("seed,G,Rh,d,n,top,window", [(1, 3, 4, 64, 20, 1500, 0), (2, 2, 8, 128, 40, 900, 0), (3, 1, 1, 32, 3, 9000, 0), (4, 4, 5, 80, 9, 3000, 700), (5, 1, 2, 256, 12, 2500, 0), (6, 8, 1, 16, 30, 600, 0)])
+def test_attention_in_runs(dev, seed, G, Rh, d, n, top, window, i8):
+    """few rows over sequences of all lengths: equal runs of keys begin and end anywhere in them"""
+    r = np.random.default_rng(seed)
+    pos0 = np.where(r.random(n) < 0.3, r.integers(0, 70, n), r.integers(0, top, n)).tolist()
+    counts = r.choice([0, 1, 1, 1, 2, 32 // Rh], n).tolist()
+    pos0[0], counts[0] = top, 1
+    check_attention(dev, 32, G, Rh, d, d, i8, pos0, counts, window=window, seed=seed)
+
+
+@pytest.mark.parametrize("i8", [False, True], ids=["f16", "i8"])
+def test_rows_over_thousands_of_keys(dev, i8):
+    """eight rows at a time over more keys than a CTA holds page numbers of"""
+    d, Rh, pos0, n = 256, 8, 4400, 1190
+    c = Case(dev, 16, 1, d, d, i8, [pos0], [n], seed=3)
+    q = c.rng.normal(size=(n, Rh, d)).astype(np.float32)
+    scale = d ** -0.5 / (60 if i8 else 1)
+    got = take(dev, paged.attention(c.plan(), c.cache, give(dev, q.reshape(n, -1)), Rh, scale)).reshape(n, Rh, d)
+    k, v = (c.ref.rows(m, c.table[0], pos0 + n, c.slot(0)) for m in ("k", "v"))
+    for t in (0, 600, n - 3):
+        want, mass, reach = R.attention(q[t:t + 3], k[:, :pos0 + t + 3], v[:, :pos0 + t + 3], pos0 + t, float(np.float32(scale)))
+        assert (np.abs(got[t:t + 3] - want) <= R.attention_bound(mass, reach, d, pos0 + t + 3)).all()
+
+
+@pytest.mark.parametrize("i8", [False, True], ids=["f16", "i8"])
+def test_many_rows_over_many_keys(dev, i8):
+    """many rows whose keys and values, all heads' together, are more than are unpacked at a time"""
+    G, d, pos0, n, seqs = 8, 128, 2968, 40, 24
+    c = Case(dev, 64, G, d, d, i8, [pos0] + [0] * (seqs - 1), [n] + [0] * (seqs - 1), spare=seqs, seed=4)
+    assert (pos0 + n) % 64 == 0
+    last, spare = c.table[0][-1], sorted(set(range(c.n_pages)) - set(c.table[0]))
+    for name in ("k", "v") + (("k_scale", "v_scale") if i8 else ()):
+        c.ref.a[name][spare] = c.ref.a[name][last]
+    c.cache = paged.PagedCache(**{m: give(dev, a) for m, a in c.ref.a.items()})
+    table = [c.table[0][:-1] + [p] for p in [last] + spare[:seqs - 1]]               # all read the same pages but the last, whose contents are the same
+    plan = paged.PagePlan(dev, 64, c.n_pages, table, [pos0] * seqs, [n] * seqs, c.n_slots, c.slots)
+    q = c.rng.normal(size=(n, G, d)).astype(np.float32)
+    scale = d ** -0.5 / (60 if i8 else 1)
+    got = take(dev, paged.attention(plan, c.cache, give(dev, np.tile(q.reshape(n, -1), (seqs, 1))), G, scale)).reshape(seqs, n, G, d)
+    k, v = (c.ref.rows(m, c.table[0], pos0 + n, c.slot(0)) for m in ("k", "v"))
+    want, mass, reach = R.attention(q, k, v, pos0, float(np.float32(scale)))
+    assert (np.abs(got[0] - want) <= R.attention_bound(mass, reach, d, pos0 + n)).all()
+    for i in range(1, seqs):
+        np.testing.assert_array_equal(got[i], got[0])
+
+
+@pytest.mark.parametrize("i8", [False, True], ids=["f16", "i8"])
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1e-20])
+def test_attention_scales(dev, scale, i8):
+    """the smallest scores are the largest, and every key weighs the same"""
+    c = Case(dev, 16, 1, 32, 32, i8, [700, 20], [2, 60], seed=12)
+    q = (c.rng.normal(size=(62, 2, 32)) / (60 if i8 else 1)).astype(np.float32)
+    got = take(dev, paged.attention(c.plan(), c.cache, give(dev, q.reshape(62, -1)), 2, scale)).reshape(62, 2, 32)
+    for i, (lo, hi) in enumerate(((0, 2), (2, 62))):
+        end = c.pos0[i] + hi - lo
+        k, v = (c.ref.rows(m, c.table[i], end, c.slot(i)) for m in ("k", "v"))
+        want, mass, reach = R.attention(q[lo:hi], k, v, c.pos0[i], float(np.float32(scale)))
+        assert (np.abs(got[lo:hi] - want) <= R.attention_bound(mass, reach, 32, end)).all()
+
+
 def test_offsets_beyond_32_bits(dev):
     """pages behind element 2^31 of their tensor"""
     G, d, P, n = 8, 128, 64, 33000
