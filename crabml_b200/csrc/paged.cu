@@ -191,8 +191,8 @@ __global__ void __launch_bounds__(PA_THREADS, 4) paged_append_kernel(const PaArg
     __shared__ unsigned tops[PA_WARPS];
     const int job = blockIdx.y, tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
     const bool is_k = job < a.G, is_v = !is_k && job < 2 * a.G, is_q = !is_k && !is_v;
-    if (!is_q && blockIdx.x >= n_items) return;
     pdl_enter();
+    if (!is_q && blockIdx.x >= n_items) return;
     for (int at = blockIdx.x; at >= 0;) {
         const PgSegment g = a.segments[at];
         at = is_q ? -1 : g.next;
@@ -323,7 +323,7 @@ extern "C" CC_API int cc_paged_append(cc_device* dev, const cc_page_plan* plan, 
     if (q_src) PG_ROWS(dev, q_src, "paged_append queries");
     const int64_t T = plan->tokens;
     CC_REQUIRE(dev, k_src->shape[0] == T && v_src->shape[0] == T && (!q_src || q_src->shape[0] == T), "paged_append: the plan has %lld tokens, not the sources' rows", (long long)T);
-    CC_REQUIRE(dev, !q_src || (H > 0 && H <= 65536 && H % c.G == 0), "paged_append: %d query heads over %d", H, c.G);
+    CC_REQUIRE(dev, !q_src || (H > 0 && H <= 8192 && H % c.G == 0), "paged_append: %d query heads over %d", H, c.G);
     CC_REQUIRE(dev, k_col0 >= 0 && v_col0 >= 0 && k_col0 + (int64_t)c.G * c.dk <= k_src->shape[1] && v_col0 + (int64_t)c.G * c.dv <= v_src->shape[1] &&
                (!q_src || (q_col0 >= 0 && q_col0 + (int64_t)H * c.dk <= q_src->shape[1])), "paged_append: columns %d / %d / %d do not fit %d and %d heads of %d and %d", q_col0,
                k_col0, v_col0, H, c.G, c.dk, c.dv);

@@ -36,7 +36,7 @@ CC_API void cc_page_plan_release(cc_page_plan* plan);
 CC_API int64_t cc_page_plan_tokens(const cc_page_plan* plan);
 
 /* ---- a layer's cache -------------------------------------------------------------------------------------------------------------- */
-/* k: [n_pages, n_kv, page_size, dk], v: [n_pages, n_kv, page_size, dv]; dk and dv multiples of 16, up to 256.
+/* k: [n_pages, n_kv, page_size, dk], v: [n_pages, n_kv, page_size, dv]; dk and dv multiples of 16, up to 256; n_kv up to 1024, and n_heads, a multiple of it, up to 8192.
  * F16: every row rounded to 16 bits; the other four are not used (buf NULL).
  * I8: a page holds a block of page_size tokens once all of them are there.  Per head, with a the largest magnitude of the block's 16-bit numbers x: the factor
  *   a / 127 in k_scale, v_scale [n_pages, n_kv] (F32) and the codes round(127 x / a), ties to even; every number is rounded to 8 bits once, whatever portions a
