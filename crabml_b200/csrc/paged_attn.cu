@@ -7,6 +7,8 @@
 // products are one instruction whose accumulators a thread adds up itself.  A warp takes 16 keys at a time.  Its lanes keep, read and convert the pieces of the
 // cache that the instruction's layout gives them and no others: which four columns of a row a lane puts into a step is free as long as queries and keys agree, and so
 // is the order of the value columns, so a lane takes 16 neighbouring bytes of a row, and the way through shared memory (cp.async, a ring per warp) needs no barrier.
+// Keys and values are read once, so memory bounds it: 64 sequences of up to 4000 tokens (268 MB, 41 us) take 82 us, 16 sequences in 16-bit pages (311 MB, 47 us) 75.  While all CTAs
+// stream they read 5.6 to 6 TB/s; the rest is what a CTA does before and behind each segment (7 us to its first rows), and the kernel that adds up cut segments (5 us).
 #include <math.h>
 
 #include <algorithm>
@@ -20,8 +22,9 @@
 #define PT_STEP 64                            // keys that few rows are dealt out by
 #define PT_BEGIN 5                            // what a segment's begin and end cost, in steps (finding it, the queries, the sums: 13 thousand cycles)
 #define PT_CHUNK 4096                         // keys whose page numbers and factors a CTA holds at a time
-#define PT_FEW 32
-#define PT_TILE 72
+#define PT_FEW 32                             // rows of a sequence and key head, 8 at a time; more go to tiles of 128.  16 sequences at 2000 tokens, 32 heads on 8, 8-bit pages, us by 8 and by 128:
+                                              // 16 rows 52 and 118, 32 rows 86 and 123, 64 rows 149 and 135; one sequence at 4000: 25 and 39 with 32 rows, 49 and 42 with 128
+#define PT_TILE 72                            // floats from one tile of 8 x 8 sums to the next
 #define PT_LOG2E 1.4426950408889634f
 
 struct TiInfo;
@@ -378,7 +381,7 @@ __global__ void __launch_bounds__(PT_THREADS, D <= 64 ? 4 : D <= 128 ? 3 : 1) pa
     const PgSeq s = a.seqs[seq];
     pt_range(s, a, &from, &to);
     const int all = pt_steps(s, a), upto = deal.ctas ? min(all, off + run - at) : all;
-    const int rows = s.count * a.R, tile = seg / a.G, kvh = seg - tile * a.G, slot = 2 * c + (at == 0 ? 0 : 1);
+    const int rows = s.count * a.R, nth = seg / a.G, kvh = seg - nth * a.G, tile = deal.ctas ? nth : (rows + 7) / 8 - 1 - nth, slot = 2 * c + (at == 0 ? 0 : 1);
     const bool whole = off <= PT_BEGIN && upto == all;
     at += upto - off;
     if (upto <= PT_BEGIN) break;                                   // the next CTA has all its keys
@@ -616,8 +619,10 @@ static int pt_deal(const cc_page_plan* plan, const PtArgs& a, int64_t steps, PtD
     }
     return n_cuts;
 }
-// Sequences of few rows.  Segments of up to PT_WHOLE steps, or very many of them: a CTA each, nothing to add up.  Longer ones: all steps in equal runs, as many CTAs as the device holds
-// at a time, so that none waits for a last wave and few begin anew.  (Slices of up to 1024 keys, a CTA each: 64 sequences of up to 4000 tokens, 32 heads on 8, 8-bit pages: 90 us, in runs 82; 16-bit pages 77 and 75)
+// Sequences of few rows, or of any where heads are too wide for tiles of 128.  All steps in equal runs, as many CTAs as the device holds at a time, so that none waits for a last wave and few
+// begin anew.  (Slices of up to 1024 keys, a CTA each: 64 sequences of up to 4000 tokens, 32 heads on 8, 8-bit pages: 90 us, in runs 82; 16-bit pages 77 and 75.)
+// Segments of up to PT_WHOLE steps: a CTA each, nothing to add up (64 sequences at 250 tokens 28 us, in runs 35; at 500 38 and 39, at 1000 57 and 52; 16 at 500 15 and 22, at 1000 32 and 25).
+// Prompts of wide heads likewise, late rows first: their early rows see less than a run counts (1000 tokens, 16 heads of 256 on 4: 346 us, in runs 561)
 #define PT_WHOLE 8
 static int pt_run_few(cc_device* dev, const cc_page_plan* plan, PtArgs a, bool i8) {
     int64_t segments = 0, steps = 0;
@@ -636,7 +641,7 @@ static int pt_run_few(cc_device* dev, const cc_page_plan* plan, PtArgs a, bool i
     const int64_t slots = std::min<int64_t>(PT_CTAS, (int64_t)per_sm * dev->sm_count);
     PtDeal deal;
     PtCuts cuts;
-    deal.ctas = most <= PT_WHOLE || segments >= 8 * slots ? 0 : (int)std::min<int64_t>(slots, (steps + PT_BEGIN + 1) / (PT_BEGIN + 2));
+    deal.ctas = most <= PT_WHOLE || (a.rows_hi > PT_FEW && segments >= 8 * slots) ? 0 : (int)std::min<int64_t>(slots, (steps + PT_BEGIN + 1) / (PT_BEGIN + 2));
     const int n_cuts = deal.ctas ? pt_deal(plan, a, steps, deal, cuts) : 0;
     void* ws = nullptr; size_t cls = 0;
     if (n_cuts) {
@@ -720,7 +725,7 @@ extern "C" CC_API int cc_paged_attention(cc_device* dev, const cc_page_plan* pla
     PG_ROWS(dev, q, "paged_attention q");
     CC_REQUIRE(dev, view_contiguous(q), "paged_attention q: not contiguous");
     const int64_t T = plan->tokens;
-    CC_REQUIRE(dev, H > 0 && H <= 65536 && H % c.G == 0, "paged_attention: %d query heads over %d", H, c.G);
+    CC_REQUIRE(dev, H > 0 && H <= 8192 && H % c.G == 0, "paged_attention: %d query heads over %d", H, c.G);
     CC_REQUIRE(dev, q->shape[0] == T && q->shape[1] == (int64_t)H * c.dk, "paged_attention: q is not [%lld, %d * %d]", (long long)T, H, c.dk);
     if (sink) {
         if (!view_ok(sink)) return cc_fail(dev, CC_ERR_ARG, "paged_attention: bad view of sink");
@@ -738,7 +743,7 @@ extern "C" CC_API int cc_paged_attention(cc_device* dev, const cc_page_plan* pla
         a.scale = scale; a.softcap = softcap; a.window = window > 0 ? window : 0;
         a.n_seqs = plan->n_seqs; a.table_cols = plan->table_cols; a.page = plan->page; a.shift = plan->shift;
         a.H = H; a.G = c.G; a.R = H / c.G; a.dk = c.dk; a.dv = c.dv;
-        // rows of a sequence and key head: up to PT_FEW in tiles of 8, more in tiles of 128 where a head's numbers have room there
+        // up to PT_FEW rows in tiles of 8, more in tiles of 128 where a head's numbers have room there
         a.rows_lo = 1; a.rows_hi = c.dk <= TI_D && c.dv <= TI_D ? PT_FEW : 0x7fffffff; a.tile_rows = 8; a.align = 16;
         rc = pt_run_few(dev, plan, a, c.i8);
         if (!rc && a.rows_hi == PT_FEW) {

@@ -16,26 +16,30 @@ from .capi import TensorError
 from .tensor import CudaTensor, TensorStrider, _Buf
 
 
+def _whole(what, a, kind):
+    """an array of whole numbers that `kind` can hold, or a refusal: none is cut off or wrapped on its way"""
+    a = np.asarray(a)
+    if a.size and (a.dtype.kind not in "iu" or int(a.min()) < np.iinfo(kind).min or int(a.max()) > np.iinfo(kind).max):
+        raise TensorError(f"page_plan: {what} are not whole numbers of {np.dtype(kind).itemsize * 8} bits")
+    return np.ascontiguousarray(a, kind)
+
+
 class PagePlan:
     """What the sequences of a step have in the cache (pos0), bring along (counts) and own (table: rows of page numbers, an array or lists of any lengths; slots:
     their open blocks, sequence i slot i where it is None).  Checked once; every layer's append and attention take it."""
 
     def __init__(self, device, page_size, n_pages, table, pos0, counts, n_slots=0, slots=None):
         self.device, self.handle = device, None
-        counts = np.ascontiguousarray(counts, np.int32).reshape(-1)
-        pos0 = np.ascontiguousarray(pos0, np.int64).reshape(-1)
+        counts, pos0 = _whole("counts", counts, np.int32).reshape(-1), _whole("positions", pos0, np.int64).reshape(-1)
         n = len(counts)
         if not isinstance(table, np.ndarray):
             rows, width = [list(r) for r in table], max([len(r) for r in table], default=0)
             table = np.full((len(rows), width), -1, np.int32)       # a page that is needed and was not given is refused
             for i, r in enumerate(rows):
-                table[i, :len(r)] = r
+                table[i, :len(r)] = _whole("page numbers", r, np.int32)
         if len(pos0) != n or table.ndim != 2 or len(table) != n or (slots is not None and len(slots) != n):
             raise TensorError(f"page_plan: {n} counts, {len(pos0)} positions, table {table.shape}" + ("" if slots is None else f", {len(slots)} slots"))
-        if table.size and (table.min() < -(1 << 31) or table.max() >= 1 << 31):
-            raise TensorError("page_plan: page numbers of more than 32 bits")
-        table = np.ascontiguousarray(table, np.int32)
-        slots = None if slots is None else np.ascontiguousarray(slots, np.int32)
+        table, slots = _whole("page numbers", table, np.int32), None if slots is None else _whole("slots", slots, np.int32).reshape(-1)
         d = capi.cc_page_plan_desc(n, int(page_size), table.shape[1], int(n_pages), int(n_slots), *(None if a is None else a.ctypes.data for a in (pos0, counts, table, slots)))
         h = C.c_void_p()
         device.check(device.lib.cc_page_plan_create(device.handle, C.byref(d), C.byref(h)))

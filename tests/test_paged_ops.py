@@ -521,6 +521,9 @@ def test_refusals(dev):
         for call in (append, attend):
             with pytest.raises((TensorError, CudaError)):
                 call(cache=paged.PagedCache(**x))
+    for call in (append, attend):
+        with pytest.raises((TensorError, CudaError)):
+            call(heads=8194)
     for kw in (dict(src=short), dict(kc=H * d + 1, vc=(H + G) * d + 1), dict(kc=-1), dict(vc=1 << 30), dict(heads=3), dict(heads=0), dict(pairing=2), dict(freq=f, offset=1),
                dict(freq=f, offset=-1), dict(freq=give(dev, np.zeros(4, np.int8)))):
         with pytest.raises((TensorError, CudaError)):

@@ -114,3 +114,15 @@ def test_segments(build, seed):
             reads = h["row0"] > 0 and h["flags"] & FULL
             if a != b and g["flags"] & KEPT and reads and g["half"] == h["half"]:
                 assert where[a][0] == where[b][0] and where[a][1] > where[b][1]
+
+
+def test_numbers_that_are_not_whole_or_too_large():
+    """a plan takes them as they are or not at all"""
+    import numpy as np
+
+    from crabml_b200 import TensorError, paged
+    good = dict(table=[[0, 1]], pos0=[3], counts=[1], slots=[0])
+    for bad in (dict(counts=[1.5]), dict(counts=np.array([(1 << 32) + 1])), dict(pos0=[0.5]), dict(slots=np.array([1 << 32])), dict(table=[[0, 1.5]]), dict(table=[[1 << 40]]),
+                dict(table=np.array([[1 << 32]])), dict(table=np.array([[0.0]])), dict(pos0=np.array([1 << 63], np.uint64)), dict(slots=[0, 1]), dict(pos0=[0, 0])):
+        with pytest.raises(TensorError):
+            paged.PagePlan(None, 16, 4, n_slots=1, **{**good, **bad})
