@@ -1,7 +1,7 @@
 // paged_attn.cu -- attention over the pages of a cache (include/crabml_paged.h).
 //
 // 32-bit results from 16-bit tensor-core products.  Codes and 16-bit numbers are exact as f16 operands; a query or weight x is two of them, h = f16(x) and
-// l = f16(x - h), 22 bits together.  A query row is first brought near 2^14 by a power of two, weights go up to 2^15, so that l keeps its bits.
+// l = f16(x - h), 22 bits together.  A query row is first brought near 2^14 by a power of two, weights go up to 2^14, so that l keeps its bits.
 //
 // Few rows (paged_few_kernel; a row is a query of one head).  mma.sync.m16n8k16 has room for 16 rows: eight rows' h above, the same rows' l below, and both
 // products are one instruction whose accumulators a thread adds up itself.  A warp takes 16 keys at a time.  Its lanes keep, read and convert the pieces of the
@@ -17,8 +17,8 @@
 
 #define PT_WARPS 4
 #define PT_THREADS (PT_WARPS * 32)
-#define PT_SHIFT 9.0f                         // weights are exp2(score - base + PT_SHIFT), base the largest score so far, or up to PT_LAG less: weights stay below 2^15, and the sums
-#define PT_LAG 6.0f                           // of a row are not scaled again for every score that is a little larger
+#define PT_SHIFT 9.0f                         // weights are exp2(score - base + PT_SHIFT), base the largest score so far, or up to PT_LAG less, so that the sums of a row are not scaled
+#define PT_LAG 5.0f                           // again for every score that is a little larger.  Weights stay at 2^14, times a value's factor (below 2 of its unit) below 2^15: f16 ends at 65504
 #define PT_STEP 64                            // keys that few rows are dealt out by
 #define PT_BEGIN 5                            // what a segment's begin and end cost, in steps (finding it, the queries, the sums: 13 thousand cycles)
 #define PT_CHUNK 4096                         // keys whose page numbers and factors a CTA holds at a time

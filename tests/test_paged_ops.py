@@ -402,6 +402,34 @@ def test_attention_in_runs(dev, seed, G, Rh, d, n, top, window, i8):
 
 
 @pytest.mark.parametrize("i8", [False, True], ids=["f16", "i8"])
+@pytest.mark.parametrize("window,softcap,sink", [(0, 0.0, True), (1500, 30.0, False), (2999, 3.0, True)])
+def test_attention_in_runs_masks(dev, window, softcap, sink, i8):
+    """a sink's share and capped scores where a row's sums come from several CTAs"""
+    check_attention(dev, 16, 2, 3, 48, 80, i8, [4000, 2500, 100, 3100], [1, 3, 2, 10], window=window, softcap=softcap, sink=sink, seed=window)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("lead", [1.0, 3.0, 4.999, 5.9995, 5.99995, 6.01, 9.0])
+def test_attention_of_a_later_larger_score(dev, lead, n):
+    """a score that outgrows the ones before it by a little, beside the largest value factor that a power of two leaves room for"""
+    P, d, end = 16, 16, 160
+    c = Case(dev, P, 1, d, d, True, [end - n], [n], seed=2)
+    a = c.ref.a
+    a["k"][:] = 0
+    a["k_scale"][:] = 1
+    a["v_scale"][:] = np.float32(1.9999999)
+    a["k"][c.table[0][4], 0, 3, 0] = 1                       # key 67: score of lead * ln 2, the others 0
+    a["k_scale"][c.table[0][4]] = np.float32(lead * np.log(2.0))
+    c.cache = paged.PagedCache(**{m: give(dev, x) for m, x in a.items()})
+    q = np.zeros((n, 1, d), np.float32)
+    q[:, 0, 0] = 1
+    got = take(dev, paged.attention(c.plan(), c.cache, give(dev, q.reshape(n, -1)), 1, 1.0)).reshape(n, 1, d)
+    k, v = (c.ref.rows(m, c.table[0], end, c.slot(0)) for m in ("k", "v"))
+    want, mass, reach = R.attention(q, k, v, end - n, 1.0)
+    assert (np.abs(got - want) <= R.attention_bound(mass, reach, d, end)).all()
+
+
+@pytest.mark.parametrize("i8", [False, True], ids=["f16", "i8"])
 def test_rows_over_thousands_of_keys(dev, i8):
     """eight rows at a time over more keys than a CTA holds page numbers of"""
     d, Rh, pos0, n = 256, 8, 4400, 1190
