@@ -145,6 +145,10 @@ __device__ __forceinline__ __half pa_half(float x) {
     if (__hisinf(h) && !isinf(x)) h = __ushort_as_half((unsigned short)(x > 0.0f ? 0x7bff : 0xfbff));
     return h;
 }
+__device__ __forceinline__ __half2 pa_half2(float2 v) {
+    if (fmaxf(fabsf(v.x), fabsf(v.y)) >= 65520.0f) return __halves2half2(pa_half(v.x), pa_half(v.y));
+    return __floats2half2_rn(v.x, v.y);
+}
 __device__ __forceinline__ double2 pa_angle(const PaArgs& a, int pos, int i) {
     double s, c;
     sincos((double)pos * (double)a.freq[i], &s, &c);
@@ -161,23 +165,52 @@ __global__ void __launch_bounds__(PA_THREADS) paged_angles_kernel(const PaArgs a
         }
     }
 }
-// Units of a head's row: pairs, which are turned, and behind them the columns that stay.  Where unit u lies, and its numbers through `put` (column, number)
+// Units of a head's row: pairs, which are turned, and behind them the columns that stay.  Where unit u lies
 __device__ __forceinline__ int pa_column(const PaArgs& a, int u) {
     if (u < a.pairs) return a.offset + a.step * u;
     const int c = u - a.pairs;
     return c >= a.offset ? c + 2 * a.pairs : c;
 }
-__device__ __forceinline__ float2 pa_read(const PaArgs& a, const float* row, int u, int c) {
-    if (u >= a.pairs) return make_float2(__ldg(row + c), 0.0f);
-    if (a.vec) return __ldg((const float2*)(row + c));
-    return make_float2(__ldg(row + c), __ldg(row + c + a.gap));
+// what a unit reads and writes at its first column: a pair (its second number `gap` further on), or one number
+__device__ __forceinline__ float2 pa_read(const PaArgs& a, const float* p, bool pair) {
+    if (!pair) return make_float2(__ldg(p), 0.0f);
+    if (a.vec) return __ldg((const float2*)p);
+    return make_float2(__ldg(p), __ldg(p + a.gap));
 }
-template <class Put>
-__device__ __forceinline__ void pa_write(const PaArgs& a, float2 v, int u, int c, const double2& t, Put put) {
-    if (u >= a.pairs) { put(c, v.x); return; }
+__device__ __forceinline__ float2 pa_turn(float2 v, const double2& t) {
     const double x = (double)v.x, y = (double)v.y;
-    put(c, (float)fma(x, t.x, -(y * t.y)));
-    put(c + a.gap, (float)fma(x, t.y, y * t.x));
+    return make_float2((float)fma(x, t.x, -(y * t.y)), (float)fma(x, t.y, y * t.x));
+}
+__device__ __forceinline__ void pa_write(const PaArgs& a, float* p, float2 v, bool pair) {
+    if (pair && a.step == 2 && ((uintptr_t)p & 7) == 0) { *(float2*)p = v; return; }
+    p[0] = v.x;
+    if (pair) p[a.gap] = v.y;
+}
+__device__ __forceinline__ void pa_write(const PaArgs& a, __half* p, float2 v, bool pair) {
+    if (!pair) { p[0] = pa_half(v.x); return; }
+    const __half2 h = pa_half2(v);
+    if (a.step == 2 && ((uintptr_t)p & 3) == 0) { *(__half2*)p = h; return; }
+    p[0] = __low2half(h); p[a.gap] = __high2half(h);
+}
+// round(127 x / most) of four of a block's numbers, ties to even, as the exact quotient rounds.  x and most have 11 bits, so 127 x is exact and a quotient that is not a tie is further from one than
+// a 32-bit division errs; 127 / most and the product err by less than 2e-5, and where that leaves it open the quotient is taken
+__device__ __forceinline__ unsigned pa_code4(uint2 u, float most, float r) {
+    constexpr float M = 12582912.0f;
+    const float2 lo = __half22float2(*(const __half2*)&u.x), hi = __half22float2(*(const __half2*)&u.y);
+    const float x[4] = {lo.x, lo.y, hi.x, hi.y};
+    float n[4], far = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float y = x[i] * r;
+        n[i] = y + M;
+        far = fmaxf(far, fabsf(y - (n[i] - M)));
+    }
+    if (far < 0.49998f)
+        return __byte_perm(__byte_perm(__float_as_uint(n[0]), __float_as_uint(n[1]), 0x0040), __byte_perm(__float_as_uint(n[2]), __float_as_uint(n[3]), 0x0040), 0x5410);
+    unsigned c = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) c |= ((unsigned)(int)rintf(x[i] * 127.0f / most) & 255u) << (8 * i);
+    return c;
 }
 #define PA_Q_ROWS 16
 #define PA_AHEAD 4                           // rows of a head, or heads of a row, that a warp reads before it turns the first
@@ -200,7 +233,8 @@ __global__ void __launch_bounds__(PA_THREADS, 4) paged_append_kernel(const PaArg
         // f(row r0, so many rows, their angles): all rows of the job, or portions whose angles the CTA makes first
         auto portions = [&](bool turned, auto f) {
             if (TABLE || !turned || a.pairs == 0) { f(row_from, row_to - row_from, a.angles + (int64_t)(g.token0 + row_from) * a.pairs); return; }
-            for (int r0 = 0; r0 < g.rows && !TABLE; r0 += PA_ROWS) {
+            if constexpr (!TABLE)
+            for (int r0 = 0; r0 < g.rows; r0 += PA_ROWS) {
                 const int rows = min(PA_ROWS, g.rows - r0);
                 __syncthreads();
                 for (int e = tid; e < rows * a.pairs; e += PA_THREADS) { const int r = e / a.pairs; made[e] = pa_angle(a, g.pos0 + r0 + r, e - r * a.pairs); }
@@ -220,19 +254,21 @@ __global__ void __launch_bounds__(PA_THREADS, 4) paged_append_kernel(const PaArg
                 share(runs * batches, [&](int kind, int first, int by) {
                     const int b = kind / runs, u = (kind - b * runs) * 32 + lane, n = min(PA_AHEAD, nh - b * PA_AHEAD), c = pa_column(a, u);
                     if (u >= units) return;
-                    for (int r = first; r < rows; r += by) {
-                        const int64_t t = g.token0 + r0 + r;
-                        const float* src = a.q + t * a.qrs + (int64_t)(h0 + b * PA_AHEAD) * a.dk;
-                        float* dst = a.qo + (t * a.H + h0 + b * PA_AHEAD) * a.dk;
+                    const bool pair = u < a.pairs;
+                    const int64_t t = g.token0 + r0 + first, at_head = (int64_t)(h0 + b * PA_AHEAD) * a.dk + c, out_step = (int64_t)by * a.H * a.dk;
+                    const float* src = a.q + t * a.qrs + at_head;
+                    float* dst = a.qo + t * a.H * a.dk + at_head;
+                    const double2* angle = cs + first * a.pairs + u;
+                    for (int r = first; r < rows; r += by, src += by * a.qrs, dst += out_step, angle += by * a.pairs) {
                         float2 v[PA_AHEAD];
                         double2 z = make_double2(0.0, 0.0);
 #pragma unroll
                         for (int i = 0; i < PA_AHEAD; i++)
-                            if (i < n) v[i] = pa_read(a, src + i * a.dk, u, c);
-                        if (u < a.pairs) z = cs[r * a.pairs + u];
+                            if (i < n) v[i] = pa_read(a, src + i * a.dk, pair);
+                        if (pair) z = *angle;
 #pragma unroll
                         for (int i = 0; i < PA_AHEAD; i++)
-                            if (i < n) pa_write(a, v[i], u, c, z, [&](int col, float x) { dst[i * a.dk + col] = x; });
+                            if (i < n) pa_write(a, dst + i * a.dk, pair ? pa_turn(v[i], z) : v[i], pair);
                     }
                 });
             });
@@ -252,27 +288,22 @@ __global__ void __launch_bounds__(PA_THREADS, 4) paged_append_kernel(const PaArg
                 constexpr int AHEAD = TABLE ? PA_AHEAD : 1;
                 const int u = kind * 32 + lane, c = is_k ? pa_column(a, u) : u;
                 if (u >= units) return;
-                for (int r = first; r < rows; r += by * AHEAD) {
+                const bool pair = is_k && u < a.pairs;
+                const float* from = src + (g.token0 + r0 + first) * rs + c;
+                __half* dst = to + (r0 + first) * d + c;
+                const double2* angle = cs + first * a.pairs + u;
+                for (int r = first; r < rows; r += by * AHEAD, from += by * AHEAD * rs, dst += by * AHEAD * d, angle += by * AHEAD * a.pairs) {
                     float2 v[AHEAD];
                     double2 z[AHEAD];
 #pragma unroll
                     for (int i = 0; i < AHEAD; i++) {
-                        const int x = r + i * by;
-                        if (x >= rows) continue;
-                        const float* row = src + (g.token0 + r0 + x) * rs;
-                        if (is_k) {
-                            v[i] = pa_read(a, row, u, c);
-                            if (u < a.pairs) z[i] = cs[x * a.pairs + u];
-                        } else v[i].x = __ldg(row + c);
+                        if (r + i * by >= rows) continue;
+                        v[i] = pa_read(a, from + i * by * rs, pair);
+                        if (pair) z[i] = angle[i * by * a.pairs];
                     }
 #pragma unroll
-                    for (int i = 0; i < AHEAD; i++) {
-                        const int x = r + i * by;
-                        if (x >= rows) continue;
-                        __half* dst = to + (r0 + x) * d;
-                        if (is_k) pa_write(a, v[i], u, c, z[i], [&](int col, float y) { dst[col] = pa_half(y); });
-                        else dst[c] = pa_half(v[i].x);
-                    }
+                    for (int i = 0; i < AHEAD; i++)
+                        if (r + i * by < rows) pa_write(a, dst + i * by * d, pair ? pa_turn(v[i], z[i]) : v[i], pair);
                 }
             });
         });
@@ -291,19 +322,12 @@ __global__ void __launch_bounds__(PA_THREADS, 4) paged_append_kernel(const PaArg
             for (int i = 0; i < PA_WARPS; i++) top = max(top, tops[i]);
             const bool finite = top < 0x7c00u;
             const float most = __half2float(__ushort_as_half((unsigned short)top));
-            // numbers and their largest have 11 bits: 127 x is exact, and a quotient that is not a tie is further from one than a 32-bit division errs
             uint2* codes = (uint2*)((is_k ? a.kp : a.vp) + page_at);
+            const bool some = finite && top;
+            const float r = 127.0f / most;
             for (int e = tid; e < a.page * d / 8; e += PA_THREADS) {
                 const uint4 x = ((const uint4*)block)[e];
-                const unsigned in[4] = {x.x, x.y, x.z, x.w};
-                unsigned c[8];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float2 y = __half22float2(*(const __half2*)&in[i]);
-                    c[2 * i] = finite && top ? (unsigned)(int)rintf(y.x * 127.0f / most) & 255u : 0u;
-                    c[2 * i + 1] = finite && top ? (unsigned)(int)rintf(y.y * 127.0f / most) & 255u : 0u;
-                }
-                codes[e] = make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
+                codes[e] = some ? make_uint2(pa_code4(make_uint2(x.x, x.y), most, r), pa_code4(make_uint2(x.z, x.w), most, r)) : make_uint2(0u, 0u);
             }
             if (tid == 0) (is_k ? a.ks : a.vs)[(size_t)g.page * a.G + head] = finite ? most / 127.0f : NAN;
         }
@@ -353,7 +377,7 @@ extern "C" CC_API int cc_paged_append(cc_device* dev, const cc_page_plan* plan, 
         a.vec = pairing == CC_ROPE_NEIGHBOURS && ((offset | c.dk | k_col0 | (int)(a.krs & 1)) & 1) == 0 && (!q_src || ((q_col0 | (int)(a.qrs & 1)) & 1) == 0) &&
                 (((uintptr_t)k_src->buf->plane[0] | (q_src ? (uintptr_t)q_src->buf->plane[0] : 0)) & 7) == 0;
         // a portion of many rows a block: the angles once for all heads, in a kernel of their own (64 rows of 64 pairs made by each of 16 CTAs:
-        // three prompts of 1657 tokens, 32 heads on 8, 125 us, with the table 4 + 33); single tokens: by every CTA
+        // three prompts of 1657 tokens, 32 heads on 8, 125 us, with the table 4 + 32); single tokens: by every CTA
         const bool table = pairs > 0 && T > 4 * (int64_t)plan->n_segments;
         a.hq = table ? 4 : 8; a.q_parts = table ? plan->page / PA_Q_ROWS : 1;
         void* ws = nullptr; size_t cls = 0;
