@@ -233,8 +233,7 @@ __global__ void __launch_bounds__(PA_THREADS, 4) paged_append_kernel(const PaArg
         // f(row r0, so many rows, their angles): all rows of the job, or portions whose angles the CTA makes first
         auto portions = [&](bool turned, auto f) {
             if (TABLE || !turned || a.pairs == 0) { f(row_from, row_to - row_from, a.angles + (int64_t)(g.token0 + row_from) * a.pairs); return; }
-            if constexpr (!TABLE)
-            for (int r0 = 0; r0 < g.rows; r0 += PA_ROWS) {
+            for (int r0 = TABLE ? g.rows : 0; r0 < g.rows; r0 += PA_ROWS) {
                 const int rows = min(PA_ROWS, g.rows - r0);
                 __syncthreads();
                 for (int e = tid; e < rows * a.pairs; e += PA_THREADS) { const int r = e / a.pairs; made[e] = pa_angle(a, g.pos0 + r0 + r, e - r * a.pairs); }
