@@ -576,19 +576,48 @@ __global__ void __launch_bounds__(32 * PT_JOIN) paged_join_kernel(const PtArgs a
     const int tok = row / a.R, head = kvh * a.R + row - tok * a.R;
     pt_join(a, cut.n, [&](int x) { return (size_t)(x == 0 ? cut.slot : 2 * (cut.cta + x - 1)) * 8 + y; }, a.out + ((int64_t)(s.first + tok) * a.H + head) * a.dv, head);
 }
-// tiles of 128 rows: the slices of a row, grid (rows, key heads)
-__global__ void __launch_bounds__(32 * PT_JOIN) paged_sum_kernel(const PtArgs a) {
-    const int lane = threadIdx.x & 31, kvh = a.head0 + blockIdx.y;
+// tiles of 128 rows: the slices of a row, grid (PT_SUM rows of a sequence, key heads); a warp a row, four times, a lane 4 neighbouring columns.  (A CTA a row, which finds its place by itself: 6600
+// rows of 8 key heads took 107 us longer in two slices than in one, 42 so)
+#define PT_SUM 32
+__global__ void __launch_bounds__(256) paged_sum_kernel(const PtArgs a) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, kvh = a.head0 + blockIdx.y, col = lane * 4;
     pdl_enter();
-    int row, items = 0;
-    const int seq = pt_find(a, blockIdx.x, [&](const PgSeq& s) { return pt_splits(s, a) > 1 ? s.count * a.R : 0; }, &row);
+    int group, items = 0;
+    const int seq = pt_find(a, blockIdx.x, [&](const PgSeq& s) { return pt_splits(s, a) > 1 ? (s.count * a.R + PT_SUM - 1) / PT_SUM : 0; }, &group);
     if (seq < 0) return;
     for (int x = lane; x < seq; x += 32) items += pt_splits(a.seqs[x], a) * ((a.seqs[x].count * a.R + a.tile_rows - 1) / a.tile_rows);
     items = warp_sum_i(items);
     const PgSeq s = a.seqs[seq];
-    const int tiles = (s.count * a.R + a.tile_rows - 1) / a.tile_rows, n = pt_splits(s, a), tile = row / a.tile_rows, y = row - tile * a.tile_rows;
-    const int tok = row / a.R, head = kvh * a.R + row - tok * a.R, first = items + (tiles - 1 - tile) * n;      // items of a sequence: tile by tile from the last one on
-    pt_join(a, n, [&](int x) { return ((size_t)(first + x) * a.heads + blockIdx.y) * a.tile_rows + y; }, a.out + ((int64_t)(s.first + tok) * a.H + head) * a.dv, head);
+    const int tiles = (s.count * a.R + a.tile_rows - 1) / a.tile_rows, n = pt_splits(s, a), end = min(s.count * a.R, (group + 1) * PT_SUM);
+    for (int row = group * PT_SUM + w; row < end; row += 8) {
+        const int tile = row / a.tile_rows, y = row - tile * a.tile_rows, tok = row / a.R, head = kvh * a.R + row - tok * a.R, first = items + (tiles - 1 - tile) * n;      // tile by tile from the last one on
+        auto place = [&](int x) { return ((size_t)(first + x) * a.heads + blockIdx.y) * a.tile_rows + y; };
+        float m = -INFINITY, l = 0.0f;
+        for (int x = lane; x < n; x += 32) m = fmaxf(m, a.ml[place(x)].x);
+        m = warp_max(m);
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int x0 = 0; x0 < n; x0 += 32) {
+            const float2 z = x0 + lane < n ? a.ml[place(x0 + lane)] : make_float2(-INFINITY, 0.0f);
+            const float f = z.x == -INFINITY ? (z.y == 0.0f ? 0.0f : 1.0f) : exp2f(z.x - m);
+            l = fmaf(f, z.y, l);
+#pragma unroll 4
+            for (int x = x0; x < min(n, x0 + 32); x++) {
+                const float by = __shfl_sync(0xffffffffu, f, x - x0);
+                if (col < a.dv) {
+                    const float4 v = *(const float4*)(a.part + place(x) * a.dv + col);
+                    o.x = fmaf(by, v.x, o.x); o.y = fmaf(by, v.y, o.y); o.z = fmaf(by, v.z, o.z); o.w = fmaf(by, v.w, o.w);
+                }
+            }
+        }
+        l = warp_sum(l);
+        float f = 1.0f;
+        if (a.sink) {
+            const float sk = a.sink[head] * PT_LOG2E, m2 = fmaxf(m, sk);
+            f = m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : exp2f(m - m2);
+            l = f * l + (sk == -INFINITY ? 0.0f : exp2f(sk - m2 + PT_SHIFT));
+        }
+        if (col < a.dv) *(float4*)(a.out + ((int64_t)(s.first + tok) * a.H + head) * a.dv + col) = make_float4(o.x * f / l, o.y * f / l, o.z * f / l, o.w * f / l);
+    }
 }
 
 template <int D, bool I8>
@@ -665,9 +694,27 @@ static int pt_run_few(cc_device* dev, const cc_page_plan* plan, PtArgs a, bool i
 
 #define TI_WORKSPACE ((int64_t)256 << 20)     // bytes of images that a call has at a time, as long as one head's are no more
 
-// sequences of many rows: slices of TI_MOST keys at most, as many as leave no SM without one
+// How long a call takes with slices of a.split keys, in cycles.  An item's start and end 18000, a step of 128 keys 3900; CTAs take items in turn, so that the SMs end half of the longest one apart;
+// sums of slices are written and read at 3 TB/s (1600 bytes a cycle), 10000 cycles for the kernel that adds them up
+static double pt_guess(const cc_page_plan* plan, const PtArgs& a, int sms) {
+    double all = 0.0, longest = 0.0, sums = 0.0, items = 0.0;
+    for (const PgSeq& s : plan->seqs) {
+        const int n = pt_splits(s, a);
+        if (!n) continue;
+        int from, to;
+        pt_range(s, a, &from, &to);
+        const double rows = (double)s.count * a.R, heads = std::ceil(rows / TI_ROWS) * a.G;
+        all += heads * (18000.0 * n + 3900.0 / TI_KEYS * (std::max(to - from - 0.5 * s.count, 0.5 * TI_KEYS)));
+        items += heads * n;
+        longest = std::max(longest, 18000.0 + 3900.0 / TI_KEYS * std::min(pt_each(to - from, n), to - from));
+        if (n > 1) sums += rows * a.G * (2 * n + 1) * a.dv * 4 / 1600.0;
+    }
+    return (items <= sms ? longest : std::max(longest, all / sms + 0.5 * longest)) + (sums > 0.0 ? sums + 10000.0 : 0.0);
+}
+// sequences of many rows: of some lengths of slices the one that should take least time.  (As many as give every SM one, against this, 32 heads on 8: 4 sequences of 3000 to 6000 tokens
+// with 16 to 128 new ones 120 us and 92, 8 of 3000 with 64 106 and 93, 16 of 500 to 3000 with 16 to 64 146 and 132; 256 tokens over 8000 149 and 148, where slices of 2560 take 130)
 static int pt_run_tiles(cc_device* dev, const cc_page_plan* plan, PtArgs a, bool i8) {
-    int64_t keys = 0, items = 0, split_rows = 0, key_tiles = 0;
+    int64_t keys = 0, items = 0, split_rows = 0, key_tiles = 0;             // split_rows: groups of PT_SUM rows of sequences in several slices
     for (const PgSeq& s : plan->seqs) {
         const int64_t rows = (int64_t)s.count * a.R;
         if (rows < a.rows_lo || rows > a.rows_hi) continue;
@@ -677,12 +724,18 @@ static int pt_run_tiles(cc_device* dev, const cc_page_plan* plan, PtArgs a, bool
         key_tiles += ti_key_tiles(s, a);
     }
     if (!keys) return CC_OK;
-    const int64_t each = (keys + dev->sm_count - 1) / dev->sm_count;
-    a.split = (int)std::min<int64_t>(TI_MOST, std::max<int64_t>(512, (each + 127) / 128 * 128));
+    int best = 0;
+    double least = 0.0;
+    for (int split : {TI_MOST, 2560, 2048, 1536, 1024, 768, 512}) {
+        a.split = split;
+        const double t = pt_guess(plan, a, dev->sm_count);
+        if (!best || t < 0.97 * least) { best = split; least = t; }
+    }
+    a.split = best;
     for (const PgSeq& s : plan->seqs) {
         const int n = pt_splits(s, a);
         items += (int64_t)n * (((int64_t)s.count * a.R + a.tile_rows - 1) / a.tile_rows);
-        if (n > 1) split_rows += (int64_t)s.count * a.R;
+        if (n > 1) split_rows += ((int64_t)s.count * a.R + PT_SUM - 1) / PT_SUM;
     }
     CC_REQUIRE(dev, items * a.G < ((int64_t)1 << 31) && split_rows < ((int64_t)1 << 31) && key_tiles < ((int64_t)1 << 31), "paged_attention: too many rows");
     const size_t kb = (size_t)((a.dk + 63) / 64) * TI_BLOCK, vb = (size_t)((a.dv + 63) / 64) * TI_BLOCK, per_head = (size_t)key_tiles * (kb + vb + sizeof(TiInfo));
@@ -705,7 +758,7 @@ static int pt_run_tiles(cc_device* dev, const cc_page_plan* plan, PtArgs a, bool
         if (e == cudaSuccess) e = cc_launch_pdl(dev, kernel, (unsigned)(items * a.heads), TI_THREADS, TI_SMEM, a, dev->err_dev, dev->err_host);
         dev->launches += 2;
         if (e == cudaSuccess && split_rows) {
-            e = cc_launch_pdl(dev, paged_sum_kernel, dim3((unsigned)split_rows, (unsigned)a.heads), 32 * PT_JOIN, 0, a);
+            e = cc_launch_pdl(dev, paged_sum_kernel, dim3((unsigned)split_rows, (unsigned)a.heads), 256, 0, a);
             dev->launches++;
         }
     }
