@@ -466,6 +466,13 @@ def test_many_rows_over_many_keys(dev, i8):
 
 
 @pytest.mark.parametrize("i8", [False, True], ids=["f16", "i8"])
+@pytest.mark.parametrize("sink", [False, True])
+def test_many_slices(dev, sink, i8):
+    """a few dozen rows over so many keys that each has more slices than a warp has lanes"""
+    check_attention(dev, 128, 1, 1, 16, 32, i8, [140000, 90], [40, 40], sink=sink, seed=17)
+
+
+@pytest.mark.parametrize("i8", [False, True], ids=["f16", "i8"])
 @pytest.mark.parametrize("scale", [-0.3, 0.0, 1e-20])
 def test_attention_scales(dev, scale, i8):
     """the smallest scores are the largest, and every key weighs the same"""
