@@ -77,7 +77,7 @@ class CudaTensorDevice:
         if rc != capi.CC_OK:
             raise CudaError(self.lib.cc_last_error(None).decode())
         self.handle = h
-        self.debug_named_tensors = debug_named_tensors
+        self.debug_named_tensors, self._lazy = debug_named_tensors, bool(lazy)
 
     def check(self, rc):
         if rc == capi.CC_OK:
@@ -182,7 +182,7 @@ def _shape_arr(shape):
 class CudaTensor:
     def __init__(self, buf: _Buf, strider: TensorStrider, device: CudaTensorDevice, name=None):
         self.buf, self._strider, self.device, self.name = buf, strider, device, name
-        self._cview = self._cview_of = None
+        self._cview = self._cview_of = self._array = self._array_of = None
 
     # -- plumbing ------------------------------------------------------------------------------
     def _view(self):
@@ -201,13 +201,20 @@ class CudaTensor:
     @property
     def __cuda_array_interface__(self):
         """the tensor's own memory for other libraries (torch.as_tensor and the like), ordered by the device's stream"""
+        if not self.device.handle:
+            raise CudaError("the tensor's device is closed")
+        if self._array_of is self._strider:                            # asked for twice by those who look whether it is there
+            return dict(self._array)
         kind, size = capi.ARRAY_TYPES.get(self.dtype(), (None, 0))
         if kind is None:
             raise AttributeError(f"a tensor of type {self.dtype()} is not a plain array")
         self.device.flush()
         shape = tuple(self._strider.shape)
-        return {"shape": shape, "typestr": kind, "data": (0 if 0 in shape else self.device.lib.cc_tensor_data(self.buf.handle), False),
-                "strides": None if self._strider.is_contiguous() else tuple(s * size for s in self._strider.strides), "stream": self.device.stream(), "version": 3}
+        array = {"shape": shape, "typestr": kind, "data": (0 if 0 in shape else self.device.lib.cc_tensor_data(self.buf.handle), False),
+                 "strides": None if self._strider.is_contiguous() else tuple(s * size for s in self._strider.strides), "stream": self.device.stream(), "version": 3}
+        if not self.device._lazy:                                      # (eager: a buffer stays where it is, with all work on it queued)
+            self._array, self._array_of = array, self._strider
+        return dict(array)
 
     def _new(self, handle, shape):
         return CudaTensor(_Buf(self.device, handle), TensorStrider(shape), self.device)

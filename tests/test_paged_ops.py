@@ -598,6 +598,19 @@ def test_arrays_of_a_tensor(dev):
     torch.as_tensor(t, device="cuda").add_(1.0)
     torch.cuda.synchronize()
     np.testing.assert_array_equal(t.export().reshape(4, 6), a + 1)
+    first = t.__cuda_array_interface__
+    first["data"] = None                                     # what a caller does to it is the caller's
+    assert t.__cuda_array_interface__["data"][0] == torch.as_tensor(t, device="cuda").data_ptr()
+    u = CudaTensor.new(a, [4, 6], dev)
+    assert u.__cuda_array_interface__["shape"] == (4, 6)
+    v = u.reshape([6, 4])
+    assert v.__cuda_array_interface__["shape"] == (6, 4) and v.__cuda_array_interface__["data"] == u.__cuda_array_interface__["data"]
+    gone = make_device()
+    w = CudaTensor.new(a, [4, 6], gone)
+    assert w.__cuda_array_interface__["data"][0]
+    gone.close()
+    with pytest.raises(CudaError):
+        w.__cuda_array_interface__
     q = CudaTensor.from_cpu(np.zeros(34 * 2, np.uint8), [2, 32], capi.Q8_0, dev)
     assert not hasattr(q, "__cuda_array_interface__")
     assert CudaTensor.alloc([0, 3], capi.I8, dev).__cuda_array_interface__["data"][0] == 0
