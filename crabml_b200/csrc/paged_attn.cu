@@ -169,7 +169,8 @@ __device__ __forceinline__ void pt_weights(PtRows<D>& r, float (&x)[4], int key0
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     // the largest value factor so far, as the power of two below it: a block that the row does not see leaves its bits as they are
     const float vp = fminf(fmaxf(__uint_as_float(__float_as_uint(vf) & 0x7f800000u), 0x1p-100f), 0x1p100f);
-    const bool up = mx > r.m + PT_LAG, wider = vp > r.vref && vf > 0.0f;      // (r.m -inf: every score is more)
+    // differences of scores before anything is added to them: from 2^27 on a score's last place is more than PT_LAG or PT_SHIFT, which the sum would round to more than f16 has room for
+    const bool up = mx - r.m > PT_LAG, wider = vp > r.vref && vf > 0.0f;      // (r.m -inf: every score is more)
     if (__any_sync(0xffffffffu, up || wider)) {
         float alpha = 1.0f;
         if (up) {
@@ -184,9 +185,9 @@ __device__ __forceinline__ void pt_weights(PtRows<D>& r, float (&x)[4], int key0
 #pragma unroll
         for (int i = 0; i < D / 8; i++) { r.o[i][0] *= alpha; r.o[i][1] *= alpha; r.o[i][2] *= alpha; r.o[i][3] *= alpha; }
     }
-    const float base = r.m == -INFINITY ? 0.0f : PT_SHIFT - r.m, vr = vf * r.ivref;
+    const float base = r.m == -INFINITY ? 0.0f : r.m, vr = vf * r.ivref;
 #pragma unroll
-    for (int i = 0; i < 4; i++) x[i] = pt_exp2(x[i] + base);
+    for (int i = 0; i < 4; i++) x[i] = pt_exp2((x[i] - base) + PT_SHIFT);
     r.l += (x[0] + x[1]) + (x[2] + x[3]);
 #pragma unroll
     for (int i = 0; i < 4; i++) x[i] = seen & (1u << i) ? x[i] * vr : 0.0f;

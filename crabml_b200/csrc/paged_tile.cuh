@@ -53,7 +53,8 @@ struct TiShared {
 };
 #define TI_OPERAND (TI_KEYS * TI_D * 2)       // bytes of a tile of f16: two blocks of 64 columns, rows of 128 bytes under the 128-byte swizzle
 #define TI_SMEM (6 * TI_OPERAND + 1024)
-#define TI_SFU 10                             // of 16 weights those that the special function unit makes
+#define TI_TOP 512.0f                         // the largest weight, 2^PT_SHIFT
+#define TI_SFU 14                             // of 16 weights those that the special function unit makes: 214 us for the portions of three prompts; 10 of them 222, 12 216, all 217
 #define TI_O 256                              // TMEM columns: S and P at 0 and 128
 #define TI_Q 384
 #define TI_BLOCK (TI_OPERAND / 2)             // 64 columns of an operand; an image is as many as d has
@@ -401,12 +402,9 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
         for (int k = 0; k < steps; k++) {
             const unsigned slot = k & 1;
             const int key0 = lo + k * TI_KEYS + part * TI_XC;
-            float f[TI_XC / 16];                                               // factor of 16 keys' sums; 0 (a block of zeros) must not meet the -inf of a hidden key
+            float f[TI_XC / 16];                                               // factor of 16 keys' sums
 #pragma unroll
-            for (int g = 0; g < TI_XC / 16; g++) {
-                f[g] = f0 * sh.info[k].kf[part * (TI_XC / 16) + g];
-                f[g] = f[g] == 0.0f ? 1e-37f : f[g];
-            }
+            for (int g = 0; g < TI_XC / 16; g++) f[g] = f0 * sh.info[k].kf[part * (TI_XC / 16) + g];
             ok = ok && ti_wait_warp(pg_smem(&sh.s_full[slot]), (k >> 1) & 1u, &sh.fail);
             unsigned x[TI_XC];
             if (ok) {
@@ -417,11 +415,17 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
 #pragma unroll
                 for (int c = 0; c < TI_XC; c++) asm volatile("" : "+r"(x[c]));
             }
-            if (CAP) {
+            // scores, each rounded once, so that the largest is one of them and their differences from it end at 0.  (x f + base in one multiply-add, of a largest score and a base that
+            // are rounded, makes weights beyond what f16 holds once their last places pass 8, from 2^27 on)
 #pragma unroll
-                for (int c = 0; c < TI_XC; c++) x[c] = __float_as_uint(a.softcap * tanhf(__uint_as_float(x[c]) * f[c / 16] / a.softcap) * PT_LOG2E);
-#pragma unroll
-                for (int g = 0; g < TI_XC / 16; g++) f[g] = 1.0f;
+            for (int c = 0; c < TI_XC; c += 2) {
+                if (CAP) {
+                    x[c] = __float_as_uint(a.softcap * tanhf(__uint_as_float(x[c]) * f[c / 16] / a.softcap) * PT_LOG2E);
+                    x[c + 1] = __float_as_uint(a.softcap * tanhf(__uint_as_float(x[c + 1]) * f[c / 16] / a.softcap) * PT_LOG2E);
+                } else {
+                    const float2 y = ti_one(ti_mul2(ti_two(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), ti_two(f[c / 16], f[c / 16])));
+                    x[c] = __float_as_uint(y.x); x[c + 1] = __float_as_uint(y.y);
+                }
             }
             if (lo + k * TI_KEYS + TI_KEYS - 1 > min(pos_first, k1 - 1) || (a.window > 0 && lo + k * TI_KEYS < pos_last - a.window + 1)) {
                 const int c_lo = key_lo - key0, c_hi = key_hi - key0;
@@ -431,32 +435,27 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
             }
             float mx = -INFINITY;
 #pragma unroll
-            for (int g = 0; g < TI_XC / 16; g++) {
-                float y = fmaxf(__uint_as_float(x[g * 16]), __uint_as_float(x[g * 16 + 1]));
-#pragma unroll
-                for (int c = 2; c < 16; c += 2) y = ti_max3(y, __uint_as_float(x[g * 16 + c]), __uint_as_float(x[g * 16 + c + 1]));
-                mx = fmaxf(mx, y * f[g]);
-            }
+            for (int c = 0; c < TI_XC; c += 2) mx = ti_max3(mx, __uint_as_float(x[c]), __uint_as_float(x[c + 1]));
             sh.top[slot][part][row] = mx;
             ti_soft_sync();                                           // .. and all parts have read S
 #pragma unroll
             for (int i = 0; i < TI_SPLIT; i++) mx = fmaxf(mx, sh.top[slot][i][row]);
             const float* vfs = sh.info[k].vf;
-            const float m_new = fmaxf(m, mx), base = m_new == -INFINITY ? 0.0f : PT_SHIFT - m_new;
+            const float m_new = fmaxf(m, mx), base = m_new == -INFINITY ? 0.0f : -m_new;
             const float alpha = m == m_new ? 1.0f : pt_exp2(m - m_new);
             m = m_new;
             ti_f2 sum = 0ull;
             const ti_f2 base2 = ti_two(base, base), minus = ti_two(-1.0f, -1.0f);
             auto weights = [&](int g) {                               // of 16 keys: 8 words of h, 8 of l
                 unsigned h[8], w[8];
-                const float vr = I8 ? vfs[part * (TI_XC / 16) + g] : 1.0f;
-                const ti_f2 f2 = ti_two(f[g], f[g]), vr2 = ti_two(vr, vr);
+                const float vr = I8 ? TI_TOP * vfs[part * (TI_XC / 16) + g] : TI_TOP;
+                const ti_f2 vr2 = ti_two(vr, vr);
 #pragma unroll
                 for (int c = 0; c < 16; c += 2) {
-                    const float2 y = ti_one(ti_fma2(ti_two(__uint_as_float(x[g * 16 + c]), __uint_as_float(x[g * 16 + c + 1])), f2, base2));
+                    const float2 y = ti_one(ti_add2(ti_two(__uint_as_float(x[g * 16 + c]), __uint_as_float(x[g * 16 + c + 1])), base2));
                     ti_f2 p = c % 16 >= TI_SFU ? ti_exp2_pair(y) : ti_two(pt_exp2(y.x), pt_exp2(y.y));
                     sum = ti_add2(sum, p);
-                    if (I8) p = ti_mul2(p, vr2);
+                    p = ti_mul2(p, vr2);
                     const float2 q = ti_one(p);
                     const __half2 a2 = __floats2half2_rn(q.x, q.y);
                     const float2 b2 = __half22float2(a2), rest2 = ti_one(ti_fma2(ti_two(b2.x, b2.y), minus, p));
@@ -479,7 +478,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
                 sg_arrive(pg_smem(&sh.p_full[slot]));
             }
             const float2 sums = ti_one(sum);
-            l = fmaf(l, alpha, sums.x + sums.y);
+            l = fmaf(l, alpha, (sums.x + sums.y) * TI_TOP);
             alpha_prev = alpha; vref_prev = I8 ? sh.info[k].vref : 1.0f;
         }
         if (steps > 0) add(steps - 1);
