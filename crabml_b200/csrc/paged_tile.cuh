@@ -284,7 +284,9 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const int r = r0 + i;
-                const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)))));
+                // as bits, so that NaN is the largest of all
+                const unsigned top = __reduce_max_sync(0xffffffffu, max(max(__float_as_uint(v[i].x) & 0x7fffffffu, __float_as_uint(v[i].y) & 0x7fffffffu),
+                                                                        max(__float_as_uint(v[i].z) & 0x7fffffffu, __float_as_uint(v[i].w) & 0x7fffffffu)));
                 // 2^(14 - e) for a largest number in [2^(e - 1), 2^e); zeros, subnormal and wild ones as they are
                 int ex = (int)(top >> 23) - 126;
                 if (top < 0x00800000u || top >= 0x7f800000u) ex = 14;
@@ -294,7 +296,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
                 pt_cut(v[i].x * f, v[i].y * f, h.x, l.x); pt_cut(v[i].z * f, v[i].w * f, h.y, l.y);
                 uint8_t* at = qs + r * 512 + (((lane >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8;
                 *(uint2*)at = h; *(uint2*)(at + 256) = l;
-                if (lane == 0) sh.inv[r] = __uint_as_float((unsigned)(ex - 14 + 127) << 23);
+                if (lane == 0) sh.inv[r] = top >= 0x7f800000u ? NAN : __uint_as_float((unsigned)(ex - 14 + 127) << 23);
             }
         }
         ti_soft_sync();
@@ -482,6 +484,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
             alpha_prev = alpha; vref_prev = I8 ? sh.info[k].vref : 1.0f;
         }
         if (steps > 0) add(steps - 1);
+        if (isnan(f0)) l = NAN;                                       // a query that is not finite: maxima and the pairs' exponentials drop NaN
         // values and factors that are not finite were left out: NaN for the rows that see them
         unsigned long long lost = 0;
 #pragma unroll 1

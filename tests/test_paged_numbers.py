@@ -1,4 +1,4 @@
-"""Attention over pages at the ends of its numbers: scores whose last place is more than one."""
+"""Attention over pages at the ends of its numbers: scores whose last place is more than one, queries that are not finite."""
 import numpy as np
 import pytest
 
@@ -54,3 +54,31 @@ def test_scores_of_large_numbers(dev, size, sign, n, i8):  # noqa: F811
         want, mass = v[best].mean(0), np.abs(v[best]).mean(0)
         tol = R.attention_bound(mass[None, None], np.zeros((1, 1)), d, pos0 + t + 1)[0, 0]
         assert (np.abs(got[t, 0] - want) <= tol).all(), (t, got[t, 0][:4], want[:4])
+
+
+# ---- queries that are not finite ---------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("i8", [False, True], ids=["f16", "i8"])
+@pytest.mark.parametrize("n", [5, 40, 150])
+@pytest.mark.parametrize("window,kw", [(1, {}), (2, {}), (6, {}), (0, {}), (3, dict(softcap=5.0)), (4, dict(sink=True)), (0, dict(softcap=5.0, sink=True))])
+def test_queries_that_are_not_finite(dev, window, kw, n, i8):  # noqa: F811
+    """their results are NaN, all of them; the other queries' stay as they are"""
+    P, d, Rh, pos0 = 16, 48, 1, 23
+    c = Case(dev, P, 1, d, d, i8, [pos0], [n], seed=5)
+    if i8:
+        c.ref.a["k_scale"] /= np.float32(60)
+        c.ref.a["v_scale"] /= np.float32(60)
+        refill(c)
+    q = c.rng.normal(size=(n, Rh, d)).astype(np.float32)
+    kw = dict(kw, window=window)
+    if kw.pop("sink", False):
+        kw["sink"] = give(dev, np.zeros(Rh, np.float32))
+    clean = attend(c, q, 0.2, **kw)
+    assert np.isfinite(clean).all()
+    for what in (np.nan, np.inf, -np.inf):
+        for first in (0, 1):
+            x, hit = q.copy(), np.arange(first, n, 2)
+            x[hit, 0, hit % d] = what
+            got = attend(c, x, 0.2, **kw)
+            assert np.isnan(got[hit]).all(), (what, np.argwhere(~np.isnan(got[hit]))[:3])
+            rest = np.arange(1 - first, n, 2)
+            np.testing.assert_array_equal(got[rest], clean[rest])
