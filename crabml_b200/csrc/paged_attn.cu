@@ -18,7 +18,8 @@
 #define PT_WARPS 4
 #define PT_THREADS (PT_WARPS * 32)
 #define PT_SHIFT 9.0f                         // weights are exp2(score - base + PT_SHIFT), base the largest score so far, or up to PT_LAG less, so that the sums of a row are not scaled
-#define PT_LAG 5.0f                           // again for every score that is a little larger.  Weights stay at 2^14, times a value's factor (below 2 of its unit) below 2^15: f16 ends at 65504
+#define PT_LAG 5.0f                           // again for every score that is a little larger.  Weights stay at 2^14, times a value factor's mantissa (below 2) below 2^15: f16 ends at 65504
+#define PT_FAR 64.0f                          // 8-bit pages: products of a weight and its value's factor keep their bits down to 2^-64 of the largest weight (exp2 ends at 2^-126)
 #define PT_STEP 64                            // keys that few rows are dealt out by
 #define PT_BEGIN 5                            // what a segment's begin and end cost, in steps (finding it, the queries, the sums: 13 thousand cycles)
 #define PT_CHUNK 4096                         // keys whose page numbers and factors a CTA holds at a time
@@ -141,11 +142,17 @@ template <int D>
 struct PtRows {
     unsigned q[D / 16][4];                    // h and l of the lane's columns, as the instruction takes them
     float o[D / 8][4];                        // sums of weighted values: tile i, columns 2 t and 2 t + 1 of its eight, rows h and l
-    float inv, m, l, vref, ivref;             // power of two that q was divided by; base of the weights; the lane's sum of weights; power of two at the largest value factor so far
+    float inv, m, l, n, c;                    // power of two that q was divided by; base of the weights; the lane's sum of weights; base of the products of a weight and its value's factor, which o is in; 2^(m - n)
     int pos, lo;                              // the row's position and the first key it sees (pos -1: no row)
 };
-// 16 scores of the row -> weights; x: raw sums of keys 2 t, 2 t + 1, 8 + 2 t, 9 + 2 t.  kf, vf: the keys' and values' factors.  edge: some row does not see some key
-template <int D>
+// 2^x of a whole number; 0 below 2^-126 and for NaN
+__device__ __forceinline__ float pt_pow2(float x) { return __int_as_float(((int)fminf(fmaxf(x, -127.0f), 128.0f) + 127) << 23); }
+// the power of two below a factor, as a score: what it adds to the scores of its block; -inf for a block of zeros
+__device__ __forceinline__ float pt_log2(float vf) { return vf > 0.0f ? (float)((__float_as_int(vf) >> 23) - 127) : -INFINITY; }
+// 16 scores of the row -> weights; x: raw sums of keys 2 t, 2 t + 1, 8 + 2 t, 9 + 2 t.  kf, vf: the keys' and values' factors.  edge: some row does not see some key.
+// FACTORS (8-bit pages): a row's largest weight and its largest product of a weight and a factor may lie in blocks whose factors are far apart; the weights' sum counts from the one (m), the
+// operands of the values' product from the other (n), so that the product that counts keeps its bits whatever the factors of others.  Both are whole numbers: what is scaled is exact
+template <int D, bool FACTORS>
 __device__ __forceinline__ void pt_weights(PtRows<D>& r, float (&x)[4], int key0, float kf, float vf, bool edge, const PtArgs& a, unsigned (&p)[4], unsigned& seen) {
     const int t = threadIdx.x & 3;
     const float f = a.softcap > 0.0f ? r.inv * kf * a.scale : r.inv * kf * (a.scale * PT_LOG2E);
@@ -167,25 +174,27 @@ __device__ __forceinline__ void pt_weights(PtRows<D>& r, float (&x)[4], int key0
     float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    // the largest value factor so far, as the power of two below it: a block that the row does not see leaves its bits as they are
-    const float vp = fminf(fmaxf(__uint_as_float(__float_as_uint(vf) & 0x7f800000u), 0x1p-100f), 0x1p100f);
     // differences of scores before anything is added to them: from 2^27 on a score's last place is more than PT_LAG or PT_SHIFT, which the sum would round to more than f16 has room for
-    const bool up = mx - r.m > PT_LAG, wider = vp > r.vref && vf > 0.0f;      // (r.m -inf: every score is more)
-    if (__any_sync(0xffffffffu, up || wider)) {
+    const float top = FACTORS ? mx + pt_log2(vf) : mx;
+    const bool up = mx - r.m > PT_LAG, more = FACTORS && top - r.n > PT_LAG;      // (r.m, r.n -inf: every score is more)
+    if (__any_sync(0xffffffffu, up || more)) {
         float alpha = 1.0f;
         if (up) {
-            alpha = r.m == -INFINITY ? 0.0f : pt_exp2(r.m - mx);
-            r.m = mx;
+            const float m = FACTORS ? ceilf(mx) : mx;
+            alpha = r.m == -INFINITY ? 0.0f : FACTORS ? pt_pow2(r.m - m) : pt_exp2(r.m - m);
+            r.m = m;
+            r.l *= alpha;
         }
-        r.l *= alpha;
-        if (wider) {
-            alpha *= r.vref / vp;
-            r.vref = vp; r.ivref = 1.0f / vp;
+        if (FACTORS) {
+            const float n = fmaxf(more ? ceilf(top) : r.n, r.m - PT_FAR);
+            alpha = n == r.n || r.n == -INFINITY ? 1.0f : pt_pow2(r.n - n);      // (nothing in o so far but zeros)
+            r.n = n;
+            r.c = pt_pow2(r.m - n);
         }
 #pragma unroll
         for (int i = 0; i < D / 8; i++) { r.o[i][0] *= alpha; r.o[i][1] *= alpha; r.o[i][2] *= alpha; r.o[i][3] *= alpha; }
     }
-    const float base = r.m == -INFINITY ? 0.0f : r.m, vr = vf * r.ivref;
+    const float base = r.m == -INFINITY ? 0.0f : r.m, vr = FACTORS ? vf * r.c : vf;
 #pragma unroll
     for (int i = 0; i < 4; i++) x[i] = pt_exp2((x[i] - base) + PT_SHIFT);
     r.l += (x[0] + x[1]) + (x[2] + x[3]);
@@ -238,7 +247,7 @@ struct PtI8 {
         }
         float x[4] = {s[0][0] + s[0][2], s[0][1] + s[0][3], s[1][0] + s[1][2], s[1][1] + s[1][3]};
         unsigned p[4], seen;
-        pt_weights<D>(r, x, key0, kf, vf, edge, a, p, seen);
+        pt_weights<D, true>(r, x, key0, kf, vf, edge, a, p, seen);
         st += 2 * KC * 512;
 #pragma unroll
         for (int c = 0; c < VC; c++) {
@@ -311,7 +320,7 @@ struct PtF16 {
         }
         float x[4] = {s[0][0] + s[0][2], s[0][1] + s[0][3], s[1][0] + s[1][2], s[1][1] + s[1][3]};
         unsigned p[4], seen;
-        pt_weights<D>(r, x, key0, 1.0f, 1.0f, edge, a, p, seen);
+        pt_weights<D, WIDE>(r, x, key0, 1.0f, 1.0f, edge, a, p, seen);
         st += 2 * KC * KP * 512;
         // a value that is not finite must not meet a weight of zero in the sums of a row that does not see it
         bool wild = false;
@@ -455,7 +464,7 @@ __global__ void __launch_bounds__(PT_THREADS, D <= 64 ? 4 : D <= 128 ? 3 : 1) pa
         }
         r.pos = in ? s.pos0 + tok : -1;
         r.lo = a.window > 0 ? r.pos - a.window + 1 : 0;
-        r.m = -INFINITY; r.l = 0.0f; r.vref = I8 ? 0.0f : 1.0f; r.ivref = I8 ? 0.0f : 1.0f;
+        r.m = r.n = -INFINITY; r.l = r.c = 0.0f;
 #pragma unroll
         for (int i = 0; i < D / 8; i++) r.o[i][0] = r.o[i][1] = r.o[i][2] = r.o[i][3] = 0.0f;
     }
@@ -487,9 +496,10 @@ __global__ void __launch_bounds__(PT_THREADS, D <= 64 ? 4 : D <= 128 ? 3 : 1) pa
     r.l += __shfl_xor_sync(0xffffffffu, r.l, 2);
     // [warp][tile of 8 columns][row][column], tiles PT_TILE floats apart: no two lanes in one bank, neither here nor below
     float* sums = (float*)pt_sm;
+    const float back = I8 ? pt_pow2(r.n - r.m) : 1.0f;             // (no key: both -inf, all 0)
 #pragma unroll
     for (int i = 0; i < D / 8; i++)
-        *(float2*)(sums + (w * (D / 8) + i) * PT_TILE + g * 8 + 2 * t) = make_float2((r.o[i][0] + r.o[i][2]) * r.vref, (r.o[i][1] + r.o[i][3]) * r.vref);
+        *(float2*)(sums + (w * (D / 8) + i) * PT_TILE + g * 8 + 2 * t) = make_float2((r.o[i][0] + r.o[i][2]) * back, (r.o[i][1] + r.o[i][3]) * back);
     if (t == 0) ml[w][g] = make_float2(r.m, r.l);
     __syncthreads();
     const int n = min(8, rows - tile * 8);

@@ -38,21 +38,24 @@ static_assert(TI_SOFT * TI_REGS_SOFT + (TI_THREADS - TI_SOFT) * TI_REGS_REST <= 
 #define TI_STEPS (TI_MOST / TI_KEYS)
 
 // what stands beside the images of 128 keys of a head
-struct TiInfo {
-    float kf[TI_KEYS / 16], vf[TI_KEYS / 16]; // factors of 16 keys each; vf relative to vref, a power of two near the largest
-    float vref;
+struct __align__(16) TiInfo {
+    float kf[TI_KEYS / 16], vf[TI_KEYS / 16]; // factors of 16 keys each (0 where there are none)
+    float lv[TI_KEYS / 16];                   // 8-bit pages: how large the values of 16 keys are, as a score: log2 of their block's largest number / 127, down to a whole number (-inf: zeros)
     int wild;                                 // values that are not finite are zeros in the image
     unsigned bad[TI_KEYS / 32];               // keys whose factors or numbers are not finite (they count as 0): NaN for the rows that see one
+    int pad[3];
 };
 struct TiShared {
     unsigned long long k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full, drained;
     unsigned tmem_base;
     int fail;
     TiInfo info[TI_STEPS];
-    float top[2][TI_SPLIT][TI_ROWS], sum[TI_SPLIT][TI_ROWS], inv[TI_ROWS];
+    float2 top[2][TI_SPLIT][TI_ROWS];         // of a step: largest score, and largest sum of a score and its block's lv
+    float sum[TI_SPLIT][TI_ROWS], inv[TI_ROWS];
 };
 #define TI_OPERAND (TI_KEYS * TI_D * 2)       // bytes of a tile of f16: two blocks of 64 columns, rows of 128 bytes under the 128-byte swizzle
 #define TI_SMEM (6 * TI_OPERAND + 1024)
+#define TI_UP 30                              // the smallest numbers of f16, 2^-24, reach 2^6
 #define TI_TOP 512.0f                         // the largest weight, 2^PT_SHIFT
 #define TI_SFU 14                             // of 16 weights those that the special function unit makes: 214 us for the portions of three prompts; 10 of them 222, 12 216, all 217
 #define TI_O 256                              // TMEM columns: S and P at 0 and 128
@@ -147,6 +150,8 @@ __host__ __device__ __forceinline__ int ti_key_tiles(const PgSeq& s, const PtArg
 template <bool I8>
 __global__ void __launch_bounds__(TU_THREADS) paged_unpack_kernel(const PtArgs a) {
     __shared__ int pages[TI_KEYS / 16];
+    __shared__ unsigned top[TI_KEYS];                          // of open rows: their largest value, as bits of f16
+    __shared__ float up[TI_KEYS / 16];                         // powers of two that the open block's values are multiplied by, 16 keys each
     __shared__ TiInfo info;
     const int tid = threadIdx.x, kvh = a.head0 + blockIdx.y;
     pdl_enter();
@@ -158,7 +163,7 @@ __global__ void __launch_bounds__(TU_THREADS) paged_unpack_kernel(const PtArgs a
     pt_range(s, a, &from, &to);
     const int key0 = from + kt * TI_KEYS, opens = I8 ? to >> a.shift << a.shift : 0, open = 2 * s.slot + ((to >> a.shift) & 1);
     if (tid < 32) {
-        float kf = 1.0f, vf = 1.0f;
+        float kf = 1.0f, vf = 1.0f, lv = 0.0f;
         const int key = key0 + (tid & 7) * 16;
         int page = -1;                                        // nothing there, or the open block
         if (key < to && (!I8 || key < opens)) {
@@ -166,14 +171,37 @@ __global__ void __launch_bounds__(TU_THREADS) paged_unpack_kernel(const PtArgs a
             if (I8) { kf = a.ks[(int64_t)page * a.G + kvh]; vf = a.vs[(int64_t)page * a.G + kvh]; }
         }
         const bool bad = !(vf >= 0.0f && vf < INFINITY && kf >= 0.0f && kf < INFINITY);
-        if (bad) kf = vf = 0.0f;
-        const float vmax = warp_max(vf), vref = fminf(fmaxf(__uint_as_float(__float_as_uint(vmax) & 0x7f800000u), 0x1p-100f), 0x1p100f);
+        if (bad || key >= to) kf = vf = 0.0f;
+        lv = pt_log2(vf);
         const unsigned nan = __ballot_sync(0xffffffffu, bad) >> 2 * (tid & 3);      // the lanes' groups repeat after 8
-        if (tid < TI_KEYS / 16) { pages[tid] = page; info.kf[tid] = kf; info.vf[tid] = vf / vref; }
+        if (tid < TI_KEYS / 16) { pages[tid] = page; info.kf[tid] = kf; info.vf[tid] = vf; info.lv[tid] = lv; }
         if (tid < TI_KEYS / 32) info.bad[tid] = (nan & 1u ? 0xffffu : 0u) | (nan & 2u ? 0xffff0000u : 0u);
-        if (tid == 0) info.vref = vref;
     }
     __syncthreads();
+    // The open block's values are made as large as codes are, by a power of two that its 16 keys' first one sets (any query that sees one of them sees that, but for windows) as far as all
+    // of them stay in range: exactly, for it only multiplies.  Its factor is the inverse
+    if (I8 && key0 + TI_KEYS > opens && opens < to) {
+        if (tid < TI_KEYS) top[tid] = 0u;
+        __syncthreads();
+        for (int e = tid; e < TI_KEYS * (a.dv / 8); e += TU_THREADS) {
+            const int r = e / (a.dv / 8), key = key0 + r;
+            if (key < opens || key >= to) continue;
+            const uint4 x = __ldg((const uint4*)(a.vo + (((size_t)open * a.G + kvh) * a.page + (key & (a.page - 1))) * a.dv) + (e - r * (a.dv / 8)));
+            const unsigned m = __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu & ~pt_wild(x.x), x.y & 0x7fff7fffu & ~pt_wild(x.y)), __vmaxu2(x.z & 0x7fff7fffu & ~pt_wild(x.z), x.w & 0x7fff7fffu & ~pt_wild(x.w)));
+            atomicMax(&top[r], max(m & 0xffffu, m >> 16));
+        }
+        __syncthreads();
+        if (tid < TI_KEYS / 16 && pages[tid] < 0 && key0 + tid * 16 < to) {
+            unsigned most = 0;
+            for (int i = 0; i < 16; i++) most = max(most, top[tid * 16 + i]);
+            const unsigned first = top[tid * 16] ? top[tid * 16] : most;
+            auto log2_of = [](unsigned h) { return (__float_as_int(__half2float(__ushort_as_half((unsigned short)h))) >> 23) - 127; };
+            const int by = most ? max(0, min(TI_UP, min(6 - log2_of(first), 14 - log2_of(most)))) : 0;
+            up[tid] = pt_pow2((float)by); info.vf[tid] = pt_pow2((float)-by);
+            info.lv[tid] = most ? (float)max(log2_of(first) - 6, -by) : -INFINITY;
+        }
+        __syncthreads();
+    }
     const size_t at = (size_t)blockIdx.x * a.heads + blockIdx.y;
     bool wild = false;
 #pragma unroll
@@ -202,6 +230,15 @@ __global__ void __launch_bounds__(TU_THREADS) paged_unpack_kernel(const PtArgs a
                 }
                 if (any && v) wild = true;
                 if (any && !v) atomicOr(&info.bad[r >> 5], 1u << (r & 31));
+                if (I8 && v) {                                 // (2^15 at a time: f16 ends there)
+                    const float by = up[r >> 4];
+                    const __half2 f = __float2half2_rn(fminf(by, 32768.0f)), g = __float2half2_rn(fmaxf(by / 32768.0f, 1.0f));
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const __half2 z = __hmul2(__hmul2(*(const __half2*)u[i], f), g);
+                        *u[i] = *(const unsigned*)&z;
+                    }
+                }
             }
             *(uint4*)(image + ti_at(r, 2 * piece)) = x;
             *(uint4*)(image + ti_at(r, 2 * piece + 1)) = y;
@@ -374,14 +411,14 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
         const int pos = in ? s.pos0 + tok : -1, key_lo = a.window > 0 ? pos - a.window + 1 : 0, key_hi = min(pos, k1 - 1);      // the last step may reach into the next slice
         const float f0 = sh.inv[row] * fabsf(a.scale) * (CAP ? 1.0f : PT_LOG2E);
         ti_f2 acc[TI_OC / 2];
-        float m = -INFINITY, l = 0.0f, alpha_prev = 0.0f, vref_prev = 0.0f;
+        float m = -INFINITY, l = 0.0f, alpha_prev = 0.0f, unit_prev = 0.0f;
 #pragma unroll
         for (int i = 0; i < TI_OC / 2; i++) acc[i] = 0ull;
         bool ok = true;
         auto add = [&](int k) {                                       // the sums of step k
             if (!(ok = ok && ti_wait_warp(pg_smem(&sh.o_full), k & 1, &sh.fail))) return;
             pg_fence_after();
-            const ti_f2 alpha2 = ti_two(alpha_prev, alpha_prev), vref2 = ti_two(vref_prev, vref_prev);
+            const ti_f2 alpha2 = ti_two(alpha_prev, alpha_prev), unit2 = ti_two(unit_prev, unit_prev);
 #pragma unroll
             for (int c = 0; c < TI_OC; c += 32) {
                 if (c >= cols) break;
@@ -395,7 +432,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
                     asm volatile("" : "+r"(v[i]), "+r"(v[i + 1]));
                     const ti_f2 o = ti_two(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
                     ti_f2& to = acc[(c + i) / 2];
-                    to = I8 ? ti_fma2(o, vref2, ti_mul2(to, alpha2)) : ti_fma2(to, alpha2, o);
+                    to = I8 ? ti_fma2(o, unit2, ti_mul2(to, alpha2)) : ti_fma2(to, alpha2, o);
                 }
             }
             pg_fence_before();
@@ -435,22 +472,34 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
                 for (int c = 0; c < TI_XC; c++)
                     if (c > c_hi || c < c_lo) x[c] = 0xff800000u;
             }
-            float mx = -INFINITY;
+            float mx = -INFINITY, nx = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < TI_XC; c += 2) mx = ti_max3(mx, __uint_as_float(x[c]), __uint_as_float(x[c + 1]));
-            sh.top[slot][part][row] = mx;
+            for (int g = 0; g < TI_XC / 16; g++) {
+                float y = fmaxf(__uint_as_float(x[g * 16]), __uint_as_float(x[g * 16 + 1]));
+#pragma unroll
+                for (int c = 2; c < 16; c += 2) y = ti_max3(y, __uint_as_float(x[g * 16 + c]), __uint_as_float(x[g * 16 + c + 1]));
+                mx = fmaxf(mx, y);
+                if (I8) nx = fmaxf(nx, y + sh.info[k].lv[part * (TI_XC / 16) + g]);
+            }
+            sh.top[slot][part][row] = make_float2(mx, nx);
             ti_soft_sync();                                           // .. and all parts have read S
 #pragma unroll
-            for (int i = 0; i < TI_SPLIT; i++) mx = fmaxf(mx, sh.top[slot][i][row]);
+            for (int i = 0; i < TI_SPLIT; i++) {
+                const float2 z = sh.top[slot][i][row];
+                mx = fmaxf(mx, z.x); nx = fmaxf(nx, z.y);
+            }
             const float* vfs = sh.info[k].vf;
             const float m_new = fmaxf(m, mx), base = m_new == -INFINITY ? 0.0f : -m_new;
             const float alpha = m == m_new ? 1.0f : pt_exp2(m - m_new);
             m = m_new;
+            // The operands of the values' product, a weight times its block's factor, are near 2^9 where that is largest for this row in this step, whatever the other factors and weights: `unit`
+            // is the power of two that they are in, 2^-PT_FAR at least: a hidden key's 2^-126 stays 0
+            const float unit = I8 ? pt_pow2(fmaxf(floorf(nx - m_new), -PT_FAR)) : 1.0f, per_unit = I8 ? TI_TOP * pt_pow2(-fmaxf(floorf(nx - m_new), -PT_FAR)) : TI_TOP;
             ti_f2 sum = 0ull;
             const ti_f2 base2 = ti_two(base, base), minus = ti_two(-1.0f, -1.0f);
             auto weights = [&](int g) {                               // of 16 keys: 8 words of h, 8 of l
                 unsigned h[8], w[8];
-                const float vr = I8 ? TI_TOP * vfs[part * (TI_XC / 16) + g] : TI_TOP;
+                const float vr = I8 ? per_unit * vfs[part * (TI_XC / 16) + g] : per_unit;
                 const ti_f2 vr2 = ti_two(vr, vr);
 #pragma unroll
                 for (int c = 0; c < 16; c += 2) {
@@ -481,7 +530,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
             }
             const float2 sums = ti_one(sum);
             l = fmaf(l, alpha, (sums.x + sums.y) * TI_TOP);
-            alpha_prev = alpha; vref_prev = I8 ? sh.info[k].vref : 1.0f;
+            alpha_prev = alpha; unit_prev = unit;
         }
         if (steps > 0) add(steps - 1);
         if (isnan(f0)) l = NAN;                                       // a query that is not finite: maxima and the pairs' exponentials drop NaN

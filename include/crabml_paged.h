@@ -62,7 +62,8 @@ CC_API int cc_paged_append(cc_device* dev, const cc_page_plan* plan, const cc_pa
  * cache holds them after the append:
  *   score = scale * (q . k), or softcap * tanh(that / softcap) with softcap > 0; softmax with a denominator that also holds exp(sink[h]) (sink: [n_heads] or
  *   NULL); the weighted sum of the values.
- * Head h reads key head h / (n_heads / n_kv).  out: F32 [T, n_heads * dv], as exact as 32-bit sums are.  A key or value that is not finite reaches the results of
+ * Head h reads key head h / (n_heads / n_kv).  out: F32 [T, n_heads * dv], sums of 32 bits of weights of 22: a weight (8-bit pages: times
+ * its block's factor) is off by 2^-22 of itself, or by 2^-33 of the row's largest if that is more.  A key or value that is not finite reaches the results of
  * the queries that see it (not all of them, where its weight is zero) and no others; a query that holds a NaN or an infinity has the result NaN; rows behind a
  * sequence's end are not looked at. */
 CC_API int cc_paged_attention(cc_device* dev, const cc_page_plan* plan, const cc_paged_cache* cache, const cc_view* q, int32_t n_heads, float scale, int32_t window,
