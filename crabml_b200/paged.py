@@ -26,7 +26,10 @@ def _whole(what, a, kind):
 
 class PagePlan:
     """What the sequences of a step have in the cache (pos0), bring along (counts) and own (table: rows of page numbers, an array or lists of any lengths; slots:
-    their open blocks, sequence i slot i where it is None).  Checked once; every layer's append and attention take it."""
+    their open blocks, sequence i slot i where it is None).  Checked once; every layer's append and attention take it.
+
+    A position below what a sequence has had takes it back (rejected drafts): to the start of any block, or, with 8-bit pages, to a token of the block that its next token
+    falls into or of the one before, counted from the furthest it has reached; include/crabml_paged.h has the rule."""
 
     def __init__(self, device, page_size, n_pages, table, pos0, counts, n_slots=0, slots=None):
         self.device, self.handle = device, None

@@ -41,8 +41,10 @@ CC_API int64_t cc_page_plan_tokens(const cc_page_plan* plan);
  * I8: a page holds a block of page_size tokens once all of them are there.  Per head, with a the largest magnitude of the block's 16-bit numbers x: the factor
  *   a / 127 in k_scale, v_scale [n_pages, n_kv] (F32) and the codes round(127 x / a), ties to even; every number is rounded to 8 bits once, whatever portions a
  *   sequence came in.  Tokens of a block that is not complete lie in k_open, v_open [2 * n_slots, n_kv, page_size, dk / dv] (F16): block b of the sequence with
- *   slot s in row 2 s + b mod 2.  A block stays there until the second next begins, so that a sequence may go back to any token of its last block or of the one
- *   before it (rejected drafts), or to the start of any block.
+ *   slot s in row 2 s + b mod 2.  So do those of the block before it; of blocks that a call completes further back it leaves no 16-bit rows.  A sequence may go
+ *   back (rejected drafts: a plan with pos0 below its length) to the start of any block, and to any token from page_size * (e / page_size - 1) on, though not
+ *   below the start that it last went back to, where e is the furthest it has reached since then.  Of a sequence at the end of a block that is page_size tokens.
+ *   Nothing notices one that goes back elsewhere: its block takes rows that are not its own.
  * Finite numbers beyond the range of 16 bits become its largest.  A block that holds an infinity or a NaN has the factor NaN. */
 typedef struct cc_paged_cache {
     cc_view k, v, k_scale, v_scale, k_open, v_open;

@@ -197,6 +197,33 @@ def test_going_back(dev, back):
         np.testing.assert_array_equal(got, c.ref.a[name + "_open"][2 * c.slot(0) + end // P % 2, :, :end % P])
 
 
+@pytest.mark.parametrize("first", [16, 32, 48, 61])
+@pytest.mark.parametrize("back", [0, 1, 15, 16])
+def test_going_back_from_the_end_of_a_block(dev, first, back):
+    """portions that end with a block, and drafts behind them: from there a sequence goes back by up to a block's tokens, or to the start of any"""
+    G, d, P = 1, 16, 16
+    r = np.random.default_rng(first + back)
+    for at in (64 - back, 0, 16, 48):
+        c = Case(dev, P, G, d, d, True, [0], [90], seed=back)
+        a, b = r.normal(size=(64, 2 * d)).astype(np.float32), r.normal(size=(21, 2 * d)).astype(np.float32)
+        for lo, hi in ((0, first), (first, 64)):
+            if hi > lo:
+                t = give(dev, a[lo:hi])
+                paged.append(c.plan([lo], [hi - lo]), c.cache, None, 0, t, 0, t, d)
+        t = give(dev, b)
+        paged.append(c.plan([at], [21]), c.cache, None, 0, t, 0, t, d)
+        every = np.concatenate([a[:at], b])
+        x = {"k": every[:, None, :d], "v": every[:, None, d:]}
+        end = len(every)
+        for name in ("k", "v"):
+            for blk in range(end // P):                      # the reference's block from all of the sequence's rows, not by way of open ones
+                code, factor = R.codes(R.f16(x[name][blk * P:(blk + 1) * P, 0]))
+                np.testing.assert_array_equal(take(dev, getattr(c.cache, name))[c.table[0][blk], 0], code)
+                assert take(dev, getattr(c.cache, name + "_scale"))[c.table[0][blk], 0] == factor
+            got = take(dev, getattr(c.cache, name + "_open"))[2 * c.slot(0) + end // P % 2, 0, :end % P]
+            np.testing.assert_array_equal(got, R.f16(x[name][end // P * P:, 0]))
+
+
 def test_numbers_at_the_ends(dev):
     """numbers beyond 16 bits, zeros, subnormal ones, ties, infinities and NaN; blocks of other heads stay clean"""
     G, d, P = 4, 16, 16

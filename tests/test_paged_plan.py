@@ -126,3 +126,38 @@ def test_numbers_that_are_not_whole_or_too_large():
                 dict(table=np.array([[1 << 32]])), dict(table=np.array([[0.0]])), dict(pos0=np.array([1 << 63], np.uint64)), dict(slots=[0, 1]), dict(pos0=[0, 0])):
         with pytest.raises(TensorError):
             paged.PagePlan(None, 16, 4, n_slots=1, **{**good, **bad})
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_where_a_sequence_may_go_back(build, seed):
+    """what the header allows, played on the segments: every open row that a block is completed from is the sequence's own, portions that end with a block among them"""
+    r = random.Random(seed)
+    P, borders = r.choice([16, 32]), 0
+    have, half = [], [[None] * P, [None] * P]                # the sequence's tokens as (position, call); what its two open blocks hold
+    start = far = 0                                          # where it last went back to a block's start; the furthest since then
+    for call in range(60):
+        lowest = max(start, P * (far // P - 1))
+        at = r.choice([len(have), len(have), min(lowest, len(have)), r.randint(min(lowest, len(have)), len(have)), P * r.randint(0, len(have) // P)])
+        n = r.choice([1, 1, r.randint(1, 3 * P), P * ((at + P - 1) // P + r.randint(0, 3)) - at])
+        n = max(n, 1)
+        if at < lowest:                                      # to the start of a block further back
+            start, far = at, at
+        have = have[:at] + [(p, call) for p in range(at, at + n)]
+        far = max(far, at + n)
+        borders += (at + n) % P == 0
+        pages = (at + n + P - 1) // P
+        (items, _, _), segs = build(P, pages, [list(range(pages))], [at], [n], 1)
+        for first in range(items):
+            i = first
+            while i >= 0:
+                g = segs[i]
+                own = have[g["block"] * P:(g["block"] + 1) * P]
+                rows = half[g["half"]]
+                if g["flags"] & FULL:
+                    assert rows[:g["row0"]] == own[:g["row0"]], (call, at, n, g)
+                if g["flags"] & KEPT:
+                    rows[g["row0"]:g["row0"] + g["rows"]] = own[g["row0"]:g["row0"] + g["rows"]]
+                i = g["next"]
+        if (at + n) % P:                                     # attention reads the open block
+            assert half[(at + n) // P % 2][:(at + n) % P] == have[(at + n) // P * P:], (call, at, n)
+    assert borders > 5
