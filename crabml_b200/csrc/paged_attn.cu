@@ -61,7 +61,7 @@ __host__ __device__ __forceinline__ int pt_splits(const PgSeq& s, const PtArgs& 
     if (rows < a.rows_lo || rows > a.rows_hi) return 0;
     int from, to;
     pt_range(s, a, &from, &to);
-    return (to - from + a.split - 1) / a.split;
+    return (to - from - 1) / a.split + 1;
 }
 // keys of a slice: the sequence's in equal parts
 __host__ __device__ __forceinline__ int pt_each(int keys, int n_split) { return ((keys + n_split - 1) / n_split + 127) / 128 * 128; }
@@ -703,13 +703,14 @@ static int pt_run_few(cc_device* dev, const cc_page_plan* plan, PtArgs a, bool i
 }
 #include "paged_tile.cuh"
 
-#define TI_WORKSPACE ((int64_t)256 << 20)     // bytes of images that a call has at a time, as long as one head's are no more
+#define TI_WORKSPACE ((int64_t)256 << 20)     // bytes of images that a call has at a time, as long as those of one sequence and head are no more; and of sums of slices
 
 // How long a call takes with slices of a.split keys, in cycles.  An item's start and end 18000, a step of 128 keys 3900; CTAs take items in turn, so that the SMs end half of the longest one apart;
 // sums of slices are written and read at 3 TB/s (1600 bytes a cycle), 10000 cycles for the kernel that adds them up
-static double pt_guess(const cc_page_plan* plan, const PtArgs& a, int sms) {
+static double pt_guess(const PgSeq* seqs, const PtArgs& a, int sms) {
     double all = 0.0, longest = 0.0, sums = 0.0, items = 0.0;
-    for (const PgSeq& s : plan->seqs) {
+    for (int i = 0; i < a.n_seqs; i++) {
+        const PgSeq& s = seqs[i];
         const int n = pt_splits(s, a);
         if (!n) continue;
         int from, to;
@@ -722,34 +723,34 @@ static double pt_guess(const cc_page_plan* plan, const PtArgs& a, int sms) {
     }
     return (items <= sms ? longest : std::max(longest, all / sms + 0.5 * longest)) + (sums > 0.0 ? sums + 10000.0 : 0.0);
 }
-// sequences of many rows: of some lengths of slices the one that should take least time.  (As many as give every SM one, against this, 32 heads on 8: 4 sequences of 3000 to 6000 tokens
-// with 16 to 128 new ones 120 us and 92, 8 of 3000 with 64 106 and 93, 16 of 500 to 3000 with 16 to 64 146 and 132; 256 tokens over 8000 149 and 148, where slices of 2560 take 130)
-static int pt_run_tiles(cc_device* dev, const cc_page_plan* plan, PtArgs a, bool i8) {
-    int64_t keys = 0, items = 0, split_rows = 0, key_tiles = 0;             // split_rows: groups of PT_SUM rows of sequences in several slices
-    for (const PgSeq& s : plan->seqs) {
-        const int64_t rows = (int64_t)s.count * a.R;
-        if (rows < a.rows_lo || rows > a.rows_hi) continue;
-        int from, to;
-        pt_range(s, a, &from, &to);
-        keys += (int64_t)(to - from) * ((rows + a.tile_rows - 1) / a.tile_rows) * a.G;
-        key_tiles += ti_key_tiles(s, a);
+// slices of a.split keys: the items of a head, and the groups of PT_SUM rows whose slices are to be added up
+static void pt_count(const PgSeq* seqs, const PtArgs& a, int64_t* items, int64_t* split_rows) {
+    *items = *split_rows = 0;
+    for (int i = 0; i < a.n_seqs; i++) {
+        const int n = pt_splits(seqs[i], a);
+        *items += (int64_t)n * (((int64_t)seqs[i].count * a.R + a.tile_rows - 1) / a.tile_rows);
+        if (n > 1) *split_rows += ((int64_t)seqs[i].count * a.R + PT_SUM - 1) / PT_SUM;
     }
-    if (!keys) return CC_OK;
+}
+// Sequences of many rows: of some lengths of slices the one that should take least time.  (As many as give every SM one, against this, 32 heads on 8: 4 sequences of 3000 to 6000 tokens
+// with 16 to 128 new ones 120 us and 92, 8 of 3000 with 64 106 and 93, 16 of 500 to 3000 with 16 to 64 146 and 132; 256 tokens over 8000 149 and 148, where slices of 2560 take 130.)
+// A row that is cut leaves its sums for each slice: those of a long prompt would be gigabytes, while it has rows enough for every SM without; so not beyond TI_WORKSPACE
+static int pt_tiles(cc_device* dev, const PgSeq* seqs, PtArgs a, int64_t key_tiles, bool i8) {
+    const size_t kb = (size_t)((a.dk + 63) / 64) * TI_BLOCK, vb = (size_t)((a.dv + 63) / 64) * TI_BLOCK, per_head = (size_t)key_tiles * (kb + vb + sizeof(TiInfo));
+    const size_t per_row = (size_t)a.dv * sizeof(float) + sizeof(float2);
     int best = 0;
     double least = 0.0;
-    for (int split : {TI_MOST, 2560, 2048, 1536, 1024, 768, 512}) {
+    int64_t items, split_rows;
+    for (int split : {TI_WHOLE, 4096, 2560, 2048, 1536, 1024, 768, 512}) {
         a.split = split;
-        const double t = pt_guess(plan, a, dev->sm_count);
+        pt_count(seqs, a, &items, &split_rows);
+        if (split_rows && (double)items * a.G * a.tile_rows * per_row > (double)TI_WORKSPACE) continue;
+        const double t = pt_guess(seqs, a, dev->sm_count);
         if (!best || t < 0.97 * least) { best = split; least = t; }
     }
     a.split = best;
-    for (const PgSeq& s : plan->seqs) {
-        const int n = pt_splits(s, a);
-        items += (int64_t)n * (((int64_t)s.count * a.R + a.tile_rows - 1) / a.tile_rows);
-        if (n > 1) split_rows += ((int64_t)s.count * a.R + PT_SUM - 1) / PT_SUM;
-    }
+    pt_count(seqs, a, &items, &split_rows);
     CC_REQUIRE(dev, items * a.G < ((int64_t)1 << 31) && split_rows < ((int64_t)1 << 31) && key_tiles < ((int64_t)1 << 31), "paged_attention: too many rows");
-    const size_t kb = (size_t)((a.dk + 63) / 64) * TI_BLOCK, vb = (size_t)((a.dv + 63) / 64) * TI_BLOCK, per_head = (size_t)key_tiles * (kb + vb + sizeof(TiInfo));
     a.heads = (int64_t)per_head * a.G <= TI_WORKSPACE ? a.G : (int)std::max<int64_t>(1, TI_WORKSPACE / (int64_t)per_head);
     const size_t part = split_rows ? (size_t)items * a.heads * a.tile_rows * a.dv * sizeof(float) : 0, ml = split_rows ? (size_t)items * a.heads * a.tile_rows * sizeof(float2) : 0;
     void* ws = nullptr; size_t cls = 0;
@@ -775,6 +776,22 @@ static int pt_run_tiles(cc_device* dev, const cc_page_plan* plan, PtArgs a, bool
     }
     if (ws) cc_pool_free(dev, ws, cls);
     if (e != cudaSuccess) return cc_fail(dev, CC_ERR_CUDA, "paged_attention: %s", cudaGetErrorString(e));
+    return CC_OK;
+}
+// as many sequences at a time as have their images of one head in TI_WORKSPACE
+static int pt_run_tiles(cc_device* dev, const cc_page_plan* plan, PtArgs a, bool i8) {
+    const int64_t per_tile = (int64_t)((a.dk + 63) / 64 + (a.dv + 63) / 64) * TI_BLOCK + (int64_t)sizeof(TiInfo);
+    for (int first = 0, end; first < plan->n_seqs; first = end) {
+        int64_t key_tiles = 0;
+        for (end = first; end < plan->n_seqs; end++) {
+            const int n = ti_key_tiles(plan->seqs[end], a);
+            if (key_tiles && (key_tiles + n) * per_tile > TI_WORKSPACE) break;
+            key_tiles += n;
+        }
+        a.seqs = plan->d_seqs + first; a.n_seqs = end - first; a.table = plan->d_table + (int64_t)first * a.table_cols;
+        const int rc = key_tiles ? pt_tiles(dev, plan->seqs.data() + first, a, key_tiles, i8) : CC_OK;
+        if (rc) return rc;
+    }
     return CC_OK;
 }
 

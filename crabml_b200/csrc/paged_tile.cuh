@@ -11,12 +11,14 @@
 //                             thousands of keys would drift (1e-5 of a result after 2000 keys of one sign)
 // TMEM holds S twice, O, Q_h and Q_l (512 columns), shared memory two stages of K and V (128 KB): while 8 warps make the weights of one step, the tensor core computes the
 // scores of the next and the sums of the one before.  With Q in shared memory a step's products read 192 KB there and took 3100 cycles instead of 2050.
-// A row's 128 scores lie with two threads, a half each, which exchange their largest score once a step.  Warps 0-7 weights and sums, 8 the copies, 9 the products.
+// A row's 128 scores lie with two threads, a half each, which exchange their largest score once a step.  Warps 0-7 weights and sums, 8 the copies, 9 the products, 10 what stands beside the images.
 // Portions of three prompts (3000 rows of 32 heads on 8, 8-bit pages): 12 us of images and 214 of tiles, 318 TFLOP/s of the four products' 68 GFLOP, of which the h and l of
 // queries and weights make two.  A step takes 3900 cycles, its products 2050 of them, the weights' instructions 1500; the rest is the way of a step's scores through one group of warps
 // in turn (wait, read, largest, meet, weights, store).  Sums of four steps left to the tensor core, fewer reads of O, took 3 % more.
 // Every wait is bounded (sg_wait); where one ran out all roles run to their ends without waiting (the barrier of warps 0-7 included) and the host reports it.
 #pragma once
+#include <stddef.h>
+
 #include "split_gemm.cuh"
 
 #define TI_ROWS 128
@@ -33,9 +35,9 @@
 static_assert(TI_SOFT * TI_REGS_SOFT + (TI_THREADS - TI_SOFT) * TI_REGS_REST <= TI_THREADS * TI_REGS, "more registers than the block was launched with");
 #define TI_XC (TI_KEYS / TI_SPLIT)
 #define TI_OC (TI_D / TI_SPLIT)
-#define TI_MOST 4096                          // keys of a slice
+#define TI_WHOLE 0x7fffff00                   // keys of a slice: all
 #define TI_D 128                              // largest dk and dv
-#define TI_STEPS (TI_MOST / TI_KEYS)
+#define TI_STEPS 32                           // whose TiInfo a CTA holds at a time
 
 // what stands beside the images of 128 keys of a head
 struct __align__(16) TiInfo {
@@ -45,10 +47,15 @@ struct __align__(16) TiInfo {
     unsigned bad[TI_KEYS / 32];               // keys whose factors or numbers are not finite (they count as 0): NaN for the rows that see one
     int pad[3];
 };
+#define TI_WORDS ((int)(sizeof(TiInfo) / 4))
+static_assert(TI_WORDS == 32, "a word for each lane");
+__device__ __forceinline__ bool ti_odd(int word) { return word >= (int)(offsetof(TiInfo, wild) / 4) && word < (int)(offsetof(TiInfo, pad) / 4); }      // wild, or bad
 struct TiShared {
     unsigned long long k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full, drained;
     unsigned tmem_base;
     int fail;
+    int odd;                                  // some TiInfo says wild or bad
+    const TiInfo* first;                      // of the first step
     TiInfo info[TI_STEPS];
     float2 top[2][TI_SPLIT][TI_ROWS];         // of a step: largest score, and largest sum of a score and its block's lv
     float sum[TI_SPLIT][TI_ROWS], inv[TI_ROWS];
@@ -135,6 +142,7 @@ __device__ __forceinline__ float ti_max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
+__device__ __forceinline__ void ti_step_sync() { asm volatile("bar.sync 2, %0;" ::"n"(TI_SOFT + 32) : "memory"); }
 __device__ __forceinline__ void ti_soft_sync() { asm volatile("bar.sync 1, %0;" ::"n"(TI_SOFT) : "memory"); }
 
 // images of the sequences with a tile of 128 rows: their tiles of keys count from the first that a new token sees, sequence after sequence
@@ -265,6 +273,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
         pg_mbar_init(pg_smem(&sh.o_full), 1);
         pg_mbar_init(pg_smem(&sh.drained), 1);
         sh.fail = 0;
+        sh.odd = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == (TI_SOFT_WARPS + 1)) {
@@ -286,13 +295,15 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
     const int each = pt_each(to - from, n_split), k0 = from + split * each, k1 = min(min(to, k0 + each), pos_last + 1);
     const int lo = a.window > 0 ? max(k0, (pos_first - a.window + 1) & ~(TI_KEYS - 1)) : k0, steps = k1 > lo ? (k1 - lo + TI_KEYS - 1) / TI_KEYS : 0;
     const int opens = I8 ? to >> a.shift << a.shift : 0;
-    // the images of the first step, and what stands beside those of all steps
+    // the images of the first step, and what stands beside those of the first TI_STEPS
     int before = 0;
     for (int x = lane; x < seq; x += 32) before += ti_key_tiles(a.seqs[x], a);
     const size_t image = (size_t)(warp_sum_i(before) + (lo - from) / TI_KEYS) * a.heads + head_at;
-    for (int i = tid; i < steps * (int)(sizeof(TiInfo) / 4); i += TI_THREADS) {
-        const int k = i / (int)(sizeof(TiInfo) / 4);
-        ((int*)sh.info)[i] = ((const int*)(a.info + image + (size_t)k * a.heads))[i - k * (int)(sizeof(TiInfo) / 4)];
+    if (tid == 0) sh.first = a.info + image;
+    for (int i = tid; i < min(steps, TI_STEPS) * TI_WORDS; i += TI_THREADS) {
+        const int x = ((const int*)(a.info + image + (size_t)(i / TI_WORDS) * a.heads))[i % TI_WORDS];
+        ((int*)sh.info)[i] = x;
+        if (x && ti_odd(i % TI_WORDS)) sh.odd = 1;
     }
     // the queries as h and l, near 2^14
     const int row = (warp & 3) * 32 + lane, part = warp >> 2;         // of weights and sums: TMEM lane, part of the columns
@@ -403,6 +414,16 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
             for (int i = max(0, v - 2); i < v; i++) ti_wait(pg_smem(&sh.v_full[i & 1]), (i >> 1) & 1u, &never);
         }
         __syncwarp();
+        } else if (warp == TI_SOFT_WARPS + 2) {
+        // ===== what stands beside the images: the place of the step before goes to the one TI_STEPS behind it =====
+            for (int k = 0; k < steps; k++) {
+                ti_step_sync();                                       // the weights are through with step k - 1
+                const int next = k - 1 + TI_STEPS;
+                if (k == 0 || next >= steps) continue;
+                const int x = ((const int*)(sh.first + (size_t)next * a.heads))[lane];
+                ((int*)(sh.info + next % TI_STEPS))[lane] = x;
+                if (x && ti_odd(lane)) sh.odd = 1;
+            }
         }
     } else {
         // ===== weights and sums =====
@@ -443,7 +464,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
             const int key0 = lo + k * TI_KEYS + part * TI_XC;
             float f[TI_XC / 16];                                               // factor of 16 keys' sums
 #pragma unroll
-            for (int g = 0; g < TI_XC / 16; g++) f[g] = f0 * sh.info[k].kf[part * (TI_XC / 16) + g];
+            for (int g = 0; g < TI_XC / 16; g++) f[g] = f0 * sh.info[k & (TI_STEPS - 1)].kf[part * (TI_XC / 16) + g];
             ok = ok && ti_wait_warp(pg_smem(&sh.s_full[slot]), (k >> 1) & 1u, &sh.fail);
             unsigned x[TI_XC];
             if (ok) {
@@ -479,16 +500,16 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
 #pragma unroll
                 for (int c = 2; c < 16; c += 2) y = ti_max3(y, __uint_as_float(x[g * 16 + c]), __uint_as_float(x[g * 16 + c + 1]));
                 mx = fmaxf(mx, y);
-                if (I8) nx = fmaxf(nx, y + sh.info[k].lv[part * (TI_XC / 16) + g]);
+                if (I8) nx = fmaxf(nx, y + sh.info[k & (TI_STEPS - 1)].lv[part * (TI_XC / 16) + g]);
             }
             sh.top[slot][part][row] = make_float2(mx, nx);
-            ti_soft_sync();                                           // .. and all parts have read S
+            ti_step_sync();                                           // .. and all parts have read S
 #pragma unroll
             for (int i = 0; i < TI_SPLIT; i++) {
                 const float2 z = sh.top[slot][i][row];
                 mx = fmaxf(mx, z.x); nx = fmaxf(nx, z.y);
             }
-            const float* vfs = sh.info[k].vf;
+            const float* vfs = sh.info[k & (TI_STEPS - 1)].vf;
             const float m_new = fmaxf(m, mx), base = m_new == -INFINITY ? 0.0f : -m_new;
             const float alpha = m == m_new ? 1.0f : pt_exp2(m - m_new);
             m = m_new;
@@ -537,9 +558,10 @@ __global__ void __launch_bounds__(TI_THREADS, 1) paged_tile_kernel(const __grid_
         // values and factors that are not finite were left out: NaN for the rows that see them
         unsigned long long lost = 0;
 #pragma unroll 1
-        for (int k = 0; k < steps; k++) {
-            const unsigned* bad = sh.info[k].bad;
-            if (!(bad[0] | bad[1] | bad[2] | bad[3] | (unsigned)sh.info[k].wild)) continue;
+        for (int k = 0; sh.odd && k < steps; k++) {
+            const TiInfo& info = sh.first[(size_t)k * a.heads];
+            const unsigned* bad = info.bad;
+            if (!(bad[0] | bad[1] | bad[2] | bad[3] | (unsigned)info.wild)) continue;
             const int key0 = lo + k * TI_KEYS;
 #pragma unroll 1
             for (int key = max(key0, key_lo); key <= min(key0 + TI_KEYS - 1, key_hi); key++) {

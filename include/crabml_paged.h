@@ -67,7 +67,10 @@ CC_API int cc_paged_append(cc_device* dev, const cc_page_plan* plan, const cc_pa
  * Head h reads key head h / (n_heads / n_kv).  out: F32 [T, n_heads * dv], sums of 32 bits of weights of 22: a weight (8-bit pages: times
  * its block's factor) is off by 2^-22 of itself, or by 2^-33 of the row's largest if that is more.  A key or value that is not finite reaches the results of
  * the queries that see it (not all of them, where its weight is zero) and no others; a query that holds a NaN or an infinity has the result NaN; rows behind a
- * sequence's end are not looked at. */
+ * sequence's end are not looked at.
+ * Workspace, which the device's pool keeps: sequences with more than 32 rows (new tokens x n_heads / n_kv) have their visible keys and values of heads up to 128
+ * laid out as 16-bit numbers, 64 columns and 128 tokens at a time, within 256 MB or one sequence and key head at a time, and up to 256 MB for sums of slices of
+ * their keys; the others 10 MB. */
 CC_API int cc_paged_attention(cc_device* dev, const cc_page_plan* plan, const cc_paged_cache* cache, const cc_view* q, int32_t n_heads, float scale, int32_t window,
                               float softcap, const cc_view* sink, cc_buf** out);
 
