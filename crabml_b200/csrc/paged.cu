@@ -127,6 +127,7 @@ int pg_check_cache(cc_device* dev, const cc_page_plan* plan, const cc_paged_cach
 #define PA_THREADS 256
 #define PA_WARPS (PA_THREADS / 32)
 #define PA_ROWS 4                            // rows of angles that a CTA makes for itself at a time
+#define PA_SMEM ((int)(PA_ROWS * 128 * sizeof(double2)) + 128 * 256 * 2)      // .. of 128 pairs, and a block of 128 rows of 256
 struct PaArgs {
     const PgSegment* segments;
     const float *q, *k, *v, *freq;
@@ -394,7 +395,8 @@ extern "C" CC_API int cc_paged_append(cc_device* dev, const cc_page_plan* plan, 
             dev->launches++;
         }
         auto kernel = c.i8 ? (table ? paged_append_kernel<true, true> : paged_append_kernel<true, false>) : (table ? paged_append_kernel<false, true> : paged_append_kernel<false, false>);
-        if (e == cudaSuccess && smem > 40 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        // the most that any call needs, always: the attribute is the kernel's, not this call's, and another thread's device may be between here and its launch
+        if (e == cudaSuccess && smem > 40 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PA_SMEM);
         if (e == cudaSuccess) e = cc_launch_pdl(dev, kernel, grid, PA_THREADS, smem, a, plan->n_items);
         dev->launches++;
         if (ws) cc_pool_free(dev, ws, cls);

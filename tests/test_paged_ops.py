@@ -558,6 +558,37 @@ def test_a_plan_outlives_nothing(dev):
         np.testing.assert_array_equal(take(dev, y), want)
 
 
+def test_two_devices_at_once():
+    """two threads, a device each, append to blocks of different sizes: one's launches do not depend on what the other asks of the same kernel in between"""
+    import threading
+    failed, devs, work = [], [make_device(), make_device()], []
+    for dev, d in zip(devs, (256, 192)):  # noqa: F402
+        P, G = 128, 1
+        cache = paged.PagedCache.alloc(dev, 2, G, P, d, dtype=capi.I8, n_slots=1)
+        src = give(dev, np.random.default_rng(d).normal(size=(1, 2 * d)).astype(np.float32))
+        plan = paged.PagePlan(dev, P, 2, [[0]], [5], [1], 1)
+        paged.append(plan, cache, None, 0, src, 0, src, d)
+        work.append((plan, cache, src, d))
+
+    def go(plan, cache, src, d):
+        try:
+            for _ in range(20000):
+                paged.append(plan, cache, None, 0, src, 0, src, d)
+        except Exception as e:                               # noqa: BLE001
+            failed.append(e)
+    threads = [threading.Thread(target=go, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for dev in devs:
+        dev.synchronize()
+    del work
+    for dev in devs:
+        dev.close()
+    assert not failed, failed
+
+
 # ---- refusals -------------------------------------------------------------------------------------------------------------------------------
 def test_refusals(dev):
     G, H, d, P = 2, 4, 32, 16
