@@ -8,6 +8,7 @@
 from __future__ import annotations
 
 import ctypes as C
+import operator
 
 import numpy as np
 
@@ -22,6 +23,17 @@ def _whole(what, a, kind):
     if a.size and (a.dtype.kind not in "iu" or int(a.min()) < np.iinfo(kind).min or int(a.max()) > np.iinfo(kind).max):
         raise TensorError(f"page_plan: {what} are not whole numbers of {np.dtype(kind).itemsize * 8} bits")
     return np.ascontiguousarray(a, kind)
+
+
+def _number(call, what, x, bits=32):
+    """a whole number that the C call's argument can hold, or a refusal"""
+    try:
+        n = int(x) if isinstance(x, float) and x.is_integer() else operator.index(x)
+    except TypeError:
+        raise TensorError(f"{call}: {what} is {x!r}, not a whole number") from None
+    if not -(1 << bits - 1) <= n < 1 << bits - 1:
+        raise TensorError(f"{call}: {what} is {n}, beyond {bits} bits")
+    return n
 
 
 class PagePlan:
@@ -43,7 +55,8 @@ class PagePlan:
         if len(pos0) != n or table.ndim != 2 or len(table) != n or (slots is not None and len(slots) != n):
             raise TensorError(f"page_plan: {n} counts, {len(pos0)} positions, table {table.shape}" + ("" if slots is None else f", {len(slots)} slots"))
         table, slots = _whole("page numbers", table, np.int32), None if slots is None else _whole("slots", slots, np.int32).reshape(-1)
-        d = capi.cc_page_plan_desc(n, int(page_size), table.shape[1], int(n_pages), int(n_slots), *(None if a is None else a.ctypes.data for a in (pos0, counts, table, slots)))
+        d = capi.cc_page_plan_desc(n, _number("page_plan", "page_size", page_size), table.shape[1], _number("page_plan", "n_pages", n_pages, 64),
+                                   _number("page_plan", "n_slots", n_slots, 64), *(None if a is None else a.ctypes.data for a in (pos0, counts, table, slots)))
         h = C.c_void_p()
         device.check(device.lib.cc_page_plan_create(device.handle, C.byref(d), C.byref(h)))
         self.handle = h
@@ -87,14 +100,16 @@ def _v(t):
 
 def append(plan, cache, q_src, q_col0, k_src, k_col0, v_src, v_col0, n_heads=0, freq=None, pairing=capi.ROPE_NEIGHBOURS, offset=0, mag=1.0):
     """keys and values of the plan's tokens, turned by their positions, into the pages -> the turned queries [T, n_heads * dk] (q_src None: None)"""
-    dev, h = plan.device, C.c_void_p()
-    dev.check(dev.lib.cc_paged_append(dev.handle, plan.handle, C.byref(cache._c), _v(q_src), int(q_col0), _v(k_src), int(k_col0), _v(v_src), int(v_col0), int(n_heads), _v(freq),
-                                      int(pairing), int(offset), float(mag), C.byref(h)))
+    dev, h, what = plan.device, C.c_void_p(), "paged_append"
+    n_heads = _number(what, "n_heads", n_heads)
+    dev.check(dev.lib.cc_paged_append(dev.handle, plan.handle, C.byref(cache._c), _v(q_src), _number(what, "q_col0", q_col0), _v(k_src), _number(what, "k_col0", k_col0), _v(v_src),
+                                      _number(what, "v_col0", v_col0), n_heads, _v(freq), _number(what, "pairing", pairing), _number(what, "offset", offset), float(mag), C.byref(h)))
     return None if q_src is None else CudaTensor(_Buf(dev, h), TensorStrider([plan.tokens, n_heads * cache.k.shape()[3]]), dev)
 
 
 def attention(plan, cache, q, n_heads, scale, window=0, softcap=0.0, sink=None):
     """-> [T, n_heads * dv]"""
-    dev, h = plan.device, C.c_void_p()
-    dev.check(dev.lib.cc_paged_attention(dev.handle, plan.handle, C.byref(cache._c), _v(q), int(n_heads), float(scale), int(window), float(softcap), _v(sink), C.byref(h)))
+    dev, h, what = plan.device, C.c_void_p(), "paged_attention"
+    n_heads = _number(what, "n_heads", n_heads)
+    dev.check(dev.lib.cc_paged_attention(dev.handle, plan.handle, C.byref(cache._c), _v(q), n_heads, float(scale), _number(what, "window", window), float(softcap), _v(sink), C.byref(h)))
     return CudaTensor(_Buf(dev, h), TensorStrider([plan.tokens, n_heads * cache.v.shape()[3]]), dev)

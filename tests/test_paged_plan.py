@@ -161,3 +161,33 @@ def test_where_a_sequence_may_go_back(build, seed):
         if (at + n) % P:                                     # attention reads the open block
             assert half[(at + n) // P % 2][:(at + n) % P] == have[(at + n) // P * P:], (call, at, n)
     assert borders > 5
+
+
+def test_arguments_that_are_not_whole_or_too_large():
+    """a window of 2^32 + 5 would arrive as one of 5: refused before the call, like all that its argument cannot hold"""
+    from types import SimpleNamespace
+
+    from crabml_b200 import TensorError, capi, paged
+    called = []
+    lib = SimpleNamespace(cc_paged_append=lambda *a: called.append(a), cc_paged_attention=lambda *a: called.append(a), cc_page_plan_create=lambda *a: called.append(a))
+    dev = SimpleNamespace(lib=lib, handle=None, check=lambda rc: None)
+    plan = SimpleNamespace(device=dev, handle=None, tokens=1)
+    t = SimpleNamespace(_view=capi.cc_view, shape=lambda: [1, 1, 16, 16])
+    cache = paged.PagedCache(t, t)
+    wrong = (1 << 32, (1 << 32) + 5, 1 << 31, -(1 << 31) - 1, 1.5, "1", None)
+    for x in wrong:
+        for kw in (dict(window=x), dict(n_heads=x)):
+            with pytest.raises(TensorError):
+                paged.attention(plan, cache, t, **{**dict(n_heads=1, scale=1.0), **kw})
+        for kw in ("q_col0", "k_col0", "v_col0", "n_heads", "pairing", "offset"):
+            with pytest.raises(TensorError):
+                paged.append(plan, cache, **{**dict(q_src=t, q_col0=0, k_src=t, k_col0=0, v_src=t, v_col0=0, n_heads=1), kw: x})
+        with pytest.raises(TensorError):
+            paged.PagePlan(dev, x, 4, [[0]], [0], [1])
+    for x in (1 << 63, 1.5):
+        for kw in (dict(n_pages=x), dict(n_slots=x)):
+            with pytest.raises(TensorError):
+                paged.PagePlan(dev, **{**dict(page_size=16, n_pages=4, table=[[0]], pos0=[0], counts=[1]), **kw})
+    assert not called
+    paged.attention(plan, cache, t, 1, 1.0, window=5.0)
+    assert called.pop()[6] == 5
