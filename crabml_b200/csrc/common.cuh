@@ -47,7 +47,7 @@
 #define CC_MAX_PLANES 4
 #define CC_N_SLOTS 16
 #define CC_HISTORY_CAP 65536
-#define CC_PLAN_BUFFERS 4
+#define CC_PLAN_BUFFERS 64
 
 struct cc_device;
 
@@ -99,6 +99,12 @@ struct CcRopeTable {
     ~CcRopeTable();
     const void* rows(int64_t from) const { return (const uint8_t*)base + (size_t)(from - pos) * pairs * 8; }
 };
+struct CcPlanBuffer {
+    void* pinned = nullptr;
+    size_t bytes = 0;
+    cudaEvent_t through = nullptr;        // its last copy
+};
+
 struct cc_device {
     int ordinal = 0;
     cc_comm* comm = nullptr;
@@ -155,10 +161,9 @@ struct cc_device {
 
     // plans of steps over several sequences on their way to the device (paged.cu)
     std::mutex plan_mu;
-    void* plan_pinned[CC_PLAN_BUFFERS] = {};
-    size_t plan_bytes[CC_PLAN_BUFFERS] = {};
-    cudaEvent_t plan_ev[CC_PLAN_BUFFERS] = {};
-    unsigned plan_turn = 0;
+    std::vector<CcPlanBuffer> plans;
+    size_t plan_turn = 0;                 // the buffer whose copy is the oldest
+    std::vector<void*> plan_small;        // buffers that a larger plan needed more than
 
     // debug tap
     std::map<std::string, std::vector<float>> debug_tensors;

@@ -123,7 +123,8 @@ extern "C" CC_API void cc_device_destroy(cc_device* dev) {
     if (dev->export_host) cudaFreeHost(dev->export_host);
     for (int i = 0; i < 2; i++) { if (dev->up_pinned[i]) cudaFreeHost(dev->up_pinned[i]); if (dev->up_ev[i]) cudaEventDestroy(dev->up_ev[i]); }
     for (int i = 0; i < 2; i++) { if (dev->rope_pinned[i]) cudaFreeHost(dev->rope_pinned[i]); if (dev->rope_ev[i]) cudaEventDestroy(dev->rope_ev[i]); }
-    for (int i = 0; i < CC_PLAN_BUFFERS; i++) { if (dev->plan_pinned[i]) cudaFreeHost(dev->plan_pinned[i]); if (dev->plan_ev[i]) cudaEventDestroy(dev->plan_ev[i]); }
+    for (void* p : dev->plan_small) cudaFreeHost(p);
+    for (auto& b : dev->plans) { if (b.pinned) cudaFreeHost(b.pinned); if (b.through) cudaEventDestroy(b.through); }
     if (dev->err_host) cudaFreeHost(dev->err_host);
     if (dev->err_dev) cudaFree(dev->err_dev);
     if (dev->slots) cudaFree(dev->slots);

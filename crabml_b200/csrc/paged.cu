@@ -16,22 +16,28 @@
 #include "paged.cuh"
 
 // ---- the plan ---------------------------------------------------------------------------------------------------------------------------
-// pinned staging of plans on their way to the device, by turns; the oldest copy has to be through before its buffer is used again
+// Pinned staging of plans on their way to the device, by turns: a host that works ahead of the device takes another buffer, up to CC_PLAN_BUFFERS, and then waits for the oldest copy
 static int pg_upload(cc_device* dev, void* dst, const std::vector<uint8_t>& bytes) {
     std::lock_guard<std::mutex> g(dev->plan_mu);
-    const int i = dev->plan_turn++ % CC_PLAN_BUFFERS;
-    if (!dev->plan_ev[i]) CC_CUDA(dev, cudaEventCreateWithFlags(&dev->plan_ev[i], cudaEventDisableTiming));
-    CC_CUDA(dev, cudaEventSynchronize(dev->plan_ev[i]));
-    if (dev->plan_bytes[i] < bytes.size()) {
-        if (dev->plan_pinned[i]) { CC_CUDA(dev, cudaFreeHost(dev->plan_pinned[i])); dev->plan_pinned[i] = nullptr; dev->plan_bytes[i] = 0; }
+    if (dev->plans.empty() || (dev->plans.size() < CC_PLAN_BUFFERS && cudaEventQuery(dev->plans[dev->plan_turn].through) == cudaErrorNotReady)) {
+        dev->plans.insert(dev->plans.begin() + dev->plan_turn, CcPlanBuffer());
+        cudaGetLastError();                                 // (the query's answer is no error of a later call)
+    }
+    CcPlanBuffer& b = dev->plans[dev->plan_turn];
+    if (!b.through) CC_CUDA(dev, cudaEventCreateWithFlags(&b.through, cudaEventDisableTiming));
+    CC_CUDA(dev, cudaEventSynchronize(b.through));
+    if (b.bytes < bytes.size()) {
+        if (b.pinned) dev->plan_small.push_back(b.pinned);  // (to free it would wait for the device)
+        b.pinned = nullptr; b.bytes = 0;
         size_t n = 64 << 10;
         while (n < bytes.size()) n *= 2;
-        CC_CUDA(dev, cudaMallocHost(&dev->plan_pinned[i], n));
-        dev->plan_bytes[i] = n;
+        CC_CUDA(dev, cudaMallocHost(&b.pinned, n));
+        b.bytes = n;
     }
-    memcpy(dev->plan_pinned[i], bytes.data(), bytes.size());
-    CC_CUDA(dev, cudaMemcpyAsync(dst, dev->plan_pinned[i], bytes.size(), cudaMemcpyHostToDevice, dev->stream));
-    CC_CUDA(dev, cudaEventRecord(dev->plan_ev[i], dev->stream));
+    memcpy(b.pinned, bytes.data(), bytes.size());
+    CC_CUDA(dev, cudaMemcpyAsync(dst, b.pinned, bytes.size(), cudaMemcpyHostToDevice, dev->stream));
+    CC_CUDA(dev, cudaEventRecord(b.through, dev->stream));
+    dev->plan_turn = (dev->plan_turn + 1) % dev->plans.size();
     return CC_OK;
 }
 

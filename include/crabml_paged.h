@@ -30,7 +30,8 @@ typedef struct cc_page_plan_desc {
 } cc_page_plan_desc;
 /* The tokens of a call are rows of matrices, sequence after sequence.  Refused (CC_ERR_TENSOR): numbers out of range; a page that takes new tokens of one
  * sequence and belongs to another one too, or to the same one twice; a slot of two sequences.  Pages that no new token goes to may be shared (a common prefix).
- * The arrays are read during the call.  The plan stays usable until it is released; work queued before that finishes with it. */
+ * The arrays are read during the call, which waits for the device only where the copies of 64 plans are still queued.  The plan stays usable until it is released;
+ * work queued before that finishes with it. */
 CC_API int cc_page_plan_create(cc_device* dev, const cc_page_plan_desc* desc, cc_page_plan** out);
 CC_API void cc_page_plan_release(cc_page_plan* plan);
 CC_API int64_t cc_page_plan_tokens(const cc_page_plan* plan);

@@ -558,6 +558,25 @@ def test_a_plan_outlives_nothing(dev):
         np.testing.assert_array_equal(take(dev, y), want)
 
 
+def test_plans_do_not_wait_for_the_device(dev):
+    """a host that makes plans, larger ones too, for many steps ahead while the device is busy; what they say arrives all the same"""
+    G, d, P, n = 1, 32, 16, 24
+    c = Case(dev, P, G, d, d, True, [200, 40], [1, 1], seed=15)
+    q = give(dev, c.rng.normal(size=(2, 2 * d)).astype(np.float32))
+    want = [take(dev, paged.attention(c.plan([100 + i, 40 - i], [1, 1]), c.cache, q, 2, 0.1)) for i in range(n)]
+    large = [paged.PagePlan(dev, P, 1 << 20, [list(range(30000))], [16 * 30000 - 1], [1], 1) for _ in range(2)]
+    dev.synchronize()
+    stream = torch.cuda.ExternalStream(dev.stream())
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(2_000_000_000)                     # about a second
+    busy = stream.record_event()
+    plans = [c.plan([100 + i, 40 - i], [1, 1]) for i in range(n)] + [paged.PagePlan(dev, P, 1 << 20, [list(range(30000))], [16 * 30000 - 1], [1], 1)]
+    assert not busy.query()
+    for i, plan in enumerate(plans[:n]):
+        np.testing.assert_array_equal(take(dev, paged.attention(plan, c.cache, q, 2, 0.1)), want[i])
+    del large, plans
+
+
 def test_two_devices_at_once():
     """two threads, a device each, append to blocks of different sizes: one's launches do not depend on what the other asks of the same kernel in between"""
     import threading
