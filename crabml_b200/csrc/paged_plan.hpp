@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/crabml_paged.h"
@@ -49,9 +50,8 @@ inline std::string pg_build(const cc_page_plan_desc& d, PgParts& out) {
     PG_NEED(d.n_pages >= 0 && d.n_pages < ((int64_t)1 << 31) && d.n_slots >= 0 && d.n_slots < ((int64_t)1 << 30), "%lld pages, %lld slots", (ll)d.n_pages, (ll)d.n_slots);
     auto blocks = [&](int64_t tokens) { return (tokens + P - 1) / P; };
     auto page_of = [&](int i, int64_t b) { return d.table[(int64_t)i * d.table_cols + b]; };
-    std::vector<int> owner((size_t)d.n_pages, 0);        // pages that take new tokens: 1 + their sequence
-    std::vector<char> taken((size_t)d.n_slots, 0);
     std::vector<PgSegment> heads, rest;
+    std::vector<int64_t> taken;                          // slots
     for (int i = 0; i < d.n_seqs; i++) {
         const int64_t pos0 = d.pos0[i], n = d.counts[i], slot = d.slots ? d.slots[i] : i, most = ((int64_t)1 << 31) - 256;
         PG_NEED(pos0 >= 0 && n >= 0 && pos0 < most && pos0 + n < most, "sequence %d has %lld tokens and %lld new ones", i, (ll)pos0, (ll)n);
@@ -61,8 +61,7 @@ inline std::string pg_build(const cc_page_plan_desc& d, PgParts& out) {
         for (int64_t b = 0; b < blocks(end); b++) PG_NEED(page_of(i, b) >= 0 && page_of(i, b) < d.n_pages, "page %d of sequence %d is not one of %lld", page_of(i, b), i, (ll)d.n_pages);
         if (d.n_slots > 0) {
             PG_NEED(slot >= 0 && slot < d.n_slots, "slot %lld of sequence %d is not one of %lld", (ll)slot, i, (ll)d.n_slots);
-            PG_NEED(!taken[(size_t)slot], "two sequences with slot %lld", (ll)slot);
-            taken[(size_t)slot] = 1;
+            taken.push_back(slot);
         }
         PgSeq s;
         s.first = (int)out.tokens; s.count = (int)n; s.pos0 = (int)pos0; s.slot = d.n_slots > 0 ? (int)slot : 0;
@@ -76,8 +75,6 @@ inline std::string pg_build(const cc_page_plan_desc& d, PgParts& out) {
             g.half = 2 * s.slot + (int)(b & 1);
             g.flags = (hi == (b + 1) * P ? PG_FULL : 0) | (b >= end / P - 1 ? PG_KEPT : 0);
             g.next = -1;
-            PG_NEED(owner[(size_t)g.page] == 0, "page %d takes tokens of two blocks", g.page);
-            owner[(size_t)g.page] = 1 + i;
             if (b == pos0 / P) first = heads.size();
             const PgSegment* f = b == pos0 / P ? nullptr : &heads[first];
             // a block that is kept overwrites the open rows that the sequence's first block began with, where both lie in one half: the same CTA takes it behind that one (there is
@@ -89,11 +86,30 @@ inline std::string pg_build(const cc_page_plan_desc& d, PgParts& out) {
         }
         out.tokens += n;
     }
+    std::sort(taken.begin(), taken.end());
+    const auto twice = std::adjacent_find(taken.begin(), taken.end());
+    PG_NEED(twice == taken.end(), "two sequences with slot %lld", (ll)*twice);
+    // pages that take new tokens, with 1 + their sequence: as many places as it needs, not as the pool has (64 sequences of 4000 tokens took 258 us of a pool of a million pages)
+    int bits = 10;
+    while (((size_t)1 << bits) < 8 * (heads.size() + rest.size())) bits++;
+    const size_t places = (size_t)1 << bits;
+    std::vector<std::pair<int, int>> owners(places, {0, 0});
+    auto owner = [&](int page) -> std::pair<int, int>& {
+        size_t at = (uint32_t)page * 2654435769u >> (32 - bits);
+        while (owners[at].second && owners[at].first != page) at = (at + 1) & (places - 1);
+        return owners[at];
+    };
+    for (auto* v : {&heads, &rest})
+        for (auto& g : *v) {
+            auto& o = owner(g.page);
+            PG_NEED(!o.second, "page %d takes tokens of two blocks", g.page);
+            o = {g.page, 1 + g.seq};
+        }
     // no page that takes new tokens may be read by another sequence, nor stand twice in its own row
     for (int i = 0; i < d.n_seqs; i++) {
         const int64_t end = d.pos0[i] + d.counts[i], first_new = d.counts[i] > 0 ? d.pos0[i] / P : blocks(end);
         for (int64_t b = 0; b < blocks(end); b++) {
-            const int own = owner[(size_t)page_of(i, b)];
+            const int own = owner(page_of(i, b)).second;
             PG_NEED(own == 0 || (own == 1 + i && b >= first_new), "page %d takes new tokens and is block %lld of sequence %d too", page_of(i, b), (ll)b, i);
         }
     }

@@ -191,3 +191,32 @@ def test_arguments_that_are_not_whole_or_too_large():
     assert not called
     paged.attention(plan, cache, t, 1, 1.0, window=5.0)
     assert called.pop()[6] == 5
+
+
+def test_a_pool_of_any_size(build, monkeypatch):
+    """a plan takes memory for its step, not for the pages and slots that there are"""
+    import resource
+    plain, most = subprocess.run, 256 << 20
+    monkeypatch.setattr(subprocess, "run", lambda *a, **kw: plain(*a, preexec_fn=lambda: resource.setrlimit(resource.RLIMIT_AS, (most, most)), **kw))
+    head, segs = build(16, (1 << 31) - 1, [[(1 << 31) - 2, 7], [(1 << 30) + 3]], [17, 0], [1, 16], (1 << 30) - 1, [(1 << 30) - 2, 5])
+    assert head == [2, 17, 2] and sorted(g["page"] for g in segs) == [7, (1 << 30) + 3]
+    for table, text in (([[1 << 30, 7], [7]], "page 7 takes"), ([[9, 1 << 30], [1 << 30]], f"page {1 << 30} takes")):
+        assert text in build(16, (1 << 31) - 1, table, [17, 0], [1, 16], (1 << 30) - 1, [(1 << 30) - 2, 5])[0]
+    assert "two sequences with slot 5" in build(16, (1 << 31) - 1, [[8], [9]], [0, 0], [1, 1], (1 << 30) - 1, [5, 5])[0]
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_pages_that_two_take(build, seed):
+    """a page that takes new tokens stands nowhere else: against a count of every page's places"""
+    r = random.Random(1000 + seed)
+    P, n = 16, r.randint(1, 6)
+    pos0, counts = [r.randint(0, 60) for _ in range(n)], [r.choice([0, 1, r.randint(1, 50)]) for _ in range(n)]
+    table = [[r.randrange(r.choice([60, 4000])) * r.choice([1, 1024]) % 4096 for _ in range((p + c + P - 1) // P)] for p, c in zip(pos0, counts)]
+    places, new = {}, []
+    for i, row in enumerate(table):
+        for b, page in enumerate(row):
+            places[page] = places.get(page, 0) + 1
+            if counts[i] and b >= pos0[i] // P:
+                new.append(page)
+    head, _ = build(P, 4096, table, pos0, counts)
+    assert isinstance(head, str) == any(places[p] > 1 for p in new), (table, pos0, counts)
