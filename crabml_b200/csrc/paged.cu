@@ -349,6 +349,7 @@ extern "C" CC_API int cc_paged_append(cc_device* dev, const cc_page_plan* plan, 
     PgCache c;
     int rc = pg_check_cache(dev, plan, cache, "paged_append", &c);
     if (rc) return rc;
+    CC_REQUIRE(dev, c.k != c.v && (!c.i8 || (c.ks != c.vs && c.ko != c.vo)), "paged_append: keys and values go to one tensor");      // different CTAs write them
     PG_ROWS(dev, k_src, "paged_append keys"); PG_ROWS(dev, v_src, "paged_append values");
     if (q_src) PG_ROWS(dev, q_src, "paged_append queries");
     const int64_t T = plan->tokens;

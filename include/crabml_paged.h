@@ -55,7 +55,7 @@ typedef struct cc_paged_cache {
 /* For the plan's T tokens: queries in the columns q_col0 .. q_col0 + n_heads * dk of q_src's rows, keys (n_kv * dk) and values (n_kv * dv) likewise; the three may
  * be one matrix.  freq ([P] F32 or NULL): P column pairs of every query and key head, from column `offset` on, turn by position * freq[i] (a 64-bit product), as
  *   (x, y) <- (mag (x cos - y sin), mag (y cos + x sin)); pairing as in cc_qk_prepare_append.  The turn is computed in 64 bits and rounded to F32 once.
- * The keys and values go to their pages; out: F32 [T, n_heads * dk], the queries.  q_src NULL: keys and values alone (n_heads is ignored, *out is NULL). */
+ * The keys and values go to their pages, which are tensors of their own (one tensor for both, or for their factors or open blocks, is refused); out: F32 [T, n_heads * dk], the queries.  q_src NULL: keys and values alone (n_heads is ignored, *out is NULL). */
 CC_API int cc_paged_append(cc_device* dev, const cc_page_plan* plan, const cc_paged_cache* cache, const cc_view* q_src, int32_t q_col0, const cc_view* k_src,
                            int32_t k_col0, const cc_view* v_src, int32_t v_col0, int32_t n_heads, const cc_view* freq, int32_t pairing, int32_t offset, float mag,
                            cc_buf** out);

@@ -665,6 +665,25 @@ def test_refusals(dev):
     append(), attend()
 
 
+@pytest.mark.parametrize("i8", [False, True], ids=["f16", "i8"])
+def test_one_tensor_for_keys_and_values(dev, i8):
+    """nothing says which of the two would be there in the end: the append refuses it; attention only reads, and may"""
+    G, d, P = 2, 32, 16
+    c = Case(dev, P, G, d, d, i8, [20], [2], seed=1)
+    t = give(dev, np.zeros((2, 2 * G * d), np.float32))
+    a = {n: getattr(c.cache, n) for n in c.ref.a}
+    for one, other in (("k", "v"), ("k_scale", "v_scale"), ("k_open", "v_open")):
+        if one in a:
+            with pytest.raises(TensorError):
+                paged.append(c.plan(), paged.PagedCache(**dict(a, **{other: a[one]})), None, 0, t, 0, t, G * d)
+    both = dict(a, **{n.replace("k", "v", 1): a[n] for n in a if n[0] == "k"})
+    q = give(dev, c.rng.normal(size=(2, G * d)).astype(np.float32))
+    got = take(dev, paged.attention(c.plan(), paged.PagedCache(**both), q, G, 0.1))
+    twice = {n: give(dev, c.ref.a[n if n[0] == "k" else n.replace("v", "k", 1)]) for n in a}
+    np.testing.assert_array_equal(got, take(dev, paged.attention(c.plan(), paged.PagedCache(**twice), q, G, 0.1)))
+    paged.append(c.plan(), c.cache, None, 0, t, 0, t, G * d)
+
+
 def test_arrays_of_a_tensor(dev):
     """what other libraries see of a tensor is its memory"""
     a = np.arange(24, dtype=np.float32).reshape(4, 6)
