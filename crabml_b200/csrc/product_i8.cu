@@ -580,7 +580,7 @@ static int i8_product(cc_device* dev, const int8_t* w, const float* ws, const fl
     if (e != cudaSuccess) rc = cc_fail(dev, CC_ERR_CUDA, "product_i8: %s", cudaGetErrorString(e));
     // Whole waves of tiles of 256 x 256 for pairs of SMs: those (2048 tokens, 14336 x 4096: 102 us instead of 115 with one SM a tile; 512 tokens, 11008 x 4096: 40 and 43).  Else tiles of 128
     // channels, whose depth a cluster shares where they are few (512 tokens, 4096 x 14336: 47 us, by pairs 59), as wide as the tokens: 16 columns cost a step what its weights cost
-    else if (T > 128 && (int64_t)((m + 255) / 256) * ((T + 255) / 256) >= dev->sm_count / 2) rc = gp_launch(dev, w, ws, xq, xs, out, T, m, kp);
+    else if (T > 128 && dev->sm_count > 1 && (int64_t)((m + 255) / 256) * ((T + 255) / 256) >= dev->sm_count / 2) rc = gp_launch(dev, w, ws, xq, xs, out, T, m, kp);
     else rc = T <= 16 ? gi_launch<16>(dev, w, ws, xq, xs, out, T, m, kp) : T <= 32 ? gi_launch<32>(dev, w, ws, xq, xs, out, T, m, kp)
               : T <= 64 ? gi_launch<64>(dev, w, ws, xq, xs, out, T, m, kp) : T <= 128 ? gi_launch<128>(dev, w, ws, xq, xs, out, T, m, kp) : gi_launch<256>(dev, w, ws, xq, xs, out, T, m, kp);
     cc_pool_free(dev, mem, cls);

@@ -177,3 +177,15 @@ def test_a_layer_step_by_step(dev, i8):
         np.testing.assert_allclose(out, R.product(wo, wos, yy)[0], rtol=5 * 2.0 ** -24)
     for n, a in ref.a.items():
         np.testing.assert_array_equal(take(dev, getattr(cache, n)), a, err_msg=n)
+
+
+@pytest.mark.parametrize("limit", [1, 2, 3, 5])
+def test_few_sms(limit):
+    """a device that is held to one SM has no pairs of them: the same products all the same"""
+    d = make_device()
+    d.set_sm_limit(limit)
+    r = np.random.default_rng(limit)
+    for T, m, k in ((1, 300, 640), (20, 300, 640), (129, 300, 640), (300, 700, 416)):
+        w, ws = weights(r, m, k)
+        check(d, w, ws, r.normal(size=(T, k)).astype(np.float32))
+    d.close()
