@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import operator
+import struct
 
 import numpy as np
 
@@ -34,6 +35,9 @@ def _number(call, what, x, bits=32):
     if not -(1 << bits - 1) <= n < 1 << bits - 1:
         raise TensorError(f"{call}: {what} is {n}, beyond {bits} bits")
     return n
+
+
+_TWO, _SIX = struct.Struct("=2i").pack, struct.Struct("=6i").pack      # one look at all of a call's numbers: it is made for every layer of a token
 
 
 class PagePlan:
@@ -100,16 +104,23 @@ def _v(t):
 
 def append(plan, cache, q_src, q_col0, k_src, k_col0, v_src, v_col0, n_heads=0, freq=None, pairing=capi.ROPE_NEIGHBOURS, offset=0, mag=1.0):
     """keys and values of the plan's tokens, turned by their positions, into the pages -> the turned queries [T, n_heads * dk] (q_src None: None)"""
-    dev, h, what = plan.device, C.c_void_p(), "paged_append"
-    n_heads = _number(what, "n_heads", n_heads)
-    dev.check(dev.lib.cc_paged_append(dev.handle, plan.handle, C.byref(cache._c), _v(q_src), _number(what, "q_col0", q_col0), _v(k_src), _number(what, "k_col0", k_col0), _v(v_src),
-                                      _number(what, "v_col0", v_col0), n_heads, _v(freq), _number(what, "pairing", pairing), _number(what, "offset", offset), float(mag), C.byref(h)))
+    dev, h = plan.device, C.c_void_p()
+    try:
+        _SIX(q_col0, k_col0, v_col0, n_heads, pairing, offset)
+    except struct.error:
+        q_col0, k_col0, v_col0, n_heads, pairing, offset = (_number("paged_append", what, x) for what, x in (
+            ("q_col0", q_col0), ("k_col0", k_col0), ("v_col0", v_col0), ("n_heads", n_heads), ("pairing", pairing), ("offset", offset)))
+    dev.check(dev.lib.cc_paged_append(dev.handle, plan.handle, C.byref(cache._c), _v(q_src), q_col0, _v(k_src), k_col0, _v(v_src), v_col0, n_heads, _v(freq), pairing, offset,
+                                      float(mag), C.byref(h)))
     return None if q_src is None else CudaTensor(_Buf(dev, h), TensorStrider([plan.tokens, n_heads * cache.k.shape()[3]]), dev)
 
 
 def attention(plan, cache, q, n_heads, scale, window=0, softcap=0.0, sink=None):
     """-> [T, n_heads * dv]"""
-    dev, h, what = plan.device, C.c_void_p(), "paged_attention"
-    n_heads = _number(what, "n_heads", n_heads)
-    dev.check(dev.lib.cc_paged_attention(dev.handle, plan.handle, C.byref(cache._c), _v(q), n_heads, float(scale), _number(what, "window", window), float(softcap), _v(sink), C.byref(h)))
+    dev, h = plan.device, C.c_void_p()
+    try:
+        _TWO(n_heads, window)
+    except struct.error:
+        n_heads, window = _number("paged_attention", "n_heads", n_heads), _number("paged_attention", "window", window)
+    dev.check(dev.lib.cc_paged_attention(dev.handle, plan.handle, C.byref(cache._c), _v(q), n_heads, float(scale), window, float(softcap), _v(sink), C.byref(h)))
     return CudaTensor(_Buf(dev, h), TensorStrider([plan.tokens, n_heads * cache.v.shape()[3]]), dev)
