@@ -158,7 +158,6 @@ __host__ __device__ __forceinline__ int ti_key_tiles(const PgSeq& s, const PtArg
 template <bool I8>
 __global__ void __launch_bounds__(TU_THREADS) paged_unpack_kernel(const PtArgs a) {
     __shared__ int pages[TI_KEYS / 16];
-    __shared__ unsigned top[TI_KEYS];                          // of open rows: their largest value, as bits of f16
     __shared__ float up[TI_KEYS / 16];                         // powers of two that the open block's values are multiplied by, 16 keys each
     __shared__ TiInfo info;
     const int tid = threadIdx.x, kvh = a.head0 + blockIdx.y;
@@ -170,6 +169,28 @@ __global__ void __launch_bounds__(TU_THREADS) paged_unpack_kernel(const PtArgs a
     int from, to;
     pt_range(s, a, &from, &to);
     const int key0 = from + kt * TI_KEYS, opens = I8 ? to >> a.shift << a.shift : 0, open = 2 * s.slot + ((to >> a.shift) & 1);
+    // The open block's values are made as large as codes are, by a power of two that its 16 keys' first one sets (any query that sees one of them sees that, but for windows) as far as all
+    // of them stay in range: exactly, for it only multiplies.  Their factor is the inverse.  A warp 16 keys, two lanes a key
+    if (const int group = tid >> 5, key = key0 + (tid >> 1); I8 && key0 + group * 16 >= opens && key0 + group * 16 < to) {
+        unsigned m = 0;
+        if (key < to) {
+            const uint4* p = (const uint4*)(a.vo + (((size_t)open * a.G + kvh) * a.page + (key & (a.page - 1))) * a.dv) + (tid & 1);
+#pragma unroll 4
+            for (int i = 0; i < a.dv / 16; i++) {
+                const uint4 x = __ldg(p + 2 * i);
+                m = __vmaxu2(m, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu & ~pt_wild(x.x), x.y & 0x7fff7fffu & ~pt_wild(x.y)),
+                                         __vmaxu2(x.z & 0x7fff7fffu & ~pt_wild(x.z), x.w & 0x7fff7fffu & ~pt_wild(x.w))));
+            }
+            m = max(m & 0xffffu, m >> 16);
+        }
+        const unsigned most = __reduce_max_sync(0xffffffffu, m), mine = max(__shfl_sync(0xffffffffu, m, 0), __shfl_sync(0xffffffffu, m, 1)), first = mine ? mine : most;
+        auto log2_of = [](unsigned h) { return (__float_as_int(__half2float(__ushort_as_half((unsigned short)h))) >> 23) - 127; };
+        const int by = most ? max(0, min(TI_UP, min(6 - log2_of(first), 14 - log2_of(most)))) : 0;
+        if ((tid & 31) == 0) {
+            up[group] = pt_pow2((float)by); info.vf[group] = pt_pow2((float)-by);
+            info.lv[group] = most ? (float)max(log2_of(first) - 6, -by) : -INFINITY;
+        }
+    }
     if (tid < 32) {
         float kf = 1.0f, vf = 1.0f, lv = 0.0f;
         const int key = key0 + (tid & 7) * 16;
@@ -182,34 +203,13 @@ __global__ void __launch_bounds__(TU_THREADS) paged_unpack_kernel(const PtArgs a
         if (bad || key >= to) kf = vf = 0.0f;
         lv = pt_log2(vf);
         const unsigned nan = __ballot_sync(0xffffffffu, bad) >> 2 * (tid & 3);      // the lanes' groups repeat after 8
-        if (tid < TI_KEYS / 16) { pages[tid] = page; info.kf[tid] = kf; info.vf[tid] = vf; info.lv[tid] = lv; }
+        if (tid < TI_KEYS / 16) {
+            pages[tid] = page; info.kf[tid] = kf;
+            if (!I8 || key < opens || key >= to) { info.vf[tid] = vf; info.lv[tid] = lv; }
+        }
         if (tid < TI_KEYS / 32) info.bad[tid] = (nan & 1u ? 0xffffu : 0u) | (nan & 2u ? 0xffff0000u : 0u);
     }
     __syncthreads();
-    // The open block's values are made as large as codes are, by a power of two that its 16 keys' first one sets (any query that sees one of them sees that, but for windows) as far as all
-    // of them stay in range: exactly, for it only multiplies.  Its factor is the inverse
-    if (I8 && key0 + TI_KEYS > opens && opens < to) {
-        if (tid < TI_KEYS) top[tid] = 0u;
-        __syncthreads();
-        for (int e = tid; e < TI_KEYS * (a.dv / 8); e += TU_THREADS) {
-            const int r = e / (a.dv / 8), key = key0 + r;
-            if (key < opens || key >= to) continue;
-            const uint4 x = __ldg((const uint4*)(a.vo + (((size_t)open * a.G + kvh) * a.page + (key & (a.page - 1))) * a.dv) + (e - r * (a.dv / 8)));
-            const unsigned m = __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu & ~pt_wild(x.x), x.y & 0x7fff7fffu & ~pt_wild(x.y)), __vmaxu2(x.z & 0x7fff7fffu & ~pt_wild(x.z), x.w & 0x7fff7fffu & ~pt_wild(x.w)));
-            atomicMax(&top[r], max(m & 0xffffu, m >> 16));
-        }
-        __syncthreads();
-        if (tid < TI_KEYS / 16 && pages[tid] < 0 && key0 + tid * 16 < to) {
-            unsigned most = 0;
-            for (int i = 0; i < 16; i++) most = max(most, top[tid * 16 + i]);
-            const unsigned first = top[tid * 16] ? top[tid * 16] : most;
-            auto log2_of = [](unsigned h) { return (__float_as_int(__half2float(__ushort_as_half((unsigned short)h))) >> 23) - 127; };
-            const int by = most ? max(0, min(TI_UP, min(6 - log2_of(first), 14 - log2_of(most)))) : 0;
-            up[tid] = pt_pow2((float)by); info.vf[tid] = pt_pow2((float)-by);
-            info.lv[tid] = most ? (float)max(log2_of(first) - 6, -by) : -INFINITY;
-        }
-        __syncthreads();
-    }
     const size_t at = (size_t)blockIdx.x * a.heads + blockIdx.y;
     bool wild = false;
 #pragma unroll
