@@ -221,6 +221,23 @@ __device__ __forceinline__ unsigned pa_code4(uint2 u, float most, float r) {
 }
 #define PA_Q_ROWS 16
 #define PA_AHEAD 4                           // rows of a head, or heads of a row, that a warp reads before it turns the first
+// f(row r0, so many rows, their angles): all rows of a job, or portions whose angles the CTA makes first
+template <bool TABLE, class F>
+__device__ __forceinline__ void pa_portions(const PaArgs& a, const PgSegment& g, int row_from, int row_to, bool turned, double2* made, F f) {
+    if constexpr (!TABLE) {
+        if (turned && a.pairs > 0) {
+            for (int r0 = 0; r0 < g.rows; r0 += PA_ROWS) {
+                const int rows = min(PA_ROWS, g.rows - r0);
+                __syncthreads();
+                for (int e = threadIdx.x; e < rows * a.pairs; e += PA_THREADS) { const int r = e / a.pairs; made[e] = pa_angle(a, g.pos0 + r0 + r, e - r * a.pairs); }
+                __syncthreads();
+                f(r0, rows, made);
+            }
+            return;
+        }
+    }
+    f(row_from, row_to - row_from, a.angles + (int64_t)(g.token0 + row_from) * a.pairs);
+}
 // grid (segments, jobs): jobs 0 .. G - 1 key heads, then G value heads (of the first n_items segments, and those behind them in their chains), then query heads by hq (and their rows by PA_Q_ROWS).
 // A warp takes 32 units of a head, in rows so many further on as warps share them
 template <bool I8, bool TABLE>
@@ -237,17 +254,7 @@ __global__ void __launch_bounds__(PA_THREADS, 4) paged_append_kernel(const PaArg
         const PgSegment g = a.segments[at];
         at = is_q ? -1 : g.next;
         const int part = is_q ? (job - 2 * a.G) % a.q_parts : 0, row_from = part * PA_Q_ROWS, row_to = is_q && a.q_parts > 1 ? min(g.rows, row_from + PA_Q_ROWS) : g.rows;
-        // f(row r0, so many rows, their angles): all rows of the job, or portions whose angles the CTA makes first
-        auto portions = [&](bool turned, auto f) {
-            if (TABLE || !turned || a.pairs == 0) { f(row_from, row_to - row_from, a.angles + (int64_t)(g.token0 + row_from) * a.pairs); return; }
-            for (int r0 = TABLE ? g.rows : 0; r0 < g.rows; r0 += PA_ROWS) {
-                const int rows = min(PA_ROWS, g.rows - r0);
-                __syncthreads();
-                for (int e = tid; e < rows * a.pairs; e += PA_THREADS) { const int r = e / a.pairs; made[e] = pa_angle(a, g.pos0 + r0 + r, e - r * a.pairs); }
-                __syncthreads();
-                f(r0, rows, made);
-            }
-        };
+        auto portions = [&](bool turned, auto f) { pa_portions<TABLE>(a, g, row_from, row_to, turned, made, f); };
         // the CTA's warps over `kinds` kinds of work and rows: f(kind, first row, rows from one to the next)
         auto share = [&](int kinds, auto f) {
             const int at_once = min(kinds, PA_WARPS), by = PA_WARPS / at_once, first = w / at_once;
