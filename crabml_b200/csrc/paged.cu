@@ -391,7 +391,7 @@ extern "C" CC_API int cc_paged_append(cc_device* dev, const cc_page_plan* plan, 
         a.vec = pairing == CC_ROPE_NEIGHBOURS && ((offset | c.dk | k_col0 | (int)(a.krs & 1)) & 1) == 0 && (!q_src || ((q_col0 | (int)(a.qrs & 1)) & 1) == 0) &&
                 (((uintptr_t)k_src->buf->plane[0] | (q_src ? (uintptr_t)q_src->buf->plane[0] : 0)) & 7) == 0;
         // a portion of many rows a block: the angles once for all heads, in a kernel of their own (64 rows of 64 pairs made by each of 16 CTAs:
-        // three prompts of 1657 tokens, 32 heads on 8, 125 us, with the table 4 + 32); single tokens: by every CTA
+        // three prompts of 1957 tokens, 32 heads on 8, 125 us, with the table 4 + 32); single tokens: by every CTA
         const bool table = pairs > 0 && T > 4 * (int64_t)plan->n_segments;
         a.hq = table ? 4 : 8; a.q_parts = table ? plan->page / PA_Q_ROWS : 1;
         void* ws = nullptr; size_t cls = 0;

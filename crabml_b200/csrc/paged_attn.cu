@@ -7,7 +7,7 @@
 // products are one instruction whose accumulators a thread adds up itself.  A warp takes 16 keys at a time.  Its lanes keep, read and convert the pieces of the
 // cache that the instruction's layout gives them and no others: which four columns of a row a lane puts into a step is free as long as queries and keys agree, and so
 // is the order of the value columns, so a lane takes 16 neighbouring bytes of a row, and the way through shared memory (cp.async, a ring per warp) needs no barrier.
-// Keys and values are read once, so memory bounds it: 64 sequences of up to 4000 tokens (268 MB, 41 us) take 82 us, 16 sequences in 16-bit pages (311 MB, 47 us) 75.  While all CTAs
+// Keys and values are read once, so memory bounds it: 64 sequences of up to 4000 tokens (268 MB, 41 us) take 79 us, 16 sequences in 16-bit pages (311 MB, 47 us) 75.  While all CTAs
 // stream they read 5.6 to 6 TB/s; the rest is what a CTA does before and behind each segment (7 us to its first rows), and the kernel that adds up cut segments (5 us).
 #include <math.h>
 

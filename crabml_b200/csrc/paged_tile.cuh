@@ -12,7 +12,7 @@
 // TMEM holds S twice, O, Q_h and Q_l (512 columns), shared memory two stages of K and V (128 KB): while 8 warps make the weights of one step, the tensor core computes the
 // scores of the next and the sums of the one before.  With Q in shared memory a step's products read 192 KB there and took 3100 cycles instead of 2050.
 // A row's 128 scores lie with two threads, a half each, which exchange their largest score once a step.  Warps 0-7 weights and sums, 8 the copies, 9 the products, 10 what stands beside the images.
-// Portions of three prompts (3000 rows of 32 heads on 8, 8-bit pages): 12 us of images and 214 of tiles, 318 TFLOP/s of the four products' 68 GFLOP, of which the h and l of
+// Portions of three prompts (3000 rows of 32 heads on 8, 8-bit pages): 12 us of images and 208 of tiles, 326 TFLOP/s of the four products' 68 GFLOP, of which the h and l of
 // queries and weights make two.  A step takes 3900 cycles, its products 2050 of them, the weights' instructions 1500; the rest is the way of a step's scores through one group of warps
 // in turn (wait, read, largest, meet, weights, store).  Sums of four steps left to the tensor core, fewer reads of O, took 3 % more.
 // Every wait is bounded (sg_wait); where one ran out all roles run to their ends without waiting (the barrier of warps 0-7 included) and the host reports it.
@@ -27,8 +27,8 @@
 #define TI_SOFT (TI_ROWS * TI_SPLIT)
 #define TI_SOFT_WARPS (TI_SOFT / 32)
 #define TI_THREADS (TI_SOFT + 128)
-// 384 threads of 168 registers at launch are 256 of 216 and 128 of 72 afterwards.  No register of a step may spill: shared memory leaves next to no L1, and with 80 numbers
-// a thread spilled (four threads a row, 96 registers) a step took twice as long
+// 384 threads of 168 registers at launch are 256 of 216 and 128 of 72 afterwards.  A step's numbers must not spill: shared memory leaves next to no L1, and with 80 numbers
+// a thread spilled (four threads a row, 96 registers) a step took twice as long.  Two of them do
 #define TI_REGS 168
 #define TI_REGS_SOFT 216
 #define TI_REGS_REST 72
@@ -123,7 +123,8 @@ __device__ __forceinline__ ti_f2 ti_add2(ti_f2 a, ti_f2 b) {
     return r;
 }
 // 2^x of a pair by multiply-adds: the special function unit makes 4 results a cycle and scheduler, which alone would take half of a step.  x = n + r with |r| <= 1/2 by way
-// of a number whose last place is 1; 2^r by its series up to r^6 (the rest is below 2^-22 r^7 / 5040 (ln 2)^7 < 2^-24); n goes into the exponent.  x >= -126 here
+// of a number whose last place is 1; 2^r by its series up to r^6 (the first term left out is 2^-23 at |r| = 1/2; with the roundings the result is off by up to 2^-22 of itself, as the special function
+// unit's is); n goes into the exponent.  What is below -126, a hidden key's -inf and NaN count as -126
 __device__ __forceinline__ ti_f2 ti_exp2_pair(float2 x) {
     const ti_f2 big = ti_two(12582912.0f, 12582912.0f), minus = ti_two(-1.0f, -1.0f);
     const ti_f2 v = ti_two(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f)), t = ti_add2(v, big), n = ti_add2(t, ti_two(-12582912.0f, -12582912.0f)), r = ti_fma2(n, minus, v);

@@ -4,6 +4,8 @@
     for layer in layers:                                          # rows of qkv: the new tokens, sequence after sequence
         q = append(plan, layer.cache, qkv, 0, qkv, H * d, qkv, (H + G) * d, H, freq=freq)
         y = attention(plan, layer.cache, q, H, d ** -0.5)
+
+Results are queued on the device's stream: a library that is handed one (torch.as_tensor(y)) has to be ordered with it, see CudaTensor.__cuda_array_interface__.
 """
 from __future__ import annotations
 

@@ -200,7 +200,9 @@ class CudaTensor:
 
     @property
     def __cuda_array_interface__(self):
-        """the tensor's own memory for other libraries (torch.as_tensor and the like), ordered by the device's stream"""
+        """The tensor's own memory for other libraries (torch.as_tensor and the like).  The entry "stream" names the device's stream, on which the memory is written and read; it waits for no
+        other stream, and torch does not act on the entry.  So whoever uses the memory elsewhere orders the two: device.synchronize(), work under torch.cuda.stream(
+        torch.cuda.ExternalStream(device.stream())), or an event of that stream.  That holds for the last use too: once the tensor is gone, its memory is the next call's"""
         if not self.device.handle:
             raise CudaError("the tensor's device is closed")
         if self._array_of is self._strider:                            # asked for twice by those who look whether it is there

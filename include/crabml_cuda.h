@@ -111,7 +111,7 @@ CC_API void* cc_device_stream(cc_device* dev);
  * into the device layout of the kernels (same algorithmic bytes). */
 CC_API int cc_tensor_from_cpu(cc_device* dev, const void* bytes, size_t nbytes, const int64_t* shape,
                        int32_t ndim, int32_t ggml_type, cc_buf** out);
-/* alloc: F32 zero-filled, or F16 (cpu_tensor.rs:138-165); other dtypes -> CC_ERR_TENSOR */
+/* alloc: F32 zero-filled, or F16 (cpu_tensor.rs:138-165), I32 or I8, zeroed too; other dtypes -> CC_ERR_TENSOR */
 CC_API int cc_tensor_alloc(cc_device* dev, const int64_t* shape, int32_t ndim, int32_t ggml_type, cc_buf** out);
 CC_API void cc_tensor_retain(cc_buf* buf);
 CC_API void cc_tensor_release(cc_buf* buf);

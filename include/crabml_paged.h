@@ -55,7 +55,8 @@ typedef struct cc_paged_cache {
 /* For the plan's T tokens: queries in the columns q_col0 .. q_col0 + n_heads * dk of q_src's rows, keys (n_kv * dk) and values (n_kv * dv) likewise; the three may
  * be one matrix.  freq ([P] F32 or NULL): P column pairs of every query and key head, from column `offset` on, turn by position * freq[i] (a 64-bit product), as
  *   (x, y) <- (mag (x cos - y sin), mag (y cos + x sin)); pairing as in cc_qk_prepare_append.  The turn is computed in 64 bits and rounded to F32 once.
- * The keys and values go to their pages, which are tensors of their own (one tensor for both, or for their factors or open blocks, is refused); out: F32 [T, n_heads * dk], the queries.  q_src NULL: keys and values alone (n_heads is ignored, *out is NULL). */
+ * The keys and values go to their pages, which are tensors of their own (one tensor for both, or for their factors or open blocks, is refused); out: F32
+ * [T, n_heads * dk], the queries.  q_src NULL: keys and values alone (n_heads is ignored, *out is NULL). */
 CC_API int cc_paged_append(cc_device* dev, const cc_page_plan* plan, const cc_paged_cache* cache, const cc_view* q_src, int32_t q_col0, const cc_view* k_src,
                            int32_t k_col0, const cc_view* v_src, int32_t v_col0, int32_t n_heads, const cc_view* freq, int32_t pairing, int32_t offset, float mag,
                            cc_buf** out);
@@ -65,8 +66,9 @@ CC_API int cc_paged_append(cc_device* dev, const cc_page_plan* plan, const cc_pa
  * cache holds them after the append:
  *   score = scale * (q . k), or softcap * tanh(that / softcap) with softcap > 0; softmax with a denominator that also holds exp(sink[h]) (sink: [n_heads] or
  *   NULL); the weighted sum of the values.
- * Head h reads key head h / (n_heads / n_kv).  out: F32 [T, n_heads * dv], sums of 32 bits of weights of 22: a weight (8-bit pages: times
- * its block's factor) is off by 2^-22 of itself, or by 2^-33 of the row's largest if that is more.  A key or value that is not finite reaches the results of
+ * Head h reads key head h / (n_heads / n_kv).  out: F32 [T, n_heads * dv], sums of 32 bits of weights of 22: a weight is off by 2^-22 of
+ * itself or by 2^-33 of the row's largest, whichever is more (8-bit pages: that holds for weights times their blocks' factors, down to 2^-64 of the largest
+ * weight), and 16-bit numbers below 2^-14 are summed with the rounding errors of 2^-14.  Equal calls give equal bits on a device.  A key or value that is not finite reaches the results of
  * the queries that see it (not all of them, where its weight is zero) and no others; a query that holds a NaN or an infinity has the result NaN; rows behind a
  * sequence's end are not looked at.
  * Workspace, which the device's pool keeps: sequences with more than 32 rows (new tokens x n_heads / n_kv) have their visible keys and values of heads up to 128

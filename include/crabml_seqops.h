@@ -333,7 +333,7 @@ CC_API int cc_joined_product_accumulate(cc_device* dev, const cc_view* dst, cons
 /* ---- products in 8-bit integers -------------------------------------------------------------------------------------------------- */
 /* out = W x with 8-bit operands: w: I8 [m, k] codes (-127 .. 127, as rounding to a factor gives them; -128 counts as it stands), w_scale: F32 [m] one factor per
  * output channel, x: F32 [T, k], coded on the way with one factor per token: with a the largest magnitude of the row, x_scale = a / 127 and the codes
- * round(127 x / a), ties to even.  out[t, c] = (sum of the codes' products, exact) * x_scale[t] * w_scale[c], F32 [T, m].  k <= 131072.  A row that holds an
+ * round(127 x / a), ties to even.  out[t, c] = (sum of the codes' products, exact) * w_scale[c] * x_scale[t] in this order, F32 [T, m].  k <= 131072.  A row that holds an
  * infinity or a NaN has the result NaN. */
 CC_API int cc_product_i8(cc_device* dev, const cc_view* w, const cc_view* w_scale, const cc_view* x, cc_buf** out);
 
