@@ -26,6 +26,7 @@ ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1
 ROPE_LLAMA, ROPE_NEOX = 0, 1
 QK_NORM_NONE, QK_NORM_HEAD, QK_NORM_ROW = 0, 1, 2
 ROPE_NEIGHBOURS, ROPE_HALVES = 0, 1
+LATENT_AUTO, LATENT_ABSORBED, LATENT_EXPANDED = 0, 1, 2
 
 
 class TensorError(Exception):
@@ -275,6 +276,9 @@ def load_library(build_if_missing: bool = True):
         "cc_paged_append": (i32, [vp, vp, C.POINTER(cc_paged_cache), pv, i32, pv, i32, pv, i32, i32, pv, i32, i32, f32, pp]),
         "cc_paged_attention": (i32, [vp, vp, C.POINTER(cc_paged_cache), pv, i32, f32, i32, f32, pv, pp]),
         "cc_product_i8": (i32, [vp, pv, pv, pv, pp]),
+        "cc_product": (i32, [vp, pv, pv, pv, i32, pv, i32, pp]),
+        "cc_paged_latent_append": (i32, [vp, vp, pv, i32, pv, i32, pv, f32, pv, i32, i32, i32, pv, i32, f32, pp]),
+        "cc_paged_latent_attention": (i32, [vp, vp, pv, i32, pv, i32, pv, pv, f32, i32, pv, i32, i32, pp]),
     })
     sig.update({
         "ccr_runner_create": (i32, [vp, C.POINTER(ccr_llama_config), C.POINTER(ccr_llama_weights), i32, pp]),

@@ -1,0 +1,177 @@
+// product.cu -- out = act(W x + bias) + residual in one call (include/crabml_seqops.h, cc_product), operands of 16 bits, sums of 32.
+//
+// Few rows (product_few_kernel): every weight is read once, so memory bounds it.  mma.sync.m16n8k16 with 16 rows of W as its first operand and 8 rows of x as the second: a lane takes
+// 16 neighbouring bytes of a row of W straight into registers, and of a row of x from shared memory.  Which eight k a lane puts into two steps is free as long as both operands agree, so
+// nothing is rearranged.  8 warps share the depth of 16 rows of W; their sums meet in shared memory, where bias, activation and residual follow.
+#include <algorithm>
+
+#include "act.cuh"
+#include "half_types.cuh"
+#include "umma.cuh"
+
+struct PrArgs {
+    const void *w, *x, *res;
+    const float* bias;
+    void* out;
+    int64_t x_stride, res_stride;
+    int m, k, rows, x_type, out_type, act, chunk;
+    bool x_vec, w_vec;
+};
+__device__ __forceinline__ float pr_finish(const PrArgs& a, float v, int row, int col) {
+    if (a.bias) v += a.bias[col];
+    v = act_apply(v, a.act);
+    if (a.res) v += ht_read(a.res, (int64_t)row * a.res_stride + col, a.out_type);
+    return v;
+}
+template <bool BF16>
+__device__ __forceinline__ void pr_mma(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    if (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <bool BF16>
+__device__ __forceinline__ uint4 pr_pack8(const float (&v)[8]) {
+    return BF16 ? make_uint4(ht_pack_bf16(v[0], v[1]), ht_pack_bf16(v[2], v[3]), ht_pack_bf16(v[4], v[5]), ht_pack_bf16(v[6], v[7]))
+                : make_uint4(ht_pack_f16(v[0], v[1]), ht_pack_f16(v[2], v[3]), ht_pack_f16(v[4], v[5]), ht_pack_f16(v[6], v[7]));
+}
+
+#define PF_WARPS 8
+#define PF_THREADS (PF_WARPS * 32)
+#define PF_AHEAD 4                            // runs of 32 k that a warp has under way
+#define PF_SMEM (160 * 1024)
+// 8 numbers of a row from column c on, zeros behind its end
+__device__ __forceinline__ uint4 pf_weights(const uint16_t* row, int c, int k, bool there, bool vec) {
+    if (!there || c >= k) return make_uint4(0, 0, 0, 0);
+    if (vec) {
+        const int4 v = ld_stream_16(row + c);
+        return make_uint4((unsigned)v.x, (unsigned)v.y, (unsigned)v.z, (unsigned)v.w);
+    }
+    unsigned u[4] = {};
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+        if (c + j < k) u[j >> 1] |= (unsigned)row[c + j] << (j & 1) * 16;
+    return make_uint4(u[0], u[1], u[2], u[3]);
+}
+// grid (tiles of 16 rows of W, groups of 8 NT rows of x); the rows of x lie in shared memory, `chunk` of their k at a time
+template <int NT, bool BF16>
+__global__ void __launch_bounds__(PF_THREADS) product_few_kernel(const __grid_constant__ PrArgs a) {
+    extern __shared__ __align__(16) uint8_t pf_raw[];
+    __shared__ float sums[PF_WARPS][16][NT * 8 + 1];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, m0 = blockIdx.x * 16, n0 = blockIdx.y * NT * 8, pitch = a.chunk * 2 + 64;      // eight lanes' 16 bytes: two rows, 64 bytes each, in all banks
+    pdl_enter();
+    const uint16_t *w0 = (const uint16_t*)a.w + (int64_t)(m0 + (lane >> 2)) * a.k, *w1 = w0 + (int64_t)8 * a.k;
+    const bool in0 = m0 + (lane >> 2) < a.m, in1 = m0 + (lane >> 2) + 8 < a.m;
+    // the tensor cores cut a sum off at 24 bits after every 16 terms, always towards zero: sums of 128 terms go to registers and are rounded there (14336 terms of one sign: off by 1.1e-5
+    // in one chain a warp)
+    float total[NT][4] = {};
+    for (int k0 = 0; k0 < a.k; k0 += a.chunk) {
+        const int depth = min(a.chunk, a.k - k0), runs = (depth + 31) / 32;
+        uint4 u[PF_AHEAD], v[PF_AHEAD];
+        auto load = [&](int i, int r) {
+            const int c = r < runs ? k0 + r * 32 + (lane & 3) * 8 : a.k;
+            u[i] = pf_weights(w0, c, a.k, in0, a.w_vec); v[i] = pf_weights(w1, c, a.k, in1, a.w_vec);
+        };
+#pragma unroll
+        for (int i = 0; i < PF_AHEAD; i++) load(i, warp + i * PF_WARPS);
+        __syncthreads();                                              // the chunk before is through
+        for (int e = tid; e < NT * 8 * runs * 4; e += PF_THREADS) {
+            const int r = e / (runs * 4), c = e % (runs * 4) * 8;
+            float x[8] = {};
+            if (n0 + r < a.rows && k0 + c < a.k) {
+                const int64_t at = (int64_t)(n0 + r) * a.x_stride + k0 + c;
+                if (k0 + c + 8 <= a.k) ht_read8(a.x, at, a.x_type, a.x_vec, x);
+                else
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        if (k0 + c + j < a.k) x[j] = ht_read(a.x, at + j, a.x_type);
+            }
+            *(uint4*)(pf_raw + r * pitch + c * 2) = pr_pack8<BF16>(x);
+        }
+        __syncthreads();
+        for (int r = warp; r < runs; r += PF_WARPS * PF_AHEAD) {
+            float acc[NT][4] = {};
+#pragma unroll
+            for (int i = 0; i < PF_AHEAD; i++) {
+                const int here = r + i * PF_WARPS;
+                if (here < runs) {
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const uint4 b = *(const uint4*)(pf_raw + (n * 8 + (lane >> 2)) * pitch + here * 64 + (lane & 3) * 16);
+                        pr_mma<BF16>(acc[n], u[i].x, v[i].x, u[i].y, v[i].y, b.x, b.y);
+                        pr_mma<BF16>(acc[n], u[i].z, v[i].z, u[i].w, v[i].w, b.z, b.w);
+                    }
+                }
+                load(i, here + PF_WARPS * PF_AHEAD);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) total[n][j] += acc[n][j];
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) sums[warp][(lane >> 2) + (j >> 1) * 8][n * 8 + (lane & 3) * 2 + (j & 1)] = total[n][j];
+    __syncthreads();
+    for (int e = tid; e < 16 * NT * 8; e += PF_THREADS) {
+        const int i = e & 15, n = e >> 4, col = m0 + i, row = n0 + n;
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < PF_WARPS; w++) s += sums[w][i][n];
+        if (col < a.m && row < a.rows) ht_write(a.out, (int64_t)row * a.m + col, a.out_type, pr_finish(a, s, row, col));
+    }
+}
+template <int NT>
+static cudaError_t pf_launch(cc_device* dev, PrArgs a, bool bf16) {
+    auto kernel = bf16 ? product_few_kernel<NT, true> : product_few_kernel<NT, false>;
+    a.chunk = std::min((a.k + 63) / 64 * 64, (PF_SMEM / (NT * 8) - 64) / 128 * 64);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PF_SMEM);
+    if (e == cudaSuccess) e = cc_launch_pdl(dev, kernel, dim3((unsigned)((a.m + 15) / 16), (unsigned)((a.rows + NT * 8 - 1) / (NT * 8))), PF_THREADS, (size_t)NT * 8 * (a.chunk * 2 + 64), a);
+    dev->launches++;
+    return e;
+}
+
+extern "C" CC_API int cc_product(cc_device* dev, const cc_view* w, const cc_view* x, const cc_view* bias, int32_t act, const cc_view* residual, int32_t out_type, cc_buf** out) {
+    if (!dev) return CC_ERR_ARG;
+    CC_ENTER(dev);
+    if (!out) return cc_fail(dev, CC_ERR_ARG, "product: out is NULL");
+    *out = nullptr;
+    if (LAZY(dev)) return cc_fail(dev, CC_ERR_UNSUPPORTED, "product: not available on a lazy (graph / megakernel) device");
+    HT_ROWS(dev, x, "product x");
+    if (!view_ok(w)) return cc_fail(dev, CC_ERR_ARG, "product: bad view of w");
+    const bool bf16 = w->buf->dtype == CC_BF16;
+    CC_REQUIRE(dev, bf16 || w->buf->dtype == CC_F16, "product: weights of type %d (F16 or BF16)", w->buf->dtype);
+    HT_WHOLE(dev, w, w->buf->dtype, "product w");
+    CC_REQUIRE(dev, w->ndim == 2 && w->shape[1] == x->shape[1], "product: w is not [rows, %lld]", (long long)x->shape[1]);
+    const int64_t m = w->shape[0], k = w->shape[1], T = x->shape[0];
+    CC_REQUIRE(dev, m >= 1 && m < (1 << 27) && k >= 1 && k < (1 << 27) && T < (1 << 27), "product: %lld rows of %lld by %lld", (long long)T, (long long)k, (long long)m);
+    CC_REQUIRE(dev, ht_plain(out_type), "product: results of type %d (F32, F16 or BF16)", out_type);
+    CC_REQUIRE(dev, act >= CC_ACT_NONE && act <= CC_ACT_RELU_SQUARED, "product: activation %d", act);
+    if (bias) {
+        HT_WHOLE(dev, bias, CC_F32, "product bias");
+        CC_REQUIRE(dev, view_len(bias) == m, "product: bias is not [%lld]", (long long)m);
+    }
+    if (residual) {
+        HT_ROWS(dev, residual, "product residual");
+        CC_REQUIRE(dev, residual->buf->dtype == out_type && residual->shape[0] == T && residual->shape[1] == m, "product: residual is not [%lld, %lld] of the result's type", (long long)T, (long long)m);
+    }
+    cc_buf* o = nullptr;
+    int rc = cc_new_activation(dev, T * m, out_type, false, &o);
+    if (rc) return rc;
+    if (T > 0) {
+        PrArgs a{};
+        a.w = w->buf->plane[0]; a.x = x->buf->plane[0]; a.res = residual ? residual->buf->plane[0] : nullptr; a.bias = bias ? (const float*)bias->buf->plane[0] : nullptr;
+        a.out = o->base; a.x_stride = x->strides[0]; a.res_stride = residual ? residual->strides[0] : 0; a.m = (int)m; a.k = (int)k; a.rows = (int)T;
+        a.x_type = x->buf->dtype; a.out_type = out_type; a.act = act;
+        a.w_vec = k % 8 == 0 && ((uintptr_t)a.w & 15) == 0; a.x_vec = a.x_stride * ht_size(a.x_type) % 16 == 0 && ((uintptr_t)a.x & 15) == 0;
+        const cudaError_t e = T <= 8 ? pf_launch<1>(dev, a, bf16) : T <= 16 ? pf_launch<2>(dev, a, bf16) : pf_launch<4>(dev, a, bf16);
+        if (e != cudaSuccess) rc = cc_fail(dev, CC_ERR_CUDA, "product: %s", cudaGetErrorString(e));
+    }
+    if (rc) { cc_tensor_release(o); return rc; }
+    *out = o;
+    return CC_OK;
+}

@@ -4,6 +4,9 @@
     for layer in layers:                                          # rows of qkv: the new tokens, sequence after sequence
         q = append(plan, layer.cache, qkv, 0, qkv, H * d, qkv, (H + G) * d, H, freq=freq)
         y = attention(plan, layer.cache, q, H, d ** -0.5)
+        # a layer whose cache is one latent row a token, [rank | rest] columns: pages is a tensor F16 [n, 64, rank + rest]
+        q = latent_append(plan, layer.pages, rank, qkv, H * (dim + rest), norm_w=layer.norm, q_src=qkv, n_heads=H, dim=dim, freq=freq)
+        y = latent_attention(plan, layer.pages, rank, q, H, layer.uk, layer.uv, (dim + rest) ** -0.5)
 
 Results are queued on the device's stream: a library that is handed one (torch.as_tensor(y)) has to be ordered with it, see CudaTensor.__cuda_array_interface__.
 """
@@ -126,3 +129,29 @@ def attention(plan, cache, q, n_heads, scale, window=0, softcap=0.0, sink=None):
         n_heads, window = _number("paged_attention", "n_heads", n_heads), _number("paged_attention", "window", window)
     dev.check(dev.lib.cc_paged_attention(dev.handle, plan.handle, C.byref(cache._c), _v(q), n_heads, float(scale), window, float(softcap), _v(sink), C.byref(h)))
     return CudaTensor(_Buf(dev, h), TensorStrider([plan.tokens, n_heads * cache.v.shape()[3]]), dev)
+
+
+def latent_append(plan, pages, rank, kv_src, kv_col0, norm_w=None, eps=1e-6, q_src=None, q_col0=0, n_heads=0, dim=0, freq=None, pairing=capi.ROPE_NEIGHBOURS, mag=1.0):
+    """the plan's tokens' latent rows, normed and turned by their positions, into the pages F16 [pages, page size, rank + rest] -> the turned queries F16
+    [T, n_heads * (dim + rest)] (q_src None: None)"""
+    dev, h = plan.device, C.c_void_p()
+    try:
+        _SIX(rank, kv_col0, q_col0, n_heads, dim, pairing)
+    except struct.error:
+        rank, kv_col0, q_col0, n_heads, dim, pairing = (_number("paged_latent_append", what, x) for what, x in (
+            ("rank", rank), ("kv_col0", kv_col0), ("q_col0", q_col0), ("n_heads", n_heads), ("dim", dim), ("pairing", pairing)))
+    dev.check(dev.lib.cc_paged_latent_append(dev.handle, plan.handle, _v(pages), rank, _v(kv_src), kv_col0, _v(norm_w), float(eps), _v(q_src), q_col0, n_heads, dim, _v(freq),
+                                             pairing, float(mag), C.byref(h)))
+    return None if q_src is None else CudaTensor(_Buf(dev, h), TensorStrider([plan.tokens, n_heads * (dim + pages.shape()[2] - rank)]), dev)
+
+
+def latent_attention(plan, pages, rank, q, n_heads, uk, uv, scale, window=0, sink=None, form=capi.LATENT_AUTO, out_type=capi.BF16):
+    """-> [T, n_heads * vdim] of out_type (BF16 or F16)"""
+    dev, h = plan.device, C.c_void_p()
+    try:
+        _SIX(rank, n_heads, window, form, out_type, 0)
+    except struct.error:
+        rank, n_heads, window, form, out_type = (_number("paged_latent_attention", what, x) for what, x in (
+            ("rank", rank), ("n_heads", n_heads), ("window", window), ("form", form), ("out_type", out_type)))
+    dev.check(dev.lib.cc_paged_latent_attention(dev.handle, plan.handle, _v(pages), rank, _v(q), n_heads, _v(uk), _v(uv), float(scale), window, _v(sink), form, out_type, C.byref(h)))
+    return CudaTensor(_Buf(dev, h), TensorStrider([plan.tokens, uv.shape()[0]]), dev)

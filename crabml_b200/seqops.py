@@ -406,3 +406,10 @@ def product_i8(w, w_scale, x):
     h = C.c_void_p()
     x.device.check(x.device.lib.cc_product_i8(x.device.handle, _v(w), _v(w_scale), _v(x), C.byref(h)))
     return _new(x.device, h, [x.shape()[0], w.shape()[0]])
+
+
+def product(w, x, bias=None, act=capi.ACT_NONE, residual=None, out_type=capi.F32):
+    """act(W x + bias) + residual, w: F16 / BF16 [m, k], x: rows of F32, F16 or BF16 -> [T, m] of out_type"""
+    h = C.c_void_p()
+    x.device.check(x.device.lib.cc_product(x.device.handle, _v(w), _v(x), _v(bias), int(act), _v(residual), int(out_type), C.byref(h)))
+    return _new(x.device, h, [x.shape()[0], w.shape()[0]])

@@ -179,6 +179,18 @@ def _shape_arr(shape):
     return (C.c_int64 * len(shape))(*[int(s) for s in shape])
 
 
+class _Bits:
+    def __init__(self, tensor):
+        if not tensor.device.handle:
+            raise CudaError("the tensor's device is closed")
+        tensor.device.flush()
+        shape, strider = tuple(tensor._strider.shape), tensor._strider
+        self.tensor = tensor
+        self.__cuda_array_interface__ = {
+            "shape": shape, "typestr": "<i2", "data": (0 if 0 in shape else tensor.device.lib.cc_tensor_data(tensor.buf.handle), False),
+            "strides": None if strider.is_contiguous() else tuple(2 * s for s in strider.strides), "stream": tensor.device.stream(), "version": 3}
+
+
 class CudaTensor:
     def __init__(self, buf: _Buf, strider: TensorStrider, device: CudaTensorDevice, name=None):
         self.buf, self._strider, self.device, self.name = buf, strider, device, name
@@ -217,6 +229,13 @@ class CudaTensor:
         if not self.device._lazy:                                      # (eager: a buffer stays where it is, with all work on it queued)
             self._array, self._array_of = array, self._strider
         return dict(array)
+
+    def bits(self):
+        """The tensor's memory as whole numbers of 16 bits, for types that other libraries' array interfaces have no name for: torch.as_tensor(t.bits(), device="cuda").view(torch.bfloat16).
+        What __cuda_array_interface__ says about order and lifetime holds; the object keeps the tensor."""
+        if self.dtype() not in (capi.F16, capi.BF16):
+            raise TensorError(f"bits: a tensor of type {self.dtype()} has no plain elements of 16 bits")
+        return _Bits(self)
 
     def _new(self, handle, shape):
         return CudaTensor(_Buf(self.device, handle), TensorStrider(shape), self.device)

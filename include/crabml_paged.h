@@ -77,6 +77,31 @@ CC_API int cc_paged_append(cc_device* dev, const cc_page_plan* plan, const cc_pa
 CC_API int cc_paged_attention(cc_device* dev, const cc_page_plan* plan, const cc_paged_cache* cache, const cc_view* q, int32_t n_heads, float scale, int32_t window,
                               float softcap, const cc_view* sink, cc_buf** out);
 
+/* ---- a layer whose keys and values all heads make of one latent row a token ---------------------------------------------------------------- */
+/* pages: F16 [n_pages, page_size, rank + rest], rank and rest multiples of 16, rank from 16 to 512, rest from 0 to 64.  A row is [c | r], as in
+ * cc_latent_ring_append.  The plan needs no slots.  A sequence may go back to any token.
+ *
+ * For the plan's T tokens: rows kv_src [T, >= kv_col0 + rank + rest]; c, the first `rank` columns, is divided by sqrt(mean(c^2) + eps) and multiplied by norm_w
+ * (F32 [rank], NULL: 1); of r the first 2 P columns turn by position * freq[i] (freq: F32 [P] or NULL), as in cc_paged_append, any further one is copied.  Queries, if q_src
+ * is given, in the columns q_col0 .. q_col0 + n_heads * (dim + rest): of every head's last `rest` columns the first 2 P turn likewise, the others are copied (dim: a
+ * multiple of 16 up to 256).  Sources are F32, F16 or BF16, out F16 [T, n_heads * (dim + rest)]; computed in 32 bits (angles in 64) and rounded to F16 once; finite numbers beyond
+ * its range become its largest.  q_src NULL: n_heads and dim are ignored, *out is NULL. */
+CC_API int cc_paged_latent_append(cc_device* dev, const cc_page_plan* plan, const cc_view* pages, int32_t rank, const cc_view* kv_src, int32_t kv_col0, const cc_view* norm_w,
+                                  float eps, const cc_view* q_src, int32_t q_col0, int32_t n_heads, int32_t dim, const cc_view* freq, int32_t pairing, float mag, cc_buf** out);
+
+/* q: F16 [T, n_heads * (dim + rest)], a head is [n | p].  uk: F16 [n_heads * dim, rank], uv: F16 [n_heads * vdim, rank] (dim, vdim: multiples of 16 up to 256).  Keys and values of
+ * head h are k = [U_h c | r], v = V_h c; the token at position i sees j <= i of its sequence with i - j < window (window <= 0: all):
+ *   score = scale * (q . k) ; softmax with a denominator that also holds exp(sink[h]) (sink: F32 [n_heads] or NULL) ; the weighted sum of the values.
+ * out: [T, n_heads * vdim] of out_type (CC_F16 or CC_BF16), rounded once; finite results beyond its range become its largest.
+ * form: in which order the products are taken.  CC_LATENT_ABSORBED: queries over U to the latents, attention over the cached rows themselves, its result over V.
+ * CC_LATENT_EXPANDED: keys and values of every visible row laid out, then attention (dim and vdim up to 128, dim + rest up to 192).  CC_LATENT_AUTO: what should take less time,
+ * sequence by sequence.  Both hold weights and the factors of the second product as 16-bit numbers with 32-bit sums.
+ * A row of the cache that is not finite reaches the results of the queries that see it and no others; a query that holds a NaN or an infinity has the result NaN; rows behind a
+ * sequence's end are not looked at.  Equal calls give equal bits on a device. */
+enum cc_latent_form { CC_LATENT_AUTO = 0, CC_LATENT_ABSORBED = 1, CC_LATENT_EXPANDED = 2 };
+CC_API int cc_paged_latent_attention(cc_device* dev, const cc_page_plan* plan, const cc_view* pages, int32_t rank, const cc_view* q, int32_t n_heads, const cc_view* uk,
+                                     const cc_view* uv, float scale, int32_t window, const cc_view* sink, int32_t form, int32_t out_type, cc_buf** out);
+
 #ifdef __cplusplus
 }
 #endif

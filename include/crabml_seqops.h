@@ -337,6 +337,12 @@ CC_API int cc_joined_product_accumulate(cc_device* dev, const cc_view* dst, cons
  * infinity or a NaN has the result NaN. */
 CC_API int cc_product_i8(cc_device* dev, const cc_view* w, const cc_view* w_scale, const cc_view* x, cc_buf** out);
 
+/* ---- products with bias, activation and residual -------------------------------------------------------------------------------------- */
+/* out = act(W x + bias) + residual: w: F16 or BF16 [m, k]; x: rows [T, k] (any row stride) of F32, F16 or BF16, rounded to w's type where it has another one (finite numbers beyond the
+ * range of F16 become its largest); bias: F32 [m] or NULL; act: cc_activation; residual: [T, m] of out_type or NULL.  Sums, bias, activation and residual are taken in 32 bits and
+ * rounded once.  out: [T, m] of out_type (CC_F32, CC_F16 or CC_BF16; finite numbers beyond F16 become its largest). */
+CC_API int cc_product(cc_device* dev, const cc_view* w, const cc_view* x, const cc_view* bias, int32_t act, const cc_view* residual, int32_t out_type, cc_buf** out);
+
 #ifdef __cplusplus
 }
 #endif

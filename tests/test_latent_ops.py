@@ -1,0 +1,332 @@
+"""Latent rows in pages (include/crabml_paged.h): the append and the attention in both forms against plain references in 64 bits (tests/latent_ref.py), with the lengths,
+strides, masks and numbers at which they can go wrong."""
+import numpy as np
+import pytest
+
+from crabml_b200 import CudaTensor, TensorError, CudaError, TensorStrider, capi, paged
+from tests import latent_ref as R
+from tests.gpu_common import make_device
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+FORMS = {"absorbed": capi.LATENT_ABSORBED, "expanded": capi.LATENT_EXPANDED}
+
+
+@pytest.fixture(scope="module")
+def dev():
+    d = make_device()
+    yield d
+    d.close()
+
+
+TYPES = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}
+
+
+def view(t):
+    return torch.as_tensor(t.bits(), device="cuda").view(torch.bfloat16) if t.dtype() == capi.BF16 else torch.as_tensor(t, device="cuda")
+
+
+def give(dev, a, dtype=None):
+    a = torch.from_numpy(np.ascontiguousarray(a))
+    a = a if dtype is None else a.to(dtype)
+    t = CudaTensor.alloc(list(a.shape), TYPES[a.dtype], dev)
+    dev.synchronize()
+    if a.numel():
+        view(t).copy_(a)
+    torch.cuda.synchronize()
+    return t
+
+
+def take(dev, t):
+    dev.synchronize()
+    return view(t).float().cpu().numpy()
+
+
+def freqs(n, base=10000.0):
+    return (base ** (-np.arange(n) / max(n, 1))).astype(np.float32)
+
+
+class Case:
+    """sequences of given lengths over shuffled pages; what lies behind a sequence's end, and pages that no one has, is NaN"""
+
+    def __init__(self, dev, P, rank, rest, pos0, counts, spare=2, seed=0):
+        r = np.random.default_rng(seed)
+        self.dev, self.P, self.rank, self.rest, self.pos0, self.counts, self.rng = dev, P, rank, rest, list(pos0), list(counts), r
+        need = [(p + c + P - 1) // P for p, c in zip(pos0, counts)]
+        self.n_pages = sum(need) + spare
+        pages, cut = r.permutation(self.n_pages), np.cumsum([0] + need)
+        self.table = [pages[cut[i]:cut[i + 1]].tolist() for i in range(len(need))]
+        self.a = np.full((self.n_pages, P, rank + rest), np.nan, np.float16)
+        for i in range(len(need)):
+            self.put(i, 0, r.normal(size=(pos0[i] + counts[i], rank + rest)).astype(np.float16))
+
+    def put(self, i, pos, rows):
+        for j, x in enumerate(rows):
+            self.a[self.table[i][(pos + j) // self.P], (pos + j) % self.P] = x
+
+    def rows(self, i, n):
+        return np.stack([self.a[self.table[i][j // self.P], j % self.P] for j in range(n)]) if n else np.zeros((0, self.rank + self.rest), np.float16)
+
+    def plan(self):
+        return paged.PagePlan(self.dev, self.P, self.n_pages, self.table, self.pos0, self.counts)
+
+    def positions(self):
+        return np.concatenate([np.arange(p, p + n) for p, n in zip(self.pos0, self.counts)]) if self.counts else np.zeros(0)
+
+
+# ---- append -------------------------------------------------------------------------------------------------------------------------------
+LENGTHS = [([0], [1]), ([15], [1]), ([16], [1]), ([300], [1]), ([127], [2]), ([0], [128]), ([5], [300]), ([130, 7, 64], [1, 0, 1]), ([0, 0, 40], [0, 33, 100]), ([63, 64, 65, 1000], [1, 1, 70, 16])]
+
+
+def near16(got, want, steps=1.0):
+    """16-bit results of 32-bit steps: half a step of 2^-11 and what the steps before it are off by (2^-22 of the value and its terms: norm and turn are a few operations), beside
+    the smallest numbers' 2^-25"""
+    want = np.asarray(want, np.float64)
+    np.testing.assert_allclose(got, np.clip(want, -65504, 65504), rtol=steps * 2.0 ** -11 + 2.0 ** -19, atol=2.0 ** -25 + 2.0 ** -19)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("P", [16, 64, 128])
+@pytest.mark.parametrize("pos0,counts", LENGTHS, ids=[str(i) for i in range(len(LENGTHS))])
+def test_append(dev, P, dtype, pos0, counts):
+    H, dim, rest, rank = 3, 32, 16, 48
+    c = Case(dev, P, rank, rest, pos0, counts, seed=P)
+    T, odd = sum(counts), 8 if dtype == torch.float32 else 3                # rows that start at a multiple of 16 bytes, and others
+    src = torch.from_numpy(c.rng.normal(size=(T, H * (dim + rest) + odd + rank + rest + 5)) * np.exp(c.rng.normal(size=(T, 1)))).to(dtype)
+    kc, w, f = H * (dim + rest) + odd, c.rng.normal(size=rank).astype(np.float32), freqs(rest // 2)
+    pages, t = give(dev, c.a), give(dev, src.float().numpy(), dtype)
+    q = paged.latent_append(c.plan(), pages, rank, t, kc, norm_w=give(dev, w), eps=1e-5, q_src=t, n_heads=H, dim=dim, freq=give(dev, f))
+    x, pos, was = src.double().numpy(), c.positions(), c.a.copy()
+    want = x[:, :H * (dim + rest)].reshape(T, H, dim + rest).copy()
+    want[..., dim:] = R.turn(want[..., dim:], pos, f, 0, 1.0)
+    assert q.shape() == [T, H * (dim + rest)] and q.dtype() == capi.F16
+    near16(take(dev, q).reshape(want.shape), want)
+    rows, at = R.row(x[:, kc:kc + rank + rest], rank, w, 1e-5, pos, f, 0, 1.0), 0
+    got = take(dev, pages)
+    for i, n in enumerate(counts):
+        for j in range(n):
+            p = pos0[i] + j
+            near16(got[c.table[i][p // P], p % P], rows[at + j])
+            was[c.table[i][p // P], p % P] = got[c.table[i][p // P], p % P]
+        at += n
+    np.testing.assert_array_equal(got, was.astype(np.float32))               # every other row is as it was
+
+
+@pytest.mark.parametrize("pairing,n,mag", [(0, 32, 1.0), (1, 32, 1.0), (0, 8, 1.25), (1, 17, 0.7), (1, 0, 1.0), (0, 1, 1.0)])
+def test_append_turns(dev, pairing, n, mag):
+    """both pairings, part of the columns, a factor; at positions where 32 bits lose the angle"""
+    H, dim, rest, rank, P = 2, 16, 64, 16, 16
+    pos0, counts = [1000003 // P * P - 5, 31], [23, 1]
+    need = [(p + k + P - 1) // P for p, k in zip(pos0, counts)]
+    table = [[0] * (need[0] - 3) + [1, 2, 3], [4, 5]]
+    r = np.random.default_rng(n)
+    T, f = sum(counts), freqs(n)
+    src = r.normal(size=(T, H * (dim + rest) + rank + rest)).astype(np.float32)
+    pages, t = give(dev, np.zeros((6, P, rank + rest), np.float16)), give(dev, src)
+    plan = paged.PagePlan(dev, P, 6, table, pos0, counts)
+    q = paged.latent_append(plan, pages, rank, t, H * (dim + rest), eps=0.0, q_src=t, n_heads=H, dim=dim, freq=give(dev, f), pairing=pairing, mag=mag)
+    pos = np.concatenate([np.arange(p, p + k) for p, k in zip(pos0, counts)])
+    want = src[:, :H * (dim + rest)].reshape(T, H, -1).astype(np.float64)
+    want[..., dim:] = R.turn(want[..., dim:], pos, f, pairing, mag)
+    near16(take(dev, q).reshape(want.shape), want)
+    rows, got = R.row(src[:, H * (dim + rest):], rank, None, 0.0, pos, f, pairing, mag), take(dev, pages)
+    for j, p in enumerate(pos):
+        i = 0 if j < counts[0] else 1
+        near16(got[table[i][p // P], p % P], rows[j])
+
+
+def test_append_of_extremes(dev):
+    """numbers beyond 16 bits become its largest, infinities and NaN stay, rows of zeros stay zeros"""
+    rank, rest, P, H, dim = 16, 16, 16, 1, 16
+    src = np.zeros((5, dim + rest + rank + rest), np.float32)
+    src[0, :4] = [1e6, -7e4, np.inf, np.nan]
+    src[0, dim + rest + rank] = 3e38
+    src[1, dim + rest + rank + 1] = -np.inf
+    src[2, dim + rest + 3] = np.nan                                          # the whole of c
+    src[3, dim + rest:dim + rest + rank] = 1e-30                             # squares that vanish
+    src[4, dim + rest:dim + rest + rank] = 1e18
+    pages, t = give(dev, np.ones((1, P, rank + rest), np.float16)), give(dev, src)
+    q = take(dev, paged.latent_append(paged.PagePlan(dev, P, 1, [[0]], [0], [5]), pages, rank, t, dim + rest, eps=1e-6, q_src=t, n_heads=H, dim=dim))
+    got = take(dev, pages)[0]
+    np.testing.assert_array_equal(q[0, :4], [65504.0, -65504.0, np.inf, np.nan])
+    assert got[0, rank] == 65504.0 and got[1, rank + 1] == -np.inf and np.isnan(got[2, :rank]).all() and (got[2, rank:] == 0).all()
+    assert (got[0, :rank] == 0).all() and (got[3, :rank] == 0).all() and (np.abs(got[4, :rank] - 1.0) < 1e-3).all()
+    assert (got[5:] == 1.0).all()
+
+
+def test_append_rows_alone(dev):
+    c = Case(dev, 32, 32, 0, [3], [40])
+    src = c.rng.normal(size=(40, 32)).astype(np.float32)
+    pages = give(dev, c.a)
+    assert paged.latent_append(c.plan(), pages, 32, give(dev, src), 0, eps=1e-6) is None
+    got = take(dev, pages)
+    near16(np.stack([got[c.table[0][p // 32], p % 32] for p in range(3, 43)]), R.row(src, 32, None, 1e-6, np.arange(3, 43), [], 0, 1.0))
+
+
+# ---- attention ----------------------------------------------------------------------------------------------------------------------------
+def bound(want, size, q, rows, uk, rank, H, scale, out_eps):
+    """How far a result may be off.  2^-11 is half a step of f16.
+    a weight: 2^-11 of itself by its rounding, and its score's error e: the query over the latents (absorbed) or the key (expanded) rounded to f16, 2^-11 of a term at most, in a sum of
+    terms q_j k_j whose roundings have no common sign: 4 standard deviations of it, 4 x 2^-11 / sqrt(3) x the root of the sum of (q_j k_j)^2, at most |q| |k|; 32-bit sums of up to 576 terms beside
+    it.  A score's error multiplies weights by 1 +- e, in the sum and its divisor: 2 e of sum(w |v|).
+    values: 2^-11 of sum(w |v|) in the expanded form.  The result: its own rounding, out_eps of itself."""
+    e = abs(scale) * 4 * 2.0 ** -11 / 3 ** 0.5 * q                            # (an error has no sign)
+    return out_eps * np.abs(want) + (2 * e + 3 * 2.0 ** -11) * size * 1.1 + 2.0 ** -24
+
+
+def attend(dev, c, q, uk, uv, H, scale, window, sink, form, out_type=capi.BF16):
+    y = paged.latent_attention(c.plan(), give(dev, c.a), c.rank, give(dev, q), H, give(dev, uk), give(dev, uv), scale, window=window, sink=None if sink is None else give(dev, sink),
+                               form=form, out_type=out_type)
+    assert y.shape() == [sum(c.counts), uv.shape[0]] and y.dtype() == out_type
+    return take(dev, y)
+
+
+def check(dev, c, H, dim, vdim, scale, window=0, sink=None, form=capi.LATENT_AUTO, out_type=capi.BF16, q=None, uk=None, uv=None):
+    T, rank, rest, r = sum(c.counts), c.rank, c.rest, c.rng
+    uk = (r.normal(size=(H * dim, rank)) * rank ** -0.5).astype(np.float16) if uk is None else uk
+    uv = (r.normal(size=(H * vdim, rank)) * rank ** -0.5).astype(np.float16) if uv is None else uv
+    q = r.normal(size=(T, H * (dim + rest))).astype(np.float16) if q is None else q
+    got = attend(dev, c, q, uk, uv, H, scale, window, sink, form, out_type).reshape(T, H, vdim)
+    eps, at = 2.0 ** -8 if out_type == capi.BF16 else 2.0 ** -11, 0
+    for i, n in enumerate(c.counts):
+        rows, mine = c.rows(i, c.pos0[i] + n), q[at:at + n].reshape(n, H, dim + rest)
+        want, size = R.attention(rows, c.pos0[i], mine, uk, uv, rank, H, scale, window, sink)
+        with np.errstate(invalid="ignore", over="ignore"):
+            k = np.concatenate([np.einsum("jr,hdr->hjd", rows[:, :rank].astype(np.float64), uk.astype(np.float64).reshape(H, dim, rank)),
+                                np.broadcast_to(rows[None, :, rank:].astype(np.float64), (H, len(rows), rest))], 2) if n else np.zeros((H, 0, dim + rest))
+            far = np.sqrt(np.nansum(k ** 2, 2)).max(1) if n else np.zeros(H)       # of keys that are finite
+            # absorbed: terms are those of the query over the latents and the row
+            over = np.concatenate([np.einsum("thd,hdr->thr", mine[..., :dim].astype(np.float64), uk.astype(np.float64).reshape(H, dim, rank)), mine[..., dim:].astype(np.float64)], 2)
+            terms = np.maximum(np.sqrt((mine.astype(np.float64) ** 2).sum(2)) * far[None],
+                               np.sqrt((over ** 2).sum(2)) * np.sqrt(np.nanmax(np.where(np.isfinite(rows), rows.astype(np.float64) ** 2, np.nan), initial=0.0)))
+        off = np.abs(got[at:at + n] - want)
+        lim = bound(want, size, terms[..., None], rows, uk, rank, H, scale, eps)
+        bad = ~((off <= lim) | (np.isnan(got[at:at + n]) & np.isnan(want)))
+        assert not bad.any(), (i, np.argwhere(bad)[:5].tolist(), got[at:at + n][bad][:5], want[bad][:5], lim[bad][:5])
+        at += n
+    return got
+
+
+SHAPES = [  # heads, dim, rest, vdim, rank
+    (16, 128, 64, 128, 512), (3, 32, 16, 32, 64), (1, 16, 0, 16, 16), (5, 48, 16, 80, 160), (8, 64, 32, 64, 256), (24, 32, 48, 16, 80), (33, 16, 16, 32, 48),
+]
+SEQS = [([0], [1]), ([31], [1]), ([32], [1]), ([200], [1]), ([1000, 3, 0, 64], [1, 1, 1, 1]), ([40, 0, 5], [3, 0, 2]), ([0, 100], [9, 6]), ([70], [17]), ([0], [150])]
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("shape", SHAPES, ids=[str(s) for s in SHAPES])
+@pytest.mark.parametrize("pos0,counts", SEQS, ids=[str(i) for i in range(len(SEQS))])
+def test_attention(dev, form, shape, pos0, counts):
+    H, dim, rest, vdim, rank = shape
+    c = Case(dev, 16, rank, rest, pos0, counts, seed=H)
+    check(dev, c, H, dim, vdim, 1.5 * (dim + rest) ** -0.5, form=FORMS[form])
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("out_type", [capi.F16, capi.BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("window,sink", [(0, False), (1, False), (2, True), (33, False), (100, True), (1000, True)])
+@pytest.mark.parametrize("P", [16, 32, 128])
+def test_masks(dev, form, P, window, sink, out_type):
+    c = Case(dev, P, 64, 16, [300, 0, 64], [7, 1, 33], seed=window)
+    check(dev, c, 6, 32, 32, 0.2, window=window, sink=c.rng.normal(size=6).astype(np.float32) if sink else None, form=FORMS[form], out_type=out_type)
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+def test_sinks_far_away(dev, form):
+    """sinks that take all of the weight, none of it, and -inf"""
+    c = Case(dev, 16, 32, 16, [50], [3])
+    check(dev, c, 4, 16, 16, 0.3, sink=np.array([-np.inf, 80.0, -80.0, 1e30], np.float32), form=FORMS[form])
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+def test_rows_that_are_not_finite(dev, form):
+    """they reach the queries that see them and no others: later tokens of the call, windows that have left them, other sequences"""
+    for window in (0, 12):
+        c = Case(dev, 16, 32, 16, [40, 40, 90], [20, 20, 40], seed=window)
+        for i, (at, col, x) in enumerate([(50, 3, np.nan), (45, 35, np.inf), (100, 0, -np.inf)]):
+            row = c.rows(i, c.pos0[i] + c.counts[i])[at].copy()
+            row[col] = x
+            c.put(i, at, row[None])
+        H, dim, vdim = 3, 32, 32
+        q = np.abs(c.rng.normal(size=(80, H * (dim + 16)))).astype(np.float16)
+        uk, uv = (np.abs(c.rng.normal(size=(H * d, 32)) * 0.2).astype(np.float16) for d in (dim, vdim))
+        got = attend(dev, c, q, uk, uv, H, 0.2, window, None, FORMS[form]).reshape(80, H, vdim)
+        at = 0
+        for i, n in enumerate(c.counts):
+            want, size = R.attention(c.rows(i, c.pos0[i] + n), c.pos0[i], q[at:at + n].reshape(n, H, -1), uk, uv, 32, H, 0.2, window)
+            clean = ~np.isnan(want)
+            assert np.isfinite(got[at:at + n][clean]).all()
+            np.testing.assert_allclose(got[at:at + n][clean], want[clean], rtol=0.03, atol=0.03)
+            # a weight of exactly 0 may drop it: a score of -inf
+            lost = ~np.isfinite(got[at:at + n][~clean])
+            assert lost.all() or (i > 0 and x == -np.inf)
+            at += n
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+def test_queries_that_are_not_finite(dev, form):
+    c = Case(dev, 16, 32, 16, [40], [20])
+    H, dim = 3, 32
+    q = c.rng.normal(size=(20, H * (dim + 16))).astype(np.float16)
+    q[3, 5], q[4, dim + 16 + dim + 3], q[19, 2 * (dim + 16)] = np.nan, np.inf, -np.inf
+    check(dev, c, H, dim, 32, 0.2, form=FORMS[form], q=q)
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("scale", [0.0, -0.3, 30.0, 3000.0])
+def test_scores_of_any_size(dev, form, scale):
+    """a score of thousands: one key has all of the weight.  Scores whose difference is far above their errors: the queries pick keys out by their rotated part alone"""
+    c = Case(dev, 16, 32, 16, [30], [2], seed=3)
+    for j in range(32):                                                      # row j: latents of its own, and the j-th of 32 directions, as +-1 and powers of two
+        row = c.rows(0, 32)[j].copy()
+        row[32:] = [(1.0 if j >> (b % 5) & 1 else -1.0) * (1.0 + 0.25 * (b // 5)) for b in range(16)]
+        c.put(0, j, row[None])
+    H, dim, vdim = 2, 16, 32
+    q = np.zeros((2, H, dim + 16), np.float16)
+    q[..., dim:] = 2.0 * c.rows(0, 32)[13, 32:]
+    check(dev, c, H, dim, vdim, scale, form=FORMS[form], q=q.reshape(2, -1))
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+def test_large_and_small_numbers(dev, form):
+    """queries and latents near the ends of 16 bits"""
+    for big, small in ((60000.0, 1.0 / 60000.0), (1.0 / 4096.0, 4096.0), (1.0, 1.0)):
+        c = Case(dev, 16, 32, 16, [60], [3], seed=5)
+        q = np.clip(c.rng.normal(size=(3, 2 * 32)) * big / 4, -65504, 65504).astype(np.float16)
+        check(dev, c, 2, 16, 32, 0.2 * small * 4, form=FORMS[form], q=q)
+
+
+def test_strided_and_reused(dev):
+    """the same plan for two layers, a call after another, and equal calls give equal bits"""
+    c = Case(dev, 32, 64, 16, [500, 90, 2000], [1, 4, 1], seed=9)
+    H, dim, vdim = 16, 32, 32
+    q, uk, uv = (give(dev, (c.rng.normal(size=s) * k).astype(np.float16)) for s, k in (((6, H * (dim + 16)), 1.0), ((H * dim, 64), 0.125), ((H * vdim, 64), 0.125)))
+    plan, pages = c.plan(), give(dev, c.a)
+    for form in FORMS.values():
+        first = [take(dev, paged.latent_attention(plan, pages, 64, q, H, uk, uv, 0.2, form=form)) for _ in range(3)]
+        assert all(np.array_equal(first[0], y) for y in first[1:])
+
+
+def test_shared_prefix(dev):
+    """two sequences over the same pages of a prefix"""
+    P, rank, rest, H = 16, 32, 16, 4
+    r = np.random.default_rng(1)
+    a = r.normal(size=(8, P, rank + rest)).astype(np.float16)
+    table, pos0, counts = [[3, 5, 0], [3, 5, 1]], [40, 37], [1, 3]
+    q, uk, uv = ((r.normal(size=s) * k).astype(np.float16) for s, k in (((4, H * 32), 1.0), ((H * 16, rank), 0.2), ((H * 16, rank), 0.2)))
+    for form in FORMS.values():
+        y = take(dev, paged.latent_attention(paged.PagePlan(dev, P, 8, table, pos0, counts), give(dev, a), rank, give(dev, q), H, give(dev, uk), give(dev, uv), 0.2, form=form))
+        at = 0
+        for i, n in enumerate(counts):
+            rows = np.concatenate([a[p] for p in table[i]])[:pos0[i] + n]
+            want, _ = R.attention(rows, pos0[i], q[at:at + n].reshape(n, H, 32), uk, uv, rank, H, 0.2)
+            np.testing.assert_allclose(y[at:at + n].reshape(want.shape), want, rtol=0.02, atol=0.01)
+            at += n
+
+
+def test_nothing(dev):
+    c = Case(dev, 16, 32, 16, [5, 9], [0, 0])
+    y = paged.latent_attention(c.plan(), give(dev, c.a), 32, CudaTensor.alloc([0, 64], capi.F16, dev), 2, give(dev, np.ones((32, 32), np.float16)), give(dev, np.ones((64, 32), np.float16)), 1.0)
+    assert y.shape() == [0, 64]
+    assert paged.latent_append(c.plan(), give(dev, c.a), 32, CudaTensor.alloc([0, 48], capi.F32, dev), 0, q_src=CudaTensor.alloc([0, 64], capi.F32, dev), n_heads=2, dim=16).shape() == [0, 64]
