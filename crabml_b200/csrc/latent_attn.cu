@@ -587,6 +587,10 @@ static int lr_run(cc_device* dev, const cc_page_plan* plan, LrArgs a, const LtRu
     return CC_OK;
 }
 
+#include "latent_tile.cuh"
+
+#define LT_FEW 64                             // new tokens of a sequence; with more its keys and values are laid out
+
 extern "C" CC_API int cc_paged_latent_attention(cc_device* dev, const cc_page_plan* plan, const cc_view* pages, int32_t rank, const cc_view* q, int32_t H, const cc_view* uk,
                                                 const cc_view* uv, float scale, int32_t window, const cc_view* sink, int32_t form, int32_t out_type, cc_buf** out) {
     PG_ENTER(dev, plan, "paged_latent_attention");
@@ -612,6 +616,9 @@ extern "C" CC_API int cc_paged_latent_attention(cc_device* dev, const cc_page_pl
     for (const cc_view* v : {q, uk, uv}) CC_REQUIRE(dev, ((uintptr_t)v->buf->plane[0] & 15) == 0, "paged_latent_attention: a tensor does not start at a multiple of 16 bytes");
     CC_REQUIRE(dev, form == CC_LATENT_AUTO || form == CC_LATENT_ABSORBED || form == CC_LATENT_EXPANDED, "paged_latent_attention: form %d", form);
     CC_REQUIRE(dev, out_type == CC_F16 || out_type == CC_BF16, "paged_latent_attention: results of type %d (F16 or BF16)", out_type);
+    // tensor maps count rows in 32 bits
+    const bool expands = dim <= TL_DIM && vdim <= TL_DIM && plan->n_pages * plan->page < ((int64_t)1 << 31) && (int64_t)H * LT_DIM < ((int64_t)1 << 31);
+    CC_REQUIRE(dev, form != CC_LATENT_EXPANDED || expands, "paged_latent_attention: heads of %lld and %lld are not expanded (up to %d)", (long long)dim, (long long)vdim, TL_DIM);
     cc_buf* o = nullptr;
     rc = cc_new_activation(dev, T * H * vdim, out_type, false, &o);
     if (rc) return rc;
@@ -621,7 +628,8 @@ extern "C" CC_API int cc_paged_latent_attention(cc_device* dev, const cc_page_pl
         a.q = (const __half*)q->buf->plane[0]; a.uk = (const __half*)uk->buf->plane[0]; a.uv = (const __half*)uv->buf->plane[0];
         a.sink = sink ? (const float*)sink->buf->plane[0] : nullptr; a.out = o->base; a.scale = scale;
         a.n_seqs = plan->n_seqs; a.table_cols = plan->table_cols; a.page = plan->page; a.shift = plan->shift; a.H = H; a.dim = (int)dim; a.vdim = (int)vdim;
-        a.rank = c.rank; a.rest = c.rest; a.cols = c.cols; a.window = window > 0 ? window : 0; a.most = 0x7fffffff; a.out_bf16 = out_type == CC_BF16;
+        a.rank = c.rank; a.rest = c.rest; a.cols = c.cols; a.window = window > 0 ? window : 0; a.out_bf16 = out_type == CC_BF16;
+        a.most = form == CC_LATENT_EXPANDED ? 0 : form == CC_LATENT_ABSORBED || !expands ? 0x7fffffff : LT_FEW;
         LtRuns runs{};
         bool wide = false;
         for (const PgSeq& s : plan->seqs) {
@@ -633,6 +641,7 @@ extern "C" CC_API int cc_paged_latent_attention(cc_device* dev, const cc_page_pl
         }
         for (int i = 0; i < runs.n; i++) { runs.tile0[i] = runs.tiles; runs.tiles += (runs.hi[i] - runs.lo[i] + 15) / 16; }
         rc = wide ? lr_run<2>(dev, plan, a, runs) : lr_run<1>(dev, plan, a, runs);
+        if (!rc && a.most < 0x7fffffff) rc = tl_run(dev, plan, a);      // behind the others: their last products may run over tokens of these
     }
     if (rc) { cc_tensor_release(o); return rc; }
     *out = o;

@@ -1,0 +1,582 @@
+// latent_tile.cuh -- attention over pages of latent rows, expanded: many new tokens of a sequence.  Included by latent_attn.cu behind the absorbed form.
+//
+// latent_expand_kernel makes the keys U_h c and values V_h c of 128 cached rows and a run of heads: one product of 128 x (dim + vdim) x rank for each head on tcgen05.mma, the rows staying in
+// shared memory for all heads.  The results go to images, f16 in the order of the 128-byte swizzle, which bulk copies bring back as they are.  r, which all heads share, is read from the pages.
+//
+// latent_tile_kernel: a CTA takes 256 tokens of a head, as two tiles of 128 rows, over the keys that they see, 128 at a time:
+//   S = Q K^T (128 x 128 x (dim + rest)), P = exp2(S f - base) as f16 written over S in TMEM, O += P V in TMEM
+// The two tiles alternate: while the 128 threads of one make its weights, a row each, the tensor core multiplies for the other.  TMEM holds both S and both O (512 columns), shared memory
+// Q (96 KB) and a ring of 16 KB blocks of keys and values (128 KB).  base lags: a row's sums are scaled only when its largest score is 2^TL_LAG times what it was (sums in TMEM would have
+// to be read and written back), so that weights are up to 2^TL_LAG and f16 still holds them and all that counts beside them.
+// Warps 0-3 and 4-7 the rows of the two tiles, 8 the copies, 9 the products.  Every wait is bounded; where one ran out all roles run to their ends and the host reports it.
+#pragma once
+#include <cuda.h>
+
+#define TL_ROWS 128
+#define TL_KEYS 128
+#define TL_THREADS 384
+// 384 threads of 168 registers at launch are 256 of 216 and 128 of 72 afterwards: 128 scores of a row stay in registers
+#define TL_REGS 168
+#define TL_REGS_SOFT 216
+#define TL_REGS_REST 72
+static_assert(256 * TL_REGS_SOFT + 128 * TL_REGS_REST <= TL_THREADS * TL_REGS, "more registers than the block was launched with");
+#define TL_BLOCK 16384                        // 128 rows of 64 f16 under the 128-byte swizzle
+#define TL_SLOTS 8
+#define TL_QBLOCKS 3                          // of a row of Q: dim in two, rest in one
+#define TL_SMEM ((2 * TL_QBLOCKS + TL_SLOTS) * TL_BLOCK + 1024)
+#define TL_LAG 8.0f
+#define TL_O 256                              // TMEM columns: S (and P) of the tiles at 0 and 128, O behind
+#define TL_DIM 128                            // largest dim and vdim
+#define TL_SFU 14                             // of 16 weights those that the special function unit makes
+
+struct TlArgs {
+    LrArgs a;
+    uint8_t *k_image, *v_image;               // [key tile][head of this launch][block]
+    int head0, heads, key_tiles, items;
+};
+// keys count from a multiple of 128, so that a tile is whole pages
+__host__ __device__ __forceinline__ void tl_range(const PgSeq& s, const LrArgs& a, int* from, int* to) {
+    lr_range(s, a, from, to);
+    *from &= ~(TL_KEYS - 1);
+}
+__host__ __device__ __forceinline__ int tl_key_tiles(const PgSeq& s, const LrArgs& a) {
+    if (s.count <= a.most) return 0;
+    int from, to;
+    tl_range(s, a, &from, &to);
+    return (to - from + TL_KEYS - 1) / TL_KEYS;
+}
+__host__ __device__ __forceinline__ int tl_items(const PgSeq& s, const LrArgs& a) { return s.count <= a.most ? 0 : (s.count + 2 * TL_ROWS - 1) / (2 * TL_ROWS); }
+// the place of number n in the sequences' counts: every lane gets the sequence and what is left of n
+template <class Count>
+__device__ __forceinline__ int tl_find(const LrArgs& a, int n, Count count, int* rest) {
+    const int lane = threadIdx.x & 31;
+    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
+        const int s = s0 + lane, mine = s < a.n_seqs ? count(a.seqs[s]) : 0;
+        int sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const int x = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += x;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, n < sum);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            *rest = n - __shfl_sync(0xffffffffu, sum - mine, l);
+            return s0 + l;
+        }
+        n -= __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return -1;
+}
+__device__ __forceinline__ unsigned tl_at(int row, int chunk) { return (unsigned)(row * 128 + ((chunk ^ (row & 7)) << 4)); }      // chunk of 8 numbers of a row of a block
+// for warps that have nothing else to do for long: the hardware holds them for up to 2 us a look, so that they leave the issue slots to others
+__device__ __forceinline__ bool tl_wait(unsigned bar, unsigned parity, int* fail) {
+    unsigned done = 0;
+    for (unsigned it = 0; it < (1u << 21); it++) {
+        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(done) : "r"(bar), "r"(parity), "r"(2000u) : "memory");
+        if (done) return true;
+        if (*(volatile int*)fail) return false;
+    }
+    *(volatile int*)fail = 1;
+    return false;
+}
+__device__ __forceinline__ bool tl_wait_warp(unsigned bar, unsigned parity, int* fail) { return __all_sync(0xffffffffu, tl_wait(bar, parity, fail)); }
+__device__ __forceinline__ void tl_report(int fail, unsigned* err_dev, unsigned* err_host) {
+    if (threadIdx.x == 0 && fail) {
+        if (err_dev) atomicExch(err_dev, 5u);
+        if (err_host) { *(volatile unsigned*)err_host = 5u; __threadfence_system(); }
+    }
+}
+// the pages that hold keys key0 .. key0 + 127 of a sequence: a box of 64 columns from x on for each, those behind its last token left out.  Returns the bytes
+__device__ __forceinline__ unsigned tl_pages(const LrArgs& a, int seq, int key0, int to) { return (unsigned)((min(TL_KEYS, to - key0) + a.page - 1) / a.page * a.page * 128); }
+__device__ __forceinline__ void tl_load_pages(const LrArgs& a, const CUtensorMap* map, unsigned dst, unsigned bar, int x, int seq, int key0, int to) {
+    for (int i = 0; i < TL_KEYS && key0 + i < to; i += a.page) pg_tma_load_2d(dst + i * 128, map, bar, x, a.table[(int64_t)seq * a.table_cols + ((key0 + i) >> a.shift)] * a.page);
+}
+
+// ---- keys and values of 128 rows ------------------------------------------------------------------------------------------------------------------------
+#define TE_THREADS 384
+#define TE_ABLOCKS (LT_RANK / 64)
+#define TE_STAGES 2
+#define TE_STAGE (2 * TL_DIM * 128)           // 64 columns of U_h and V_h
+#define TE_SMEM (TE_ABLOCKS * TL_BLOCK + TE_STAGES * TE_STAGE + 1024)
+struct TeShared {
+    unsigned long long a_full[TE_ABLOCKS], full[TE_STAGES], empty[TE_STAGES], acc_full[2], acc_empty[2], drained;
+    unsigned tmem_base;
+    int fail;
+};
+// grid (key tiles, runs of heads)
+__global__ void __launch_bounds__(TE_THREADS, 1) latent_expand_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_uk, const __grid_constant__ CUtensorMap map_uv,
+                                                                      const __grid_constant__ TlArgs t, unsigned* err_dev, unsigned* err_host) {
+    extern __shared__ __align__(1024) uint8_t tl_raw[];
+    __shared__ TeShared sh;
+    const LrArgs& a = t.a;
+    uint8_t *as = (uint8_t*)(((uintptr_t)tl_raw + 1023) & ~(uintptr_t)1023), *bs = as + TE_ABLOCKS * TL_BLOCK;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, width = a.dim + a.vdim, blocks = (a.rank + 63) >> 6;
+    const int h0 = (int)((int64_t)t.heads * blockIdx.y / gridDim.y), h1 = (int)((int64_t)t.heads * (blockIdx.y + 1) / gridDim.y);
+    if (tid == 0) {
+        for (int i = 0; i < TE_ABLOCKS; i++) pg_mbar_init(pg_smem(&sh.a_full[i]), 1);
+        for (int i = 0; i < TE_STAGES; i++) { pg_mbar_init(pg_smem(&sh.full[i]), 1); pg_mbar_init(pg_smem(&sh.empty[i]), 1); }
+        for (int i = 0; i < 2; i++) { pg_mbar_init(pg_smem(&sh.acc_full[i]), 1); pg_mbar_init(pg_smem(&sh.acc_empty[i]), 8); }
+        pg_mbar_init(pg_smem(&sh.drained), 1);
+        sh.fail = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pg_smem(&sh.tmem_base)), "n"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pg_fence_before();
+    __syncthreads();
+    pg_fence_after();
+    const unsigned tmem = sh.tmem_base;
+    pdl_enter();
+    int kt;
+    const int seq = max(0, tl_find(a, blockIdx.x, [&](const PgSeq& s) { return tl_key_tiles(s, a); }, &kt));      // (the grid has as many rows as there are tiles)
+    const PgSeq s = a.seqs[seq];
+    int from, to;
+    tl_range(s, a, &from, &to);
+    const int key0 = from + kt * TL_KEYS;
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int b = 0; b < blocks; b++) {
+                pg_mbar_expect_tx(pg_smem(&sh.a_full[b]), tl_pages(a, seq, key0, to));
+                tl_load_pages(a, &map_rows, pg_smem(as + b * TL_BLOCK), pg_smem(&sh.a_full[b]), b * 64, seq, key0, to);
+            }
+            unsigned g = 0;
+            bool ok = true;
+            for (int h = h0; h < h1 && ok; h++)
+                for (int b = 0; b < blocks; b++, g++) {
+                    const unsigned slot = g % TE_STAGES, full = pg_smem(&sh.full[slot]), at = pg_smem(bs + slot * TE_STAGE);
+                    if (!(ok = tl_wait(pg_smem(&sh.empty[slot]), ((g / TE_STAGES) & 1u) ^ 1u, &sh.fail))) break;
+                    pg_mbar_expect_tx(full, (unsigned)width * 128);
+                    pg_tma_load_2d(at, &map_uk, full, b * 64, (t.head0 + h) * a.dim);
+                    pg_tma_load_2d(at + a.dim * 128, &map_uv, full, b * 64, (t.head0 + h) * a.vdim);
+                }
+            int never = 0;                                            // no copy is under way when the CTA ends
+            for (unsigned i = g > TE_STAGES ? g - TE_STAGES : 0; i < g; i++) tl_wait(pg_smem(&sh.full[i % TE_STAGES]), (i / TE_STAGES) & 1u, &never);
+            for (int b = 0; b < blocks; b++) tl_wait(pg_smem(&sh.a_full[b]), 0, &never);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const unsigned idesc = pg_instr_desc(128, width);
+            unsigned g = 0;
+            bool ok = true;
+            for (int h = h0; h < h1 && ok; h++) {
+                const unsigned n = (unsigned)(h - h0), acc = tmem + (n & 1u) * 256;
+                if (!(ok = tl_wait(pg_smem(&sh.acc_empty[n & 1u]), ((n >> 1) & 1u) ^ 1u, &sh.fail))) break;
+                for (int b = 0; b < blocks; b++, g++) {
+                    const unsigned slot = g % TE_STAGES;
+                    if (!(ok = tl_wait(pg_smem(&sh.a_full[b]), 0, &sh.fail) && tl_wait(pg_smem(&sh.full[slot]), (g / TE_STAGES) & 1u, &sh.fail))) break;
+                    pg_fence_after();
+                    const uint64_t x = pg_smem_desc(pg_smem(as + b * TL_BLOCK)), y = pg_smem_desc(pg_smem(bs + slot * TE_STAGE));
+                    for (int kk = 0; kk < min(4, (a.rank - b * 64) / 16); kk++) pg_umma_f16(acc, x + 2 * kk, y + 2 * kk, idesc, b > 0 || kk > 0);
+                    pg_umma_commit(pg_smem(&sh.empty[slot]));
+                }
+                if (ok) pg_umma_commit(pg_smem(&sh.acc_full[n & 1u]));
+            }
+            int never = 0;                                            // nothing of this CTA is in flight when its TMEM is given back
+            pg_umma_commit(pg_smem(&sh.drained));
+            tl_wait(pg_smem(&sh.drained), 0, &never);
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        // a lane a key, the two warps of its lanes every second run of 16 columns
+        const int q = warp & 3, row = q * 32 + lane;
+        const bool in = key0 + row < to;
+        for (int h = h0; h < h1; h++) {
+            const unsigned n = (unsigned)(h - h0);
+            if (!tl_wait_warp(pg_smem(&sh.acc_full[n & 1u]), (n >> 1) & 1u, &sh.fail)) break;
+            pg_fence_after();
+            const size_t image = (size_t)blockIdx.x * t.heads + h;
+            uint8_t *ki = t.k_image + image * ((a.dim + 63) >> 6) * TL_BLOCK, *vi = t.v_image + image * ((a.vdim + 63) >> 6) * TL_BLOCK;
+            for (int c = ((warp - 4) >> 2) * 16; c < width; c += 32) {
+                unsigned v[16], w[8];
+                sg_tmem16(tmem + (n & 1u) * 256 + ((unsigned)(q * 32) << 16) + c, v);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                // a cached row that is not finite makes all of its keys and values so: a NaN in a key reaches the queries that see it, a zero in its value no one
+                const bool is_k = c < a.dim;
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    asm volatile("" : "+r"(v[j]));
+                    if (!(fabsf(__uint_as_float(v[j])) < INFINITY)) v[j] = is_k ? 0x7fc00000u : 0u;
+                    if (!is_k && !in) v[j] = 0u;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++) w[j] = ht_pack_f16(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+                const int col = is_k ? c : c - a.dim;
+                uint8_t* at = (is_k ? ki : vi) + (col >> 6) * TL_BLOCK;
+                *(uint4*)(at + tl_at(row, (col & 63) >> 3)) = make_uint4(w[0], w[1], w[2], w[3]);
+                *(uint4*)(at + tl_at(row, ((col & 63) >> 3) + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
+            }
+            pg_fence_before();
+            sg_arrive(pg_smem(&sh.acc_empty[n & 1u]));
+        }
+    }
+    pg_fence_before();
+    __syncthreads();
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
+    tl_report(sh.fail, err_dev, err_host);
+}
+
+// ---- attention -----------------------------------------------------------------------------------------------------------------------------------------------
+struct TlShared {
+    unsigned long long q_full, full[TL_SLOTS], empty[TL_SLOTS], s_full[2], p_full[2], o_full[2], drained;
+    unsigned tmem_base;
+    int fail;
+};
+// B whose rows are the sum's index and whose columns (64 of them in 128 bytes) are the result's: blocks of 64 columns `block` bytes apart, groups of 8 rows 1024 bytes
+__device__ __forceinline__ uint64_t tl_desc_mn(unsigned addr, unsigned block) {
+    return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)(block >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+__device__ __forceinline__ void tl_umma_ts(unsigned d, unsigned a, uint64_t b, unsigned idesc, unsigned accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tl_store8(unsigned addr, const unsigned* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
+                 "r"(v[7]) : "memory");
+}
+typedef unsigned long long tl_f2;             // pairs of 32-bit numbers in one instruction
+__device__ __forceinline__ tl_f2 tl_two(float x, float y) {
+    tl_f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 tl_one(tl_f2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ tl_f2 tl_fma2(tl_f2 a, tl_f2 b, tl_f2 c) {
+    tl_f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ tl_f2 tl_add2(tl_f2 a, tl_f2 b) {
+    tl_f2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ tl_f2 tl_mul2(tl_f2 a, tl_f2 b) {
+    tl_f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// the largest of three, NaN if one of them is: a row that sees a score which is none has no result
+__device__ __forceinline__ float tl_max3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^x of a pair by multiply-adds: x = n + r with |r| <= 1/2 by way of a number whose last place is 1; 2^r by its series up to r^4 (the first term left out is 2^-14.5 at |r| = 1/2 before
+// its coefficients are fitted; see below), n into the exponent.  What is below -126 counts as -126
+__device__ __forceinline__ tl_f2 tl_exp2_pair(float2 x) {
+    const tl_f2 big = tl_two(12582912.0f, 12582912.0f), minus = tl_two(-1.0f, -1.0f);
+    const tl_f2 v = tl_two(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f)), u = tl_add2(v, big), n = tl_add2(u, tl_two(-12582912.0f, -12582912.0f)), r = tl_fma2(n, minus, v);
+    tl_f2 p = tl_two(1.3333558e-3f, 1.3333558e-3f);                  // (ln 2)^i / i!, i = 5 .. 0: the first term left out is 2^-19 at |r| = 1/2, far below the weights' 2^-11
+    p = tl_fma2(p, r, tl_two(9.6181291e-3f, 9.6181291e-3f));
+    p = tl_fma2(p, r, tl_two(5.5504109e-2f, 5.5504109e-2f));
+    p = tl_fma2(p, r, tl_two(2.4022651e-1f, 2.4022651e-1f));
+    p = tl_fma2(p, r, tl_two(6.9314718e-1f, 6.9314718e-1f));
+    p = tl_fma2(p, r, tl_two(1.0f, 1.0f));
+    const float2 q = tl_one(p), m = tl_one(u);
+    return tl_two(__uint_as_float(__float_as_uint(q.x) + (__float_as_uint(m.x) << 23)), __uint_as_float(__float_as_uint(q.y) + (__float_as_uint(m.y) << 23)));
+}
+// grid: items x heads, heads fastest
+__global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ TlArgs t, unsigned* err_dev,
+                                                                    unsigned* err_host) {
+    extern __shared__ __align__(1024) uint8_t tl_raw[];
+    __shared__ TlShared sh;
+    const LrArgs& a = t.a;
+    uint8_t *qs = (uint8_t*)(((uintptr_t)tl_raw + 1023) & ~(uintptr_t)1023), *ring = qs + 2 * TL_QBLOCKS * TL_BLOCK;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, item = (int)(blockIdx.x / (unsigned)t.heads), head_at = (int)(blockIdx.x - (unsigned)item * t.heads), head = t.head0 + head_at;
+    const int nb = (a.dim + 63) >> 6, rb = a.rest ? 1 : 0, vb = (a.vdim + 63) >> 6;      // blocks of keys, of r, of values
+    if (tid == 0) {
+        pg_mbar_init(pg_smem(&sh.q_full), 1);
+        for (int i = 0; i < TL_SLOTS; i++) { pg_mbar_init(pg_smem(&sh.full[i]), 1); pg_mbar_init(pg_smem(&sh.empty[i]), 1); }
+        for (int i = 0; i < 2; i++) { pg_mbar_init(pg_smem(&sh.s_full[i]), 1); pg_mbar_init(pg_smem(&sh.p_full[i]), 4); pg_mbar_init(pg_smem(&sh.o_full[i]), 1); }
+        pg_mbar_init(pg_smem(&sh.drained), 1);
+        sh.fail = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pg_smem(&sh.tmem_base)), "n"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pg_fence_before();
+    __syncthreads();
+    pg_fence_after();
+    const unsigned tmem = sh.tmem_base;
+    pdl_enter();
+    int rest;
+    const int seq = max(0, tl_find(a, item, [&](const PgSeq& s) { return tl_items(s, a); }, &rest));
+    const PgSeq s = a.seqs[seq];
+    const int row0 = (tl_items(s, a) - 1 - rest) * 2 * TL_ROWS;      // late rows, which see most, first
+    int from, to, before = 0;
+    tl_range(s, a, &from, &to);
+    for (int x = lane; x < seq; x += 32) before += tl_key_tiles(a.seqs[x], a);
+    before = warp_sum_i(before);
+    // the steps of a tile: keys that one of its rows sees, from `lo` for both
+    auto last = [&](int i) { return min(s.count, row0 + (i + 1) * TL_ROWS) - 1; };
+    const int lo = a.window > 0 ? max(from, (s.pos0 + row0 - a.window + 1) & ~(TL_KEYS - 1)) : from;
+    auto steps_of = [&](int i) { return row0 + i * TL_ROWS < s.count ? (s.pos0 + last(i) + 1 - lo + TL_KEYS - 1) / TL_KEYS : 0; };
+    const int steps0 = steps_of(0), steps1 = steps_of(1), steps = max(steps0, steps1), kt0 = before + (lo - from) / TL_KEYS, per = nb + rb + vb;
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TL_REGS_REST));
+        if (warp == 8) {
+            // ===== copies: Q, then the blocks of each step =====
+            if (lane == 0) {
+                const int width = a.dim + a.rest;
+                pg_mbar_expect_tx(pg_smem(&sh.q_full), (unsigned)(2 * (nb + rb) * TL_BLOCK));
+                for (int i = 0; i < 2; i++)
+                    for (int b = 0; b < nb + rb; b++)
+                        pg_tma_load_2d(pg_smem(qs + (i * TL_QBLOCKS + b) * TL_BLOCK), &map_q, pg_smem(&sh.q_full), head * width + (b < nb ? b * 64 : a.dim), s.first + row0 + i * TL_ROWS);
+                unsigned g = 0;
+                bool ok = true;
+                for (int k = 0; k < steps && ok; k++) {
+                    const size_t image = (size_t)(kt0 + k) * t.heads + head_at;
+                    for (int b = 0; b < per; b++, g++) {
+                        const unsigned slot = g % TL_SLOTS, full = pg_smem(&sh.full[slot]), at = pg_smem(ring + slot * TL_BLOCK);
+                        if (!(ok = tl_wait(pg_smem(&sh.empty[slot]), ((g / TL_SLOTS) & 1u) ^ 1u, &sh.fail))) break;
+                        if (b >= nb && b < nb + rb) {
+                            pg_mbar_expect_tx(full, tl_pages(a, seq, lo + k * TL_KEYS, to));
+                            tl_load_pages(a, &map_rows, at, full, a.rank, seq, lo + k * TL_KEYS, to);
+                        } else {
+                            const uint8_t* src = b < nb ? t.k_image + (image * nb + b) * TL_BLOCK : t.v_image + (image * vb + b - nb - rb) * TL_BLOCK;
+                            pg_mbar_expect_tx(full, TL_BLOCK);
+                            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(at), "l"(src), "r"(TL_BLOCK), "r"(full) : "memory");
+                        }
+                    }
+                }
+                int never = 0;                                        // no copy is under way when the CTA ends
+                for (unsigned i = g > TL_SLOTS ? g - TL_SLOTS : 0; i < g; i++) tl_wait(pg_smem(&sh.full[i % TL_SLOTS]), (i / TL_SLOTS) & 1u, &never);
+                tl_wait(pg_smem(&sh.q_full), 0, &never);
+            }
+            __syncwarp();
+        } else if (warp == 9) {
+            // ===== products: one thread =====
+            if (lane == 0) {
+                const unsigned idesc_s = pg_instr_desc(128, TL_KEYS), idesc_o = pg_instr_desc(128, a.vdim) | 1u << 16;
+                bool ok = tl_wait(pg_smem(&sh.q_full), 0, &sh.fail);
+                auto wait_blocks = [&](unsigned g, int n) {
+                    for (int b = 0; b < n && ok; b++, g++) ok = tl_wait(pg_smem(&sh.full[g % TL_SLOTS]), (g / TL_SLOTS) & 1u, &sh.fail);
+                    pg_fence_after();
+                };
+                auto free_blocks = [&](unsigned g, int n) {
+                    for (int b = 0; b < n; b++, g++) pg_umma_commit(pg_smem(&sh.empty[g % TL_SLOTS]));
+                };
+                auto scores = [&](int i, unsigned g) {               // of tile i against the keys in blocks g ..
+                    unsigned on = 0;
+                    for (int b = 0; b < nb + rb; b++, g++) {
+                        const uint64_t x = pg_smem_desc(pg_smem(qs + (i * TL_QBLOCKS + b) * TL_BLOCK)), y = pg_smem_desc(pg_smem(ring + (g % TL_SLOTS) * TL_BLOCK));
+                        for (int kk = 0; kk < min(4, (b < nb ? a.dim - b * 64 : a.rest) / 16); kk++, on = 1u) pg_umma_f16(tmem + i * 128, x + 2 * kk, y + 2 * kk, idesc_s, on);
+                    }
+                    pg_umma_commit(pg_smem(&sh.s_full[i]));
+                };
+                auto values = [&](int i, unsigned g, int k) {
+                    const unsigned v0 = pg_smem(ring + (g % TL_SLOTS) * TL_BLOCK), v1 = pg_smem(ring + ((g + 1) % TL_SLOTS) * TL_BLOCK);
+                    // the ring's blocks lie side by side, but for the last and the first
+                    for (int kk = 0; kk < TL_KEYS / 16; kk++) {
+                        if (vb == 1 || v1 == v0 + TL_BLOCK) tl_umma_ts(tmem + TL_O + i * 128, tmem + i * 128 + kk * 8, tl_desc_mn(v0 + kk * 2048, TL_BLOCK), idesc_o, k > 0 || kk > 0);
+                        else {
+                            tl_umma_ts(tmem + TL_O + i * 128, tmem + i * 128 + kk * 8, tl_desc_mn(v0 + kk * 2048, TL_BLOCK), pg_instr_desc(128, 64) | 1u << 16, k > 0 || kk > 0);
+                            tl_umma_ts(tmem + TL_O + i * 128 + 64, tmem + i * 128 + kk * 8, tl_desc_mn(v1 + kk * 2048, TL_BLOCK), pg_instr_desc(128, a.vdim - 64) | 1u << 16, k > 0 || kk > 0);
+                        }
+                    }
+                    pg_umma_commit(pg_smem(&sh.o_full[i]));
+                };
+                if (ok && steps > 0) {
+                    wait_blocks(0, nb + rb);
+                    if (ok && steps0 > 0) scores(0, 0);
+                    if (ok && steps1 > 0) scores(1, 0);
+                    free_blocks(0, nb + rb);
+                }
+                for (int k = 0; k < steps && ok; k++) {
+                    const unsigned gv = (unsigned)(k * per + nb + rb), gk = (unsigned)((k + 1) * per);
+                    wait_blocks(gv, vb);
+                    bool there = false;
+#pragma unroll 1
+                    for (int i = 0; i < 2 && ok; i++) {
+                        const int mine = i ? steps1 : steps0;
+                        if (k < mine) {
+                            if (!(ok = tl_wait(pg_smem(&sh.p_full[i]), k & 1, &sh.fail))) break;
+                            pg_fence_after();
+                            values(i, gv, k);
+                        }
+                        if (i == 1) free_blocks(gv, vb);
+                        if (k + 1 < mine) {
+                            if (!there) { wait_blocks(gk, nb + rb); there = true; }
+                            if (ok) scores(i, gk);
+                        }
+                    }
+                    if (ok && k + 1 < steps) free_blocks(gk, nb + rb);
+                }
+                int never = 0;                                        // nothing of this CTA is in flight when its TMEM is given back
+                pg_umma_commit(pg_smem(&sh.drained));
+                tl_wait(pg_smem(&sh.drained), 0, &never);
+            }
+            __syncwarp();
+        }
+    } else {
+        // ===== weights: a thread a row =====
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TL_REGS_SOFT));
+        const int i = warp >> 2, row = row0 + i * TL_ROWS + (warp & 3) * 32 + lane, mine = i ? steps1 : steps0, pos = s.pos0 + row, key_lo = a.window > 0 ? pos - a.window + 1 : 0;
+        const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, st = tmem + lanes + i * 128, ot = tmem + lanes + TL_O + i * 128;
+        const float f = a.scale * LR_LOG2E;
+        const int pos_first = s.pos0 + row0 + i * TL_ROWS, pos_last = s.pos0 + last(i);
+        float base = -INFINITY, l = 0.0f;
+        bool ok = true;
+#pragma unroll 1
+        for (int k = 0; k < mine; k++) {
+            const int key0 = lo + k * TL_KEYS;
+            ok = ok && tl_wait_warp(pg_smem(&sh.s_full[i]), k & 1, &sh.fail);
+            unsigned x[TL_KEYS];
+            if (ok) {
+                pg_fence_after();
+#pragma unroll
+                for (int c = 0; c < TL_KEYS; c += 16) sg_tmem16(st + c, *(unsigned(*)[16])(x + c));
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                for (int c = 0; c < TL_KEYS; c++) asm volatile("" : "+r"(x[c]));
+            }
+            // scores, each rounded once, so that their differences from the base end at 0
+#pragma unroll
+            for (int c = 0; c < TL_KEYS; c += 2) {
+                const float2 y = tl_one(tl_mul2(tl_two(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), tl_two(f, f)));
+                x[c] = __float_as_uint(y.x); x[c + 1] = __float_as_uint(y.y);
+            }
+            if (key0 + TL_KEYS - 1 > pos_first || (a.window > 0 && key0 < pos_last - a.window + 1)) {
+                const int c_lo = key_lo - key0, c_hi = pos - key0;
+#pragma unroll
+                for (int c = 0; c < TL_KEYS; c++)
+                    if (c > c_hi || c < c_lo) x[c] = 0xff800000u;
+            }
+            float mx = __uint_as_float(x[0]);
+#pragma unroll
+            for (int c = 1; c + 1 < TL_KEYS; c += 2) mx = tl_max3(mx, __uint_as_float(x[c]), __uint_as_float(x[c + 1]));
+            mx = tl_max3(mx, mx, __uint_as_float(x[TL_KEYS - 1]));
+            // the sums are scaled where a row's base has to follow its largest score
+            float alpha = 1.0f;
+            if (!(mx <= base + TL_LAG)) {
+                if (base != -INFINITY) alpha = lt_exp2(base - mx);
+                base = mx;
+            }
+            if (__any_sync(0xffffffffu, alpha != 1.0f)) {
+                if (k > 0 && ok) {
+                    ok = tl_wait_warp(pg_smem(&sh.o_full[i]), (k - 1) & 1, &sh.fail);
+                    pg_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < a.vdim && ok; c += 16) {
+                        unsigned v[16];
+                        sg_tmem16(ot + c, v);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                        for (int j = 0; j < 16; j++) {
+                            asm volatile("" : "+r"(v[j]));
+                            v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
+                        }
+                        tl_store8(ot + c, v); tl_store8(ot + c + 8, v + 8);
+                    }
+                }
+                l *= alpha;
+            }
+            const float minus = base == -INFINITY ? 0.0f : -base;
+            const tl_f2 minus2 = tl_two(minus, minus);
+            tl_f2 sum = 0ull;
+#pragma unroll
+            for (int g = 0; g < TL_KEYS; g += 16) {
+                unsigned w[8];
+#pragma unroll
+                for (int c = 0; c < 16; c += 2) {
+                    const float2 y = tl_one(tl_add2(tl_two(__uint_as_float(x[g + c]), __uint_as_float(x[g + c + 1])), minus2));
+                    const tl_f2 p = c >= TL_SFU ? tl_exp2_pair(y) : tl_two(lt_exp2(y.x), lt_exp2(y.y));
+                    sum = tl_add2(sum, p);
+                    const float2 z = tl_one(p);
+                    w[c / 2] = lt_pack(z.x, z.y);
+                }
+                if (ok) tl_store8(st + g / 2, w);
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            pg_fence_before();
+            sg_arrive(pg_smem(&sh.p_full[i]));
+            const float2 sums = tl_one(sum);
+            l += sums.x + sums.y;
+        }
+        if (mine > 0 && ok && (ok = tl_wait_warp(pg_smem(&sh.o_full[i]), (mine - 1) & 1, &sh.fail))) {
+            pg_fence_after();
+            float g = 1.0f, total = l;
+            if (a.sink) {
+                const float sk = a.sink[head] * LR_LOG2E, m2 = fmaxf(base, sk);
+                g = exp2f(base - m2);
+                total = g * l + (sk == -INFINITY ? 0.0f : exp2f(sk - m2));
+            }
+            const float by = base != base ? NAN : g / total;
+            uint16_t* out = (uint16_t*)a.out + ((int64_t)(s.first + row) * a.H + head) * a.vdim;
+#pragma unroll 1
+            for (int c = 0; c < a.vdim; c += 16) {
+                unsigned v[16], w[8];
+                sg_tmem16(ot + c, v);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                for (int j = 0; j < 16; j++) asm volatile("" : "+r"(v[j]));
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float u = __uint_as_float(v[2 * j]) * by, z = __uint_as_float(v[2 * j + 1]) * by;
+                    w[j] = a.out_bf16 ? ht_pack_bf16(u, z) : ht_pack_f16(u, z);
+                }
+                if (row < s.count) {
+                    *(uint4*)(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
+                    *(uint4*)(out + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                }
+            }
+        }
+    }
+    pg_fence_before();
+    __syncthreads();
+    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
+    tl_report(sh.fail, err_dev, err_host);
+}
+
+#define TL_WORKSPACE ((int64_t)256 << 20)     // bytes of images that a call has at a time, as long as those of one sequence and head are no more
+static int tl_run(cc_device* dev, const cc_page_plan* plan, const LrArgs& all) {
+    const int64_t per = (int64_t)((all.dim + 63) / 64 + (all.vdim + 63) / 64) * TL_BLOCK, width = all.dim + all.rest;
+    CUtensorMap rows, q, uk, uv;
+    int rc = cc_make_tmap_rows(dev, &rows, all.rows, plan->n_pages * plan->page, all.cols, (int64_t)all.cols * 2, plan->page, false);
+    if (!rc) rc = cc_make_tmap_rows(dev, &q, all.q, plan->tokens, all.H * width, all.H * width * 2, TL_ROWS, false);
+    if (!rc) rc = cc_make_tmap_rows(dev, &uk, all.uk, (int64_t)all.H * all.dim, all.rank, (int64_t)all.rank * 2, all.dim, false);
+    if (!rc) rc = cc_make_tmap_rows(dev, &uv, all.uv, (int64_t)all.H * all.vdim, all.rank, (int64_t)all.rank * 2, all.vdim, false);
+    if (rc) return rc;
+    CC_CUDA(dev, cudaFuncSetAttribute(latent_expand_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TE_SMEM));
+    CC_CUDA(dev, cudaFuncSetAttribute(latent_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TL_SMEM));
+    // as many sequences at a time as have their images of one head in TL_WORKSPACE, and as many heads
+    for (int first = 0, end; first < plan->n_seqs; first = end) {
+        TlArgs t{};
+        t.a = all;
+        int64_t tiles = 0, items = 0;
+        for (end = first; end < plan->n_seqs; end++) {
+            const int n = tl_key_tiles(plan->seqs[end], all);
+            if (tiles && (tiles + n) * per > TL_WORKSPACE) break;
+            tiles += n; items += tl_items(plan->seqs[end], all);
+        }
+        if (!items) continue;
+        t.a.seqs = plan->d_seqs + first; t.a.n_seqs = end - first; t.a.table = plan->d_table + (int64_t)first * all.table_cols;
+        const int heads = (int)std::max<int64_t>(1, std::min<int64_t>(all.H, TL_WORKSPACE / (tiles * per)));
+        CC_REQUIRE(dev, items * heads < ((int64_t)1 << 31) && tiles < ((int64_t)1 << 31), "paged_latent_attention: too many rows");
+        void* ws = nullptr; size_t cls = 0;
+        rc = cc_pool_alloc(dev, (size_t)(tiles * heads * per), &ws, &cls);
+        if (rc) return rc;
+        t.k_image = (uint8_t*)ws; t.v_image = t.k_image + tiles * heads * ((all.dim + 63) / 64) * TL_BLOCK;
+        t.key_tiles = (int)tiles; t.items = (int)items;
+        cudaError_t e = cudaSuccess;
+        for (t.head0 = 0; t.head0 < all.H && e == cudaSuccess; t.head0 += heads) {
+            t.heads = std::min(heads, all.H - t.head0);
+            const int runs = (int)std::max<int64_t>(1, std::min<int64_t>(t.heads, dev->sm_count / tiles));
+            e = cc_launch_pdl(dev, latent_expand_kernel, dim3((unsigned)tiles, (unsigned)runs), TE_THREADS, TE_SMEM, rows, uk, uv, t, dev->err_dev, dev->err_host);
+            if (e == cudaSuccess) e = cc_launch_pdl(dev, latent_tile_kernel, (unsigned)(items * t.heads), TL_THREADS, TL_SMEM, rows, q, t, dev->err_dev, dev->err_host);
+            dev->launches += 2;
+        }
+        cc_pool_free(dev, ws, cls);
+        if (e != cudaSuccess) return cc_fail(dev, CC_ERR_CUDA, "paged_latent_attention: %s", cudaGetErrorString(e));
+    }
+    return CC_OK;
+}

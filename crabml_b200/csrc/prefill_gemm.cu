@@ -432,6 +432,16 @@ static int pg_make_tmap(cc_device* dev, CUtensorMap* tm, const void* base, int64
     return CC_OK;
 }
 
+// rows of 16-bit numbers any multiple of 16 bytes apart, box 64 columns x box_rows rows, 128-byte swizzle, out of bounds read as zero
+int cc_make_tmap_rows(cc_device* dev, void* tm, const void* base, int64_t rows, int64_t cols, int64_t stride_bytes, int box_rows, bool bf16) {
+    PFN_encodeTiled enc = pg_encode();
+    if (!enc) return cc_fail(dev, CC_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride_bytes};
+    cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    const CUresult r = enc((CUtensorMap*)tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, (void*)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? CC_OK : cc_fail(dev, CC_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+}
 int cc_make_tmap_i8(cc_device* dev, void* tm, const void* base, int64_t rows, int64_t k, int box_rows) { return pg_make_tmap(dev, (CUtensorMap*)tm, base, rows, k, box_rows, false, 1); }
 int cc_make_tmap_bf16(cc_device* dev, void* tm, const void* base, int64_t rows, int64_t k, int box_rows) { return pg_make_tmap(dev, (CUtensorMap*)tm, base, rows, k, box_rows, true); }
 

@@ -15,7 +15,7 @@ struct PrArgs {
     void* out;
     int64_t x_stride, res_stride;
     int m, k, rows, x_type, out_type, act, chunk;
-    bool x_vec, w_vec;
+    bool x_vec, w_vec;                        // rows start at multiples of 16 bytes
 };
 __device__ __forceinline__ float pr_finish(const PrArgs& a, float v, int row, int col) {
     if (a.bias) v += a.bias[col];
@@ -42,6 +42,7 @@ __device__ __forceinline__ uint4 pr_pack8(const float (&v)[8]) {
 #define PF_THREADS (PF_WARPS * 32)
 #define PF_AHEAD 4                            // runs of 32 k that a warp has under way
 #define PF_SMEM (160 * 1024)
+#define PF_ROWS 32                            // rows of x; more go to the tensor cores' tiles
 // 8 numbers of a row from column c on, zeros behind its end
 __device__ __forceinline__ uint4 pf_weights(const uint16_t* row, int c, int k, bool there, bool vec) {
     if (!there || c >= k) return make_uint4(0, 0, 0, 0);
@@ -55,12 +56,12 @@ __device__ __forceinline__ uint4 pf_weights(const uint16_t* row, int c, int k, b
         if (c + j < k) u[j >> 1] |= (unsigned)row[c + j] << (j & 1) * 16;
     return make_uint4(u[0], u[1], u[2], u[3]);
 }
-// grid (tiles of 16 rows of W, groups of 8 NT rows of x); the rows of x lie in shared memory, `chunk` of their k at a time
+// grid: tiles of 16 rows of W; the (up to 8 NT) rows of x lie in shared memory, `chunk` of their k at a time
 template <int NT, bool BF16>
 __global__ void __launch_bounds__(PF_THREADS) product_few_kernel(const __grid_constant__ PrArgs a) {
     extern __shared__ __align__(16) uint8_t pf_raw[];
     __shared__ float sums[PF_WARPS][16][NT * 8 + 1];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, m0 = blockIdx.x * 16, n0 = blockIdx.y * NT * 8, pitch = a.chunk * 2 + 64;      // eight lanes' 16 bytes: two rows, 64 bytes each, in all banks
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, m0 = blockIdx.x * 16, pitch = a.chunk * 2 + 64;      // eight lanes' 16 bytes: two rows, 64 bytes each, in all banks
     pdl_enter();
     const uint16_t *w0 = (const uint16_t*)a.w + (int64_t)(m0 + (lane >> 2)) * a.k, *w1 = w0 + (int64_t)8 * a.k;
     const bool in0 = m0 + (lane >> 2) < a.m, in1 = m0 + (lane >> 2) + 8 < a.m;
@@ -80,8 +81,8 @@ __global__ void __launch_bounds__(PF_THREADS) product_few_kernel(const __grid_co
         for (int e = tid; e < NT * 8 * runs * 4; e += PF_THREADS) {
             const int r = e / (runs * 4), c = e % (runs * 4) * 8;
             float x[8] = {};
-            if (n0 + r < a.rows && k0 + c < a.k) {
-                const int64_t at = (int64_t)(n0 + r) * a.x_stride + k0 + c;
+            if (r < a.rows && k0 + c < a.k) {
+                const int64_t at = (int64_t)r * a.x_stride + k0 + c;
                 if (k0 + c + 8 <= a.k) ht_read8(a.x, at, a.x_type, a.x_vec, x);
                 else
 #pragma unroll
@@ -118,11 +119,11 @@ __global__ void __launch_bounds__(PF_THREADS) product_few_kernel(const __grid_co
         for (int j = 0; j < 4; j++) sums[warp][(lane >> 2) + (j >> 1) * 8][n * 8 + (lane & 3) * 2 + (j & 1)] = total[n][j];
     __syncthreads();
     for (int e = tid; e < 16 * NT * 8; e += PF_THREADS) {
-        const int i = e & 15, n = e >> 4, col = m0 + i, row = n0 + n;
+        const int i = e & 15, n = e >> 4, col = m0 + i;
         float s = 0.0f;
 #pragma unroll
         for (int w = 0; w < PF_WARPS; w++) s += sums[w][i][n];
-        if (col < a.m && row < a.rows) ht_write(a.out, (int64_t)row * a.m + col, a.out_type, pr_finish(a, s, row, col));
+        if (col < a.m && n < a.rows) ht_write(a.out, (int64_t)n * a.m + col, a.out_type, pr_finish(a, s, n, col));
     }
 }
 template <int NT>
@@ -130,9 +131,106 @@ static cudaError_t pf_launch(cc_device* dev, PrArgs a, bool bf16) {
     auto kernel = bf16 ? product_few_kernel<NT, true> : product_few_kernel<NT, false>;
     a.chunk = std::min((a.k + 63) / 64 * 64, (PF_SMEM / (NT * 8) - 64) / 128 * 64);
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PF_SMEM);
-    if (e == cudaSuccess) e = cc_launch_pdl(dev, kernel, dim3((unsigned)((a.m + 15) / 16), (unsigned)((a.rows + NT * 8 - 1) / (NT * 8))), PF_THREADS, (size_t)NT * 8 * (a.chunk * 2 + 64), a);
+    if (e == cudaSuccess) e = cc_launch_pdl(dev, kernel, (unsigned)((a.m + 15) / 16), PF_THREADS, (size_t)NT * 8 * (a.chunk * 2 + 64), a);
     dev->launches++;
     return e;
+}
+
+#include "product_tile.cuh"
+
+// rows of any of the types and any stride -> rows of `to` 16-bit numbers, zeros behind their k: what TMA can read
+template <bool BF16>
+__global__ void __launch_bounds__(256) product_rows_kernel(const void* __restrict__ x, int64_t stride, int type, int vec, int k, int to, int64_t n8, uint4* __restrict__ out) {
+    pdl_enter();
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n8) return;
+    const int64_t row = i / (to / 8);
+    const int c = (int)(i - row * (to / 8)) * 8;
+    float v[8] = {};
+    if (c + 8 <= k) ht_read8(x, row * stride + c, type, vec, v);
+    else
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (c + j < k) v[j] = ht_read(x, row * stride + c + j, type);
+    out[i] = pr_pack8<BF16>(v);
+}
+static cudaError_t pr_rows(cc_device* dev, bool bf16, const void* x, int64_t stride, int type, bool vec, int64_t rows, int k, int to, void* out) {
+    const int64_t n8 = rows * (to / 8);
+    dev->launches++;
+    return cc_launch_pdl(dev, bf16 ? product_rows_kernel<true> : product_rows_kernel<false>, (unsigned)((n8 + 255) / 256), 256, 0, x, stride, type, (int)vec, k, to, n8, (uint4*)out);
+}
+template <int BN, bool BF16, bool DRAIN>
+static int pt_launch(cc_device* dev, const PrArgs& a, const void* w, const void* x, int64_t x_stride, int kp) {
+    CUtensorMap mw, mx;
+    int rc = cc_make_tmap_rows(dev, &mw, w, a.m, a.k, (int64_t)kp * 2, 128, BF16);
+    if (!rc) rc = cc_make_tmap_rows(dev, &mx, x, a.rows, a.k, x_stride * 2, BN, BF16);
+    if (rc) return rc;
+    const int64_t tiles = (int64_t)((a.m + 127) / 128) * ((a.rows + BN - 1) / BN);
+    const int steps = (a.k + 63) / 64;
+    int parts = 1;
+    while (parts < 4 && tiles * parts * 2 <= dev->sm_count && steps / (parts * 2) >= 2) parts *= 2;
+    CC_REQUIRE(dev, tiles < ((int64_t)1 << 30), "product: %lld tiles", (long long)tiles);
+    auto kernel = product_tile_kernel<BN, BF16, DRAIN>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(parts > 1 ? tiles * parts : std::min<int64_t>(tiles, dev->sm_count)));
+    cfg.blockDim = dim3(PT_THREADS); cfg.dynamicSmemBytes = pt_smem(BN, false); cfg.stream = dev->stream;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = dev->pdl ? 1 : 0;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)parts; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = 2;
+    CC_CUDA(dev, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pt_smem(BN, false)));
+    CC_CUDA(dev, cudaLaunchKernelEx(&cfg, kernel, mw, mx, a, steps, (int)tiles, parts, dev->err_dev, dev->err_host));
+    CC_LAUNCH_CHECK(dev);
+    return CC_OK;
+}
+template <bool BF16, bool DRAIN>
+static int pt_launch_pair(cc_device* dev, const PrArgs& a, const void* w, const void* x, int64_t x_stride, int kp) {
+    const int64_t tiles = (int64_t)((a.m + 255) / 256) * ((a.rows + 255) / 256);
+    CC_REQUIRE(dev, tiles < ((int64_t)1 << 30), "product: %lld tiles", (long long)tiles);
+    const int pairs = dev->sm_count / 2, rest = (int)(tiles % pairs), whole = (int)tiles - rest;
+    int cut = 1;
+    while (cut < 8 && rest * cut * 2 <= pairs) cut *= 2;
+    CUtensorMap mw, mx, mc;
+    int rc = cc_make_tmap_rows(dev, &mw, w, a.m, a.k, (int64_t)kp * 2, 128, BF16);
+    if (!rc) rc = cc_make_tmap_rows(dev, &mx, x, a.rows, a.k, x_stride * 2, 128, BF16);
+    if (!rc) rc = cc_make_tmap_rows(dev, &mc, x, a.rows, a.k, x_stride * 2, 128 / cut, BF16);
+    if (rc) return rc;
+    auto kernel = product_pair_kernel<BF16, DRAIN>;
+    CC_CUDA(dev, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pt_smem(256, true)));
+    CC_CUDA(dev, cc_launch_pdl(dev, kernel, (unsigned)(2 * std::min(whole + rest * cut, pairs)), PT_THREADS, pt_smem(256, true), mw, mx, mc, a, (a.k + 63) / 64, whole, cut, whole + rest * cut,
+                               dev->err_dev, dev->err_host));
+    dev->launches++;
+    return CC_OK;
+}
+template <bool BF16, bool DRAIN>
+static int pt_tiles(cc_device* dev, const PrArgs& a, const void* w, const void* x, int64_t x_stride, int kp) {
+    if (a.rows > 128 && dev->sm_count > 1 && (int64_t)((a.m + 255) / 256) * ((a.rows + 255) / 256) >= dev->sm_count / 2) return pt_launch_pair<BF16, DRAIN>(dev, a, w, x, x_stride, kp);
+    return a.rows <= 32 ? pt_launch<32, BF16, DRAIN>(dev, a, w, x, x_stride, kp) : a.rows <= 64 ? pt_launch<64, BF16, DRAIN>(dev, a, w, x, x_stride, kp)
+           : a.rows <= 128 ? pt_launch<128, BF16, DRAIN>(dev, a, w, x, x_stride, kp) : pt_launch<256, BF16, DRAIN>(dev, a, w, x, x_stride, kp);
+}
+static int pr_many(cc_device* dev, const PrArgs& a, bool bf16) {
+    // operands that TMA cannot read, or x of another type, are laid out first
+    const int kp = (a.k + 7) / 8 * 8, type = bf16 ? CC_BF16 : CC_F16;
+    const bool copy_w = kp != a.k || ((uintptr_t)a.w & 15), copy_x = kp != a.k || a.x_type != type || !a.x_vec;
+    const size_t wb = copy_w ? (size_t)a.m * kp * 2 : 0, xb = copy_x ? (size_t)a.rows * kp * 2 : 0;
+    void* mem = nullptr; size_t cls = 0;
+    if (wb + xb) {
+        const int rc = cc_pool_alloc(dev, wb + xb, &mem, &cls);
+        if (rc) return rc;
+    }
+    const void *w = a.w, *x = a.x;
+    int64_t x_stride = a.x_stride;
+    cudaError_t e = cudaSuccess;
+    if (copy_w) { e = pr_rows(dev, bf16, a.w, a.k, type, a.w_vec, a.m, a.k, kp, mem); w = mem; }
+    if (copy_x && e == cudaSuccess) { x = (uint8_t*)mem + wb; e = pr_rows(dev, bf16, a.x, a.x_stride, a.x_type, a.x_vec, a.rows, a.k, kp, (void*)x); x_stride = kp; }
+    int rc = e == cudaSuccess ? CC_OK : cc_fail(dev, CC_ERR_CUDA, "product: %s", cudaGetErrorString(e));
+    const bool drain = a.out_type == CC_F32;
+    if (!rc) rc = bf16 ? (drain ? pt_tiles<true, true>(dev, a, w, x, x_stride, kp) : pt_tiles<true, false>(dev, a, w, x, x_stride, kp))
+                       : (drain ? pt_tiles<false, true>(dev, a, w, x, x_stride, kp) : pt_tiles<false, false>(dev, a, w, x, x_stride, kp));
+    if (mem) cc_pool_free(dev, mem, cls);
+    return rc;
 }
 
 extern "C" CC_API int cc_product(cc_device* dev, const cc_view* w, const cc_view* x, const cc_view* bias, int32_t act, const cc_view* residual, int32_t out_type, cc_buf** out) {
@@ -168,8 +266,11 @@ extern "C" CC_API int cc_product(cc_device* dev, const cc_view* w, const cc_view
         a.out = o->base; a.x_stride = x->strides[0]; a.res_stride = residual ? residual->strides[0] : 0; a.m = (int)m; a.k = (int)k; a.rows = (int)T;
         a.x_type = x->buf->dtype; a.out_type = out_type; a.act = act;
         a.w_vec = k % 8 == 0 && ((uintptr_t)a.w & 15) == 0; a.x_vec = a.x_stride * ht_size(a.x_type) % 16 == 0 && ((uintptr_t)a.x & 15) == 0;
-        const cudaError_t e = T <= 8 ? pf_launch<1>(dev, a, bf16) : T <= 16 ? pf_launch<2>(dev, a, bf16) : pf_launch<4>(dev, a, bf16);
-        if (e != cudaSuccess) rc = cc_fail(dev, CC_ERR_CUDA, "product: %s", cudaGetErrorString(e));
+        if (T > PF_ROWS) rc = pr_many(dev, a, bf16);
+        else {
+            const cudaError_t e = T <= 8 ? pf_launch<1>(dev, a, bf16) : T <= 16 ? pf_launch<2>(dev, a, bf16) : pf_launch<4>(dev, a, bf16);
+            if (e != cudaSuccess) rc = cc_fail(dev, CC_ERR_CUDA, "product: %s", cudaGetErrorString(e));
+        }
     }
     if (rc) { cc_tensor_release(o); return rc; }
     *out = o;

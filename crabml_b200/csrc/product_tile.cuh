@@ -1,0 +1,406 @@
+// product_tile.cuh -- products of many rows on tcgen05.mma with bias, activation and residual in their epilogue.  Included by product.cu.
+//
+// Tiles of 128 output channels x BN rows of x (product_tile_kernel), or, where there are enough of them, of 256 x 256 for a pair of SMs (product_pair_kernel): each holds 128 channels and half of
+// the rows of a step, the pair's instruction reads both halves, so that a step brings 32 KB to an SM instead of 48.  TMA stages steps of 64 k, one thread issues the products, the sums lie
+// twice in TMEM, so that 8 warps finish a tile while the next one is under way; a warp's lanes are consecutive channels, which a row of the result has side by side.
+//
+// DRAIN (32-bit results): the tensor cores cut a sum off at 24 bits after every 16 terms.  Over 14336 terms that is 1e-5 of a result and more; so sums of 64 * PT_DRAIN terms leave TMEM for
+// registers, are rounded there, and the whole sum goes back for the epilogue.  16-bit results are rounded 2^9 times more coarsely.
+//
+// Every wait is bounded (sg_wait): on expiry the CTA raises `fail`, all roles leave their loops, TMEM is freed and the host reports it.
+#pragma once
+#include <cooperative_groups.h>
+#include <cuda.h>
+
+#include "split_gemm.cuh"
+
+#define PT_THREADS 384
+#define PT_WORKERS 8                          // warps that finish: the first four the left half of a tile's rows of x, the others the right one
+#define PT_DRAIN 4                            // steps of a sum that leaves for registers
+#define PT_STEP 128                           // bytes of a row in a step
+struct PtShared {
+    unsigned long long full[8], empty[8], acc_full[2], acc_empty[2], drained;
+    unsigned tmem_base;
+    int fail;
+};
+__host__ __device__ constexpr int pt_bytes(int bn, bool pair) { return (128 + (pair ? bn / 2 : bn)) * PT_STEP; }
+__host__ __device__ constexpr int pt_stages(int bn, bool pair) { return 192 * 1024 / pt_bytes(bn, pair) < 8 ? 192 * 1024 / pt_bytes(bn, pair) : 8; }
+__host__ __device__ constexpr size_t pt_smem(int bn, bool pair) { return (size_t)pt_stages(bn, pair) * pt_bytes(bn, pair) + 1024; }
+
+__device__ __forceinline__ void pt_load16(unsigned addr, unsigned (&v)[16]) {
+    sg_tmem16(addr, v);
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 16; i++) asm volatile("" : "+r"(v[i]));      // nothing is done with them before
+}
+__device__ __forceinline__ void pt_store16(unsigned addr, const float* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
+                 "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]) : "memory");
+}
+// Sums of this thread's COLS columns over the chunks of a tile: all but the last are read out and handed back, the last one's buffer gets the whole sum.  false: a wait ran out
+template <int COLS, class Release>
+__device__ __forceinline__ bool pt_collect(PtShared& sh, unsigned tmem, int bn, unsigned& nth, int chunks, unsigned lane_col, Release release) {
+    float acc[COLS];
+#pragma unroll
+    for (int i = 0; i < COLS; i++) acc[i] = 0.0f;
+    for (int c = 0; c < chunks; c++, nth++) {
+        if (!sg_wait_warp(pg_smem(&sh.acc_full[nth & 1u]), (nth >> 1) & 1u, &sh.fail)) return false;
+        pg_fence_after();
+        const unsigned from = tmem + (nth & 1u) * (unsigned)bn + lane_col;
+#pragma unroll
+        for (int i = 0; i < COLS; i += 16) {
+            unsigned v[16];
+            pt_load16(from + i, v);
+#pragma unroll
+            for (int j = 0; j < 16; j++) acc[i + j] += __uint_as_float(v[j]);
+        }
+        if (c + 1 < chunks) release(nth);
+        else {
+#pragma unroll
+            for (int i = 0; i < COLS; i += 16) pt_store16(from + i, acc + i);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            break;                                                    // (nth: the last one's)
+        }
+    }
+    return true;
+}
+// bias, activation, residual and rounding of 16 rows n0 .. of x at channel col; v: their sums
+template <class Act>
+__device__ __forceinline__ void pt_finish16(const PrArgs& a, const unsigned (&v)[16], int n0, int n_end, int col, float bias, Act act) {
+    float res[16];
+    if (a.res) {
+#pragma unroll
+        for (int j = 0; j < 16; j++) res[j] = n0 + j < n_end && col < a.m ? ht_read(a.res, (int64_t)(n0 + j) * a.res_stride + col, a.out_type) : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+        float y = act(__uint_as_float(v[j]) + bias);
+        if (a.res) y += res[j];
+        if (n0 + j < n_end && col < a.m) ht_write(a.out, (int64_t)(n0 + j) * a.m + col, a.out_type, y);
+    }
+}
+// with the activation as a function that is known: each has its own loop
+template <class Body>
+__device__ __forceinline__ void pt_with_act(int act, Body body) {
+    switch (act) {
+    case CC_ACT_NONE: body([](float z) { return z; }); break;
+    case CC_ACT_GELU_TANH: body([](float z) { return act_gelu_tanh(z); }); break;
+    case CC_ACT_SIGMOID: body([](float z) { return act_sigmoid(z); }); break;
+    case CC_ACT_RELU_SQUARED: body([](float z) { return act_relu_squared(z); }); break;
+    default: body([](float z) { return act_silu(z); });               // SWISH with alpha 1
+    }
+}
+__device__ __forceinline__ void pt_report(const PtShared& sh, unsigned* err_dev, unsigned* err_host) {
+    if (threadIdx.x == 0 && sh.fail) {
+        if (err_dev) atomicExch(err_dev, 5u);
+        if (err_host) { *(volatile unsigned*)err_host = 5u; __threadfence_system(); }
+    }
+}
+
+// a CTA walks over the tiles of its cluster; the `parts` CTAs of a cluster share a tile's depth (then there is one tile for each cluster), and each finishes every parts-th run of 16 rows of x
+// with the sums of all, in the order of the parts
+template <int BN, bool BF16, bool DRAIN>
+__global__ void __launch_bounds__(PT_THREADS, 1) product_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ PrArgs a, int steps_all, int n_tiles,
+                                                                     int parts, unsigned* err_dev, unsigned* err_host) {
+    namespace cg = cooperative_groups;
+    constexpr int ST = pt_stages(BN, false), HALF = BN / 2;
+    constexpr unsigned A_BYTES = 128 * PT_STEP, BYTES = pt_bytes(BN, false), COLS = 2 * BN;
+    extern __shared__ __align__(1024) uint8_t pt_raw[];
+    __shared__ PtShared sh;
+    uint8_t* ring = (uint8_t*)(((uintptr_t)pt_raw + 1023) & ~(uintptr_t)1023);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int part = parts > 1 ? (int)cg::this_cluster().block_rank() : 0;
+    const int s0 = (int)((int64_t)steps_all * part / parts), steps = (int)((int64_t)steps_all * (part + 1) / parts) - s0, chunk = DRAIN ? PT_DRAIN : steps, chunks = (steps + chunk - 1) / chunk;
+    const int tiles_n = (a.rows + BN - 1) / BN, first = blockIdx.x / parts, stride = gridDim.x / parts;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < ST; i++) { pg_mbar_init(pg_smem(&sh.full[i]), 1); pg_mbar_init(pg_smem(&sh.empty[i]), 1); }
+        for (int i = 0; i < 2; i++) { pg_mbar_init(pg_smem(&sh.acc_full[i]), 1); pg_mbar_init(pg_smem(&sh.acc_empty[i]), PT_WORKERS); }
+        pg_mbar_init(pg_smem(&sh.drained), 1);
+        sh.fail = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pg_smem(&sh.tmem_base)), "n"(COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pg_fence_before();
+    __syncthreads();
+    pg_fence_after();
+    const unsigned tmem = sh.tmem_base;
+    pdl_enter();
+    if (warp == 0) {
+        if (lane == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
+            unsigned g = 0;
+            bool ok = true;
+            for (int tile = first; tile < n_tiles && ok; tile += stride) {
+                const int mt = tile / tiles_n, nt = tile - mt * tiles_n;
+                for (int s = 0; s < steps; s++, g++) {
+                    const unsigned slot = g % ST, full = pg_smem(&sh.full[slot]), at = pg_smem(ring + (size_t)slot * BYTES);
+                    if (!(ok = sg_wait(pg_smem(&sh.empty[slot]), ((g / ST) & 1u) ^ 1u, &sh.fail))) break;
+                    pg_mbar_expect_tx(full, BYTES);
+                    pg_tma_load_2d(at, &map_w, full, (s0 + s) * 64, mt * 128);
+                    pg_tma_load_2d(at + A_BYTES, &map_x, full, (s0 + s) * 64, nt * BN);
+                }
+            }
+            int never = 0;                                            // no copy is under way when the CTA ends
+            for (unsigned i = g > ST ? g - ST : 0; i < g; i++) sg_wait(pg_smem(&sh.full[i % ST]), (i / ST) & 1u, &never);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr unsigned idesc = pg_instr_desc(128, BN, BF16 ? 1 : 0);
+            unsigned g = 0, nth = 0;
+            bool ok = true;
+            for (int tile = first; tile < n_tiles && ok; tile += stride)
+                for (int s = 0; s < steps && ok; s++, g++) {
+                    const unsigned acc = tmem + (nth & 1u) * BN;
+                    if (s % chunk == 0) {
+                        if (!(ok = sg_wait(pg_smem(&sh.acc_empty[nth & 1u]), ((nth >> 1) & 1u) ^ 1u, &sh.fail))) break;
+                        pg_fence_after();
+                    }
+                    const unsigned slot = g % ST, at = pg_smem(ring + (size_t)slot * BYTES);
+                    if (!(ok = sg_wait(pg_smem(&sh.full[slot]), (g / ST) & 1u, &sh.fail))) break;
+                    pg_fence_after();
+                    const uint64_t x = pg_smem_desc(at), y = pg_smem_desc(at + A_BYTES);
+#pragma unroll
+                    for (int kk = 0; kk < 4; kk++) pg_umma_f16(acc, x + 2 * kk, y + 2 * kk, idesc, s % chunk > 0 || kk > 0);
+                    pg_umma_commit(pg_smem(&sh.empty[slot]));
+                    if (s % chunk == chunk - 1 || s == steps - 1) pg_umma_commit(pg_smem(&sh.acc_full[nth++ & 1u]));
+                }
+            int never = 0;                                            // nothing of this CTA is in flight when its TMEM is given back
+            pg_umma_commit(pg_smem(&sh.drained));
+            sg_wait(pg_smem(&sh.drained), 0, &never);
+        }
+        __syncwarp();
+    }
+    const int q = warp & 3, half = (warp - 4) >> 2;
+    const unsigned lane_col = ((unsigned)(q * 32) << 16) + half * HALF;
+    auto release = [&](unsigned n) {
+        pg_fence_before();
+        sg_arrive(pg_smem(&sh.acc_empty[n & 1u]));
+    };
+    auto collect = [&](unsigned& nth) {                               // the tile's sums are in the buffer of chunk nth
+        if (DRAIN) return pt_collect<HALF>(sh, tmem, BN, nth, chunks, lane_col, release);
+        if (!sg_wait_warp(pg_smem(&sh.acc_full[nth & 1u]), (nth >> 1) & 1u, &sh.fail)) return false;
+        pg_fence_after();
+        return true;
+    };
+    if (warp >= 4 && parts == 1) {
+        unsigned nth = 0;
+        for (int tile = first; tile < n_tiles; tile += stride, nth++) {
+            const int mt = tile / tiles_n, n0 = (tile - mt * tiles_n) * BN + half * HALF, col = mt * 128 + q * 32 + lane;
+            if (!collect(nth)) break;
+            const unsigned from = tmem + (nth & 1u) * BN + lane_col;
+            const float bias = a.bias && col < a.m ? a.bias[col] : 0.0f;
+            pt_with_act(a.act, [&](auto act) {
+#pragma unroll 1
+                for (int c0 = 0; c0 < HALF && n0 + c0 < a.rows; c0 += 16) {
+                    unsigned v[16];
+                    pt_load16(from + c0, v);
+                    pt_finish16(a, v, n0 + c0, a.rows, col, bias, act);
+                }
+            });
+            release(nth);
+        }
+    }
+    if (parts > 1) {
+        cg::cluster_group cluster = cg::this_cluster();
+        const int mt = first / tiles_n, n0 = (first - mt * tiles_n) * BN + half * HALF, col = mt * 128 + q * 32 + lane;
+        unsigned nth = 0;
+        if (warp >= 4) collect(nth);
+        const unsigned from = tmem + (nth & 1u) * BN + lane_col;
+        __syncthreads();
+        cluster.sync();                                               // every CTA's products are done: the rings are free
+        // [sender][run of the owner][half][row of x][channel]
+        constexpr int RUNS = HALF / 16;
+        auto box = [&](int sender, int owner, int run) { return ((((size_t)(sender < owner ? sender : sender - 1) * ((RUNS + parts - 1) / parts) + run / parts) * 2 + half) * 16) * 128 + q * 32 + lane; };
+        if (warp >= 4) {
+#pragma unroll 1
+            for (int run = 0; run < RUNS && n0 + run * 16 < a.rows; run++) {
+                const int owner = run % parts;
+                if (owner == part) continue;
+                unsigned v[16];
+                pt_load16(from + run * 16, v);
+                float* to = cluster.map_shared_rank((float*)ring, owner) + box(part, owner, run);
+#pragma unroll
+                for (int j = 0; j < 16; j++) to[j * 128] = __uint_as_float(v[j]);
+            }
+        }
+        cluster.sync();
+        if (warp >= 4 && !*(volatile int*)&sh.fail) {
+            const float bias = a.bias && col < a.m ? a.bias[col] : 0.0f;
+            pt_with_act(a.act, [&](auto act) {
+#pragma unroll 1
+                for (int run = part; run < RUNS && n0 + run * 16 < a.rows; run += parts) {
+                    unsigned v[16];
+                    float sum[16];
+                    pt_load16(from + run * 16, v);
+#pragma unroll
+                    for (int j = 0; j < 16; j++) sum[j] = 0.0f;
+                    for (int p = 0; p < parts; p++) {
+                        const float* o = (const float*)ring + (p == part ? 0 : box(p, part, run));
+#pragma unroll
+                        for (int j = 0; j < 16; j++) sum[j] += p == part ? __uint_as_float(v[j]) : o[j * 128];
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; j++) v[j] = __float_as_uint(sum[j]);
+                    pt_finish16(a, v, n0 + run * 16, a.rows, col, bias, act);
+                }
+            });
+        }
+    }
+    pg_fence_before();
+    __syncthreads();
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(COLS) : "memory");
+    pt_report(sh, err_dev, err_host);
+}
+
+// ---- two SMs on a tile -----------------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void pt_umma2(unsigned tmem_d, uint64_t a, uint64_t b, unsigned idesc, unsigned accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// what this thread has issued so far arrives on the barrier, when it is complete, in both CTAs
+__device__ __forceinline__ void pt_commit2(unsigned bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ unsigned pt_even(unsigned addr) {         // the even CTA's own of it
+    unsigned a;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(addr));
+    return a;
+}
+__device__ __forceinline__ void pt_tma2(unsigned dst, const void* tmap, unsigned bar, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(tmap), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+// the first n_whole tiles are 256 x 256, those of the last wave that is not full are cut across the rows of x, `cut` pieces each.  The even CTA issues the products; the copies of both are
+// counted on its barriers, and what it commits arrives in both
+template <bool BF16, bool DRAIN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) product_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                                                                                              const __grid_constant__ CUtensorMap map_cut, const __grid_constant__ PrArgs a, int steps, int n_whole, int cut,
+                                                                                              int n_tiles, unsigned* err_dev, unsigned* err_host) {
+    namespace cg = cooperative_groups;
+    constexpr int BN = 256, ST = pt_stages(BN, true);
+    constexpr unsigned A_BYTES = 128 * PT_STEP, BYTES = pt_bytes(BN, true), COLS = 2 * BN;
+    extern __shared__ __align__(1024) uint8_t pt_raw[];
+    __shared__ PtShared sh;
+    uint8_t* ring = (uint8_t*)(((uintptr_t)pt_raw + 1023) & ~(uintptr_t)1023);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cg::this_cluster().block_rank();
+    const int tiles_n = (a.rows + BN - 1) / BN, first = blockIdx.x / 2, stride = gridDim.x / 2, chunk = DRAIN ? PT_DRAIN : steps, chunks = (steps + chunk - 1) / chunk;
+    auto place = [&](int tile, int& mt, int& n0) {
+        const int of = tile < n_whole ? tile : n_whole + (tile - n_whole) / cut;
+        mt = of / tiles_n;
+        n0 = (of - mt * tiles_n) * BN + (tile < n_whole ? 0 : (tile - n_whole) % cut * (BN / cut));
+        return tile < n_whole ? BN : BN / cut;
+    };
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < ST; i++) { pg_mbar_init(pg_smem(&sh.full[i]), 1); pg_mbar_init(pg_smem(&sh.empty[i]), 1); }
+        for (int i = 0; i < 2; i++) { pg_mbar_init(pg_smem(&sh.acc_full[i]), 1); pg_mbar_init(pg_smem(&sh.acc_empty[i]), 2 * PT_WORKERS); }
+        pg_mbar_init(pg_smem(&sh.drained), 1);
+        sh.fail = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pg_smem(&sh.tmem_base)), "n"(COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    pg_fence_before();
+    __syncthreads();
+    cg::this_cluster().sync();
+    pg_fence_after();
+    const unsigned tmem = sh.tmem_base;
+    pdl_enter();
+    if (warp == 0) {
+        if (lane == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
+            unsigned g = 0;
+            bool ok = true;
+            for (int tile = first; tile < n_tiles && ok; tile += stride) {
+                int mt, n0;
+                const int wide = place(tile, mt, n0);
+                for (int s = 0; s < steps; s++, g++) {
+                    const unsigned slot = g % ST, own = pg_smem(&sh.full[slot]), full = pt_even(own), at = pg_smem(ring + (size_t)slot * BYTES);
+                    if (!(ok = sg_wait(pg_smem(&sh.empty[slot]), ((g / ST) & 1u) ^ 1u, &sh.fail))) break;
+                    if (rank == 0) pg_mbar_expect_tx(own, 2 * A_BYTES + wide * PT_STEP);
+                    pt_tma2(at, &map_w, full, s * 64, mt * 256 + rank * 128);
+                    pt_tma2(at + A_BYTES, wide == BN ? &map_x : &map_cut, full, s * 64, n0 + rank * (wide / 2));
+                }
+            }
+            int never = 0;                                            // no copy is under way when the CTAs end (the even one sees those of both), and no arrival
+            for (unsigned i = g > ST ? g - ST : 0; i < g; i++) {
+                if (rank == 0) sg_wait(pg_smem(&sh.full[i % ST]), (i / ST) & 1u, &never);
+                sg_wait(pg_smem(&sh.empty[i % ST]), (i / ST) & 1u, &never);
+            }
+            if (!ok || never)                                         // something did not come in time: a while for whatever is still to
+                for (int i = 0; i < 1000; i++) __nanosleep(1000);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        int never = 0;                                                // nothing is in flight when the TMEM is given back
+        if (lane == 0 && rank == 1) sg_wait(pg_smem(&sh.drained), 0, &never);
+        if (lane == 0 && rank == 0) {
+            unsigned g = 0, nth = 0;
+            bool ok = true;
+            for (int tile = first; tile < n_tiles && ok; tile += stride) {
+                int mt, n0;
+                const unsigned idesc = pg_instr_desc(256, place(tile, mt, n0), BF16 ? 1 : 0);
+                for (int s = 0; s < steps && ok; s++, g++) {
+                    const unsigned acc = tmem + (nth & 1u) * BN;
+                    if (s % chunk == 0) {
+                        if (!(ok = sg_wait(pg_smem(&sh.acc_empty[nth & 1u]), ((nth >> 1) & 1u) ^ 1u, &sh.fail))) break;
+                        pg_fence_after();
+                    }
+                    const unsigned slot = g % ST, at = pg_smem(ring + (size_t)slot * BYTES);
+                    if (!(ok = sg_wait(pg_smem(&sh.full[slot]), (g / ST) & 1u, &sh.fail))) break;
+                    pg_fence_after();
+                    const uint64_t x = pg_smem_desc(at), y = pg_smem_desc(at + A_BYTES);
+#pragma unroll
+                    for (int kk = 0; kk < 4; kk++) pt_umma2(acc, x + 2 * kk, y + 2 * kk, idesc, s % chunk > 0 || kk > 0);
+                    pt_commit2(pg_smem(&sh.empty[slot]));
+                    if (s % chunk == chunk - 1 || s == steps - 1) pt_commit2(pg_smem(&sh.acc_full[nth++ & 1u]));
+                }
+            }
+            pt_commit2(pg_smem(&sh.drained));
+            sg_wait(pg_smem(&sh.drained), 0, &never);
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        const int q = warp & 3, half = (warp - 4) >> 2;
+        unsigned nth = 0;
+        auto release = [&](unsigned n) {
+            pg_fence_before();
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(pt_even(pg_smem(&sh.acc_empty[n & 1u]))) : "memory");
+        };
+        for (int tile = first; tile < n_tiles; tile += stride, nth++) {
+            int mt, at;
+            // a cut tile's columns are shared by both halves, but those that a warp has added up are its own
+            const int wide = place(tile, mt, at), c_first = half * (DRAIN ? BN / 2 : wide / 2), mine = DRAIN ? min(BN / 2, wide - c_first) : wide / 2, n0 = at + c_first;
+            const int col = mt * 256 + rank * 128 + q * 32 + lane;
+            const unsigned lane_col = ((unsigned)(q * 32) << 16) + (unsigned)c_first;
+            if (DRAIN) {
+                if (!pt_collect<BN / 2>(sh, tmem, BN, nth, chunks, lane_col, release)) break;
+            } else {
+                if (!sg_wait_warp(pg_smem(&sh.acc_full[nth & 1u]), (nth >> 1) & 1u, &sh.fail)) break;
+                pg_fence_after();
+            }
+            const unsigned from = tmem + (nth & 1u) * BN + lane_col;
+            const float bias = a.bias && col < a.m ? a.bias[col] : 0.0f;
+            pt_with_act(a.act, [&](auto act) {
+#pragma unroll 1
+                for (int c0 = 0; c0 < mine && n0 + c0 < a.rows; c0 += 16) {
+                    unsigned v[16];
+                    pt_load16(from + c0, v);
+                    pt_finish16(a, v, n0 + c0, a.rows, col, bias, act);
+                }
+            });
+            release(nth);
+        }
+    }
+    pg_fence_before();
+    __syncthreads();
+    cg::this_cluster().sync();
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(COLS) : "memory");
+    pt_report(sh, err_dev, err_host);
+}

@@ -37,20 +37,19 @@ def attention(rows, pos0, q, uk, uv, rank, H, scale, window=0, sink=None):
     rows, q = np.asarray(rows, F), np.asarray(q, F)
     n, dim, vdim = q.shape[0], uk.shape[0] // H, uv.shape[0] // H
     U, V = np.asarray(uk, F).reshape(H, dim, rank), np.asarray(uv, F).reshape(H, vdim, rank)
-    out, size = np.empty((n, H, vdim)), np.empty((n, H, vdim))
-    for t in range(n):
-        i = pos0 + t
-        lo = max(0, i - window + 1) if window > 0 else 0
-        seen = rows[lo:i + 1]
-        bad = not np.isfinite(seen).all()
-        for h in range(H):
-            if bad or not np.isfinite(q[t, h]).all():
-                out[t, h] = size[t, h] = np.nan
+    out, size = np.full((n, H, vdim), np.nan), np.full((n, H, vdim), np.nan)
+    wild = ~np.isfinite(rows).all(1)
+    clean = np.where(wild[:, None], 0.0, rows)
+    for h in range(H):
+        k, v = np.concatenate([clean[:, :rank] @ U[h].T, clean[:, rank:]], 1), clean[:, :rank] @ V[h].T
+        for t in range(n):
+            i = pos0 + t
+            lo = max(0, i - window + 1) if window > 0 else 0
+            if wild[lo:i + 1].any() or not np.isfinite(q[t, h]).all():
                 continue
-            k, v = np.concatenate([seen[:, :rank] @ U[h].T, seen[:, rank:]], 1), seen[:, :rank] @ V[h].T
-            z = scale * (k @ q[t, h])
+            z = scale * (k[lo:i + 1] @ q[t, h])
             top = z.max() if sink is None else max(z.max(), float(sink[h]))
             w = np.exp(z - top)
             total = w.sum() + (0.0 if sink is None else np.exp(float(sink[h]) - top))
-            out[t, h], size[t, h] = (w / total) @ v, (w / total) @ np.abs(v)
+            out[t, h], size[t, h] = (w / total) @ v[lo:i + 1], (w / total) @ np.abs(v[lo:i + 1])
     return out, size

@@ -233,6 +233,22 @@ def test_masks(dev, form, P, window, sink, out_type):
 
 
 @pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("P,window", [(16, 0), (128, 0), (64, 200)])
+@pytest.mark.parametrize("shape", [(2, 128, 64, 128, 512), (3, 32, 16, 32, 64), (2, 80, 32, 112, 96)], ids=str)
+def test_prompts(dev, form, P, window, shape):
+    """portions of many tokens: several tiles of rows and of keys, beside sequences of one token and of none"""
+    H, dim, rest, vdim, rank = shape
+    c = Case(dev, P, rank, rest, [0, 333, 70, 9, 1000], [513, 256, 0, 1, 129], seed=P)
+    check(dev, c, H, dim, vdim, 1.2 * (dim + rest) ** -0.5, window=window, form=FORMS[form])
+
+
+def test_both_forms_in_a_call(dev):
+    """a step of portions and single tokens, by the rule"""
+    c = Case(dev, 32, 64, 16, [100, 7, 0, 40, 300, 5], [1, 300, 64, 65, 1, 200], seed=4)
+    check(dev, c, 4, 32, 48, 0.2)
+
+
+@pytest.mark.parametrize("form", list(FORMS))
 def test_sinks_far_away(dev, form):
     """sinks that take all of the weight, none of it, and -inf"""
     c = Case(dev, 16, 32, 16, [50], [3])
