@@ -1,7 +1,7 @@
 // latent.cu -- from projections to pages of latent rows (include/crabml_paged.h): norm, rotation and rounding of a token's row, and of its queries on the way.
 //
 // Bound by bytes: a token of 16 heads of 128 + 64 over rows of 512 + 64 is 3648 numbers of 2 or 4 bytes in and as many of 2 out.  The unit of work is a segment of
-// the plan (new tokens of one sequence in one page), so that a CTA knows its page without a search; a CTA takes its rows one by one, 8 neighbouring numbers a thread.
+// the plan (new tokens of one sequence in one page), so that a CTA knows its page without a search; a CTA takes 8 of its rows, 8 neighbouring numbers a thread.
 // The angles are made once a row and CTA: position x frequency in 64 bits and brought to a turn there (position 100000: 0.008 of a radian would be lost in 32), sine
 // and cosine of the remainder in 32.
 #include <algorithm>
@@ -9,8 +9,10 @@
 #include "latent.cuh"
 
 #define LA_THREADS 256
-#define LA_WARPS (LA_THREADS / 32)
-static_assert(LA_THREADS * 8 >= LT_RANK + LT_REST, "a thread holds one run of 8 columns of a row");
+#define LA_ROWS (LA_THREADS / 32)             // of a segment that a CTA takes
+#define LA_RUNS 3                             // runs of 8 columns of a cached row that a lane holds
+#define LA_AHEAD 4                            // .. of the queries that a thread has under way
+static_assert(LA_RUNS * 256 >= LT_RANK + LT_REST, "a warp holds a row");
 
 int lt_check_pages(cc_device* dev, const cc_page_plan* plan, const cc_view* pages, int32_t rank, const char* what, LtPages* o) {
     if (!view_ok(pages)) return cc_fail(dev, CC_ERR_ARG, "%s: bad view of pages", what);
@@ -59,61 +61,73 @@ __device__ __forceinline__ void la_turn(const LaArgs& a, const void* src, int ty
 }
 __device__ __forceinline__ uint4 la_pack(const float (&v)[8]) { return make_uint4(ht_pack_f16(v[0], v[1]), ht_pack_f16(v[2], v[3]), ht_pack_f16(v[4], v[5]), ht_pack_f16(v[6], v[7])); }
 
-// grid (segments, rows of a segment by turns, 1 + parts of the heads)
+// grid (segments, groups of LA_ROWS of their rows, 1 + parts of the heads): the first CTAs the rows of the cache, a warp each, the others queries, 8 columns a thread
 __global__ void __launch_bounds__(LA_THREADS) latent_append_kernel(const LaArgs a) {
-    __shared__ float2 cs[LT_REST / 2];
-    __shared__ float sums[2][LA_WARPS];
-    const int tid = threadIdx.x;
+    __shared__ float2 cs[LA_ROWS][LT_REST / 2];
+    const int tid = threadIdx.x, lane = tid & 31;
     pdl_enter();
     const PgSegment g = a.segments[blockIdx.x];
-    int turn = 0;
-    for (int r = blockIdx.y; r < g.rows; r += gridDim.y, turn ^= 1) {
-        const int64_t token = g.token0 + r;
-        __syncthreads();                                                 // cs of the row before
-        for (int i = tid; i < a.pairs; i += LA_THREADS) {
-            // a whole number of turns leaves the fraction exactly; what is left of the angle, in turns, has 2^-53 of the position's turns as its error
-            const double turns = (double)(g.pos0 + r) * (double)a.freq[i] * 0.15915494309189533577;
-            const float part = (float)(turns - rint(turns));
-            float s, c;
-            sincospif(2.0f * part, &s, &c);
-            cs[i] = make_float2(c, s);
+    const int r0 = blockIdx.y * LA_ROWS, n = min(LA_ROWS, g.rows - r0);
+    if (n <= 0) return;
+    for (int e = tid; e < n * a.pairs; e += LA_THREADS) {
+        // a whole number of turns leaves the fraction exactly; what is left of the angle, in turns, has 2^-53 of the position's turns as its error
+        const int r = e / a.pairs, i = e - r * a.pairs;
+        const double turns = (double)(g.pos0 + r0 + r) * (double)a.freq[i] * 0.15915494309189533577;
+        const float part = (float)(turns - rint(turns));
+        float s, c;
+        sincospif(2.0f * part, &s, &c);
+        cs[r][i] = make_float2(c, s);
+    }
+    __syncthreads();
+    if (blockIdx.z == 0) {
+        const int r = tid >> 5;
+        if (r >= n) return;
+        const int64_t from = (int64_t)(g.token0 + r0 + r) * a.kv_stride;
+        __half* to = a.rows + ((int64_t)g.page * a.page + g.row0 + r0 + r) * a.cols;
+        float v[LA_RUNS][8], s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < LA_RUNS; i++) {
+            const int c = (i * 32 + lane) * 8;
+            if (c < a.cols) ht_read8(a.kv, from + c, a.kv_type, a.kv_vec, v[i]);
         }
-        if (blockIdx.z == 0) {
-            // a thread holds one run of 8 columns: rows are at most LT_RANK + LT_REST of them
-            const int64_t at = token * a.kv_stride + tid * 8;
-            const bool in = tid * 8 < a.cols;
-            float v[8], s = 0.0f;
-            if (in) ht_read8(a.kv, at, a.kv_type, a.kv_vec, v);
-            if (in && tid * 8 < a.rank) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) s = fmaf(v[j], v[j], s);
-            }
-            s = warp_sum(s);
-            if ((tid & 31) == 0) sums[turn][tid >> 5] = s;
-            __syncthreads();
-            s = 0.0f;
+        for (int i = 0; i < LA_RUNS; i++)
+            if ((i * 32 + lane) * 8 < a.rank) {
 #pragma unroll
-            for (int i = 0; i < LA_WARPS; i++) s += sums[turn][i];
-            if (in) {
-                if (tid * 8 < a.rank) {
-                    const float size = sqrtf(s / (float)a.rank + a.eps);
+                for (int j = 0; j < 8; j++) s = fmaf(v[i][j], v[i][j], s);
+            }
+        const float size = sqrtf(warp_sum(s) / (float)a.rank + a.eps);
 #pragma unroll
-                    for (int j = 0; j < 8; j++) v[j] = v[j] / size * (a.norm ? a.norm[tid * 8 + j] : 1.0f);
-                } else la_turn(a, a.kv, a.kv_type, at, tid * 8 - a.rank, cs, v);
-                *(uint4*)(a.rows + ((int64_t)g.page * a.page + g.row0 + r) * a.cols + tid * 8) = la_pack(v);
-            }
-        } else {
-            __syncthreads();
-            const int runs = (a.dim + a.rest) / 8, all = a.H * runs, parts = gridDim.z - 1;
-            const int lo = (int)((int64_t)all * (blockIdx.z - 1) / parts), hi = (int)((int64_t)all * blockIdx.z / parts);
-            for (int e = lo + tid; e < hi; e += LA_THREADS) {
-                const int c = (e % runs) * 8 - a.dim;
-                const int64_t at = token * a.q_stride + (int64_t)e * 8;
-                float v[8];
-                ht_read8(a.q, at, a.q_type, a.q_vec, v);
-                if (c >= 0) la_turn(a, a.q, a.q_type, at, c, cs, v);
-                ((uint4*)a.qo)[token * all + e] = la_pack(v);
-            }
+        for (int i = 0; i < LA_RUNS; i++) {
+            const int c = (i * 32 + lane) * 8;
+            if (c >= a.cols) continue;
+            if (c < a.rank) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[i][j] = v[i][j] / size * (a.norm ? a.norm[c + j] : 1.0f);
+            } else la_turn(a, a.kv, a.kv_type, from + c, c - a.rank, cs[r], v[i]);
+            *(uint4*)(to + c) = la_pack(v[i]);
+        }
+        return;
+    }
+    const int runs = (a.dim + a.rest) / 8, all = a.H * runs, parts = gridDim.z - 1;
+    const int lo = (int)((int64_t)all * (blockIdx.z - 1) / parts), each = (int)((int64_t)all * blockIdx.z / parts) - lo;
+    for (int e0 = tid; e0 < n * each; e0 += LA_THREADS * LA_AHEAD) {
+        float v[LA_AHEAD][8];
+        int at[LA_AHEAD], row[LA_AHEAD];
+#pragma unroll
+        for (int i = 0; i < LA_AHEAD; i++) {
+            const int e = e0 + i * LA_THREADS;
+            if (e >= n * each) continue;
+            row[i] = e / each; at[i] = lo + e - row[i] * each;
+            ht_read8(a.q, (int64_t)(g.token0 + r0 + row[i]) * a.q_stride + (int64_t)at[i] * 8, a.q_type, a.q_vec, v[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < LA_AHEAD; i++) {
+            if (e0 + i * LA_THREADS >= n * each) continue;
+            const int c = at[i] % runs * 8 - a.dim;
+            const int64_t token = g.token0 + r0 + row[i];
+            if (c >= 0) la_turn(a, a.q, a.q_type, token * a.q_stride + (int64_t)at[i] * 8, c, cs[row[i]], v[i]);
+            ((uint4*)a.qo)[token * all + at[i]] = la_pack(v[i]);
         }
     }
 }
@@ -165,11 +179,11 @@ extern "C" CC_API int cc_paged_latent_append(cc_device* dev, const cc_page_plan*
         }
         a.norm = norm_w ? (const float*)norm_w->buf->plane[0] : nullptr; a.freq = freq ? (const float*)freq->buf->plane[0] : nullptr;
         a.rows = c.rows; a.rank = c.rank; a.rest = c.rest; a.cols = c.cols; a.page = plan->page; a.pairs = (int)pairs; a.halves = pairing == CC_ROPE_HALVES; a.eps = eps; a.mag = mag;
-        // portions: a few CTAs a segment, each its rows by turns; single tokens: their heads over several CTAs
-        const bool many = T > 4 * (int64_t)plan->n_segments;
-        const int64_t runs = q_src ? (int64_t)H * (dim + c.rest) / 8 : 0;
-        const unsigned parts = q_src ? (unsigned)std::max<int64_t>(1, std::min<int64_t>(many ? 1 : 16, (runs + LA_THREADS - 1) / LA_THREADS)) : 0;
-        const cudaError_t e = cc_launch_pdl(dev, latent_append_kernel, dim3((unsigned)plan->n_segments, many ? (unsigned)plan->page / 4 : 1u, 1 + parts), LA_THREADS, 0, a);
+        // the queries' columns over as many CTAs as let each thread have LA_AHEAD runs or fewer of one token, or of LA_ROWS of a portion
+        const int64_t runs = q_src ? (int64_t)H * (dim + c.rest) / 8 * (T > 4 * (int64_t)plan->n_segments ? LA_ROWS : 1) : 0;
+        const unsigned parts = (unsigned)std::min<int64_t>(64, (runs + LA_THREADS * LA_AHEAD - 1) / (LA_THREADS * LA_AHEAD));
+        const unsigned groups = T == plan->n_segments ? 1u : (unsigned)(plan->page + LA_ROWS - 1) / LA_ROWS;
+        const cudaError_t e = cc_launch_pdl(dev, latent_append_kernel, dim3((unsigned)plan->n_segments, groups, 1 + parts), LA_THREADS, 0, a);
         dev->launches++;
         if (e != cudaSuccess) {
             if (o) cc_tensor_release(o);

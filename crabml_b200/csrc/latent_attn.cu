@@ -495,39 +495,59 @@ __global__ void __launch_bounds__(LR_THREADS, 1) latent_rows_kernel(const __grid
         if (err_host) { *(volatile unsigned*)err_host = 5u; __threadfence_system(); }
     }
 }
-// segments in several runs: grid (segments, rows, 128 columns)
+// segments in several runs: grid (segments, rows, 128 columns); a warp takes every eighth slice.  (One thread a column, one slice after another: 43 us for the 148 slices of a long cache)
+#define LJ_WARPS 8
 template <int MT>
-__global__ void __launch_bounds__(128) latent_join_kernel(const LrArgs a, const __grid_constant__ LrCuts cuts) {
-    __shared__ float2 red[4];
+__global__ void __launch_bounds__(LJ_WARPS * 32) latent_join_kernel(const LrArgs a, const __grid_constant__ LrCuts cuts) {
+    __shared__ float factor[LR_CTAS], red[2][LJ_WARPS];
+    __shared__ float4 sums[LJ_WARPS][32];
     pdl_enter();
     constexpr int ROWS = 16 * MT;
     const auto cut = cuts.at[blockIdx.x];
     const PgSeq s = a.seqs[cut.seq];
-    const int y = blockIdx.y, row = cut.tile * ROWS + y, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int y = blockIdx.y, row = cut.tile * ROWS + y, lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.z * 128 + lane * 4;
     if (row >= s.count * a.H) return;
     auto place = [&](int x) { return (size_t)(x == 0 ? cut.slot : 2 * (cut.cta + x - 1)) * ROWS + y; };
-    float m = -INFINITY, l = 0.0f;
-    for (int x = threadIdx.x; x < cut.n; x += 128) m = fmaxf(m, a.ml[place(x)].x);
-    m = warp_max(m);
-    if (lane == 0) red[w].x = m;
+    static_assert(LR_CTAS <= LJ_WARPS * 32, "a thread a slice");
+    const int x = threadIdx.x;
+    const float2 z = x < cut.n ? a.ml[place(x)] : make_float2(-INFINITY, 0.0f);
+    float m = warp_max(z.x);
+    if (lane == 0) red[0][w] = m;
     __syncthreads();
-    m = fmaxf(fmaxf(red[0].x, red[1].x), fmaxf(red[2].x, red[3].x));
-    const int c = blockIdx.z * 128 + threadIdx.x;
-    float o = 0.0f;
+#pragma unroll
+    for (int i = 0; i < LJ_WARPS; i++) m = fmaxf(m, red[0][i]);
+    const float f = z.x == -INFINITY ? (z.y == 0.0f ? 0.0f : 1.0f) : exp2f(z.x - m);
+    if (x < cut.n) factor[x] = f;
+    float l = warp_sum(f * z.y);
+    if (lane == 0) red[1][w] = l;
+    __syncthreads();
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (c < a.rank) {
 #pragma unroll 4
-    for (int x = 0; x < cut.n; x++) {
-        const float2 z = a.ml[place(x)];
-        const float f = z.x == -INFINITY ? (z.y == 0.0f ? 0.0f : 1.0f) : exp2f(z.x - m);
-        l = fmaf(f, z.y, l);
-        if (c < a.rank && f != 0.0f) o = fmaf(f, a.part[place(x) * a.rank + c], o);
+        for (int i = w; i < cut.n; i += LJ_WARPS) {
+            const float by = factor[i];
+            const float4 v = *(const float4*)(a.part + place(i) * a.rank + c);
+            if (by != 0.0f) { o.x = fmaf(by, v.x, o.x); o.y = fmaf(by, v.y, o.y); o.z = fmaf(by, v.z, o.z); o.w = fmaf(by, v.w, o.w); }
+        }
     }
+    sums[w][lane] = o;
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < LJ_WARPS; i++) l += red[1][i];
+    __syncthreads();
     float g = 1.0f;
     if (a.sink) {
         const float sk = a.sink[row % a.H] * LR_LOG2E, m2 = fmaxf(m, sk);
         g = m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : exp2f(m - m2);
         l = g * l + (sk == -INFINITY ? 0.0f : exp2f(sk - m2 + LR_SHIFT));
     }
-    if (c < a.rank) a.lat[((int64_t)s.first * a.H + row) * a.rank + c] = o * (g / l);
+    const int col = blockIdx.z * 128 + threadIdx.x;
+    if (threadIdx.x < 128 && col < a.rank) {
+        float t = 0.0f;
+#pragma unroll
+        for (int i = 0; i < LJ_WARPS; i++) t += ((const float*)sums[i])[threadIdx.x];
+        a.lat[((int64_t)s.first * a.H + row) * a.rank + col] = t * (g / l);
+    }
 }
 
 // the runs of deal.ctas CTAs over all steps, and the segments that are in several of them (returned: how many)
@@ -579,7 +599,7 @@ static int lr_run(cc_device* dev, const cc_page_plan* plan, LrArgs a, const LtRu
     if (e == cudaSuccess) e = cudaFuncSetAttribute(latent_unfold_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (LU_COLS + 32) * (LT_RANK + 8) * 2);
     if (e == cudaSuccess) e = cc_launch_pdl(dev, latent_fold_kernel, dim3((unsigned)a.H, (unsigned)((a.rank + LF_COLS - 1) / LF_COLS + (a.rest ? 1 : 0)), z), 128, fold, a, runs);
     if (e == cudaSuccess) e = cc_launch_pdl(dev, latent_rows_kernel<MT>, (unsigned)deal.ctas, LR_THREADS, (size_t)a.slots * slot, a, deal, dev->err_dev, dev->err_host);
-    if (e == cudaSuccess && n_cuts) { e = cc_launch_pdl(dev, latent_join_kernel<MT>, dim3((unsigned)n_cuts, ROWS, (unsigned)(a.rank + 127) / 128), 128, 0, a, cuts); dev->launches++; }
+    if (e == cudaSuccess && n_cuts) { e = cc_launch_pdl(dev, latent_join_kernel<MT>, dim3((unsigned)n_cuts, ROWS, (unsigned)(a.rank + 127) / 128), LJ_WARPS * 32, 0, a, cuts); dev->launches++; }
     if (e == cudaSuccess) e = cc_launch_pdl(dev, latent_unfold_kernel, dim3((unsigned)a.H, (unsigned)((a.vdim + LU_COLS - 1) / LU_COLS), z), 128, unfold, a, runs);
     dev->launches += 3;
     cc_pool_free(dev, ws, cls);

@@ -5,21 +5,24 @@
 //
 // latent_tile_kernel: a CTA takes 256 tokens of a head, as two tiles of 128 rows, over the keys that they see, 128 at a time:
 //   S = Q K^T (128 x 128 x (dim + rest)), P = exp2(S f - base) as f16 written over S in TMEM, O += P V in TMEM
-// The two tiles alternate: while the 128 threads of one make its weights, a row each, the tensor core multiplies for the other.  TMEM holds both S and both O (512 columns), shared memory
+// The two tiles alternate: while the 256 threads of one make its weights, two a row, the tensor core multiplies for the other.  (With a thread a row a step's 128 scores were a chain of
+// 4500 cycles for the one warp a scheduler that a tile had: 4000 tokens of 16 heads took 147 us.)  TMEM holds both S and both O (512 columns), shared memory
 // Q (96 KB) and a ring of 16 KB blocks of keys and values (128 KB).  base lags: a row's sums are scaled only when its largest score is 2^TL_LAG times what it was (sums in TMEM would have
 // to be read and written back), so that weights are up to 2^TL_LAG and f16 still holds them and all that counts beside them.
-// Warps 0-3 and 4-7 the rows of the two tiles, 8 the copies, 9 the products.  Every wait is bounded; where one ran out all roles run to their ends and the host reports it.
+// Warps 0-7 and 8-15 the rows of the two tiles, 16 the copies, 17 the products.  Every wait is bounded; where one ran out all roles run to their ends and the host reports it.
 #pragma once
 #include <cuda.h>
 
 #define TL_ROWS 128
 #define TL_KEYS 128
-#define TL_THREADS 384
-// 384 threads of 168 registers at launch are 256 of 216 and 128 of 72 afterwards: 128 scores of a row stay in registers
-#define TL_REGS 168
-#define TL_REGS_SOFT 216
-#define TL_REGS_REST 72
-static_assert(256 * TL_REGS_SOFT + 128 * TL_REGS_REST <= TL_THREADS * TL_REGS, "more registers than the block was launched with");
+#define TL_HALF (TL_KEYS / 2)
+#define TL_SOFT 16                            // warps that make weights
+#define TL_THREADS (TL_SOFT * 32 + 128)
+// 640 threads of 96 registers at launch are 512 of 104 and 128 of 64 afterwards: 64 scores stay in registers
+#define TL_REGS 96
+#define TL_REGS_SOFT 104
+#define TL_REGS_REST 64
+static_assert(TL_SOFT * 32 * TL_REGS_SOFT + 128 * TL_REGS_REST <= TL_THREADS * TL_REGS, "more registers than the block was launched with");
 #define TL_BLOCK 16384                        // 128 rows of 64 f16 under the 128-byte swizzle
 #define TL_SLOTS 8
 #define TL_QBLOCKS 3                          // of a row of Q: dim in two, rest in one
@@ -158,28 +161,33 @@ __global__ void __launch_bounds__(TE_THREADS, 1) latent_expand_kernel(const __gr
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            const unsigned idesc = pg_instr_desc(128, width);
-            unsigned g = 0;
-            bool ok = true;
-            for (int h = h0; h < h1 && ok; h++) {
-                const unsigned n = (unsigned)(h - h0), acc = tmem + (n & 1u) * 256;
-                if (!(ok = tl_wait(pg_smem(&sh.acc_empty[n & 1u]), ((n >> 1) & 1u) ^ 1u, &sh.fail))) break;
-                for (int b = 0; b < blocks; b++, g++) {
-                    const unsigned slot = g % TE_STAGES;
-                    if (!(ok = tl_wait(pg_smem(&sh.a_full[b]), 0, &sh.fail) && tl_wait(pg_smem(&sh.full[slot]), (g / TE_STAGES) & 1u, &sh.fail))) break;
-                    pg_fence_after();
-                    const uint64_t x = pg_smem_desc(pg_smem(as + b * TL_BLOCK)), y = pg_smem_desc(pg_smem(bs + slot * TE_STAGE));
-                    for (int kk = 0; kk < min(4, (a.rank - b * 64) / 16); kk++) pg_umma_f16(acc, x + 2 * kk, y + 2 * kk, idesc, b > 0 || kk > 0);
+        const unsigned idesc = pg_instr_desc(128, width);
+        const uint64_t a_desc = pg_smem_desc(pg_smem(as)), b_desc = pg_smem_desc(pg_smem(bs));
+        unsigned slot = 0, phase = 0;
+        bool ok = true;
+        for (int h = h0; h < h1 && ok; h++) {
+            const unsigned n = (unsigned)(h - h0), acc = tmem + (n & 1u) * 256;
+            if (!(ok = tl_wait_warp(pg_smem(&sh.acc_empty[n & 1u]), ((n >> 1) & 1u) ^ 1u, &sh.fail))) break;
+            for (int b = 0; b < blocks; b++) {
+                if (!(ok = (h > h0 || tl_wait_warp(pg_smem(&sh.a_full[b]), 0, &sh.fail)) && tl_wait_warp(pg_smem(&sh.full[slot]), phase, &sh.fail))) break;
+                pg_fence_after();
+                const uint64_t x = a_desc + b * (TL_BLOCK >> 4), y = b_desc + slot * (TE_STAGE >> 4);
+                const int steps = min(4, (a.rank - b * 64) >> 4);
+                if (pg_elect()) {
+#pragma unroll
+                    for (int kk = 0; kk < 4; kk++)
+                        if (kk < steps) pg_umma_f16(acc, x + 2 * kk, y + 2 * kk, idesc, b > 0 || kk > 0);
                     pg_umma_commit(pg_smem(&sh.empty[slot]));
+                    if (b == blocks - 1) pg_umma_commit(pg_smem(&sh.acc_full[n & 1u]));
                 }
-                if (ok) pg_umma_commit(pg_smem(&sh.acc_full[n & 1u]));
+                __syncwarp();
+                if (++slot == TE_STAGES) { slot = 0; phase ^= 1u; }
             }
-            int never = 0;                                            // nothing of this CTA is in flight when its TMEM is given back
-            pg_umma_commit(pg_smem(&sh.drained));
-            tl_wait(pg_smem(&sh.drained), 0, &never);
         }
+        int never = 0;                                                // nothing of this CTA is in flight when its TMEM is given back
+        if (pg_elect()) pg_umma_commit(pg_smem(&sh.drained));
         __syncwarp();
+        tl_wait_warp(pg_smem(&sh.drained), 0, &never);
     } else if (warp >= 4) {
         // a lane a key, the two warps of its lanes every second run of 16 columns
         const int q = warp & 3, row = q * 32 + lane;
@@ -224,7 +232,15 @@ struct TlShared {
     unsigned long long q_full, full[TL_SLOTS], empty[TL_SLOTS], s_full[2], p_full[2], o_full[2], drained;
     unsigned tmem_base;
     int fail;
+    float top[2][TL_ROWS];                    // what the two threads of a row tell each other
 };
+// the 256 threads of a tile
+__device__ __forceinline__ void tl_sync(int bar) { asm volatile("bar.sync %0, %1;" ::"r"(bar), "n"(TL_SOFT * 16) : "memory"); }
+__device__ __forceinline__ bool tl_sync_or(int bar, bool x) {
+    unsigned r;
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbar.red.or.pred q, %2, %3, p;\nselp.u32 %0, 1, 0, q;\n}\n" : "=r"(r) : "r"((unsigned)x), "r"(bar), "n"(TL_SOFT * 16) : "memory");
+    return r;
+}
 // B whose rows are the sum's index and whose columns (64 of them in 128 bytes) are the result's: blocks of 64 columns `block` bytes apart, groups of 8 rows 1024 bytes
 __device__ __forceinline__ uint64_t tl_desc_mn(unsigned addr, unsigned block) {
     return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)(block >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
@@ -268,12 +284,12 @@ __device__ __forceinline__ float tl_max3(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// 2^x of a pair by multiply-adds: x = n + r with |r| <= 1/2 by way of a number whose last place is 1; 2^r by its series up to r^4 (the first term left out is 2^-14.5 at |r| = 1/2 before
-// its coefficients are fitted; see below), n into the exponent.  What is below -126 counts as -126
+// 2^x of a pair by multiply-adds: x = n + r with |r| <= 1/2 by way of a number whose last place is 1; 2^r by its series up to r^5 (the first term left out is 2^-19 at |r| = 1/2, far below
+// the weights' 2^-11), n into the exponent.  What is below -126 counts as -126
 __device__ __forceinline__ tl_f2 tl_exp2_pair(float2 x) {
     const tl_f2 big = tl_two(12582912.0f, 12582912.0f), minus = tl_two(-1.0f, -1.0f);
     const tl_f2 v = tl_two(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f)), u = tl_add2(v, big), n = tl_add2(u, tl_two(-12582912.0f, -12582912.0f)), r = tl_fma2(n, minus, v);
-    tl_f2 p = tl_two(1.3333558e-3f, 1.3333558e-3f);                  // (ln 2)^i / i!, i = 5 .. 0: the first term left out is 2^-19 at |r| = 1/2, far below the weights' 2^-11
+    tl_f2 p = tl_two(1.3333558e-3f, 1.3333558e-3f);                  // (ln 2)^i / i!, i = 5 .. 0
     p = tl_fma2(p, r, tl_two(9.6181291e-3f, 9.6181291e-3f));
     p = tl_fma2(p, r, tl_two(5.5504109e-2f, 5.5504109e-2f));
     p = tl_fma2(p, r, tl_two(2.4022651e-1f, 2.4022651e-1f));
@@ -294,12 +310,12 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
     if (tid == 0) {
         pg_mbar_init(pg_smem(&sh.q_full), 1);
         for (int i = 0; i < TL_SLOTS; i++) { pg_mbar_init(pg_smem(&sh.full[i]), 1); pg_mbar_init(pg_smem(&sh.empty[i]), 1); }
-        for (int i = 0; i < 2; i++) { pg_mbar_init(pg_smem(&sh.s_full[i]), 1); pg_mbar_init(pg_smem(&sh.p_full[i]), 4); pg_mbar_init(pg_smem(&sh.o_full[i]), 1); }
+        for (int i = 0; i < 2; i++) { pg_mbar_init(pg_smem(&sh.s_full[i]), 1); pg_mbar_init(pg_smem(&sh.p_full[i]), TL_SOFT / 2); pg_mbar_init(pg_smem(&sh.o_full[i]), 1); }
         pg_mbar_init(pg_smem(&sh.drained), 1);
         sh.fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 9) {
+    if (warp == TL_SOFT + 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pg_smem(&sh.tmem_base)), "n"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -321,9 +337,9 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
     const int lo = a.window > 0 ? max(from, (s.pos0 + row0 - a.window + 1) & ~(TL_KEYS - 1)) : from;
     auto steps_of = [&](int i) { return row0 + i * TL_ROWS < s.count ? (s.pos0 + last(i) + 1 - lo + TL_KEYS - 1) / TL_KEYS : 0; };
     const int steps0 = steps_of(0), steps1 = steps_of(1), steps = max(steps0, steps1), kt0 = before + (lo - from) / TL_KEYS, per = nb + rb + vb;
-    if (warp >= 8) {
+    if (warp >= TL_SOFT) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TL_REGS_REST));
-        if (warp == 8) {
+        if (warp == TL_SOFT) {
             // ===== copies: Q, then the blocks of each step =====
             if (lane == 0) {
                 const int width = a.dim + a.rest;
@@ -353,154 +369,188 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
                 tl_wait(pg_smem(&sh.q_full), 0, &never);
             }
             __syncwarp();
-        } else if (warp == 9) {
-            // ===== products: one thread =====
-            if (lane == 0) {
-                const unsigned idesc_s = pg_instr_desc(128, TL_KEYS), idesc_o = pg_instr_desc(128, a.vdim) | 1u << 16;
-                bool ok = tl_wait(pg_smem(&sh.q_full), 0, &sh.fail);
-                auto wait_blocks = [&](unsigned g, int n) {
-                    for (int b = 0; b < n && ok; b++, g++) ok = tl_wait(pg_smem(&sh.full[g % TL_SLOTS]), (g / TL_SLOTS) & 1u, &sh.fail);
-                    pg_fence_after();
-                };
-                auto free_blocks = [&](unsigned g, int n) {
+        } else if (warp == TL_SOFT + 1) {
+            // ===== products =====
+            const unsigned idesc_s = pg_instr_desc(128, TL_KEYS), idesc_o = pg_instr_desc(128, a.vdim) | 1u << 16, idesc_lo = pg_instr_desc(128, 64) | 1u << 16, idesc_hi = pg_instr_desc(128, a.vdim - 64) | 1u << 16;
+            const uint64_t q_desc = pg_smem_desc(pg_smem(qs)), ring_desc = pg_smem_desc(pg_smem(ring)), v_desc = tl_desc_mn(pg_smem(ring), TL_BLOCK);
+            bool ok = tl_wait_warp(pg_smem(&sh.q_full), 0, &sh.fail);
+            auto wait_blocks = [&](unsigned g, int n) {
+                for (int b = 0; b < n && ok; b++, g++) ok = tl_wait_warp(pg_smem(&sh.full[g % TL_SLOTS]), (g / TL_SLOTS) & 1u, &sh.fail);
+                pg_fence_after();
+            };
+            auto free_blocks = [&](unsigned g, int n) {
+                if (pg_elect())
                     for (int b = 0; b < n; b++, g++) pg_umma_commit(pg_smem(&sh.empty[g % TL_SLOTS]));
-                };
-                auto scores = [&](int i, unsigned g) {               // of tile i against the keys in blocks g ..
-                    unsigned on = 0;
-                    for (int b = 0; b < nb + rb; b++, g++) {
-                        const uint64_t x = pg_smem_desc(pg_smem(qs + (i * TL_QBLOCKS + b) * TL_BLOCK)), y = pg_smem_desc(pg_smem(ring + (g % TL_SLOTS) * TL_BLOCK));
-                        for (int kk = 0; kk < min(4, (b < nb ? a.dim - b * 64 : a.rest) / 16); kk++, on = 1u) pg_umma_f16(tmem + i * 128, x + 2 * kk, y + 2 * kk, idesc_s, on);
+                __syncwarp();
+            };
+            auto scores = [&](int i, unsigned g) {                   // of tile i against the keys in blocks g ..
+                const unsigned to_s = tmem + i * 128;
+                for (int b = 0; b < nb + rb; b++, g++) {
+                    const uint64_t x = q_desc + (unsigned)(i * TL_QBLOCKS + b) * (TL_BLOCK >> 4), y = ring_desc + (g % TL_SLOTS) * (TL_BLOCK >> 4);
+                    const int n = min(4, (b < nb ? a.dim - b * 64 : a.rest) >> 4);
+                    if (pg_elect()) {
+#pragma unroll
+                        for (int kk = 0; kk < 4; kk++)
+                            if (kk < n) pg_umma_f16(to_s, x + 2 * kk, y + 2 * kk, idesc_s, b > 0 || kk > 0);
+                        if (b == nb + rb - 1) pg_umma_commit(pg_smem(&sh.s_full[i]));
                     }
-                    pg_umma_commit(pg_smem(&sh.s_full[i]));
-                };
-                auto values = [&](int i, unsigned g, int k) {
-                    const unsigned v0 = pg_smem(ring + (g % TL_SLOTS) * TL_BLOCK), v1 = pg_smem(ring + ((g + 1) % TL_SLOTS) * TL_BLOCK);
-                    // the ring's blocks lie side by side, but for the last and the first
-                    for (int kk = 0; kk < TL_KEYS / 16; kk++) {
-                        if (vb == 1 || v1 == v0 + TL_BLOCK) tl_umma_ts(tmem + TL_O + i * 128, tmem + i * 128 + kk * 8, tl_desc_mn(v0 + kk * 2048, TL_BLOCK), idesc_o, k > 0 || kk > 0);
-                        else {
-                            tl_umma_ts(tmem + TL_O + i * 128, tmem + i * 128 + kk * 8, tl_desc_mn(v0 + kk * 2048, TL_BLOCK), pg_instr_desc(128, 64) | 1u << 16, k > 0 || kk > 0);
-                            tl_umma_ts(tmem + TL_O + i * 128 + 64, tmem + i * 128 + kk * 8, tl_desc_mn(v1 + kk * 2048, TL_BLOCK), pg_instr_desc(128, a.vdim - 64) | 1u << 16, k > 0 || kk > 0);
+                    __syncwarp();
+                }
+            };
+            auto values = [&](int i, unsigned g, int k) {
+                const unsigned to_o = tmem + TL_O + i * 128, p = tmem + i * 128;
+                const uint64_t v0 = v_desc + (g % TL_SLOTS) * (TL_BLOCK >> 4), v1 = v_desc + ((g + 1) % TL_SLOTS) * (TL_BLOCK >> 4);
+                const bool apart = vb == 2 && (g + 1) % TL_SLOTS == 0;       // the ring's blocks lie side by side, but for the last and the first
+                if (pg_elect()) {
+                    if (!apart) {
+#pragma unroll
+                        for (int kk = 0; kk < TL_KEYS / 16; kk++) tl_umma_ts(to_o, p + kk * 8, v0 + kk * (2048 >> 4), idesc_o, k > 0 || kk > 0);
+                    } else {
+#pragma unroll
+                        for (int kk = 0; kk < TL_KEYS / 16; kk++) {
+                            tl_umma_ts(to_o, p + kk * 8, v0 + kk * (2048 >> 4), idesc_lo, k > 0 || kk > 0);
+                            tl_umma_ts(to_o + 64, p + kk * 8, v1 + kk * (2048 >> 4), idesc_hi, k > 0 || kk > 0);
                         }
                     }
                     pg_umma_commit(pg_smem(&sh.o_full[i]));
-                };
-                if (ok && steps > 0) {
-                    wait_blocks(0, nb + rb);
-                    if (ok && steps0 > 0) scores(0, 0);
-                    if (ok && steps1 > 0) scores(1, 0);
-                    free_blocks(0, nb + rb);
                 }
-                for (int k = 0; k < steps && ok; k++) {
-                    const unsigned gv = (unsigned)(k * per + nb + rb), gk = (unsigned)((k + 1) * per);
-                    wait_blocks(gv, vb);
-                    bool there = false;
-#pragma unroll 1
-                    for (int i = 0; i < 2 && ok; i++) {
-                        const int mine = i ? steps1 : steps0;
-                        if (k < mine) {
-                            if (!(ok = tl_wait(pg_smem(&sh.p_full[i]), k & 1, &sh.fail))) break;
-                            pg_fence_after();
-                            values(i, gv, k);
-                        }
-                        if (i == 1) free_blocks(gv, vb);
-                        if (k + 1 < mine) {
-                            if (!there) { wait_blocks(gk, nb + rb); there = true; }
-                            if (ok) scores(i, gk);
-                        }
-                    }
-                    if (ok && k + 1 < steps) free_blocks(gk, nb + rb);
-                }
-                int never = 0;                                        // nothing of this CTA is in flight when its TMEM is given back
-                pg_umma_commit(pg_smem(&sh.drained));
-                tl_wait(pg_smem(&sh.drained), 0, &never);
+                __syncwarp();
+            };
+            if (ok && steps > 0) {
+                wait_blocks(0, nb + rb);
+                if (ok && steps0 > 0) scores(0, 0);
+                if (ok && steps1 > 0) scores(1, 0);
+                free_blocks(0, nb + rb);
             }
+            for (int k = 0; k < steps && ok; k++) {
+                const unsigned gv = (unsigned)(k * per + nb + rb), gk = (unsigned)((k + 1) * per);
+                wait_blocks(gv, vb);
+                if (ok && k + 1 < steps) wait_blocks(gk, nb + rb);   // (they are asked for ahead: the next scores' keys are there by now)
+#pragma unroll 1
+                for (int i = 0; i < 2 && ok; i++) {
+                    const int mine = i ? steps1 : steps0;
+                    if (k < mine) {
+                        if (!(ok = tl_wait_warp(pg_smem(&sh.p_full[i]), k & 1, &sh.fail))) break;
+                        pg_fence_after();
+                        values(i, gv, k);
+                    }
+                    if (i == 1) free_blocks(gv, vb);
+                    if (k + 1 < mine) scores(i, gk);
+                }
+                if (ok && k + 1 < steps) free_blocks(gk, nb + rb);
+            }
+            int never = 0;                                            // nothing of this CTA is in flight when its TMEM is given back
+            if (pg_elect()) pg_umma_commit(pg_smem(&sh.drained));
             __syncwarp();
+            tl_wait_warp(pg_smem(&sh.drained), 0, &never);
         }
     } else {
-        // ===== weights: a thread a row =====
+        // ===== weights: two threads a row, 64 keys of a step each =====
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TL_REGS_SOFT));
-        const int i = warp >> 2, row = row0 + i * TL_ROWS + (warp & 3) * 32 + lane, mine = i ? steps1 : steps0, pos = s.pos0 + row, key_lo = a.window > 0 ? pos - a.window + 1 : 0;
+        const int i = warp >> 3, half = (warp >> 2) & 1, in_tile = (warp & 3) * 32 + lane, row = row0 + i * TL_ROWS + in_tile, mine = i ? steps1 : steps0;
+        const int pos = s.pos0 + row, key_lo = a.window > 0 ? pos - a.window + 1 : 0, pos_first = s.pos0 + row0 + i * TL_ROWS, pos_last = s.pos0 + last(i);
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, st = tmem + lanes + i * 128, ot = tmem + lanes + TL_O + i * 128;
         const float f = a.scale * LR_LOG2E;
-        const int pos_first = s.pos0 + row0 + i * TL_ROWS, pos_last = s.pos0 + last(i);
         float base = -INFINITY, l = 0.0f;
         bool ok = true;
 #pragma unroll 1
         for (int k = 0; k < mine; k++) {
-            const int key0 = lo + k * TL_KEYS;
+            const int key0 = lo + k * TL_KEYS + half * TL_HALF;
             ok = ok && tl_wait_warp(pg_smem(&sh.s_full[i]), k & 1, &sh.fail);
-            unsigned x[TL_KEYS];
+            unsigned x[TL_HALF];
             if (ok) {
                 pg_fence_after();
 #pragma unroll
-                for (int c = 0; c < TL_KEYS; c += 16) sg_tmem16(st + c, *(unsigned(*)[16])(x + c));
+                for (int c = 0; c < TL_HALF; c += 16) sg_tmem16(st + half * TL_HALF + c, *(unsigned(*)[16])(x + c));
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                for (int c = 0; c < TL_KEYS; c++) asm volatile("" : "+r"(x[c]));
+                for (int c = 0; c < TL_HALF; c++) asm volatile("" : "+r"(x[c]));
             }
-            // scores, each rounded once, so that their differences from the base end at 0
+            // x ff are the scores in powers of 2
+            float ff = f;
+            auto scaled = [&]() {
 #pragma unroll
-            for (int c = 0; c < TL_KEYS; c += 2) {
-                const float2 y = tl_one(tl_mul2(tl_two(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), tl_two(f, f)));
-                x[c] = __float_as_uint(y.x); x[c + 1] = __float_as_uint(y.y);
-            }
-            if (key0 + TL_KEYS - 1 > pos_first || (a.window > 0 && key0 < pos_last - a.window + 1)) {
+                for (int c = 0; c < TL_HALF; c += 2) {
+                    const float2 y = tl_one(tl_mul2(tl_two(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), tl_two(f, f)));
+                    x[c] = __float_as_uint(y.x); x[c + 1] = __float_as_uint(y.y);
+                }
+                ff = 1.0f;
+            };
+            if (!(f > 0.0f)) scaled();
+            if (lo + k * TL_KEYS + TL_KEYS - 1 > pos_first || (a.window > 0 && lo + k * TL_KEYS < pos_last - a.window + 1)) {
                 const int c_lo = key_lo - key0, c_hi = pos - key0;
 #pragma unroll
-                for (int c = 0; c < TL_KEYS; c++)
+                for (int c = 0; c < TL_HALF; c++)
                     if (c > c_hi || c < c_lo) x[c] = 0xff800000u;
             }
-            float mx = __uint_as_float(x[0]);
+            float m0 = __uint_as_float(x[0]), m1 = __uint_as_float(x[1]);
 #pragma unroll
-            for (int c = 1; c + 1 < TL_KEYS; c += 2) mx = tl_max3(mx, __uint_as_float(x[c]), __uint_as_float(x[c + 1]));
-            mx = tl_max3(mx, mx, __uint_as_float(x[TL_KEYS - 1]));
-            // the sums are scaled where a row's base has to follow its largest score
-            float alpha = 1.0f;
-            if (!(mx <= base + TL_LAG)) {
-                if (base != -INFINITY) alpha = lt_exp2(base - mx);
-                base = mx;
-            }
-            if (__any_sync(0xffffffffu, alpha != 1.0f)) {
-                if (k > 0 && ok) {
-                    ok = tl_wait_warp(pg_smem(&sh.o_full[i]), (k - 1) & 1, &sh.fail);
-                    pg_fence_after();
-#pragma unroll 1
-                    for (int c = 0; c < a.vdim && ok; c += 16) {
-                        unsigned v[16];
-                        sg_tmem16(ot + c, v);
-                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-                        for (int j = 0; j < 16; j++) {
-                            asm volatile("" : "+r"(v[j]));
-                            v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
-                        }
-                        tl_store8(ot + c, v); tl_store8(ot + c + 8, v + 8);
-                    }
+            for (int c = 2; c + 3 < TL_HALF; c += 4) { m0 = tl_max3(m0, __uint_as_float(x[c]), __uint_as_float(x[c + 1])); m1 = tl_max3(m1, __uint_as_float(x[c + 2]), __uint_as_float(x[c + 3])); }
+            m0 = tl_max3(m0, __uint_as_float(x[TL_HALF - 2]), __uint_as_float(x[TL_HALF - 1]));
+            const float mx = tl_max3(m0, m1, m1) * ff;
+            // The sums are scaled where a row's base has to follow its largest score; else the halves need not meet.  (Behind this all have read S, too)
+            if (tl_sync_or(1 + i, !(mx <= base + TL_LAG))) {
+                if (half) sh.top[i][in_tile] = mx;
+                tl_sync(1 + i);
+                if (!half) sh.top[i][in_tile] = tl_max3(mx, sh.top[i][in_tile], mx);
+                tl_sync(1 + i);
+                const float both = sh.top[i][in_tile];
+                float alpha = 1.0f;
+                if (!(both <= base + TL_LAG)) {
+                    if (base != -INFINITY) alpha = lt_exp2(base - both);
+                    base = both;
                 }
-                l *= alpha;
+                if (__any_sync(0xffffffffu, alpha != 1.0f)) {
+                    if (k > 0 && ok) {
+                        ok = tl_wait_warp(pg_smem(&sh.o_full[i]), (k - 1) & 1, &sh.fail);
+                        pg_fence_after();
+#pragma unroll 1
+                        for (int c = half * 16; c < a.vdim && ok; c += 32) {
+                            unsigned v[16];
+                            sg_tmem16(ot + c, v);
+                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                            for (int j = 0; j < 16; j++) {
+                                asm volatile("" : "+r"(v[j]));
+                                v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
+                            }
+                            tl_store8(ot + c, v); tl_store8(ot + c + 8, v + 8);
+                        }
+                    }
+                    l *= alpha;
+                }
             }
             const float minus = base == -INFINITY ? 0.0f : -base;
-            const tl_f2 minus2 = tl_two(minus, minus);
-            tl_f2 sum = 0ull;
+            // score - base in one multiply-add, whose rest of the largest score's rounding is the same for the whole row; scores beyond 2^26, whose rests leave what f16 holds, are rounded first
+            if (__any_sync(0xffffffffu, fabsf(minus) >= 67108864.0f) && ff == f) scaled();
+            const tl_f2 ff2 = tl_two(ff, ff), minus2 = tl_two(minus, minus);
+            tl_f2 sum = 0ull, more = 0ull;
 #pragma unroll
-            for (int g = 0; g < TL_KEYS; g += 16) {
+            for (int g = 0; g < TL_HALF; g += 16) {
                 unsigned w[8];
 #pragma unroll
                 for (int c = 0; c < 16; c += 2) {
-                    const float2 y = tl_one(tl_add2(tl_two(__uint_as_float(x[g + c]), __uint_as_float(x[g + c + 1])), minus2));
+                    const float2 y = tl_one(tl_fma2(tl_two(__uint_as_float(x[g + c]), __uint_as_float(x[g + c + 1])), ff2, minus2));
                     const tl_f2 p = c >= TL_SFU ? tl_exp2_pair(y) : tl_two(lt_exp2(y.x), lt_exp2(y.y));
-                    sum = tl_add2(sum, p);
+                    if (c & 2) more = tl_add2(more, p);
+                    else sum = tl_add2(sum, p);
                     const float2 z = tl_one(p);
                     w[c / 2] = lt_pack(z.x, z.y);
                 }
-                if (ok) tl_store8(st + g / 2, w);
+                if (ok) tl_store8(st + half * (TL_HALF / 2) + g / 2, w);
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             pg_fence_before();
             sg_arrive(pg_smem(&sh.p_full[i]));
-            const float2 sums = tl_one(sum);
+            const float2 sums = tl_one(tl_add2(sum, more));
             l += sums.x + sums.y;
+        }
+        if (mine > 0) {
+            if (half) sh.top[i][in_tile] = l;
+            tl_sync(1 + i);
+            if (!half) sh.top[i][in_tile] += l;
+            tl_sync(1 + i);
+            l = sh.top[i][in_tile];
         }
         if (mine > 0 && ok && (ok = tl_wait_warp(pg_smem(&sh.o_full[i]), (mine - 1) & 1, &sh.fail))) {
             pg_fence_after();
@@ -513,7 +563,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
             const float by = base != base ? NAN : g / total;
             uint16_t* out = (uint16_t*)a.out + ((int64_t)(s.first + row) * a.H + head) * a.vdim;
 #pragma unroll 1
-            for (int c = 0; c < a.vdim; c += 16) {
+            for (int c = half * 16; c < a.vdim; c += 32) {
                 unsigned v[16], w[8];
                 sg_tmem16(ot + c, v);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -533,7 +583,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
     }
     pg_fence_before();
     __syncthreads();
-    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
+    if (warp == TL_SOFT + 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
     tl_report(sh.fail, err_dev, err_host);
 }
 

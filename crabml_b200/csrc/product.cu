@@ -38,10 +38,10 @@ __device__ __forceinline__ uint4 pr_pack8(const float (&v)[8]) {
                 : make_uint4(ht_pack_f16(v[0], v[1]), ht_pack_f16(v[2], v[3]), ht_pack_f16(v[4], v[5]), ht_pack_f16(v[6], v[7]));
 }
 
-#define PF_WARPS 8
+#define PF_WARPS 16
 #define PF_THREADS (PF_WARPS * 32)
-#define PF_AHEAD 4                            // runs of 32 k that a warp has under way
-#define PF_SMEM (160 * 1024)
+#define PF_AHEAD 4                            // runs of 32 k that a warp has under way: 64 KB an SM
+#define PF_SMEM (200 * 1024)
 #define PF_ROWS 32                            // rows of x; more go to the tensor cores' tiles
 // 8 numbers of a row from column c on, zeros behind its end
 __device__ __forceinline__ uint4 pf_weights(const uint16_t* row, int c, int k, bool there, bool vec) {
@@ -56,82 +56,101 @@ __device__ __forceinline__ uint4 pf_weights(const uint16_t* row, int c, int k, b
         if (c + j < k) u[j >> 1] |= (unsigned)row[c + j] << (j & 1) * 16;
     return make_uint4(u[0], u[1], u[2], u[3]);
 }
-// grid: tiles of 16 rows of W; the (up to 8 NT) rows of x lie in shared memory, `chunk` of their k at a time
+// A CTA walks over the tiles of 16 rows of W blockIdx.x, + gridDim.x, ..; its warps take a tile's runs of 32 k by turns, the loads of the next ones, also of the next tile, under way.  The rows of
+// x lie in shared memory, all of their k (`chunk`) where they fit; else a portion at a time, laid out again for every tile
 template <int NT, bool BF16>
-__global__ void __launch_bounds__(PF_THREADS) product_few_kernel(const __grid_constant__ PrArgs a) {
+__global__ void __launch_bounds__(PF_THREADS, 1) product_few_kernel(const __grid_constant__ PrArgs a) {
     extern __shared__ __align__(16) uint8_t pf_raw[];
-    __shared__ float sums[PF_WARPS][16][NT * 8 + 1];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, m0 = blockIdx.x * 16, pitch = a.chunk * 2 + 64;      // eight lanes' 16 bytes: two rows, 64 bytes each, in all banks
+    constexpr int BUFFERS = NT == 4 ? 1 : 2;
+    __shared__ float sums[BUFFERS][PF_WARPS][16][NT * 8 + 1];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, pitch = a.chunk * 2 + 64;      // eight lanes' 16 bytes: two rows, 64 bytes each, in all banks
+    const int tiles = (a.m + 15) >> 4, chunks = (a.k + a.chunk - 1) / a.chunk;
     pdl_enter();
-    const uint16_t *w0 = (const uint16_t*)a.w + (int64_t)(m0 + (lane >> 2)) * a.k, *w1 = w0 + (int64_t)8 * a.k;
-    const bool in0 = m0 + (lane >> 2) < a.m, in1 = m0 + (lane >> 2) + 8 < a.m;
-    // the tensor cores cut a sum off at 24 bits after every 16 terms, always towards zero: sums of 128 terms go to registers and are rounded there (14336 terms of one sign: off by 1.1e-5
-    // in one chain a warp)
-    float total[NT][4] = {};
-    for (int k0 = 0; k0 < a.k; k0 += a.chunk) {
-        const int depth = min(a.chunk, a.k - k0), runs = (depth + 31) / 32;
-        uint4 u[PF_AHEAD], v[PF_AHEAD];
-        auto load = [&](int i, int r) {
-            const int c = r < runs ? k0 + r * 32 + (lane & 3) * 8 : a.k;
-            u[i] = pf_weights(w0, c, a.k, in0, a.w_vec); v[i] = pf_weights(w1, c, a.k, in1, a.w_vec);
-        };
-#pragma unroll
-        for (int i = 0; i < PF_AHEAD; i++) load(i, warp + i * PF_WARPS);
-        __syncthreads();                                              // the chunk before is through
-        for (int e = tid; e < NT * 8 * runs * 4; e += PF_THREADS) {
-            const int r = e / (runs * 4), c = e % (runs * 4) * 8;
-            float x[8] = {};
-            if (r < a.rows && k0 + c < a.k) {
-                const int64_t at = (int64_t)r * a.x_stride + k0 + c;
-                if (k0 + c + 8 <= a.k) ht_read8(a.x, at, a.x_type, a.x_vec, x);
-                else
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        if (k0 + c + j < a.k) x[j] = ht_read(a.x, at + j, a.x_type);
-            }
-            *(uint4*)(pf_raw + r * pitch + c * 2) = pr_pack8<BF16>(x);
+    uint4 u[PF_AHEAD], v[PF_AHEAD];
+    // this warp's runs in order: run r of chunk lc of tile lt is the next one to be asked for
+    int lt = blockIdx.x, lc = 0, lr = warp;
+    auto runs_of = [&](int c) { return (min(a.chunk, a.k - c * a.chunk) + 31) >> 5; };
+    auto load = [&](uint4& x, uint4& y) {
+        while (lt < tiles && lr >= runs_of(lc)) {
+            lr = warp;
+            if (++lc == chunks) { lc = 0; lt += gridDim.x; }
         }
-        __syncthreads();
-        for (int r = warp; r < runs; r += PF_WARPS * PF_AHEAD) {
-            float acc[NT][4] = {};
+        if (lt >= tiles) return;
+        const int row = lt * 16 + (lane >> 2), c = lc * a.chunk + lr * 32 + (lane & 3) * 8;
+        const uint16_t* w = (const uint16_t*)a.w + (int64_t)row * a.k;
+        x = pf_weights(w, c, a.k, row < a.m, a.w_vec); y = pf_weights(w + (int64_t)8 * a.k, c, a.k, row + 8 < a.m, a.w_vec);
+        lr += PF_WARPS;
+    };
 #pragma unroll
-            for (int i = 0; i < PF_AHEAD; i++) {
-                const int here = r + i * PF_WARPS;
-                if (here < runs) {
+    for (int i = 0; i < PF_AHEAD; i++) load(u[i], v[i]);
+    int z = 0;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, z = (z + 1) % BUFFERS) {
+        // the tensor cores cut a sum off at 24 bits after every 16 terms, always towards zero: sums of 128 terms go to registers and are rounded there (14336 terms of one sign: off by 1.1e-5
+        // in one chain a warp)
+        float total[NT][4] = {};
+        for (int c = 0; c < chunks; c++) {
+            const int k0 = c * a.chunk, runs = runs_of(c);
+            if (tile == (int)blockIdx.x || chunks > 1) {
+                __syncthreads();                                      // the portion before is through
+                for (int e = tid; e < a.rows * runs * 4; e += PF_THREADS) {
+                    const int r = e / (runs * 4), col = e % (runs * 4) * 8;
+                    float x[8] = {};
+                    if (k0 + col < a.k) {
+                        const int64_t at = (int64_t)r * a.x_stride + k0 + col;
+                        if (k0 + col + 8 <= a.k) ht_read8(a.x, at, a.x_type, a.x_vec, x);
+                        else
+#pragma unroll
+                            for (int j = 0; j < 8; j++)
+                                if (k0 + col + j < a.k) x[j] = ht_read(a.x, at + j, a.x_type);
+                    }
+                    *(uint4*)(pf_raw + r * pitch + col * 2) = pr_pack8<BF16>(x);
+                }
+                __syncthreads();
+            }
+            for (int r = warp; r < runs; r += PF_WARPS * PF_AHEAD) {
+                float acc[NT][4] = {};
+#pragma unroll
+                for (int i = 0; i < PF_AHEAD; i++) {
+                    const int here = r + i * PF_WARPS;
+                    if (here >= runs) break;                          // (the loads stay in their order: the next run's are in u[0] again below)
 #pragma unroll
                     for (int n = 0; n < NT; n++) {
-                        const uint4 b = *(const uint4*)(pf_raw + (n * 8 + (lane >> 2)) * pitch + here * 64 + (lane & 3) * 16);
-                        pr_mma<BF16>(acc[n], u[i].x, v[i].x, u[i].y, v[i].y, b.x, b.y);
-                        pr_mma<BF16>(acc[n], u[i].z, v[i].z, u[i].w, v[i].w, b.z, b.w);
+                        const uint4 b = *(const uint4*)(pf_raw + min(n * 8 + (lane >> 2), a.rows - 1) * pitch + here * 64 + (lane & 3) * 16);      // rows behind the last one: any, no one reads their sums
+                        pr_mma<BF16>(acc[n], u[0].x, v[0].x, u[0].y, v[0].y, b.x, b.y);
+                        pr_mma<BF16>(acc[n], u[0].z, v[0].z, u[0].w, v[0].w, b.z, b.w);
                     }
+#pragma unroll
+                    for (int j = 0; j + 1 < PF_AHEAD; j++) { u[j] = u[j + 1]; v[j] = v[j + 1]; }
+                    load(u[PF_AHEAD - 1], v[PF_AHEAD - 1]);
                 }
-                load(i, here + PF_WARPS * PF_AHEAD);
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) total[n][j] += acc[n][j];
             }
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) total[n][j] += acc[n][j];
         }
-    }
 #pragma unroll
-    for (int n = 0; n < NT; n++)
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) sums[warp][(lane >> 2) + (j >> 1) * 8][n * 8 + (lane & 3) * 2 + (j & 1)] = total[n][j];
-    __syncthreads();
-    for (int e = tid; e < 16 * NT * 8; e += PF_THREADS) {
-        const int i = e & 15, n = e >> 4, col = m0 + i;
-        float s = 0.0f;
+            for (int j = 0; j < 4; j++) sums[z][warp][(lane >> 2) + (j >> 1) * 8][n * 8 + (lane & 3) * 2 + (j & 1)] = total[n][j];
+        __syncthreads();
+        for (int e = tid; e < 16 * a.rows; e += PF_THREADS) {
+            const int i = e & 15, n = e >> 4, col = tile * 16 + i;
+            float s = 0.0f;
 #pragma unroll
-        for (int w = 0; w < PF_WARPS; w++) s += sums[w][i][n];
-        if (col < a.m && n < a.rows) ht_write(a.out, (int64_t)n * a.m + col, a.out_type, pr_finish(a, s, n, col));
+            for (int w = 0; w < PF_WARPS; w++) s += sums[z][w][i][n];
+            if (col < a.m) ht_write(a.out, (int64_t)n * a.m + col, a.out_type, pr_finish(a, s, n, col));
+        }
+        if (BUFFERS == 1) __syncthreads();
     }
 }
 template <int NT>
 static cudaError_t pf_launch(cc_device* dev, PrArgs a, bool bf16) {
     auto kernel = bf16 ? product_few_kernel<NT, true> : product_few_kernel<NT, false>;
-    a.chunk = std::min((a.k + 63) / 64 * 64, (PF_SMEM / (NT * 8) - 64) / 128 * 64);
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PF_SMEM);
-    if (e == cudaSuccess) e = cc_launch_pdl(dev, kernel, (unsigned)((a.m + 15) / 16), PF_THREADS, (size_t)NT * 8 * (a.chunk * 2 + 64), a);
+    constexpr int room = NT == 1 ? PF_SMEM : PF_SMEM - 12 * 1024;      // beside 17 and 34 KB of sums
+    a.chunk = std::min((a.k + 63) / 64 * 64, (room / a.rows - 64) / 128 * 64);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, room);
+    if (e == cudaSuccess) e = cc_launch_pdl(dev, kernel, (unsigned)std::min((a.m + 15) / 16, dev->sm_count), PF_THREADS, (size_t)a.rows * (a.chunk * 2 + 64), a);
     dev->launches++;
     return e;
 }

@@ -79,15 +79,19 @@ __device__ __forceinline__ void pt_finish16(const PrArgs& a, const unsigned (&v)
         if (n0 + j < n_end && col < a.m) ht_write(a.out, (int64_t)(n0 + j) * a.m + col, a.out_type, y);
     }
 }
-// with the activation as a function that is known: each has its own loop
-template <class Body>
+// With the activation as a function that is known: each has its own loop.  16-bit results: by the special function unit's exponential and reciprocal, 2^-20 of a result, in a dozen instructions
+// where tanhf and a division take sixty (8 warps finished a tile of 256 x 256 no sooner than 64 steps of its products were done)
+template <bool EXACT, class Body>
 __device__ __forceinline__ void pt_with_act(int act, Body body) {
+    auto sigmoid = [](float z) { return EXACT ? act_sigmoid(z) : __fdividef(1.0f, 1.0f + __expf(-z)); };
     switch (act) {
     case CC_ACT_NONE: body([](float z) { return z; }); break;
-    case CC_ACT_GELU_TANH: body([](float z) { return act_gelu_tanh(z); }); break;
-    case CC_ACT_SIGMOID: body([](float z) { return act_sigmoid(z); }); break;
+    case CC_ACT_GELU_TANH:                                            // (1 + tanh u) / 2 = sigmoid(2 u)
+        body([=](float z) { return EXACT ? act_gelu_tanh(z) : z * sigmoid(1.5957691216057308f * fmaf(0.044715f * z, z * z, z)); });
+        break;
+    case CC_ACT_SIGMOID: body(sigmoid); break;
     case CC_ACT_RELU_SQUARED: body([](float z) { return act_relu_squared(z); }); break;
-    default: body([](float z) { return act_silu(z); });               // SWISH with alpha 1
+    default: body([=](float z) { return EXACT ? act_silu(z) : z * sigmoid(z); });      // SWISH with alpha 1
     }
 }
 __device__ __forceinline__ void pt_report(const PtShared& sh, unsigned* err_dev, unsigned* err_host) {
@@ -149,31 +153,32 @@ __global__ void __launch_bounds__(PT_THREADS, 1) product_tile_kernel(const __gri
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr unsigned idesc = pg_instr_desc(128, BN, BF16 ? 1 : 0);
-            unsigned g = 0, nth = 0;
-            bool ok = true;
-            for (int tile = first; tile < n_tiles && ok; tile += stride)
-                for (int s = 0; s < steps && ok; s++, g++) {
-                    const unsigned acc = tmem + (nth & 1u) * BN;
-                    if (s % chunk == 0) {
-                        if (!(ok = sg_wait(pg_smem(&sh.acc_empty[nth & 1u]), ((nth >> 1) & 1u) ^ 1u, &sh.fail))) break;
-                        pg_fence_after();
-                    }
-                    const unsigned slot = g % ST, at = pg_smem(ring + (size_t)slot * BYTES);
-                    if (!(ok = sg_wait(pg_smem(&sh.full[slot]), (g / ST) & 1u, &sh.fail))) break;
-                    pg_fence_after();
-                    const uint64_t x = pg_smem_desc(at), y = pg_smem_desc(at + A_BYTES);
+        constexpr unsigned idesc = pg_instr_desc(128, BN, BF16 ? 1 : 0);
+        const uint64_t ring_desc = pg_smem_desc(pg_smem(ring));
+        unsigned nth = 0, slot = 0, phase = 0;
+        bool ok = true;
+        for (int tile = first; tile < n_tiles && ok; tile += stride)
+            for (int s = 0; s < steps && ok; s++) {
+                const unsigned acc = tmem + (nth & 1u) * BN;
+                if (s % chunk == 0 && !(ok = sg_wait_warp(pg_smem(&sh.acc_empty[nth & 1u]), ((nth >> 1) & 1u) ^ 1u, &sh.fail))) break;
+                if (!(ok = sg_wait_warp(pg_smem(&sh.full[slot]), phase, &sh.fail))) break;
+                pg_fence_after();
+                const uint64_t x = ring_desc + slot * (BYTES >> 4), y = x + (A_BYTES >> 4);
+                const bool last = s % chunk == chunk - 1 || s == steps - 1;
+                if (pg_elect()) {
 #pragma unroll
                     for (int kk = 0; kk < 4; kk++) pg_umma_f16(acc, x + 2 * kk, y + 2 * kk, idesc, s % chunk > 0 || kk > 0);
                     pg_umma_commit(pg_smem(&sh.empty[slot]));
-                    if (s % chunk == chunk - 1 || s == steps - 1) pg_umma_commit(pg_smem(&sh.acc_full[nth++ & 1u]));
+                    if (last) pg_umma_commit(pg_smem(&sh.acc_full[nth & 1u]));
                 }
-            int never = 0;                                            // nothing of this CTA is in flight when its TMEM is given back
-            pg_umma_commit(pg_smem(&sh.drained));
-            sg_wait(pg_smem(&sh.drained), 0, &never);
-        }
+                __syncwarp();
+                nth += last;
+                if (++slot == ST) { slot = 0; phase ^= 1u; }
+            }
+        int never = 0;                                                // nothing of this CTA is in flight when its TMEM is given back
+        if (pg_elect()) pg_umma_commit(pg_smem(&sh.drained));
         __syncwarp();
+        sg_wait_warp(pg_smem(&sh.drained), 0, &never);
     }
     const int q = warp & 3, half = (warp - 4) >> 2;
     const unsigned lane_col = ((unsigned)(q * 32) << 16) + half * HALF;
@@ -194,7 +199,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) product_tile_kernel(const __gri
             if (!collect(nth)) break;
             const unsigned from = tmem + (nth & 1u) * BN + lane_col;
             const float bias = a.bias && col < a.m ? a.bias[col] : 0.0f;
-            pt_with_act(a.act, [&](auto act) {
+            pt_with_act<DRAIN>(a.act, [&](auto act) {
 #pragma unroll 1
                 for (int c0 = 0; c0 < HALF && n0 + c0 < a.rows; c0 += 16) {
                     unsigned v[16];
@@ -231,7 +236,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) product_tile_kernel(const __gri
         cluster.sync();
         if (warp >= 4 && !*(volatile int*)&sh.fail) {
             const float bias = a.bias && col < a.m ? a.bias[col] : 0.0f;
-            pt_with_act(a.act, [&](auto act) {
+            pt_with_act<DRAIN>(a.act, [&](auto act) {
 #pragma unroll 1
                 for (int run = part; run < RUNS && n0 + run * 16 < a.rows; run += parts) {
                     unsigned v[16];
@@ -338,33 +343,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
         __syncwarp();
     } else if (warp == 1) {
         int never = 0;                                                // nothing is in flight when the TMEM is given back
-        if (lane == 0 && rank == 1) sg_wait(pg_smem(&sh.drained), 0, &never);
-        if (lane == 0 && rank == 0) {
-            unsigned g = 0, nth = 0;
+        if (rank == 0) {
+            const uint64_t ring_desc = pg_smem_desc(pg_smem(ring));
+            unsigned nth = 0, slot = 0, phase = 0;
             bool ok = true;
             for (int tile = first; tile < n_tiles && ok; tile += stride) {
                 int mt, n0;
                 const unsigned idesc = pg_instr_desc(256, place(tile, mt, n0), BF16 ? 1 : 0);
-                for (int s = 0; s < steps && ok; s++, g++) {
+                for (int s = 0; s < steps && ok; s++) {
                     const unsigned acc = tmem + (nth & 1u) * BN;
-                    if (s % chunk == 0) {
-                        if (!(ok = sg_wait(pg_smem(&sh.acc_empty[nth & 1u]), ((nth >> 1) & 1u) ^ 1u, &sh.fail))) break;
-                        pg_fence_after();
-                    }
-                    const unsigned slot = g % ST, at = pg_smem(ring + (size_t)slot * BYTES);
-                    if (!(ok = sg_wait(pg_smem(&sh.full[slot]), (g / ST) & 1u, &sh.fail))) break;
+                    if (s % chunk == 0 && !(ok = sg_wait_warp(pg_smem(&sh.acc_empty[nth & 1u]), ((nth >> 1) & 1u) ^ 1u, &sh.fail))) break;
+                    if (!(ok = sg_wait_warp(pg_smem(&sh.full[slot]), phase, &sh.fail))) break;
                     pg_fence_after();
-                    const uint64_t x = pg_smem_desc(at), y = pg_smem_desc(at + A_BYTES);
+                    const uint64_t x = ring_desc + slot * (BYTES >> 4), y = x + (A_BYTES >> 4);
+                    const bool last = s % chunk == chunk - 1 || s == steps - 1;
+                    if (pg_elect()) {
 #pragma unroll
-                    for (int kk = 0; kk < 4; kk++) pt_umma2(acc, x + 2 * kk, y + 2 * kk, idesc, s % chunk > 0 || kk > 0);
-                    pt_commit2(pg_smem(&sh.empty[slot]));
-                    if (s % chunk == chunk - 1 || s == steps - 1) pt_commit2(pg_smem(&sh.acc_full[nth++ & 1u]));
+                        for (int kk = 0; kk < 4; kk++) pt_umma2(acc, x + 2 * kk, y + 2 * kk, idesc, s % chunk > 0 || kk > 0);
+                        pt_commit2(pg_smem(&sh.empty[slot]));
+                        if (last) pt_commit2(pg_smem(&sh.acc_full[nth & 1u]));
+                    }
+                    __syncwarp();
+                    nth += last;
+                    if (++slot == ST) { slot = 0; phase ^= 1u; }
                 }
             }
-            pt_commit2(pg_smem(&sh.drained));
-            sg_wait(pg_smem(&sh.drained), 0, &never);
+            if (pg_elect()) pt_commit2(pg_smem(&sh.drained));
+            __syncwarp();
         }
-        __syncwarp();
+        sg_wait_warp(pg_smem(&sh.drained), 0, &never);
     } else if (warp >= 4) {
         const int q = warp & 3, half = (warp - 4) >> 2;
         unsigned nth = 0;
@@ -387,7 +394,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
             }
             const unsigned from = tmem + (nth & 1u) * BN + lane_col;
             const float bias = a.bias && col < a.m ? a.bias[col] : 0.0f;
-            pt_with_act(a.act, [&](auto act) {
+            pt_with_act<DRAIN>(a.act, [&](auto act) {
 #pragma unroll 1
                 for (int c0 = 0; c0 < mine && n0 + c0 < a.rows; c0 += 16) {
                     unsigned v[16];

@@ -55,3 +55,10 @@ __host__ __device__ constexpr unsigned pg_instr_desc(int umma_m, int umma_n, int
            | ((unsigned)(umma_n >> 3) << 17)  // bits [17, 23): N >> 3
            | ((unsigned)(umma_m >> 4) << 24); // bits [24, 29): M >> 4
 }
+// One lane of a converged warp.  A warp that issues products runs its loops as a whole and lets this lane issue: its addresses and descriptors then stay in uniform registers, where
+// tcgen05.mma wants them.  (With the loops under `if (lane == 0)` each of them was moved there for each instruction: 110 cycles from one 128 x 128 x 16 product to the next, which takes 64)
+__device__ __forceinline__ bool pg_elect() {
+    unsigned r;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+    return r != 0;
+}
