@@ -1,6 +1,6 @@
 // latent_tile.cuh -- attention over pages of latent rows, expanded: many new tokens of a sequence.  Included by latent_attn.cu behind the absorbed form.
 //
-// latent_expand_kernel makes the keys U_h c and values V_h c of 128 cached rows and a run of heads: one product of 128 x (dim + vdim) x rank for each head on tcgen05.mma, the rows staying in
+// latent_expand_kernel makes the keys U_h c and values V_h c of 256 cached rows and a run of heads: one product of 256 x (dim + vdim) x rank for each head on tcgen05.mma, the rows staying in
 // shared memory for all heads.  The results go to images, f16 in the order of the 128-byte swizzle, which bulk copies bring back as they are.  r, which all heads share, is read from the pages.
 //
 // latent_tile_kernel: a CTA takes 256 tokens of a head, as two tiles of 128 rows, over the keys that they see, 128 at a time:
@@ -9,7 +9,7 @@
 // 4500 cycles for the one warp a scheduler that a tile had: 4000 tokens of 16 heads took 147 us.)  TMEM holds both S and both O (512 columns), shared memory
 // Q (96 KB) and a ring of 16 KB blocks of keys and values (128 KB).  base lags: a row's sums are scaled only when its largest score is 2^TL_LAG times what it was (sums in TMEM would have
 // to be read and written back), so that weights are up to 2^TL_LAG and f16 still holds them and all that counts beside them.
-// Warps 0-7 and 8-15 the rows of the two tiles, 16 the copies, 17 the products.  Every wait is bounded; where one ran out all roles run to their ends and the host reports it.
+// Warps 0-7 and 8-15 the rows of the two tiles, 16 the copies, 17 the products, 18 says what has come.  Every wait is bounded; where one ran out all roles run to their ends and the host reports it.
 #pragma once
 #include <cuda.h>
 
@@ -25,12 +25,13 @@
 static_assert(TL_SOFT * 32 * TL_REGS_SOFT + 128 * TL_REGS_REST <= TL_THREADS * TL_REGS, "more registers than the block was launched with");
 #define TL_BLOCK 16384                        // 128 rows of 64 f16 under the 128-byte swizzle
 #define TL_SLOTS 8
+#define TL_GROUPS 8                           // barriers of the ring: a step's keys, or its values (a wait costs the warp that issues the products 150 to 200 cycles, one for each block 1000 a step)
 #define TL_QBLOCKS 3                          // of a row of Q: dim in two, rest in one
 #define TL_SMEM ((2 * TL_QBLOCKS + TL_SLOTS) * TL_BLOCK + 1024)
 #define TL_LAG 8.0f
 #define TL_O 256                              // TMEM columns: S (and P) of the tiles at 0 and 128, O behind
 #define TL_DIM 128                            // largest dim and vdim
-#define TL_SFU 14                             // of 16 weights those that the special function unit makes
+#define TL_SFU 16                             // of 16 weights those that the special function unit makes
 
 struct TlArgs {
     LrArgs a;
@@ -72,11 +73,11 @@ __device__ __forceinline__ int tl_find(const LrArgs& a, int n, Count count, int*
     return -1;
 }
 __device__ __forceinline__ unsigned tl_at(int row, int chunk) { return (unsigned)(row * 128 + ((chunk ^ (row & 7)) << 4)); }      // chunk of 8 numbers of a row of a block
-// for warps that have nothing else to do for long: the hardware holds them for up to 2 us a look, so that they leave the issue slots to others
+// a wait that ends after some seconds, or when another one has (asked to hold the thread for up to 2 us a look, it came back later: 136 us instead of 131)
 __device__ __forceinline__ bool tl_wait(unsigned bar, unsigned parity, int* fail) {
     unsigned done = 0;
-    for (unsigned it = 0; it < (1u << 21); it++) {
-        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(done) : "r"(bar), "r"(parity), "r"(2000u) : "memory");
+    for (unsigned it = 0; it < (1u << 24); it++) {
+        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
         if (done) return true;
         if (*(volatile int*)fail) return false;
     }
@@ -97,100 +98,128 @@ __device__ __forceinline__ void tl_load_pages(const LrArgs& a, const CUtensorMap
 }
 
 // ---- keys and values of 128 rows ------------------------------------------------------------------------------------------------------------------------
+// A pair of SMs takes two tiles of 128 keys, which stay in shared memory for all heads of its run, and each of them half of a step's weights: 64 columns of U_h the even one, of V_h the other.  (A
+// tile by one SM needs all of them from L2, 32 KB for 512 cycles of products, two under way: 32 us for 4000 keys of 16 heads.)
 #define TE_THREADS 384
 #define TE_ABLOCKS (LT_RANK / 64)
-#define TE_STAGES 2
-#define TE_STAGE (2 * TL_DIM * 128)           // 64 columns of U_h and V_h
+#define TE_STAGES 4
+#define TE_STAGE (TL_DIM * 128)               // 64 columns of U_h or V_h
 #define TE_SMEM (TE_ABLOCKS * TL_BLOCK + TE_STAGES * TE_STAGE + 1024)
 struct TeShared {
     unsigned long long a_full[TE_ABLOCKS], full[TE_STAGES], empty[TE_STAGES], acc_full[2], acc_empty[2], drained;
     unsigned tmem_base;
     int fail;
 };
-// grid (key tiles, runs of heads)
-__global__ void __launch_bounds__(TE_THREADS, 1) latent_expand_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_uk, const __grid_constant__ CUtensorMap map_uv,
-                                                                      const __grid_constant__ TlArgs t, unsigned* err_dev, unsigned* err_host) {
+__device__ __forceinline__ unsigned te_even(unsigned addr) {         // the even CTA's own of it
+    unsigned a;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(addr));
+    return a;
+}
+__device__ __forceinline__ void te_expect(unsigned bar, unsigned bytes) { asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
+__device__ __forceinline__ void te_tma(unsigned dst, const void* tmap, unsigned bar, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(tmap), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void te_umma(unsigned tmem_d, uint64_t a, uint64_t b, unsigned idesc, unsigned accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// what this thread has issued so far arrives on the barrier, when it is complete, in both CTAs
+__device__ __forceinline__ void te_commit(unsigned bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+// grid (key tiles, up to a whole pair, runs of heads)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TE_THREADS, 1) latent_expand_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_uk,
+                                                                                               const __grid_constant__ CUtensorMap map_uv, const __grid_constant__ TlArgs t, unsigned* err_dev, unsigned* err_host) {
+    namespace cg = cooperative_groups;
     extern __shared__ __align__(1024) uint8_t tl_raw[];
     __shared__ TeShared sh;
     const LrArgs& a = t.a;
     uint8_t *as = (uint8_t*)(((uintptr_t)tl_raw + 1023) & ~(uintptr_t)1023), *bs = as + TE_ABLOCKS * TL_BLOCK;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, width = a.dim + a.vdim, blocks = (a.rank + 63) >> 6;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = (int)cg::this_cluster().block_rank(), wide = max(a.dim, a.vdim), blocks = (a.rank + 63) >> 6;
     const int h0 = (int)((int64_t)t.heads * blockIdx.y / gridDim.y), h1 = (int)((int64_t)t.heads * (blockIdx.y + 1) / gridDim.y);
     if (tid == 0) {
-        for (int i = 0; i < TE_ABLOCKS; i++) pg_mbar_init(pg_smem(&sh.a_full[i]), 1);
+        for (int i = 0; i < TE_ABLOCKS; i++) pg_mbar_init(pg_smem(&sh.a_full[i]), 2);
         for (int i = 0; i < TE_STAGES; i++) { pg_mbar_init(pg_smem(&sh.full[i]), 1); pg_mbar_init(pg_smem(&sh.empty[i]), 1); }
-        for (int i = 0; i < 2; i++) { pg_mbar_init(pg_smem(&sh.acc_full[i]), 1); pg_mbar_init(pg_smem(&sh.acc_empty[i]), 8); }
+        for (int i = 0; i < 2; i++) { pg_mbar_init(pg_smem(&sh.acc_full[i]), 1); pg_mbar_init(pg_smem(&sh.acc_empty[i]), 16); }
         pg_mbar_init(pg_smem(&sh.drained), 1);
         sh.fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 2) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pg_smem(&sh.tmem_base)), "n"(512) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pg_smem(&sh.tmem_base)), "n"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     pg_fence_before();
     __syncthreads();
+    cg::this_cluster().sync();
     pg_fence_after();
     const unsigned tmem = sh.tmem_base;
     pdl_enter();
-    int kt;
-    const int seq = max(0, tl_find(a, blockIdx.x, [&](const PgSeq& s) { return tl_key_tiles(s, a); }, &kt));      // (the grid has as many rows as there are tiles)
-    const PgSeq s = a.seqs[seq];
-    int from, to;
-    tl_range(s, a, &from, &to);
+    int kt = 0, from, to;
+    const int found = (int)blockIdx.x < t.key_tiles ? tl_find(a, blockIdx.x, [&](const PgSeq& s) { return tl_key_tiles(s, a); }, &kt) : -1, seq = max(0, found);
+    tl_range(a.seqs[seq], a, &from, &to);
     const int key0 = from + kt * TL_KEYS;
+    if (found < 0) to = key0;                                         // the second CTA of the last pair may have no keys
     if (warp == 0) {
         if (lane == 0) {
             for (int b = 0; b < blocks; b++) {
-                pg_mbar_expect_tx(pg_smem(&sh.a_full[b]), tl_pages(a, seq, key0, to));
-                tl_load_pages(a, &map_rows, pg_smem(as + b * TL_BLOCK), pg_smem(&sh.a_full[b]), b * 64, seq, key0, to);
+                const unsigned bar = te_even(pg_smem(&sh.a_full[b]));
+                te_expect(bar, tl_pages(a, seq, key0, to));
+                for (int i = 0; i < TL_KEYS && key0 + i < to; i += a.page)
+                    te_tma(pg_smem(as + b * TL_BLOCK) + i * 128, &map_rows, bar, b * 64, a.table[(int64_t)seq * a.table_cols + ((key0 + i) >> a.shift)] * a.page);
             }
             unsigned g = 0;
             bool ok = true;
             for (int h = h0; h < h1 && ok; h++)
                 for (int b = 0; b < blocks; b++, g++) {
-                    const unsigned slot = g % TE_STAGES, full = pg_smem(&sh.full[slot]), at = pg_smem(bs + slot * TE_STAGE);
+                    const unsigned slot = g % TE_STAGES, own = pg_smem(&sh.full[slot]);
                     if (!(ok = tl_wait(pg_smem(&sh.empty[slot]), ((g / TE_STAGES) & 1u) ^ 1u, &sh.fail))) break;
-                    pg_mbar_expect_tx(full, (unsigned)width * 128);
-                    pg_tma_load_2d(at, &map_uk, full, b * 64, (t.head0 + h) * a.dim);
-                    pg_tma_load_2d(at + a.dim * 128, &map_uv, full, b * 64, (t.head0 + h) * a.vdim);
+                    if (rank == 0) pg_mbar_expect_tx(own, (unsigned)wide * 256);
+                    te_tma(pg_smem(bs + slot * TE_STAGE), rank ? &map_uv : &map_uk, te_even(own), b * 64, (t.head0 + h) * (rank ? a.vdim : a.dim));
                 }
-            int never = 0;                                            // no copy is under way when the CTA ends
-            for (unsigned i = g > TE_STAGES ? g - TE_STAGES : 0; i < g; i++) tl_wait(pg_smem(&sh.full[i % TE_STAGES]), (i / TE_STAGES) & 1u, &never);
-            for (int b = 0; b < blocks; b++) tl_wait(pg_smem(&sh.a_full[b]), 0, &never);
+            int never = 0;                                            // no copy is under way when the CTAs end (the even one sees those of both), and no arrival
+            if (rank == 0)
+                for (int b = 0; b < blocks; b++) tl_wait(pg_smem(&sh.a_full[b]), 0, &never);
+            for (unsigned i = g > TE_STAGES ? g - TE_STAGES : 0; i < g; i++) {
+                if (rank == 0) tl_wait(pg_smem(&sh.full[i % TE_STAGES]), (i / TE_STAGES) & 1u, &never);
+                tl_wait(pg_smem(&sh.empty[i % TE_STAGES]), (i / TE_STAGES) & 1u, &never);
+            }
+            if (!ok || never)                                         // something did not come in time: a while for whatever is still to
+                for (int i = 0; i < 1000; i++) __nanosleep(1000);
         }
         __syncwarp();
     } else if (warp == 1) {
-        const unsigned idesc = pg_instr_desc(128, width);
-        const uint64_t a_desc = pg_smem_desc(pg_smem(as)), b_desc = pg_smem_desc(pg_smem(bs));
-        unsigned slot = 0, phase = 0;
-        bool ok = true;
-        for (int h = h0; h < h1 && ok; h++) {
-            const unsigned n = (unsigned)(h - h0), acc = tmem + (n & 1u) * 256;
-            if (!(ok = tl_wait_warp(pg_smem(&sh.acc_empty[n & 1u]), ((n >> 1) & 1u) ^ 1u, &sh.fail))) break;
-            for (int b = 0; b < blocks; b++) {
-                if (!(ok = (h > h0 || tl_wait_warp(pg_smem(&sh.a_full[b]), 0, &sh.fail)) && tl_wait_warp(pg_smem(&sh.full[slot]), phase, &sh.fail))) break;
-                pg_fence_after();
-                const uint64_t x = a_desc + b * (TL_BLOCK >> 4), y = b_desc + slot * (TE_STAGE >> 4);
-                const int steps = min(4, (a.rank - b * 64) >> 4);
-                if (pg_elect()) {
+        int never = 0;                                                // nothing is in flight when the TMEM is given back
+        if (rank == 0) {
+            const unsigned idesc = pg_instr_desc(256, 2 * wide);
+            const uint64_t a_desc = pg_smem_desc(pg_smem(as)), b_desc = pg_smem_desc(pg_smem(bs));
+            unsigned slot = 0, phase = 0;
+            bool ok = true;
+            for (int h = h0; h < h1 && ok; h++) {
+                const unsigned n = (unsigned)(h - h0), acc = tmem + (n & 1u) * 256;
+                if (!(ok = tl_wait_warp(pg_smem(&sh.acc_empty[n & 1u]), ((n >> 1) & 1u) ^ 1u, &sh.fail))) break;
+                for (int b = 0; b < blocks; b++) {
+                    if (!(ok = (h > h0 || tl_wait_warp(pg_smem(&sh.a_full[b]), 0, &sh.fail)) && tl_wait_warp(pg_smem(&sh.full[slot]), phase, &sh.fail))) break;
+                    pg_fence_after();
+                    const uint64_t x = a_desc + b * (TL_BLOCK >> 4), y = b_desc + slot * (TE_STAGE >> 4);
+                    const int steps = min(4, (a.rank - b * 64) >> 4);
+                    if (pg_elect()) {
 #pragma unroll
-                    for (int kk = 0; kk < 4; kk++)
-                        if (kk < steps) pg_umma_f16(acc, x + 2 * kk, y + 2 * kk, idesc, b > 0 || kk > 0);
-                    pg_umma_commit(pg_smem(&sh.empty[slot]));
-                    if (b == blocks - 1) pg_umma_commit(pg_smem(&sh.acc_full[n & 1u]));
+                        for (int kk = 0; kk < 4; kk++)
+                            if (kk < steps) te_umma(acc, x + 2 * kk, y + 2 * kk, idesc, b > 0 || kk > 0);
+                        te_commit(pg_smem(&sh.empty[slot]));
+                        if (b == blocks - 1) te_commit(pg_smem(&sh.acc_full[n & 1u]));
+                    }
+                    __syncwarp();
+                    if (++slot == TE_STAGES) { slot = 0; phase ^= 1u; }
                 }
-                __syncwarp();
-                if (++slot == TE_STAGES) { slot = 0; phase ^= 1u; }
             }
+            if (pg_elect()) te_commit(pg_smem(&sh.drained));
+            __syncwarp();
         }
-        int never = 0;                                                // nothing of this CTA is in flight when its TMEM is given back
-        if (pg_elect()) pg_umma_commit(pg_smem(&sh.drained));
-        __syncwarp();
         tl_wait_warp(pg_smem(&sh.drained), 0, &never);
     } else if (warp >= 4) {
         // a lane a key, the two warps of its lanes every second run of 16 columns
-        const int q = warp & 3, row = q * 32 + lane;
+        const int q = warp & 3, row = q * 32 + lane, width = a.dim + a.vdim;
         const bool in = key0 + row < to;
         for (int h = h0; h < h1; h++) {
             const unsigned n = (unsigned)(h - h0);
@@ -199,11 +228,12 @@ __global__ void __launch_bounds__(TE_THREADS, 1) latent_expand_kernel(const __gr
             const size_t image = (size_t)blockIdx.x * t.heads + h;
             uint8_t *ki = t.k_image + image * ((a.dim + 63) >> 6) * TL_BLOCK, *vi = t.v_image + image * ((a.vdim + 63) >> 6) * TL_BLOCK;
             for (int c = ((warp - 4) >> 2) * 16; c < width; c += 32) {
+                const bool is_k = c < a.dim;
+                const int col = is_k ? c : c - a.dim;
                 unsigned v[16], w[8];
-                sg_tmem16(tmem + (n & 1u) * 256 + ((unsigned)(q * 32) << 16) + c, v);
+                sg_tmem16(tmem + (n & 1u) * 256 + ((unsigned)(q * 32) << 16) + (is_k ? 0 : wide) + col, v);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                 // a cached row that is not finite makes all of its keys and values so: a NaN in a key reaches the queries that see it, a zero in its value no one
-                const bool is_k = c < a.dim;
 #pragma unroll
                 for (int j = 0; j < 16; j++) {
                     asm volatile("" : "+r"(v[j]));
@@ -212,24 +242,27 @@ __global__ void __launch_bounds__(TE_THREADS, 1) latent_expand_kernel(const __gr
                 }
 #pragma unroll
                 for (int j = 0; j < 8; j++) w[j] = ht_pack_f16(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
-                const int col = is_k ? c : c - a.dim;
                 uint8_t* at = (is_k ? ki : vi) + (col >> 6) * TL_BLOCK;
-                *(uint4*)(at + tl_at(row, (col & 63) >> 3)) = make_uint4(w[0], w[1], w[2], w[3]);
-                *(uint4*)(at + tl_at(row, ((col & 63) >> 3) + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
+                if ((int)blockIdx.x < t.key_tiles) {
+                    *(uint4*)(at + tl_at(row, (col & 63) >> 3)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    *(uint4*)(at + tl_at(row, ((col & 63) >> 3) + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
+                }
             }
             pg_fence_before();
-            sg_arrive(pg_smem(&sh.acc_empty[n & 1u]));
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(te_even(pg_smem(&sh.acc_empty[n & 1u]))) : "memory");
         }
     }
     pg_fence_before();
     __syncthreads();
-    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
+    cg::this_cluster().sync();
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
     tl_report(sh.fail, err_dev, err_host);
 }
 
 // ---- attention -----------------------------------------------------------------------------------------------------------------------------------------------
 struct TlShared {
-    unsigned long long q_full, full[TL_SLOTS], empty[TL_SLOTS], s_full[2], p_full[2], o_full[2], drained;
+    unsigned long long q_full, full[TL_GROUPS], empty[TL_GROUPS], s_full[2], p_full[2], o_full[2], drained;
     unsigned tmem_base;
     int fail;
     float top[2][TL_ROWS];                    // what the two threads of a row tell each other
@@ -309,8 +342,8 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
     const int nb = (a.dim + 63) >> 6, rb = a.rest ? 1 : 0, vb = (a.vdim + 63) >> 6;      // blocks of keys, of r, of values
     if (tid == 0) {
         pg_mbar_init(pg_smem(&sh.q_full), 1);
-        for (int i = 0; i < TL_SLOTS; i++) { pg_mbar_init(pg_smem(&sh.full[i]), 1); pg_mbar_init(pg_smem(&sh.empty[i]), 1); }
-        for (int i = 0; i < 2; i++) { pg_mbar_init(pg_smem(&sh.s_full[i]), 1); pg_mbar_init(pg_smem(&sh.p_full[i]), TL_SOFT / 2); pg_mbar_init(pg_smem(&sh.o_full[i]), 1); }
+        for (int i = 0; i < TL_GROUPS; i++) { pg_mbar_init(pg_smem(&sh.full[i]), 1); pg_mbar_init(pg_smem(&sh.empty[i]), 1); }
+        for (int i = 0; i < 2; i++) { pg_mbar_init(pg_smem(&sh.s_full[i]), 1); pg_mbar_init(pg_smem(&sh.p_full[i]), TL_SOFT / 2 + 1); pg_mbar_init(pg_smem(&sh.o_full[i]), 1); }
         pg_mbar_init(pg_smem(&sh.drained), 1);
         sh.fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -347,25 +380,29 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
                 for (int i = 0; i < 2; i++)
                     for (int b = 0; b < nb + rb; b++)
                         pg_tma_load_2d(pg_smem(qs + (i * TL_QBLOCKS + b) * TL_BLOCK), &map_q, pg_smem(&sh.q_full), head * width + (b < nb ? b * 64 : a.dim), s.first + row0 + i * TL_ROWS);
-                unsigned g = 0;
+                unsigned g = 0, groups = 0;
                 bool ok = true;
                 for (int k = 0; k < steps && ok; k++) {
                     const size_t image = (size_t)(kt0 + k) * t.heads + head_at;
                     for (int b = 0; b < per; b++, g++) {
-                        const unsigned slot = g % TL_SLOTS, full = pg_smem(&sh.full[slot]), at = pg_smem(ring + slot * TL_BLOCK);
-                        if (!(ok = tl_wait(pg_smem(&sh.empty[slot]), ((g / TL_SLOTS) & 1u) ^ 1u, &sh.fail))) break;
-                        if (b >= nb && b < nb + rb) {
-                            pg_mbar_expect_tx(full, tl_pages(a, seq, lo + k * TL_KEYS, to));
-                            tl_load_pages(a, &map_rows, at, full, a.rank, seq, lo + k * TL_KEYS, to);
-                        } else {
+                        const unsigned at = pg_smem(ring + g % TL_SLOTS * TL_BLOCK), full = pg_smem(&sh.full[(2 * k + (b >= nb + rb)) % TL_GROUPS]);
+                        if (g >= TL_SLOTS) {                          // the group of the block that was here is through
+                            const unsigned was = g - TL_SLOTS, of = 2 * (was / per) + (was % per >= (unsigned)(nb + rb));
+                            if (!(ok = tl_wait(pg_smem(&sh.empty[of % TL_GROUPS]), (of / TL_GROUPS) & 1u, &sh.fail))) break;
+                        }
+                        if (b == 0) { pg_mbar_expect_tx(full, (unsigned)(nb * TL_BLOCK) + (rb ? tl_pages(a, seq, lo + k * TL_KEYS, to) : 0u)); groups++; }
+                        if (b == nb + rb) { pg_mbar_expect_tx(full, (unsigned)(vb * TL_BLOCK)); groups++; }
+                        if (b >= nb && b < nb + rb) tl_load_pages(a, &map_rows, at, full, a.rank, seq, lo + k * TL_KEYS, to);
+                        else {
                             const uint8_t* src = b < nb ? t.k_image + (image * nb + b) * TL_BLOCK : t.v_image + (image * vb + b - nb - rb) * TL_BLOCK;
-                            pg_mbar_expect_tx(full, TL_BLOCK);
                             asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(at), "l"(src), "r"(TL_BLOCK), "r"(full) : "memory");
                         }
                     }
                 }
-                int never = 0;                                        // no copy is under way when the CTA ends
-                for (unsigned i = g > TL_SLOTS ? g - TL_SLOTS : 0; i < g; i++) tl_wait(pg_smem(&sh.full[i % TL_SLOTS]), (i / TL_SLOTS) & 1u, &never);
+                // no copy is under way when the CTA ends.  Where a wait ran out in the midst of a group, what it lacks never comes: a while for what does
+                int never = 0;
+                if (ok) for (unsigned i = groups > TL_GROUPS ? groups - TL_GROUPS : 0; i < groups; i++) tl_wait(pg_smem(&sh.full[i % TL_GROUPS]), (i / TL_GROUPS) & 1u, &never);
+                else for (int i = 0; i < 1000; i++) __nanosleep(1000);
                 tl_wait(pg_smem(&sh.q_full), 0, &never);
             }
             __syncwarp();
@@ -374,13 +411,8 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
             const unsigned idesc_s = pg_instr_desc(128, TL_KEYS), idesc_o = pg_instr_desc(128, a.vdim) | 1u << 16, idesc_lo = pg_instr_desc(128, 64) | 1u << 16, idesc_hi = pg_instr_desc(128, a.vdim - 64) | 1u << 16;
             const uint64_t q_desc = pg_smem_desc(pg_smem(qs)), ring_desc = pg_smem_desc(pg_smem(ring)), v_desc = tl_desc_mn(pg_smem(ring), TL_BLOCK);
             bool ok = tl_wait_warp(pg_smem(&sh.q_full), 0, &sh.fail);
-            auto wait_blocks = [&](unsigned g, int n) {
-                for (int b = 0; b < n && ok; b++, g++) ok = tl_wait_warp(pg_smem(&sh.full[g % TL_SLOTS]), (g / TL_SLOTS) & 1u, &sh.fail);
-                pg_fence_after();
-            };
-            auto free_blocks = [&](unsigned g, int n) {
-                if (pg_elect())
-                    for (int b = 0; b < n; b++, g++) pg_umma_commit(pg_smem(&sh.empty[g % TL_SLOTS]));
+            auto free_group = [&](int g) {
+                if (pg_elect()) pg_umma_commit(pg_smem(&sh.empty[g % TL_GROUPS]));
                 __syncwarp();
             };
             auto scores = [&](int i, unsigned g) {                   // of tile i against the keys in blocks g ..
@@ -417,32 +449,40 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
                 __syncwarp();
             };
             if (ok && steps > 0) {
-                wait_blocks(0, nb + rb);
+                ok = tl_wait_warp(pg_smem(&sh.full[0]), 0, &sh.fail);
+                pg_fence_after();
                 if (ok && steps0 > 0) scores(0, 0);
                 if (ok && steps1 > 0) scores(1, 0);
-                free_blocks(0, nb + rb);
+                free_group(0);
             }
             for (int k = 0; k < steps && ok; k++) {
                 const unsigned gv = (unsigned)(k * per + nb + rb), gk = (unsigned)((k + 1) * per);
-                wait_blocks(gv, vb);
-                if (ok && k + 1 < steps) wait_blocks(gk, nb + rb);   // (they are asked for ahead: the next scores' keys are there by now)
 #pragma unroll 1
                 for (int i = 0; i < 2 && ok; i++) {
                     const int mine = i ? steps1 : steps0;
                     if (k < mine) {
-                        if (!(ok = tl_wait_warp(pg_smem(&sh.p_full[i]), k & 1, &sh.fail))) break;
+                        if (!(ok = tl_wait_warp(pg_smem(&sh.p_full[i]), k & 1, &sh.fail))) break;      // weights, values and the next keys
                         pg_fence_after();
                         values(i, gv, k);
                     }
-                    if (i == 1) free_blocks(gv, vb);
+                    if (i == 1) free_group(2 * k + 1);
                     if (k + 1 < mine) scores(i, gk);
                 }
-                if (ok && k + 1 < steps) free_blocks(gk, nb + rb);
+                if (ok && k + 1 < steps) free_group(2 * k + 2);
             }
             int never = 0;                                            // nothing of this CTA is in flight when its TMEM is given back
             if (pg_elect()) pg_umma_commit(pg_smem(&sh.drained));
             __syncwarp();
             tl_wait_warp(pg_smem(&sh.drained), 0, &never);
+        } else if (warp == TL_SOFT + 2) {
+            // ===== a step's values and the next one's keys are there: said where the products wait for the weights, so that they wait once (200 to 350 cycles each, among 16 busy warps) =====
+            bool ok = true;
+            for (int k = 0; k < steps && ok; k++) {
+                ok = tl_wait_warp(pg_smem(&sh.full[(2 * k + 1) % TL_GROUPS]), ((2 * k + 1) / TL_GROUPS) & 1, &sh.fail);
+                if (ok && k + 1 < steps) ok = tl_wait_warp(pg_smem(&sh.full[(2 * k + 2) % TL_GROUPS]), ((2 * k + 2) / TL_GROUPS) & 1, &sh.fail);
+                if (k < steps0) sg_arrive(pg_smem(&sh.p_full[0]));
+                if (k < steps1) sg_arrive(pg_smem(&sh.p_full[1]));
+            }
         }
     } else {
         // ===== weights: two threads a row, 64 keys of a step each =====
@@ -593,8 +633,9 @@ static int tl_run(cc_device* dev, const cc_page_plan* plan, const LrArgs& all) {
     CUtensorMap rows, q, uk, uv;
     int rc = cc_make_tmap_rows(dev, &rows, all.rows, plan->n_pages * plan->page, all.cols, (int64_t)all.cols * 2, plan->page, false);
     if (!rc) rc = cc_make_tmap_rows(dev, &q, all.q, plan->tokens, all.H * width, all.H * width * 2, TL_ROWS, false);
-    if (!rc) rc = cc_make_tmap_rows(dev, &uk, all.uk, (int64_t)all.H * all.dim, all.rank, (int64_t)all.rank * 2, all.dim, false);
-    if (!rc) rc = cc_make_tmap_rows(dev, &uv, all.uv, (int64_t)all.H * all.vdim, all.rank, (int64_t)all.rank * 2, all.vdim, false);
+    const int wide = std::max(all.dim, all.vdim);
+    if (!rc) rc = cc_make_tmap_rows(dev, &uk, all.uk, (int64_t)all.H * all.dim, all.rank, (int64_t)all.rank * 2, wide, false);
+    if (!rc) rc = cc_make_tmap_rows(dev, &uv, all.uv, (int64_t)all.H * all.vdim, all.rank, (int64_t)all.rank * 2, wide, false);
     if (rc) return rc;
     CC_CUDA(dev, cudaFuncSetAttribute(latent_expand_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TE_SMEM));
     CC_CUDA(dev, cudaFuncSetAttribute(latent_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TL_SMEM));
@@ -620,8 +661,8 @@ static int tl_run(cc_device* dev, const cc_page_plan* plan, const LrArgs& all) {
         cudaError_t e = cudaSuccess;
         for (t.head0 = 0; t.head0 < all.H && e == cudaSuccess; t.head0 += heads) {
             t.heads = std::min(heads, all.H - t.head0);
-            const int runs = (int)std::max<int64_t>(1, std::min<int64_t>(t.heads, dev->sm_count / tiles));
-            e = cc_launch_pdl(dev, latent_expand_kernel, dim3((unsigned)tiles, (unsigned)runs), TE_THREADS, TE_SMEM, rows, uk, uv, t, dev->err_dev, dev->err_host);
+            const int runs = (int)std::max<int64_t>(1, std::min<int64_t>(t.heads, dev->sm_count / (tiles + 1)));
+            e = cc_launch_pdl(dev, latent_expand_kernel, dim3((unsigned)(tiles + 1) / 2 * 2, (unsigned)runs), TE_THREADS, TE_SMEM, rows, uk, uv, t, dev->err_dev, dev->err_host);
             if (e == cudaSuccess) e = cc_launch_pdl(dev, latent_tile_kernel, (unsigned)(items * t.heads), TL_THREADS, TL_SMEM, rows, q, t, dev->err_dev, dev->err_host);
             dev->launches += 2;
         }
