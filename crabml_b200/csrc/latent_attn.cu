@@ -3,27 +3,35 @@
 //
 // A row of the scores is a query of one head: 16 heads of one token are 16 rows over the same keys, one tile of mma.sync.m16n8k16.  One token of 16 heads over rows of 512 + 64
 // makes 30 operations a byte of the cache, so bytes bound it, as long as every row comes from memory once: a CTA (one per SM) brings 32 rows at a time into a ring of shared memory
-// by bulk copies, a warp of its own issuing them, and 8 warps take them twice, as keys and as values:
+// by copies of 64 columns, and 8 warps take them twice, as keys and as values:
 //   scores   warp w adds up the columns 16 (w % 4 + 4 i) of 16 keys (w / 4); the queries stay in registers, sums of the four column groups meet in shared memory
-//   weights  a thread 2 (or 4) keys of a row: exp2(score - largest), rounded to f16, back to shared memory
+//   weights  a thread two keys of a row: exp2(score - largest), rounded to f16, back to shared memory
 //   values   warp w adds up the columns 16 (w + 8 i) of all rows in registers; scaled when a row's largest score grows
-// One barrier a step: scores of step k and values of step k - 1 lie on the same side of it.
+// That is a chain of 2700 cycles a step, mostly latencies, while the step's bytes take 1600; so two such groups of 8 warps take the steps by turns and add up their sums at a segment's end.
 // All steps of a call are dealt out in equal runs over the SMs; sums of cut segments are joined by latent_join_kernel.
 //
 // Sums, largest scores and sums of weights have 32 bits; queries on their way to the latents are brought near 2^4 by a power of two and rounded to f16, weights are rounded to f16 near
 // 2^10 (2^-11 of each: the operands of the tensor cores; the result is rounded to 16 bits anyway), sums of latents enter the last product as two f16 numbers.
+#include <cuda.h>
+
 #include <algorithm>
 
 #include "latent.cuh"
 #include "split_gemm.cuh"
 
-#define LR_WARPS 8
-#define LR_CONS (LR_WARPS * 32)
-#define LR_THREADS (LR_CONS + 32)
+#define LR_GROUPS 2
+#define LR_THREADS (LR_GROUPS * 256)
+#define LR_ALL (LR_THREADS + 128)             // a warp more brings the rows
+// 640 threads of 96 registers at launch are 512 of 112 and 128 of 32 afterwards
+#define LR_REGS 112
+#define LR_REGS_REST 32
+static_assert(LR_THREADS * LR_REGS + 128 * LR_REGS_REST <= LR_ALL * 96, "more registers than the block was launched with");
+#define LR_BLOCK 4096                         // 32 rows of 64 columns
+#define LR_ROWS 16                            // queries of a tile
 #define LR_KEYS 32                            // of a step
 #define LR_BEGIN 4                            // what a segment's begin and end cost, in steps
 #define LR_SLOTS 8                            // most slots of the ring
-#define LR_SMEM (226 * 1024)
+#define LR_SMEM (226 * 1024)                  // with what stands in LrShared
 #define LR_SHIFT 10.0f                        // weights are exp2(score - largest + LR_SHIFT)
 #define LR_KB 9                               // column blocks of 16 of a warp's scores: (LT_RANK + LT_REST) / 16 / 4
 #define LR_VB 4                               // .. of its values: LT_RANK / 16 / 8
@@ -38,8 +46,8 @@ struct LrArgs {
     const int* table;
     const __half *rows, *q, *uk, *uv;
     const float* sink;
-    float *qf, *lat, *part;                   // queries over the latents [T H][cols]; results over the latents [T H][rank]; sums of cut segments [2 x CTA][16 MT][rank]
-    float2* ml;                               // [2 x CTA][16 MT]: largest score (base 2), sum of weights
+    float *qf, *lat, *part;                   // queries over the latents [T H][cols]; results over the latents [T H][rank]; sums of cut segments [2 x CTA][LR_ROWS][rank]
+    float2* ml;                               // [2 x CTA][LR_ROWS]: largest score (base 2), sum of weights
     void* out;
     float scale;
     int n_seqs, table_cols, page, shift, H, dim, vdim, rank, rest, cols, window, most, out_bf16, slots;      // most: sequences with more new tokens take the other form
@@ -49,9 +57,9 @@ struct LrCuts { struct { int seq, tile, slot, cta, n; } at[LR_CTAS]; };
 
 __host__ __device__ __forceinline__ void lr_range(const PgSeq& s, const LrArgs& a, int* from, int* to) {
     *to = s.pos0 + s.count;
-    *from = a.window > 0 && s.pos0 - a.window + 1 > 0 ? s.pos0 - a.window + 1 : 0;
+    *from = a.window > 0 && s.pos0 - a.window + 1 > 0 ? (s.pos0 - a.window + 1) & ~(LR_KEYS - 1) : 0;      // steps are whole pages, or parts of one
 }
-__host__ __device__ __forceinline__ int lr_tiles(const PgSeq& s, const LrArgs& a, int rows) { return s.count > a.most ? 0 : (int)(((int64_t)s.count * a.H + rows - 1) / rows); }
+__host__ __device__ __forceinline__ int lr_tiles(const PgSeq& s, const LrArgs& a) { return s.count > a.most ? 0 : (int)(((int64_t)s.count * a.H + LR_ROWS - 1) / LR_ROWS); }
 __host__ __device__ __forceinline__ int lr_steps(const PgSeq& s, const LrArgs& a) {
     int from, to;
     lr_range(s, a, &from, &to);
@@ -194,320 +202,354 @@ __global__ void __launch_bounds__(128) latent_unfold_kernel(const LrArgs a, cons
 }
 
 // ---- the cached rows as keys and values ----------------------------------------------------------------------------------------------------------
-template <int MT>
 struct LrShared {
     unsigned long long full[LR_SLOTS], empty[LR_SLOTS];
     int fail;
     unsigned wild;                            // rows whose sums are not finite
-    float top[16 * MT], sum[16 * MT], inv[16 * MT];      // of a segment: factor of a row's scores, then its largest score and sum of weights; what a row is divided by
-    float alpha[2][16 * MT];
-    __align__(16) float sums[2][4][16 * MT][40];      // of a step: scores by column groups
-    __align__(16) __half p[2][16 * MT][40];
+    float top[LR_GROUPS][LR_ROWS], sum[LR_GROUPS][LR_ROWS];      // of a segment: largest score and sum of weights of each group
+    float factor[LR_ROWS], up[LR_ROWS];       // of a row's scores; what its query is multiplied by
+    float alpha[LR_GROUPS][LR_ROWS];
+    __align__(16) float sums[LR_GROUPS][4][LR_ROWS][40];      // of a step: scores by column groups.  At a segment's end, sums on their way from group to group
+    __align__(16) __half p[LR_GROUPS][LR_ROWS][40];
 };
-__device__ __forceinline__ void lr_sync() { asm volatile("bar.sync 1, %0;" ::"n"(LR_CONS) : "memory"); }
-__device__ __forceinline__ bool lr_sync_or(bool x) {
+static_assert(sizeof(float) * LR_GROUPS * 4 * LR_ROWS * 40 >= LR_THREADS / LR_GROUPS * 16 * sizeof(float), "half of a group's sums");
+__device__ __forceinline__ void lr_sync(int group) { asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(LR_THREADS / LR_GROUPS) : "memory"); }
+__device__ __forceinline__ bool lr_sync_or(int group, bool x) {
     unsigned r;
-    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbar.red.or.pred q, 1, %2, p;\nselp.u32 %0, 1, 0, q;\n}\n" : "=r"(r) : "r"((unsigned)x), "n"(LR_CONS) : "memory");
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbar.red.or.pred q, %2, %3, p;\nselp.u32 %0, 1, 0, q;\n}\n" : "=r"(r) : "r"((unsigned)x), "r"(1 + group), "n"(LR_THREADS / LR_GROUPS) : "memory");
     return r;
 }
-// Values that are not finite, times the weight 0 of a row that does not see them, make a NaN.  Rows whose sums hold one though their scores do not are added up again, one by one, over
-// the keys that they see: a dot product over the block, which then adds 2 columns a thread.
-template <int MT>
-__device__ __noinline__ void lr_again(const LrArgs& a, LrShared<MT>& sh, const PgSeq s, int seq, int row0, int lo, int hi, float* lat, int64_t lat_stride) {
-    for (unsigned left = sh.wild; left; left &= left - 1) {
-        const int r = __ffs(left) - 1, tok = (row0 + r) / a.H, pos = s.pos0 + tok;
-        const float* q = a.qf + ((int64_t)s.first * a.H + row0 + r) * a.cols;
-        const float m = sh.top[r];
-        float o0 = 0.0f, o1 = 0.0f;
-        const int c = threadIdx.x * 2;
-        for (int key = max(lo, a.window > 0 ? pos - a.window + 1 : 0); key <= min(hi - 1, pos); key++) {
-            const __half* row = a.rows + ((int64_t)a.table[(int64_t)seq * a.table_cols + (key >> a.shift)] * a.page + (key & (a.page - 1))) * a.cols;
-            float d = 0.0f;
-            for (int e = threadIdx.x; e < a.cols; e += LR_CONS) d = fmaf(q[e], __half2float(row[e]), d);
-            d = warp_sum(d);
-            if ((threadIdx.x & 31) == 0) sh.sums[0][0][0][threadIdx.x >> 5] = d;
-            lr_sync();
-            d = 0.0f;
-#pragma unroll
-            for (int w = 0; w < LR_WARPS; w++) d += sh.sums[0][0][0][w];
-            lr_sync();
-            const float p = lt_exp2(d * (a.scale * LR_LOG2E) - m + LR_SHIFT);
-            if (c < a.rank) { o0 = fmaf(p, __half2float(row[c]), o0); o1 = fmaf(p, __half2float(row[c + 1]), o1); }
-        }
-        if (c < a.rank) { lat[r * lat_stride + c] = o0 * sh.inv[r]; lat[r * lat_stride + c + 1] = o1 * sh.inv[r]; }
-    }
+__device__ __forceinline__ void lr_sync_all() { asm volatile("bar.sync 3, %0;" ::"n"(LR_THREADS) : "memory"); }
+__device__ __forceinline__ bool lr_sync_all_or(bool x) {
+    unsigned r;
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbar.red.or.pred q, 3, %2, p;\nselp.u32 %0, 1, 0, q;\n}\n" : "=r"(r) : "r"((unsigned)x), "n"(LR_THREADS) : "memory");
+    return r;
 }
+__device__ __forceinline__ void lr_zero(unsigned at) { asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory"); }
+// a CTA's run of steps, segment by segment; the begin of a segment counts LR_BEGIN of them
+struct LrWalk {
+    int seq, tile, off, left;
+    // the next piece: false at the end.  first and last step of its keys; whether others have the rest of the segment
+    template <class F>
+    __device__ __forceinline__ bool piece(const LrArgs& a, F body) {
+        while (left > 0 && seq < a.n_seqs) {
+            const PgSeq s = a.seqs[seq];
+            if (tile >= lr_tiles(s, a)) { seq++; tile = 0; off = 0; continue; }
+            const int all = lr_steps(s, a), take = min(left, all - off), from = off;
+            left -= take;
+            body(s, seq, tile, max(from - LR_BEGIN, 0), max(from + take - LR_BEGIN, 0), from > LR_BEGIN || from + take < all);
+            if (from + take == all) { tile++; off = 0; } else off += take;
+            return true;
+        }
+        return false;
+    }
+};
+// Values that are not finite, times the weight 0 of a row that does not see them, make a NaN.  Rows whose sums hold one though their scores do not are added up again, one by one, over
+// the keys that they see: a dot product over the block, which then adds a column a thread.
+__device__ __noinline__ void lr_again(const LrArgs& a, LrShared& sh, const PgSeq s, int seq, int row0, int lo, int hi, float m, float by, int r, float* lat) {
+    const int tok = (row0 + r) / a.H, pos = s.pos0 + tok, c = threadIdx.x;
+    const float* q = a.qf + ((int64_t)s.first * a.H + row0 + r) * a.cols;
+    float o = 0.0f;
+    for (int key = max(lo, a.window > 0 ? pos - a.window + 1 : 0); key <= min(hi - 1, pos); key++) {
+        const __half* row = a.rows + ((int64_t)a.table[(int64_t)seq * a.table_cols + (key >> a.shift)] * a.page + (key & (a.page - 1))) * a.cols;
+        float d = 0.0f;
+        for (int e = threadIdx.x; e < a.cols; e += LR_THREADS) d = fmaf(q[e], __half2float(row[e]), d);
+        d = warp_sum(d);
+        if ((threadIdx.x & 31) == 0) sh.sums[0][0][0][threadIdx.x >> 5] = d;
+        lr_sync_all();
+        d = 0.0f;
+#pragma unroll
+        for (int w = 0; w < LR_THREADS / 32; w++) d += sh.sums[0][0][0][w];
+        lr_sync_all();
+        const float p = lt_exp2(d * (a.scale * LR_LOG2E) - m + LR_SHIFT);
+        if (c < a.rank) o = fmaf(p, __half2float(row[c]), o);
+    }
+    if (c < a.rank) lat[c] = o * by;
+}
+static_assert(LR_THREADS >= LT_RANK, "a thread a column");
 
-template <int MT>
-__global__ void __launch_bounds__(LR_THREADS, 1) latent_rows_kernel(const __grid_constant__ LrArgs a, const __grid_constant__ LrDeal deal, unsigned* err_dev, unsigned* err_host) {
-    extern __shared__ __align__(16) uint8_t lr_raw[];
-    __shared__ LrShared<MT> sh;
-    constexpr int ROWS = 16 * MT, LANES = LR_CONS / ROWS, PER = LR_KEYS / LANES;      // threads of a row in a step's weights, and the keys of each
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const unsigned pitch = (unsigned)a.cols * 2 + 16, ring = pg_smem(lr_raw), slot_bytes = LR_KEYS * pitch;      // a row's pitch is an odd number of 16 bytes: ldmatrix without conflicts
+__global__ void __launch_bounds__(LR_ALL, 1) latent_rows_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ LrArgs a, const __grid_constant__ LrDeal deal, unsigned* err_dev,
+                                                                unsigned* err_host) {
+    extern __shared__ __align__(1024) uint8_t lr_raw[];
+    __shared__ LrShared sh;
+    const int tid = threadIdx.x, lane = tid & 31, group = tid / (LR_THREADS / LR_GROUPS), in_group = tid % (LR_THREADS / LR_GROUPS), warp = in_group >> 5;
+    const unsigned ring = (pg_smem(lr_raw) + 1023) & ~1023u, slot_bytes = (unsigned)((a.cols + 63) >> 6) * LR_BLOCK;
     if (tid == 0) {
-        for (int i = 0; i < a.slots; i++) { pg_mbar_init(pg_smem(&sh.full[i]), 1); pg_mbar_init(pg_smem(&sh.empty[i]), LR_WARPS); }
+        for (int i = 0; i < a.slots; i++) { pg_mbar_init(pg_smem(&sh.full[i]), 1); pg_mbar_init(pg_smem(&sh.empty[i]), 8); }
         sh.fail = 0; sh.wild = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    // keys behind a segment's last one have the weight 0, and zeros, or a row from before, in their place
-    for (unsigned i = tid * 16; i < a.slots * slot_bytes; i += LR_THREADS * 16) *(uint4*)(lr_raw + i) = make_uint4(0, 0, 0, 0);
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     pdl_enter();
     __syncthreads();
-    const int c = blockIdx.x;
-    int seq = deal.at[c].seq, tile = deal.at[c].tile, off = deal.at[c].off, left = deal.run_lo + (c < deal.run_more ? 1 : 0);
-    unsigned slot = 0, phase = 0;
-    bool ok = true;
-    auto advance = [&]() { if (++slot == (unsigned)a.slots) { slot = 0; phase ^= 1u; } };
-    // the segments of this CTA's run: body(sequence, first and last step of its keys, whether it is cut)
-    auto walk = [&](auto body) {
-        bool first = true;
-        while (left > 0 && seq < a.n_seqs) {
-            const PgSeq s = a.seqs[seq];
-            const int tiles = lr_tiles(s, a, ROWS);
-            if (tile >= tiles) { seq++; tile = 0; off = 0; continue; }
-            const int all = lr_steps(s, a), take = min(left, all - off);
-            body(s, max(off - LR_BEGIN, 0), max(off + take - LR_BEGIN, 0), off > LR_BEGIN || off + take < all, first);
-            first = false;
-            left -= take;
-            if (off + take == all) { tile++; off = 0; } else off += take;
-        }
-    };
-    if (warp == LR_WARPS) {
-        // ===== copies: a lane a row =====
-        int issued = 0;
-        walk([&](const PgSeq& s, int k0, int k1, bool, bool) {
-            int from, to;
-            lr_range(s, a, &from, &to);
-            const int* table = a.table + (int64_t)seq * a.table_cols;
-            auto row_of = [&](int k) {
-                const int key = from + k * LR_KEYS + lane;
-                return key < to ? a.rows + ((int64_t)table[key >> a.shift] * a.page + (key & (a.page - 1))) * a.cols : nullptr;
-            };
-            const __half* next = k0 < k1 ? row_of(k0) : nullptr;
-            for (int k = k0; k < k1; k++) {
-                const __half* row = next;
-                if (k + 1 < k1) next = row_of(k + 1);
-                if (ok) ok = sg_wait_warp(pg_smem(&sh.empty[slot]), phase ^ 1u, &sh.fail);
-                if (ok) {
-                    const unsigned bar = pg_smem(&sh.full[slot]);
-                    if (lane == 0) pg_mbar_expect_tx(bar, (unsigned)(min(LR_KEYS, to - (from + k * LR_KEYS)) * a.cols * 2));
+    LrWalk walk = {deal.at[blockIdx.x].seq, deal.at[blockIdx.x].tile, deal.at[blockIdx.x].off, deal.run_lo + ((int)blockIdx.x < deal.run_more ? 1 : 0)};
+    if (tid >= LR_THREADS) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(LR_REGS_REST));
+        if (tid < LR_THREADS + 32) {
+            // ===== copies: a box of 64 columns for each page of a step =====
+            int n = 0;
+            bool ok = true;
+            const int rows = min(a.page, LR_KEYS), boxes = LR_KEYS / rows;      // of a page at a time; pages of a step
+            while (ok && walk.piece(a, [&](const PgSeq& s, int seq, int, int k0, int k1, bool) {
+                int from, to;
+                lr_range(s, a, &from, &to);
+                const int* table = a.table + (int64_t)seq * a.table_cols;
+                auto look_up = [&](int k) {
+                    const int key = from + k * LR_KEYS + lane * rows;
+                    return lane < boxes && key < to ? table[key >> a.shift] : 0;
+                };
+                int next = k0 < k1 ? look_up(k0) : 0;
+                for (int k = k0; k < k1 && ok; k++, n++) {
+                    const int key0 = from + k * LR_KEYS, there = (min(LR_KEYS, to - key0) + rows - 1) / rows, mine = next, slot = n % a.slots;
+                    if (k + 1 < k1) next = look_up(k + 1);
+                    if (!(ok = sg_wait_warp(pg_smem(&sh.empty[slot]), ((unsigned)(n / a.slots) & 1u) ^ 1u, &sh.fail))) break;
+                    const unsigned bar = pg_smem(&sh.full[slot]), at = ring + slot * slot_bytes;
+                    if (pg_elect()) pg_mbar_expect_tx(bar, (unsigned)there * rows * (slot_bytes / LR_KEYS));
                     __syncwarp();
-                    if (row) asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                                          ::"r"(ring + slot * slot_bytes + lane * pitch), "l"(row), "r"((unsigned)a.cols * 2), "r"(bar) : "memory");
-                    issued++;
-                }
-                advance();
-            }
-        });
-        int never = 0;                                                    // no copy is under way when the CTA ends
-        for (int i = max(0, issued - a.slots); i < issued; i++) sg_wait(pg_smem(&sh.full[i % a.slots]), (unsigned)(i / a.slots) & 1u, &never);
-    } else {
-        const int kg = warp & 3, kh = warp >> 2, blocks = a.cols >> 4, v_blocks = a.rank >> 4;
-        const int row = tid / LANES, part = tid % LANES;                  // of the weights
-        const unsigned k_lane = (unsigned)(kh * 16 + (lane >> 4) * 8 + (lane & 7)) * pitch + (lane >> 3 & 1) * 16;      // scores: this lane's row of four 8 x 8 blocks
-        const unsigned v_lane = (unsigned)((lane >> 3 & 1) * 8 + (lane & 7)) * pitch + (lane >> 4) * 16;
-        const unsigned p_lane = (unsigned)((lane >> 3 & 1) * 8 + (lane & 7)) * 80 + (lane >> 4) * 16;
-        walk([&](const PgSeq& s, int k0, int k1, bool cut, bool first) {
-            int from, to;
-            lr_range(s, a, &from, &to);
-            const int row0 = tile * ROWS, n_rows = min(ROWS, s.count * a.H - row0);
-            const float* qs = a.qf + ((int64_t)s.first * a.H + row0) * a.cols;
-            // factors of the rows: near 2^4 by a power of two
-            lr_sync();                                                    // the segment before is through
-            if (tid == 0) sh.wild = 0;
-            for (int r = warp; r < ROWS; r += LR_WARPS) {
-                unsigned top = 0;                                        // as bits, so that NaN is the largest of all
-                if (r < n_rows)
-                    for (int e = lane * 4; e < a.cols; e += 128) {
-                        const uint4 v = *(const uint4*)(qs + (int64_t)r * a.cols + e);
-                        top = max(max(top, max(v.x & 0x7fffffffu, v.y & 0x7fffffffu)), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
-                    }
-                top = __reduce_max_sync(0xffffffffu, top);
-                const int ex = top < 0x00800000u || top >= 0x7f800000u ? 4 : max((int)(top >> 23) - 126, -100);
-                if (lane == 0) {
-                    sh.inv[r] = __uint_as_float((unsigned)(4 - ex + 127) << 23);
-                    sh.top[r] = top >= 0x7f800000u ? NAN : __uint_as_float((unsigned)(ex - 4 + 127) << 23);
-                }
-            }
-            lr_sync();
-            unsigned q[MT][LR_KB][4];
-#pragma unroll
-            for (int t = 0; t < MT; t++)
-#pragma unroll
-                for (int i = 0; i < LR_KB; i++) {
-                    const int b = kg + 4 * i;
-#pragma unroll
-                    for (int x = 0; x < 4; x++) {
-                        const int r = t * 16 + (lane >> 2) + (x & 1) * 8;
-                        float2 v = make_float2(0.0f, 0.0f);
-                        if (b < blocks && r < n_rows) v = *(const float2*)(qs + (int64_t)r * a.cols + b * 16 + (x >> 1) * 8 + (lane & 3) * 2);
-                        q[t][i][x] = lt_pack(v.x * sh.inv[r], v.y * sh.inv[r]);
+                    for (int i = 0; i < there; i++) {
+                        const int page = __shfl_sync(0xffffffffu, mine, i), y = (key0 + i * rows) & (a.page - 1);
+                        if (pg_elect())
+                            for (int b = 0; b * 64 < a.cols; b++)
+                                asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                                             ::"r"(at + b * LR_BLOCK + i * rows * 128), "l"(&map_rows), "r"(bar), "r"(b * 64), "r"(y), "r"(page) : "memory");
+                        __syncwarp();
                     }
                 }
-            const float f = sh.top[row] * (a.scale * LR_LOG2E);
-            const int pos = row < n_rows ? s.pos0 + (row0 + row) / a.H : -1, key_lo = a.window > 0 ? pos - a.window + 1 : 0;
-            float m = -INFINITY, l = 0.0f;
-            float o[MT][LR_VB][2][4];
+            })) {}
+            int never = 0;                                            // no copy is under way when the CTA ends
+            for (int i = max(0, n - a.slots); i < n; i++) sg_wait_warp(pg_smem(&sh.full[i % a.slots]), (unsigned)(i / a.slots) & 1u, &never);
+            if (!ok) for (int i = 0; i < 1000; i++) __nanosleep(1000);
+        }
+        return;
+    }
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(LR_REGS));
+    const int kg = warp & 3, kh = warp >> 2, blocks = a.cols >> 4, v_blocks = a.rank >> 4;
+    const int row = in_group >> 4, part = in_group & 15;              // of the weights: 16 threads a row, two keys each
+    // a slot: blocks of 64 columns, 32 rows of 128 bytes under the 128-byte swizzle.  This lane's row of four 8 x 8 blocks: scores take columns 16 (kg + 4 i), block i; values 16 (warp + 8 i), block warp / 4 + 2 i
+    const unsigned k_lane = (unsigned)(kh * 16 + (lane >> 4) * 8 + (lane & 7)) * 128 + (((kg * 2 + (lane >> 3 & 1)) ^ (lane & 7)) << 4);
+    const unsigned v_lane = (unsigned)(warp >> 2) * LR_BLOCK + (unsigned)((lane >> 3 & 1) * 8 + (lane & 7)) * 128 + ((((warp & 3) * 2 + (lane >> 4)) ^ (lane & 7)) << 4);
+    const unsigned p_at = pg_smem(&sh.p[group][0][0]) + (unsigned)((lane >> 3 & 1) * 8 + (lane & 7)) * 80 + (lane >> 4) * 16;
+    int n = 0;                                                        // steps of the run so far
+    bool ok = true, first = true;
+    while (walk.piece(a, [&](const PgSeq& s, int seq, int tile, int k0, int k1, bool cut) {
+        int from, to;
+        lr_range(s, a, &from, &to);
+        const int row0 = tile * LR_ROWS, n_rows = min(LR_ROWS, s.count * a.H - row0);
+        const float* qs = a.qf + ((int64_t)s.first * a.H + row0) * a.cols;
+        // factors of the rows: near 2^4 by a power of two.  A warp a row
+        if (tid == 0) sh.wild = 0;
+        {
+            const int r = tid >> 5;
+            unsigned top = 0;                                        // as bits, so that NaN is the largest of all
+            if (r < n_rows)
+                for (int e = lane * 4; e < a.cols; e += 128) {
+                    const uint4 v = *(const uint4*)(qs + (int64_t)r * a.cols + e);
+                    top = max(max(top, max(v.x & 0x7fffffffu, v.y & 0x7fffffffu)), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
+                }
+            top = __reduce_max_sync(0xffffffffu, top);
+            const int ex = top < 0x00800000u || top >= 0x7f800000u ? 4 : max((int)(top >> 23) - 126, -100);
+            if (lane == 0) {
+                sh.up[r] = __uint_as_float((unsigned)(4 - ex + 127) << 23);
+                sh.factor[r] = top >= 0x7f800000u ? NAN : __uint_as_float((unsigned)(ex - 4 + 127) << 23);
+            }
+        }
+        lr_sync_all();
+        unsigned q[LR_KB][4];
 #pragma unroll
-            for (int t = 0; t < MT; t++)
+        for (int i = 0; i < LR_KB; i++) {
+            const int b = kg + 4 * i;
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int r = (lane >> 2) + (x & 1) * 8;
+                float2 v = make_float2(0.0f, 0.0f);
+                if (b < blocks && r < n_rows) v = *(const float2*)(qs + (int64_t)r * a.cols + b * 16 + (x >> 1) * 8 + (lane & 3) * 2);
+                q[i][x] = lt_pack(v.x * sh.up[r], v.y * sh.up[r]);
+            }
+        }
+        const float f = sh.factor[row] * (a.scale * LR_LOG2E);
+        const int pos = row < n_rows ? s.pos0 + (row0 + row) / a.H : -1, key_lo = a.window > 0 ? pos - a.window + 1 : 0;
+        float m = -INFINITY, l = 0.0f;
+        float o[LR_VB][2][4];
+#pragma unroll
+        for (int i = 0; i < LR_VB; i++)
+#pragma unroll
+            for (int x = 0; x < 8; x++) o[i][x >> 2][x & 3] = 0.0f;
+        const int skip = (n + group) & 1;                             // the run's even steps are group 0's
+#pragma unroll 1
+        for (int k = k0 + skip; k < k1; k += LR_GROUPS) {
+            const int here = n + k - k0, slot = here % a.slots;
+            ok = ok && sg_wait_warp(pg_smem(&sh.full[slot]), (unsigned)(here / a.slots) & 1u, &sh.fail);
+            const unsigned at = ring + slot * slot_bytes;
+            float x[2][4];
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i >> 2][i & 3] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < LR_KB; i++) {
+                const int b = kg + 4 * i;
+                if (b < blocks) {
+                    unsigned kb[4];
+                    lt_ldsm(kb, at + k_lane + i * LR_BLOCK);
+                    lt_mma(x[0], q[i], kb[0], kb[1]);
+                    lt_mma(x[1], q[i], kb[2], kb[3]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int y = 0; y < 2; y++) *(float2*)&sh.sums[group][kg][(lane >> 2) + y * 8][kh * 16 + i * 8 + (lane & 3) * 2] = make_float2(x[i][2 * y], x[i][2 * y + 1]);
+            if (const int there = to - (from + k * LR_KEYS); there < LR_KEYS) {      // what lies behind a sequence's end has the weight 0, which would make a NaN of a NaN
+                const unsigned n16 = (unsigned)(LR_KEYS - there) * 8 * ((a.cols + 63) >> 6);
+                for (unsigned e = in_group; e < n16; e += LR_THREADS / LR_GROUPS)
+                    lr_zero(at + e / ((LR_KEYS - there) * 8) * LR_BLOCK + there * 128 + e % ((LR_KEYS - there) * 8) * 16);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // before the slot's next rows
+            }
+            lr_sync(group);
+            float z[2];
+            {
+                const float2 u0 = *(const float2*)&sh.sums[group][0][row][part * 2], u1 = *(const float2*)&sh.sums[group][1][row][part * 2], u2 = *(const float2*)&sh.sums[group][2][row][part * 2],
+                             u3 = *(const float2*)&sh.sums[group][3][row][part * 2];
+                const int key = from + k * LR_KEYS + part * 2;        // (a row sees no key behind `to`)
+                z[0] = key <= pos && key >= key_lo ? ((u0.x + u1.x) + (u2.x + u3.x)) * f : -INFINITY;
+                z[1] = key + 1 <= pos && key + 1 >= key_lo ? ((u0.y + u1.y) + (u2.y + u3.y)) * f : -INFINITY;
+            }
+            float mx = fmaxf(z[0], z[1]);
+#pragma unroll
+            for (int d = 1; d < 16; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+            const float m_new = fmaxf(m, mx), base = m_new == -INFINITY ? 0.0f : m_new, alpha = m == m_new ? 1.0f : lt_exp2(m - m_new);
+            m = m_new;
+            z[0] = lt_exp2(z[0] - base + LR_SHIFT); z[1] = lt_exp2(z[1] - base + LR_SHIFT);
+            l = fmaf(l, alpha, z[0] + z[1]);
+            *(unsigned*)&sh.p[group][row][part * 2] = lt_pack(z[0], z[1]);
+            if (part == 0) sh.alpha[group][row] = alpha;
+            if (lr_sync_or(group, alpha != 1.0f)) {
+                const float a0 = sh.alpha[group][lane >> 2], a1 = sh.alpha[group][(lane >> 2) + 8];
 #pragma unroll
                 for (int i = 0; i < LR_VB; i++)
 #pragma unroll
-                    for (int x = 0; x < 8; x++) o[t][i][x >> 2][x & 3] = 0.0f;
-            bool grew = false;
-            unsigned v_slot = slot;
-#pragma unroll 1
-            for (int k = k0; k <= k1; k++) {
-                const int z = k & 1;
-                const unsigned here = slot;
-                if (k < k1) {
-                    ok = ok && sg_wait_warp(pg_smem(&sh.full[slot]), phase, &sh.fail);
-                    float x[MT][2][4];
-#pragma unroll
-                    for (int t = 0; t < MT; t++)
-#pragma unroll
-                        for (int i = 0; i < 8; i++) x[t][i >> 2][i & 3] = 0.0f;
-                    const unsigned at = ring + slot * slot_bytes + k_lane;
-#pragma unroll
-                    for (int i = 0; i < LR_KB; i++) {
-                        const int b = kg + 4 * i;
-                        if (b < blocks) {
-                            unsigned kb[4];
-                            lt_ldsm(kb, at + b * 32);
-#pragma unroll
-                            for (int t = 0; t < MT; t++) { lt_mma(x[t][0], q[t][i], kb[0], kb[1]); lt_mma(x[t][1], q[t][i], kb[2], kb[3]); }
-                        }
-                    }
-#pragma unroll
-                    for (int t = 0; t < MT; t++)
-#pragma unroll
-                        for (int n = 0; n < 2; n++)
-#pragma unroll
-                            for (int y = 0; y < 2; y++)
-                                *(float2*)&sh.sums[z][kg][t * 16 + (lane >> 2) + y * 8][kh * 16 + n * 8 + (lane & 3) * 2] = make_float2(x[t][n][2 * y], x[t][n][2 * y + 1]);
-                    advance();
-                }
-                const bool scale = lr_sync_or(grew);
-                if (k < k1) {
-                    float x[PER], mx = -INFINITY, sum = 0.0f;
-                    const int key0 = from + k * LR_KEYS + part * PER;
-#pragma unroll
-                    for (int i = 0; i < PER; i++) {
-                        const float d = (sh.sums[z][0][row][part * PER + i] + sh.sums[z][1][row][part * PER + i]) + (sh.sums[z][2][row][part * PER + i] + sh.sums[z][3][row][part * PER + i]);
-                        x[i] = key0 + i <= pos && key0 + i >= key_lo ? d * f : -INFINITY;      // (a row sees no key behind `to`)
-                        mx = fmaxf(mx, x[i]);
-                    }
-#pragma unroll
-                    for (int d = 1; d < LANES; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-                    const float m_new = fmaxf(m, mx), base = m_new == -INFINITY ? 0.0f : m_new, alpha = m == m_new ? 1.0f : lt_exp2(m - m_new);
-                    grew = alpha != 1.0f;
-                    m = m_new;
-#pragma unroll
-                    for (int i = 0; i < PER; i++) { x[i] = lt_exp2(x[i] - base + LR_SHIFT); sum += x[i]; }
-                    l = fmaf(l, alpha, sum);
-#pragma unroll
-                    for (int i = 0; i < PER; i += 2) *(unsigned*)&sh.p[z][row][part * PER + i] = lt_pack(x[i], x[i + 1]);
-                    if (part == 0) sh.alpha[z][row] = alpha;
-                }
-                if (k > k0) {                                             // the values of the step before
-                    const unsigned at = ring + v_slot * slot_bytes + v_lane, ps = pg_smem(&sh.p[z ^ 1][0][0]) + p_lane;
-                    if (scale) {
-#pragma unroll
-                        for (int t = 0; t < MT; t++) {
-                            const float a0 = sh.alpha[z ^ 1][t * 16 + (lane >> 2)], a1 = sh.alpha[z ^ 1][t * 16 + (lane >> 2) + 8];
-#pragma unroll
-                            for (int i = 0; i < LR_VB; i++)
-#pragma unroll
-                                for (int n = 0; n < 2; n++) { o[t][i][n][0] *= a0; o[t][i][n][1] *= a0; o[t][i][n][2] *= a1; o[t][i][n][3] *= a1; }
-                        }
-                    }
-#pragma unroll
-                    for (int kk = 0; kk < LR_KEYS / 16; kk++) {
-                        unsigned p[MT][4];
-#pragma unroll
-                        for (int t = 0; t < MT; t++) lt_ldsm(p[t], ps + t * 16 * 80 + kk * 32);
-#pragma unroll
-                        for (int i = 0; i < LR_VB; i++) {
-                            const int b = warp + LR_WARPS * i;
-                            if (b < v_blocks) {
-                                unsigned v[4];
-                                lt_ldsm_t(v, at + kk * 16 * pitch + b * 32);
-#pragma unroll
-                                for (int t = 0; t < MT; t++) { lt_mma(o[t][i][0], p[t], v[0], v[1]); lt_mma(o[t][i][1], p[t], v[2], v[3]); }
-                            }
-                        }
-                    }
-                    sg_arrive(pg_smem(&sh.empty[v_slot]));
-                }
-                v_slot = here;
+                    for (int y = 0; y < 2; y++) { o[i][y][0] *= a0; o[i][y][1] *= a0; o[i][y][2] *= a1; o[i][y][3] *= a1; }
             }
-            // a cut segment leaves its sums, the others their result
 #pragma unroll
-            for (int d = 1; d < LANES; d *= 2) l += __shfl_xor_sync(0xffffffffu, l, d);
-            const int place = 2 * c + (first ? 0 : 1);
-            const bool any = k1 > k0 || !cut;
-            if (part == 0) {
-                float by = 1.0f;
-                if (!cut) {
-                    float total = l, g = 1.0f;
-                    if (a.sink && row < n_rows) {
-                        const float sk = a.sink[(row0 + row) % a.H] * LR_LOG2E, m2 = fmaxf(m, sk);
-                        g = m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : exp2f(m - m2);
-                        total = g * l + (sk == -INFINITY ? 0.0f : exp2f(sk - m2 + LR_SHIFT));
+            for (int kk = 0; kk < LR_KEYS / 16; kk++) {
+                unsigned p[4];
+                lt_ldsm(p, p_at + kk * 32);
+#pragma unroll
+                for (int i = 0; i < LR_VB; i++) {
+                    const int b = warp + 8 * i;
+                    if (b < v_blocks) {
+                        unsigned v[4];
+                        lt_ldsm_t(v, at + v_lane + kk * 2048 + i * 2 * LR_BLOCK);
+                        lt_mma(o[i][0], p, v[0], v[1]);
+                        lt_mma(o[i][1], p, v[2], v[3]);
                     }
-                    by = g / total;
                 }
-                if (cut && any) a.ml[(size_t)place * ROWS + row] = make_float2(m, l);
-                sh.inv[row] = by;
-                sh.top[row] = m;
-                sh.sum[row] = l;
             }
-            lr_sync();
-            float* lat = cut ? a.part + (size_t)place * ROWS * a.rank : a.lat + ((int64_t)s.first * a.H + row0) * a.rank;
-            unsigned wild = 0;
+            sg_arrive(pg_smem(&sh.empty[slot]));
+        }
+        n += k1 - k0;
+        // both groups' sums: group 1 gives the first half of its columns' blocks, group 0 the second.  A cut segment leaves its sums, the others their result
 #pragma unroll
-            for (int t = 0; t < MT; t++)
+        for (int d = 1; d < 16; d *= 2) l += __shfl_xor_sync(0xffffffffu, l, d);
+        if (part == 0) { sh.top[group][row] = m; sh.sum[group][row] = l; }
+        float4* box = (float4*)&sh.sums[0][0][0][0] + in_group;
+        auto give = [&](int half) {
+#pragma unroll
+            for (int i = 0; i < 2; i++)
 #pragma unroll
                 for (int y = 0; y < 2; y++) {
-                    const int r = t * 16 + (lane >> 2) + y * 8;
-                    const float by = sh.inv[r];
+                    const float* v = o[half * 2 + i][y];
+                    box[(i * 2 + y) * (LR_THREADS / LR_GROUPS)] = make_float4(v[0], v[1], v[2], v[3]);
+                }
+        };
+        lr_sync_all();                                                // scores and weights are read
+        if (group == 1) give(0);
+        const int place = 2 * blockIdx.x + (first ? 0 : 1);
+        const bool any = k1 > k0 || !cut;
+        float* lat = cut ? a.part + (size_t)place * LR_ROWS * a.rank : a.lat + ((int64_t)s.first * a.H + row0) * a.rank;
+        float mine[2], other[2], by[2], both[2];                      // of the rows lane / 4 and that + 8: factors of the groups' sums, then of the result; the largest score
+        unsigned wild = 0;
 #pragma unroll
-                    for (int i = 0; i < LR_VB; i++) {
-                        const int b = warp + LR_WARPS * i;
-                        if (b < v_blocks && r < n_rows && any)
+        for (int y = 0; y < 2; y++) {
+            const int r = (lane >> 2) + y * 8;
+            const float m0 = sh.top[0][r], m1 = sh.top[1][r], l0 = sh.sum[0][r], l1 = sh.sum[1][r], mm = fmaxf(m0, m1);
+            const float f0 = m0 == -INFINITY ? (l0 == 0.0f ? 0.0f : 1.0f) : lt_exp2(m0 - mm), f1 = m1 == -INFINITY ? (l1 == 0.0f ? 0.0f : 1.0f) : lt_exp2(m1 - mm);
+            float total = f0 * l0 + f1 * l1, g = 1.0f;
+            if (cut) {
+                by[y] = 1.0f;
+                if (any && group == 0 && warp == 0 && (lane & 3) == 0) a.ml[(size_t)place * LR_ROWS + r] = make_float2(mm, total);
+            } else {
+                float all = total;
+                if (a.sink && r < n_rows) {
+                    const float sk = a.sink[(row0 + r) % a.H] * LR_LOG2E, m2 = fmaxf(mm, sk);
+                    g = mm == -INFINITY ? (total == 0.0f ? 0.0f : 1.0f) : exp2f(mm - m2);
+                    all = g * total + (sk == -INFINITY ? 0.0f : exp2f(sk - m2 + LR_SHIFT));
+                }
+                by[y] = g / all;
+            }
+            mine[y] = group ? f1 : f0; other[y] = group ? f0 : f1;
+            both[y] = fabsf(total) < INFINITY ? mm : NAN;
+        }
+        auto finish = [&](int half) {
 #pragma unroll
-                            for (int n = 0; n < 2; n++) {
-                                const float u = o[t][i][n][2 * y], v = o[t][i][n][2 * y + 1];
-                                if (!(fabsf(u) < INFINITY && fabsf(v) < INFINITY) && fabsf(sh.sum[r]) < INFINITY) wild |= 1u << r;
-                                *(float2*)(lat + (int64_t)r * a.rank + b * 16 + n * 8 + (lane & 3) * 2) = make_float2(u * by, v * by);
-                            }
+            for (int i = 0; i < 2; i++) {
+                const int b = warp + 8 * (half * 2 + i);
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const float4 u = box[(i * 2 + c) * (LR_THREADS / LR_GROUPS)];
+                    const float theirs[4] = {u.x, u.y, u.z, u.w};
+                    if (b < v_blocks && any) {
+#pragma unroll
+                        for (int y = 0; y < 2; y++) {
+                            const int r = (lane >> 2) + y * 8;
+                            if (r >= n_rows) continue;
+                            // (a group without keys has sums of 0 and the factor 0)
+                            const float v0 = fmaf(o[half * 2 + i][c][2 * y], mine[y], theirs[2 * y] * other[y]), v1 = fmaf(o[half * 2 + i][c][2 * y + 1], mine[y], theirs[2 * y + 1] * other[y]);
+                            if (!(fabsf(v0) < INFINITY && fabsf(v1) < INFINITY) && both[y] == both[y]) wild |= 1u << r;
+                            *(float2*)(lat + (int64_t)r * a.rank + b * 16 + c * 8 + (lane & 3) * 2) = make_float2(v0 * by[y], v1 * by[y]);
+                        }
                     }
                 }
-            if (wild) atomicOr(&sh.wild, wild);
-            if (lr_sync_or(wild != 0)) lr_again<MT>(a, sh, s, seq, row0, from + k0 * LR_KEYS, min(to, from + k1 * LR_KEYS), lat, a.rank);
-        });
-    }
-    __syncthreads();
-    if (tid == 0 && sh.fail) {
+            }
+        };
+        lr_sync_all();
+        if (group == 0) finish(0);
+        lr_sync_all();
+        if (group == 0) give(1);
+        lr_sync_all();
+        if (group == 1) finish(1);
+        if (wild) atomicOr(&sh.wild, wild);
+        if (lr_sync_all_or(wild != 0)) {
+            for (unsigned left = sh.wild; left; left &= left - 1) {
+                const int r = __ffs(left) - 1;
+                const float m0 = sh.top[0][r], m1 = sh.top[1][r];
+                const float mm = fmaxf(m0, m1), l0 = sh.sum[0][r], l1 = sh.sum[1][r];
+                const float f0 = m0 == -INFINITY ? 0.0f : lt_exp2(m0 - mm), f1 = m1 == -INFINITY ? 0.0f : lt_exp2(m1 - mm);
+                float total = f0 * l0 + f1 * l1, g = 1.0f;
+                if (!cut && a.sink) {
+                    const float sk = a.sink[(row0 + r) % a.H] * LR_LOG2E, m2 = fmaxf(mm, sk);
+                    g = exp2f(mm - m2);
+                    total = g * total + (sk == -INFINITY ? 0.0f : exp2f(sk - m2 + LR_SHIFT));
+                }
+                lr_again(a, sh, s, seq, row0, from + k0 * LR_KEYS, min(to, from + k1 * LR_KEYS), mm, cut ? 1.0f : g / total, r, lat + (int64_t)r * a.rank);
+            }
+            lr_sync_all();
+        }
+        first = false;
+    })) {}
+    if (tid == 0 && *(volatile int*)&sh.fail) {
         if (err_dev) atomicExch(err_dev, 5u);
         if (err_host) { *(volatile unsigned*)err_host = 5u; __threadfence_system(); }
     }
 }
 // segments in several runs: grid (segments, rows, 128 columns); a warp takes every eighth slice.  (One thread a column, one slice after another: 43 us for the 148 slices of a long cache)
 #define LJ_WARPS 8
-template <int MT>
 __global__ void __launch_bounds__(LJ_WARPS * 32) latent_join_kernel(const LrArgs a, const __grid_constant__ LrCuts cuts) {
     __shared__ float factor[LR_CTAS], red[2][LJ_WARPS];
     __shared__ float4 sums[LJ_WARPS][32];
     pdl_enter();
-    constexpr int ROWS = 16 * MT;
     const auto cut = cuts.at[blockIdx.x];
     const PgSeq s = a.seqs[cut.seq];
-    const int y = blockIdx.y, row = cut.tile * ROWS + y, lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.z * 128 + lane * 4;
+    const int y = blockIdx.y, row = cut.tile * LR_ROWS + y, lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.z * 128 + lane * 4;
     if (row >= s.count * a.H) return;
-    auto place = [&](int x) { return (size_t)(x == 0 ? cut.slot : 2 * (cut.cta + x - 1)) * ROWS + y; };
+    auto place = [&](int x) { return (size_t)(x == 0 ? cut.slot : 2 * (cut.cta + x - 1)) * LR_ROWS + y; };
     static_assert(LR_CTAS <= LJ_WARPS * 32, "a thread a slice");
     const int x = threadIdx.x;
     const float2 z = x < cut.n ? a.ml[place(x)] : make_float2(-INFINITY, 0.0f);
@@ -551,12 +593,12 @@ __global__ void __launch_bounds__(LJ_WARPS * 32) latent_join_kernel(const LrArgs
 }
 
 // the runs of deal.ctas CTAs over all steps, and the segments that are in several of them (returned: how many)
-static int lr_deal(const cc_page_plan* plan, const LrArgs& a, int rows, int64_t steps, LrDeal& deal, LrCuts& cuts) {
+static int lr_deal(const cc_page_plan* plan, const LrArgs& a, int64_t steps, LrDeal& deal, LrCuts& cuts) {
     deal.run_lo = (int)(steps / deal.ctas); deal.run_more = (int)(steps % deal.ctas);
     int64_t before = 0, next = 0;                                  // steps in front of the sequence, and of run c
     int c = 0, n_cuts = 0;
     for (int seq = 0; seq < (int)plan->seqs.size() && c < deal.ctas; seq++) {
-        const int n = lr_tiles(plan->seqs[seq], a, rows), all = n ? lr_steps(plan->seqs[seq], a) : 0;
+        const int n = lr_tiles(plan->seqs[seq], a), all = n ? lr_steps(plan->seqs[seq], a) : 0;
         for (; c < deal.ctas && next < before + (int64_t)n * all; next += deal.run_lo + (c < deal.run_more ? 1 : 0), c++) {
             const int tile = (int)((next - before) / all), off = (int)((next - before) - (int64_t)tile * all);
             deal.at[c] = {seq, tile, off};
@@ -570,12 +612,10 @@ static int lr_deal(const cc_page_plan* plan, const LrArgs& a, int rows, int64_t 
     }
     return n_cuts;
 }
-template <int MT>
 static int lr_run(cc_device* dev, const cc_page_plan* plan, LrArgs a, const LtRuns& runs) {
-    constexpr int ROWS = 16 * MT;
     int64_t steps = 0, tiles = 0;
     for (const PgSeq& s : plan->seqs) {
-        const int n = lr_tiles(s, a, ROWS);
+        const int n = lr_tiles(s, a);
         tiles += n;
         steps += (int64_t)n * (n ? lr_steps(s, a) : 0);
     }
@@ -584,22 +624,25 @@ static int lr_run(cc_device* dev, const cc_page_plan* plan, LrArgs a, const LtRu
     LrCuts cuts;
     CC_REQUIRE(dev, steps < ((int64_t)1 << 31) * 64, "paged_latent_attention: too many rows");
     deal.ctas = (int)std::min<int64_t>(std::min(LR_CTAS, dev->sm_count), (steps + LR_BEGIN + 1) / (LR_BEGIN + 2));
-    const int n_cuts = lr_deal(plan, a, ROWS, steps, deal, cuts);
-    const size_t qf = (size_t)plan->tokens * a.H * a.cols * 4, lat = (size_t)plan->tokens * a.H * a.rank * 4, part = n_cuts ? (size_t)2 * deal.ctas * ROWS * a.rank * 4 : 0;
+    const int n_cuts = lr_deal(plan, a, steps, deal, cuts);
+    const size_t qf = (size_t)plan->tokens * a.H * a.cols * 4, lat = (size_t)plan->tokens * a.H * a.rank * 4, part = n_cuts ? (size_t)2 * deal.ctas * LR_ROWS * a.rank * 4 : 0;
     void* ws = nullptr; size_t cls = 0;
-    const int rc = cc_pool_alloc(dev, qf + lat + part + (size_t)2 * deal.ctas * ROWS * sizeof(float2), &ws, &cls);
+    int rc = cc_pool_alloc(dev, qf + lat + part + (size_t)2 * deal.ctas * LR_ROWS * sizeof(float2), &ws, &cls);
     if (rc) return rc;
     a.qf = (float*)ws; a.lat = (float*)((uint8_t*)ws + qf); a.part = (float*)((uint8_t*)ws + qf + lat); a.ml = (float2*)((uint8_t*)ws + qf + lat + part);
-    const int slot = LR_KEYS * (a.cols * 2 + 16);
-    a.slots = std::min(LR_SLOTS, (LR_SMEM - (int)sizeof(LrShared<MT>)) / slot);
+    const int slot = (a.cols + 63) / 64 * LR_BLOCK;
+    a.slots = std::min(LR_SLOTS, (LR_SMEM - (int)sizeof(LrShared) - 1024) / slot);
+    CUtensorMap map;
+    rc = cc_make_tmap_pages(dev, &map, a.rows, plan->n_pages, plan->page, a.cols, std::min(plan->page, LR_KEYS));
+    if (rc) { cc_pool_free(dev, ws, cls); return rc; }
     const unsigned z = (unsigned)std::min(runs.tiles, 64);
     const size_t fold = (size_t)a.dim * (LF_COLS + 8) * 2 + 16 * (a.dim + 8) * 2, unfold = (size_t)(LU_COLS + 32) * (a.rank + 8) * 2;
     cudaError_t e = cudaFuncSetAttribute(latent_fold_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LT_DIM * (LF_COLS + 8) * 2 + 16 * (LT_DIM + 8) * 2);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(latent_rows_kernel<MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, LR_SMEM - (int)sizeof(LrShared<MT>));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(latent_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LR_SMEM - (int)sizeof(LrShared));
     if (e == cudaSuccess) e = cudaFuncSetAttribute(latent_unfold_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (LU_COLS + 32) * (LT_RANK + 8) * 2);
     if (e == cudaSuccess) e = cc_launch_pdl(dev, latent_fold_kernel, dim3((unsigned)a.H, (unsigned)((a.rank + LF_COLS - 1) / LF_COLS + (a.rest ? 1 : 0)), z), 128, fold, a, runs);
-    if (e == cudaSuccess) e = cc_launch_pdl(dev, latent_rows_kernel<MT>, (unsigned)deal.ctas, LR_THREADS, (size_t)a.slots * slot, a, deal, dev->err_dev, dev->err_host);
-    if (e == cudaSuccess && n_cuts) { e = cc_launch_pdl(dev, latent_join_kernel<MT>, dim3((unsigned)n_cuts, ROWS, (unsigned)(a.rank + 127) / 128), LJ_WARPS * 32, 0, a, cuts); dev->launches++; }
+    if (e == cudaSuccess) e = cc_launch_pdl(dev, latent_rows_kernel, (unsigned)deal.ctas, LR_ALL, (size_t)a.slots * slot + 1024, map, a, deal, dev->err_dev, dev->err_host);
+    if (e == cudaSuccess && n_cuts) { e = cc_launch_pdl(dev, latent_join_kernel, dim3((unsigned)n_cuts, LR_ROWS, (unsigned)(a.rank + 127) / 128), LJ_WARPS * 32, 0, a, cuts); dev->launches++; }
     if (e == cudaSuccess) e = cc_launch_pdl(dev, latent_unfold_kernel, dim3((unsigned)a.H, (unsigned)((a.vdim + LU_COLS - 1) / LU_COLS), z), 128, unfold, a, runs);
     dev->launches += 3;
     cc_pool_free(dev, ws, cls);
@@ -636,8 +679,7 @@ extern "C" CC_API int cc_paged_latent_attention(cc_device* dev, const cc_page_pl
     for (const cc_view* v : {q, uk, uv}) CC_REQUIRE(dev, ((uintptr_t)v->buf->plane[0] & 15) == 0, "paged_latent_attention: a tensor does not start at a multiple of 16 bytes");
     CC_REQUIRE(dev, form == CC_LATENT_AUTO || form == CC_LATENT_ABSORBED || form == CC_LATENT_EXPANDED, "paged_latent_attention: form %d", form);
     CC_REQUIRE(dev, out_type == CC_F16 || out_type == CC_BF16, "paged_latent_attention: results of type %d (F16 or BF16)", out_type);
-    // tensor maps count rows in 32 bits
-    const bool expands = dim <= TL_DIM && vdim <= TL_DIM && plan->n_pages * plan->page < ((int64_t)1 << 31) && (int64_t)H * LT_DIM < ((int64_t)1 << 31);
+    const bool expands = dim <= TL_DIM && vdim <= TL_DIM;
     CC_REQUIRE(dev, form != CC_LATENT_EXPANDED || expands, "paged_latent_attention: heads of %lld and %lld are not expanded (up to %d)", (long long)dim, (long long)vdim, TL_DIM);
     cc_buf* o = nullptr;
     rc = cc_new_activation(dev, T * H * vdim, out_type, false, &o);
@@ -651,16 +693,14 @@ extern "C" CC_API int cc_paged_latent_attention(cc_device* dev, const cc_page_pl
         a.rank = c.rank; a.rest = c.rest; a.cols = c.cols; a.window = window > 0 ? window : 0; a.out_bf16 = out_type == CC_BF16;
         a.most = form == CC_LATENT_EXPANDED ? 0 : form == CC_LATENT_ABSORBED || !expands ? 0x7fffffff : LT_FEW;
         LtRuns runs{};
-        bool wide = false;
         for (const PgSeq& s : plan->seqs) {
             if (s.count == 0 || s.count > a.most) continue;
-            wide = wide || (int64_t)s.count * H > 16;
             if (runs.n && runs.hi[runs.n - 1] == s.first) { runs.hi[runs.n - 1] = s.first + s.count; continue; }
             if (runs.n == LT_RUNS) { runs.hi[runs.n - 1] = s.first + s.count; continue; }      // many runs: the last one takes all that lies behind (other tokens' results are overwritten)
             runs.lo[runs.n] = s.first; runs.hi[runs.n++] = s.first + s.count;
         }
         for (int i = 0; i < runs.n; i++) { runs.tile0[i] = runs.tiles; runs.tiles += (runs.hi[i] - runs.lo[i] + 15) / 16; }
-        rc = wide ? lr_run<2>(dev, plan, a, runs) : lr_run<1>(dev, plan, a, runs);
+        rc = lr_run(dev, plan, a, runs);
         if (!rc && a.most < 0x7fffffff) rc = tl_run(dev, plan, a);      // behind the others: their last products may run over tokens of these
     }
     if (rc) { cc_tensor_release(o); return rc; }

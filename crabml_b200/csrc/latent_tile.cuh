@@ -91,10 +91,11 @@ __device__ __forceinline__ void tl_report(int fail, unsigned* err_dev, unsigned*
         if (err_host) { *(volatile unsigned*)err_host = 5u; __threadfence_system(); }
     }
 }
-// the pages that hold keys key0 .. key0 + 127 of a sequence: a box of 64 columns from x on for each, those behind its last token left out.  Returns the bytes
-__device__ __forceinline__ unsigned tl_pages(const LrArgs& a, int seq, int key0, int to) { return (unsigned)((min(TL_KEYS, to - key0) + a.page - 1) / a.page * a.page * 128); }
-__device__ __forceinline__ void tl_load_pages(const LrArgs& a, const CUtensorMap* map, unsigned dst, unsigned bar, int x, int seq, int key0, int to) {
-    for (int i = 0; i < TL_KEYS && key0 + i < to; i += a.page) pg_tma_load_2d(dst + i * 128, map, bar, x, a.table[(int64_t)seq * a.table_cols + ((key0 + i) >> a.shift)] * a.page);
+// The pages that hold keys key0 .. key0 + 127 of a sequence, those behind its last token left out: lane i has the i-th one's number (a look-up by each copy's thread took 700 cycles of it), a
+// copy brings 64 columns of one
+__device__ __forceinline__ int tl_look_up(const LrArgs& a, int seq, int key0, int to) {
+    const int key = key0 + (int)(threadIdx.x & 31) * a.page;
+    return (int)(threadIdx.x & 31) < TL_KEYS / a.page && key < to ? a.table[(int64_t)seq * a.table_cols + (key >> a.shift)] : 0;
 }
 
 // ---- keys and values of 128 rows ------------------------------------------------------------------------------------------------------------------------
@@ -104,7 +105,7 @@ __device__ __forceinline__ void tl_load_pages(const LrArgs& a, const CUtensorMap
 #define TE_ABLOCKS (LT_RANK / 64)
 #define TE_STAGES 4
 #define TE_STAGE (TL_DIM * 128)               // 64 columns of U_h or V_h
-#define TE_SMEM (TE_ABLOCKS * TL_BLOCK + TE_STAGES * TE_STAGE + 1024)
+#define TE_SMEM (TE_ABLOCKS * TL_BLOCK + TE_STAGES * TE_STAGE + 2 * TL_BLOCK + 1024)      // the rows, weights, two blocks of results
 struct TeShared {
     unsigned long long a_full[TE_ABLOCKS], full[TE_STAGES], empty[TE_STAGES], acc_full[2], acc_empty[2], drained;
     unsigned tmem_base;
@@ -119,6 +120,9 @@ __device__ __forceinline__ void te_expect(unsigned bar, unsigned bytes) { asm vo
 __device__ __forceinline__ void te_tma(unsigned dst, const void* tmap, unsigned bar, int x, int y) {
     asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(tmap), "r"(bar), "r"(x), "r"(y) : "memory");
 }
+__device__ __forceinline__ void te_tma_page(unsigned dst, const void* tmap, unsigned bar, int x, int page) {
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(tmap), "r"(bar), "r"(x), "r"(0), "r"(page) : "memory");
+}
 __device__ __forceinline__ void te_umma(unsigned tmem_d, uint64_t a, uint64_t b, unsigned idesc, unsigned accumulate) {
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
@@ -126,6 +130,7 @@ __device__ __forceinline__ void te_umma(unsigned tmem_d, uint64_t a, uint64_t b,
 __device__ __forceinline__ void te_commit(unsigned bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
+__device__ __forceinline__ void te_sync(int which) { asm volatile("bar.sync %0, 128;" ::"r"(1 + which) : "memory"); }      // the four warps of a block
 // grid (key tiles, up to a whole pair, runs of heads)
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TE_THREADS, 1) latent_expand_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_uk,
                                                                                                const __grid_constant__ CUtensorMap map_uv, const __grid_constant__ TlArgs t, unsigned* err_dev, unsigned* err_host) {
@@ -160,13 +165,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TE_THREADS, 1) laten
     const int key0 = from + kt * TL_KEYS;
     if (found < 0) to = key0;                                         // the second CTA of the last pair may have no keys
     if (warp == 0) {
-        if (lane == 0) {
-            for (int b = 0; b < blocks; b++) {
-                const unsigned bar = te_even(pg_smem(&sh.a_full[b]));
-                te_expect(bar, tl_pages(a, seq, key0, to));
-                for (int i = 0; i < TL_KEYS && key0 + i < to; i += a.page)
-                    te_tma(pg_smem(as + b * TL_BLOCK) + i * 128, &map_rows, bar, b * 64, a.table[(int64_t)seq * a.table_cols + ((key0 + i) >> a.shift)] * a.page);
+        const int pages = found < 0 ? 0 : (min(TL_KEYS, to - key0) + a.page - 1) >> a.shift, mine = tl_look_up(a, seq, key0, to);
+        for (int b = 0; b < blocks; b++) {
+            const unsigned bar = te_even(pg_smem(&sh.a_full[b]));
+            if (lane == 0) te_expect(bar, (unsigned)(pages * a.page * 128));
+            __syncwarp();
+            for (int i = 0; i < pages; i++) {
+                const int page = __shfl_sync(0xffffffffu, mine, i);
+                if (pg_elect()) te_tma_page(pg_smem(as + b * TL_BLOCK) + i * a.page * 128, &map_rows, bar, b * 64, page);
             }
+        }
+        __syncwarp();
+        if (lane == 0) {
             unsigned g = 0;
             bool ok = true;
             for (int h = h0; h < h1 && ok; h++)
@@ -218,40 +228,63 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TE_THREADS, 1) laten
         }
         tl_wait_warp(pg_smem(&sh.drained), 0, &never);
     } else if (warp >= 4) {
-        // a lane a key, the two warps of its lanes every second run of 16 columns
-        const int q = warp & 3, row = q * 32 + lane, width = a.dim + a.vdim;
+        // a lane a key; four warps the keys' blocks of 64 columns, the others the values': by way of shared memory, from where a block goes to its image as a whole.  (Stored by each lane 16 bytes
+        // at a time, 128 apart, a head took 5500 cycles, its products 4100)
+        const int q = warp & 3, row = q * 32 + lane, is_v = (warp - 4) >> 2, d = is_v ? a.vdim : a.dim;
         const bool in = key0 + row < to;
+        uint8_t* stage = bs + TE_STAGES * TE_STAGE + is_v * TL_BLOCK;
         for (int h = h0; h < h1; h++) {
             const unsigned n = (unsigned)(h - h0);
             if (!tl_wait_warp(pg_smem(&sh.acc_full[n & 1u]), (n >> 1) & 1u, &sh.fail)) break;
             pg_fence_after();
-            const size_t image = (size_t)blockIdx.x * t.heads + h;
-            uint8_t *ki = t.k_image + image * ((a.dim + 63) >> 6) * TL_BLOCK, *vi = t.v_image + image * ((a.vdim + 63) >> 6) * TL_BLOCK;
-            for (int c = ((warp - 4) >> 2) * 16; c < width; c += 32) {
-                const bool is_k = c < a.dim;
-                const int col = is_k ? c : c - a.dim;
-                unsigned v[16], w[8];
-                sg_tmem16(tmem + (n & 1u) * 256 + ((unsigned)(q * 32) << 16) + (is_k ? 0 : wide) + col, v);
+            uint8_t* image = (is_v ? t.v_image : t.k_image) + ((size_t)blockIdx.x * t.heads + h) * ((d + 63) >> 6) * TL_BLOCK;
+#pragma unroll 1
+            for (int c = 0; c < d; c += 64) {
+                unsigned v[4][16];
+#pragma unroll
+                for (int x = 0; x < 4; x++)
+                    if (c + x * 16 < d) sg_tmem16(tmem + (n & 1u) * 256 + ((unsigned)(q * 32) << 16) + is_v * wide + c + x * 16, v[x]);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                // a cached row that is not finite makes all of its keys and values so: a NaN in a key reaches the queries that see it, a zero in its value no one
+                if (row == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the block before has left
+                te_sync(is_v);
 #pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    asm volatile("" : "+r"(v[j]));
-                    if (!(fabsf(__uint_as_float(v[j])) < INFINITY)) v[j] = is_k ? 0x7fc00000u : 0u;
-                    if (!is_k && !in) v[j] = 0u;
+                for (int x = 0; x < 4; x++) {
+#pragma unroll
+                    for (int j = 0; j < 16; j++) asm volatile("" : "+r"(v[x][j]));
+                    if (c + x * 16 >= d) continue;
+                    unsigned w[8], wild = 0;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        w[j] = lt_pack(__uint_as_float(v[x][2 * j]), __uint_as_float(v[x][2 * j + 1]));
+                        wild |= (w[j] & 0x7c007c00u) + 0x04000400u;   // the exponent of an infinity or a NaN carries into the sign's place
+                    }
+                    if (wild & 0x80008000u) {
+                        // beyond f16; or a cached row that is not finite, which makes all of its keys and values so: a NaN in a key reaches the queries that see it, a zero in its value no one
+#pragma unroll
+                        for (int j = 0; j < 16; j++)
+                            if (!(fabsf(__uint_as_float(v[x][j])) < INFINITY)) v[x][j] = is_v ? 0u : 0x7fc00000u;
+#pragma unroll
+                        for (int j = 0; j < 8; j++) w[j] = ht_pack_f16(__uint_as_float(v[x][2 * j]), __uint_as_float(v[x][2 * j + 1]));
+                    }
+                    if (is_v && !in) {
+#pragma unroll
+                        for (int j = 0; j < 8; j++) w[j] = 0u;
+                    }
+                    *(uint4*)(stage + tl_at(row, 2 * x)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    *(uint4*)(stage + tl_at(row, 2 * x + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
                 }
-#pragma unroll
-                for (int j = 0; j < 8; j++) w[j] = ht_pack_f16(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
-                uint8_t* at = (is_k ? ki : vi) + (col >> 6) * TL_BLOCK;
-                if ((int)blockIdx.x < t.key_tiles) {
-                    *(uint4*)(at + tl_at(row, (col & 63) >> 3)) = make_uint4(w[0], w[1], w[2], w[3]);
-                    *(uint4*)(at + tl_at(row, ((col & 63) >> 3) + 1)) = make_uint4(w[4], w[5], w[6], w[7]);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                te_sync(is_v);
+                if (row == 0 && (int)blockIdx.x < t.key_tiles) {
+                    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(image + (c >> 6) * TL_BLOCK), "r"(pg_smem(stage)), "r"(TL_BLOCK) : "memory");
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                 }
             }
             pg_fence_before();
             __syncwarp();
             if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(te_even(pg_smem(&sh.acc_empty[n & 1u]))) : "memory");
         }
+        if (row == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     pg_fence_before();
     __syncthreads();
@@ -273,6 +306,9 @@ __device__ __forceinline__ bool tl_sync_or(int bar, bool x) {
     unsigned r;
     asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbar.red.or.pred q, %2, %3, p;\nselp.u32 %0, 1, 0, q;\n}\n" : "=r"(r) : "r"((unsigned)x), "r"(bar), "n"(TL_SOFT * 16) : "memory");
     return r;
+}
+__device__ __forceinline__ void tl_tma_page(unsigned dst, const void* tmap, unsigned bar, int x, int page) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(tmap), "r"(bar), "r"(x), "r"(0), "r"(page) : "memory");
 }
 // B whose rows are the sum's index and whose columns (64 of them in 128 bytes) are the result's: blocks of 64 columns `block` bytes apart, groups of 8 rows 1024 bytes
 __device__ __forceinline__ uint64_t tl_desc_mn(unsigned addr, unsigned block) {
@@ -374,38 +410,49 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TL_REGS_REST));
         if (warp == TL_SOFT) {
             // ===== copies: Q, then the blocks of each step =====
-            if (lane == 0) {
-                const int width = a.dim + a.rest;
+            const int width = a.dim + a.rest;
+            if (pg_elect()) {
                 pg_mbar_expect_tx(pg_smem(&sh.q_full), (unsigned)(2 * (nb + rb) * TL_BLOCK));
                 for (int i = 0; i < 2; i++)
                     for (int b = 0; b < nb + rb; b++)
                         pg_tma_load_2d(pg_smem(qs + (i * TL_QBLOCKS + b) * TL_BLOCK), &map_q, pg_smem(&sh.q_full), head * width + (b < nb ? b * 64 : a.dim), s.first + row0 + i * TL_ROWS);
-                unsigned g = 0, groups = 0;
-                bool ok = true;
-                for (int k = 0; k < steps && ok; k++) {
-                    const size_t image = (size_t)(kt0 + k) * t.heads + head_at;
-                    for (int b = 0; b < per; b++, g++) {
-                        const unsigned at = pg_smem(ring + g % TL_SLOTS * TL_BLOCK), full = pg_smem(&sh.full[(2 * k + (b >= nb + rb)) % TL_GROUPS]);
-                        if (g >= TL_SLOTS) {                          // the group of the block that was here is through
-                            const unsigned was = g - TL_SLOTS, of = 2 * (was / per) + (was % per >= (unsigned)(nb + rb));
-                            if (!(ok = tl_wait(pg_smem(&sh.empty[of % TL_GROUPS]), (of / TL_GROUPS) & 1u, &sh.fail))) break;
-                        }
-                        if (b == 0) { pg_mbar_expect_tx(full, (unsigned)(nb * TL_BLOCK) + (rb ? tl_pages(a, seq, lo + k * TL_KEYS, to) : 0u)); groups++; }
-                        if (b == nb + rb) { pg_mbar_expect_tx(full, (unsigned)(vb * TL_BLOCK)); groups++; }
-                        if (b >= nb && b < nb + rb) tl_load_pages(a, &map_rows, at, full, a.rank, seq, lo + k * TL_KEYS, to);
-                        else {
-                            const uint8_t* src = b < nb ? t.k_image + (image * nb + b) * TL_BLOCK : t.v_image + (image * vb + b - nb - rb) * TL_BLOCK;
-                            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(at), "l"(src), "r"(TL_BLOCK), "r"(full) : "memory");
-                        }
-                    }
-                }
-                // no copy is under way when the CTA ends.  Where a wait ran out in the midst of a group, what it lacks never comes: a while for what does
-                int never = 0;
-                if (ok) for (unsigned i = groups > TL_GROUPS ? groups - TL_GROUPS : 0; i < groups; i++) tl_wait(pg_smem(&sh.full[i % TL_GROUPS]), (i / TL_GROUPS) & 1u, &never);
-                else for (int i = 0; i < 1000; i++) __nanosleep(1000);
-                tl_wait(pg_smem(&sh.q_full), 0, &never);
             }
             __syncwarp();
+            unsigned g = 0, groups = 0;
+            bool ok = true;
+            int mine = tl_look_up(a, seq, lo, to);
+            for (int k = 0; k < steps && ok; k++) {
+                const size_t image = (size_t)(kt0 + k) * t.heads + head_at;
+                const int key0 = lo + k * TL_KEYS, pages = (min(TL_KEYS, to - key0) + a.page - 1) >> a.shift, those = mine;
+                if (k + 1 < steps) mine = tl_look_up(a, seq, key0 + TL_KEYS, to);
+                for (int b = 0; b < per; b++, g++) {
+                    const unsigned at = pg_smem(ring + g % TL_SLOTS * TL_BLOCK), full = pg_smem(&sh.full[(2 * k + (b >= nb + rb)) % TL_GROUPS]);
+                    if (g >= TL_SLOTS) {                              // the group of the block that was here is through
+                        const unsigned was = g - TL_SLOTS, of = 2 * (was / per) + (was % per >= (unsigned)(nb + rb));
+                        if (!(ok = tl_wait_warp(pg_smem(&sh.empty[of % TL_GROUPS]), (of / TL_GROUPS) & 1u, &sh.fail))) break;
+                    }
+                    if (b == 0 || b == nb + rb) {
+                        if (pg_elect()) pg_mbar_expect_tx(full, b ? (unsigned)(vb * TL_BLOCK) : (unsigned)(nb * TL_BLOCK + rb * pages * a.page * 128));
+                        __syncwarp();
+                        groups++;
+                    }
+                    if (b >= nb && b < nb + rb)
+                        for (int i = 0; i < pages; i++) {
+                            const int page = __shfl_sync(0xffffffffu, those, i);
+                            if (pg_elect()) tl_tma_page(at + i * a.page * 128, &map_rows, full, a.rank, page);
+                        }
+                    else if (pg_elect()) {
+                        const uint8_t* src = b < nb ? t.k_image + (image * nb + b) * TL_BLOCK : t.v_image + (image * vb + b - nb - rb) * TL_BLOCK;
+                        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(at), "l"(src), "r"(TL_BLOCK), "r"(full) : "memory");
+                    }
+                    __syncwarp();
+                }
+            }
+            // no copy is under way when the CTA ends.  Where a wait ran out in the midst of a group, what it lacks never comes: a while for what does
+            int never = 0;
+            if (ok) for (unsigned i = groups > TL_GROUPS ? groups - TL_GROUPS : 0; i < groups; i++) tl_wait_warp(pg_smem(&sh.full[i % TL_GROUPS]), (i / TL_GROUPS) & 1u, &never);
+            else for (int i = 0; i < 1000; i++) __nanosleep(1000);
+            tl_wait_warp(pg_smem(&sh.q_full), 0, &never);
         } else if (warp == TL_SOFT + 1) {
             // ===== products =====
             const unsigned idesc_s = pg_instr_desc(128, TL_KEYS), idesc_o = pg_instr_desc(128, a.vdim) | 1u << 16, idesc_lo = pg_instr_desc(128, 64) | 1u << 16, idesc_hi = pg_instr_desc(128, a.vdim - 64) | 1u << 16;
@@ -631,7 +678,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
 static int tl_run(cc_device* dev, const cc_page_plan* plan, const LrArgs& all) {
     const int64_t per = (int64_t)((all.dim + 63) / 64 + (all.vdim + 63) / 64) * TL_BLOCK, width = all.dim + all.rest;
     CUtensorMap rows, q, uk, uv;
-    int rc = cc_make_tmap_rows(dev, &rows, all.rows, plan->n_pages * plan->page, all.cols, (int64_t)all.cols * 2, plan->page, false);
+    int rc = cc_make_tmap_pages(dev, &rows, all.rows, plan->n_pages, plan->page, all.cols, plan->page);
     if (!rc) rc = cc_make_tmap_rows(dev, &q, all.q, plan->tokens, all.H * width, all.H * width * 2, TL_ROWS, false);
     const int wide = std::max(all.dim, all.vdim);
     if (!rc) rc = cc_make_tmap_rows(dev, &uk, all.uk, (int64_t)all.H * all.dim, all.rank, (int64_t)all.rank * 2, wide, false);

@@ -442,6 +442,16 @@ int cc_make_tmap_rows(cc_device* dev, void* tm, const void* base, int64_t rows, 
                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? CC_OK : cc_fail(dev, CC_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
 }
+// pages [n_pages][page][cols] of 16-bit numbers, box 64 columns x box_rows rows of one page
+int cc_make_tmap_pages(cc_device* dev, void* tm, const void* base, int64_t n_pages, int page, int cols, int box_rows) {
+    PFN_encodeTiled enc = pg_encode();
+    if (!enc) return cc_fail(dev, CC_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+    cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)page, (cuuint64_t)n_pages}, strides[2] = {(cuuint64_t)cols * 2, (cuuint64_t)cols * 2 * page};
+    cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, estr[3] = {1, 1, 1};
+    const CUresult r = enc((CUtensorMap*)tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, (void*)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? CC_OK : cc_fail(dev, CC_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+}
 int cc_make_tmap_i8(cc_device* dev, void* tm, const void* base, int64_t rows, int64_t k, int box_rows) { return pg_make_tmap(dev, (CUtensorMap*)tm, base, rows, k, box_rows, false, 1); }
 int cc_make_tmap_bf16(cc_device* dev, void* tm, const void* base, int64_t rows, int64_t k, int box_rows) { return pg_make_tmap(dev, (CUtensorMap*)tm, base, rows, k, box_rows, true); }
 
