@@ -378,7 +378,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
         auto release = [&](unsigned n) {
             pg_fence_before();
             __syncwarp();
-            if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(pt_even(pg_smem(&sh.acc_empty[n & 1u]))) : "memory");
+            if (lane == 0) pg_arrive_relaxed(pt_even(pg_smem(&sh.acc_empty[n & 1u])));
         };
         for (int tile = first; tile < n_tiles; tile += stride, nth++) {
             int mt, at;

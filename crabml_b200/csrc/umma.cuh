@@ -62,3 +62,6 @@ __device__ __forceinline__ bool pg_elect() {
     asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
     return r != 0;
 }
+// Arrival on a barrier of the cluster by a thread whose reads of tensor memory are complete (tcgen05.wait::ld) and that has written nothing for those who wait: relaxed, since a release to the
+// cluster waits for the thread's stores to memory, 1300 cycles and more
+__device__ __forceinline__ void pg_arrive_relaxed(unsigned bar) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
