@@ -21,11 +21,6 @@
 
 #define LR_GROUPS 2
 #define LR_THREADS (LR_GROUPS * 256)
-#define LR_ALL (LR_THREADS + 128)             // a warp more brings the rows
-// 640 threads of 96 registers at launch are 512 of 112 and 128 of 32 afterwards
-#define LR_REGS 112
-#define LR_REGS_REST 32
-static_assert(LR_THREADS * LR_REGS + 128 * LR_REGS_REST <= LR_ALL * 96, "more registers than the block was launched with");
 #define LR_BLOCK 4096                         // 32 rows of 64 columns
 #define LR_ROWS 16                            // queries of a tile
 #define LR_KEYS 32                            // of a step
@@ -35,11 +30,14 @@ static_assert(LR_THREADS * LR_REGS + 128 * LR_REGS_REST <= LR_ALL * 96, "more re
 #define LR_SHIFT 10.0f                        // weights are exp2(score - largest + LR_SHIFT)
 #define LR_KB 9                               // column blocks of 16 of a warp's scores: (LT_RANK + LT_REST) / 16 / 4
 #define LR_VB 4                               // .. of its values: LT_RANK / 16 / 8
+#define LR_RUNS 5                             // runs of 128 columns of a row
 #define LR_CTAS 160
+#define LJ_FEW 8                              // slices of a segment that are added up over all columns at a time
 #define LR_LOG2E 1.4426950408889634f
 
 // runs of consecutive tokens whose sequences take this form
 #define LT_RUNS 64
+#define LT_TOKENS 32                          // of a tile of the products in front and behind
 struct LtRuns { int n, tiles; int lo[LT_RUNS], hi[LT_RUNS], tile0[LT_RUNS]; };
 struct LrArgs {
     const PgSeq* seqs;
@@ -48,6 +46,7 @@ struct LrArgs {
     const float* sink;
     float *qf, *lat, *part;                   // queries over the latents [T H][cols]; results over the latents [T H][rank]; sums of cut segments [2 x CTA][LR_ROWS][rank]
     float2* ml;                               // [2 x CTA][LR_ROWS]: largest score (base 2), sum of weights
+    int4* steps;                              // [CTA][run_lo + 1]: what each step asks for
     void* out;
     float scale;
     int n_seqs, table_cols, page, shift, H, dim, vdim, rank, rest, cols, window, most, out_bf16, slots;      // most: sequences with more new tokens take the other form
@@ -97,135 +96,11 @@ __device__ __forceinline__ void lt_copies_done() { asm volatile("cp.async.commit
 __device__ __forceinline__ bool lt_tile(const LtRuns& runs, int tile, int* lo, int* hi) {
     for (int i = 0; i < runs.n; i++) {
         const int t = tile - runs.tile0[i];
-        if (t >= 0 && runs.lo[i] + t * 16 < runs.hi[i]) { *lo = runs.lo[i] + t * 16; *hi = min(*lo + 16, runs.hi[i]); return true; }
+        if (t >= 0 && runs.lo[i] + t * LT_TOKENS < runs.hi[i]) { *lo = runs.lo[i] + t * LT_TOKENS; *hi = min(*lo + LT_TOKENS, runs.hi[i]); return true; }
     }
     return false;
 }
 
-// ---- queries to the latents, results back ---------------------------------------------------------------------------------------------------
-// qf[t, h, :rank] = U_h^T n[t, h], qf[t, h, rank:] = p[t, h], in 32 bits.  grid (heads, blocks of 64 columns and one for p, tiles of 16 tokens by turns); a warp 16 columns
-#define LF_COLS 64
-__global__ void __launch_bounds__(128) latent_fold_kernel(const LrArgs a, const __grid_constant__ LtRuns runs) {
-    extern __shared__ __align__(16) uint8_t lf_raw[];
-    __half *bs = (__half*)lf_raw, *as = bs + a.dim * (LF_COLS + 8);      // U_h's rows, 64 columns of them; queries [16][dim + 8]
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.x, c0 = blockIdx.y * LF_COLS, width = a.dim + a.rest;
-    pdl_enter();
-    if (c0 >= a.rank) {                                                  // p
-        for (int tile = blockIdx.z; tile < runs.tiles; tile += gridDim.z) {
-            int lo, hi;
-            if (!lt_tile(runs, tile, &lo, &hi)) return;
-            for (int e = tid; e < (hi - lo) * a.rest; e += 128) {
-                const int64_t row = (int64_t)(lo + e / a.rest) * a.H + h;
-                a.qf[row * a.cols + a.rank + e % a.rest] = __half2float(a.q[row * width + a.dim + e % a.rest]);
-            }
-        }
-        return;
-    }
-    for (int e = tid; e < a.dim * (LF_COLS / 8); e += 128) {
-        const int r = e / (LF_COLS / 8), c = e % (LF_COLS / 8) * 8;
-        if (c0 + c < a.rank) lt_copy16(pg_smem(bs + r * (LF_COLS + 8) + c), a.uk + ((int64_t)h * a.dim + r) * a.rank + c0 + c);
-    }
-    for (int tile = blockIdx.z; tile < runs.tiles; tile += gridDim.z) {
-        int lo, hi;
-        if (!lt_tile(runs, tile, &lo, &hi)) return;
-        __syncthreads();
-        for (int e = tid; e < 16 * a.dim / 8; e += 128) {
-            const int r = e / (a.dim / 8), c = e % (a.dim / 8) * 8;
-            *(uint4*)(as + r * (a.dim + 8) + c) = lo + r < hi ? __ldg((const uint4*)(a.q + ((int64_t)(lo + r) * a.H + h) * width + c)) : make_uint4(0, 0, 0, 0);
-        }
-        lt_copies_done();
-        __syncthreads();
-        if (c0 + warp * 16 >= a.rank) continue;
-        float acc[2][4] = {};
-#pragma unroll 4
-        for (int k = 0; k < a.dim; k += 16) {
-            unsigned x[4], b[4];
-            lt_ldsm(x, pg_smem(as + ((lane & 7) + (lane >> 3 & 1) * 8) * (a.dim + 8) + k + (lane >> 4) * 8));
-            lt_ldsm_t(b, pg_smem(bs + (k + (lane & 7) + (lane >> 3 & 1) * 8) * (LF_COLS + 8) + warp * 16 + (lane >> 4) * 8));
-            lt_mma(acc[0], x, b[0], b[1]);
-            lt_mma(acc[1], x, b[2], b[3]);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int y = 0; y < 2; y++) {
-                const int t = lo + (lane >> 2) + y * 8;
-                if (t < hi) *(float2*)(a.qf + ((int64_t)t * a.H + h) * a.cols + c0 + warp * 16 + i * 8 + (lane & 3) * 2) = make_float2(acc[i][2 * y], acc[i][2 * y + 1]);
-            }
-    }
-}
-// out[t, h] = V_h lat[t, h].  grid (heads, blocks of 32 columns, tiles of 16 tokens by turns); a warp 8 columns
-#define LU_COLS 32
-__global__ void __launch_bounds__(128) latent_unfold_kernel(const LrArgs a, const __grid_constant__ LtRuns runs) {
-    extern __shared__ __align__(16) uint8_t lf_raw[];
-    const int pitch = a.rank + 8;
-    __half *bs = (__half*)lf_raw, *as = bs + LU_COLS * pitch;          // V_h's rows; sums of latents [h, l][16][pitch]
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.x, c0 = blockIdx.y * LU_COLS;
-    pdl_enter();
-    for (int e = tid; e < LU_COLS * (a.rank / 8); e += 128) {
-        const int r = e / (a.rank / 8), c = e % (a.rank / 8) * 8;
-        if (c0 + r < a.vdim) lt_copy16(pg_smem(bs + r * pitch + c), a.uv + ((int64_t)h * a.vdim + c0 + r) * a.rank + c);
-        else *(uint4*)(bs + r * pitch + c) = make_uint4(0, 0, 0, 0);
-    }
-    for (int tile = blockIdx.z; tile < runs.tiles; tile += gridDim.z) {
-        int lo, hi;
-        if (!lt_tile(runs, tile, &lo, &hi)) break;
-        __syncthreads();
-        for (int e = tid; e < 16 * a.rank / 4; e += 128) {
-            const int r = e / (a.rank / 4), c = e % (a.rank / 4) * 4;
-            const float4 v = lo + r < hi ? *(const float4*)(a.lat + ((int64_t)(lo + r) * a.H + h) * a.rank + c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            uint2 x, y;
-            lt_cut(v.x, v.y, x.x, y.x); lt_cut(v.z, v.w, x.y, y.y);
-            *(uint2*)(as + r * pitch + c) = x;
-            *(uint2*)(as + (16 + r) * pitch + c) = y;
-        }
-        lt_copies_done();
-        __syncthreads();
-        float acc[4] = {};
-        const int r = (lane & 7) + (lane >> 3 & 1) * 8, kc = (lane >> 4) * 8;
-#pragma unroll 4
-        for (int k = 0; k < a.rank; k += 16) {
-            unsigned x[4], y[4], b0, b1;
-            lt_ldsm(x, pg_smem(as + r * pitch + k + kc));
-            lt_ldsm(y, pg_smem(as + (16 + r) * pitch + k + kc));
-            asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];" : "=r"(b0), "=r"(b1) : "r"(pg_smem(bs + (warp * 8 + (lane & 7)) * pitch + k + (lane >> 3 & 1) * 8)));
-            lt_mma(acc, x, b0, b1);
-            lt_mma(acc, y, b0, b1);
-        }
-        const int c = c0 + warp * 8 + (lane & 3) * 2;
-#pragma unroll
-        for (int y = 0; y < 2; y++) {
-            const int t = lo + (lane >> 2) + y * 8;
-            if (t < hi && c < a.vdim) *(unsigned*)((uint16_t*)a.out + ((int64_t)t * a.H + h) * a.vdim + c) = a.out_bf16 ? ht_pack_bf16(acc[2 * y], acc[2 * y + 1]) : ht_pack_f16(acc[2 * y], acc[2 * y + 1]);
-        }
-    }
-}
-
-// ---- the cached rows as keys and values ----------------------------------------------------------------------------------------------------------
-struct LrShared {
-    unsigned long long full[LR_SLOTS], empty[LR_SLOTS];
-    int fail;
-    unsigned wild;                            // rows whose sums are not finite
-    float top[LR_GROUPS][LR_ROWS], sum[LR_GROUPS][LR_ROWS];      // of a segment: largest score and sum of weights of each group
-    float factor[LR_ROWS], up[LR_ROWS];       // of a row's scores; what its query is multiplied by
-    float alpha[LR_GROUPS][LR_ROWS];
-    __align__(16) float sums[LR_GROUPS][4][LR_ROWS][40];      // of a step: scores by column groups.  At a segment's end, sums on their way from group to group
-    __align__(16) __half p[LR_GROUPS][LR_ROWS][40];
-};
-static_assert(sizeof(float) * LR_GROUPS * 4 * LR_ROWS * 40 >= LR_THREADS / LR_GROUPS * 16 * sizeof(float), "half of a group's sums");
-__device__ __forceinline__ void lr_sync(int group) { asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(LR_THREADS / LR_GROUPS) : "memory"); }
-__device__ __forceinline__ bool lr_sync_or(int group, bool x) {
-    unsigned r;
-    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbar.red.or.pred q, %2, %3, p;\nselp.u32 %0, 1, 0, q;\n}\n" : "=r"(r) : "r"((unsigned)x), "r"(1 + group), "n"(LR_THREADS / LR_GROUPS) : "memory");
-    return r;
-}
-__device__ __forceinline__ void lr_sync_all() { asm volatile("bar.sync 3, %0;" ::"n"(LR_THREADS) : "memory"); }
-__device__ __forceinline__ bool lr_sync_all_or(bool x) {
-    unsigned r;
-    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbar.red.or.pred q, 3, %2, p;\nselp.u32 %0, 1, 0, q;\n}\n" : "=r"(r) : "r"((unsigned)x), "n"(LR_THREADS) : "memory");
-    return r;
-}
-__device__ __forceinline__ void lr_zero(unsigned at) { asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory"); }
 // a CTA's run of steps, segment by segment; the begin of a segment counts LR_BEGIN of them
 struct LrWalk {
     int seq, tile, off, left;
@@ -244,6 +119,188 @@ struct LrWalk {
         return false;
     }
 };
+// what a step asks for: two pages, the row in them where it begins, how many of them (0: nothing)
+__device__ __forceinline__ int4 lr_pages(const LrArgs& a, int seq, int key0, int to) {
+    const int rows = min(a.page, LR_KEYS), there = (min(LR_KEYS, to - key0) + rows - 1) / rows;
+    const int* t = a.table + (int64_t)seq * a.table_cols + (key0 >> a.shift);
+    return make_int4(t[0], there > 1 ? t[1] : 0, key0 & (a.page - 1), there);
+}
+
+// ---- queries to the latents, results back ---------------------------------------------------------------------------------------------------
+// qf[t, h, :rank] = U_h^T n[t, h], qf[t, h, rank:] = p[t, h], in 32 bits.  grid (heads, blocks of 64 columns and one for p, tiles of LT_TOKENS tokens by turns); a warp 16 columns.
+// The blocks behind write down what the steps of each CTA of latent_rows_kernel ask for, a warp a CTA
+#define LF_COLS 64
+__global__ void __launch_bounds__(128) latent_fold_kernel(const __grid_constant__ LrArgs a, const __grid_constant__ LtRuns runs, const __grid_constant__ LrDeal deal) {
+    extern __shared__ __align__(16) uint8_t lf_raw[];
+    __half *bs = (__half*)lf_raw, *as = bs + a.dim * (LF_COLS + 8);      // U_h's rows, 64 columns of them; queries [LT_TOKENS][dim + 8]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.x, c0 = blockIdx.y * LF_COLS, width = a.dim + a.rest;
+    pdl_enter();
+    const int fold_blocks = (a.rank + LF_COLS - 1) / LF_COLS;
+    if ((int)blockIdx.y > fold_blocks) {
+        const int c = (((int)blockIdx.y - fold_blocks - 1) * a.H + h) * 4 + warp, room = deal.run_lo + 1;
+        if (c >= deal.ctas || blockIdx.z) return;
+        LrWalk walk = {deal.at[c].seq, deal.at[c].tile, deal.at[c].off, deal.run_lo + (c < deal.run_more ? 1 : 0)};
+        int4* to_list = a.steps + (int64_t)c * room;
+        int n = 0;
+        while (walk.piece(a, [&](const PgSeq& s, int seq, int, int k0, int k1, bool) {
+            int from, to;
+            lr_range(s, a, &from, &to);
+            for (int k = k0 + lane; k < k1; k += 32) to_list[n + k - k0] = lr_pages(a, seq, from + k * LR_KEYS, to);
+            n += k1 - k0;
+        })) {}
+        for (int i = n + lane; i < room; i += 32) to_list[i] = make_int4(0, 0, 0, 0);
+        return;
+    }
+    if ((int)blockIdx.y == fold_blocks) {                                // p
+        for (int tile = blockIdx.z; tile < runs.tiles; tile += gridDim.z) {
+            int lo, hi;
+            if (!lt_tile(runs, tile, &lo, &hi)) return;
+#pragma unroll 2
+            for (int e = tid; e < (hi - lo) * (a.rest / 8); e += 128) {
+                const int64_t row = (int64_t)(lo + e / (a.rest / 8)) * a.H + h;
+                const int c = e % (a.rest / 8) * 8;
+                const uint4 v = __ldg((const uint4*)(a.q + row * width + a.dim + c));
+                const float2 x = __half22float2(*(const __half2*)&v.x), y = __half22float2(*(const __half2*)&v.y), z = __half22float2(*(const __half2*)&v.z), w = __half22float2(*(const __half2*)&v.w);
+                float4* at = (float4*)(a.qf + row * a.cols + a.rank + c);
+                at[0] = make_float4(x.x, x.y, y.x, y.y); at[1] = make_float4(z.x, z.y, w.x, w.y);
+            }
+        }
+        return;
+    }
+    for (int e = tid; e < a.dim * (LF_COLS / 8); e += 128) {
+        const int r = e / (LF_COLS / 8), c = e % (LF_COLS / 8) * 8;
+        if (c0 + c < a.rank) lt_copy16(pg_smem(bs + r * (LF_COLS + 8) + c), a.uk + ((int64_t)h * a.dim + r) * a.rank + c0 + c);
+    }
+    for (int tile = blockIdx.z; tile < runs.tiles; tile += gridDim.z) {
+        int lo, hi;
+        if (!lt_tile(runs, tile, &lo, &hi)) return;
+        const int mt = (hi - lo + 15) >> 4, runs8 = a.dim / 8;
+        __syncthreads();
+        for (int e = tid; e < mt * 16 * runs8; e += 128) {
+            const int r = e / runs8, c = e % runs8 * 8;
+            if (lo + r < hi) lt_copy16(pg_smem(as + r * (a.dim + 8) + c), a.q + ((int64_t)(lo + r) * a.H + h) * width + c);
+            else *(uint4*)(as + r * (a.dim + 8) + c) = make_uint4(0, 0, 0, 0);
+        }
+        lt_copies_done();
+        __syncthreads();
+        if (c0 + warp * 16 >= a.rank) continue;
+        float acc[LT_TOKENS / 16][2][4];
+#pragma unroll
+        for (int i = 0; i < LT_TOKENS / 16 * 8; i++) acc[i >> 3][i >> 2 & 1][i & 3] = 0.0f;
+#pragma unroll 2
+        for (int k = 0; k < a.dim; k += 16) {
+            unsigned x[4], b[4];
+            lt_ldsm_t(b, pg_smem(bs + (k + (lane & 7) + (lane >> 3 & 1) * 8) * (LF_COLS + 8) + warp * 16 + (lane >> 4) * 8));
+#pragma unroll
+            for (int m = 0; m < LT_TOKENS / 16; m++)
+                if (m < mt) {
+                    lt_ldsm(x, pg_smem(as + (m * 16 + (lane & 7) + (lane >> 3 & 1) * 8) * (a.dim + 8) + k + (lane >> 4) * 8));
+                    lt_mma(acc[m][0], x, b[0], b[1]);
+                    lt_mma(acc[m][1], x, b[2], b[3]);
+                }
+        }
+#pragma unroll
+        for (int m = 0; m < LT_TOKENS / 16; m++)
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int y = 0; y < 2; y++) {
+                    const int t = lo + m * 16 + (lane >> 2) + y * 8;
+                    if (t < hi) *(float2*)(a.qf + ((int64_t)t * a.H + h) * a.cols + c0 + warp * 16 + i * 8 + (lane & 3) * 2) = make_float2(acc[m][i][2 * y], acc[m][i][2 * y + 1]);
+                }
+    }
+}
+// out[t, h] = V_h lat[t, h].  grid (heads, blocks of 32 columns, tiles of LT_TOKENS tokens by turns); a warp 8 columns and half of the depth
+#define LU_COLS 32
+#define LU_THREADS 256
+__host__ __device__ constexpr int lu_smem(int rank) { return (LU_COLS + 2 * LT_TOKENS) * (rank + 8) * 2; }
+__global__ void __launch_bounds__(LU_THREADS) latent_unfold_kernel(const __grid_constant__ LrArgs a, const __grid_constant__ LtRuns runs) {
+    extern __shared__ __align__(16) uint8_t lf_raw[];
+    __shared__ float sums[LT_TOKENS][LU_COLS + 1];
+    const int pitch = a.rank + 8;
+    __half *bs = (__half*)lf_raw, *as = bs + LU_COLS * pitch;          // V_h's rows; sums of latents [h, l][LT_TOKENS][pitch]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.x, c0 = blockIdx.y * LU_COLS, cg = warp & 3, part = warp >> 2;
+    pdl_enter();
+    for (int e = tid; e < LU_COLS * (a.rank / 8); e += LU_THREADS) {
+        const int r = e / (a.rank / 8), c = e % (a.rank / 8) * 8;
+        if (c0 + r < a.vdim) lt_copy16(pg_smem(bs + r * pitch + c), a.uv + ((int64_t)h * a.vdim + c0 + r) * a.rank + c);
+        else *(uint4*)(bs + r * pitch + c) = make_uint4(0, 0, 0, 0);
+    }
+    for (int tile = blockIdx.z; tile < runs.tiles; tile += gridDim.z) {
+        int lo, hi;
+        if (!lt_tile(runs, tile, &lo, &hi)) break;
+        const int mt = (hi - lo + 15) >> 4, runs4 = a.rank / 4;
+        __syncthreads();
+#pragma unroll 4
+        for (int e = tid; e < mt * 16 * runs4; e += LU_THREADS) {
+            const int r = e / runs4, c = e % runs4 * 4;
+            const float4 v = lo + r < hi ? *(const float4*)(a.lat + ((int64_t)(lo + r) * a.H + h) * a.rank + c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            uint2 x, y;
+            lt_cut(v.x, v.y, x.x, y.x); lt_cut(v.z, v.w, x.y, y.y);
+            *(uint2*)(as + r * pitch + c) = x;
+            *(uint2*)(as + (LT_TOKENS + r) * pitch + c) = y;
+        }
+        lt_copies_done();
+        __syncthreads();
+        float acc[LT_TOKENS / 16][2][4];
+#pragma unroll
+        for (int i = 0; i < LT_TOKENS / 16 * 8; i++) acc[i >> 3][i >> 2 & 1][i & 3] = 0.0f;
+        const int r = (lane & 7) + (lane >> 3 & 1) * 8, kc = (lane >> 4) * 8, half = a.rank / 32 * 16;
+#pragma unroll 4
+        for (int k = part ? half : 0; k < (part ? a.rank : half); k += 16) {
+            unsigned b0, b1;
+            asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];" : "=r"(b0), "=r"(b1) : "r"(pg_smem(bs + (cg * 8 + (lane & 7)) * pitch + k + (lane >> 3 & 1) * 8)));
+#pragma unroll
+            for (int m = 0; m < LT_TOKENS / 16; m++)
+                if (m < mt) {
+                    unsigned x[4], y[4];
+                    lt_ldsm(x, pg_smem(as + (m * 16 + r) * pitch + k + kc));
+                    lt_ldsm(y, pg_smem(as + (LT_TOKENS + m * 16 + r) * pitch + k + kc));
+                    lt_mma(acc[m][0], x, b0, b1);
+                    lt_mma(acc[m][1], y, b0, b1);
+                }
+        }
+        const int c = cg * 8 + (lane & 3) * 2;
+#pragma unroll
+        for (int m = 0; m < LT_TOKENS / 16; m++)
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+                const int t = m * 16 + (lane >> 2) + y * 8;
+                if (part == 1) { sums[t][c] = acc[m][0][2 * y] + acc[m][1][2 * y]; sums[t][c + 1] = acc[m][0][2 * y + 1] + acc[m][1][2 * y + 1]; }
+            }
+        __syncthreads();
+        if (part == 0) {
+#pragma unroll
+            for (int m = 0; m < LT_TOKENS / 16; m++)
+#pragma unroll
+                for (int y = 0; y < 2; y++) {
+                    const int t = m * 16 + (lane >> 2) + y * 8;
+                    const float u = acc[m][0][2 * y] + acc[m][1][2 * y] + sums[t][c], v = acc[m][0][2 * y + 1] + acc[m][1][2 * y + 1] + sums[t][c + 1];
+                    if (lo + t < hi && c0 + c < a.vdim) *(unsigned*)((uint16_t*)a.out + ((int64_t)(lo + t) * a.H + h) * a.vdim + c0 + c) = a.out_bf16 ? ht_pack_bf16(u, v) : ht_pack_f16(u, v);
+                }
+        }
+    }
+}
+
+// ---- the cached rows as keys and values ----------------------------------------------------------------------------------------------------------
+struct LrShared {
+    unsigned long long full[LR_SLOTS];
+    int fail;
+    unsigned wild;                            // rows whose sums are not finite
+    float top[LR_GROUPS][LR_ROWS], sum[LR_GROUPS][LR_ROWS];      // of a segment: largest score and sum of weights of each group
+    float factor[LR_ROWS];                    // of a row's scores
+    float alpha[LR_GROUPS][LR_ROWS];
+    __align__(16) float sums[LR_GROUPS][4][LR_ROWS][40];      // of a step: scores by column groups.  At a segment's end, sums on their way from group to group
+    __align__(16) __half p[LR_GROUPS][LR_ROWS][40];
+};
+static_assert(sizeof(float) * LR_GROUPS * 4 * LR_ROWS * 40 >= LR_THREADS / LR_GROUPS * 16 * sizeof(float) && sizeof(float) * LR_GROUPS * 4 * LR_ROWS * 40 >= LR_ROWS * (LT_RANK + LT_REST + 8) * 2, "half of a group's sums, and the queries, pass here");
+__device__ __forceinline__ void lr_sync(int group) { asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(LR_THREADS / LR_GROUPS) : "memory"); }
+__device__ __forceinline__ bool lr_sync_or(int group, bool x) {
+    unsigned r;
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbar.red.or.pred q, %2, %3, p;\nselp.u32 %0, 1, 0, q;\n}\n" : "=r"(r) : "r"((unsigned)x), "r"(1 + group), "n"(LR_THREADS / LR_GROUPS) : "memory");
+    return r;
+}
+__device__ __forceinline__ void lr_zero(unsigned at) { asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory"); }
 // Values that are not finite, times the weight 0 of a row that does not see them, make a NaN.  Rows whose sums hold one though their scores do not are added up again, one by one, over
 // the keys that they see: a dot product over the block, which then adds a column a thread.
 __device__ __noinline__ void lr_again(const LrArgs& a, LrShared& sh, const PgSeq s, int seq, int row0, int lo, int hi, float m, float by, int r, float* lat) {
@@ -256,11 +313,11 @@ __device__ __noinline__ void lr_again(const LrArgs& a, LrShared& sh, const PgSeq
         for (int e = threadIdx.x; e < a.cols; e += LR_THREADS) d = fmaf(q[e], __half2float(row[e]), d);
         d = warp_sum(d);
         if ((threadIdx.x & 31) == 0) sh.sums[0][0][0][threadIdx.x >> 5] = d;
-        lr_sync_all();
+        __syncthreads();
         d = 0.0f;
 #pragma unroll
         for (int w = 0; w < LR_THREADS / 32; w++) d += sh.sums[0][0][0][w];
-        lr_sync_all();
+        __syncthreads();
         const float p = lt_exp2(d * (a.scale * LR_LOG2E) - m + LR_SHIFT);
         if (c < a.rank) o = fmaf(p, __half2float(row[c]), o);
     }
@@ -268,103 +325,100 @@ __device__ __noinline__ void lr_again(const LrArgs& a, LrShared& sh, const PgSeq
 }
 static_assert(LR_THREADS >= LT_RANK, "a thread a column");
 
-__global__ void __launch_bounds__(LR_ALL, 1) latent_rows_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ LrArgs a, const __grid_constant__ LrDeal deal, unsigned* err_dev,
-                                                                unsigned* err_host) {
+__global__ void __launch_bounds__(LR_THREADS, 1) latent_rows_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ LrArgs a, const __grid_constant__ LrDeal deal, unsigned* err_dev,
+                                                                    unsigned* err_host) {
     extern __shared__ __align__(1024) uint8_t lr_raw[];
     __shared__ LrShared sh;
     const int tid = threadIdx.x, lane = tid & 31, group = tid / (LR_THREADS / LR_GROUPS), in_group = tid % (LR_THREADS / LR_GROUPS), warp = in_group >> 5;
-    const unsigned ring = (pg_smem(lr_raw) + 1023) & ~1023u, slot_bytes = (unsigned)((a.cols + 63) >> 6) * LR_BLOCK;
+    const unsigned ring = (pg_smem(lr_raw) + 1023) & ~1023u, n_blocks = (unsigned)((a.cols + 63) >> 6), slot_bytes = n_blocks * LR_BLOCK;
     if (tid == 0) {
-        for (int i = 0; i < a.slots; i++) { pg_mbar_init(pg_smem(&sh.full[i]), 1); pg_mbar_init(pg_smem(&sh.empty[i]), 8); }
+        for (int i = 0; i < a.slots; i++) pg_mbar_init(pg_smem(&sh.full[i]), 1);
         sh.fail = 0; sh.wild = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_rows) : "memory");
     }
     pdl_enter();
     __syncthreads();
     LrWalk walk = {deal.at[blockIdx.x].seq, deal.at[blockIdx.x].tile, deal.at[blockIdx.x].off, deal.run_lo + ((int)blockIdx.x < deal.run_more ? 1 : 0)};
-    if (tid >= LR_THREADS) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(LR_REGS_REST));
-        if (tid < LR_THREADS + 32) {
-            // ===== copies: a box of 64 columns for each page of a step =====
-            int n = 0;
-            bool ok = true;
-            const int rows = min(a.page, LR_KEYS), boxes = LR_KEYS / rows;      // of a page at a time; pages of a step
-            while (ok && walk.piece(a, [&](const PgSeq& s, int seq, int, int k0, int k1, bool) {
-                int from, to;
-                lr_range(s, a, &from, &to);
-                const int* table = a.table + (int64_t)seq * a.table_cols;
-                auto look_up = [&](int k) {
-                    const int key = from + k * LR_KEYS + lane * rows;
-                    return lane < boxes && key < to ? table[key >> a.shift] : 0;
-                };
-                int next = k0 < k1 ? look_up(k0) : 0;
-                for (int k = k0; k < k1 && ok; k++, n++) {
-                    const int key0 = from + k * LR_KEYS, there = (min(LR_KEYS, to - key0) + rows - 1) / rows, mine = next, slot = n % a.slots;
-                    if (k + 1 < k1) next = look_up(k + 1);
-                    if (!(ok = sg_wait_warp(pg_smem(&sh.empty[slot]), ((unsigned)(n / a.slots) & 1u) ^ 1u, &sh.fail))) break;
-                    const unsigned bar = pg_smem(&sh.full[slot]), at = ring + slot * slot_bytes;
-                    if (pg_elect()) pg_mbar_expect_tx(bar, (unsigned)there * rows * (slot_bytes / LR_KEYS));
-                    __syncwarp();
-                    for (int i = 0; i < there; i++) {
-                        const int page = __shfl_sync(0xffffffffu, mine, i), y = (key0 + i * rows) & (a.page - 1);
-                        if (pg_elect())
-                            for (int b = 0; b * 64 < a.cols; b++)
-                                asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-                                             ::"r"(at + b * LR_BLOCK + i * rows * 128), "l"(&map_rows), "r"(bar), "r"(b * 64), "r"(y), "r"(page) : "memory");
-                        __syncwarp();
-                    }
-                }
-            })) {}
-            int never = 0;                                            // no copy is under way when the CTA ends
-            for (int i = max(0, n - a.slots); i < n; i++) sg_wait_warp(pg_smem(&sh.full[i % a.slots]), (unsigned)(i / a.slots) & 1u, &never);
-            if (!ok) for (int i = 0; i < 1000; i++) __nanosleep(1000);
+    // A step's rows come as boxes of 64 columns of a page, each asked for by a warp of its own (all by one, 1100 cycles a step; row by row, a lane a row, 2500)
+    const int box_rows = min(a.page, LR_KEYS);
+    auto ask = [&](int slot, const int4& p, unsigned first_block, unsigned by) {
+        const unsigned bar = pg_smem(&sh.full[slot]), at = ring + slot * slot_bytes;
+        if (first_block == 0) {
+            if (pg_elect()) pg_mbar_expect_tx(bar, (unsigned)(p.w * box_rows) * (slot_bytes / LR_KEYS));
+            __syncwarp();
         }
-        return;
+        for (unsigned b = first_block; b < n_blocks; b += by)
+            for (int i = 0; i < p.w; i++)
+                if (pg_elect())
+                    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                                 ::"r"(at + b * LR_BLOCK + i * box_rows * 128), "l"(&map_rows), "r"(bar), "r"(b * 64), "r"(p.z), "r"(i ? p.y : p.x) : "memory");
+        __syncwarp();
+    };
+    const int room = deal.run_lo + 1;
+    const int4* list = a.steps + (int64_t)blockIdx.x * room;
+    auto what = [&](int i) { return i < room ? list[i] : make_int4(0, 0, 0, 0); };
+    int coming = a.slots + group;                                     // group 0 asks for the steps slots, slots + 2, .., group 1 for those between
+    int4 next = what(coming);
+    for (int i = 0; i < a.slots; i++) {                               // the first slots: all 16 warps
+        const int4 p = what(i);
+        if (p.w && (unsigned)(tid >> 5) < n_blocks) ask(i, p, (unsigned)(tid >> 5), LR_THREADS / 32);
     }
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(LR_REGS));
     const int kg = warp & 3, kh = warp >> 2, blocks = a.cols >> 4, v_blocks = a.rank >> 4;
     const int row = in_group >> 4, part = in_group & 15;              // of the weights: 16 threads a row, two keys each
     // a slot: blocks of 64 columns, 32 rows of 128 bytes under the 128-byte swizzle.  This lane's row of four 8 x 8 blocks: scores take columns 16 (kg + 4 i), block i; values 16 (warp + 8 i), block warp / 4 + 2 i
     const unsigned k_lane = (unsigned)(kh * 16 + (lane >> 4) * 8 + (lane & 7)) * 128 + (((kg * 2 + (lane >> 3 & 1)) ^ (lane & 7)) << 4);
     const unsigned v_lane = (unsigned)(warp >> 2) * LR_BLOCK + (unsigned)((lane >> 3 & 1) * 8 + (lane & 7)) * 128 + ((((warp & 3) * 2 + (lane >> 4)) ^ (lane & 7)) << 4);
     const unsigned p_at = pg_smem(&sh.p[group][0][0]) + (unsigned)((lane >> 3 & 1) * 8 + (lane & 7)) * 80 + (lane >> 4) * 16;
-    int n = 0;                                                        // steps of the run so far
+    int n = 0, last = -1;                                             // steps of the run so far; this group's last one whose slot is free and not asked for
     bool ok = true, first = true;
+    auto again = [&]() {                                              // (all warps of the group are through with step `last`)
+        if (last < 0) return;
+        if (next.w && ok) ask(last % a.slots, next, (unsigned)warp, LR_THREADS / LR_GROUPS / 32);
+        coming += LR_GROUPS;
+        next = what(coming);
+        last = -1;
+    };
     while (walk.piece(a, [&](const PgSeq& s, int seq, int tile, int k0, int k1, bool cut) {
         int from, to;
         lr_range(s, a, &from, &to);
         const int row0 = tile * LR_ROWS, n_rows = min(LR_ROWS, s.count * a.H - row0);
         const float* qs = a.qf + ((int64_t)s.first * a.H + row0) * a.cols;
-        // factors of the rows: near 2^4 by a power of two.  A warp a row
+        // the rows near 2^4 by a power of two, as f16, by way of shared memory.  A warp a row
         if (tid == 0) sh.wild = 0;
+        __half* staged = (__half*)&sh.sums[0][0][0][0];
+        const int staged_pitch = a.cols + 8;                          // an odd number of 16 bytes: ldmatrix without conflicts
         {
             const int r = tid >> 5;
             unsigned top = 0;                                        // as bits, so that NaN is the largest of all
-            if (r < n_rows)
-                for (int e = lane * 4; e < a.cols; e += 128) {
-                    const uint4 v = *(const uint4*)(qs + (int64_t)r * a.cols + e);
-                    top = max(max(top, max(v.x & 0x7fffffffu, v.y & 0x7fffffffu)), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
-                }
+            uint4 v[LR_RUNS];
+#pragma unroll
+            for (int i = 0; i < LR_RUNS; i++) {
+                const int e = (i * 32 + lane) * 4;
+                v[i] = r < n_rows && e < a.cols ? *(const uint4*)(qs + (int64_t)r * a.cols + e) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < LR_RUNS; i++) top = max(max(top, max(v[i].x & 0x7fffffffu, v[i].y & 0x7fffffffu)), max(v[i].z & 0x7fffffffu, v[i].w & 0x7fffffffu));
             top = __reduce_max_sync(0xffffffffu, top);
             const int ex = top < 0x00800000u || top >= 0x7f800000u ? 4 : max((int)(top >> 23) - 126, -100);
-            if (lane == 0) {
-                sh.up[r] = __uint_as_float((unsigned)(4 - ex + 127) << 23);
-                sh.factor[r] = top >= 0x7f800000u ? NAN : __uint_as_float((unsigned)(ex - 4 + 127) << 23);
+            const float up = __uint_as_float((unsigned)(4 - ex + 127) << 23);
+            if (lane == 0) sh.factor[r] = top >= 0x7f800000u ? NAN : __uint_as_float((unsigned)(ex - 4 + 127) << 23);
+#pragma unroll
+            for (int i = 0; i < LR_RUNS; i++) {
+                const int e = (i * 32 + lane) * 4;
+                if (e < a.cols)
+                    *(uint2*)(staged + r * staged_pitch + e) = make_uint2(lt_pack(__uint_as_float(v[i].x) * up, __uint_as_float(v[i].y) * up), lt_pack(__uint_as_float(v[i].z) * up, __uint_as_float(v[i].w) * up));
             }
         }
-        lr_sync_all();
+        __syncthreads();
+        again();
         unsigned q[LR_KB][4];
 #pragma unroll
         for (int i = 0; i < LR_KB; i++) {
-            const int b = kg + 4 * i;
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const int r = (lane >> 2) + (x & 1) * 8;
-                float2 v = make_float2(0.0f, 0.0f);
-                if (b < blocks && r < n_rows) v = *(const float2*)(qs + (int64_t)r * a.cols + b * 16 + (x >> 1) * 8 + (lane & 3) * 2);
-                q[i][x] = lt_pack(v.x * sh.up[r], v.y * sh.up[r]);
-            }
+            if (kg + 4 * i < blocks) lt_ldsm(q[i], pg_smem(staged + ((lane & 7) + (lane >> 3 & 1) * 8) * staged_pitch + (kg + 4 * i) * 16 + (lane >> 4) * 8));
+            else q[i][0] = q[i][1] = q[i][2] = q[i][3] = 0u;
         }
+        __syncthreads();                                              // the staged rows are read: sums go there
         const float f = sh.factor[row] * (a.scale * LR_LOG2E);
         const int pos = row < n_rows ? s.pos0 + (row0 + row) / a.H : -1, key_lo = a.window > 0 ? pos - a.window + 1 : 0;
         float m = -INFINITY, l = 0.0f;
@@ -383,15 +437,13 @@ __global__ void __launch_bounds__(LR_ALL, 1) latent_rows_kernel(const __grid_con
 #pragma unroll
             for (int i = 0; i < 8; i++) x[i >> 2][i & 3] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < LR_KB; i++) {
-                const int b = kg + 4 * i;
-                if (b < blocks) {
+            for (int i = 0; i < LR_KB; i++)
+                if (kg + 4 * i < blocks) {
                     unsigned kb[4];
                     lt_ldsm(kb, at + k_lane + i * LR_BLOCK);
                     lt_mma(x[0], q[i], kb[0], kb[1]);
                     lt_mma(x[1], q[i], kb[2], kb[3]);
                 }
-            }
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -403,6 +455,7 @@ __global__ void __launch_bounds__(LR_ALL, 1) latent_rows_kernel(const __grid_con
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // before the slot's next rows
             }
             lr_sync(group);
+            again();
             float z[2];
             {
                 const float2 u0 = *(const float2*)&sh.sums[group][0][row][part * 2], u1 = *(const float2*)&sh.sums[group][1][row][part * 2], u2 = *(const float2*)&sh.sums[group][2][row][part * 2],
@@ -432,17 +485,15 @@ __global__ void __launch_bounds__(LR_ALL, 1) latent_rows_kernel(const __grid_con
                 unsigned p[4];
                 lt_ldsm(p, p_at + kk * 32);
 #pragma unroll
-                for (int i = 0; i < LR_VB; i++) {
-                    const int b = warp + 8 * i;
-                    if (b < v_blocks) {
+                for (int i = 0; i < LR_VB; i++)
+                    if (warp + 8 * i < v_blocks) {
                         unsigned v[4];
                         lt_ldsm_t(v, at + v_lane + kk * 2048 + i * 2 * LR_BLOCK);
                         lt_mma(o[i][0], p, v[0], v[1]);
                         lt_mma(o[i][1], p, v[2], v[3]);
                     }
-                }
             }
-            sg_arrive(pg_smem(&sh.empty[slot]));
+            last = here;
         }
         n += k1 - k0;
         // both groups' sums: group 1 gives the first half of its columns' blocks, group 0 the second.  A cut segment leaves its sums, the others their result
@@ -459,7 +510,8 @@ __global__ void __launch_bounds__(LR_ALL, 1) latent_rows_kernel(const __grid_con
                     box[(i * 2 + y) * (LR_THREADS / LR_GROUPS)] = make_float4(v[0], v[1], v[2], v[3]);
                 }
         };
-        lr_sync_all();                                                // scores and weights are read
+        __syncthreads();                                              // scores and weights are read
+        again();
         if (group == 1) give(0);
         const int place = 2 * blockIdx.x + (first ? 0 : 1);
         const bool any = k1 > k0 || !cut;
@@ -509,14 +561,14 @@ __global__ void __launch_bounds__(LR_ALL, 1) latent_rows_kernel(const __grid_con
                 }
             }
         };
-        lr_sync_all();
+        __syncthreads();
         if (group == 0) finish(0);
-        lr_sync_all();
+        __syncthreads();
         if (group == 0) give(1);
-        lr_sync_all();
+        __syncthreads();
         if (group == 1) finish(1);
         if (wild) atomicOr(&sh.wild, wild);
-        if (lr_sync_all_or(wild != 0)) {
+        if (__syncthreads_or(wild != 0)) {
             for (unsigned left = sh.wild; left; left &= left - 1) {
                 const int r = __ffs(left) - 1;
                 const float m0 = sh.top[0][r], m1 = sh.top[1][r];
@@ -530,52 +582,61 @@ __global__ void __launch_bounds__(LR_ALL, 1) latent_rows_kernel(const __grid_con
                 }
                 lr_again(a, sh, s, seq, row0, from + k0 * LR_KEYS, min(to, from + k1 * LR_KEYS), mm, cut ? 1.0f : g / total, r, lat + (int64_t)r * a.rank);
             }
-            lr_sync_all();
+            __syncthreads();
         }
         first = false;
     })) {}
+    // no copy is under way when the CTA ends: all steps of the run have been waited for, but where a wait ran out
+    if (*(volatile int*)&sh.fail)
+        for (int i = 0; i < 1000; i++) __nanosleep(1000);
     if (tid == 0 && *(volatile int*)&sh.fail) {
         if (err_dev) atomicExch(err_dev, 5u);
         if (err_host) { *(volatile unsigned*)err_host = 5u; __threadfence_system(); }
     }
 }
-// segments in several runs: grid (segments, rows, 128 columns); a warp takes every eighth slice.  (One thread a column, one slice after another: 43 us for the 148 slices of a long cache)
-#define LJ_WARPS 8
-__global__ void __launch_bounds__(LJ_WARPS * 32) latent_join_kernel(const LrArgs a, const __grid_constant__ LrCuts cuts) {
-    __shared__ float factor[LR_CTAS], red[2][LJ_WARPS];
-    __shared__ float4 sums[LJ_WARPS][32];
+// segments in several runs: grid (segments, rows, COLS columns); a thread 4 columns of every SLICES-th slice.  Many slices, few segments: 64 columns a CTA, 16 slices at a time (one thread a column,
+// one slice after another: 43 us for the 148 slices of a long cache, so 4); many segments of a few slices: all columns (9 us for 54 of them in 128 columns a CTA)
+#define LJ_THREADS 256
+template <int COLS>
+__global__ void __launch_bounds__(LJ_THREADS) latent_join_kernel(const __grid_constant__ LrArgs a, const __grid_constant__ LrCuts cuts) {
+    constexpr int SLICES = LJ_THREADS / (COLS / 4), TURNS = COLS == 64 ? (LR_CTAS + SLICES - 1) / SLICES : LJ_FEW / SLICES;
+    __shared__ float factor[LR_CTAS], red[2][LJ_THREADS / 32];
+    __shared__ float4 sums[SLICES][COLS / 4];
     pdl_enter();
     const auto cut = cuts.at[blockIdx.x];
     const PgSeq s = a.seqs[cut.seq];
-    const int y = blockIdx.y, row = cut.tile * LR_ROWS + y, lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.z * 128 + lane * 4;
+    const int x = threadIdx.x, y = blockIdx.y, row = cut.tile * LR_ROWS + y, lane = x & 31, w = x >> 5, c = blockIdx.z * COLS + x % (COLS / 4) * 4, which = x / (COLS / 4);
     if (row >= s.count * a.H) return;
-    auto place = [&](int x) { return (size_t)(x == 0 ? cut.slot : 2 * (cut.cta + x - 1)) * LR_ROWS + y; };
-    static_assert(LR_CTAS <= LJ_WARPS * 32, "a thread a slice");
-    const int x = threadIdx.x;
+    auto place = [&](int i) { return (size_t)(i == 0 ? cut.slot : 2 * (cut.cta + i - 1)) * LR_ROWS + y; };
+    static_assert(LR_CTAS <= LJ_THREADS, "a thread a slice");
     const float2 z = x < cut.n ? a.ml[place(x)] : make_float2(-INFINITY, 0.0f);
+    float4 v[TURNS];
+#pragma unroll
+    for (int i = 0; i < TURNS; i++) {
+        const int at = i * SLICES + which;
+        v[i] = at < cut.n && c < a.rank ? *(const float4*)(a.part + place(at) * a.rank + c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
     float m = warp_max(z.x);
     if (lane == 0) red[0][w] = m;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < LJ_WARPS; i++) m = fmaxf(m, red[0][i]);
+    for (int i = 0; i < LJ_THREADS / 32; i++) m = fmaxf(m, red[0][i]);
     const float f = z.x == -INFINITY ? (z.y == 0.0f ? 0.0f : 1.0f) : exp2f(z.x - m);
-    if (x < cut.n) factor[x] = f;
+    if (x < LR_CTAS) factor[x] = f;
     float l = warp_sum(f * z.y);
     if (lane == 0) red[1][w] = l;
     __syncthreads();
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (c < a.rank) {
-#pragma unroll 4
-        for (int i = w; i < cut.n; i += LJ_WARPS) {
-            const float by = factor[i];
-            const float4 v = *(const float4*)(a.part + place(i) * a.rank + c);
-            if (by != 0.0f) { o.x = fmaf(by, v.x, o.x); o.y = fmaf(by, v.y, o.y); o.z = fmaf(by, v.z, o.z); o.w = fmaf(by, v.w, o.w); }
-        }
+#pragma unroll
+    for (int i = 0; i < TURNS; i++) {
+        const int at = i * SLICES + which;
+        const float by = at < LR_CTAS ? factor[at] : 0.0f;
+        if (by != 0.0f) { o.x = fmaf(by, v[i].x, o.x); o.y = fmaf(by, v[i].y, o.y); o.z = fmaf(by, v[i].z, o.z); o.w = fmaf(by, v[i].w, o.w); }
     }
-    sums[w][lane] = o;
+    sums[which][x % (COLS / 4)] = o;
     l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < LJ_WARPS; i++) l += red[1][i];
+    for (int i = 0; i < LJ_THREADS / 32; i++) l += red[1][i];
     __syncthreads();
     float g = 1.0f;
     if (a.sink) {
@@ -583,12 +644,11 @@ __global__ void __launch_bounds__(LJ_WARPS * 32) latent_join_kernel(const LrArgs
         g = m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : exp2f(m - m2);
         l = g * l + (sk == -INFINITY ? 0.0f : exp2f(sk - m2 + LR_SHIFT));
     }
-    const int col = blockIdx.z * 128 + threadIdx.x;
-    if (threadIdx.x < 128 && col < a.rank) {
+    for (int col = x; col < COLS && blockIdx.z * COLS + col < a.rank; col += LJ_THREADS) {
         float t = 0.0f;
 #pragma unroll
-        for (int i = 0; i < LJ_WARPS; i++) t += ((const float*)sums[i])[threadIdx.x];
-        a.lat[((int64_t)s.first * a.H + row) * a.rank + col] = t * (g / l);
+        for (int i = 0; i < SLICES; i++) t += ((const float*)sums[i])[col];
+        a.lat[((int64_t)s.first * a.H + row) * a.rank + blockIdx.z * COLS + col] = t * (g / l);
     }
 }
 
@@ -625,25 +685,33 @@ static int lr_run(cc_device* dev, const cc_page_plan* plan, LrArgs a, const LtRu
     CC_REQUIRE(dev, steps < ((int64_t)1 << 31) * 64, "paged_latent_attention: too many rows");
     deal.ctas = (int)std::min<int64_t>(std::min(LR_CTAS, dev->sm_count), (steps + LR_BEGIN + 1) / (LR_BEGIN + 2));
     const int n_cuts = lr_deal(plan, a, steps, deal, cuts);
-    const size_t qf = (size_t)plan->tokens * a.H * a.cols * 4, lat = (size_t)plan->tokens * a.H * a.rank * 4, part = n_cuts ? (size_t)2 * deal.ctas * LR_ROWS * a.rank * 4 : 0;
+    const size_t qf = (size_t)plan->tokens * a.H * a.cols * 4, lat = (size_t)plan->tokens * a.H * a.rank * 4, part = n_cuts ? (size_t)2 * deal.ctas * LR_ROWS * a.rank * 4 : 0,
+                 ml = (size_t)2 * deal.ctas * LR_ROWS * sizeof(float2), list = (size_t)deal.ctas * (deal.run_lo + 1) * sizeof(int4);
     void* ws = nullptr; size_t cls = 0;
-    int rc = cc_pool_alloc(dev, qf + lat + part + (size_t)2 * deal.ctas * LR_ROWS * sizeof(float2), &ws, &cls);
+    int rc = cc_pool_alloc(dev, qf + lat + part + ml + list, &ws, &cls);
     if (rc) return rc;
     a.qf = (float*)ws; a.lat = (float*)((uint8_t*)ws + qf); a.part = (float*)((uint8_t*)ws + qf + lat); a.ml = (float2*)((uint8_t*)ws + qf + lat + part);
+    a.steps = (int4*)((uint8_t*)ws + qf + lat + part + ml);
     const int slot = (a.cols + 63) / 64 * LR_BLOCK;
     a.slots = std::min(LR_SLOTS, (LR_SMEM - (int)sizeof(LrShared) - 1024) / slot);
     CUtensorMap map;
     rc = cc_make_tmap_pages(dev, &map, a.rows, plan->n_pages, plan->page, a.cols, std::min(plan->page, LR_KEYS));
     if (rc) { cc_pool_free(dev, ws, cls); return rc; }
     const unsigned z = (unsigned)std::min(runs.tiles, 64);
-    const size_t fold = (size_t)a.dim * (LF_COLS + 8) * 2 + 16 * (a.dim + 8) * 2, unfold = (size_t)(LU_COLS + 32) * (a.rank + 8) * 2;
-    cudaError_t e = cudaFuncSetAttribute(latent_fold_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LT_DIM * (LF_COLS + 8) * 2 + 16 * (LT_DIM + 8) * 2);
+    const size_t fold = (size_t)a.dim * (LF_COLS + 8) * 2 + LT_TOKENS * (a.dim + 8) * 2;
+    cudaError_t e = cudaFuncSetAttribute(latent_fold_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LT_DIM * (LF_COLS + 8) * 2 + LT_TOKENS * (LT_DIM + 8) * 2);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(latent_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LR_SMEM - (int)sizeof(LrShared));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(latent_unfold_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (LU_COLS + 32) * (LT_RANK + 8) * 2);
-    if (e == cudaSuccess) e = cc_launch_pdl(dev, latent_fold_kernel, dim3((unsigned)a.H, (unsigned)((a.rank + LF_COLS - 1) / LF_COLS + (a.rest ? 1 : 0)), z), 128, fold, a, runs);
-    if (e == cudaSuccess) e = cc_launch_pdl(dev, latent_rows_kernel, (unsigned)deal.ctas, LR_ALL, (size_t)a.slots * slot + 1024, map, a, deal, dev->err_dev, dev->err_host);
-    if (e == cudaSuccess && n_cuts) { e = cc_launch_pdl(dev, latent_join_kernel, dim3((unsigned)n_cuts, LR_ROWS, (unsigned)(a.rank + 127) / 128), LJ_WARPS * 32, 0, a, cuts); dev->launches++; }
-    if (e == cudaSuccess) e = cc_launch_pdl(dev, latent_unfold_kernel, dim3((unsigned)a.H, (unsigned)((a.vdim + LU_COLS - 1) / LU_COLS), z), 128, unfold, a, runs);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(latent_unfold_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, lu_smem(LT_RANK));
+    if (e == cudaSuccess) e = cc_launch_pdl(dev, latent_fold_kernel, dim3((unsigned)a.H, (unsigned)((a.rank + LF_COLS - 1) / LF_COLS + 1 + (deal.ctas + 4 * a.H - 1) / (4 * a.H)), z), 128, fold, a, runs, deal);
+    if (e == cudaSuccess) e = cc_launch_pdl(dev, latent_rows_kernel, (unsigned)deal.ctas, LR_THREADS, (size_t)a.slots * slot + 1024, map, a, deal, dev->err_dev, dev->err_host);
+    if (e == cudaSuccess && n_cuts) {
+        int most = 0;
+        for (int i = 0; i < n_cuts; i++) most = std::max(most, cuts.at[i].n);
+        e = most <= LJ_FEW ? cc_launch_pdl(dev, latent_join_kernel<LT_RANK>, dim3((unsigned)n_cuts, LR_ROWS, 1), LJ_THREADS, 0, a, cuts)
+                           : cc_launch_pdl(dev, latent_join_kernel<64>, dim3((unsigned)n_cuts, LR_ROWS, (unsigned)(a.rank + 63) / 64), LJ_THREADS, 0, a, cuts);
+        dev->launches++;
+    }
+    if (e == cudaSuccess) e = cc_launch_pdl(dev, latent_unfold_kernel, dim3((unsigned)a.H, (unsigned)((a.vdim + LU_COLS - 1) / LU_COLS), z), LU_THREADS, lu_smem(a.rank), a, runs);
     dev->launches += 3;
     cc_pool_free(dev, ws, cls);
     if (e != cudaSuccess) return cc_fail(dev, CC_ERR_CUDA, "paged_latent_attention: %s", cudaGetErrorString(e));
@@ -699,7 +767,7 @@ extern "C" CC_API int cc_paged_latent_attention(cc_device* dev, const cc_page_pl
             if (runs.n == LT_RUNS) { runs.hi[runs.n - 1] = s.first + s.count; continue; }      // many runs: the last one takes all that lies behind (other tokens' results are overwritten)
             runs.lo[runs.n] = s.first; runs.hi[runs.n++] = s.first + s.count;
         }
-        for (int i = 0; i < runs.n; i++) { runs.tile0[i] = runs.tiles; runs.tiles += (runs.hi[i] - runs.lo[i] + 15) / 16; }
+        for (int i = 0; i < runs.n; i++) { runs.tile0[i] = runs.tiles; runs.tiles += (runs.hi[i] - runs.lo[i] + LT_TOKENS - 1) / LT_TOKENS; }
         rc = lr_run(dev, plan, a, runs);
         if (!rc && a.most < 0x7fffffff) rc = tl_run(dev, plan, a);      // behind the others: their last products may run over tokens of these
     }
