@@ -255,7 +255,7 @@ int cc_launch_prefill_operand(cc_device* dev, const cc_buf* w, float* out, int64
 // tensor map (CUtensorMap) of a bfloat16 matrix [rows][k], box 64 columns x box_rows rows, 128-byte swizzle
 int cc_make_tmap_bf16(cc_device* dev, void* tm, const void* base, int64_t rows, int64_t k, int box_rows);
 int cc_make_tmap_rows(cc_device* dev, void* tm, const void* base, int64_t rows, int64_t cols, int64_t stride_bytes, int box_rows, bool bf16);      // .. of 16-bit numbers, rows stride_bytes apart
-int cc_make_tmap_pages(cc_device* dev, void* tm, const void* base, int64_t n_pages, int page, int cols, int box_rows);      // .. of pages of 16-bit rows
+int cc_make_tmap_pages(cc_device* dev, void* tm, const void* base, int64_t n_pages, int page, int cols, int box_rows, int blocks);      // .. of pages of 16-bit rows
 int cc_make_tmap_i8(cc_device* dev, void* tm, const void* base, int64_t rows, int64_t k, int box_rows);      // .. of 8-bit numbers, 128 columns; k a multiple of 16
 
 // ---- dense.cu: plain F32 / BF16 weight matrices with a batch of activation rows -------------------

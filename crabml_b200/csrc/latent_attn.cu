@@ -325,7 +325,7 @@ __device__ __noinline__ void lr_again(const LrArgs& a, LrShared& sh, const PgSeq
 }
 static_assert(LR_THREADS >= LT_RANK, "a thread a column");
 
-__global__ void __launch_bounds__(LR_THREADS, 1) latent_rows_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ LrArgs a, const __grid_constant__ LrDeal deal, unsigned* err_dev,
+__global__ void __launch_bounds__(LR_THREADS, 1) latent_rows_kernel(const __grid_constant__ CUtensorMap map_whole, const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ LrArgs a, const __grid_constant__ LrDeal deal, unsigned* err_dev,
                                                                     unsigned* err_host) {
     extern __shared__ __align__(1024) uint8_t lr_raw[];
     __shared__ LrShared sh;
@@ -335,24 +335,30 @@ __global__ void __launch_bounds__(LR_THREADS, 1) latent_rows_kernel(const __grid
         for (int i = 0; i < a.slots; i++) pg_mbar_init(pg_smem(&sh.full[i]), 1);
         sh.fail = 0; sh.wild = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_rows) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_whole) : "memory");
     }
     pdl_enter();
     __syncthreads();
     LrWalk walk = {deal.at[blockIdx.x].seq, deal.at[blockIdx.x].tile, deal.at[blockIdx.x].off, deal.run_lo + ((int)blockIdx.x < deal.run_more ? 1 : 0)};
-    // A step's rows come as boxes of 64 columns of a page, each asked for by a warp of its own (all by one, 1100 cycles a step; row by row, a lane a row, 2500)
-    const int box_rows = min(a.page, LR_KEYS);
-    auto ask = [&](int slot, const int4& p, unsigned first_block, unsigned by) {
+    // a step's rows: one copy for all whole blocks of 64 columns of a page, and one for the columns behind them.  (A copy for each block, by all 8 warps, took the group 1000 cycles of a step; row by row,
+    // a lane a row, 2500)
+    const int box_rows = min(a.page, LR_KEYS), whole = a.cols >> 6;
+    auto ask = [&](int slot, const int4& p) {
         const unsigned bar = pg_smem(&sh.full[slot]), at = ring + slot * slot_bytes;
-        if (first_block == 0) {
-            if (pg_elect()) pg_mbar_expect_tx(bar, (unsigned)(p.w * box_rows) * (slot_bytes / LR_KEYS));
-            __syncwarp();
-        }
-        for (unsigned b = first_block; b < n_blocks; b += by)
-            for (int i = 0; i < p.w; i++)
-                if (pg_elect())
+        if (pg_elect()) {
+            pg_mbar_expect_tx(bar, (unsigned)(p.w * box_rows) * (slot_bytes / LR_KEYS));
+            for (int i = 0; i < p.w; i++) {
+                const int page = i ? p.y : p.x;
+                const unsigned to = at + i * box_rows * 128;
+                // (a box's blocks lie one behind the other: those of a page of 16 rows go to half a block each, so they come one by one)
+                if (box_rows == LR_KEYS && whole)
+                    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+                                 ::"r"(to), "l"(&map_whole), "r"(bar), "r"(0), "r"(p.z), "r"(0), "r"(page) : "memory");
+                for (unsigned b = box_rows == LR_KEYS ? (unsigned)whole : 0u; b < n_blocks; b++)
                     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-                                 ::"r"(at + b * LR_BLOCK + i * box_rows * 128), "l"(&map_rows), "r"(bar), "r"(b * 64), "r"(p.z), "r"(i ? p.y : p.x) : "memory");
+                                 ::"r"(to + b * LR_BLOCK), "l"(&map_rows), "r"(bar), "r"(b * 64), "r"(p.z), "r"(page) : "memory");
+            }
+        }
         __syncwarp();
     };
     const int room = deal.run_lo + 1;
@@ -360,9 +366,9 @@ __global__ void __launch_bounds__(LR_THREADS, 1) latent_rows_kernel(const __grid
     auto what = [&](int i) { return i < room ? list[i] : make_int4(0, 0, 0, 0); };
     int coming = a.slots + group;                                     // group 0 asks for the steps slots, slots + 2, .., group 1 for those between
     int4 next = what(coming);
-    for (int i = 0; i < a.slots; i++) {                               // the first slots: all 16 warps
-        const int4 p = what(i);
-        if (p.w && (unsigned)(tid >> 5) < n_blocks) ask(i, p, (unsigned)(tid >> 5), LR_THREADS / 32);
+    if (tid < 32 * a.slots) {                                         // the first slots, a warp each
+        const int4 p = what(tid >> 5);
+        if (p.w) ask(tid >> 5, p);
     }
     const int kg = warp & 3, kh = warp >> 2, blocks = a.cols >> 4, v_blocks = a.rank >> 4;
     const int row = in_group >> 4, part = in_group & 15;              // of the weights: 16 threads a row, two keys each
@@ -374,9 +380,11 @@ __global__ void __launch_bounds__(LR_THREADS, 1) latent_rows_kernel(const __grid
     bool ok = true, first = true;
     auto again = [&]() {                                              // (all warps of the group are through with step `last`)
         if (last < 0) return;
-        if (next.w && ok) ask(last % a.slots, next, (unsigned)warp, LR_THREADS / LR_GROUPS / 32);
-        coming += LR_GROUPS;
-        next = what(coming);
+        if (warp == 0) {
+            if (next.w && ok) ask(last % a.slots, next);
+            coming += LR_GROUPS;
+            next = what(coming);
+        }
         last = -1;
     };
     while (walk.piece(a, [&](const PgSeq& s, int seq, int tile, int k0, int k1, bool cut) {
@@ -694,8 +702,10 @@ static int lr_run(cc_device* dev, const cc_page_plan* plan, LrArgs a, const LtRu
     a.steps = (int4*)((uint8_t*)ws + qf + lat + part + ml);
     const int slot = (a.cols + 63) / 64 * LR_BLOCK;
     a.slots = std::min(LR_SLOTS, (LR_SMEM - (int)sizeof(LrShared) - 1024) / slot);
-    CUtensorMap map;
-    rc = cc_make_tmap_pages(dev, &map, a.rows, plan->n_pages, plan->page, a.cols, std::min(plan->page, LR_KEYS));
+    CUtensorMap map, whole;
+    rc = cc_make_tmap_pages(dev, &map, a.rows, plan->n_pages, plan->page, a.cols, std::min(plan->page, LR_KEYS), 0);
+    if (!rc && a.cols >= 64) rc = cc_make_tmap_pages(dev, &whole, a.rows, plan->n_pages, plan->page, a.cols, std::min(plan->page, LR_KEYS), a.cols / 64);
+    else whole = map;
     if (rc) { cc_pool_free(dev, ws, cls); return rc; }
     const unsigned z = (unsigned)std::min(runs.tiles, 64);
     const size_t fold = (size_t)a.dim * (LF_COLS + 8) * 2 + LT_TOKENS * (a.dim + 8) * 2;
@@ -703,7 +713,7 @@ static int lr_run(cc_device* dev, const cc_page_plan* plan, LrArgs a, const LtRu
     if (e == cudaSuccess) e = cudaFuncSetAttribute(latent_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LR_SMEM - (int)sizeof(LrShared));
     if (e == cudaSuccess) e = cudaFuncSetAttribute(latent_unfold_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, lu_smem(LT_RANK));
     if (e == cudaSuccess) e = cc_launch_pdl(dev, latent_fold_kernel, dim3((unsigned)a.H, (unsigned)((a.rank + LF_COLS - 1) / LF_COLS + 1 + (deal.ctas + 4 * a.H - 1) / (4 * a.H)), z), 128, fold, a, runs, deal);
-    if (e == cudaSuccess) e = cc_launch_pdl(dev, latent_rows_kernel, (unsigned)deal.ctas, LR_THREADS, (size_t)a.slots * slot + 1024, map, a, deal, dev->err_dev, dev->err_host);
+    if (e == cudaSuccess) e = cc_launch_pdl(dev, latent_rows_kernel, (unsigned)deal.ctas, LR_THREADS, (size_t)a.slots * slot + 1024, whole, map, a, deal, dev->err_dev, dev->err_host);
     if (e == cudaSuccess && n_cuts) {
         int most = 0;
         for (int i = 0; i < n_cuts; i++) most = std::max(most, cuts.at[i].n);

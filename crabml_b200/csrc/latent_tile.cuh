@@ -679,7 +679,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
 static int tl_run(cc_device* dev, const cc_page_plan* plan, const LrArgs& all) {
     const int64_t per = (int64_t)((all.dim + 63) / 64 + (all.vdim + 63) / 64) * TL_BLOCK, width = all.dim + all.rest;
     CUtensorMap rows, q, uk, uv;
-    int rc = cc_make_tmap_pages(dev, &rows, all.rows, plan->n_pages, plan->page, all.cols, plan->page);
+    int rc = cc_make_tmap_pages(dev, &rows, all.rows, plan->n_pages, plan->page, all.cols, plan->page, 0);
     if (!rc) rc = cc_make_tmap_rows(dev, &q, all.q, plan->tokens, all.H * width, all.H * width * 2, TL_ROWS, false);
     const int wide = std::max(all.dim, all.vdim);
     if (!rc) rc = cc_make_tmap_rows(dev, &uk, all.uk, (int64_t)all.H * all.dim, all.rank, (int64_t)all.rank * 2, wide, false);

@@ -442,13 +442,15 @@ int cc_make_tmap_rows(cc_device* dev, void* tm, const void* base, int64_t rows, 
                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? CC_OK : cc_fail(dev, CC_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
 }
-// pages [n_pages][page][cols] of 16-bit numbers, box 64 columns x box_rows rows of one page
-int cc_make_tmap_pages(cc_device* dev, void* tm, const void* base, int64_t n_pages, int page, int cols, int box_rows) {
+// Pages [n_pages][page][cols] of 16-bit numbers.  blocks = 0: a box is 64 columns x box_rows rows of one page, coordinates {column, row, page}.  Else it is that many blocks of 64 columns, side by side
+// in a row but one behind the other in the box; coordinates {0, row, block, page}; all of them inside the row
+int cc_make_tmap_pages(cc_device* dev, void* tm, const void* base, int64_t n_pages, int page, int cols, int box_rows, int blocks) {
     PFN_encodeTiled enc = pg_encode();
     if (!enc) return cc_fail(dev, CC_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
-    cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)page, (cuuint64_t)n_pages}, strides[2] = {(cuuint64_t)cols * 2, (cuuint64_t)cols * 2 * page};
-    cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, estr[3] = {1, 1, 1};
-    const CUresult r = enc((CUtensorMap*)tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, (void*)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    const cuuint64_t row = (cuuint64_t)cols * 2, whole = row * page;
+    cuuint64_t dims[4] = {blocks ? 64u : (cuuint64_t)cols, (cuuint64_t)page, blocks ? (cuuint64_t)blocks : (cuuint64_t)n_pages, (cuuint64_t)n_pages}, strides[3] = {row, blocks ? 128u : whole, whole};
+    cuuint32_t box[4] = {64, (cuuint32_t)box_rows, blocks ? (cuuint32_t)blocks : 1u, 1}, estr[4] = {1, 1, 1, 1};
+    const CUresult r = enc((CUtensorMap*)tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, blocks ? 4 : 3, (void*)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? CC_OK : cc_fail(dev, CC_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
 }
