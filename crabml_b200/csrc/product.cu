@@ -42,7 +42,8 @@ __device__ __forceinline__ uint4 pr_pack8(const float (&v)[8]) {
 #define PF_THREADS (PF_WARPS * 32)
 #define PF_AHEAD 4                            // runs of 32 k that a warp has under way: 64 KB an SM
 #define PF_SMEM (200 * 1024)
-#define PF_ROWS 32                            // rows of x; more go to the tensor cores' tiles
+#define PF_ROWS 32                            // rows of x; more go to the tensor cores' tiles,
+#define PF_ROOM (90 * 1024)                   // .. and so do those whose numbers shared memory does not hold
 // 8 numbers of a row from column c on, zeros behind its end
 __device__ __forceinline__ uint4 pf_weights(const uint16_t* row, int c, int k, bool there, bool vec) {
     if (!there || c >= k) return make_uint4(0, 0, 0, 0);
@@ -56,79 +57,36 @@ __device__ __forceinline__ uint4 pf_weights(const uint16_t* row, int c, int k, b
         if (c + j < k) u[j >> 1] |= (unsigned)row[c + j] << (j & 1) * 16;
     return make_uint4(u[0], u[1], u[2], u[3]);
 }
-// A CTA walks over the tiles of 16 rows of W blockIdx.x, + gridDim.x, ..; its warps take a tile's runs of 32 k by turns, the loads of the next ones, also of the next tile, under way.  The rows of
-// x lie in shared memory, all of their k (`chunk`) where they fit; else a portion at a time, laid out again for every tile
-template <int NT, bool BF16>
+// rows of x into shared memory as 16-bit numbers: their k from k0 on, zeros behind the end of the last run
+template <bool BF16>
+__device__ __forceinline__ void pf_stage(const PrArgs& a, uint8_t* to, int pitch, int k0, int runs) {
+    for (int e = threadIdx.x; e < a.rows * runs * 4; e += PF_THREADS) {
+        const int r = e / (runs * 4), col = e % (runs * 4) * 8;
+        float x[8] = {};
+        if (k0 + col < a.k) {
+            const int64_t at = (int64_t)r * a.x_stride + k0 + col;
+            if (k0 + col + 8 <= a.k) ht_read8(a.x, at, a.x_type, a.x_vec, x);
+            else
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (k0 + col + j < a.k) x[j] = ht_read(a.x, at + j, a.x_type);
+        }
+        *(uint4*)(to + r * pitch + col * 2) = pr_pack8<BF16>(x);
+    }
+}
+// A CTA walks over the tiles of 16 rows of W blockIdx.x, + gridDim.x, ..; its warps take a tile's runs of 32 k by turns.
+// WHOLE (rows of W at multiples of 16 bytes, all k of x in shared memory): four runs of a warp are computed while the next four, also of the next tile, are under way: 64 KB an SM and more.
+// Else, k of any size: x lies in shared memory a portion (`chunk`) at a time, laid out again for every tile, weights number by number where their rows start anywhere
+template <int NT, bool BF16, bool WHOLE>
 __global__ void __launch_bounds__(PF_THREADS, 1) product_few_kernel(const __grid_constant__ PrArgs a) {
     extern __shared__ __align__(16) uint8_t pf_raw[];
     constexpr int BUFFERS = NT == 4 ? 1 : 2;
     __shared__ float sums[BUFFERS][PF_WARPS][16][NT * 8 + 1];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, pitch = a.chunk * 2 + 64;      // eight lanes' 16 bytes: two rows, 64 bytes each, in all banks
-    const int tiles = (a.m + 15) >> 4, chunks = (a.k + a.chunk - 1) / a.chunk;
-    pdl_enter();
-    uint4 u[PF_AHEAD], v[PF_AHEAD];
-    // this warp's runs in order: run r of chunk lc of tile lt is the next one to be asked for
-    int lt = blockIdx.x, lc = 0, lr = warp;
-    auto runs_of = [&](int c) { return (min(a.chunk, a.k - c * a.chunk) + 31) >> 5; };
-    auto load = [&](uint4& x, uint4& y) {
-        while (lt < tiles && lr >= runs_of(lc)) {
-            lr = warp;
-            if (++lc == chunks) { lc = 0; lt += gridDim.x; }
-        }
-        if (lt >= tiles) return;
-        const int row = lt * 16 + (lane >> 2), c = lc * a.chunk + lr * 32 + (lane & 3) * 8;
-        const uint16_t* w = (const uint16_t*)a.w + (int64_t)row * a.k;
-        x = pf_weights(w, c, a.k, row < a.m, a.w_vec); y = pf_weights(w + (int64_t)8 * a.k, c, a.k, row + 8 < a.m, a.w_vec);
-        lr += PF_WARPS;
-    };
-#pragma unroll
-    for (int i = 0; i < PF_AHEAD; i++) load(u[i], v[i]);
+    const int tiles = (a.m + 15) >> 4, all = (a.k + 31) >> 5, mine = (all - warp + PF_WARPS - 1) / PF_WARPS;      // runs of a tile, and this warp's
+    const uint8_t* x_lane = pf_raw + min(lane >> 2, a.rows - 1) * pitch + (lane & 3) * 16;        // rows behind the last one: any, no one reads their sums
     int z = 0;
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, z = (z + 1) % BUFFERS) {
-        // the tensor cores cut a sum off at 24 bits after every 16 terms, always towards zero: sums of 128 terms go to registers and are rounded there (14336 terms of one sign: off by 1.1e-5
-        // in one chain a warp)
-        float total[NT][4] = {};
-        for (int c = 0; c < chunks; c++) {
-            const int k0 = c * a.chunk, runs = runs_of(c);
-            if (tile == (int)blockIdx.x || chunks > 1) {
-                __syncthreads();                                      // the portion before is through
-                for (int e = tid; e < a.rows * runs * 4; e += PF_THREADS) {
-                    const int r = e / (runs * 4), col = e % (runs * 4) * 8;
-                    float x[8] = {};
-                    if (k0 + col < a.k) {
-                        const int64_t at = (int64_t)r * a.x_stride + k0 + col;
-                        if (k0 + col + 8 <= a.k) ht_read8(a.x, at, a.x_type, a.x_vec, x);
-                        else
-#pragma unroll
-                            for (int j = 0; j < 8; j++)
-                                if (k0 + col + j < a.k) x[j] = ht_read(a.x, at + j, a.x_type);
-                    }
-                    *(uint4*)(pf_raw + r * pitch + col * 2) = pr_pack8<BF16>(x);
-                }
-                __syncthreads();
-            }
-            for (int r = warp; r < runs; r += PF_WARPS * PF_AHEAD) {
-                float acc[NT][4] = {};
-#pragma unroll
-                for (int i = 0; i < PF_AHEAD; i++) {
-                    const int here = r + i * PF_WARPS;
-                    if (here >= runs) break;                          // (the loads stay in their order: the next run's are in u[0] again below)
-#pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        const uint4 b = *(const uint4*)(pf_raw + min(n * 8 + (lane >> 2), a.rows - 1) * pitch + here * 64 + (lane & 3) * 16);      // rows behind the last one: any, no one reads their sums
-                        pr_mma<BF16>(acc[n], u[0].x, v[0].x, u[0].y, v[0].y, b.x, b.y);
-                        pr_mma<BF16>(acc[n], u[0].z, v[0].z, u[0].w, v[0].w, b.z, b.w);
-                    }
-#pragma unroll
-                    for (int j = 0; j + 1 < PF_AHEAD; j++) { u[j] = u[j + 1]; v[j] = v[j + 1]; }
-                    load(u[PF_AHEAD - 1], v[PF_AHEAD - 1]);
-                }
-#pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) total[n][j] += acc[n][j];
-            }
-        }
+    auto finish = [&](int tile, const float (&total)[NT][4]) {
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -142,13 +100,89 @@ __global__ void __launch_bounds__(PF_THREADS, 1) product_few_kernel(const __grid
             if (col < a.m) ht_write(a.out, (int64_t)n * a.m + col, a.out_type, pr_finish(a, s, n, col));
         }
         if (BUFFERS == 1) __syncthreads();
+        z = (z + 1) % BUFFERS;
+    };
+    auto multiply = [&](float (&acc)[NT][4], const uint4& u, const uint4& v, int run) {
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const uint4 b = *(const uint4*)((n == 0 ? x_lane : pf_raw + min(n * 8 + (lane >> 2), a.rows - 1) * pitch + (lane & 3) * 16) + run * 64);
+            pr_mma<BF16>(acc[n], u.x, v.x, u.y, v.y, b.x, b.y);
+            pr_mma<BF16>(acc[n], u.z, v.z, u.w, v.w, b.z, b.w);
+        }
+    };
+    // the tensor cores cut a sum off at 24 bits after every 16 terms, always towards zero: sums of 128 terms go to registers and are rounded there (14336 terms of one sign: off by 1.1e-5 in
+    // one chain a warp)
+    if (WHOLE) {
+        uint4 u[PF_AHEAD], v[PF_AHEAD];
+        const int64_t half = (int64_t)8 * a.k;
+        auto load = [&](uint4 (&x)[PF_AHEAD], uint4 (&y)[PF_AHEAD], int tile, int i0) {
+            // rows behind the last one: the last one again, no one reads their sums
+            const uint16_t* w = (const uint16_t*)a.w + (int64_t)min(tile * 16 + (lane >> 2), a.m - 1) * a.k;
+            const int64_t lower = tile * 16 + (lane >> 2) + 8 < a.m ? half : 0;
+#pragma unroll
+            for (int i = 0; i < PF_AHEAD; i++) {
+                const int c = (warp + (i0 + i) * PF_WARPS) * 32 + (lane & 3) * 8;
+                x[i] = y[i] = make_uint4(0, 0, 0, 0);
+                if (tile < tiles && c < a.k) {
+                    const int4 p = ld_stream_16(w + c), q = ld_stream_16(w + lower + c);
+                    x[i] = make_uint4((unsigned)p.x, (unsigned)p.y, (unsigned)p.z, (unsigned)p.w); y[i] = make_uint4((unsigned)q.x, (unsigned)q.y, (unsigned)q.z, (unsigned)q.w);
+                }
+            }
+        };
+        pdl_enter();
+        load(u, v, blockIdx.x, 0);
+        pf_stage<BF16>(a, pf_raw, pitch, 0, all);
+        __syncthreads();
+        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+            float total[NT][4] = {};
+            for (int i0 = 0; i0 < mine; i0 += PF_AHEAD) {
+                uint4 nu[PF_AHEAD], nv[PF_AHEAD];
+                const bool over = i0 + PF_AHEAD >= mine;
+                load(nu, nv, over ? tile + (int)gridDim.x : tile, over ? 0 : i0 + PF_AHEAD);
+                float acc[NT][4] = {};
+#pragma unroll
+                for (int i = 0; i < PF_AHEAD; i++) multiply(acc, u[i], v[i], min(warp + (i0 + i) * PF_WARPS, all - 1));      // (runs behind the last one: weights 0)
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) total[n][j] += acc[n][j];
+#pragma unroll
+                for (int i = 0; i < PF_AHEAD; i++) { u[i] = nu[i]; v[i] = nv[i]; }
+            }
+            if (mine <= 0) load(u, v, tile + (int)gridDim.x, 0);
+            finish(tile, total);
+        }
+        return;
+    }
+    pdl_enter();
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        float total[NT][4] = {};
+        for (int k0 = 0; k0 < a.k; k0 += a.chunk) {
+            const int runs = (min(a.chunk, a.k - k0) + 31) >> 5;
+            __syncthreads();                                          // the portion before is through
+            pf_stage<BF16>(a, pf_raw, pitch, k0, runs);
+            __syncthreads();
+            const int row = tile * 16 + (lane >> 2);
+            const uint16_t* w = (const uint16_t*)a.w + (int64_t)row * a.k;
+            for (int r = warp; r < runs; r += PF_WARPS) {
+                float acc[NT][4] = {};
+                const int c = k0 + r * 32 + (lane & 3) * 8;
+                multiply(acc, pf_weights(w, c, a.k, row < a.m, a.w_vec), pf_weights(w + (int64_t)8 * a.k, c, a.k, row + 8 < a.m, a.w_vec), r);
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) total[n][j] += acc[n][j];
+            }
+        }
+        finish(tile, total);
     }
 }
 template <int NT>
 static cudaError_t pf_launch(cc_device* dev, PrArgs a, bool bf16) {
-    auto kernel = bf16 ? product_few_kernel<NT, true> : product_few_kernel<NT, false>;
     constexpr int room = NT == 1 ? PF_SMEM : PF_SMEM - 12 * 1024;      // beside 17 and 34 KB of sums
     a.chunk = std::min((a.k + 63) / 64 * 64, (room / a.rows - 64) / 128 * 64);
+    const bool whole = a.w_vec && a.chunk >= a.k;
+    auto kernel = whole ? (bf16 ? product_few_kernel<NT, true, true> : product_few_kernel<NT, false, true>) : (bf16 ? product_few_kernel<NT, true, false> : product_few_kernel<NT, false, false>);
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, room);
     if (e == cudaSuccess) e = cc_launch_pdl(dev, kernel, (unsigned)std::min((a.m + 15) / 16, dev->sm_count), PF_THREADS, (size_t)a.rows * (a.chunk * 2 + 64), a);
     dev->launches++;
@@ -192,7 +226,7 @@ static int pt_launch(cc_device* dev, const PrArgs& a, const void* w, const void*
     auto kernel = product_tile_kernel<BN, BF16, DRAIN>;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(parts > 1 ? tiles * parts : std::min<int64_t>(tiles, dev->sm_count)));
-    cfg.blockDim = dim3(PT_THREADS); cfg.dynamicSmemBytes = pt_smem(BN, false); cfg.stream = dev->stream;
+    cfg.blockDim = dim3(pt_threads(BN, DRAIN)); cfg.dynamicSmemBytes = pt_smem(BN, false); cfg.stream = dev->stream;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = dev->pdl ? 1 : 0;
@@ -205,27 +239,40 @@ static int pt_launch(cc_device* dev, const PrArgs& a, const void* w, const void*
     return CC_OK;
 }
 template <bool BF16, bool DRAIN>
-static int pt_launch_pair(cc_device* dev, const PrArgs& a, const void* w, const void* x, int64_t x_stride, int kp) {
+static int pt_launch_pair(cc_device* dev, const PrArgs& a, const void* w, const void* x, int64_t x_stride, int kp, int parts) {
     const int64_t tiles = (int64_t)((a.m + 255) / 256) * ((a.rows + 255) / 256);
-    CC_REQUIRE(dev, tiles < ((int64_t)1 << 30), "product: %lld tiles", (long long)tiles);
-    const int pairs = dev->sm_count / 2, rest = (int)(tiles % pairs), whole = (int)tiles - rest;
+    CC_REQUIRE(dev, tiles < ((int64_t)1 << 28), "product: %lld tiles", (long long)tiles);
+    const int pairs = dev->sm_count / 2, rest = parts > 1 ? 0 : (int)(tiles % pairs), whole = (int)tiles - rest;
     int cut = 1;
-    while (cut < 8 && rest * cut * 2 <= pairs) cut *= 2;
+    while (cut < 4 && rest * cut * 2 <= pairs) cut *= 2;             // pieces of 64 rows: 16 for each group of the warps that finish
     CUtensorMap mw, mx, mc;
     int rc = cc_make_tmap_rows(dev, &mw, w, a.m, a.k, (int64_t)kp * 2, 128, BF16);
     if (!rc) rc = cc_make_tmap_rows(dev, &mx, x, a.rows, a.k, x_stride * 2, 128, BF16);
     if (!rc) rc = cc_make_tmap_rows(dev, &mc, x, a.rows, a.k, x_stride * 2, 128 / cut, BF16);
     if (rc) return rc;
     auto kernel = product_pair_kernel<BF16, DRAIN>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(2 * (parts > 1 ? tiles * parts : std::min(whole + rest * cut, pairs))));
+    cfg.blockDim = dim3(pt_threads(256, DRAIN)); cfg.dynamicSmemBytes = pt_smem(256, true); cfg.stream = dev->stream;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = dev->pdl ? 1 : 0;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)(2 * parts); at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = 2;
     CC_CUDA(dev, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pt_smem(256, true)));
-    CC_CUDA(dev, cc_launch_pdl(dev, kernel, (unsigned)(2 * std::min(whole + rest * cut, pairs)), PT_THREADS, pt_smem(256, true), mw, mx, mc, a, (a.k + 63) / 64, whole, cut, whole + rest * cut,
-                               dev->err_dev, dev->err_host));
-    dev->launches++;
+    CC_CUDA(dev, cudaLaunchKernelEx(&cfg, kernel, mw, mx, mc, a, (a.k + 63) / 64, whole, cut, whole + rest * cut, parts, dev->err_dev, dev->err_host));
+    CC_LAUNCH_CHECK(dev);
     return CC_OK;
 }
 template <bool BF16, bool DRAIN>
 static int pt_tiles(cc_device* dev, const PrArgs& a, const void* w, const void* x, int64_t x_stride, int kp) {
-    if (a.rows > 128 && dev->sm_count > 1 && (int64_t)((a.m + 255) / 256) * ((a.rows + 255) / 256) >= dev->sm_count / 2) return pt_launch_pair<BF16, DRAIN>(dev, a, w, x, x_stride, kp);
+    const int64_t tiles = (int64_t)((a.m + 255) / 256) * ((a.rows + 255) / 256), pairs = dev->sm_count / 2;
+    if (a.rows > 128 && pairs > 0) {
+        int parts = 1;
+        while (parts < 4 && tiles * parts * 2 <= pairs && (a.k + 63) / 64 / (parts * 2) >= 8) parts *= 2;
+        if (tiles * parts * 2 > pairs) return pt_launch_pair<BF16, DRAIN>(dev, a, w, x, x_stride, kp, parts);
+    }
     return a.rows <= 32 ? pt_launch<32, BF16, DRAIN>(dev, a, w, x, x_stride, kp) : a.rows <= 64 ? pt_launch<64, BF16, DRAIN>(dev, a, w, x, x_stride, kp)
            : a.rows <= 128 ? pt_launch<128, BF16, DRAIN>(dev, a, w, x, x_stride, kp) : pt_launch<256, BF16, DRAIN>(dev, a, w, x, x_stride, kp);
 }
@@ -285,7 +332,7 @@ extern "C" CC_API int cc_product(cc_device* dev, const cc_view* w, const cc_view
         a.out = o->base; a.x_stride = x->strides[0]; a.res_stride = residual ? residual->strides[0] : 0; a.m = (int)m; a.k = (int)k; a.rows = (int)T;
         a.x_type = x->buf->dtype; a.out_type = out_type; a.act = act;
         a.w_vec = k % 8 == 0 && ((uintptr_t)a.w & 15) == 0; a.x_vec = a.x_stride * ht_size(a.x_type) % 16 == 0 && ((uintptr_t)a.x & 15) == 0;
-        if (T > PF_ROWS) rc = pr_many(dev, a, bf16);
+        if (T > PF_ROWS || (T > 1 && a.w_vec && T * k > PF_ROOM)) rc = pr_many(dev, a, bf16);
         else {
             const cudaError_t e = T <= 8 ? pf_launch<1>(dev, a, bf16) : T <= 16 ? pf_launch<2>(dev, a, bf16) : pf_launch<4>(dev, a, bf16);
             if (e != cudaSuccess) rc = cc_fail(dev, CC_ERR_CUDA, "product: %s", cudaGetErrorString(e));

@@ -14,8 +14,9 @@
 
 #include "split_gemm.cuh"
 
-#define PT_THREADS 384
-#define PT_WORKERS 8                          // warps that finish: the first four the left half of a tile's rows of x, the others the right one
+// Warps that finish: four take all lanes, each group of four its share of the tile's rows of x.  Sums that leave TMEM need a register each: with 8 warps 128 of them, which spilled
+__host__ __device__ constexpr int pt_workers(int bn, bool drain) { return drain && bn >= 64 ? 16 : 8; }
+__host__ __device__ constexpr int pt_threads(int bn, bool drain) { return 128 + 32 * pt_workers(bn, drain); }
 #define PT_DRAIN 4                            // steps of a sum that leaves for registers
 #define PT_STEP 128                           // bytes of a row in a step
 struct PtShared {
@@ -81,18 +82,16 @@ __device__ __forceinline__ void pt_finish16(const PrArgs& a, const unsigned (&v)
 }
 // With the activation as a function that is known: each has its own loop.  16-bit results: by the special function unit's exponential and reciprocal, 2^-20 of a result, in a dozen instructions
 // where tanhf and a division take sixty (8 warps finished a tile of 256 x 256 no sooner than 64 steps of its products were done)
+__device__ __noinline__ float pt_exact_act(float z, int act) { return act_apply(z, act); }      // (out of line: sixteen of them side by side spilled)
 template <bool EXACT, class Body>
 __device__ __forceinline__ void pt_with_act(int act, Body body) {
-    auto sigmoid = [](float z) { return EXACT ? act_sigmoid(z) : __fdividef(1.0f, 1.0f + __expf(-z)); };
-    switch (act) {
-    case CC_ACT_NONE: body([](float z) { return z; }); break;
-    case CC_ACT_GELU_TANH:                                            // (1 + tanh u) / 2 = sigmoid(2 u)
-        body([=](float z) { return EXACT ? act_gelu_tanh(z) : z * sigmoid(1.5957691216057308f * fmaf(0.044715f * z, z * z, z)); });
-        break;
-    case CC_ACT_SIGMOID: body(sigmoid); break;
-    case CC_ACT_RELU_SQUARED: body([](float z) { return act_relu_squared(z); }); break;
-    default: body([=](float z) { return EXACT ? act_silu(z) : z * sigmoid(z); });      // SWISH with alpha 1
-    }
+    auto sigmoid = [](float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); };
+    if (act == CC_ACT_NONE) body([](float z) { return z; });
+    else if (EXACT) body([=](float z) { return pt_exact_act(z, act); });
+    else if (act == CC_ACT_GELU_TANH) body([=](float z) { return z * sigmoid(1.5957691216057308f * fmaf(0.044715f * z, z * z, z)); });      // (1 + tanh u) / 2 = sigmoid(2 u)
+    else if (act == CC_ACT_SIGMOID) body(sigmoid);
+    else if (act == CC_ACT_RELU_SQUARED) body([](float z) { return act_relu_squared(z); });
+    else body([=](float z) { return z * sigmoid(z); });               // SILU, and SWISH with alpha 1
 }
 __device__ __forceinline__ void pt_report(const PtShared& sh, unsigned* err_dev, unsigned* err_host) {
     if (threadIdx.x == 0 && sh.fail) {
@@ -104,10 +103,10 @@ __device__ __forceinline__ void pt_report(const PtShared& sh, unsigned* err_dev,
 // a CTA walks over the tiles of its cluster; the `parts` CTAs of a cluster share a tile's depth (then there is one tile for each cluster), and each finishes every parts-th run of 16 rows of x
 // with the sums of all, in the order of the parts
 template <int BN, bool BF16, bool DRAIN>
-__global__ void __launch_bounds__(PT_THREADS, 1) product_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ PrArgs a, int steps_all, int n_tiles,
+__global__ void __launch_bounds__(pt_threads(BN, DRAIN), 1) product_tile_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ PrArgs a, int steps_all, int n_tiles,
                                                                      int parts, unsigned* err_dev, unsigned* err_host) {
     namespace cg = cooperative_groups;
-    constexpr int ST = pt_stages(BN, false), HALF = BN / 2;
+    constexpr int ST = pt_stages(BN, false), WORKERS = pt_workers(BN, DRAIN), GROUPS = WORKERS / 4, HALF = BN / GROUPS;
     constexpr unsigned A_BYTES = 128 * PT_STEP, BYTES = pt_bytes(BN, false), COLS = 2 * BN;
     extern __shared__ __align__(1024) uint8_t pt_raw[];
     __shared__ PtShared sh;
@@ -118,7 +117,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) product_tile_kernel(const __gri
     const int tiles_n = (a.rows + BN - 1) / BN, first = blockIdx.x / parts, stride = gridDim.x / parts;
     if (threadIdx.x == 0) {
         for (int i = 0; i < ST; i++) { pg_mbar_init(pg_smem(&sh.full[i]), 1); pg_mbar_init(pg_smem(&sh.empty[i]), 1); }
-        for (int i = 0; i < 2; i++) { pg_mbar_init(pg_smem(&sh.acc_full[i]), 1); pg_mbar_init(pg_smem(&sh.acc_empty[i]), PT_WORKERS); }
+        for (int i = 0; i < 2; i++) { pg_mbar_init(pg_smem(&sh.acc_full[i]), 1); pg_mbar_init(pg_smem(&sh.acc_empty[i]), WORKERS); }
         pg_mbar_init(pg_smem(&sh.drained), 1);
         sh.fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -218,9 +217,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) product_tile_kernel(const __gri
         const unsigned from = tmem + (nth & 1u) * BN + lane_col;
         __syncthreads();
         cluster.sync();                                               // every CTA's products are done: the rings are free
-        // [sender][run of the owner][half][row of x][channel]
+        // [sender][run of the owner][group of workers][row of x][channel]
         constexpr int RUNS = HALF / 16;
-        auto box = [&](int sender, int owner, int run) { return ((((size_t)(sender < owner ? sender : sender - 1) * ((RUNS + parts - 1) / parts) + run / parts) * 2 + half) * 16) * 128 + q * 32 + lane; };
+        auto box = [&](int sender, int owner, int run) { return ((((size_t)(sender < owner ? sender : sender - 1) * ((RUNS + parts - 1) / parts) + run / parts) * GROUPS + half) * 16) * 128 + q * 32 + lane; };
         if (warp >= 4) {
 #pragma unroll 1
             for (int run = 0; run < RUNS && n0 + run * 16 < a.rows; run++) {
@@ -266,32 +265,33 @@ __global__ void __launch_bounds__(PT_THREADS, 1) product_tile_kernel(const __gri
 __device__ __forceinline__ void pt_umma2(unsigned tmem_d, uint64_t a, uint64_t b, unsigned idesc, unsigned accumulate) {
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
-// what this thread has issued so far arrives on the barrier, when it is complete, in both CTAs
-__device__ __forceinline__ void pt_commit2(unsigned bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+// what this thread has issued so far arrives on the barrier, when it is complete, in both CTAs of the pair
+__device__ __forceinline__ void pt_commit2(unsigned bar, unsigned pair) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)(3u << 2 * pair)) : "memory");
 }
-__device__ __forceinline__ unsigned pt_even(unsigned addr) {         // the even CTA's own of it
+__device__ __forceinline__ unsigned pt_even(unsigned addr, unsigned pair) {      // the pair's even CTA's own of it
     unsigned a;
-    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(addr));
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(2 * pair));
     return a;
 }
 __device__ __forceinline__ void pt_tma2(unsigned dst, const void* tmap, unsigned bar, int x, int y) {
     asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(tmap), "r"(bar), "r"(x), "r"(y) : "memory");
 }
-// the first n_whole tiles are 256 x 256, those of the last wave that is not full are cut across the rows of x, `cut` pieces each.  The even CTA issues the products; the copies of both are
-// counted on its barriers, and what it commits arrives in both
+// The first n_whole tiles are 256 x 256, those of the last wave that is not full are cut across the rows of x, `cut` pieces each.  The even CTA issues the products; the copies of both are
+// counted on its barriers, and what it commits arrives in both.  parts > 1: a cluster of that many pairs shares a tile's depth (there is one tile for each cluster), and each pair finishes every
+// parts-th run of 16 rows of x with the sums of all, in the order of the parts
 template <bool BF16, bool DRAIN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) product_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
-                                                                                              const __grid_constant__ CUtensorMap map_cut, const __grid_constant__ PrArgs a, int steps, int n_whole, int cut,
-                                                                                              int n_tiles, unsigned* err_dev, unsigned* err_host) {
+__global__ void __launch_bounds__(pt_threads(256, DRAIN), 1) product_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_cut,
+                                                                                 const __grid_constant__ PrArgs a, int steps_all, int n_whole, int cut, int n_tiles, int parts, unsigned* err_dev, unsigned* err_host) {
     namespace cg = cooperative_groups;
-    constexpr int BN = 256, ST = pt_stages(BN, true);
+    constexpr int BN = 256, ST = pt_stages(BN, true), WORKERS = pt_workers(BN, DRAIN), GROUPS = WORKERS / 4;
     constexpr unsigned A_BYTES = 128 * PT_STEP, BYTES = pt_bytes(BN, true), COLS = 2 * BN;
     extern __shared__ __align__(1024) uint8_t pt_raw[];
     __shared__ PtShared sh;
     uint8_t* ring = (uint8_t*)(((uintptr_t)pt_raw + 1023) & ~(uintptr_t)1023);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cg::this_cluster().block_rank();
-    const int tiles_n = (a.rows + BN - 1) / BN, first = blockIdx.x / 2, stride = gridDim.x / 2, chunk = DRAIN ? PT_DRAIN : steps, chunks = (steps + chunk - 1) / chunk;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, of_cluster = (int)cg::this_cluster().block_rank(), rank = of_cluster & 1, part = of_cluster >> 1;
+    const int s0 = (int)((int64_t)steps_all * part / parts), steps = (int)((int64_t)steps_all * (part + 1) / parts) - s0;
+    const int tiles_n = (a.rows + BN - 1) / BN, first = blockIdx.x / (2 * parts), stride = gridDim.x / (2 * parts), chunk = DRAIN ? PT_DRAIN : steps, chunks = (steps + chunk - 1) / chunk;
     auto place = [&](int tile, int& mt, int& n0) {
         const int of = tile < n_whole ? tile : n_whole + (tile - n_whole) / cut;
         mt = of / tiles_n;
@@ -300,7 +300,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
     };
     if (threadIdx.x == 0) {
         for (int i = 0; i < ST; i++) { pg_mbar_init(pg_smem(&sh.full[i]), 1); pg_mbar_init(pg_smem(&sh.empty[i]), 1); }
-        for (int i = 0; i < 2; i++) { pg_mbar_init(pg_smem(&sh.acc_full[i]), 1); pg_mbar_init(pg_smem(&sh.acc_empty[i]), 2 * PT_WORKERS); }
+        for (int i = 0; i < 2; i++) { pg_mbar_init(pg_smem(&sh.acc_full[i]), 1); pg_mbar_init(pg_smem(&sh.acc_empty[i]), 2 * WORKERS); }
         pg_mbar_init(pg_smem(&sh.drained), 1);
         sh.fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -325,11 +325,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
                 int mt, n0;
                 const int wide = place(tile, mt, n0);
                 for (int s = 0; s < steps; s++, g++) {
-                    const unsigned slot = g % ST, own = pg_smem(&sh.full[slot]), full = pt_even(own), at = pg_smem(ring + (size_t)slot * BYTES);
+                    const unsigned slot = g % ST, own = pg_smem(&sh.full[slot]), full = pt_even(own, part), at = pg_smem(ring + (size_t)slot * BYTES);
                     if (!(ok = sg_wait(pg_smem(&sh.empty[slot]), ((g / ST) & 1u) ^ 1u, &sh.fail))) break;
                     if (rank == 0) pg_mbar_expect_tx(own, 2 * A_BYTES + wide * PT_STEP);
-                    pt_tma2(at, &map_w, full, s * 64, mt * 256 + rank * 128);
-                    pt_tma2(at + A_BYTES, wide == BN ? &map_x : &map_cut, full, s * 64, n0 + rank * (wide / 2));
+                    pt_tma2(at, &map_w, full, (s0 + s) * 64, mt * 256 + rank * 128);
+                    pt_tma2(at + A_BYTES, wide == BN ? &map_x : &map_cut, full, (s0 + s) * 64, n0 + rank * (wide / 2));
                 }
             }
             int never = 0;                                            // no copy is under way when the CTAs end (the even one sees those of both), and no arrival
@@ -360,39 +360,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
                     if (pg_elect()) {
 #pragma unroll
                         for (int kk = 0; kk < 4; kk++) pt_umma2(acc, x + 2 * kk, y + 2 * kk, idesc, s % chunk > 0 || kk > 0);
-                        pt_commit2(pg_smem(&sh.empty[slot]));
-                        if (last) pt_commit2(pg_smem(&sh.acc_full[nth & 1u]));
+                        pt_commit2(pg_smem(&sh.empty[slot]), part);
+                        if (last) pt_commit2(pg_smem(&sh.acc_full[nth & 1u]), part);
                     }
                     __syncwarp();
                     nth += last;
                     if (++slot == ST) { slot = 0; phase ^= 1u; }
                 }
             }
-            if (pg_elect()) pt_commit2(pg_smem(&sh.drained));
+            if (pg_elect()) pt_commit2(pg_smem(&sh.drained), part);
             __syncwarp();
         }
         sg_wait_warp(pg_smem(&sh.drained), 0, &never);
-    } else if (warp >= 4) {
-        const int q = warp & 3, half = (warp - 4) >> 2;
+    }
+    const int q = warp & 3, group = (warp - 4) >> 2;
+    auto release = [&](unsigned n) {
+        pg_fence_before();
+        __syncwarp();
+        if (lane == 0) pg_arrive_relaxed(pt_even(pg_smem(&sh.acc_empty[n & 1u]), part));
+    };
+    // a cut tile's columns are shared by all groups, but those that a warp has added up are its own
+    auto share = [&](int wide, int& c_first) {
+        const int each = DRAIN ? BN / GROUPS : wide / GROUPS;
+        c_first = group * each;
+        return max(0, min(each, wide - c_first));
+    };
+    auto collect = [&](unsigned& nth, int c_first) {                  // the tile's sums are in the buffer of chunk nth
+        if (DRAIN) return pt_collect<BN / GROUPS>(sh, tmem, BN, nth, chunks, ((unsigned)(q * 32) << 16) + (unsigned)c_first, release);
+        if (!sg_wait_warp(pg_smem(&sh.acc_full[nth & 1u]), (nth >> 1) & 1u, &sh.fail)) return false;
+        pg_fence_after();
+        return true;
+    };
+    if (warp >= 4 && parts == 1) {
         unsigned nth = 0;
-        auto release = [&](unsigned n) {
-            pg_fence_before();
-            __syncwarp();
-            if (lane == 0) pg_arrive_relaxed(pt_even(pg_smem(&sh.acc_empty[n & 1u])));
-        };
         for (int tile = first; tile < n_tiles; tile += stride, nth++) {
-            int mt, at;
-            // a cut tile's columns are shared by both halves, but those that a warp has added up are its own
-            const int wide = place(tile, mt, at), c_first = half * (DRAIN ? BN / 2 : wide / 2), mine = DRAIN ? min(BN / 2, wide - c_first) : wide / 2, n0 = at + c_first;
-            const int col = mt * 256 + rank * 128 + q * 32 + lane;
-            const unsigned lane_col = ((unsigned)(q * 32) << 16) + (unsigned)c_first;
-            if (DRAIN) {
-                if (!pt_collect<BN / 2>(sh, tmem, BN, nth, chunks, lane_col, release)) break;
-            } else {
-                if (!sg_wait_warp(pg_smem(&sh.acc_full[nth & 1u]), (nth >> 1) & 1u, &sh.fail)) break;
-                pg_fence_after();
-            }
-            const unsigned from = tmem + (nth & 1u) * BN + lane_col;
+            int mt, at, c_first;
+            const int wide = place(tile, mt, at), mine = share(wide, c_first), n0 = at + c_first, col = mt * 256 + rank * 128 + q * 32 + lane;
+            if (!collect(nth, c_first)) break;
+            const unsigned from = tmem + (nth & 1u) * BN + ((unsigned)(q * 32) << 16) + (unsigned)c_first;
             const float bias = a.bias && col < a.m ? a.bias[col] : 0.0f;
             pt_with_act<DRAIN>(a.act, [&](auto act) {
 #pragma unroll 1
@@ -403,6 +408,52 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PT_THREADS, 1) produ
                 }
             });
             release(nth);
+        }
+    }
+    if (parts > 1) {
+        cg::cluster_group cluster = cg::this_cluster();
+        constexpr int EACH = BN / GROUPS, RUNS = EACH / 16;
+        const int mt = first / tiles_n, n0 = (first - mt * tiles_n) * BN + group * EACH, col = mt * 256 + rank * 128 + q * 32 + lane;
+        unsigned nth = 0;
+        if (warp >= 4) collect(nth, group * EACH);
+        const unsigned from = tmem + (nth & 1u) * BN + ((unsigned)(q * 32) << 16) + (unsigned)(group * EACH);
+        __syncthreads();
+        cluster.sync();                                               // every CTA's products are done: the rings are free
+        // [sender][run of the owner][group][row of x][channel]
+        auto box = [&](int sender, int owner, int run) { return ((((size_t)(sender < owner ? sender : sender - 1) * ((RUNS + parts - 1) / parts) + run / parts) * GROUPS + group) * 16) * 128 + q * 32 + lane; };
+        if (warp >= 4) {
+#pragma unroll 1
+            for (int run = 0; run < RUNS && n0 + run * 16 < a.rows; run++) {
+                const int owner = run % parts;
+                if (owner == part) continue;
+                unsigned v[16];
+                pt_load16(from + run * 16, v);
+                float* to = cluster.map_shared_rank((float*)ring, 2 * owner + rank) + box(part, owner, run);
+#pragma unroll
+                for (int j = 0; j < 16; j++) to[j * 128] = __uint_as_float(v[j]);
+            }
+        }
+        cluster.sync();
+        if (warp >= 4 && !*(volatile int*)&sh.fail) {
+            const float bias = a.bias && col < a.m ? a.bias[col] : 0.0f;
+            pt_with_act<DRAIN>(a.act, [&](auto act) {
+#pragma unroll 1
+                for (int run = part; run < RUNS && n0 + run * 16 < a.rows; run += parts) {
+                    unsigned v[16];
+                    float sum[16];
+                    pt_load16(from + run * 16, v);
+#pragma unroll
+                    for (int j = 0; j < 16; j++) sum[j] = 0.0f;
+                    for (int p = 0; p < parts; p++) {
+                        const float* o = (const float*)ring + (p == part ? 0 : box(p, part, run));
+#pragma unroll
+                        for (int j = 0; j < 16; j++) sum[j] += p == part ? __uint_as_float(v[j]) : o[j * 128];
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; j++) v[j] = __float_as_uint(sum[j]);
+                    pt_finish16(a, v, n0 + run * 16, a.rows, col, bias, act);
+                }
+            });
         }
     }
     pg_fence_before();
