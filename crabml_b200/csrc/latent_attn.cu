@@ -49,16 +49,24 @@ struct LrArgs {
     int4* steps;                              // [CTA][run_lo + 1]: what each step asks for
     void* out;
     float scale;
-    int n_seqs, table_cols, page, shift, H, dim, vdim, rank, rest, cols, window, most, out_bf16, slots;      // most: sequences with more new tokens take the other form
+    int n_seqs, table_cols, page, shift, H, dim, vdim, rank, rest, cols, window, out_bf16, slots;
+    int most, token0, token1;                 // sequences with more new tokens take the other form; the tokens of this portion
 };
 struct LrDeal { int ctas, run_lo, run_more; struct { int seq, tile, off; } at[LR_CTAS]; };
 struct LrCuts { struct { int seq, tile, slot, cta, n; } at[LR_CTAS]; };
 
+// a sequence's part in this portion of the call's tokens: none of those that take the other form
+__host__ __device__ __forceinline__ PgSeq lr_clip(PgSeq s, const LrArgs& a) {
+    const int lo = s.first > a.token0 ? s.first : a.token0, hi = s.first + s.count < a.token1 ? s.first + s.count : a.token1;
+    if (s.count > a.most || hi <= lo) { s.count = 0; return s; }
+    s.pos0 += lo - s.first; s.first = lo; s.count = hi - lo;
+    return s;
+}
 __host__ __device__ __forceinline__ void lr_range(const PgSeq& s, const LrArgs& a, int* from, int* to) {
     *to = s.pos0 + s.count;
     *from = a.window > 0 && s.pos0 - a.window + 1 > 0 ? (s.pos0 - a.window + 1) & ~(LR_KEYS - 1) : 0;      // steps are whole pages, or parts of one
 }
-__host__ __device__ __forceinline__ int lr_tiles(const PgSeq& s, const LrArgs& a) { return s.count > a.most ? 0 : (int)(((int64_t)s.count * a.H + LR_ROWS - 1) / LR_ROWS); }
+__host__ __device__ __forceinline__ int lr_tiles(const PgSeq& s, const LrArgs& a) { return (int)(((int64_t)s.count * a.H + LR_ROWS - 1) / LR_ROWS); }
 __host__ __device__ __forceinline__ int lr_steps(const PgSeq& s, const LrArgs& a) {
     int from, to;
     lr_range(s, a, &from, &to);
@@ -108,7 +116,7 @@ struct LrWalk {
     template <class F>
     __device__ __forceinline__ bool piece(const LrArgs& a, F body) {
         while (left > 0 && seq < a.n_seqs) {
-            const PgSeq s = a.seqs[seq];
+            const PgSeq s = lr_clip(a.seqs[seq], a);
             if (tile >= lr_tiles(s, a)) { seq++; tile = 0; off = 0; continue; }
             const int all = lr_steps(s, a), take = min(left, all - off), from = off;
             left -= take;
@@ -612,7 +620,7 @@ __global__ void __launch_bounds__(LJ_THREADS) latent_join_kernel(const __grid_co
     __shared__ float4 sums[SLICES][COLS / 4];
     pdl_enter();
     const auto cut = cuts.at[blockIdx.x];
-    const PgSeq s = a.seqs[cut.seq];
+    const PgSeq s = lr_clip(a.seqs[cut.seq], a);
     const int x = threadIdx.x, y = blockIdx.y, row = cut.tile * LR_ROWS + y, lane = x & 31, w = x >> 5, c = blockIdx.z * COLS + x % (COLS / 4) * 4, which = x / (COLS / 4);
     if (row >= s.count * a.H) return;
     auto place = [&](int i) { return (size_t)(i == 0 ? cut.slot : 2 * (cut.cta + i - 1)) * LR_ROWS + y; };
@@ -666,7 +674,8 @@ static int lr_deal(const cc_page_plan* plan, const LrArgs& a, int64_t steps, LrD
     int64_t before = 0, next = 0;                                  // steps in front of the sequence, and of run c
     int c = 0, n_cuts = 0;
     for (int seq = 0; seq < (int)plan->seqs.size() && c < deal.ctas; seq++) {
-        const int n = lr_tiles(plan->seqs[seq], a), all = n ? lr_steps(plan->seqs[seq], a) : 0;
+        const PgSeq s = lr_clip(plan->seqs[seq], a);
+        const int n = lr_tiles(s, a), all = n ? lr_steps(s, a) : 0;
         for (; c < deal.ctas && next < before + (int64_t)n * all; next += deal.run_lo + (c < deal.run_more ? 1 : 0), c++) {
             const int tile = (int)((next - before) / all), off = (int)((next - before) - (int64_t)tile * all);
             deal.at[c] = {seq, tile, off};
@@ -680,25 +689,35 @@ static int lr_deal(const cc_page_plan* plan, const LrArgs& a, int64_t steps, LrD
     }
     return n_cuts;
 }
-static int lr_run(cc_device* dev, const cc_page_plan* plan, LrArgs a, const LtRuns& runs) {
+// the tokens a.token0 .. a.token1 - 1
+static int lr_portion(cc_device* dev, const cc_page_plan* plan, LrArgs a) {
     int64_t steps = 0, tiles = 0;
-    for (const PgSeq& s : plan->seqs) {
+    LtRuns runs{};
+    for (const PgSeq& whole : plan->seqs) {
+        const PgSeq s = lr_clip(whole, a);
+        if (!s.count) continue;
         const int n = lr_tiles(s, a);
         tiles += n;
-        steps += (int64_t)n * (n ? lr_steps(s, a) : 0);
+        steps += (int64_t)n * lr_steps(s, a);
+        // many runs: the last one takes all that lies behind (results of other tokens are overwritten)
+        if (runs.n && (runs.hi[runs.n - 1] == s.first || runs.n == LT_RUNS)) runs.hi[runs.n - 1] = s.first + s.count;
+        else { runs.lo[runs.n] = s.first; runs.hi[runs.n++] = s.first + s.count; }
     }
     if (!tiles) return CC_OK;
+    for (int i = 0; i < runs.n; i++) { runs.tile0[i] = runs.tiles; runs.tiles += (runs.hi[i] - runs.lo[i] + LT_TOKENS - 1) / LT_TOKENS; }
     LrDeal deal;
     LrCuts cuts;
     CC_REQUIRE(dev, steps < ((int64_t)1 << 31) * 64, "paged_latent_attention: too many rows");
     deal.ctas = (int)std::min<int64_t>(std::min(LR_CTAS, dev->sm_count), (steps + LR_BEGIN + 1) / (LR_BEGIN + 2));
     const int n_cuts = lr_deal(plan, a, steps, deal, cuts);
-    const size_t qf = (size_t)plan->tokens * a.H * a.cols * 4, lat = (size_t)plan->tokens * a.H * a.rank * 4, part = n_cuts ? (size_t)2 * deal.ctas * LR_ROWS * a.rank * 4 : 0,
+    const int64_t tokens = a.token1 - a.token0;
+    const size_t qf = (size_t)tokens * a.H * a.cols * 4, lat = (size_t)tokens * a.H * a.rank * 4, part = n_cuts ? (size_t)2 * deal.ctas * LR_ROWS * a.rank * 4 : 0,
                  ml = (size_t)2 * deal.ctas * LR_ROWS * sizeof(float2), list = (size_t)deal.ctas * (deal.run_lo + 1) * sizeof(int4);
     void* ws = nullptr; size_t cls = 0;
     int rc = cc_pool_alloc(dev, qf + lat + part + ml + list, &ws, &cls);
     if (rc) return rc;
-    a.qf = (float*)ws; a.lat = (float*)((uint8_t*)ws + qf); a.part = (float*)((uint8_t*)ws + qf + lat); a.ml = (float2*)((uint8_t*)ws + qf + lat + part);
+    // rows count from the call's first token
+    a.qf = (float*)((uintptr_t)ws - (uintptr_t)a.token0 * a.H * a.cols * 4); a.lat = (float*)((uintptr_t)ws + qf - (uintptr_t)a.token0 * a.H * a.rank * 4); a.part = (float*)((uint8_t*)ws + qf + lat); a.ml = (float2*)((uint8_t*)ws + qf + lat + part);
     a.steps = (int4*)((uint8_t*)ws + qf + lat + part + ml);
     const int slot = (a.cols + 63) / 64 * LR_BLOCK;
     a.slots = std::min(LR_SLOTS, (LR_SMEM - (int)sizeof(LrShared) - 1024) / slot);
@@ -728,6 +747,17 @@ static int lr_run(cc_device* dev, const cc_page_plan* plan, LrArgs a, const LtRu
     return CC_OK;
 }
 
+// as many tokens at a time as have their queries and sums over the latents in LT_WORKSPACE
+#define LT_WORKSPACE ((int64_t)256 << 20)
+static int lr_run(cc_device* dev, const cc_page_plan* plan, LrArgs a) {
+    const int64_t each = std::max<int64_t>(LT_TOKENS, LT_WORKSPACE / ((int64_t)a.H * (a.cols + a.rank) * 4) / LT_TOKENS * LT_TOKENS);
+    for (int64_t t = 0; t < plan->tokens; t += each) {
+        a.token0 = (int)t; a.token1 = (int)std::min(plan->tokens, t + each);
+        const int rc = lr_portion(dev, plan, a);
+        if (rc) return rc;
+    }
+    return CC_OK;
+}
 #include "latent_tile.cuh"
 
 #define LT_FEW 64                             // new tokens of a sequence; with more its keys and values are laid out
@@ -770,15 +800,7 @@ extern "C" CC_API int cc_paged_latent_attention(cc_device* dev, const cc_page_pl
         a.n_seqs = plan->n_seqs; a.table_cols = plan->table_cols; a.page = plan->page; a.shift = plan->shift; a.H = H; a.dim = (int)dim; a.vdim = (int)vdim;
         a.rank = c.rank; a.rest = c.rest; a.cols = c.cols; a.window = window > 0 ? window : 0; a.out_bf16 = out_type == CC_BF16;
         a.most = form == CC_LATENT_EXPANDED ? 0 : form == CC_LATENT_ABSORBED || !expands ? 0x7fffffff : LT_FEW;
-        LtRuns runs{};
-        for (const PgSeq& s : plan->seqs) {
-            if (s.count == 0 || s.count > a.most) continue;
-            if (runs.n && runs.hi[runs.n - 1] == s.first) { runs.hi[runs.n - 1] = s.first + s.count; continue; }
-            if (runs.n == LT_RUNS) { runs.hi[runs.n - 1] = s.first + s.count; continue; }      // many runs: the last one takes all that lies behind (other tokens' results are overwritten)
-            runs.lo[runs.n] = s.first; runs.hi[runs.n++] = s.first + s.count;
-        }
-        for (int i = 0; i < runs.n; i++) { runs.tile0[i] = runs.tiles; runs.tiles += (runs.hi[i] - runs.lo[i] + LT_TOKENS - 1) / LT_TOKENS; }
-        rc = lr_run(dev, plan, a, runs);
+        rc = lr_run(dev, plan, a);
         if (!rc && a.most < 0x7fffffff) rc = tl_run(dev, plan, a);      // behind the others: their last products may run over tokens of these
     }
     if (rc) { cc_tensor_release(o); return rc; }

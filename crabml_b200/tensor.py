@@ -18,10 +18,12 @@ class TensorStrider:
     def __init__(self, shape, strides=None):
         self.shape = [int(s) for s in shape]
         if strides is None:
-            strides = [1]
-            for i in range(len(self.shape) - 1):
-                strides.append(strides[-1] * self.shape[len(self.shape) - i - 1])
-            strides = strides[::-1]
+            strides, n = [1] * max(1, len(self.shape)), 1
+            for i in range(len(self.shape) - 1, 0, -1):
+                n *= self.shape[i]
+                strides[i - 1] = n
+            self.strides = strides
+            return
         self.strides = [int(s) for s in strides]
 
     def clone(self): return TensorStrider(self.shape, self.strides)
@@ -77,7 +79,7 @@ class CudaTensorDevice:
         if rc != capi.CC_OK:
             raise CudaError(self.lib.cc_last_error(None).decode())
         self.handle = h
-        self.debug_named_tensors, self._lazy = debug_named_tensors, bool(lazy)
+        self.debug_named_tensors, self._lazy, self._stream = debug_named_tensors, bool(lazy), None
 
     def check(self, rc):
         if rc == capi.CC_OK:
@@ -91,7 +93,9 @@ class CudaTensorDevice:
 
     def stream(self) -> int:
         """the cudaStream_t on which all work of this device runs"""
-        return int(self.lib.cc_device_stream(self.handle))
+        if self._stream is None:
+            self._stream = int(self.lib.cc_device_stream(self.handle))
+        return self._stream
 
     # ---- sharded path: exchange window of this rank (comm.cu).  `exchange(bytes) -> [bytes of every rank]` is any
     # all-gather of small host blobs (torch.distributed.all_gather_object in bench.py / the tests) ----------------------------
@@ -166,6 +170,7 @@ class _Buf:
 
     def __init__(self, device, handle):
         self.device, self.handle = device, handle
+        self.dtype = self.data = None                              # asked for once: neither changes (data: on eager devices)
 
     def __del__(self):
         try:
@@ -183,12 +188,7 @@ class _Bits:
     def __init__(self, tensor):
         if not tensor.device.handle:
             raise CudaError("the tensor's device is closed")
-        tensor.device.flush()
-        shape, strider = tuple(tensor._strider.shape), tensor._strider
-        self.tensor = tensor
-        self.__cuda_array_interface__ = {
-            "shape": shape, "typestr": "<i2", "data": (0 if 0 in shape else tensor.device.lib.cc_tensor_data(tensor.buf.handle), False),
-            "strides": None if strider.is_contiguous() else tuple(2 * s for s in strider.strides), "stream": tensor.device.stream(), "version": 3}
+        self.tensor, self.__cuda_array_interface__ = tensor, tensor._array_of_type("<i2", 2)
 
 
 class CudaTensor:
@@ -222,13 +222,18 @@ class CudaTensor:
         kind, size = capi.ARRAY_TYPES.get(self.dtype(), (None, 0))
         if kind is None:
             raise AttributeError(f"a tensor of type {self.dtype()} is not a plain array")
-        self.device.flush()
-        shape = tuple(self._strider.shape)
-        array = {"shape": shape, "typestr": kind, "data": (0 if 0 in shape else self.device.lib.cc_tensor_data(self.buf.handle), False),
-                 "strides": None if self._strider.is_contiguous() else tuple(s * size for s in self._strider.strides), "stream": self.device.stream(), "version": 3}
+        array = self._array_of_type(kind, size)
         if not self.device._lazy:                                      # (eager: a buffer stays where it is, with all work on it queued)
             self._array, self._array_of = array, self._strider
         return dict(array)
+
+    def _array_of_type(self, kind, size):
+        shape, data = tuple(self._strider.shape), self.buf.data
+        if data is None or self.device._lazy:
+            self.device.flush()
+            data = self.buf.data = self.device.lib.cc_tensor_data(self.buf.handle)
+        return {"shape": shape, "typestr": kind, "data": (0 if 0 in shape else data, False),
+                "strides": None if self._strider.is_contiguous() else tuple(s * size for s in self._strider.strides), "stream": self.device.stream(), "version": 3}
 
     def bits(self):
         """The tensor's memory as whole numbers of 16 bits, for types that other libraries' array interfaces have no name for: torch.as_tensor(t.bits(), device="cuda").view(torch.bfloat16).
@@ -283,7 +288,10 @@ class CudaTensor:
         return cls(_Buf(device, h), TensorStrider([nrows, ncols]), device)
 
     # -- metadata (host side) ------------------------------------------------------------------------------
-    def dtype(self): return int(self.device.lib.cc_tensor_dtype(self.buf.handle))
+    def dtype(self):
+        if self.buf.dtype is None:
+            self.buf.dtype = int(self.device.lib.cc_tensor_dtype(self.buf.handle))
+        return self.buf.dtype
     def shape(self): return list(self._strider.shape)
     def strider(self): return self._strider
     def is_contiguous(self): return self._strider.is_contiguous()

@@ -346,3 +346,175 @@ def test_nothing(dev):
     y = paged.latent_attention(c.plan(), give(dev, c.a), 32, CudaTensor.alloc([0, 64], capi.F16, dev), 2, give(dev, np.ones((32, 32), np.float16)), give(dev, np.ones((64, 32), np.float16)), 1.0)
     assert y.shape() == [0, 64]
     assert paged.latent_append(c.plan(), give(dev, c.a), 32, CudaTensor.alloc([0, 48], capi.F32, dev), 0, q_src=CudaTensor.alloc([0, 64], capi.F32, dev), n_heads=2, dim=16).shape() == [0, 64]
+
+
+@pytest.mark.parametrize("dim,vdim,rest,rank", [(256, 16, 64, 512), (16, 256, 0, 512), (144, 208, 48, 496)])
+def test_wide_heads(dev, dim, vdim, rest, rank):
+    """heads that are not expanded"""
+    c = Case(dev, 64, rank, rest, [100, 31], [70, 1], seed=7)
+    check(dev, c, 3, dim, vdim, 1.2 * (dim + rest) ** -0.5)
+    with pytest.raises(TensorError):
+        check(dev, c, 3, dim, vdim, 0.1, form=capi.LATENT_EXPANDED)
+
+
+def test_tokens_by_portions(dev):
+    """absorbed: more tokens than the workspace holds queries of, one sequence across two portions, beside one that takes the other form in between"""
+    rank, rest, dim, vdim, H = 512, 64, 16, 16, 128
+    each = (256 << 20) // (H * (2 * rank + rest) * 4) // 32 * 32
+    counts = [each - 40, 1, 90]
+    c = Case(dev, 128, rank, rest, [0, 50, 7], counts, seed=2)
+    T = sum(counts)
+    q, uk, uv = ((c.rng.normal(size=s) * k).astype(np.float16) for s, k in (((T, H * (dim + rest)), 1.0), ((H * dim, rank), 0.05), ((H * vdim, rank), 0.05)))
+    y = attend(dev, c, q, uk, uv, H, 0.1, 0, None, capi.LATENT_ABSORBED).reshape(T, H, vdim)
+    at = 0
+    for i, n in enumerate(counts):
+        pick = sorted({0, n // 2, n - 1, *range(max(0, n - 60), n, 7), *range(0, min(n, 60), 9)})
+        for t in pick:
+            rows = c.rows(i, c.pos0[i] + t + 1)
+            want, _ = R.attention(rows, c.pos0[i] + t, q[at + t].reshape(1, H, -1), uk, uv, rank, H, 0.1)
+            np.testing.assert_allclose(y[at + t], want[0], rtol=0.02, atol=0.01)
+        at += n
+
+
+def test_far_pages(dev):
+    """pages whose numbers lie beyond 2^31 elements, in both forms and the append"""
+    P, rank, rest, H, dim, vdim = 128, 512, 64, 4, 32, 32
+    n_pages = (1 << 31) // (P * (rank + rest)) + 40
+    if torch.cuda.mem_get_info()[0] < 3 * n_pages * P * (rank + rest):
+        pytest.skip("no room")
+    pages = CudaTensor.alloc([n_pages, P, rank + rest], capi.F16, dev)
+    r = np.random.default_rng(0)
+    table, pos0, counts = [[n_pages - 1, 3, n_pages - 7], [n_pages - 20]], [300, 0], [3, 100]
+    rows = [r.normal(size=(p + n, rank + rest)).astype(np.float16) for p, n in zip(pos0, counts)]
+    t = view(pages)
+    dev.synchronize()
+    for i, x in enumerate(rows):
+        for b, page in enumerate(table[i]):
+            part = torch.from_numpy(x[b * P:(b + 1) * P]).cuda()
+            t[page, :len(part)] = part
+    T = sum(counts)
+    plan = paged.PagePlan(dev, P, n_pages, table, pos0, counts)
+    src = r.normal(size=(T, rank + rest)).astype(np.float32)
+    torch.cuda.synchronize()
+    paged.latent_append(plan, pages, rank, give(dev, src), 0, eps=1e-6)
+    dev.synchronize()
+    new, at = R.f16(R.row(src, rank, None, 1e-6, np.zeros(T), [], 0, 1.0)), 0
+    for i, n in enumerate(counts):
+        got = np.concatenate([t[page].cpu().numpy() for page in table[i]])[pos0[i]:pos0[i] + n]
+        near16(got, new[at:at + n].astype(np.float64), 2.0)
+        rows[i][pos0[i]:] = got
+        at += n
+    q, uk, uv = ((r.normal(size=s) * k).astype(np.float16) for s, k in (((T, H * (dim + rest)), 1.0), ((H * dim, rank), 0.05), ((H * vdim, rank), 0.05)))
+    for form in FORMS.values():
+        y = take(dev, paged.latent_attention(plan, pages, rank, give(dev, q), H, give(dev, uk), give(dev, uv), 0.1, form=form)).reshape(T, H, vdim)
+        at = 0
+        for i, n in enumerate(counts):
+            want, _ = R.attention(rows[i], pos0[i], q[at:at + n].reshape(n, H, -1), uk, uv, rank, H, 0.1)
+            np.testing.assert_allclose(y[at:at + n], want, rtol=0.02, atol=0.01)
+            at += n
+
+
+@pytest.mark.parametrize("n", [1, 2, 150, 700])
+def test_many_sequences(dev, n):
+    """as many sequences as take several looks to find, most of them short; tokens of both forms by turns, more runs of them than a call lists"""
+    r = np.random.default_rng(n)
+    counts = [int(x) for x in r.choice([0, 1, 1, 2, 70], size=n)]
+    c = Case(dev, 16, 32, 16, [int(x) for x in r.integers(0, 60, size=n)], counts, seed=n)
+    check(dev, c, 3, 16, 16, 0.25)
+
+
+def test_two_devices_at_once(dev):
+    """two handles with streams of their own, calls by turns from two threads"""
+    import threading
+    other = make_device()
+    wrong = []
+
+    def work(d, seed):
+        try:
+            for k in range(3):
+                c = Case(d, 32, 64, 32, [200, 5, 1000], [1, 80, 1], seed=seed + k)
+                check(d, c, 8, 32, 32, 0.15)
+        except Exception as e:                                               # told by the thread that started this one
+            wrong.append(e)
+    threads = [threading.Thread(target=work, args=(d, i)) for i, d in enumerate((dev, other))]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    other.close()
+    assert not wrong, wrong
+
+
+def test_refusals(dev):
+    P, rank, rest, H, dim, vdim = 16, 32, 16, 2, 16, 16
+    c = Case(dev, P, rank, rest, [5], [3])
+    plan, pages = c.plan(), give(dev, c.a)
+    z = lambda *s, t=np.float16: give(dev, np.zeros(s, t))  # noqa: E731
+    q, uk, uv, src = z(3, H * (dim + rest)), z(H * dim, rank), z(H * vdim, rank), z(3, 100, t=np.float32)
+    other = make_device()
+    attention = lambda **k: paged.latent_attention(**{**dict(plan=plan, pages=pages, rank=rank, q=q, n_heads=H, uk=uk, uv=uv, scale=1.0), **k})  # noqa: E731
+    append = lambda **k: paged.latent_append(**{**dict(plan=plan, pages=pages, rank=rank, kv_src=src, kv_col0=0, q_src=src, q_col0=36, n_heads=2, dim=16), **k})  # noqa: E731
+    attention(), append()
+    for f in (attention, append):
+        for bad in (dict(rank=33), dict(rank=0), dict(rank=-16), dict(rank=48 + 16), dict(pages=z(c.n_pages, P, rank + rest, t=np.float32)), dict(pages=z(c.n_pages - 1, P, rank + rest)),
+                    dict(pages=z(c.n_pages, 2 * P, rank + rest)), dict(pages=z(c.n_pages * P, rank + rest)), dict(n_heads=0), dict(n_heads=8193), dict(rank=2 ** 40), dict(n_heads="2"),
+                    dict(pages=z(c.n_pages, P, 40), rank=32), dict(pages=z(c.n_pages, P, 640), rank=512), dict(pages=z(c.n_pages, P, 544), rank=528)):
+            with pytest.raises(TensorError):
+                f(**bad)
+    for bad in (dict(q=z(2, H * (dim + rest))), dict(q=z(3, H * (dim + rest) + 1)), dict(q=z(3, H * (dim + rest), t=np.float32)), dict(n_heads=3), dict(uk=z(H * dim, rank + 1)), dict(uk=z(H * dim + 1, rank)),
+                dict(uk=z(H * 8, rank)), dict(uv=z(H * 272, rank)), dict(uv=z(H * vdim, rank, t=np.float32)), dict(sink=z(H + 1, t=np.float32)), dict(sink=z(H)), dict(form=3), dict(form=-1), dict(out_type=capi.F32),
+                dict(q=q.with_strider(TensorStrider([3, H * (dim + rest)], [1, 3]))), dict(window=2 ** 31), dict(uk=give(other, np.zeros((H * dim, rank), np.float16)))):
+        with pytest.raises(TensorError):
+            attention(**bad)
+    for bad in (dict(kv_src=z(2, 100, t=np.float32)), dict(kv_col0=-1), dict(kv_col0=53), dict(q_col0=37), dict(q_col0=-1), dict(dim=8), dict(dim=272), dict(pairing=2), dict(norm_w=z(rank)), dict(norm_w=z(rank + 1, t=np.float32)),
+                dict(freq=z(9, t=np.float32)), dict(freq=z(4)), dict(kv_src=src.with_strider(TensorStrider([3, 100], [99, 1]))), dict(kv_src=src.with_strider(TensorStrider([3, 100], [101, 1]))),
+                dict(kv_src=pages.reshape([c.n_pages * P, rank + rest])), dict(q_src=z(4, 100, t=np.float32)), dict(kv_src=give(other, np.zeros((3, 100), np.float32)))):
+        with pytest.raises(TensorError):
+            append(**bad)
+    with pytest.raises(TensorError):
+        attention(pages=give(other, c.a))
+    with pytest.raises(TensorError):
+        attention(plan=paged.PagePlan(other, P, c.n_pages, c.table, c.pos0, c.counts))
+    lazy = make_device(lazy=True)
+    with pytest.raises((TensorError, CudaError)):
+        paged.PagePlan(lazy, P, c.n_pages, c.table, c.pos0, c.counts)
+    lazy.close()
+    other.close()
+    attention(), append()
+
+
+def test_a_layer(dev):
+    """what a program does in a step: products with their epilogue, the append, the attention and the product back into the residual stream; a prompt in portions and then single tokens for
+    two sequences, beside each whole sequence in 64 bits"""
+    from crabml_b200 import seqops
+    P, width, H, dim, rest, vdim, rank = 32, 192, 4, 32, 16, 32, 64
+    r = np.random.default_rng(11)
+    cols = H * (dim + rest) + rank + rest
+    w = {n: (r.normal(size=s) * s[1] ** -0.5).astype(np.float16) for n, s in (("in", (cols, width)), ("uk", (H * dim, rank)), ("uv", (H * vdim, rank)), ("out", (width, H * vdim)))}
+    bias, norm, f = (0.3 * r.normal(size=cols)).astype(np.float32), (1.0 + 0.2 * r.normal(size=rank)).astype(np.float32), freqs(rest // 2)
+    d = {n: give(dev, x) for n, x in w.items()}
+    db, dn, df = give(dev, bias), give(dev, norm), give(dev, f)
+    scale, steps = (dim + rest) ** -0.5, [(70, 3), (1, 90), (65, 0), (1, 1), (1, 1), (0, 4)]
+    x = [r.normal(size=(sum(s[i] for s in steps), width)).astype(np.float32) for i in range(2)]
+    table = [[4, 1, 6, 9, 2], [0, 8, 3, 5]]
+    pages, have, got = give(dev, np.full((10, P, rank + rest), np.nan, np.float16)), [0, 0], [[], []]
+    for step in steps:
+        plan = paged.PagePlan(dev, P, 10, table, have, step)
+        h = give(dev, np.concatenate([x[i][have[i]:have[i] + n] for i, n in enumerate(step)]))
+        qkv = seqops.product(d["in"], h, bias=db, out_type=capi.F16)
+        q = paged.latent_append(plan, pages, rank, qkv, H * (dim + rest), norm_w=dn, eps=1e-5, q_src=qkv, n_heads=H, dim=dim, freq=df)
+        y = paged.latent_attention(plan, pages, rank, q, H, d["uk"], d["uv"], scale, out_type=capi.F16)
+        o = take(dev, seqops.product(d["out"], y, residual=h, out_type=capi.F32))
+        at = 0
+        for i, n in enumerate(step):
+            got[i].append(o[at:at + n])
+            have[i] += n
+            at += n
+    for i in range(2):
+        n = have[i]
+        qkv = x[i].astype(np.float16).astype(np.float64) @ w["in"].astype(np.float64).T + bias
+        q = qkv[:, :H * (dim + rest)].reshape(n, H, -1).copy()
+        q[..., dim:] = R.turn(q[..., dim:], np.arange(n), f, 0, 1.0)
+        rows = R.row(qkv[:, H * (dim + rest):], rank, norm, 1e-5, np.arange(n), f, 0, 1.0)
+        y, _ = R.attention(rows, 0, q, w["uk"], w["uv"], rank, H, scale)
+        want = x[i] + y.reshape(n, -1) @ w["out"].astype(np.float64).T
+        # five roundings to 16 bits, 2^-11 of numbers of size 1 each, and a sum of 128 of them with weights of 128^-1/2
+        assert np.abs(np.concatenate(got[i]) - want).max() < 5 * 2.0 ** -11 * 6
