@@ -118,6 +118,7 @@ struct cc_device {
     std::string last_error;
     uint64_t launches = 0;
     int sm_count = 148;
+    int clusters[2] = {0, 0};                 // of 4 and of 8 CTAs, an SM each, that run at a time; 0: not asked yet
 
     // f16 LUTs (cpu_device.rs:108-124), computed on the host with libm and uploaded
     uint16_t* exp_lut = nullptr;

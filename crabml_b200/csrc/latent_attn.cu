@@ -760,7 +760,11 @@ static int lr_run(cc_device* dev, const cc_page_plan* plan, LrArgs a) {
 }
 #include "latent_tile.cuh"
 
-#define LT_FEW 64                             // new tokens of a sequence; with more its keys and values are laid out
+// New tokens of a sequence; with more its keys and values are laid out.  us, absorbed / expanded, of 8, 16, 24, 32, 64 tokens of one sequence:
+// 16 heads of 128, rank 512, behind 1000 rows: 27 / 37, 29 / 37, 30 / 37, 34 / 42, 42 / 42; behind 8000: 34 / 77, 53 / 76, 63 / 76, 79 / 76, 133 / 77; behind 32000: 75 / 228, 131 / 229, 183 / 228, 236 / 229, 446 / 227;
+// 32 heads of 64, rank 512, behind 8000: 53 / 104, 75 / 104, 105 / 102, 131 / 102, 243 / 103; of 8 sequences behind 1000: 60 / 103, 91 / 103, 130 / 104, 168 / 110, 324 / 111;
+// 64 heads of 128, rank 512, 16 sequences behind 3000: 392 / 1734, 772 / 1736, 1145 / 1736, 1518 / 1734, 3041 / 1736
+#define LT_FEW 24
 
 extern "C" CC_API int cc_paged_latent_attention(cc_device* dev, const cc_page_plan* plan, const cc_view* pages, int32_t rank, const cc_view* q, int32_t H, const cc_view* uk,
                                                 const cc_view* uv, float scale, int32_t window, const cc_view* sink, int32_t form, int32_t out_type, cc_buf** out) {

@@ -31,12 +31,13 @@ static_assert(TL_SOFT * 32 * TL_REGS_SOFT + 128 * TL_REGS_REST <= TL_THREADS * T
 #define TL_LAG 8.0f
 #define TL_O 256                              // TMEM columns: S (and P) of the tiles at 0 and 128, O behind
 #define TL_DIM 128                            // largest dim and vdim
-#define TL_SFU 16                             // of 16 weights those that the special function unit makes
 
 struct TlArgs {
     LrArgs a;
     uint8_t *k_image, *v_image;               // [key tile][head of this launch][block]
-    int head0, heads, key_tiles, items;
+    int head0, heads, key_tiles, piece;       // piece: steps, about, of what an item is cut into; 0: none is cut
+    float* part;                              // sums of pieces [piece][head][2 TL_ROWS][vdim]
+    float2* ml;                               // [piece][head][2 TL_ROWS]: base, sum of weights
 };
 // keys count from a multiple of 128, so that a tile is whole pages
 __host__ __device__ __forceinline__ void tl_range(const PgSeq& s, const LrArgs& a, int* from, int* to) {
@@ -50,6 +51,25 @@ __host__ __device__ __forceinline__ int tl_key_tiles(const PgSeq& s, const LrArg
     return (to - from + TL_KEYS - 1) / TL_KEYS;
 }
 __host__ __device__ __forceinline__ int tl_items(const PgSeq& s, const LrArgs& a) { return s.count <= a.most ? 0 : (s.count + 2 * TL_ROWS - 1) / (2 * TL_ROWS); }
+// steps of an item's two tiles: keys that one of its rows sees, from `lo` for both
+__host__ __device__ __forceinline__ void tl_steps(const PgSeq& s, const LrArgs& a, int row0, int* lo, int steps[2]) {
+    int from, to;
+    tl_range(s, a, &from, &to);
+    const int first = a.window > 0 ? (s.pos0 + row0 - a.window + 1) & ~(TL_KEYS - 1) : from;
+    *lo = first > from ? first : from;
+    for (int i = 0; i < 2; i++) {
+        const int end = s.count < row0 + (i + 1) * TL_ROWS ? s.count : row0 + (i + 1) * TL_ROWS;
+        steps[i] = row0 + i * TL_ROWS < s.count ? (s.pos0 + end - *lo + TL_KEYS - 1) / TL_KEYS : 0;
+    }
+}
+// pieces of each item of a sequence: as its last one, which sees most
+__host__ __device__ __forceinline__ int tl_pieces(const PgSeq& s, const TlArgs& t) {
+    if (!t.piece || s.count <= t.a.most) return 1;
+    int lo, steps[2];
+    tl_steps(s, t.a, (tl_items(s, t.a) - 1) * 2 * TL_ROWS, &lo, steps);
+    const int most = steps[0] > steps[1] ? steps[0] : steps[1], n = most / t.piece;
+    return n > 1 ? n : 1;
+}
 // the place of number n in the sequences' counts: every lane gets the sequence and what is left of n
 template <class Count>
 __device__ __forceinline__ int tl_find(const LrArgs& a, int n, Count count, int* rest) {
@@ -354,21 +374,7 @@ __device__ __forceinline__ float tl_max3(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// 2^x of a pair by multiply-adds: x = n + r with |r| <= 1/2 by way of a number whose last place is 1; 2^r by its series up to r^5 (the first term left out is 2^-19 at |r| = 1/2, far below
-// the weights' 2^-11), n into the exponent.  What is below -126 counts as -126
-__device__ __forceinline__ tl_f2 tl_exp2_pair(float2 x) {
-    const tl_f2 big = tl_two(12582912.0f, 12582912.0f), minus = tl_two(-1.0f, -1.0f);
-    const tl_f2 v = tl_two(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f)), u = tl_add2(v, big), n = tl_add2(u, tl_two(-12582912.0f, -12582912.0f)), r = tl_fma2(n, minus, v);
-    tl_f2 p = tl_two(1.3333558e-3f, 1.3333558e-3f);                  // (ln 2)^i / i!, i = 5 .. 0
-    p = tl_fma2(p, r, tl_two(9.6181291e-3f, 9.6181291e-3f));
-    p = tl_fma2(p, r, tl_two(5.5504109e-2f, 5.5504109e-2f));
-    p = tl_fma2(p, r, tl_two(2.4022651e-1f, 2.4022651e-1f));
-    p = tl_fma2(p, r, tl_two(6.9314718e-1f, 6.9314718e-1f));
-    p = tl_fma2(p, r, tl_two(1.0f, 1.0f));
-    const float2 q = tl_one(p), m = tl_one(u);
-    return tl_two(__uint_as_float(__float_as_uint(q.x) + (__float_as_uint(m.x) << 23)), __uint_as_float(__float_as_uint(q.y) + (__float_as_uint(m.y) << 23)));
-}
-// grid: items x heads, heads fastest
+// grid: pieces of items x heads, heads fastest
 __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ TlArgs t, unsigned* err_dev,
                                                                     unsigned* err_host) {
     extern __shared__ __align__(1024) uint8_t tl_raw[];
@@ -395,18 +401,23 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
     const unsigned tmem = sh.tmem_base;
     pdl_enter();
     int rest;
-    const int seq = max(0, tl_find(a, item, [&](const PgSeq& s) { return tl_items(s, a); }, &rest));
+    const int seq = max(0, tl_find(a, item, [&](const PgSeq& s) { return tl_items(s, a) * tl_pieces(s, t); }, &rest));
     const PgSeq s = a.seqs[seq];
-    const int row0 = (tl_items(s, a) - 1 - rest) * 2 * TL_ROWS;      // late rows, which see most, first
-    int from, to, before = 0;
+    const int pieces = tl_pieces(s, t), piece = rest % pieces, row0 = (tl_items(s, a) - 1 - rest / pieces) * 2 * TL_ROWS;      // late rows, which see most, first
+    int from, to, before = 0, slot = 0, lo, steps_of[2];
     tl_range(s, a, &from, &to);
-    for (int x = lane; x < seq; x += 32) before += tl_key_tiles(a.seqs[x], a);
+    for (int x = lane; x < seq; x += 32) {
+        const PgSeq o = a.seqs[x];
+        before += tl_key_tiles(o, a);
+        if (t.piece) { const int n = tl_pieces(o, t); slot += n > 1 ? n * tl_items(o, a) : 0; }
+    }
     before = warp_sum_i(before);
-    // the steps of a tile: keys that one of its rows sees, from `lo` for both
-    auto last = [&](int i) { return min(s.count, row0 + (i + 1) * TL_ROWS) - 1; };
-    const int lo = a.window > 0 ? max(from, (s.pos0 + row0 - a.window + 1) & ~(TL_KEYS - 1)) : from;
-    auto steps_of = [&](int i) { return row0 + i * TL_ROWS < s.count ? (s.pos0 + last(i) + 1 - lo + TL_KEYS - 1) / TL_KEYS : 0; };
-    const int steps0 = steps_of(0), steps1 = steps_of(1), steps = max(steps0, steps1), kt0 = before + (lo - from) / TL_KEYS, per = nb + rb + vb;
+    slot = warp_sum_i(slot) + rest;
+    tl_steps(s, a, row0, &lo, steps_of);
+    // this piece's steps of them
+    const int each = (max(steps_of[0], steps_of[1]) + pieces - 1) / pieces, off = piece * each, steps0 = max(0, min(steps_of[0] - off, each)), steps1 = max(0, min(steps_of[1] - off, each));
+    const int steps = max(steps0, steps1), kt0 = before + (lo - from) / TL_KEYS + off, per = nb + rb + vb;
+    lo += off * TL_KEYS;
     if (warp >= TL_SOFT) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TL_REGS_REST));
         if (warp == TL_SOFT) {
@@ -536,7 +547,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
         // ===== weights: two threads a row, 64 keys of a step each =====
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TL_REGS_SOFT));
         const int i = warp >> 3, half = (warp >> 2) & 1, in_tile = (warp & 3) * 32 + lane, row = row0 + i * TL_ROWS + in_tile, mine = i ? steps1 : steps0;
-        const int pos = s.pos0 + row, key_lo = a.window > 0 ? pos - a.window + 1 : 0, pos_first = s.pos0 + row0 + i * TL_ROWS, pos_last = s.pos0 + last(i);
+        const int pos = s.pos0 + row, key_lo = a.window > 0 ? pos - a.window + 1 : 0, pos_first = s.pos0 + row0 + i * TL_ROWS, pos_last = s.pos0 + min(s.count, row0 + (i + 1) * TL_ROWS) - 1;
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, st = tmem + lanes + i * 128, ot = tmem + lanes + TL_O + i * 128;
         const float f = a.scale * LR_LOG2E;
         float base = -INFINITY, l = 0.0f;
@@ -619,7 +630,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
 #pragma unroll
                 for (int c = 0; c < 16; c += 2) {
                     const float2 y = tl_one(tl_fma2(tl_two(__uint_as_float(x[g + c]), __uint_as_float(x[g + c + 1])), ff2, minus2));
-                    const tl_f2 p = c >= TL_SFU ? tl_exp2_pair(y) : tl_two(lt_exp2(y.x), lt_exp2(y.y));
+                    const tl_f2 p = tl_two(lt_exp2(y.x), lt_exp2(y.y));
                     if (c & 2) more = tl_add2(more, p);
                     else sum = tl_add2(sum, p);
                     const float2 z = tl_one(p);
@@ -640,6 +651,8 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
             tl_sync(1 + i);
             l = sh.top[i][in_tile];
         }
+        const int64_t at = ((int64_t)slot * t.heads + head_at) * (2 * TL_ROWS) + i * TL_ROWS + in_tile;
+        if (pieces > 1 && !half) t.ml[at] = make_float2(base, l);
         if (mine > 0 && ok && (ok = tl_wait_warp(pg_smem(&sh.o_full[i]), (mine - 1) & 1, &sh.fail))) {
             pg_fence_after();
             float g = 1.0f, total = l;
@@ -657,6 +670,11 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
                 for (int j = 0; j < 16; j++) asm volatile("" : "+r"(v[j]));
+                if (pieces > 1) {
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) *(uint4*)(t.part + at * a.vdim + c + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                    continue;
+                }
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const float u = __uint_as_float(v[2 * j]) * by, z = __uint_as_float(v[2 * j + 1]) * by;
@@ -675,6 +693,45 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
     tl_report(sh.fail, err_dev, err_host);
 }
 
+// the pieces of an item's rows: a warp a row and head.  grid (tokens' rows by 8, heads of the launch)
+__global__ void __launch_bounds__(256) latent_tile_join_kernel(const __grid_constant__ TlArgs t) {
+    const LrArgs& a = t.a;
+    const int lane = threadIdx.x & 31, head_at = blockIdx.y;
+    pdl_enter();
+    int rest, slot = 0;                                              // blocks: those of each cut sequence's tokens, by 8
+    const int seq = tl_find(a, blockIdx.x, [&](const PgSeq& s) { return tl_pieces(s, t) > 1 ? (s.count + 7) / 8 : 0; }, &rest);
+    if (seq < 0) return;
+    const PgSeq s = a.seqs[seq];
+    for (int x = lane; x < seq; x += 32) { const int n = tl_pieces(a.seqs[x], t); slot += n > 1 ? n * tl_items(a.seqs[x], a) : 0; }
+    slot = warp_sum_i(slot);
+    const int row = rest * 8 + (threadIdx.x >> 5), pieces = tl_pieces(s, t), item = row / (2 * TL_ROWS);
+    if (row >= s.count) return;
+    const int64_t at = ((int64_t)(slot + (tl_items(s, a) - 1 - item) * pieces) * t.heads + head_at) * (2 * TL_ROWS) + row % (2 * TL_ROWS), stride = (int64_t)t.heads * 2 * TL_ROWS;
+    const float sk = a.sink ? a.sink[t.head0 + head_at] * LR_LOG2E : -INFINITY;
+    float m = sk;
+    bool none = false;                                               // a score that is none
+    for (int p = 0; p < pieces; p++) { const float b = t.ml[at + p * stride].x; none |= b != b; m = fmaxf(m, b); }
+    float total = sk == -INFINITY ? 0.0f : exp2f(sk - m);
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int p = 0; p < pieces; p++) {
+        const float2 ml = t.ml[at + p * stride];
+        if (ml.x == -INFINITY) continue;                              // nothing of its keys is seen: it may have left no sums
+        const float w = exp2f(ml.x - m);
+        total = fmaf(w, ml.y, total);
+        if (lane * 4 < a.vdim) {
+            const float4 v = *(const float4*)(t.part + (at + p * stride) * a.vdim + lane * 4);
+            o.x = fmaf(w, v.x, o.x); o.y = fmaf(w, v.y, o.y); o.z = fmaf(w, v.z, o.z); o.w = fmaf(w, v.w, o.w);
+        }
+    }
+    if (lane * 4 >= a.vdim) return;
+    const float by = none ? NAN : 1.0f / total;
+    uint16_t* out = (uint16_t*)a.out + ((int64_t)(s.first + row) * a.H + t.head0 + head_at) * a.vdim + lane * 4;
+    *(uint2*)out = a.out_bf16 ? make_uint2(ht_pack_bf16(o.x * by, o.y * by), ht_pack_bf16(o.z * by, o.w * by)) : make_uint2(ht_pack_f16(o.x * by, o.y * by), ht_pack_f16(o.z * by, o.w * by));
+}
+
+#define TL_PIECE 6                            // steps of a piece, at least
+#define TL_GAIN 16                            // steps that cutting has to save
 #define TL_WORKSPACE ((int64_t)256 << 20)     // bytes of images that a call has at a time, as long as those of one sequence and head are no more
 static int tl_run(cc_device* dev, const cc_page_plan* plan, const LrArgs& all) {
     const int64_t per = (int64_t)((all.dim + 63) / 64 + (all.vdim + 63) / 64) * TL_BLOCK, width = all.dim + all.rest;
@@ -691,27 +748,45 @@ static int tl_run(cc_device* dev, const cc_page_plan* plan, const LrArgs& all) {
     for (int first = 0, end; first < plan->n_seqs; first = end) {
         TlArgs t{};
         t.a = all;
-        int64_t tiles = 0, items = 0;
+        int64_t tiles = 0, steps = 0, longest = 0;
         for (end = first; end < plan->n_seqs; end++) {
-            const int n = tl_key_tiles(plan->seqs[end], all);
+            const PgSeq& s = plan->seqs[end];
+            const int n = tl_key_tiles(s, all);
             if (tiles && (tiles + n) * per > TL_WORKSPACE) break;
-            tiles += n; items += tl_items(plan->seqs[end], all);
+            tiles += n;
+            for (int i = tl_items(s, all) - 1; i >= 0; i--) {
+                int lo, each[2];
+                tl_steps(s, all, i * 2 * TL_ROWS, &lo, each);
+                steps += std::max(each[0], each[1]); longest = std::max<int64_t>(longest, std::max(each[0], each[1]));
+            }
         }
-        if (!items) continue;
+        if (!tiles) continue;
         t.a.seqs = plan->d_seqs + first; t.a.n_seqs = end - first; t.a.table = plan->d_table + (int64_t)first * all.table_cols;
         const int heads = (int)std::max<int64_t>(1, std::min<int64_t>(all.H, TL_WORKSPACE / (tiles * per)));
+        const int64_t share = std::max<int64_t>(TL_PIECE, (steps * heads + dev->sm_count - 1) / dev->sm_count);
+        if (longest >= share + TL_GAIN) t.piece = (int)share;
+        int64_t items = 0, cut = 0, rows8 = 0;
+        for (int i = first; i < end; i++) {
+            const PgSeq& s = plan->seqs[i];
+            const int64_t n = tl_pieces(s, t), mine = n * tl_items(s, all);
+            items += mine;
+            if (n > 1) { cut += mine; rows8 += (s.count + 7) / 8; }
+        }
         CC_REQUIRE(dev, items * heads < ((int64_t)1 << 31) && tiles < ((int64_t)1 << 31), "paged_latent_attention: too many rows");
+        const int64_t images = tiles * heads * per, sums = cut * heads * 2 * TL_ROWS;
         void* ws = nullptr; size_t cls = 0;
-        rc = cc_pool_alloc(dev, (size_t)(tiles * heads * per), &ws, &cls);
+        rc = cc_pool_alloc(dev, (size_t)(images + sums * (all.vdim * 4 + 8)), &ws, &cls);
         if (rc) return rc;
+        t.part = (float*)((uint8_t*)ws + images); t.ml = (float2*)(t.part + sums * all.vdim);
         t.k_image = (uint8_t*)ws; t.v_image = t.k_image + tiles * heads * ((all.dim + 63) / 64) * TL_BLOCK;
-        t.key_tiles = (int)tiles; t.items = (int)items;
+        t.key_tiles = (int)tiles;
         cudaError_t e = cudaSuccess;
         for (t.head0 = 0; t.head0 < all.H && e == cudaSuccess; t.head0 += heads) {
             t.heads = std::min(heads, all.H - t.head0);
             const int runs = (int)std::max<int64_t>(1, std::min<int64_t>(t.heads, dev->sm_count / (tiles + 1)));
             e = cc_launch_pdl(dev, latent_expand_kernel, dim3((unsigned)(tiles + 1) / 2 * 2, (unsigned)runs), TE_THREADS, TE_SMEM, rows, uk, uv, t, dev->err_dev, dev->err_host);
             if (e == cudaSuccess) e = cc_launch_pdl(dev, latent_tile_kernel, (unsigned)(items * t.heads), TL_THREADS, TL_SMEM, rows, q, t, dev->err_dev, dev->err_host);
+            if (cut && e == cudaSuccess) { e = cc_launch_pdl(dev, latent_tile_join_kernel, dim3((unsigned)rows8, (unsigned)t.heads), 256, 0, t); dev->launches++; }
             dev->launches += 2;
         }
         cc_pool_free(dev, ws, cls);

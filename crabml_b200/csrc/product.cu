@@ -2,7 +2,7 @@
 //
 // Few rows (product_few_kernel): every weight is read once, so memory bounds it.  mma.sync.m16n8k16 with 16 rows of W as its first operand and 8 rows of x as the second: a lane takes
 // 16 neighbouring bytes of a row of W straight into registers, and of a row of x from shared memory.  Which eight k a lane puts into two steps is free as long as both operands agree, so
-// nothing is rearranged.  8 warps share the depth of 16 rows of W; their sums meet in shared memory, where bias, activation and residual follow.
+// nothing is rearranged.  16 warps share the depth of 16 rows of W; their sums meet in shared memory, where bias, activation and residual follow.
 #include <algorithm>
 
 #include "act.cuh"
@@ -14,7 +14,7 @@ struct PrArgs {
     const float* bias;
     void* out;
     int64_t x_stride, res_stride;
-    int m, k, rows, x_type, out_type, act, chunk;
+    int m, k, rows, x_type, out_type, act;
     bool x_vec, w_vec;                        // rows start at multiples of 16 bytes
 };
 __device__ __forceinline__ float pr_finish(const PrArgs& a, float v, int row, int col) {
@@ -41,48 +41,50 @@ __device__ __forceinline__ uint4 pr_pack8(const float (&v)[8]) {
 #define PF_WARPS 16
 #define PF_THREADS (PF_WARPS * 32)
 #define PF_AHEAD 4                            // runs of 32 k that a warp has under way: 64 KB an SM
-#define PF_SMEM (200 * 1024)
-#define PF_ROWS 32                            // rows of x; more go to the tensor cores' tiles,
-#define PF_ROOM (90 * 1024)                   // .. and so do those whose numbers shared memory does not hold
+#define PF_ROWS 16
+#define PF_ALONE (96 * 1024)
+#define PF_ROOM (32 * 1024)
+#define PF_ROOM_ODD (16 * 1024)
+// Whether rows of x are few.  More, or longer ones, take tiles on the tensor cores, where an instruction takes all of x instead of 8 rows.  us, few / tiles, weights of 16-bit numbers:
+// 4096 x 4096 with 1, 4, 8, 16 rows: 9.7 / 11.9, 10.7 / 12.0, 12.0 / 12.1, 15.1 / 12.3; 11008 x 4096 with 2, 16: 20.0 / 22.6, 25.1 / 21.8; 4096 x 14336 with 4: 27.0 / 24.7; 1024 x 1024 with 16: 6 / 7.7;
+// 4096 x 1024 with 32: 9.9 / 9.0.  Rows of weights that start anywhere are read number by number here and laid out for the tiles: 1024 x 1023 with 16: 8.8 / 14.5; 4096 x 4095 with 2, 8: 39.5 / 38.7,
+// 48.7 / 38.8; 4096 x 14335 with 1, 4: 98.7 / 76.2, 107 / 76.5
+static bool pr_few(int64_t rows, int64_t k, bool w_vec) {
+    return rows <= PF_ROWS && rows * k <= (!w_vec ? PF_ROOM_ODD : rows == 1 ? PF_ALONE : PF_ROOM);
+}
 // 8 numbers of a row from column c on, zeros behind its end
-__device__ __forceinline__ uint4 pf_weights(const uint16_t* row, int c, int k, bool there, bool vec) {
+__device__ __forceinline__ uint4 pf_weights(const uint16_t* row, int c, int k, bool there) {
     if (!there || c >= k) return make_uint4(0, 0, 0, 0);
-    if (vec) {
-        const int4 v = ld_stream_16(row + c);
-        return make_uint4((unsigned)v.x, (unsigned)v.y, (unsigned)v.z, (unsigned)v.w);
-    }
     unsigned u[4] = {};
 #pragma unroll
     for (int j = 0; j < 8; j++)
         if (c + j < k) u[j >> 1] |= (unsigned)row[c + j] << (j & 1) * 16;
     return make_uint4(u[0], u[1], u[2], u[3]);
 }
-// rows of x into shared memory as 16-bit numbers: their k from k0 on, zeros behind the end of the last run
+// rows of x into shared memory as 16-bit numbers, zeros behind the end of the last run
 template <bool BF16>
-__device__ __forceinline__ void pf_stage(const PrArgs& a, uint8_t* to, int pitch, int k0, int runs) {
+__device__ __forceinline__ void pf_stage(const PrArgs& a, uint8_t* to, int pitch, int runs) {
     for (int e = threadIdx.x; e < a.rows * runs * 4; e += PF_THREADS) {
         const int r = e / (runs * 4), col = e % (runs * 4) * 8;
         float x[8] = {};
-        if (k0 + col < a.k) {
-            const int64_t at = (int64_t)r * a.x_stride + k0 + col;
-            if (k0 + col + 8 <= a.k) ht_read8(a.x, at, a.x_type, a.x_vec, x);
-            else
+        const int64_t at = (int64_t)r * a.x_stride + col;
+        if (col + 8 <= a.k) ht_read8(a.x, at, a.x_type, a.x_vec, x);
+        else
 #pragma unroll
-                for (int j = 0; j < 8; j++)
-                    if (k0 + col + j < a.k) x[j] = ht_read(a.x, at + j, a.x_type);
-        }
+            for (int j = 0; j < 8; j++)
+                if (col + j < a.k) x[j] = ht_read(a.x, at + j, a.x_type);
         *(uint4*)(to + r * pitch + col * 2) = pr_pack8<BF16>(x);
     }
 }
 // A CTA walks over the tiles of 16 rows of W blockIdx.x, + gridDim.x, ..; its warps take a tile's runs of 32 k by turns.
-// WHOLE (rows of W at multiples of 16 bytes, all k of x in shared memory): four runs of a warp are computed while the next four, also of the next tile, are under way: 64 KB an SM and more.
-// Else, k of any size: x lies in shared memory a portion (`chunk`) at a time, laid out again for every tile, weights number by number where their rows start anywhere
+// WHOLE (rows of W at multiples of 16 bytes): four runs of a warp are computed while the next four, also of the next tile, are under way: 64 KB an SM and more.  Else weights are read number by
+// number
+__host__ __device__ constexpr int pf_pitch(int k) { return (k + 63) / 64 * 128 + 64; }      // eight lanes' 16 bytes: two rows, 64 bytes each, in all banks
 template <int NT, bool BF16, bool WHOLE>
 __global__ void __launch_bounds__(PF_THREADS, 1) product_few_kernel(const __grid_constant__ PrArgs a) {
     extern __shared__ __align__(16) uint8_t pf_raw[];
-    constexpr int BUFFERS = NT == 4 ? 1 : 2;
-    __shared__ float sums[BUFFERS][PF_WARPS][16][NT * 8 + 1];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, pitch = a.chunk * 2 + 64;      // eight lanes' 16 bytes: two rows, 64 bytes each, in all banks
+    __shared__ float sums[2][PF_WARPS][16][NT * 8 + 1];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, pitch = pf_pitch(a.k);
     const int tiles = (a.m + 15) >> 4, all = (a.k + 31) >> 5, mine = (all - warp + PF_WARPS - 1) / PF_WARPS;      // runs of a tile, and this warp's
     const uint8_t* x_lane = pf_raw + min(lane >> 2, a.rows - 1) * pitch + (lane & 3) * 16;        // rows behind the last one: any, no one reads their sums
     int z = 0;
@@ -99,8 +101,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) product_few_kernel(const __grid
             for (int w = 0; w < PF_WARPS; w++) s += sums[z][w][i][n];
             if (col < a.m) ht_write(a.out, (int64_t)n * a.m + col, a.out_type, pr_finish(a, s, n, col));
         }
-        if (BUFFERS == 1) __syncthreads();
-        z = (z + 1) % BUFFERS;
+        z ^= 1;
     };
     auto multiply = [&](float (&acc)[NT][4], const uint4& u, const uint4& v, int run) {
 #pragma unroll
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) product_few_kernel(const __grid
         };
         pdl_enter();
         load(u, v, blockIdx.x, 0);
-        pf_stage<BF16>(a, pf_raw, pitch, 0, all);
+        pf_stage<BF16>(a, pf_raw, pitch, all);
         __syncthreads();
         for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
             float total[NT][4] = {};
@@ -155,36 +156,30 @@ __global__ void __launch_bounds__(PF_THREADS, 1) product_few_kernel(const __grid
         return;
     }
     pdl_enter();
+    pf_stage<BF16>(a, pf_raw, pitch, all);
+    __syncthreads();
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
         float total[NT][4] = {};
-        for (int k0 = 0; k0 < a.k; k0 += a.chunk) {
-            const int runs = (min(a.chunk, a.k - k0) + 31) >> 5;
-            __syncthreads();                                          // the portion before is through
-            pf_stage<BF16>(a, pf_raw, pitch, k0, runs);
-            __syncthreads();
-            const int row = tile * 16 + (lane >> 2);
-            const uint16_t* w = (const uint16_t*)a.w + (int64_t)row * a.k;
-            for (int r = warp; r < runs; r += PF_WARPS) {
-                float acc[NT][4] = {};
-                const int c = k0 + r * 32 + (lane & 3) * 8;
-                multiply(acc, pf_weights(w, c, a.k, row < a.m, a.w_vec), pf_weights(w + (int64_t)8 * a.k, c, a.k, row + 8 < a.m, a.w_vec), r);
+        const int row = tile * 16 + (lane >> 2);
+        const uint16_t* w = (const uint16_t*)a.w + (int64_t)row * a.k;
+        for (int r = warp; r < all; r += PF_WARPS) {
+            float acc[NT][4] = {};
+            const int c = r * 32 + (lane & 3) * 8;
+            multiply(acc, pf_weights(w, c, a.k, row < a.m), pf_weights(w + (int64_t)8 * a.k, c, a.k, row + 8 < a.m), r);
 #pragma unroll
-                for (int n = 0; n < NT; n++)
+            for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) total[n][j] += acc[n][j];
-            }
+                for (int j = 0; j < 4; j++) total[n][j] += acc[n][j];
         }
         finish(tile, total);
     }
 }
 template <int NT>
-static cudaError_t pf_launch(cc_device* dev, PrArgs a, bool bf16) {
-    constexpr int room = NT == 1 ? PF_SMEM : PF_SMEM - 12 * 1024;      // beside 17 and 34 KB of sums
-    a.chunk = std::min((a.k + 63) / 64 * 64, (room / a.rows - 64) / 128 * 64);
-    const bool whole = a.w_vec && a.chunk >= a.k;
-    auto kernel = whole ? (bf16 ? product_few_kernel<NT, true, true> : product_few_kernel<NT, false, true>) : (bf16 ? product_few_kernel<NT, true, false> : product_few_kernel<NT, false, false>);
+static cudaError_t pf_launch(cc_device* dev, const PrArgs& a, bool bf16) {
+    constexpr int room = NT == 1 ? pf_pitch(PF_ALONE) : 16 * 192 + PF_ROOM * 2;
+    auto kernel = a.w_vec ? (bf16 ? product_few_kernel<NT, true, true> : product_few_kernel<NT, false, true>) : (bf16 ? product_few_kernel<NT, true, false> : product_few_kernel<NT, false, false>);
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, room);
-    if (e == cudaSuccess) e = cc_launch_pdl(dev, kernel, (unsigned)std::min((a.m + 15) / 16, dev->sm_count), PF_THREADS, (size_t)a.rows * (a.chunk * 2 + 64), a);
+    if (e == cudaSuccess) e = cc_launch_pdl(dev, kernel, (unsigned)std::min((a.m + 15) / 16, dev->sm_count), PF_THREADS, (size_t)a.rows * pf_pitch(a.k), a);
     dev->launches++;
     return e;
 }
@@ -213,15 +208,13 @@ static cudaError_t pr_rows(cc_device* dev, bool bf16, const void* x, int64_t str
     return cc_launch_pdl(dev, bf16 ? product_rows_kernel<true> : product_rows_kernel<false>, (unsigned)((n8 + 255) / 256), 256, 0, x, stride, type, (int)vec, k, to, n8, (uint4*)out);
 }
 template <int BN, bool BF16, bool DRAIN>
-static int pt_launch(cc_device* dev, const PrArgs& a, const void* w, const void* x, int64_t x_stride, int kp) {
+static int pt_launch(cc_device* dev, const PrArgs& a, const void* w, const void* x, int64_t x_stride, int kp, int parts) {
     CUtensorMap mw, mx;
     int rc = cc_make_tmap_rows(dev, &mw, w, a.m, a.k, (int64_t)kp * 2, 128, BF16);
     if (!rc) rc = cc_make_tmap_rows(dev, &mx, x, a.rows, a.k, x_stride * 2, BN, BF16);
     if (rc) return rc;
     const int64_t tiles = (int64_t)((a.m + 127) / 128) * ((a.rows + BN - 1) / BN);
     const int steps = (a.k + 63) / 64;
-    int parts = 1;
-    while (parts < 4 && tiles * parts * 2 <= dev->sm_count && steps / (parts * 2) >= 2) parts *= 2;
     CC_REQUIRE(dev, tiles < ((int64_t)1 << 30), "product: %lld tiles", (long long)tiles);
     auto kernel = product_tile_kernel<BN, BF16, DRAIN>;
     cudaLaunchConfig_t cfg = {};
@@ -236,6 +229,27 @@ static int pt_launch(cc_device* dev, const PrArgs& a, const void* w, const void*
     CC_CUDA(dev, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pt_smem(BN, false)));
     CC_CUDA(dev, cudaLaunchKernelEx(&cfg, kernel, mw, mx, a, steps, (int)tiles, parts, dev->err_dev, dev->err_host));
     CC_LAUNCH_CHECK(dev);
+    return CC_OK;
+}
+// clusters of 4 and of 8 CTAs, an SM each, that run at a time
+template <bool BF16, bool DRAIN>
+static int pt_clusters(cc_device* dev, int (&n)[2]) {
+    if (!dev->clusters[0]) {
+        auto kernel = product_pair_kernel<BF16, DRAIN>;
+        CC_CUDA(dev, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pt_smem(256, true)));
+        int found[2] = {0, 0};
+        for (int i = 0; i < 2; i++) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(1024); cfg.blockDim = dim3(pt_threads(256, DRAIN)); cfg.dynamicSmemBytes = pt_smem(256, true);
+            cudaLaunchAttribute at[1];
+            at[0].id = cudaLaunchAttributeClusterDimension;
+            at[0].val.clusterDim.x = 4u << i; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+            cfg.attrs = at; cfg.numAttrs = 1;
+            CC_CUDA(dev, cudaOccupancyMaxActiveClusters(&found[i], kernel, &cfg));
+        }
+        dev->clusters[0] = std::max(found[0], 1); dev->clusters[1] = found[1];
+    }
+    n[0] = dev->clusters[0]; n[1] = dev->clusters[1];
     return CC_OK;
 }
 template <bool BF16, bool DRAIN>
@@ -265,16 +279,35 @@ static int pt_launch_pair(cc_device* dev, const PrArgs& a, const void* w, const 
     CC_LAUNCH_CHECK(dev);
     return CC_OK;
 }
+// Several SMs share a tile's depth where there are too few tiles for all of them and the depth is worth the joining of their sums.  us, one / two / four parts (F32 results in brackets):
+// 64 rows: 4096 x 512 7.8 / 7.9 / 9.1, x 4096 23.2 / 16.5 / 14.3, x 14336 80 / 42 / 29
+template <int BN, bool BF16, bool DRAIN>
+static int pt_single(cc_device* dev, const PrArgs& a, const void* w, const void* x, int64_t x_stride, int kp) {
+    const int64_t tiles = (int64_t)((a.m + 127) / 128) * ((a.rows + BN - 1) / BN);
+    int parts = 1;
+    while (parts < 4 && tiles * parts * 2 <= dev->sm_count && (a.k + 63) / 64 / (parts * 2) >= 4) parts *= 2;
+    return pt_launch<BN, BF16, DRAIN>(dev, a, w, x, x_stride, kp, parts);
+}
+// More than 128 rows go to pairs of SMs: 512 rows of 1024 x 512 take 13.8 us (13.1) on one SM each, 7.9 (11.3) on pairs.  Four parts where that many clusters of 8 SMs run at a time (16 of them took
+// two rounds: 256 rows of 4096 x 4096 36.6 us), and else four SMs a tile of 128 channels: 512 rows of 1024 x 4096: pairs 20.7 (28.7), in two parts 23.6 (20.6), in four 19.2 (18.1), four SMs 18.6 (18.6);
+// 256 rows of 4096 x 14336: pairs 55.9 (75.1), in two parts 47.8 (44.9), four SMs 38.4 (38.5).  512 rows of 1024 x 512: pairs 7.9 (11.3), in four parts 14.4 (13.0), of 1024 x 1024 9.9 (13.6), 15.0 (13.8).
+// Two parts where four do not fit: 512 rows of 4096 x 4096 23.7 (32.6) / 25.5 (22.7), of 4096 x 14336 68.9 (88.2) / 55.9 (52.1)
 template <bool BF16, bool DRAIN>
 static int pt_tiles(cc_device* dev, const PrArgs& a, const void* w, const void* x, int64_t x_stride, int kp) {
-    const int64_t tiles = (int64_t)((a.m + 255) / 256) * ((a.rows + 255) / 256), pairs = dev->sm_count / 2;
-    if (a.rows > 128 && pairs > 0) {
-        int parts = 1;
-        while (parts < 4 && tiles * parts * 2 <= pairs && (a.k + 63) / 64 / (parts * 2) >= 8) parts *= 2;
-        if (tiles * parts * 2 > pairs) return pt_launch_pair<BF16, DRAIN>(dev, a, w, x, x_stride, kp, parts);
+    if (a.rows <= 32) return pt_single<32, BF16, DRAIN>(dev, a, w, x, x_stride, kp);
+    if (a.rows <= 64) return pt_single<64, BF16, DRAIN>(dev, a, w, x, x_stride, kp);
+    if (a.rows <= 128) return pt_single<128, BF16, DRAIN>(dev, a, w, x, x_stride, kp);
+    const int64_t tiles = (int64_t)((a.m + 255) / 256) * ((a.rows + 255) / 256), singles = (int64_t)((a.m + 127) / 128) * ((a.rows + 255) / 256);
+    const int steps = (a.k + 63) / 64;
+    if (steps >= (DRAIN ? 16 : 64)) {
+        int at_once[2];
+        const int rc = pt_clusters<BF16, DRAIN>(dev, at_once);
+        if (rc) return rc;
+        if (tiles <= at_once[1]) return pt_launch_pair<BF16, DRAIN>(dev, a, w, x, x_stride, kp, 4);
+        if (singles * 4 <= dev->sm_count) return pt_launch<256, BF16, DRAIN>(dev, a, w, x, x_stride, kp, 4);
+        if (tiles <= at_once[0] && steps >= (DRAIN ? 16 : 96)) return pt_launch_pair<BF16, DRAIN>(dev, a, w, x, x_stride, kp, 2);
     }
-    return a.rows <= 32 ? pt_launch<32, BF16, DRAIN>(dev, a, w, x, x_stride, kp) : a.rows <= 64 ? pt_launch<64, BF16, DRAIN>(dev, a, w, x, x_stride, kp)
-           : a.rows <= 128 ? pt_launch<128, BF16, DRAIN>(dev, a, w, x, x_stride, kp) : pt_launch<256, BF16, DRAIN>(dev, a, w, x, x_stride, kp);
+    return pt_launch_pair<BF16, DRAIN>(dev, a, w, x, x_stride, kp, 1);
 }
 static int pr_many(cc_device* dev, const PrArgs& a, bool bf16) {
     // operands that TMA cannot read, or x of another type, are laid out first
@@ -332,9 +365,9 @@ extern "C" CC_API int cc_product(cc_device* dev, const cc_view* w, const cc_view
         a.out = o->base; a.x_stride = x->strides[0]; a.res_stride = residual ? residual->strides[0] : 0; a.m = (int)m; a.k = (int)k; a.rows = (int)T;
         a.x_type = x->buf->dtype; a.out_type = out_type; a.act = act;
         a.w_vec = k % 8 == 0 && ((uintptr_t)a.w & 15) == 0; a.x_vec = a.x_stride * ht_size(a.x_type) % 16 == 0 && ((uintptr_t)a.x & 15) == 0;
-        if (T > PF_ROWS || (T > 1 && a.w_vec && T * k > PF_ROOM)) rc = pr_many(dev, a, bf16);
+        if (!pr_few(T, k, a.w_vec)) rc = pr_many(dev, a, bf16);
         else {
-            const cudaError_t e = T <= 8 ? pf_launch<1>(dev, a, bf16) : T <= 16 ? pf_launch<2>(dev, a, bf16) : pf_launch<4>(dev, a, bf16);
+            const cudaError_t e = T <= 8 ? pf_launch<1>(dev, a, bf16) : pf_launch<2>(dev, a, bf16);
             if (e != cudaSuccess) rc = cc_fail(dev, CC_ERR_CUDA, "product: %s", cudaGetErrorString(e));
         }
     }

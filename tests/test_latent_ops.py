@@ -518,3 +518,23 @@ def test_a_layer(dev):
         want = x[i] + y.reshape(n, -1) @ w["out"].astype(np.float64).T
         # five roundings to 16 bits, 2^-11 of numbers of size 1 each, and a sum of 128 of them with weights of 128^-1/2
         assert np.abs(np.concatenate(got[i]) - want).max() < 5 * 2.0 ** -11 * 6
+
+
+@pytest.mark.parametrize("pos0,counts,window,sink", [([9000], [70], 0, False), ([4000, 0, 2500], [300, 65, 130], 0, True), ([6000, 100], [513, 70], 1500, True), ([2000, 0], [129, 90], 0, False)])
+def test_cut_items(dev, pos0, counts, window, sink):
+    """expanded: few rows over long caches, whose keys several CTAs share; beside sequences that one takes as a whole, and pieces that see nothing"""
+    c = Case(dev, 64, 64, 16, pos0, counts, seed=5)
+    check(dev, c, 2, 32, 48, 0.2, window=window, sink=c.rng.normal(size=2).astype(np.float32) if sink else None, form=capi.LATENT_EXPANDED)
+
+
+def test_cut_items_not_finite(dev):
+    """expanded, cut: a row of the cache that is not finite reaches those who see it and no others, whichever piece it lies in"""
+    pos0, n = 5000, 200
+    for bad in (10, 3000, pos0 + 150):
+        c = Case(dev, 64, 64, 16, [pos0], [n], seed=bad)
+        q, uk, uv = ((c.rng.normal(size=s) * k).astype(np.float16) for s, k in (((n, 2 * 48), 1.0), ((64, 64), 0.1), ((64, 64), 0.1)))
+        clean = attend(dev, c, q, uk, uv, 2, 0.2, 0, None, capi.LATENT_EXPANDED).reshape(n, 2, 32)
+        c.a[c.table[0][bad // 64], bad % 64, 3] = np.nan
+        got = attend(dev, c, q, uk, uv, 2, 0.2, 0, None, capi.LATENT_EXPANDED).reshape(n, 2, 32)
+        sees = max(0, bad - pos0)
+        assert np.isnan(got[sees:]).all() and np.array_equal(got[:sees], clean[:sees])

@@ -112,6 +112,15 @@ def test_long_sums_of_one_sign(dev, rows, k):
     assert float(((got - want).abs() / want).max()) < 1e-5
 
 
+@pytest.mark.parametrize("rows,m,k", [(1, 37, 98304), (1, 37, 98312), (1, 300, 16385), (2, 300, 8191), (3, 64, 8191), (8, 300, 4096), (9, 300, 4096), (16, 200, 2048), (17, 200, 2048), (16, 130, 1023), (17, 130, 1023),
+                                      (200, 500, 4200), (290, 2300, 4200), (600, 2500, 6200), (300, 700, 100), (129, 4100, 1100)], ids=str)
+@pytest.mark.parametrize("w,out", [(BF16, BF16), (F16, F32)], ids=str)
+def test_ways(dev, rows, m, k, w, out):
+    """either side of the bounds between the kernels, and each number of parts of a depth"""
+    a, b, bias, _ = make(rows, m, k, w, w, seed=k)
+    check(dev, a, b, bias=bias, out=out)
+
+
 @pytest.mark.parametrize("rows", [2, 70, 260])
 def test_rows_of_a_wider_matrix(dev, rows):
     """x and the residual as column blocks, aligned and not, and a residual that is the same tensor for two calls"""
