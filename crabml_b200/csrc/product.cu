@@ -45,12 +45,13 @@ __device__ __forceinline__ uint4 pr_pack8(const float (&v)[8]) {
 #define PF_ALONE (96 * 1024)
 #define PF_ROOM (32 * 1024)
 #define PF_ROOM_ODD (16 * 1024)
-// Whether rows of x are few.  More, or longer ones, take tiles on the tensor cores, where an instruction takes all of x instead of 8 rows.  us, few / tiles, weights of 16-bit numbers:
+// Whether rows of x are few.  More, or longer ones, take tiles on the tensor cores, where an instruction takes all of x instead of 8 rows, and so do many rows of W, since every 16 of them cost
+// a barrier here.  us, few / tiles, weights of 16-bit numbers:
 // 4096 x 4096 with 1, 4, 8, 16 rows: 9.7 / 11.9, 10.7 / 12.0, 12.0 / 12.1, 15.1 / 12.3; 11008 x 4096 with 2, 16: 20.0 / 22.6, 25.1 / 21.8; 4096 x 14336 with 4: 27.0 / 24.7; 1024 x 1024 with 16: 6 / 7.7;
-// 4096 x 1024 with 32: 9.9 / 9.0.  Rows of weights that start anywhere are read number by number here and laid out for the tiles: 1024 x 1023 with 16: 8.8 / 14.5; 4096 x 4095 with 2, 8: 39.5 / 38.7,
+// 4096 x 1024 with 32: 9.9 / 9.0; one row: 8192 x 1024 8.4 / 8.9, 11008 x 1024 9.9 / 8.7, 11008 x 2048 12.9 / 13.2, 14336 x 2048 16.5 / 14.3, 131072 x 2048 110 / 86.  Rows of weights that start anywhere are read number by number here and laid out for the tiles: 1024 x 1023 with 16: 8.8 / 14.5; 4096 x 4095 with 2, 8: 39.5 / 38.7,
 // 48.7 / 38.8; 4096 x 14335 with 1, 4: 98.7 / 76.2, 107 / 76.5
-static bool pr_few(int64_t rows, int64_t k, bool w_vec) {
-    return rows <= PF_ROWS && rows * k <= (!w_vec ? PF_ROOM_ODD : rows == 1 ? PF_ALONE : PF_ROOM);
+static bool pr_few(int64_t rows, int64_t m, int64_t k, bool w_vec) {
+    return rows <= PF_ROWS && (!w_vec || m <= (k < 4096 ? 8192 : 12288)) && rows * k <= (!w_vec ? PF_ROOM_ODD : rows == 1 ? PF_ALONE : PF_ROOM);
 }
 // 8 numbers of a row from column c on, zeros behind its end
 __device__ __forceinline__ uint4 pf_weights(const uint16_t* row, int c, int k, bool there) {
@@ -365,7 +366,7 @@ extern "C" CC_API int cc_product(cc_device* dev, const cc_view* w, const cc_view
         a.out = o->base; a.x_stride = x->strides[0]; a.res_stride = residual ? residual->strides[0] : 0; a.m = (int)m; a.k = (int)k; a.rows = (int)T;
         a.x_type = x->buf->dtype; a.out_type = out_type; a.act = act;
         a.w_vec = k % 8 == 0 && ((uintptr_t)a.w & 15) == 0; a.x_vec = a.x_stride * ht_size(a.x_type) % 16 == 0 && ((uintptr_t)a.x & 15) == 0;
-        if (!pr_few(T, k, a.w_vec)) rc = pr_many(dev, a, bf16);
+        if (!pr_few(T, m, k, a.w_vec)) rc = pr_many(dev, a, bf16);
         else {
             const cudaError_t e = T <= 8 ? pf_launch<1>(dev, a, bf16) : pf_launch<2>(dev, a, bf16);
             if (e != cudaSuccess) rc = cc_fail(dev, CC_ERR_CUDA, "product: %s", cudaGetErrorString(e));

@@ -113,7 +113,7 @@ def test_long_sums_of_one_sign(dev, rows, k):
 
 
 @pytest.mark.parametrize("rows,m,k", [(1, 37, 98304), (1, 37, 98312), (1, 300, 16385), (2, 300, 8191), (3, 64, 8191), (8, 300, 4096), (9, 300, 4096), (16, 200, 2048), (17, 200, 2048), (16, 130, 1023), (17, 130, 1023),
-                                      (200, 500, 4200), (290, 2300, 4200), (600, 2500, 6200), (300, 700, 100), (129, 4100, 1100)], ids=str)
+                                      (200, 500, 4200), (290, 2300, 4200), (600, 2500, 6200), (300, 700, 100), (129, 4100, 1100), (2, 8192, 72), (2, 8200, 72)], ids=str)
 @pytest.mark.parametrize("w,out", [(BF16, BF16), (F16, F32)], ids=str)
 def test_ways(dev, rows, m, k, w, out):
     """either side of the bounds between the kernels, and each number of parts of a depth"""
