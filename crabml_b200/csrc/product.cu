@@ -44,23 +44,40 @@ __device__ __forceinline__ uint4 pr_pack8(const float (&v)[8]) {
 #define PF_ROWS 16
 #define PF_ALONE (96 * 1024)
 #define PF_ROOM (32 * 1024)
-#define PF_ROOM_ODD (16 * 1024)
+#define PF_ROOM_ODD (64 * 1024)
 // Whether rows of x are few.  More, or longer ones, take tiles on the tensor cores, where an instruction takes all of x instead of 8 rows, and so do many rows of W, since every 16 of them cost
 // a barrier here.  us, few / tiles, weights of 16-bit numbers:
 // 4096 x 4096 with 1, 4, 8, 16 rows: 9.7 / 11.9, 10.7 / 12.0, 12.0 / 12.1, 15.1 / 12.3; 11008 x 4096 with 2, 16: 20.0 / 22.6, 25.1 / 21.8; 4096 x 14336 with 4: 27.0 / 24.7; 1024 x 1024 with 16: 6 / 7.7;
-// 4096 x 1024 with 32: 9.9 / 9.0; one row: 8192 x 1024 8.4 / 8.9, 11008 x 1024 9.9 / 8.7, 11008 x 2048 12.9 / 13.2, 14336 x 2048 16.5 / 14.3, 131072 x 2048 110 / 86.  Rows of weights that start anywhere are read number by number here and laid out for the tiles: 1024 x 1023 with 16: 8.8 / 14.5; 4096 x 4095 with 2, 8: 39.5 / 38.7,
-// 48.7 / 38.8; 4096 x 14335 with 1, 4: 98.7 / 76.2, 107 / 76.5
+// 4096 x 1024 with 32: 9.9 / 9.0; one row: 8192 x 1024 8.4 / 8.9, 11008 x 1024 9.9 / 8.7, 11008 x 2048 12.9 / 13.2, 14336 x 2048 16.5 / 14.3, 131072 x 2048 110 / 86.  Rows of weights that start anywhere (k not a multiple of 8)
+// are laid out for the tiles: 4096 x 255 with 16: 6.8 / 12.3; 4096 x 2047 with 16: 12.9 / 16.8; 14336 x 1023 with 16: 16.0 / 20.2; 4096 x 4095 with 1, 8: 13.7 / 23.3, 16.9 / 23.7; 14336 x 4095 with 8: 40 / 66;
+// 4096 x 14335 with 1, 4: 35 / 67, 42 / 67
 static bool pr_few(int64_t rows, int64_t m, int64_t k, bool w_vec) {
     return rows <= PF_ROWS && (!w_vec || m <= (k < 4096 ? 8192 : 12288)) && rows * k <= (!w_vec ? PF_ROOM_ODD : rows == 1 ? PF_ALONE : PF_ROOM);
 }
-// 8 numbers of a row from column c on, zeros behind its end
-__device__ __forceinline__ uint4 pf_weights(const uint16_t* row, int c, int k, bool there) {
-    if (!there || c >= k) return make_uint4(0, 0, 0, 0);
-    unsigned u[4] = {};
+// the two words of 16 bytes that hold n of 8 numbers of 16 bits, which start at any of them; neither is read without one of the n in it
+__device__ __forceinline__ void pr_two_words(const uint16_t* from, int n, uint4& x, uint4& y) {
+    x = y = make_uint4(0, 0, 0, 0);
+    const int off = (int)((uintptr_t)from >> 1 & 7);
+    const uint4* at = (const uint4*)((uintptr_t)from & ~(uintptr_t)15);
+    if (n > 0) x = __ldg(at);
+    if (n > 0 && off + min(n, 8) > 8) y = __ldg(at + 1);
+}
+// .. the numbers, zeros behind
+__device__ __forceinline__ uint4 pr_join(const uint4& x, const uint4& y, int off, int n) {
+    const unsigned w[7] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z};
+    unsigned h[6], v[5];
 #pragma unroll
-    for (int j = 0; j < 8; j++)
-        if (c + j < k) u[j >> 1] |= (unsigned)row[c + j] << (j & 1) * 16;
-    return make_uint4(u[0], u[1], u[2], u[3]);
+    for (int j = 0; j < 6; j++) h[j] = off & 2 ? w[j + 1] : w[j];
+    const unsigned last = off & 2 ? y.w : y.z;
+#pragma unroll
+    for (int j = 0; j < 5; j++) v[j] = off & 4 ? (j < 4 ? h[j + 2] : last) : h[j];
+    unsigned r[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        r[j] = __funnelshift_r(v[j], v[j + 1], (off & 1) * 16);
+        r[j] = 2 * j + 1 < n ? r[j] : 2 * j < n ? r[j] & 0xffffu : 0u;
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
 }
 // rows of x into shared memory as 16-bit numbers, zeros behind the end of the last run
 template <bool BF16>
@@ -78,10 +95,9 @@ __device__ __forceinline__ void pf_stage(const PrArgs& a, uint8_t* to, int pitch
     }
 }
 // A CTA walks over the tiles of 16 rows of W blockIdx.x, + gridDim.x, ..; its warps take a tile's runs of 32 k by turns.
-// WHOLE (rows of W at multiples of 16 bytes): four runs of a warp are computed while the next four, also of the next tile, are under way: 64 KB an SM and more.  Else weights are read number by
-// number
+// PF_AHEAD runs of a warp are computed while the next ones, also of the next tile, are under way: 64 KB an SM and more.  ODD (rows of W start anywhere): a lane's 8 numbers lie in two words
 __host__ __device__ constexpr int pf_pitch(int k) { return (k + 63) / 64 * 128 + 64; }      // eight lanes' 16 bytes: two rows, 64 bytes each, in all banks
-template <int NT, bool BF16, bool WHOLE>
+template <int NT, bool BF16, bool ODD>
 __global__ void __launch_bounds__(PF_THREADS, 1) product_few_kernel(const __grid_constant__ PrArgs a) {
     extern __shared__ __align__(16) uint8_t pf_raw[];
     __shared__ float sums[2][PF_WARPS][16][NT * 8 + 1];
@@ -114,71 +130,60 @@ __global__ void __launch_bounds__(PF_THREADS, 1) product_few_kernel(const __grid
     };
     // the tensor cores cut a sum off at 24 bits after every 16 terms, always towards zero: sums of 128 terms go to registers and are rounded there (14336 terms of one sign: off by 1.1e-5 in
     // one chain a warp)
-    if (WHOLE) {
-        uint4 u[PF_AHEAD], v[PF_AHEAD];
-        const int64_t half = (int64_t)8 * a.k;
-        auto load = [&](uint4 (&x)[PF_AHEAD], uint4 (&y)[PF_AHEAD], int tile, int i0) {
-            // rows behind the last one: the last one again, no one reads their sums
-            const uint16_t* w = (const uint16_t*)a.w + (int64_t)min(tile * 16 + (lane >> 2), a.m - 1) * a.k;
-            const int64_t lower = tile * 16 + (lane >> 2) + 8 < a.m ? half : 0;
+    constexpr int AHEAD = ODD ? PF_AHEAD / 2 : PF_AHEAD;
+    uint4 u[AHEAD], v[AHEAD], u2[AHEAD], v2[AHEAD];                  // (the second words: ODD)
+    const int64_t half = (int64_t)8 * a.k;
+    auto load = [&](uint4 (&x)[AHEAD], uint4 (&y)[AHEAD], uint4 (&x2)[AHEAD], uint4 (&y2)[AHEAD], int tile, int i0) {
+        // rows behind the last one: the last one again, no one reads their sums
+        const uint16_t* w = (const uint16_t*)a.w + (int64_t)min(tile * 16 + (lane >> 2), a.m - 1) * a.k;
+        const int64_t lower = tile * 16 + (lane >> 2) + 8 < a.m ? half : 0;
 #pragma unroll
-            for (int i = 0; i < PF_AHEAD; i++) {
-                const int c = (warp + (i0 + i) * PF_WARPS) * 32 + (lane & 3) * 8;
+        for (int i = 0; i < AHEAD; i++) {
+            const int c = (warp + (i0 + i) * PF_WARPS) * 32 + (lane & 3) * 8, n = tile < tiles ? a.k - c : 0;
+            if (ODD) {
+                pr_two_words(w + c, n, x[i], x2[i]);
+                pr_two_words(w + lower + c, n, y[i], y2[i]);
+            } else {
                 x[i] = y[i] = make_uint4(0, 0, 0, 0);
-                if (tile < tiles && c < a.k) {
+                if (n > 0) {
                     const int4 p = ld_stream_16(w + c), q = ld_stream_16(w + lower + c);
                     x[i] = make_uint4((unsigned)p.x, (unsigned)p.y, (unsigned)p.z, (unsigned)p.w); y[i] = make_uint4((unsigned)q.x, (unsigned)q.y, (unsigned)q.z, (unsigned)q.w);
                 }
             }
-        };
-        pdl_enter();
-        load(u, v, blockIdx.x, 0);
-        pf_stage<BF16>(a, pf_raw, pitch, all);
-        __syncthreads();
-        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-            float total[NT][4] = {};
-            for (int i0 = 0; i0 < mine; i0 += PF_AHEAD) {
-                uint4 nu[PF_AHEAD], nv[PF_AHEAD];
-                const bool over = i0 + PF_AHEAD >= mine;
-                load(nu, nv, over ? tile + (int)gridDim.x : tile, over ? 0 : i0 + PF_AHEAD);
-                float acc[NT][4] = {};
-#pragma unroll
-                for (int i = 0; i < PF_AHEAD; i++) multiply(acc, u[i], v[i], min(warp + (i0 + i) * PF_WARPS, all - 1));      // (runs behind the last one: weights 0)
-#pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) total[n][j] += acc[n][j];
-#pragma unroll
-                for (int i = 0; i < PF_AHEAD; i++) { u[i] = nu[i]; v[i] = nv[i]; }
-            }
-            if (mine <= 0) load(u, v, tile + (int)gridDim.x, 0);
-            finish(tile, total);
         }
-        return;
-    }
+    };
     pdl_enter();
+    load(u, v, u2, v2, blockIdx.x, 0);
     pf_stage<BF16>(a, pf_raw, pitch, all);
     __syncthreads();
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        const int off = ODD ? (int)((uintptr_t)a.w / 2 + (unsigned)min(tile * 16 + (lane >> 2), a.m - 1) * (unsigned)a.k) & 7 : 0;      // (of the row 8 below, too)
         float total[NT][4] = {};
-        const int row = tile * 16 + (lane >> 2);
-        const uint16_t* w = (const uint16_t*)a.w + (int64_t)row * a.k;
-        for (int r = warp; r < all; r += PF_WARPS) {
+        for (int i0 = 0; i0 < mine; i0 += AHEAD) {
+            uint4 nu[AHEAD], nv[AHEAD], nu2[AHEAD], nv2[AHEAD];
+            const bool over = i0 + AHEAD >= mine;
+            load(nu, nv, nu2, nv2, over ? tile + (int)gridDim.x : tile, over ? 0 : i0 + AHEAD);
             float acc[NT][4] = {};
-            const int c = r * 32 + (lane & 3) * 8;
-            multiply(acc, pf_weights(w, c, a.k, row < a.m), pf_weights(w + (int64_t)8 * a.k, c, a.k, row + 8 < a.m), r);
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) {
+                const int run = warp + (i0 + i) * PF_WARPS, n = a.k - run * 32 - (lane & 3) * 8;
+                multiply(acc, ODD ? pr_join(u[i], u2[i], off, n) : u[i], ODD ? pr_join(v[i], v2[i], off, n) : v[i], min(run, all - 1));      // (runs behind the last one: weights 0)
+            }
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) total[n][j] += acc[n][j];
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) { u[i] = nu[i]; v[i] = nv[i]; u2[i] = nu2[i]; v2[i] = nv2[i]; }
         }
+        if (mine <= 0) load(u, v, u2, v2, tile + (int)gridDim.x, 0);
         finish(tile, total);
     }
 }
 template <int NT>
 static cudaError_t pf_launch(cc_device* dev, const PrArgs& a, bool bf16) {
-    constexpr int room = NT == 1 ? pf_pitch(PF_ALONE) : 16 * 192 + PF_ROOM * 2;
-    auto kernel = a.w_vec ? (bf16 ? product_few_kernel<NT, true, true> : product_few_kernel<NT, false, true>) : (bf16 ? product_few_kernel<NT, true, false> : product_few_kernel<NT, false, false>);
+    constexpr int room = NT == 1 ? pf_pitch(PF_ALONE) : PF_ROWS * 192 + PF_ROOM_ODD * 2;
+    auto kernel = a.w_vec ? (bf16 ? product_few_kernel<NT, true, false> : product_few_kernel<NT, false, false>) : (bf16 ? product_few_kernel<NT, true, true> : product_few_kernel<NT, false, true>);
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, room);
     if (e == cudaSuccess) e = cc_launch_pdl(dev, kernel, (unsigned)std::min((a.m + 15) / 16, dev->sm_count), PF_THREADS, (size_t)a.rows * pf_pitch(a.k), a);
     dev->launches++;
@@ -195,6 +200,13 @@ __global__ void __launch_bounds__(256) product_rows_kernel(const void* __restric
     if (i >= n8) return;
     const int64_t row = i / (to / 8);
     const int c = (int)(i - row * (to / 8)) * 8;
+    if (type == (BF16 ? CC_BF16 : CC_F16)) {                         // (number by number, 4096 rows of 4095 took 26 us, so 11)
+        const uint16_t* from = (const uint16_t*)x + row * stride + c;
+        uint4 u, v;
+        pr_two_words(from, k - c, u, v);
+        out[i] = pr_join(u, v, (int)((uintptr_t)from >> 1 & 7), k - c);
+        return;
+    }
     float v[8] = {};
     if (c + 8 <= k) ht_read8(x, row * stride + c, type, vec, v);
     else
