@@ -707,8 +707,8 @@ static int lr_portion(cc_device* dev, const cc_page_plan* plan, LrArgs a) {
     for (int i = 0; i < runs.n; i++) { runs.tile0[i] = runs.tiles; runs.tiles += (runs.hi[i] - runs.lo[i] + LT_TOKENS - 1) / LT_TOKENS; }
     LrDeal deal;
     LrCuts cuts;
-    CC_REQUIRE(dev, steps < ((int64_t)1 << 31) * 64, "paged_latent_attention: too many rows");
     deal.ctas = (int)std::min<int64_t>(std::min(LR_CTAS, dev->sm_count), (steps + LR_BEGIN + 1) / (LR_BEGIN + 2));
+    CC_REQUIRE(dev, steps / deal.ctas < 0x7ffffffe, "paged_latent_attention: too many rows");
     const int n_cuts = lr_deal(plan, a, steps, deal, cuts);
     const int64_t tokens = a.token1 - a.token0;
     const size_t qf = (size_t)tokens * a.H * a.cols * 4, lat = (size_t)tokens * a.H * a.rank * 4, part = n_cuts ? (size_t)2 * deal.ctas * LR_ROWS * a.rank * 4 : 0,

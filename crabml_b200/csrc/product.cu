@@ -220,6 +220,27 @@ static cudaError_t pr_rows(cc_device* dev, bool bf16, const void* x, int64_t str
     dev->launches++;
     return cc_launch_pdl(dev, bf16 ? product_rows_kernel<true> : product_rows_kernel<false>, (unsigned)((n8 + 255) / 256), 256, 0, x, stride, type, (int)vec, k, to, n8, (uint4*)out);
 }
+// clusters of 4 and of 8 CTAs, an SM each, that run at a time
+template <bool BF16, bool DRAIN>
+static int pt_clusters(cc_device* dev, int (&n)[2]) {
+    if (!dev->clusters[0]) {
+        auto kernel = product_pair_kernel<BF16, DRAIN>;
+        CC_CUDA(dev, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pt_smem(256, true)));
+        int found[2] = {0, 0};
+        for (int i = 0; i < 2; i++) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(1024); cfg.blockDim = dim3(pt_threads(256, DRAIN)); cfg.dynamicSmemBytes = pt_smem(256, true);
+            cudaLaunchAttribute at[1];
+            at[0].id = cudaLaunchAttributeClusterDimension;
+            at[0].val.clusterDim.x = 4u << i; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+            cfg.attrs = at; cfg.numAttrs = 1;
+            CC_CUDA(dev, cudaOccupancyMaxActiveClusters(&found[i], kernel, &cfg));
+        }
+        dev->clusters[0] = std::max(found[0], 1); dev->clusters[1] = found[1];
+    }
+    n[0] = std::min(dev->clusters[0], dev->sm_count / 4); n[1] = std::min(dev->clusters[1], dev->sm_count / 8);
+    return CC_OK;
+}
 template <int BN, bool BF16, bool DRAIN>
 static int pt_launch(cc_device* dev, const PrArgs& a, const void* w, const void* x, int64_t x_stride, int kp, int parts) {
     CUtensorMap mw, mx;
@@ -242,27 +263,6 @@ static int pt_launch(cc_device* dev, const PrArgs& a, const void* w, const void*
     CC_CUDA(dev, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pt_smem(BN, false)));
     CC_CUDA(dev, cudaLaunchKernelEx(&cfg, kernel, mw, mx, a, steps, (int)tiles, parts, dev->err_dev, dev->err_host));
     CC_LAUNCH_CHECK(dev);
-    return CC_OK;
-}
-// clusters of 4 and of 8 CTAs, an SM each, that run at a time
-template <bool BF16, bool DRAIN>
-static int pt_clusters(cc_device* dev, int (&n)[2]) {
-    if (!dev->clusters[0]) {
-        auto kernel = product_pair_kernel<BF16, DRAIN>;
-        CC_CUDA(dev, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pt_smem(256, true)));
-        int found[2] = {0, 0};
-        for (int i = 0; i < 2; i++) {
-            cudaLaunchConfig_t cfg = {};
-            cfg.gridDim = dim3(1024); cfg.blockDim = dim3(pt_threads(256, DRAIN)); cfg.dynamicSmemBytes = pt_smem(256, true);
-            cudaLaunchAttribute at[1];
-            at[0].id = cudaLaunchAttributeClusterDimension;
-            at[0].val.clusterDim.x = 4u << i; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
-            cfg.attrs = at; cfg.numAttrs = 1;
-            CC_CUDA(dev, cudaOccupancyMaxActiveClusters(&found[i], kernel, &cfg));
-        }
-        dev->clusters[0] = std::max(found[0], 1); dev->clusters[1] = found[1];
-    }
-    n[0] = dev->clusters[0]; n[1] = dev->clusters[1];
     return CC_OK;
 }
 template <bool BF16, bool DRAIN>
@@ -293,12 +293,19 @@ static int pt_launch_pair(cc_device* dev, const PrArgs& a, const void* w, const 
     return CC_OK;
 }
 // Several SMs share a tile's depth where there are too few tiles for all of them and the depth is worth the joining of their sums.  us, one / two / four parts (F32 results in brackets):
-// 64 rows: 4096 x 512 7.8 / 7.9 / 9.1, x 4096 23.2 / 16.5 / 14.3, x 14336 80 / 42 / 29
+// 64 rows: 4096 x 512 7.8 / 7.9 / 9.1, x 4096 23.2 / 16.5 / 14.3, x 14336 80 / 42 / 29; eight where that many clusters run at a time:
+// 16 rows of 1024 x 14336, four / eight 23 / 17; of 512 x 4096 10.7 / 10
 template <int BN, bool BF16, bool DRAIN>
 static int pt_single(cc_device* dev, const PrArgs& a, const void* w, const void* x, int64_t x_stride, int kp) {
     const int64_t tiles = (int64_t)((a.m + 127) / 128) * ((a.rows + BN - 1) / BN);
-    int parts = 1;
-    while (parts < 4 && tiles * parts * 2 <= dev->sm_count && (a.k + 63) / 64 / (parts * 2) >= 4) parts *= 2;
+    const int steps = (a.k + 63) / 64;
+    int parts = 1, at_once[2];
+    while (parts < 4 && tiles * parts * 2 <= dev->sm_count && steps / (parts * 2) >= 4) parts *= 2;
+    if (parts == 4 && steps >= 64 && 7 * (pt_workers(BN, DRAIN) / 4) * 16 * 128 * 4 <= pt_stages(BN, false) * pt_bytes(BN, false)) {      // (seven others' sums of a run of each group lie in the ring)
+        const int rc = pt_clusters<BF16, DRAIN>(dev, at_once);
+        if (rc) return rc;
+        if (tiles <= at_once[1]) parts = 8;
+    }
     return pt_launch<BN, BF16, DRAIN>(dev, a, w, x, x_stride, kp, parts);
 }
 // More than 128 rows go to pairs of SMs: 512 rows of 1024 x 512 take 13.8 us (13.1) on one SM each, 7.9 (11.3) on pairs.  Four parts where that many clusters of 8 SMs run at a time (16 of them took
@@ -312,6 +319,7 @@ static int pt_tiles(cc_device* dev, const PrArgs& a, const void* w, const void* 
     if (a.rows <= 128) return pt_single<128, BF16, DRAIN>(dev, a, w, x, x_stride, kp);
     const int64_t tiles = (int64_t)((a.m + 255) / 256) * ((a.rows + 255) / 256), singles = (int64_t)((a.m + 127) / 128) * ((a.rows + 255) / 256);
     const int steps = (a.k + 63) / 64;
+    if (dev->sm_count < 2) return pt_launch<256, BF16, DRAIN>(dev, a, w, x, x_stride, kp, 1);      // (a device held to one SM)
     if (steps >= (DRAIN ? 16 : 64)) {
         int at_once[2];
         const int rc = pt_clusters<BF16, DRAIN>(dev, at_once);

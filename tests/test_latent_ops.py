@@ -423,6 +423,17 @@ def test_many_sequences(dev, n):
     check(dev, c, 3, 16, 16, 0.25)
 
 
+@pytest.mark.parametrize("limit", [1, 3])
+def test_few_sms(limit):
+    """a device that is held to a few SMs: the same attention"""
+    d = make_device()
+    d.set_sm_limit(limit)
+    c = Case(d, 32, 64, 16, [900, 3, 2100], [1, 60, 4], seed=limit)
+    for form in (capi.LATENT_AUTO, capi.LATENT_EXPANDED):
+        check(d, c, 8, 32, 32, 0.2, form=form)
+    d.close()
+
+
 def test_two_devices_at_once(dev):
     """two handles with streams of their own, calls by turns from two threads"""
     import threading

@@ -113,7 +113,7 @@ def test_long_sums_of_one_sign(dev, rows, k):
 
 
 @pytest.mark.parametrize("rows,m,k", [(1, 37, 98304), (1, 37, 98312), (1, 300, 16385), (2, 300, 8191), (3, 64, 8191), (8, 300, 4096), (9, 300, 4096), (16, 200, 2048), (17, 200, 2048), (16, 130, 1023), (17, 130, 1023),
-                                      (200, 500, 4200), (290, 2300, 4200), (600, 2500, 6200), (300, 700, 100), (129, 4100, 1100), (2, 8192, 72), (2, 8200, 72)], ids=str)
+                                      (200, 500, 4200), (290, 2300, 4200), (600, 2500, 6200), (300, 700, 100), (129, 4100, 1100), (2, 8192, 72), (2, 8200, 72), (20, 500, 8300), (100, 500, 8300)], ids=str)
 @pytest.mark.parametrize("w,out", [(BF16, BF16), (F16, F32)], ids=str)
 def test_ways(dev, rows, m, k, w, out):
     """either side of the bounds between the kernels, and each number of parts of a depth"""
@@ -158,6 +158,18 @@ def test_ends_of_the_types(dev):
         x[:, 0] = 1e9
         got = take(dev, seqops.product(give(dev, w), give(dev, x), out_type=capi.F32)).to(F)
         assert torch.equal(got, (torch.full_like(x, 65504.0)[:, :1].to(F) * w[:, 0].to(F)[None]))
+
+
+@pytest.mark.parametrize("limit", [1, 2, 5, 9])
+def test_few_sms(limit):
+    """a device that is held to a few SMs: the same products"""
+    d = make_device()
+    d.set_sm_limit(limit)
+    for rows, m, k in ((1, 300, 640), (20, 300, 640), (129, 300, 1100), (300, 700, 4100)):
+        for t in (BF16, F32):
+            w, x, bias, _ = make(rows, m, k, BF16, BF16, rows)
+            check(d, w, x, bias=bias, out=t)
+    d.close()
 
 
 def test_equal_calls(dev):
