@@ -3,9 +3,13 @@ by anyone who builds a model out of these mechanisms in Python).  Arguments are 
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 from . import capi
+from .capi import TensorError
 from .tensor import CudaTensor, TensorStrider, _Buf
+
+_TWO = struct.Struct("=2i").pack
 
 
 def _v(t):
@@ -411,5 +415,9 @@ def product_i8(w, w_scale, x):
 def product(w, x, bias=None, act=capi.ACT_NONE, residual=None, out_type=capi.F32):
     """act(W x + bias) + residual, w: F16 / BF16 [m, k], x: rows of F32, F16 or BF16 -> [T, m] of out_type"""
     h = C.c_void_p()
+    try:
+        _TWO(act, out_type)                                              # whole numbers that are not cut off on their way
+    except struct.error:
+        raise TensorError(f"product: act {act!r} and out_type {out_type!r} are not whole numbers of 32 bits") from None
     x.device.check(x.device.lib.cc_product(x.device.handle, _v(w), _v(x), _v(bias), int(act), _v(residual), int(out_type), C.byref(h)))
     return _new(x.device, h, [x.shape()[0], w.shape()[0]])

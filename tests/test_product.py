@@ -195,6 +195,7 @@ def test_refusals(dev):
         lambda: seqops.product(w, x, residual=give(dev, torch.zeros(3, 20, device="cuda"))), lambda: seqops.product(w, x.with_strider(TensorStrider([4, 64], [63, 1]))),
         lambda: seqops.product(w, x.with_strider(TensorStrider([4, 64], [65, 1]))), lambda: seqops.product(w.with_strider(TensorStrider([20, 64], [1, 20])), x),
         lambda: seqops.product(w, give(other, torch.zeros(4, 64, device="cuda", dtype=BF16))), lambda: seqops.product(w, CudaTensor.alloc([4, 64], capi.I8, dev)),
+        lambda: seqops.product(w, x, act=1 << 32), lambda: seqops.product(w, x, out_type=-(1 << 32)), lambda: seqops.product(w, x, act="silu"), lambda: seqops.product(w, x, act=0.5),
     ]
     for f in bad:
         with pytest.raises(TensorError):
