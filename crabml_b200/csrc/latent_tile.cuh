@@ -2,12 +2,15 @@
 //
 // latent_expand_kernel makes the keys U_h c and values V_h c of 256 cached rows and a run of heads: one product of 256 x (dim + vdim) x rank for each head on tcgen05.mma, the rows staying in
 // shared memory for all heads.  The results go to images, f16 in the order of the 128-byte swizzle, which bulk copies bring back as they are.  r, which all heads share, is read from the pages.
+// 4000 rows, 16 heads of 128 and 128, rank 512: 25 us on 128 SMs (16.8 GFLOP, 0.67 PFLOP/s with the rows' way in and the last block's way out), 8000 37.
 //
 // latent_tile_kernel: a CTA takes 256 tokens of a head, as two tiles of 128 rows, over the keys that they see, 128 at a time:
 //   S = Q K^T (128 x 128 x (dim + rest)), P = exp2(S f - base) as f16 written over S in TMEM, O += P V in TMEM
 // The two tiles alternate: while the 256 threads of one make its weights, two a row, the tensor core multiplies for the other.  (With a thread a row a step's 128 scores were a chain of
 // 4500 cycles for the one warp a scheduler that a tile had: 4000 tokens of 16 heads took 147 us.)  TMEM holds both S and both O (512 columns), shared memory
-// Q (96 KB) and a ring of 16 KB blocks of keys and values (128 KB).  base lags: a row's sums are scaled only when its largest score is 2^TL_LAG times what it was (sums in TMEM would have
+// Q (96 KB) and a ring of 16 KB blocks of keys and values (128 KB).
+// Now that prompt's call takes 128 us (98.7 GFLOP with its keys and values, 0.77 PFLOP/s); 8000 tokens 359 (0.96 PFLOP/s).  Shared memory bounds the products: S reads 8 KB for each 64 cycles of the tensor core, as fast as
+// it can; then 8 us of start and end for each item.  base lags: a row's sums are scaled only when its largest score is 2^TL_LAG times what it was (sums in TMEM would have
 // to be read and written back), so that weights are up to 2^TL_LAG and f16 still holds them and all that counts beside them.
 // Warps 0-7 and 8-15 the rows of the two tiles, 16 the copies, 17 the products, 18 says what has come.  Every wait is bounded; where one ran out all roles run to their ends and the host reports it.
 #pragma once
@@ -730,6 +733,9 @@ __global__ void __launch_bounds__(256) latent_tile_join_kernel(const __grid_cons
     *(uint2*)out = a.out_bf16 ? make_uint2(ht_pack_bf16(o.x * by, o.y * by), ht_pack_bf16(o.z * by, o.w * by)) : make_uint2(ht_pack_f16(o.x * by, o.y * by), ht_pack_f16(o.z * by, o.w * by));
 }
 
+// Items over many keys are cut into pieces of about a CTA's share of all steps where that saves TL_GAIN steps, and their sums joined: 16 heads, whole / cut, us: 64 tokens behind 8000 rows 184 / 77, 512 225 / 110,
+// 128 behind 32000 681 / 230.  Asked to save 4 steps only: 1500 tokens alone 53 / 70, three prompts 83 / 85 (the sums are 128 KB a piece); 8 steps: 64 behind 8000 87, 16: 77.  Pieces of 4, 6, 8, 12, 16 steps
+// and more (64 behind 8000): 91, 77, 97, 105, 120
 #define TL_PIECE 6                            // steps of a piece, at least
 #define TL_GAIN 16                            // steps that cutting has to save
 #define TL_WORKSPACE ((int64_t)256 << 20)     // bytes of images that a call has at a time, as long as those of one sequence and head are no more

@@ -1,11 +1,16 @@
 // product_tile.cuh -- products of many rows on tcgen05.mma with bias, activation and residual in their epilogue.  Included by product.cu.
 //
-// Tiles of 128 output channels x BN rows of x (product_tile_kernel), or, where there are enough of them, of 256 x 256 for a pair of SMs (product_pair_kernel): each holds 128 channels and half of
+// Tiles of 128 output channels x BN rows of x (product_tile_kernel), or, from 129 rows on, of 256 x 256 for a pair of SMs (product_pair_kernel): each holds 128 channels and half of
 // the rows of a step, the pair's instruction reads both halves, so that a step brings 32 KB to an SM instead of 48.  TMA stages steps of 64 k, one thread issues the products, the sums lie
-// twice in TMEM, so that 8 warps finish a tile while the next one is under way; a warp's lanes are consecutive channels, which a row of the result has side by side.
+// twice in TMEM, so that 8 warps (16 for 32-bit results) finish a tile while the next one is under way; a warp's lanes are consecutive channels, which a row of the result has side by side.
+//
+// What bounds them: up to 128 rows memory (16 rows of 11008 x 4096 22.2 us, 131072 x 2048 86 us: 4.9 and 6.3 TB/s; tile heights that fill all SMs, copies of W and x by a warp each, and depths
+// begun elsewhere by each CTA changed nothing), beyond that the tensor cores: 2048 rows of 14336 x 4096 162 us, 1.48 PFLOP/s with the weights in L2, 77 % of their cycles, the rest power and
+// the operands' 64 KB a step from shared memory; 509 rows of 4096 x 14336 in two parts 52 us.
 //
 // DRAIN (32-bit results): the tensor cores cut a sum off at 24 bits after every 16 terms.  Over 14336 terms that is 1e-5 of a result and more; so sums of 64 * PT_DRAIN terms leave TMEM for
-// registers, are rounded there, and the whole sum goes back for the epilogue.  16-bit results are rounded 2^9 times more coarsely.
+// registers, are rounded there, and the whole sum goes back for the epilogue (256 terms a time: errors of 14336 random terms / of one sign 3.5e-7 / 1.2e-6, a product of 509 rows 58.1 us; 128 terms
+// 2.2e-7 / 5e-7, 61.5; 512 6.5e-7 / 2.7e-6, 57.5; none 4.3e-6 / 2.2e-5, 57.0).  16-bit results are rounded 2^9 times more coarsely.
 //
 // Every wait is bounded (sg_wait): on expiry the CTA raises `fail`, all roles leave their loops, TMEM is freed and the host reports it.
 #pragma once

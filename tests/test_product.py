@@ -172,6 +172,21 @@ def test_few_sms(limit):
     d.close()
 
 
+def test_bits(dev):
+    """16-bit memory for libraries that know no bf16: the same memory, kept by who holds it, and no other type's"""
+    t = give(dev, torch.arange(6, device="cuda", dtype=F32).reshape(2, 3).to(BF16))
+    held = t.bits()
+    at = held.__cuda_array_interface__
+    assert at["typestr"] == "<i2" and at["shape"] == (2, 3) and at["data"][0] == t.bits().__cuda_array_interface__["data"][0]
+    y = torch.as_tensor(held, device="cuda").view(BF16)
+    del t
+    assert y.float().tolist() == [[0, 1, 2], [3, 4, 5]]
+    with pytest.raises(TensorError):
+        give(dev, torch.zeros(2, 3, device="cuda")).bits()
+    with pytest.raises(AttributeError):
+        give(dev, torch.zeros(2, 3, device="cuda", dtype=BF16)).__cuda_array_interface__
+
+
 def test_equal_calls(dev):
     for rows in (1, 30, 200):
         w, x, bias, _ = make(rows, 500, 1000, BF16, BF16, 2)
