@@ -119,6 +119,7 @@ struct cc_device {
     uint64_t launches = 0;
     int sm_count = 148;
     int clusters[2] = {0, 0};                 // of 4 and of 8 CTAs, an SM each, that run at a time; 0: not asked yet
+    uint64_t limits = 0;                      // kernels whose limit of shared memory this handle has set (cc_smem_limit)
 
     // f16 LUTs (cpu_device.rs:108-124), computed on the host with libm and uploaded
     uint16_t* exp_lut = nullptr;
@@ -398,6 +399,15 @@ static inline cudaError_t cc_launch_when(bool early, cc_device* dev, void (*kern
 }
 template <class... K, class... A>
 static inline cudaError_t cc_launch_pdl(cc_device* dev, void (*kernel)(K...), dim3 grid, dim3 block, size_t smem, A... args) { return cc_launch_when(true, dev, kernel, grid, block, smem, args...); }
+// A kernel's limit of shared memory, once a handle (0.4 us a time): `bit` is the kernel's own
+enum { CC_LIMIT_PRODUCT_FEW = 0, CC_LIMIT_PRODUCT_TILE = 8, CC_LIMIT_PRODUCT_PAIR = 24, CC_LIMIT_LATENT = 28 };
+template <class... K>
+static inline cudaError_t cc_smem_limit(cc_device* dev, int bit, void (*kernel)(K...), int bytes) {
+    if (dev->limits >> bit & 1) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) dev->limits |= (uint64_t)1 << bit;
+    return e;
+}
 template <class... K, class... A>
 static inline cudaError_t cc_launch_alone(cc_device* dev, void (*kernel)(K...), dim3 grid, dim3 block, size_t smem, A... args) { return cc_launch_when(false, dev, kernel, grid, block, smem, args...); }
 #endif

@@ -730,9 +730,9 @@ static int lr_portion(cc_device* dev, const cc_page_plan* plan, LrArgs a) {
     if (rc) { cc_pool_free(dev, ws, cls); return rc; }
     const unsigned z = (unsigned)std::min(runs.tiles, 64);
     const size_t fold = (size_t)a.dim * (LF_COLS + 8) * 2 + LT_TOKENS * (a.dim + 8) * 2;
-    cudaError_t e = cudaFuncSetAttribute(latent_fold_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LT_DIM * (LF_COLS + 8) * 2 + LT_TOKENS * (LT_DIM + 8) * 2);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(latent_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LR_SMEM - (int)sizeof(LrShared));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(latent_unfold_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, lu_smem(LT_RANK));
+    cudaError_t e = cc_smem_limit(dev, CC_LIMIT_LATENT, latent_fold_kernel, LT_DIM * (LF_COLS + 8) * 2 + LT_TOKENS * (LT_DIM + 8) * 2);
+    if (e == cudaSuccess) e = cc_smem_limit(dev, CC_LIMIT_LATENT + 1, latent_rows_kernel, LR_SMEM - (int)sizeof(LrShared));
+    if (e == cudaSuccess) e = cc_smem_limit(dev, CC_LIMIT_LATENT + 2, latent_unfold_kernel, lu_smem(LT_RANK));
     if (e == cudaSuccess) e = cc_launch_pdl(dev, latent_fold_kernel, dim3((unsigned)a.H, (unsigned)((a.rank + LF_COLS - 1) / LF_COLS + 1 + (deal.ctas + 4 * a.H - 1) / (4 * a.H)), z), 128, fold, a, runs, deal);
     if (e == cudaSuccess) e = cc_launch_pdl(dev, latent_rows_kernel, (unsigned)deal.ctas, LR_THREADS, (size_t)a.slots * slot + 1024, whole, map, a, deal, dev->err_dev, dev->err_host);
     if (e == cudaSuccess && n_cuts) {

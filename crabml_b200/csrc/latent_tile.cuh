@@ -748,8 +748,8 @@ static int tl_run(cc_device* dev, const cc_page_plan* plan, const LrArgs& all) {
     if (!rc) rc = cc_make_tmap_rows(dev, &uk, all.uk, (int64_t)all.H * all.dim, all.rank, (int64_t)all.rank * 2, wide, false);
     if (!rc) rc = cc_make_tmap_rows(dev, &uv, all.uv, (int64_t)all.H * all.vdim, all.rank, (int64_t)all.rank * 2, wide, false);
     if (rc) return rc;
-    CC_CUDA(dev, cudaFuncSetAttribute(latent_expand_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TE_SMEM));
-    CC_CUDA(dev, cudaFuncSetAttribute(latent_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TL_SMEM));
+    CC_CUDA(dev, cc_smem_limit(dev, CC_LIMIT_LATENT + 3, latent_expand_kernel, TE_SMEM));
+    CC_CUDA(dev, cc_smem_limit(dev, CC_LIMIT_LATENT + 4, latent_tile_kernel, TL_SMEM));
     // as many sequences at a time as have their images of one head in TL_WORKSPACE, and as many heads
     for (int first = 0, end; first < plan->n_seqs; first = end) {
         TlArgs t{};

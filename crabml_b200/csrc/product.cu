@@ -185,7 +185,7 @@ template <int NT>
 static cudaError_t pf_launch(cc_device* dev, const PrArgs& a, bool bf16) {
     constexpr int room = NT == 1 ? pf_pitch(PF_ALONE) : PF_ROWS * 192 + PF_ROOM_ODD * 2;
     auto kernel = a.w_vec ? (bf16 ? product_few_kernel<NT, true, false> : product_few_kernel<NT, false, false>) : (bf16 ? product_few_kernel<NT, true, true> : product_few_kernel<NT, false, true>);
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, room);
+    cudaError_t e = cc_smem_limit(dev, CC_LIMIT_PRODUCT_FEW + (NT - 1) * 4 + bf16 * 2 + a.w_vec, kernel, room);
     if (e == cudaSuccess) e = cc_launch_pdl(dev, kernel, (unsigned)std::min((a.m + 15) / 16, dev->sm_count), PF_THREADS, (size_t)a.rows * pf_pitch(a.k), a);
     dev->launches++;
     return e;
@@ -226,7 +226,7 @@ template <bool BF16, bool DRAIN>
 static int pt_clusters(cc_device* dev, int (&n)[2]) {
     if (!dev->clusters[0]) {
         auto kernel = product_pair_kernel<BF16, DRAIN>;
-        CC_CUDA(dev, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pt_smem(256, true)));
+        CC_CUDA(dev, cc_smem_limit(dev, CC_LIMIT_PRODUCT_PAIR + BF16 * 2 + DRAIN, kernel, (int)pt_smem(256, true)));
         int found[2] = {0, 0};
         for (int i = 0; i < 2; i++) {
             cudaLaunchConfig_t cfg = {};
@@ -261,7 +261,7 @@ static int pt_launch(cc_device* dev, const PrArgs& a, const void* w, const void*
     at[1].id = cudaLaunchAttributeClusterDimension;
     at[1].val.clusterDim.x = (unsigned)parts; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
     cfg.attrs = at; cfg.numAttrs = 2;
-    CC_CUDA(dev, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pt_smem(BN, false)));
+    CC_CUDA(dev, cc_smem_limit(dev, CC_LIMIT_PRODUCT_TILE + (BN == 32 ? 0 : BN == 64 ? 4 : BN == 128 ? 8 : 12) + BF16 * 2 + DRAIN, kernel, (int)pt_smem(BN, false)));
     CC_CUDA(dev, cudaLaunchKernelEx(&cfg, kernel, mw, mx, a, steps, (int)tiles, parts, dev->err_dev, dev->err_host));
     CC_LAUNCH_CHECK(dev);
     return CC_OK;
@@ -288,7 +288,7 @@ static int pt_launch_pair(cc_device* dev, const PrArgs& a, const void* w, const 
     at[1].id = cudaLaunchAttributeClusterDimension;
     at[1].val.clusterDim.x = (unsigned)(2 * parts); at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
     cfg.attrs = at; cfg.numAttrs = 2;
-    CC_CUDA(dev, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pt_smem(256, true)));
+    CC_CUDA(dev, cc_smem_limit(dev, CC_LIMIT_PRODUCT_PAIR + BF16 * 2 + DRAIN, kernel, (int)pt_smem(256, true)));
     CC_CUDA(dev, cudaLaunchKernelEx(&cfg, kernel, mw, mx, mc, a, (a.k + 63) / 64, whole, cut, whole + rest * cut, parts, dev->err_dev, dev->err_host));
     CC_LAUNCH_CHECK(dev);
     return CC_OK;

@@ -142,7 +142,7 @@ def latent_append(plan, pages, rank, kv_src, kv_col0, norm_w=None, eps=1e-6, q_s
             ("rank", rank), ("kv_col0", kv_col0), ("q_col0", q_col0), ("n_heads", n_heads), ("dim", dim), ("pairing", pairing)))
     dev.check(dev.lib.cc_paged_latent_append(dev.handle, plan.handle, _v(pages), rank, _v(kv_src), kv_col0, _v(norm_w), float(eps), _v(q_src), q_col0, n_heads, dim, _v(freq),
                                              pairing, float(mag), C.byref(h)))
-    return None if q_src is None else CudaTensor(_Buf(dev, h), TensorStrider([plan.tokens, n_heads * (dim + pages.shape()[2] - rank)]), dev)
+    return None if q_src is None else CudaTensor(_Buf(dev, h, capi.F16), TensorStrider([plan.tokens, n_heads * (dim + pages._strider.shape[2] - rank)]), dev)
 
 
 def latent_attention(plan, pages, rank, q, n_heads, uk, uv, scale, window=0, sink=None, form=capi.LATENT_AUTO, out_type=capi.BF16):
@@ -154,4 +154,4 @@ def latent_attention(plan, pages, rank, q, n_heads, uk, uv, scale, window=0, sin
         rank, n_heads, window, form, out_type = (_number("paged_latent_attention", what, x) for what, x in (
             ("rank", rank), ("n_heads", n_heads), ("window", window), ("form", form), ("out_type", out_type)))
     dev.check(dev.lib.cc_paged_latent_attention(dev.handle, plan.handle, _v(pages), rank, _v(q), n_heads, _v(uk), _v(uv), float(scale), window, _v(sink), form, out_type, C.byref(h)))
-    return CudaTensor(_Buf(dev, h), TensorStrider([plan.tokens, uv.shape()[0]]), dev)
+    return CudaTensor(_Buf(dev, h, int(out_type)), TensorStrider([plan.tokens, uv._strider.shape[0]]), dev)

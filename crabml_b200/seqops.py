@@ -419,5 +419,6 @@ def product(w, x, bias=None, act=capi.ACT_NONE, residual=None, out_type=capi.F32
         _TWO(act, out_type)                                              # whole numbers that are not cut off on their way
     except struct.error:
         raise TensorError(f"product: act {act!r} and out_type {out_type!r} are not whole numbers of 32 bits") from None
-    x.device.check(x.device.lib.cc_product(x.device.handle, _v(w), _v(x), _v(bias), int(act), _v(residual), int(out_type), C.byref(h)))
-    return _new(x.device, h, [x.shape()[0], w.shape()[0]])
+    dev = x.device
+    dev.check(dev.lib.cc_product(dev.handle, _v(w), _v(x), _v(bias), int(act), _v(residual), int(out_type), C.byref(h)))
+    return CudaTensor(_Buf(dev, h, int(out_type)), TensorStrider([x._strider.shape[0], w._strider.shape[0]]), dev)

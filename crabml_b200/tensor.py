@@ -16,11 +16,14 @@ class TensorStrider:
     """crabml-core/src/tensor/strider.rs:5-236 (host-side metadata; never crosses the ABI)."""
 
     def __init__(self, shape, strides=None):
-        self.shape = [int(s) for s in shape]
+        self.shape = shape = [int(s) for s in shape]
         if strides is None:
-            strides, n = [1] * max(1, len(self.shape)), 1
-            for i in range(len(self.shape) - 1, 0, -1):
-                n *= self.shape[i]
+            if len(shape) == 2:
+                self.strides = [shape[1], 1]
+                return
+            strides, n = [1] * max(1, len(shape)), 1
+            for i in range(len(shape) - 1, 0, -1):
+                n *= shape[i]
                 strides[i - 1] = n
             self.strides = strides
             return
@@ -168,9 +171,9 @@ class CudaTensorDevice:
 class _Buf:
     """Arc<buffer>: releases the device storage when the last Python reference dies."""
 
-    def __init__(self, device, handle):
-        self.device, self.handle = device, handle
-        self.dtype = self.data = None                              # asked for once: neither changes (data: on eager devices)
+    def __init__(self, device, handle, dtype=None):
+        self.device, self.handle, self.dtype = device, handle, dtype
+        self.data = None                                            # asked for once, like the type: neither changes (data: on eager devices)
 
     def __del__(self):
         try:
@@ -229,8 +232,9 @@ class CudaTensor:
 
     def _array_of_type(self, kind, size):
         shape, data = tuple(self._strider.shape), self.buf.data
-        if data is None or self.device._lazy:
+        if self.device._lazy:
             self.device.flush()
+        if data is None or self.device._lazy:
             data = self.buf.data = self.device.lib.cc_tensor_data(self.buf.handle)
         return {"shape": shape, "typestr": kind, "data": (0 if 0 in shape else data, False),
                 "strides": None if self._strider.is_contiguous() else tuple(s * size for s in self._strider.strides), "stream": self.device.stream(), "version": 3}
