@@ -172,6 +172,28 @@ def test_few_sms(limit):
     d.close()
 
 
+@pytest.mark.parametrize("rows,m,k", [(3, 131100, 16400), (2, 131100, 16401), (70000, 32768, 16)], ids=str)
+def test_far_numbers(dev, rows, m, k):
+    """weights, or results, whose places lie beyond 2^31"""
+    if torch.cuda.mem_get_info()[0] < 8 * (m * k + rows * m):
+        pytest.skip("no room")
+    w, x = CudaTensor.alloc([m, k], capi.BF16, dev), CudaTensor.alloc([rows, k], capi.BF16, dev)
+    dev.synchronize()
+    g = torch.Generator(device="cuda").manual_seed(k)
+    view(w).normal_(0.0, k ** -0.5, generator=g)
+    view(x).normal_(0.0, 1.0, generator=g)
+    torch.cuda.synchronize()
+    y = seqops.product(w, x, out_type=capi.BF16)
+    dev.synchronize()
+    for t in sorted({0, rows // 2, rows - 1}):
+        for c in (0, m // 2, m - 40):
+            a, b = view(w)[c:c + 40].double(), view(x)[t].double()
+            want, size = a @ b, a.abs() @ b.abs()
+            # sums of 16-bit results: 24 bits cut off after every 16 terms, and one rounding to bf16
+            lim = want.abs() * 2.0 ** -8 + size * (k / 16 + 1) * 2.0 ** -23
+            assert ((view(y)[t, c:c + 40].double() - want).abs() <= lim).all()
+
+
 def test_bits(dev):
     """16-bit memory for libraries that know no bf16: the same memory, kept by who holds it, and no other type's"""
     t = give(dev, torch.arange(6, device="cuda", dtype=F32).reshape(2, 3).to(BF16))
