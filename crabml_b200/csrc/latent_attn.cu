@@ -723,10 +723,14 @@ static int lr_portion(cc_device* dev, const cc_page_plan* plan, LrArgs a) {
     a.steps = (int4*)((uint8_t*)ws + qf + lat + part + ml);
     const int slot = (a.cols + 63) / 64 * LR_BLOCK;
     a.slots = std::min(LR_SLOTS, (LR_SMEM - (int)sizeof(LrShared) - 1024) / slot);
+    // of a block of 64 columns: those behind a row's last whole one, and of pages shorter than a step all; of all whole ones
     CUtensorMap map, whole;
-    rc = cc_make_tmap_pages(dev, &map, a.rows, plan->n_pages, plan->page, a.cols, std::min(plan->page, LR_KEYS), 0);
-    if (!rc && a.cols >= 64) rc = cc_make_tmap_pages(dev, &whole, a.rows, plan->n_pages, plan->page, a.cols, std::min(plan->page, LR_KEYS), a.cols / 64);
-    else whole = map;
+    const int box = std::min(plan->page, LR_KEYS);
+    const bool by_blocks = a.cols % 64 || box < LR_KEYS, at_once = a.cols >= 64 && box == LR_KEYS;
+    if (by_blocks) rc = cc_make_tmap_pages(dev, &map, a.rows, plan->n_pages, plan->page, a.cols, box, 0);
+    if (!rc && at_once) rc = cc_make_tmap_pages(dev, &whole, a.rows, plan->n_pages, plan->page, a.cols, box, a.cols / 64);
+    if (!by_blocks) map = whole;
+    if (!at_once) whole = map;
     if (rc) { cc_pool_free(dev, ws, cls); return rc; }
     const unsigned z = (unsigned)std::min(runs.tiles, 64);
     const size_t fold = (size_t)a.dim * (LF_COLS + 8) * 2 + LT_TOKENS * (a.dim + 8) * 2;
