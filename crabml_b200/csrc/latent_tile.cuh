@@ -542,8 +542,9 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
             for (int k = 0; k < steps && ok; k++) {
                 ok = tl_wait_warp(pg_smem(&sh.full[(2 * k + 1) % TL_GROUPS]), ((2 * k + 1) / TL_GROUPS) & 1, &sh.fail);
                 if (ok && k + 1 < steps) ok = tl_wait_warp(pg_smem(&sh.full[(2 * k + 2) % TL_GROUPS]), ((2 * k + 2) / TL_GROUPS) & 1, &sh.fail);
-                if (k < steps0) sg_arrive(pg_smem(&sh.p_full[0]));
-                if (k < steps1) sg_arrive(pg_smem(&sh.p_full[1]));
+                // (narrow heads leave the ring room for two steps: once a step, when the one before is through)
+                if (k < steps0) { if (ok && k > 0) ok = tl_wait_warp(pg_smem(&sh.p_full[0]), (k - 1) & 1, &sh.fail); sg_arrive(pg_smem(&sh.p_full[0])); }
+                if (k < steps1) { if (ok && k > 0) ok = tl_wait_warp(pg_smem(&sh.p_full[1]), (k - 1) & 1, &sh.fail); sg_arrive(pg_smem(&sh.p_full[1])); }
             }
         }
     } else {

@@ -549,3 +549,16 @@ def test_cut_items_not_finite(dev):
         got = attend(dev, c, q, uk, uv, 2, 0.2, 0, None, capi.LATENT_EXPANDED).reshape(n, 2, 32)
         sees = max(0, bad - pos0)
         assert np.isnan(got[sees:]).all() and np.array_equal(got[:sees], clean[:sees])
+
+
+@pytest.mark.parametrize("dim,vdim,rest,rank", [(16, 16, 0, 16), (64, 64, 64, 64), (128, 64, 64, 128), (128, 128, 64, 512)])
+def test_equal_calls_of_many_steps(dev, dim, vdim, rest, rank):
+    """expanded: heads of which shared memory holds several steps, and those of which it holds one; whole items and pieces: equal calls give equal bits"""
+    for pos0, n in ((1200, 300), (7000, 130)):
+        c = Case(dev, 128, rank, rest, [pos0], [n], seed=3)
+        a = [give(dev, (c.rng.normal(size=s) * k).astype(np.float16)) for s, k in (((n, 4 * (dim + rest)), 1.0), ((4 * dim, rank), rank ** -0.5), ((4 * vdim, rank), rank ** -0.5))]
+        plan, pages, first = c.plan(), give(dev, c.a), None
+        for _ in range(60):
+            y = take(dev, paged.latent_attention(plan, pages, rank, a[0], 4, a[1], a[2], 0.1, form=capi.LATENT_EXPANDED))
+            first = y if first is None else first
+            assert np.array_equal(y, first) and np.isfinite(y).all()
