@@ -599,7 +599,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
                 tl_sync(1 + i);
                 const float both = sh.top[i][in_tile];
                 float alpha = 1.0f;
-                if (!(both <= base + TL_LAG)) {
+                if (base == base && !(both <= base + TL_LAG)) {      // (a base that is none stays so: keys behind it that are not seen would hide it)
                     if (base != -INFINITY) alpha = lt_exp2(base - both);
                     base = both;
                 }

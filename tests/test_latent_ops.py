@@ -541,7 +541,7 @@ def test_cut_items(dev, pos0, counts, window, sink):
 def test_cut_items_not_finite(dev):
     """expanded, cut: a row of the cache that is not finite reaches those who see it and no others, whichever piece it lies in"""
     pos0, n = 5000, 200
-    for bad in (10, 3000, pos0 + 150):
+    for bad in (10, 3000, pos0 + 110, pos0 + 119, pos0 + 150):      # also a row's last keys, with steps behind them that it does not see
         c = Case(dev, 64, 64, 16, [pos0], [n], seed=bad)
         q, uk, uv = ((c.rng.normal(size=s) * k).astype(np.float16) for s, k in (((n, 2 * 48), 1.0), ((64, 64), 0.1), ((64, 64), 0.1)))
         clean = attend(dev, c, q, uk, uv, 2, 0.2, 0, None, capi.LATENT_EXPANDED).reshape(n, 2, 32)
