@@ -10,7 +10,7 @@
 // 4500 cycles for the one warp a scheduler that a tile had: 4000 tokens of 16 heads took 147 us.)  TMEM holds both S and both O (512 columns), shared memory
 // Q (96 KB) and a ring of 16 KB blocks of keys and values (128 KB).
 // Now that prompt's call takes 128 us (98.7 GFLOP with its keys and values, 0.77 PFLOP/s); 8000 tokens 359 (0.96 PFLOP/s).  Shared memory bounds the products: S reads 8 KB for each 64 cycles of the tensor core, as fast as
-// it can; then 8 us of start and end for each item.  base lags: a row's sums are scaled only when its largest score is 2^TL_LAG times what it was (sums in TMEM would have
+// it can; then 7 us of start and end for each item.  base lags: a row's sums are scaled only when its largest score is 2^TL_LAG times what it was (sums in TMEM would have
 // to be read and written back), so that weights are up to 2^TL_LAG and f16 still holds them and all that counts beside them.
 // Warps 0-7 and 8-15 the rows of the two tiles, 16 the copies, 17 the products, 18 says what has come.  Every wait is bounded; where one ran out all roles run to their ends and the host reports it.
 #pragma once
