@@ -19,15 +19,14 @@
 #include <algorithm>
 
 #include "latent.cuh"
+#include "latent_ring.cuh"
 #include "split_gemm.cuh"
 
-#define LR_GROUPS 2
 #define LR_THREADS (LR_GROUPS * 256)
 #define LR_BLOCK 4096                         // 32 rows of 64 columns
 #define LR_ROWS 16                            // queries of a tile
 #define LR_KEYS 32                            // of a step
 #define LR_BEGIN 6                            // what a segment's begin and end cost, in steps (64 sequences of 20 to 4000 tokens: counted as 4 59 us, 6 56.5, 9 57)
-#define LR_SLOTS 8                            // most slots of the ring
 #define LR_SMEM (226 * 1024)                  // with what stands in LrShared
 #define LR_SHIFT 10.0f                        // weights are exp2(score - largest + LR_SHIFT)
 #define LR_KB 9                               // column blocks of 16 of a warp's scores: (LT_RANK + LT_REST) / 16 / 4
@@ -294,7 +293,7 @@ __global__ void __launch_bounds__(LU_THREADS) latent_unfold_kernel(const __grid_
 
 // ---- the cached rows as keys and values ----------------------------------------------------------------------------------------------------------
 struct LrShared {
-    unsigned long long full[LR_SLOTS];
+    unsigned long long full[LR_GROUPS * LR_SLOTS];
     int fail;
     unsigned wild;                            // rows whose sums are not finite
     float top[LR_GROUPS][LR_ROWS], sum[LR_GROUPS][LR_ROWS];      // of a segment: largest score and sum of weights of each group
@@ -304,6 +303,7 @@ struct LrShared {
     __align__(16) __half p[LR_GROUPS][LR_ROWS][40];
 };
 static_assert(sizeof(float) * LR_GROUPS * 4 * LR_ROWS * 40 >= LR_THREADS / LR_GROUPS * 16 * sizeof(float) && sizeof(float) * LR_GROUPS * 4 * LR_ROWS * 40 >= LR_ROWS * (LT_RANK + LT_REST + 8) * 2, "half of a group's sums, and the queries, pass here");
+static_assert((LR_SMEM - (int)sizeof(LrShared) - 1024) / ((LT_RANK + LT_REST) / 64 * LR_BLOCK) >= LR_SLOTS_LEAST, "the widest rows leave too few slots");
 __device__ __forceinline__ void lr_sync(int group) { asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(LR_THREADS / LR_GROUPS) : "memory"); }
 __device__ __forceinline__ bool lr_sync_or(int group, bool x) {
     unsigned r;
@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(LR_THREADS, 1) latent_rows_kernel(const __grid
     const int tid = threadIdx.x, lane = tid & 31, group = tid / (LR_THREADS / LR_GROUPS), in_group = tid % (LR_THREADS / LR_GROUPS), warp = in_group >> 5;
     const unsigned ring = (pg_smem(lr_raw) + 1023) & ~1023u, n_blocks = (unsigned)((a.cols + 63) >> 6), slot_bytes = n_blocks * LR_BLOCK;
     if (tid == 0) {
-        for (int i = 0; i < a.slots; i++) pg_mbar_init(pg_smem(&sh.full[i]), 1);
+        for (int i = 0; i < LR_GROUPS * a.slots; i++) pg_mbar_init(pg_smem(&sh.full[i]), 1);
         sh.fail = 0; sh.wild = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_whole) : "memory");
@@ -353,8 +353,9 @@ __global__ void __launch_bounds__(LR_THREADS, 1) latent_rows_kernel(const __grid
     // a step's rows: one copy for all whole blocks of 64 columns of a page, and one for the columns behind them.  (A copy for each block, by all 8 warps, took the group 1000 cycles of a step; row by row,
     // a lane a row, 2500)
     const int box_rows = min(a.page, LR_KEYS), whole = a.cols >> 6;
-    auto ask = [&](int slot, const int4& p) {
-        const unsigned bar = pg_smem(&sh.full[slot]), at = ring + slot * slot_bytes;
+    auto ask = [&](int step, const int4& p) {
+        const LrPlace place = lr_place(step, a.slots);
+        const unsigned bar = pg_smem(&sh.full[place.bar]), at = ring + place.slot * slot_bytes;
         if (pg_elect()) {
             pg_mbar_expect_tx(bar, (unsigned)(p.w * box_rows) * (slot_bytes / LR_KEYS));
             for (int i = 0; i < p.w; i++) {
@@ -391,7 +392,7 @@ __global__ void __launch_bounds__(LR_THREADS, 1) latent_rows_kernel(const __grid
     auto again = [&]() {                                              // (all warps of the group are through with step `last`)
         if (last < 0) return;
         if (warp == 0) {
-            if (next.w && ok) ask(last % a.slots, next);
+            if (next.w && ok) ask(last + a.slots, next);
             coming += LR_GROUPS;
             next = what(coming);
         }
@@ -445,12 +446,13 @@ __global__ void __launch_bounds__(LR_THREADS, 1) latent_rows_kernel(const __grid
         for (int i = 0; i < LR_VB; i++)
 #pragma unroll
             for (int x = 0; x < 8; x++) o[i][x >> 2][x & 3] = 0.0f;
-        const int skip = (n + group) & 1;                             // the run's even steps are group 0's
+        const int skip = (n + group) % LR_GROUPS;                       // the run's even steps are group 0's
 #pragma unroll 1
         for (int k = k0 + skip; k < k1; k += LR_GROUPS) {
-            const int here = n + k - k0, slot = here % a.slots;
-            ok = ok && sg_wait_warp(pg_smem(&sh.full[slot]), (unsigned)(here / a.slots) & 1u, &sh.fail);
-            const unsigned at = ring + slot * slot_bytes;
+            const int here = n + k - k0;
+            const LrPlace place = lr_place(here, a.slots);
+            ok = ok && sg_wait_warp(pg_smem(&sh.full[place.bar]), place.parity, &sh.fail);
+            const unsigned at = ring + place.slot * slot_bytes;
             float x[2][4];
 #pragma unroll
             for (int i = 0; i < 8; i++) x[i >> 2][i & 3] = 0.0f;

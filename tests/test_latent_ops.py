@@ -562,3 +562,19 @@ def test_equal_calls_of_many_steps(dev, dim, vdim, rest, rank):
             y = take(dev, paged.latent_attention(plan, pages, rank, a[0], 4, a[1], a[2], 0.1, form=capi.LATENT_EXPANDED))
             first = y if first is None else first
             assert np.array_equal(y, first) and np.isfinite(y).all()
+
+
+@pytest.mark.parametrize("rank,rest", [(512, 64), (512, 16), (384, 48), (256, 64)])
+def test_equal_calls_of_long_rings(dev, rank, rest):
+    """absorbed: rows of which the ring holds an odd number of steps (nine blocks of 64 columns 5, seven 7), and an even one: equal calls give equal bits, with all SMs asking at once"""
+    H, dim, vdim = 16, 32, 32
+    r = np.random.default_rng(rank + rest)
+    pos0 = [int(x) for x in r.integers(20, 1500, size=64)]
+    c = Case(dev, 32, rank, rest, pos0, [1] * 64, seed=rest)
+    q, uk, uv = ((c.rng.normal(size=s) * k).astype(np.float16) for s, k in (((64, H * (dim + rest)), 1.0), ((H * dim, rank), rank ** -0.5), ((H * vdim, rank), rank ** -0.5)))
+    plan, pages, t, first = c.plan(), give(dev, c.a), [give(dev, x) for x in (q, uk, uv)], None
+    for _ in range(100):
+        y = take(dev, paged.latent_attention(plan, pages, rank, t[0], H, t[1], t[2], 0.15, form=capi.LATENT_ABSORBED))
+        first = y if first is None else first
+        assert np.array_equal(y, first)
+    check(dev, c, H, dim, vdim, 0.15, form=capi.LATENT_ABSORBED, q=q, uk=uk, uv=uv)
