@@ -649,6 +649,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
             l += sums.x + sums.y;
         }
         if (mine > 0) {
+            tl_sync(1 + i);                                           // the last step's largest scores are read
             if (half) sh.top[i][in_tile] = l;
             tl_sync(1 + i);
             if (!half) sh.top[i][in_tile] += l;

@@ -578,3 +578,17 @@ def test_equal_calls_of_long_rings(dev, rank, rest):
         first = y if first is None else first
         assert np.array_equal(y, first)
     check(dev, c, H, dim, vdim, 0.15, form=capi.LATENT_ABSORBED, q=q, uk=uk, uv=uv)
+
+
+@pytest.mark.parametrize("dim,vdim,rest,rank", [(16, 16, 0, 16), (128, 128, 64, 128)])
+def test_equal_calls_of_one_step(dev, dim, vdim, rest, rank):
+    """expanded: items of a single step of 128 keys, in which each row's base moves and its sum follows at once, and of two: equal calls give equal bits"""
+    H = 8
+    c = Case(dev, 32, rank, rest, [0, 0, 3, 100, 0, 90], [128, 1, 125, 28, 77, 60], seed=rank)
+    q, uk, uv = ((c.rng.normal(size=s) * k).astype(np.float16) for s, k in (((sum(c.counts), H * (dim + rest)), 1.0), ((H * dim, rank), rank ** -0.5), ((H * vdim, rank), rank ** -0.5)))
+    plan, pages, t, first = c.plan(), give(dev, c.a), [give(dev, x) for x in (q, uk, uv)], None
+    for _ in range(200):
+        y = take(dev, paged.latent_attention(plan, pages, rank, t[0], H, t[1], t[2], 0.2, form=capi.LATENT_EXPANDED))
+        first = y if first is None else first
+        assert np.array_equal(y, first)
+    check(dev, c, H, dim, vdim, 0.2, form=capi.LATENT_EXPANDED, q=q, uk=uk, uv=uv)
