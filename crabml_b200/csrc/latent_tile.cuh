@@ -257,9 +257,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TE_THREADS, 1) laten
         const int q = warp & 3, row = q * 32 + lane, is_v = (warp - 4) >> 2, d = is_v ? a.vdim : a.dim;
         const bool in = key0 + row < to;
         uint8_t* stage = bs + TE_STAGES * TE_STAGE + is_v * TL_BLOCK;
-        for (int h = h0; h < h1; h++) {
+        lt_rounds(h0, h1, [&](int h) { return tl_wait_warp(pg_smem(&sh.acc_full[(h - h0) & 1]), (unsigned)(h - h0) >> 1 & 1u, &sh.fail); }, [&](int h, bool ok) {
             const unsigned n = (unsigned)(h - h0);
-            if (!tl_wait_warp(pg_smem(&sh.acc_full[n & 1u]), (n >> 1) & 1u, &sh.fail)) break;
             pg_fence_after();
             uint8_t* image = (is_v ? t.v_image : t.k_image) + ((size_t)blockIdx.x * t.heads + h) * ((d + 63) >> 6) * TL_BLOCK;
 #pragma unroll 1
@@ -267,7 +266,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TE_THREADS, 1) laten
                 unsigned v[4][16];
 #pragma unroll
                 for (int x = 0; x < 4; x++)
-                    if (c + x * 16 < d) sg_tmem16(tmem + (n & 1u) * 256 + ((unsigned)(q * 32) << 16) + is_v * wide + c + x * 16, v[x]);
+                    if (ok && c + x * 16 < d) sg_tmem16(tmem + (n & 1u) * 256 + ((unsigned)(q * 32) << 16) + is_v * wide + c + x * 16, v[x]);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                 if (row == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the block before has left
                 te_sync(is_v);
@@ -275,7 +274,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TE_THREADS, 1) laten
                 for (int x = 0; x < 4; x++) {
 #pragma unroll
                     for (int j = 0; j < 16; j++) asm volatile("" : "+r"(v[x][j]));
-                    if (c + x * 16 >= d) continue;
+                    if (!ok || c + x * 16 >= d) continue;
                     unsigned w[8], wild = 0;
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
@@ -299,7 +298,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TE_THREADS, 1) laten
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 te_sync(is_v);
-                if (row == 0 && (int)blockIdx.x < t.key_tiles) {
+                if (row == 0 && ok && (int)blockIdx.x < t.key_tiles) {
                     asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(image + (c >> 6) * TL_BLOCK), "r"(pg_smem(stage)), "r"(TL_BLOCK) : "memory");
                     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                 }
@@ -307,7 +306,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TE_THREADS, 1) laten
             pg_fence_before();
             __syncwarp();
             if (lane == 0) pg_arrive_relaxed(te_even(pg_smem(&sh.acc_empty[n & 1u])));
-        }
+        });
         if (row == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     pg_fence_before();
