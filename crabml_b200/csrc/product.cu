@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) product_few_kernel(const __grid
 #pragma unroll
             for (int i = 0; i < AHEAD; i++) {
                 const int run = warp + (i0 + i) * PF_WARPS, n = a.k - run * 32 - (lane & 3) * 8;
-                multiply(acc, ODD ? pr_join(u[i], u2[i], off, n) : u[i], ODD ? pr_join(v[i], v2[i], off, n) : v[i], min(run, all - 1));      // (runs behind the last one: weights 0)
+                if (run < all) multiply(acc, ODD ? pr_join(u[i], u2[i], off, n) : u[i], ODD ? pr_join(v[i], v2[i], off, n) : v[i], run);      // (one for the warp)
             }
 #pragma unroll
             for (int n = 0; n < NT; n++)

@@ -239,3 +239,22 @@ def test_refusals(dev):
             f()
     other.close()
     check(dev, *make(4, 20, 64, BF16, BF16)[:2])
+
+
+@pytest.mark.parametrize("w", [F16, BF16], ids=str)
+@pytest.mark.parametrize("k", [128, 512, 1000, 1001, 2048, 3000])
+@pytest.mark.parametrize("rows", [1, 8, 16, 40, 140])
+def test_infinities(dev, rows, k, w):
+    """an infinity in a row of x, in its last columns too, gives that row infinities of the weights' signs, by every kernel; one in W its column"""
+    a, x, _, _ = make(rows, 70, k, w, w, k)
+    a[a == 0] = 1.0
+    for at in (k - 1, k - 20, 3):
+        b = x.clone()
+        b[rows // 2, at], b[0, k // 2] = float("inf"), -float("inf")
+        got, want = take(dev, seqops.product(give(dev, a), give(dev, b))).to(F), b.to(F) @ a.to(F).T
+        for v in (float("inf"), -float("inf")):
+            assert torch.equal(got == v, want == v)
+        assert torch.equal(got.isnan(), want.isnan())
+    a[9, k - 2] = float("inf")
+    got, want = take(dev, seqops.product(give(dev, a), give(dev, x))).to(F), x.to(F) @ a.to(F).T
+    assert torch.equal(got == float("inf"), want == float("inf")) and torch.equal(got == -float("inf"), want == -float("inf")) and torch.equal(got.isnan(), want.isnan())
