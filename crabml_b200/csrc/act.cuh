@@ -6,7 +6,7 @@
 __device__ __forceinline__ float act_silu(float z) { return z / (1.0f + expf(-z)); }
 __device__ __forceinline__ float act_sigmoid(float z) { return 1.0f / (1.0f + expf(-z)); }
 __device__ __forceinline__ float act_gelu_tanh(float z) { return 0.5f * z * (1.0f + tanhf(0.7978845608028654f * (z + 0.044715f * z * z * z))); }
-__device__ __forceinline__ float act_relu_squared(float z) { const float r = fmaxf(z, 0.0f); return r * r; }
+__device__ __forceinline__ float act_relu_squared(float z) { const float r = z < 0.0f ? 0.0f : z; return r * r; }      // (fmaxf would make 0 of a NaN)
 // alpha: CC_ACT_SWISH only
 __device__ __forceinline__ float act_apply(float z, int act, float alpha = 1.0f) {
     switch (act) {

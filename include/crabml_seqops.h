@@ -22,7 +22,7 @@ extern "C" {
 #endif
 
 /* CC_ACT_SWISH: z * sigmoid(alpha * z) with alpha given beside it (cc_glu_params; 1 elsewhere); the others take no constant.
- * CC_ACT_RELU_SQUARED: max(z, 0)^2. */
+ * CC_ACT_RELU_SQUARED: max(z, 0)^2.  A NaN stays one under all of them. */
 enum cc_activation { CC_ACT_NONE = 0, CC_ACT_SILU = 1, CC_ACT_GELU_TANH = 2, CC_ACT_SWISH = 3, CC_ACT_SIGMOID = 4, CC_ACT_RELU_SQUARED = 5 };
 
 /* The device address of a plain tensor's first element (NULL: a quantised one), for kernels and libraries of the caller's own: it stays valid while the caller

@@ -56,6 +56,20 @@ def test_activations_in_place(dev):
         assert np.abs(seqops.activate_inplace(T32(dev, z), act).export() - w).max() < 1e-5, act
 
 
+@pytest.mark.parametrize("act", [capi.ACT_NONE, capi.ACT_SILU, capi.ACT_GELU_TANH, capi.ACT_SWISH, capi.ACT_SIGMOID, capi.ACT_RELU_SQUARED])
+@pytest.mark.parametrize("T", [1, 40])
+def test_activations_keep_a_nan(dev, act, T):
+    z = np.linspace(-2, 2, 9)
+    z[4] = np.nan
+    assert np.array_equal(np.isnan(seqops.activate_inplace(T32(dev, z), act).export()), np.isnan(z))
+    rng = np.random.default_rng(T)
+    x, wu, wd = rng.standard_normal((T, 64)), rng.standard_normal((128, 64)) / 8, rng.standard_normal((64, 128)) / 12
+    x[T // 2, 5] = np.nan
+    for dtype in (capi.F32, capi.BF16):
+        got = out(seqops.feed_forward_act(T32(dev, x), W(dev, wu, dtype), W(dev, wd, dtype), act), T, 64)
+        assert np.isnan(got[T // 2]).all() and np.isfinite(np.delete(got, T // 2, 0)).all()
+
+
 def test_softcap(dev):
     z = np.array([0.0, 0.3, -4.0, 29.0, 500.0, -1e4])
     assert np.abs(seqops.softcap_inplace(T32(dev, z), 7.5).export() - R.soft_cap(z, 7.5)).max() < 1e-5

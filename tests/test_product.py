@@ -258,3 +258,28 @@ def test_infinities(dev, rows, k, w):
     a[9, k - 2] = float("inf")
     got, want = take(dev, seqops.product(give(dev, a), give(dev, x))).to(F), x.to(F) @ a.to(F).T
     assert torch.equal(got == float("inf"), want == float("inf")) and torch.equal(got == -float("inf"), want == -float("inf")) and torch.equal(got.isnan(), want.isnan())
+
+
+@pytest.mark.parametrize("act", [capi.ACT_NONE, capi.ACT_SILU, capi.ACT_GELU_TANH, capi.ACT_SWISH, capi.ACT_SIGMOID, capi.ACT_RELU_SQUARED])
+@pytest.mark.parametrize("out", [F32, F16, BF16], ids=str)
+@pytest.mark.parametrize("rows", [1, 12, 40, 140])
+def test_activations_of_numbers_that_are_not_finite(dev, rows, out, act):
+    """a NaN stays one under every activation, an infinity has the activation's limit; with and without a residual"""
+    w, x, bias, res = make(rows, 70, 512, F16, F16, 3)
+    w = w.abs() + 2.0 ** -10
+    x[rows // 2, 500] = float("nan")
+    if rows > 2:
+        x[0, 500], x[2, 500] = float("inf"), -float("inf")
+    for r in (None, res.to(out)):
+        got = take(dev, seqops.product(give(dev, w), give(dev, x), bias=give(dev, bias), act=act, residual=None if r is None else give(dev, r), out_type=TYPES[out])).to(F)
+        assert got[rows // 2].isnan().all() and torch.isfinite(got[3:rows // 2]).all() and torch.isfinite(got[rows // 2 + 1:] if rows > 2 else got[1:]).all()
+        if rows > 2:
+            up = 1.0 if act == capi.ACT_SIGMOID else float("inf")
+            low = {capi.ACT_NONE: -float("inf"), capi.ACT_SIGMOID: 0.0, capi.ACT_RELU_SQUARED: 0.0}.get(act)
+            for row, limit in ((0, up), (2, low)):
+                if limit is not None:
+                    want = torch.full((70,), limit, dtype=F, device="cuda") + (0.0 if r is None else r[row].to(out).to(F))
+                    assert torch.equal(torch.isinf(got[row]), torch.isinf(want)) and torch.equal(got[row].sign(), want.sign())
+                    fine = torch.isfinite(want)
+                    # one rounding of the sum, beside a 32-bit step of a sigmoid of an infinity
+                    assert ((got[row] - want)[fine].abs() <= (EPS[out] + 2.0 ** -23) * want[fine].abs() + 2.0 ** -25).all()
