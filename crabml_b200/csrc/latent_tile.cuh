@@ -376,6 +376,19 @@ __device__ __forceinline__ float tl_max3(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
+// whether 8 numbers of a query at a time, from the `from`-th on, every `step`-th, hold one that is not finite.  A row all of whose scores are -infinity has sums of 0, which a sink makes a result of 0:
+// right where its keys make them so, but a query that is not finite has the result NaN
+__device__ __forceinline__ bool tl_wild(const LrArgs& a, int64_t token, int head, int from, int step) {
+    const int n = (a.dim + a.rest) / 8;
+    const uint4* q = (const uint4*)(a.q + (token * a.H + head) * (a.dim + a.rest));
+    unsigned wild = 0;
+#pragma unroll 1
+    for (int i = from; i < n; i += step) {
+        const uint4 v = q[i];
+        wild |= ((v.x & 0x7c007c00u) + 0x04000400u) | ((v.y & 0x7c007c00u) + 0x04000400u) | ((v.z & 0x7c007c00u) + 0x04000400u) | ((v.w & 0x7c007c00u) + 0x04000400u);
+    }
+    return wild & 0x80008000u;
+}
 // grid: pieces of items x heads, heads fastest
 __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ TlArgs t, unsigned* err_dev,
                                                                     unsigned* err_host) {
@@ -665,7 +678,8 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
                 g = exp2f(base - m2);
                 total = g * l + (sk == -INFINITY ? 0.0f : exp2f(sk - m2));
             }
-            const float by = base != base ? NAN : g / total;
+            const bool none = base != base || (base == -INFINITY && row < s.count && tl_wild(a, s.first + row, head, 0, 1));
+            const float by = none ? NAN : g / total;
             uint16_t* out = (uint16_t*)a.out + ((int64_t)(s.first + row) * a.H + head) * a.vdim;
 #pragma unroll 1
             for (int c = half * 16; c < a.vdim; c += 32) {
@@ -713,8 +727,9 @@ __global__ void __launch_bounds__(256) latent_tile_join_kernel(const __grid_cons
     const int64_t at = ((int64_t)(slot + (tl_items(s, a) - 1 - item) * pieces) * t.heads + head_at) * (2 * TL_ROWS) + row % (2 * TL_ROWS), stride = (int64_t)t.heads * 2 * TL_ROWS;
     const float sk = a.sink ? a.sink[t.head0 + head_at] * LR_LOG2E : -INFINITY;
     float m = sk;
-    bool none = false;                                               // a score that is none
-    for (int p = 0; p < pieces; p++) { const float b = t.ml[at + p * stride].x; none |= b != b; m = fmaxf(m, b); }
+    bool none = false, seen = false;                                 // a score that is none, one that is not -infinity
+    for (int p = 0; p < pieces; p++) { const float b = t.ml[at + p * stride].x; none |= b != b; seen |= b != -INFINITY; m = fmaxf(m, b); }
+    if (!seen) none = __any_sync(0xffffffffu, tl_wild(a, s.first + row, t.head0 + head_at, lane, 32));
     float total = sk == -INFINITY ? 0.0f : exp2f(sk - m);
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4

@@ -99,8 +99,8 @@ CC_API int cc_paged_latent_append(cc_device* dev, const cc_page_plan* plan, cons
  * Workspace, which the device's pool keeps: absorbed, the queries and sums over the latents of as many tokens as have them in 256 MB, beside 10 MB of sums and 16 bytes for every 32 rows
  * that 16 queries see; expanded, keys and values of a call's
  * visible rows, 64 columns and 128 tokens at a time, within 256 MB or those of one sequence and head, beside some 30 MB of sums.  Expanded keys and values beyond the range of 16 bits count as its largest; uk and uv are finite.
- * A row of the cache that is not finite reaches the results of the queries that see it and no others; a query that holds a NaN or an infinity has the result NaN; rows behind a
- * sequence's end are not looked at.  Equal calls give equal bits on a device. */
+ * A row of the cache that is not finite reaches the results of the queries that see it and no others (a key whose score is -infinity by its r has the weight 0); a query that holds a NaN or an
+ * infinity has the result NaN; rows behind a sequence's end are not looked at.  Equal calls give equal bits on a device. */
 enum cc_latent_form { CC_LATENT_AUTO = 0, CC_LATENT_ABSORBED = 1, CC_LATENT_EXPANDED = 2 };
 CC_API int cc_paged_latent_attention(cc_device* dev, const cc_page_plan* plan, const cc_view* pages, int32_t rank, const cc_view* q, int32_t n_heads, const cc_view* uk,
                                      const cc_view* uv, float scale, int32_t window, const cc_view* sink, int32_t form, int32_t out_type, cc_buf** out);

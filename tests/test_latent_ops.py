@@ -592,3 +592,34 @@ def test_equal_calls_of_one_step(dev, dim, vdim, rest, rank):
         first = y if first is None else first
         assert np.array_equal(y, first)
     check(dev, c, H, dim, vdim, 0.2, form=capi.LATENT_EXPANDED, q=q, uk=uk, uv=uv)
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("with_sink", [False, True])
+@pytest.mark.parametrize("pos0,counts", [([40], [20]), ([5000], [70]), ([0, 3000, 7], [1, 130, 3])])
+def test_scores_of_minus_infinity(dev, form, with_sink, pos0, counts):
+    """a query with an infinity that makes all of its scores -infinity has the result NaN, beside a sink too, whole or cut into pieces; a query that is finite sees such a key with the weight 0: beside a
+    sink 0 where there is no other key, and NaN without one"""
+    H, dim, vdim, rank, rest = 3, 32, 32, 64, 16
+    c = Case(dev, 64, rank, rest, pos0, counts, seed=sum(pos0))
+    for i, n in enumerate(counts):
+        rows = c.rows(i, pos0[i] + n)
+        rows[:, rank] = -np.abs(rows[:, rank]) - np.float16(0.5)
+        c.put(i, 0, rows)
+    T = sum(counts)
+    q = c.rng.normal(size=(T, H, dim + rest)).astype(np.float16)
+    q[-1, 1, dim] = np.inf
+    if T > 2:
+        q[T - 3, 0, dim], q[T - 2, 2, dim] = np.inf, np.inf
+    sink = np.array([0.5, -1.0, 2.0], np.float32) if with_sink else None
+    check(dev, c, H, dim, vdim, 0.2, sink=sink, form=FORMS[form], q=q.reshape(T, -1))
+    # now keys: every row's r is -infinity in a column that queries weigh by a positive number
+    for i, n in enumerate(counts):
+        rows = c.rows(i, pos0[i] + n)
+        rows[:, rank] = -np.inf
+        c.put(i, 0, rows)
+    q = np.abs(q) + np.float16(0.25)
+    q[~np.isfinite(q)] = 1.0
+    uk, uv = ((c.rng.normal(size=s) * rank ** -0.5).astype(np.float16) for s in ((H * dim, rank), (H * vdim, rank)))
+    got = attend(dev, c, q.reshape(T, -1), uk, uv, H, 0.2, 0, sink, FORMS[form])
+    assert (got == 0).all() if with_sink else np.isnan(got).all()
