@@ -312,15 +312,18 @@ __device__ __forceinline__ bool lr_sync_or(int group, bool x) {
 }
 __device__ __forceinline__ void lr_zero(unsigned at) { asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory"); }
 // Values that are not finite, times the weight 0 of a row that does not see them, make a NaN.  Rows whose sums hold one though their scores do not are added up again, one by one, over
-// the keys that they see: a dot product over the block, which then adds a column a thread.
-__device__ __noinline__ void lr_again(const LrArgs& a, LrShared& sh, const PgSeq s, int seq, int row0, int lo, int hi, float m, float by, int r, float* lat) {
+// the keys that they see: a dot product over the block, which then adds a column a thread.  The query is rounded as it was, so that a cut segment's other pieces go with this one; the largest score
+// and the sum of weights are made again with the sums, whose scores are added up in another order
+__device__ __noinline__ float lr_again(const LrArgs& a, LrShared& sh, const PgSeq s, int seq, int row0, int lo, int hi, int r, float& m, float& l) {
     const int tok = (row0 + r) / a.H, pos = s.pos0 + tok, c = threadIdx.x;
     const float* q = a.qf + ((int64_t)s.first * a.H + row0 + r) * a.cols;
+    const float factor = sh.factor[r], up = 1.0f / factor;          // a power of two
     float o = 0.0f;
+    m = -INFINITY; l = 0.0f;
     for (int key = max(lo, a.window > 0 ? pos - a.window + 1 : 0); key <= min(hi - 1, pos); key++) {
         const __half* row = a.rows + ((int64_t)a.table[(int64_t)seq * a.table_cols + (key >> a.shift)] * a.page + (key & (a.page - 1))) * a.cols;
         float d = 0.0f;
-        for (int e = threadIdx.x; e < a.cols; e += LR_THREADS) d = fmaf(q[e], __half2float(row[e]), d);
+        for (int e = threadIdx.x; e < a.cols; e += LR_THREADS) d = fmaf(__half2float(__float2half_rn(q[e] * up)), __half2float(row[e]), d);
         d = warp_sum(d);
         if ((threadIdx.x & 31) == 0) sh.sums[0][0][0][threadIdx.x >> 5] = d;
         __syncthreads();
@@ -328,10 +331,12 @@ __device__ __noinline__ void lr_again(const LrArgs& a, LrShared& sh, const PgSeq
 #pragma unroll
         for (int w = 0; w < LR_THREADS / 32; w++) d += sh.sums[0][0][0][w];
         __syncthreads();
-        const float p = lt_exp2(d * (a.scale * LR_LOG2E) - m + LR_SHIFT);
-        if (c < a.rank) o = fmaf(p, __half2float(row[c]), o);
+        const float z = d * (factor * (a.scale * LR_LOG2E)), m_new = fmaxf(m, z), alpha = m == m_new ? 1.0f : lt_exp2(m - m_new), p = lt_exp2(z - (m_new == -INFINITY ? 0.0f : m_new) + LR_SHIFT);
+        m = m_new;
+        l = fmaf(l, alpha, p);
+        if (c < a.rank) o = fmaf(p, __half2float(row[c]), o * alpha);
     }
-    if (c < a.rank) lat[c] = o * by;
+    return o;
 }
 static_assert(LR_THREADS >= LT_RANK, "a thread a column");
 
@@ -591,16 +596,19 @@ __global__ void __launch_bounds__(LR_THREADS, 1) latent_rows_kernel(const __grid
         if (__syncthreads_or(wild != 0)) {
             for (unsigned left = sh.wild; left; left &= left - 1) {
                 const int r = __ffs(left) - 1;
-                const float m0 = sh.top[0][r], m1 = sh.top[1][r];
-                const float mm = fmaxf(m0, m1), l0 = sh.sum[0][r], l1 = sh.sum[1][r];
-                const float f0 = m0 == -INFINITY ? 0.0f : lt_exp2(m0 - mm), f1 = m1 == -INFINITY ? 0.0f : lt_exp2(m1 - mm);
-                float total = f0 * l0 + f1 * l1, g = 1.0f;
-                if (!cut && a.sink) {
-                    const float sk = a.sink[(row0 + r) % a.H] * LR_LOG2E, m2 = fmaxf(mm, sk);
-                    g = exp2f(mm - m2);
-                    total = g * total + (sk == -INFINITY ? 0.0f : exp2f(sk - m2 + LR_SHIFT));
+                float m, l, g = 1.0f;
+                const float sum = lr_again(a, sh, s, seq, row0, from + k0 * LR_KEYS, min(to, from + k1 * LR_KEYS), r, m, l);
+                if (cut) {
+                    if (tid == 0) a.ml[(size_t)place * LR_ROWS + r] = make_float2(m, l);
+                } else {
+                    if (a.sink) {
+                        const float sk = a.sink[(row0 + r) % a.H] * LR_LOG2E, m2 = fmaxf(m, sk);
+                        g = m == -INFINITY ? 0.0f : exp2f(m - m2);
+                        l = g * l + (sk == -INFINITY ? 0.0f : exp2f(sk - m2 + LR_SHIFT));
+                    }
+                    g /= l;
                 }
-                lr_again(a, sh, s, seq, row0, from + k0 * LR_KEYS, min(to, from + k1 * LR_KEYS), mm, cut ? 1.0f : g / total, r, lat + (int64_t)r * a.rank);
+                if (tid < a.rank) lat[(int64_t)r * a.rank + tid] = sum * g;
             }
             __syncthreads();
         }

@@ -623,3 +623,28 @@ def test_scores_of_minus_infinity(dev, form, with_sink, pos0, counts):
     uk, uv = ((c.rng.normal(size=s) * rank ** -0.5).astype(np.float16) for s in ((H * dim, rank), (H * vdim, rank)))
     got = attend(dev, c, q.reshape(T, -1), uk, uv, H, 0.2, 0, sink, FORMS[form])
     assert (got == 0).all() if with_sink else np.isnan(got).all()
+
+
+@pytest.mark.parametrize("with_sink", [False, True])
+@pytest.mark.parametrize("pos0,counts,P", [([0], [3], 16), ([20, 0], [4, 2], 32), ([5000], [3], 64), ([700, 40], [2, 6], 16)])
+def test_large_scores_beside_rows_that_are_not_finite(dev, pos0, counts, P, with_sink):
+    """rows whose neighbours in a tile see a NaN, which they do not: where all their keys have one and the same latent row, the result is its value whatever the scores, here in the hundreds and thousands"""
+    H, dim, vdim, rank, rest = 5, 64, 32, 128, 32
+    c = Case(dev, P, rank, rest, pos0, counts, seed=P)
+    uk, uv = ((c.rng.normal(size=s) * k).astype(np.float16) for s, k in (((H * dim, rank), 0.5), ((H * vdim, rank), rank ** -0.5)))
+    T, at = sum(counts), 0
+    q = (8.0 * c.rng.normal(size=(T, H, dim + rest))).astype(np.float16)
+    sink = np.full(H, -1e30, np.float32) if with_sink else None
+    same = []
+    for i, n in enumerate(counts):
+        row = c.rng.normal(size=rank + rest).astype(np.float16)
+        c.put(i, 0, np.tile(row, (pos0[i] + n, 1)))
+        c.put(i, pos0[i] + n - 1, np.full((1, rank + rest), np.nan, np.float16))
+        same.append(uv.astype(np.float64).reshape(H, vdim, rank) @ row[:rank].astype(np.float64))
+    got = attend(dev, c, q.reshape(T, -1), uk, uv, H, 1.0, 0, sink, capi.LATENT_ABSORBED, capi.F16).reshape(T, H, vdim)
+    for i, n in enumerate(counts):
+        assert np.isnan(got[at + n - 1]).all()
+        # the same weights over and under the line: their roundings to f16, 2^-11 each where one has all of the weight, the result's own, and what is left of latents in two f16 numbers
+        size = np.abs(uv.astype(np.float64)).reshape(H, vdim, rank).sum(2) * 4
+        assert (np.abs(got[at:at + n - 1] - same[i]) <= 2.0 ** -11 * np.abs(same[i]) * 2 + 2.0 ** -20 * size).all()
+        at += n
