@@ -93,12 +93,13 @@ __device__ __forceinline__ unsigned lt_pack(float x, float y) {
     const __half2 h = __floats2half2_rn(x, y);
     return *(const unsigned*)&h;
 }
-// x, y as f16 (h) and what is left of them as f16 (l); an infinity's or NaN's rest is NaN
+// x, y as f16 (h) and LT_UP times what is left of them as f16 (l), at most |x|, so that small numbers, which f16 holds in steps of 2^-24, keep their bits; an infinity's or NaN's rest is NaN
+#define LT_UP 2048.0f
 __device__ __forceinline__ void lt_cut(float x, float y, unsigned& h, unsigned& l) {
     const __half2 a = __floats2half2_rn(x, y);
     const float2 b = __half22float2(a);
     h = *(const unsigned*)&a;
-    l = lt_pack(x - b.x, y - b.y);
+    l = lt_pack((x - b.x) * LT_UP, (y - b.y) * LT_UP);
 }
 __device__ __forceinline__ void lt_copy16(unsigned dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void lt_copies_done() { asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory"); }
@@ -275,7 +276,7 @@ __global__ void __launch_bounds__(LU_THREADS) latent_unfold_kernel(const __grid_
 #pragma unroll
             for (int y = 0; y < 2; y++) {
                 const int t = m * 16 + (lane >> 2) + y * 8;
-                if (part == 1) { sums[t][c] = acc[m][0][2 * y] + acc[m][1][2 * y]; sums[t][c + 1] = acc[m][0][2 * y + 1] + acc[m][1][2 * y + 1]; }
+                if (part == 1) { sums[t][c] = fmaf(acc[m][1][2 * y], 1.0f / LT_UP, acc[m][0][2 * y]); sums[t][c + 1] = fmaf(acc[m][1][2 * y + 1], 1.0f / LT_UP, acc[m][0][2 * y + 1]); }
             }
         __syncthreads();
         if (part == 0) {
@@ -284,7 +285,7 @@ __global__ void __launch_bounds__(LU_THREADS) latent_unfold_kernel(const __grid_
 #pragma unroll
                 for (int y = 0; y < 2; y++) {
                     const int t = m * 16 + (lane >> 2) + y * 8;
-                    const float u = acc[m][0][2 * y] + acc[m][1][2 * y] + sums[t][c], v = acc[m][0][2 * y + 1] + acc[m][1][2 * y + 1] + sums[t][c + 1];
+                    const float u = fmaf(acc[m][1][2 * y], 1.0f / LT_UP, acc[m][0][2 * y]) + sums[t][c], v = fmaf(acc[m][1][2 * y + 1], 1.0f / LT_UP, acc[m][0][2 * y + 1]) + sums[t][c + 1];
                     if (lo + t < hi && c0 + c < a.vdim) *(unsigned*)((uint16_t*)a.out + ((int64_t)(lo + t) * a.H + h) * a.vdim + c0 + c) = a.out_bf16 ? ht_pack_bf16(u, v) : ht_pack_f16(u, v);
                 }
         }

@@ -648,3 +648,27 @@ def test_large_scores_beside_rows_that_are_not_finite(dev, pos0, counts, P, with
         size = np.abs(uv.astype(np.float64)).reshape(H, vdim, rank).sum(2) * 4
         assert (np.abs(got[at:at + n - 1] - same[i]) <= 2.0 ** -11 * np.abs(same[i]) * 2 + 2.0 ** -20 * size).all()
         at += n
+
+
+@pytest.mark.parametrize("rank,size", [(512, 1e-5), (512, 1.0), (80, 3e-6), (256, 60000.0)])
+@pytest.mark.parametrize("pos0,counts", [([6], [1]), ([3000], [2]), ([20, 0, 90], [1, 3, 2])])
+def test_small_latents_keep_their_bits(dev, rank, size, pos0, counts):
+    """absorbed: latents whose mean lies where f16 has steps of a hundredth of it, and large ones; queries of zeros, so that all weights are one number and nothing else is rounded"""
+    H, dim, vdim = 3, 16, 48
+    c = Case(dev, 32, rank, 16, pos0, counts, seed=rank)
+    for i, n in enumerate(counts):
+        rows = c.rng.normal(size=(pos0[i] + n, rank + 16)) * min(size, 15000.0)
+        c.put(i, 0, np.clip(rows, -65504, 65504).astype(np.float16))
+    T, at = sum(counts), 0
+    uk, uv = c.rng.normal(size=(H * dim, rank)).astype(np.float16), (c.rng.normal(size=(H * vdim, rank)) * rank ** -0.5 * min(200.0 / size ** 0.5, 200.0, 10.0 / size)).astype(np.float16)
+    got = attend(dev, c, np.zeros((T, H * (dim + 16)), np.float16), uk, uv, H, 0.1, 0, None, capi.LATENT_ABSORBED, capi.F16).reshape(T, H, vdim)
+    V = uv.astype(np.float64).reshape(H, vdim, rank)
+    for i, n in enumerate(counts):
+        rows = c.rows(i, pos0[i] + n)[:, :rank].astype(np.float64)
+        for t in range(n):
+            lat = rows[:pos0[i] + t + 1].mean(0)
+            want, terms = V @ lat, np.abs(V) @ np.abs(rows[:pos0[i] + t + 1]).mean(0)
+            # the result's rounding; sums over up to 3000 keys and 512 columns in 32 bits, of which the tensor cores cut off 2^-23 of the sum after every 16 terms
+            lim = 2.0 ** -11 * np.abs(want) + (len(rows) / 16 + rank / 16 + 8) * 2.0 ** -23 * terms + 2.0 ** -25
+            assert (np.abs(got[at + t] - want) <= lim).all(), float((np.abs(got[at + t] - want) / lim).max())
+        at += n
