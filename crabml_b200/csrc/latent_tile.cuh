@@ -10,8 +10,9 @@
 // 4500 cycles for the one warp a scheduler that a tile had: 4000 tokens of 16 heads took 147 us.)  TMEM holds both S and both O (512 columns), shared memory
 // Q (96 KB) and a ring of 16 KB blocks of keys and values (128 KB).
 // Now that prompt's call takes 128 us (98.7 GFLOP with its keys and values, 0.77 PFLOP/s); 8000 tokens 359 (0.96 PFLOP/s).  Shared memory bounds the products: S reads 8 KB for each 64 cycles of the tensor core, as fast as
-// it can; then 7 us of start and end for each item.  base lags: a row's sums are scaled only when its largest score is 2^TL_LAG times what it was (sums in TMEM would have
-// to be read and written back), so that weights are up to 2^TL_LAG and f16 still holds them and all that counts beside them.
+// it can; then 7 us of start and end for each item.  base lags: a row's sums are scaled only when a score is TL_LAG above it (sums in TMEM would have to be read and written
+// back), and then it goes TL_SHIFT below that score.  So weights reach 2^TL_LAG, which f16 holds, and the largest one is 2^TL_SHIFT at least: those beside it keep f16's 11 bits down to 2^-21 of it.  (With the
+// largest at 1 the tail of 32000 equal keys, each 2^-22 of one that stands out, came out in steps of 2^-24: off by 4e-4 of the result.)
 // Warps 0-7 and 8-15 the rows of the two tiles, 16 the copies, 17 the products, 18 says what has come.  Every wait is bounded; where one ran out all roles run to their ends and the host reports it.
 #pragma once
 #include <cuda.h>
@@ -31,7 +32,8 @@ static_assert(TL_SOFT * 32 * TL_REGS_SOFT + 128 * TL_REGS_REST <= TL_THREADS * T
 #define TL_GROUPS 8                           // barriers of the ring: a step's keys, or its values (a wait costs the warp that issues the products 150 to 200 cycles, one for each block 1000 a step)
 #define TL_QBLOCKS 3                          // of a row of Q: dim in two, rest in one
 #define TL_SMEM ((2 * TL_QBLOCKS + TL_SLOTS) * TL_BLOCK + 1024)
-#define TL_LAG 8.0f
+#define TL_LAG 15.0f
+#define TL_SHIFT 7.0f
 #define TL_O 256                              // TMEM columns: S (and P) of the tiles at 0 and 128, O behind
 #define TL_DIM 128                            // largest dim and vdim
 
@@ -604,16 +606,17 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
             m0 = tl_max3(m0, __uint_as_float(x[TL_HALF - 2]), __uint_as_float(x[TL_HALF - 1]));
             const float mx = tl_max3(m0, m1, m1) * ff;
             // The sums are scaled where a row's base has to follow its largest score; else the halves need not meet.  (Behind this all have read S, too)
-            if (tl_sync_or(1 + i, !(mx <= base + TL_LAG))) {
+            if (tl_sync_or(1 + i, !(mx <= __fadd_rd(base, TL_LAG)))) {      // (rounded down: no weight is above 2^TL_LAG)
                 if (half) sh.top[i][in_tile] = mx;
                 tl_sync(1 + i);
                 if (!half) sh.top[i][in_tile] = tl_max3(mx, sh.top[i][in_tile], mx);
                 tl_sync(1 + i);
                 const float both = sh.top[i][in_tile];
                 float alpha = 1.0f;
-                if (base == base && !(both <= base + TL_LAG)) {      // (a base that is none stays so: keys behind it that are not seen would hide it)
-                    if (base != -INFINITY) alpha = lt_exp2(base - both);
-                    base = both;
+                if (base == base && !(both <= __fadd_rd(base, TL_LAG))) {      // (a base that is none stays so: keys behind it that are not seen would hide it)
+                    const float was = base;
+                    base = __fadd_ru(both, -TL_SHIFT);
+                    if (was != -INFINITY) alpha = lt_exp2(was - base);
                 }
                 if (__any_sync(0xffffffffu, alpha != 1.0f)) {
                     if (k > 0 && ok) {
@@ -636,8 +639,9 @@ __global__ void __launch_bounds__(TL_THREADS, 1) latent_tile_kernel(const __grid
                 }
             }
             const float minus = base == -INFINITY ? 0.0f : -base;
-            // score - base in one multiply-add, whose rest of the largest score's rounding is the same for the whole row; scores beyond 2^26, whose rests leave what f16 holds, are rounded first
-            if (__any_sync(0xffffffffu, fabsf(minus) >= 67108864.0f) && ff == f) scaled();
+            // score - base in one multiply-add, whose rest of the largest score's rounding is the same for the whole row; scores from 2^24 on, whose rests of 1 and more could lift a weight out of f16, are
+            // rounded first
+            if (__any_sync(0xffffffffu, fabsf(minus) >= 16777200.0f) && ff == f) scaled();
             const tl_f2 ff2 = tl_two(ff, ff), minus2 = tl_two(minus, minus);
             tl_f2 sum = 0ull, more = 0ull;
 #pragma unroll

@@ -672,3 +672,44 @@ def test_small_latents_keep_their_bits(dev, rank, size, pos0, counts):
             lim = 2.0 ** -11 * np.abs(want) + (len(rows) / 16 + rank / 16 + 8) * 2.0 ** -23 * terms + 2.0 ** -25
             assert (np.abs(got[at + t] - want) <= lim).all(), float((np.abs(got[at + t] - want) / lim).max())
         at += n
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("pos0,n", [(120, 1), (3000, 30), (9000, 70)])
+def test_a_flat_tail(dev, form, pos0, n):
+    """one key stands out, thousands lie 15 below it: their weights count together, and each keeps the bits of a 16-bit number"""
+    H, dim, vdim, rank, rest = 2, 16, 32, 16, 16
+    c = Case(dev, 64, rank, rest, [pos0], [n])
+    rows = np.zeros((pos0 + n, rank + rest), np.float16)
+    rows[:, 0], rows[:, rank] = 1.0, -15.0
+    rows[7, 0], rows[7, rank] = 0.0, 0.0
+    c.put(0, 0, rows)
+    q = np.zeros((n, H, dim + rest), np.float16)
+    q[..., dim] = 1.0
+    uk, uv = np.zeros((H * dim, rank), np.float16), np.ones((H * vdim, rank), np.float16)
+    got = attend(dev, c, q.reshape(n, -1), uk, uv, H, 1.0, 0, None, FORMS[form], capi.F16)
+    tail = (np.arange(pos0, pos0 + n)) * np.exp(-15.0)
+    # a weight is 2^7 e^-15 = 2^-14.6 or more, where f16 has steps of 2^-24: half of one is 2^-10.4 of it; the result's rounding 2^-11 of itself, or half of a step of 2^-24
+    assert (np.abs(got - (tail / (1 + tail))[:, None]) <= (2.0 ** -10.4 + 2.0 ** -11) * (tail / (1 + tail))[:, None] + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("scale", [2.0 ** -12, 1e-3, 0.01, 0.037, 0.1, 0.61, 1.0, -0.05])
+@pytest.mark.parametrize("pos0,n", [(0, 100), (700, 40), (6000, 33)])
+def test_scores_of_millions(dev, form, scale, pos0, n):
+    """scores up to 2^30 and beyond, growing from key to key by a little or a lot: all keys have one value, so that is the result, and no weight leaves its type"""
+    H, dim, vdim, rank, rest = 3, 16, 32, 32, 16
+    c = Case(dev, 32, rank, rest, [pos0], [n], seed=n)
+    rows = np.tile(c.rng.normal(size=rank + rest), (pos0 + n, 1))
+    j = np.arange(pos0 + n)
+    rows[:, rank] = 30000.0 + 16.0 * (j % 700)
+    rows[:, rank + 1] = c.rng.integers(-3, 4, size=pos0 + n)
+    c.put(0, 0, rows.astype(np.float16))
+    q = c.rng.normal(size=(n, H, dim + rest))
+    q[:, 0, dim], q[:, 1, dim], q[:, 2, dim] = 2000.0, 30000.0, 100.0
+    uk, uv = ((c.rng.normal(size=s) * 0.2).astype(np.float16) for s in ((H * dim, rank), (H * vdim, rank)))
+    got = attend(dev, c, q.astype(np.float16).reshape(n, -1), uk, uv, H, scale, 0, None, FORMS[form], capi.F16).reshape(n, H, vdim)
+    V, lat = uv.astype(np.float64).reshape(H, vdim, rank), rows[0, :rank].astype(np.float16).astype(np.float64)
+    # roundings of the weights (over the line, not under it), of the expanded values and of the result, 2^-11 each, beside 32-bit sums
+    lim = 3 * 2.0 ** -11 * np.abs(V @ lat) + 2.0 ** -17 * (np.abs(V) @ np.abs(lat)) + 2.0 ** -24
+    assert (np.abs(got - V @ lat) <= lim).all()
