@@ -713,3 +713,85 @@ def test_scores_of_millions(dev, form, scale, pos0, n):
     # roundings of the weights (over the line, not under it), of the expanded values and of the result, 2^-11 each, beside 32-bit sums
     lim = 3 * 2.0 ** -11 * np.abs(V @ lat) + 2.0 ** -17 * (np.abs(V) @ np.abs(lat)) + 2.0 ** -24
     assert (np.abs(got - V @ lat) <= lim).all()
+
+
+def whole(c, i, q, uk, uv, H, scale, window, sink, leave_out=None):
+    """one sequence's results in 64 bits, all tokens at a time; leave_out: keys that are lost"""
+    n, rank, rest = c.counts[i], c.rank, c.rest
+    rows = c.rows(i, c.pos0[i] + n).astype(np.float64)
+    dim, vdim = uk.shape[0] // H, uv.shape[0] // H
+    pos, keys = c.pos0[i] + np.arange(n)[:, None], np.arange(len(rows))[None]
+    seen = (keys <= pos) & ((pos - keys < window) if window > 0 else True)
+    if leave_out is not None:
+        seen[:, leave_out] = False
+    out = np.zeros((n, H, vdim))
+    for h in range(H):
+        k = np.concatenate([rows[:, :rank] @ uk[h * dim:(h + 1) * dim].astype(np.float64).T, rows[:, rank:]], 1)
+        z = np.where(seen, scale * (q[:, h].astype(np.float64) @ k.T), -np.inf)
+        top = np.maximum(z.max(1, keepdims=True), -np.inf if sink is None else float(sink[h]))
+        w = np.exp(z - top)
+        w /= w.sum(1, keepdims=True) + (0.0 if sink is None else np.exp(float(sink[h]) - top))
+        out[:, h] = w @ (rows[:, :rank] @ uv[h * vdim:(h + 1) * vdim].astype(np.float64).T)
+    return out
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("out_type", [capi.F16, capi.BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("shape", [(2, 32, 16, 48, 64), (16, 128, 64, 128, 512), (64, 64, 32, 64, 128)], ids=str)
+@pytest.mark.parametrize("P,pos0,counts,window,sink", [(64, [5000], [10], 0, False), (16, [1000, 0, 300], [1, 200, 3], 0, True), (32, [2500, 40], [130, 2], 700, False), (128, [3000, 700, 31], [1, 1, 1], 0, False)])
+def test_results_as_a_whole(dev, form, out_type, shape, P, pos0, counts, window, sink):
+    """the root mean square of a whole result's error: a step of 32 keys that is lost among thousands shows in it, and in F16 results one key, where the bound on single numbers lets it pass"""
+    H, dim, rest, vdim, rank = shape
+    c = Case(dev, P, rank, rest, pos0, counts, seed=H + P)
+    r, T, at = c.rng, sum(counts), 0
+    uk, uv = ((r.normal(size=s) * rank ** -0.5).astype(np.float16) for s in ((H * dim, rank), (H * vdim, rank)))
+    q, s = r.normal(size=(T, H, dim + rest)).astype(np.float16), r.normal(size=H).astype(np.float32) if sink else None
+    scale = (dim + rest) ** -0.5
+    got = attend(dev, c, q.reshape(T, -1), uk, uv, H, scale, window, s, FORMS[form], out_type).reshape(T, H, vdim)
+    # Relative, of independent errors: the result's rounding, at most half a step of 2^-8 or 2^-11 of it; a weight's and a value's, 2^-11 / sqrt(3) at most each; and a weight by its score, whose terms
+    # add up to scores of about 1 with a rounding of 2^-11 / sqrt(3) each.  Three of 2^-11.8 beside the result's own
+    own = 2.0 ** -8 if out_type == capi.BF16 else 2.0 ** -11
+    lim = (own ** 2 / 3 + 3 * (2.0 ** -11.8) ** 2) ** 0.5 * 1.25
+    for i, n in enumerate(counts):
+        mine = slice(at, at + n)
+        want = whole(c, i, q[mine], uk, uv, H, scale, window, s)
+        size = np.sqrt((want ** 2).mean())
+        assert np.sqrt(((got[mine] - want) ** 2).mean()) <= lim * size, (i, np.sqrt(((got[mine] - want) ** 2).mean()) / size, lim)
+        # .. for every token, whose results are H * vdim numbers
+        each = np.sqrt(((got[mine] - want) ** 2).mean((1, 2))) / np.sqrt((want ** 2).mean((1, 2)))
+        assert (each <= 1.5 * lim).all(), (i, each.max(), lim)
+        if pos0[i] >= 300 and H <= 16:
+            key = c.pos0[i] - (100 if window else 200)
+            lost = whole(c, i, q[mine], uk, uv, H, scale, window, s, leave_out=slice(key, key + 32) if out_type == capi.BF16 else key)
+            assert np.sqrt(((lost - want) ** 2).mean()) > 1.5 * lim * size
+        at += n
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("window", [0, 12])
+def test_each_row_that_is_not_finite(dev, form, window):
+    """a NaN or an infinity in c, and a NaN or the infinity that the query's sign makes +infinity in r: NaN for the queries that see the row.  The other infinity in r: the weight 0"""
+    bad = [(50, 3, np.nan), (45, 35, np.inf), (100, 0, -np.inf), (41, 7, np.inf), (60, 40, np.nan), (47, 33, -np.inf)]
+    pos0, counts, H, dim, vdim, rank = [40, 40, 90, 40, 50, 40], [20, 20, 40, 3, 33, 20], 3, 32, 32, 32
+    c = Case(dev, 16, rank, 16, pos0, counts, seed=window)
+    clean = [c.rows(i, pos0[i] + counts[i]).copy() for i in range(len(bad))]
+    for i, (at, col, x) in enumerate(bad):
+        row = clean[i][at].copy()
+        row[col] = x
+        c.put(i, at, row[None])
+    T = sum(counts)
+    q = (np.abs(c.rng.normal(size=(T, H, dim + 16))) + 0.25).astype(np.float16)
+    uk, uv = (np.abs(c.rng.normal(size=(H * d, rank)) * 0.2).astype(np.float16) + np.float16(0.01) for d in (dim, vdim))
+    got, first = attend(dev, c, q.reshape(T, -1), uk, uv, H, 0.2, window, None, FORMS[form]).reshape(T, H, vdim), 0
+    for i, (at, col, x) in enumerate(bad):
+        n = counts[i]
+        rows, mine = clean[i].copy(), got[first:first + n]
+        weightless = col >= rank and x == -np.inf
+        if weightless:
+            rows[at, col] = -65504.0                                         # x 0.25 x 0.2: a weight of 0 in 64 bits too
+        want, size = R.attention(rows, pos0[i], q[first:first + n], uk, uv, rank, H, 0.2, window)
+        pos = pos0[i] + np.arange(n)
+        sees = (pos >= at) & ((pos - at < window) if window else True) & (not weightless)
+        assert np.isnan(mine[sees]).all() and np.isfinite(mine[~sees]).all(), i
+        np.testing.assert_allclose(mine[~sees], want[~sees], rtol=0.01, atol=0.01)
+        first += n
