@@ -287,7 +287,7 @@ static int64_t prod(const int64_t* shape, int ndim) {
 extern "C" CC_API int cc_tensor_alloc(cc_device* dev, const int64_t* shape, int32_t ndim, int32_t t, cc_buf** out) {
     if (!dev || !shape || !out || ndim < 1 || ndim > CC_MAX_DIMS) return cc_fail(dev, CC_ERR_ARG, "cc_tensor_alloc: bad argument");
     CC_ENTER(dev);
-    CC_REQUIRE(dev, t == CC_F32 || t == CC_F16 || t == CC_BF16 || t == CC_I32 || t == CC_I8, "only f32/f16 is supported");   // cpu_tensor.rs:139-141; BF16: activations of 16 bits; I32: index state of the sequence ops; I8: pages of codes
+    CC_REQUIRE(dev, t == CC_F32 || t == CC_F16 || t == CC_BF16 || t == CC_I32 || t == CC_I8, "alloc: a tensor of type %d (only f32, f16, bf16, i32 and i8 are supported)", t);   // cpu_tensor.rs:139-141 (f32, f16); BF16: activations of 16 bits; I32: index state of the sequence ops; I8: pages of codes
     // F32 is zero-filled (vec![0.0; n]); F16 is uninitialised in the reference (buf_f16.rs:23-28), zeroed here
     return cc_new_activation(dev, prod(shape, ndim), t, true, out);
 }

@@ -283,3 +283,12 @@ def test_activations_of_numbers_that_are_not_finite(dev, rows, out, act):
                     fine = torch.isfinite(want)
                     # one rounding of the sum, beside a 32-bit step of a sigmoid of an infinity
                     assert ((got[row] - want)[fine].abs() <= (EPS[out] + 2.0 ** -23) * want[fine].abs() + 2.0 ** -25).all()
+
+
+def test_types_that_are_allocated(dev):
+    """plain types, as zeros; a refusal names them"""
+    for t in (BF16, F16, F32):
+        assert (take(dev, CudaTensor.alloc([3, 5], TYPES[t], dev)) == 0).all()
+    for t in (capi.Q8_0 if hasattr(capi, "Q8_0") else 8, 99, -1):
+        with pytest.raises(TensorError, match="f32, f16, bf16, i32 and i8"):
+            CudaTensor.alloc([32], t, dev)
