@@ -98,17 +98,8 @@ __device__ __forceinline__ int tl_find(const LrArgs& a, int n, Count count, int*
     return -1;
 }
 __device__ __forceinline__ unsigned tl_at(int row, int chunk) { return (unsigned)(row * 128 + ((chunk ^ (row & 7)) << 4)); }      // chunk of 8 numbers of a row of a block
-// a wait that ends after some seconds, or when another one has (asked to hold the thread for up to 2 us a look, it came back later: 136 us instead of 131)
-__device__ __forceinline__ bool tl_wait(unsigned bar, unsigned parity, int* fail) {
-    unsigned done = 0;
-    for (unsigned it = 0; it < (1u << 24); it++) {
-        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-        if (done) return true;
-        if (*(volatile int*)fail) return false;
-    }
-    *(volatile int*)fail = 1;
-    return false;
-}
+// waits that end after some seconds, or when another one has: they look whether it has every time (asked to hold the thread for up to 2 us a look, it came back later: 136 us instead of 131)
+__device__ __forceinline__ bool tl_wait(unsigned bar, unsigned parity, int* fail) { return sg_wait<1>(bar, parity, fail); }
 __device__ __forceinline__ bool tl_wait_warp(unsigned bar, unsigned parity, int* fail) { return __all_sync(0xffffffffu, tl_wait(bar, parity, fail)); }
 __device__ __forceinline__ void tl_report(int fail, unsigned* err_dev, unsigned* err_host) {
     if (threadIdx.x == 0 && fail) {
@@ -136,25 +127,10 @@ struct TeShared {
     unsigned tmem_base;
     int fail;
 };
-__device__ __forceinline__ unsigned te_even(unsigned addr) {         // the even CTA's own of it
-    unsigned a;
-    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(addr));
-    return a;
-}
 // (relaxed: nothing that this thread has written is read behind the barrier, and a release to the cluster waits 1300 cycles for what it has under way)
 __device__ __forceinline__ void te_expect(unsigned bar, unsigned bytes) { asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
-__device__ __forceinline__ void te_tma(unsigned dst, const void* tmap, unsigned bar, int x, int y) {
-    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(tmap), "r"(bar), "r"(x), "r"(y) : "memory");
-}
 __device__ __forceinline__ void te_tma_page(unsigned dst, const void* tmap, unsigned bar, int x, int page) {
     asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(tmap), "r"(bar), "r"(x), "r"(0), "r"(page) : "memory");
-}
-__device__ __forceinline__ void te_umma(unsigned tmem_d, uint64_t a, uint64_t b, unsigned idesc, unsigned accumulate) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-}
-// what this thread has issued so far arrives on the barrier, when it is complete, in both CTAs
-__device__ __forceinline__ void te_commit(unsigned bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
 __device__ __forceinline__ void te_sync(int which) { asm volatile("bar.sync %0, 128;" ::"r"(1 + which) : "memory"); }      // the four warps of a block
 // grid (key tiles, up to a whole pair, runs of heads)
@@ -193,7 +169,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TE_THREADS, 1) laten
     if (warp == 0) {
         const int pages = found < 0 ? 0 : (min(TL_KEYS, to - key0) + a.page - 1) >> a.shift, mine = tl_look_up(a, seq, key0, to);
         for (int b = 0; b < blocks; b++) {
-            const unsigned bar = te_even(pg_smem(&sh.a_full[b]));
+            const unsigned bar = pg_even(pg_smem(&sh.a_full[b]));
             if (lane == 0) te_expect(bar, (unsigned)(pages * a.page * 128));
             __syncwarp();
             for (int i = 0; i < pages; i++) {
@@ -210,7 +186,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TE_THREADS, 1) laten
                     const unsigned slot = g % TE_STAGES, own = pg_smem(&sh.full[slot]);
                     if (!(ok = tl_wait(pg_smem(&sh.empty[slot]), ((g / TE_STAGES) & 1u) ^ 1u, &sh.fail))) break;
                     if (rank == 0) pg_mbar_expect_tx(own, (unsigned)wide * 256);
-                    te_tma(pg_smem(bs + slot * TE_STAGE), rank ? &map_uv : &map_uk, te_even(own), b * 64, (t.head0 + h) * (rank ? a.vdim : a.dim));
+                    pg_tma_load_2d_pair(pg_smem(bs + slot * TE_STAGE), rank ? &map_uv : &map_uk, pg_even(own), b * 64, (t.head0 + h) * (rank ? a.vdim : a.dim));
                 }
             int never = 0;                                            // no copy is under way when the CTAs end (the even one sees those of both), and no arrival
             if (rank == 0)
@@ -241,15 +217,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TE_THREADS, 1) laten
                     if (pg_elect()) {
 #pragma unroll
                         for (int kk = 0; kk < 4; kk++)
-                            if (kk < steps) te_umma(acc, x + 2 * kk, y + 2 * kk, idesc, b > 0 || kk > 0);
-                        te_commit(pg_smem(&sh.empty[slot]));
-                        if (b == blocks - 1) te_commit(pg_smem(&sh.acc_full[n & 1u]));
+                            if (kk < steps) pg_umma_f16_pair(acc, x + 2 * kk, y + 2 * kk, idesc, b > 0 || kk > 0);
+                        pg_umma_commit_pair(pg_smem(&sh.empty[slot]));
+                        if (b == blocks - 1) pg_umma_commit_pair(pg_smem(&sh.acc_full[n & 1u]));
                     }
                     __syncwarp();
                     if (++slot == TE_STAGES) { slot = 0; phase ^= 1u; }
                 }
             }
-            if (pg_elect()) te_commit(pg_smem(&sh.drained));
+            if (pg_elect()) pg_umma_commit_pair(pg_smem(&sh.drained));
             __syncwarp();
         }
         tl_wait_warp(pg_smem(&sh.drained), 0, &never);
@@ -307,7 +283,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TE_THREADS, 1) laten
             }
             pg_fence_before();
             __syncwarp();
-            if (lane == 0) pg_arrive_relaxed(te_even(pg_smem(&sh.acc_empty[n & 1u])));
+            if (lane == 0) pg_arrive_relaxed(pg_even(pg_smem(&sh.acc_empty[n & 1u])));
         });
         if (row == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }

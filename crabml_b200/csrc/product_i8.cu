@@ -382,18 +382,6 @@ __host__ __device__ constexpr size_t gp_smem(int bn) { return (size_t)gp_stages(
 __device__ __forceinline__ void gp_umma(unsigned tmem_d, uint64_t a, uint64_t b, unsigned idesc, unsigned accumulate) {
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
-// what this thread has issued so far arrives on the barrier, when it is complete, in both CTAs
-__device__ __forceinline__ void gp_commit(unsigned bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
-}
-__device__ __forceinline__ unsigned gp_even(unsigned addr) {         // the even CTA's own of it
-    unsigned a;
-    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(addr));
-    return a;
-}
-__device__ __forceinline__ void gp_tma_load(unsigned dst, const void* tmap, unsigned bar, int x, int y) {
-    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(tmap), "r"(bar), "r"(x), "r"(y) : "memory");
-}
 template <int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GI_THREADS, 1) i8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_cut,
                                                                                          const float* __restrict__ ws, const float* __restrict__ xs, float* __restrict__ out, int T, int m, int steps, int n_whole, int cut,
@@ -440,11 +428,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GI_THREADS, 1) i8_pa
                 int mt, n0;
                 const int wide = place(tile, mt, n0);
                 for (int s = 0; s < steps; s++, g++) {
-                    const unsigned slot = g % ST, own = pg_smem(&sh.full[slot]), full = gp_even(own), at = pg_smem(ring + (size_t)slot * BYTES);
+                    const unsigned slot = g % ST, own = pg_smem(&sh.full[slot]), full = pg_even(own), at = pg_smem(ring + (size_t)slot * BYTES);
                     if (!(ok = sg_wait(pg_smem(&sh.empty[slot]), ((g / ST) & 1u) ^ 1u, &sh.fail))) break;
                     if (rank == 0) pg_mbar_expect_tx(own, 2 * A_BYTES + wide * GI_K);
-                    gp_tma_load(at, &map_w, full, s * GI_K, mt * 256 + rank * 128);
-                    gp_tma_load(at + A_BYTES, wide == BN ? &map_x : &map_cut, full, s * GI_K, n0 + rank * (wide / 2));
+                    pg_tma_load_2d_pair(at, &map_w, full, s * GI_K, mt * 256 + rank * 128);
+                    pg_tma_load_2d_pair(at + A_BYTES, wide == BN ? &map_x : &map_cut, full, s * GI_K, n0 + rank * (wide / 2));
                 }
             }
             int never = 0;                                            // no copy is under way when the CTAs end (the even one sees those of both), and no arrival
@@ -474,11 +462,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GI_THREADS, 1) i8_pa
                     const uint64_t a = pg_smem_desc(at), b = pg_smem_desc(at + A_BYTES);
 #pragma unroll
                     for (int kk = 0; kk < GI_K / 32; kk++) gp_umma(acc, a + 2 * kk, b + 2 * kk, desc, s > 0 || kk > 0);
-                    gp_commit(pg_smem(&sh.empty[slot]));
+                    pg_umma_commit_pair(pg_smem(&sh.empty[slot]));
                 }
-                if (ok) gp_commit(pg_smem(&sh.acc_full[nth & 1u]));
+                if (ok) pg_umma_commit_pair(pg_smem(&sh.acc_full[nth & 1u]));
             }
-            gp_commit(pg_smem(&sh.drained));
+            pg_umma_commit_pair(pg_smem(&sh.drained));
             sg_wait(pg_smem(&sh.drained), 0, &never);
         }
         __syncwarp();
@@ -507,7 +495,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GI_THREADS, 1) i8_pa
             }
             pg_fence_before();                                        // the accumulator may be filled again
             __syncwarp();
-            if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(gp_even(pg_smem(&sh.acc_empty[nth & 1u]))) : "memory");
+            if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(pg_even(pg_smem(&sh.acc_empty[nth & 1u]))) : "memory");
         }
     }
     pg_fence_before();

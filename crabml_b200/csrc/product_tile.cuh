@@ -267,21 +267,6 @@ __global__ void __launch_bounds__(pt_threads(BN, DRAIN), 1) product_tile_kernel(
 }
 
 // ---- two SMs on a tile -----------------------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ void pt_umma2(unsigned tmem_d, uint64_t a, uint64_t b, unsigned idesc, unsigned accumulate) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-}
-// what this thread has issued so far arrives on the barrier, when it is complete, in both CTAs of the pair
-__device__ __forceinline__ void pt_commit2(unsigned bar, unsigned pair) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)(3u << 2 * pair)) : "memory");
-}
-__device__ __forceinline__ unsigned pt_even(unsigned addr, unsigned pair) {      // the pair's even CTA's own of it
-    unsigned a;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(2 * pair));
-    return a;
-}
-__device__ __forceinline__ void pt_tma2(unsigned dst, const void* tmap, unsigned bar, int x, int y) {
-    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(tmap), "r"(bar), "r"(x), "r"(y) : "memory");
-}
 // The first n_whole tiles are 256 x 256, those of the last wave that is not full are cut across the rows of x, `cut` pieces each.  The even CTA issues the products; the copies of both are
 // counted on its barriers, and what it commits arrives in both.  parts > 1: a cluster of that many pairs shares a tile's depth (there is one tile for each cluster), and each pair finishes every
 // parts-th run of 16 rows of x with the sums of all, in the order of the parts
@@ -330,11 +315,11 @@ __global__ void __launch_bounds__(pt_threads(256, DRAIN), 1) product_pair_kernel
                 int mt, n0;
                 const int wide = place(tile, mt, n0);
                 for (int s = 0; s < steps; s++, g++) {
-                    const unsigned slot = g % ST, own = pg_smem(&sh.full[slot]), full = pt_even(own, part), at = pg_smem(ring + (size_t)slot * BYTES);
+                    const unsigned slot = g % ST, own = pg_smem(&sh.full[slot]), full = pg_even(own, part), at = pg_smem(ring + (size_t)slot * BYTES);
                     if (!(ok = sg_wait(pg_smem(&sh.empty[slot]), ((g / ST) & 1u) ^ 1u, &sh.fail))) break;
                     if (rank == 0) pg_mbar_expect_tx(own, 2 * A_BYTES + wide * PT_STEP);
-                    pt_tma2(at, &map_w, full, (s0 + s) * 64, mt * 256 + rank * 128);
-                    pt_tma2(at + A_BYTES, wide == BN ? &map_x : &map_cut, full, (s0 + s) * 64, n0 + rank * (wide / 2));
+                    pg_tma_load_2d_pair(at, &map_w, full, (s0 + s) * 64, mt * 256 + rank * 128);
+                    pg_tma_load_2d_pair(at + A_BYTES, wide == BN ? &map_x : &map_cut, full, (s0 + s) * 64, n0 + rank * (wide / 2));
                 }
             }
             int never = 0;                                            // no copy is under way when the CTAs end (the even one sees those of both), and no arrival
@@ -364,16 +349,16 @@ __global__ void __launch_bounds__(pt_threads(256, DRAIN), 1) product_pair_kernel
                     const bool last = s % chunk == chunk - 1 || s == steps - 1;
                     if (pg_elect()) {
 #pragma unroll
-                        for (int kk = 0; kk < 4; kk++) pt_umma2(acc, x + 2 * kk, y + 2 * kk, idesc, s % chunk > 0 || kk > 0);
-                        pt_commit2(pg_smem(&sh.empty[slot]), part);
-                        if (last) pt_commit2(pg_smem(&sh.acc_full[nth & 1u]), part);
+                        for (int kk = 0; kk < 4; kk++) pg_umma_f16_pair(acc, x + 2 * kk, y + 2 * kk, idesc, s % chunk > 0 || kk > 0);
+                        pg_umma_commit_pair(pg_smem(&sh.empty[slot]), part);
+                        if (last) pg_umma_commit_pair(pg_smem(&sh.acc_full[nth & 1u]), part);
                     }
                     __syncwarp();
                     nth += last;
                     if (++slot == ST) { slot = 0; phase ^= 1u; }
                 }
             }
-            if (pg_elect()) pt_commit2(pg_smem(&sh.drained), part);
+            if (pg_elect()) pg_umma_commit_pair(pg_smem(&sh.drained), part);
             __syncwarp();
         }
         sg_wait_warp(pg_smem(&sh.drained), 0, &never);
@@ -382,7 +367,7 @@ __global__ void __launch_bounds__(pt_threads(256, DRAIN), 1) product_pair_kernel
     auto release = [&](unsigned n) {
         pg_fence_before();
         __syncwarp();
-        if (lane == 0) pg_arrive_relaxed(pt_even(pg_smem(&sh.acc_empty[n & 1u]), part));
+        if (lane == 0) pg_arrive_relaxed(pg_even(pg_smem(&sh.acc_empty[n & 1u]), part));
     };
     // a cut tile's columns are shared by all groups, but those that a warp has added up are its own
     auto share = [&](int wide, int& c_first) {

@@ -56,12 +56,14 @@ struct SgShared {
     unsigned tmem_base;
     int fail;                               // a wait ran out
 };
+// false: it ran out, or another one of the CTA had, which it looks for every EVERY-th time
+template <unsigned EVERY = 256>
 __device__ __forceinline__ bool sg_wait(unsigned bar, unsigned parity, int* fail) {
     unsigned done = 0;
     for (unsigned it = 0; it < SG_WAIT_LIMIT; it++) {
         asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
         if (done) return true;
-        if ((it & 255u) == 255u && *(volatile int*)fail) return false;
+        if (it % EVERY == EVERY - 1 && *(volatile int*)fail) return false;
     }
     *(volatile int*)fail = 1;
     return false;

@@ -65,3 +65,21 @@ __device__ __forceinline__ bool pg_elect() {
 // Arrival on a barrier of the cluster by a thread whose reads of tensor memory are complete (tcgen05.wait::ld) and that has written nothing for those who wait: relaxed, since a release to the
 // cluster waits for the thread's stores to memory, 1300 cycles and more
 __device__ __forceinline__ void pg_arrive_relaxed(unsigned bar) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+
+// ---- pairs of SMs (cta_group::2): CTAs 2 p and 2 p + 1 of a cluster share a product, which the even one issues ------------------------------
+__device__ __forceinline__ unsigned pg_even(unsigned addr, unsigned pair = 0) {      // the even CTA's own of it
+    unsigned a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(2 * pair));
+    return a;
+}
+// into this CTA's shared memory, counted on a barrier of either of the two
+__device__ __forceinline__ void pg_tma_load_2d_pair(unsigned dst, const void* tmap, unsigned bar, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(tmap), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void pg_umma_f16_pair(unsigned tmem_d, uint64_t desc_a, uint64_t desc_b, unsigned idesc, unsigned accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// what this thread has issued so far arrives on the barrier, when it is complete, in both CTAs
+__device__ __forceinline__ void pg_umma_commit_pair(unsigned bar, unsigned pair = 0) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)(3u << 2 * pair)) : "memory");
+}
