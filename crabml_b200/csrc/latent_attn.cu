@@ -9,11 +9,11 @@
 //   values   warp w adds up the columns 16 (w + 8 i) of all rows in registers; scaled when a row's largest score grows
 // That is a chain of 2700 cycles a step, mostly latencies, while the step's bytes take 1600; so two such groups of 8 warps take the steps by turns and add up their sums at a segment's end.
 // All steps of a call are dealt out in equal runs over the SMs; sums of cut segments are joined by latent_join_kernel.
-// 64 sequences of 20 to 4000 rows, 16 heads of 128 + 64 over 512 + 64: 57 us, of which this kernel 41 (154 MB: 3.7 TB/s with starts, restarts at segments and sums); one token over 32000 rows 29, this
+// 64 sequences of 20 to 4000 rows, 16 heads of 128 + 64 over 512 + 64: 56 us, of which this kernel 41 (154 MB: 3.7 TB/s with starts, restarts at segments and sums); one token over 32000 rows 29, this
 // kernel 17 (37 MB), of which 11 start and end, fold 4, join 4, unfold 5.
 //
 // Sums, largest scores and sums of weights have 32 bits; queries on their way to the latents are brought near 2^4 by a power of two and rounded to f16, weights are rounded to f16 near
-// 2^10 (2^-11 of each: the operands of the tensor cores; the result is rounded to 16 bits anyway), sums of latents enter the last product as two f16 numbers.
+// 2^10 (2^-11 of each: the operands of the tensor cores; the result is rounded to 16 bits anyway), sums of latents enter the last product as two f16 numbers, the number and 2^11 times its rest.
 #include <cuda.h>
 
 #include <algorithm>

@@ -9,8 +9,9 @@
 // The two tiles alternate: while the 256 threads of one make its weights, two a row, the tensor core multiplies for the other.  (With a thread a row a step's 128 scores were a chain of
 // 4500 cycles for the one warp a scheduler that a tile had: 4000 tokens of 16 heads took 147 us.)  TMEM holds both S and both O (512 columns), shared memory
 // Q (96 KB) and a ring of 16 KB blocks of keys and values (128 KB).
-// Now that prompt's call takes 128 us (98.7 GFLOP with its keys and values, 0.77 PFLOP/s); 8000 tokens 359 (0.96 PFLOP/s).  Shared memory bounds the products: S reads 8 KB for each 64 cycles of the tensor core, as fast as
-// it can; then 7 us of start and end for each item.  base lags: a row's sums are scaled only when a score is TL_LAG above it (sums in TMEM would have to be read and written
+// Now that prompt's call takes 131 us (98.7 GFLOP with its keys and values, 0.75 PFLOP/s); 8000 tokens about 370 (0.93 PFLOP/s).  A step takes 2.7 us, 5100 cycles, whether both tiles have it or one: what
+// bounds it is a tile's chain (scores, their way to registers, the largest, the barrier behind it, exponentials, the way back, values, and only then the next scores, since P lies over S).  The step's
+// products, fed by shared memory as fast as it can (S reads 8 KB for each 64 cycles of the tensor core), would take 2560 cycles.  Then 7 us of start and end for each item.  base lags: a row's sums are scaled only when a score is TL_LAG above it (sums in TMEM would have to be read and written
 // back), and then it goes TL_SHIFT below that score.  So weights reach 2^TL_LAG, which f16 holds, and the largest one is 2^TL_SHIFT at least: those beside it keep f16's 11 bits down to 2^-21 of it.  (With the
 // largest at 1 the tail of 32000 equal keys, each 2^-22 of one that stands out, came out in steps of 2^-24: off by 4e-4 of the result.)
 // Warps 0-7 and 8-15 the rows of the two tiles, 16 the copies, 17 the products, 18 says what has come.  Every wait is bounded; where one ran out all roles run to their ends and the host reports it.

@@ -85,7 +85,8 @@ __device__ __forceinline__ void pt_finish16(const PrArgs& a, const unsigned (&v)
         if (n0 + j < n_end && col < a.m) ht_write(a.out, (int64_t)(n0 + j) * a.m + col, a.out_type, y);
     }
 }
-// With the activation as a function that is known: each has its own loop.  16-bit results: by the special function unit's exponential and reciprocal, 2^-20 of a result, in a dozen instructions
+// With the activation as a function that is known: each has its own loop.  16-bit results: by the special function unit's exponential and reciprocal, off by 2^-19 of a sigmoid for |z| up to 8 and 2^-16 up to 80 (below
+// -87, where it is under 2^-125, it is 0), in a dozen instructions
 // where tanhf and a division take sixty (8 warps finished a tile of 256 x 256 no sooner than 64 steps of its products were done)
 __device__ __noinline__ float pt_exact_act(float z, int act) { return act_apply(z, act); }      // (out of line: sixteen of them side by side spilled)
 template <bool EXACT, class Body>

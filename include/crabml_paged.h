@@ -96,9 +96,10 @@ CC_API int cc_paged_latent_append(cc_device* dev, const cc_page_plan* plan, cons
  * form: in which order the products are taken.  CC_LATENT_ABSORBED: queries over U to the latents, attention over the cached rows themselves, its result over V.
  * CC_LATENT_EXPANDED: keys and values of every visible row laid out, then attention (dim and vdim up to 128, dim + rest up to 192).  CC_LATENT_AUTO: what should take less time,
  * sequence by sequence.  Both hold weights and the factors of the second product as 16-bit numbers with 32-bit sums.
- * Workspace, which the device's pool keeps: absorbed, the queries and sums over the latents of as many tokens as have them in 256 MB, beside 10 MB of sums and 16 bytes for every 32 rows
- * that 16 queries see; expanded, keys and values of a call's
- * visible rows, 64 columns and 128 tokens at a time, within 256 MB or those of one sequence and head, beside some 30 MB of sums.  Expanded keys and values beyond the range of 16 bits count as its largest; uk and uv are finite.
+ * Workspace, which the device's pool keeps (in blocks of powers of two): absorbed, the queries and sums over the latents of as many tokens as have them in 256 MB, 32 at least, beside 10 MB of sums
+ * and 16 bytes for every 32 rows that 16 queries see; expanded, keys and values of a call's
+ * visible rows, 64 columns and 128 tokens at a time, within 256 MB or those of one sequence and head, beside some 30 MB of sums.  Expanded keys and values beyond the range of 16 bits count as its largest, those below 2^-14 are rounded to steps of
+ * 2^-24; uk and uv are finite.
  * A row of the cache that is not finite reaches the results of the queries that see it and no others (a key whose score is -infinity by its r has the weight 0); a query that holds a NaN or an
  * infinity has the result NaN; rows behind a sequence's end are not looked at.  Equal calls give equal bits on a device. */
 enum cc_latent_form { CC_LATENT_AUTO = 0, CC_LATENT_ABSORBED = 1, CC_LATENT_EXPANDED = 2 };
