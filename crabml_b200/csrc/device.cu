@@ -16,6 +16,7 @@ int cc_fail(cc_device* dev, int code, const char* fmt, ...) {
     vsnprintf(buf, sizeof(buf), fmt, ap);
     va_end(ap);
     if (dev) dev->last_error = buf; else g_create_error = buf;
+    if (code == CC_ERR_CUDA) cudaGetLastError();                    // this call's error, not that of the next one that looks whether its launch went well
     return code;
 }
 

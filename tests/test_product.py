@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from crabml_b200 import CudaTensor, TensorError, TensorStrider, capi, seqops
+from crabml_b200 import CudaError, CudaTensor, TensorError, TensorStrider, capi, seqops
 from tests.gpu_common import make_device
 
 pytestmark = pytest.mark.gpu
@@ -292,3 +292,16 @@ def test_types_that_are_allocated(dev):
     for t in (capi.Q8_0 if hasattr(capi, "Q8_0") else 8, 99, -1):
         with pytest.raises(TensorError, match="f32, f16, bf16, i32 and i8"):
             CudaTensor.alloc([32], t, dev)
+
+
+@pytest.mark.parametrize("rows", [1, 40, 300])
+def test_after_a_call_that_found_no_memory(dev, rows):
+    """memory that is not there is that call's error, and no later one's: a tensor of 32 TB, then products by every kernel, and an older operation"""
+    w, x, bias, _ = make(rows, 200, 320, BF16, F32, rows)
+    with pytest.raises(CudaError):
+        CudaTensor.alloc([1 << 44], capi.F16, dev)
+    check(dev, w, x, bias=bias, out=F32)
+    with pytest.raises(CudaError):
+        CudaTensor.alloc([1 << 44], capi.F16, dev)
+    y = CudaTensor.new(np.ones((4, 8), np.float32), [4, 8], dev)
+    assert (seqops.activate_inplace(y, capi.ACT_RELU_SQUARED).export() == 1.0).all()
